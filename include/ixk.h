@@ -360,6 +360,40 @@ int ixk_residual_add(int dtype, int64_t rows, int64_t cols, const void* x,
                      const void* partial, const void* bias, void* out,
                      void* cuda_stream);
 
+/* --------------------------------------------------------- row norms, training */
+/* LayerNorm and RMSNorm with gain and shift, the row statistics kept for the backward pass (XLA
+ * compiles both from the model's own expressions; the reference has no custom call for them).  Per
+ * row, with mean = 0 for RMS and rstd = 1 / sqrt(mean((x - mean)^2) + eps):
+ *   xh = (x - mean) * rstd                  y  = xh * (gain_offset + gain) + shift
+ *   h  = grad_y * (gain_offset + gain)      dx = rstd * (h - [LAYER: mean(h)] - xh * mean(h * xh))
+ *   dgain = sum over rows of grad_y * xh    dshift = sum over rows of grad_y
+ * dtype (x, y, grad_y, dx) in {BF16, F16, F32}; param_dtype (gain, shift, dgain, dshift) the same or
+ * F32.  Statistics and sums are fp32, each result is rounded once; the sums over the rows are taken
+ * in a fixed order.  Any cols up to 16384 (else IXK_UNIMPLEMENTED) and any strides and addresses that
+ * elements can have; rows that all start on 16-byte boundaries and hold whole 16-byte vectors go
+ * fastest.  y may be x, dx may be grad_y or x. */
+typedef struct ixk_row_norm_desc {
+  int32_t dtype;
+  int32_t param_dtype;
+  int32_t kind;            /* ixk_norm_kind */
+  float eps;
+  float gain_offset;       /* 1 for the (1 + w) scale of Gemma's RMSNorm */
+  int32_t reserved;        /* must be 0 */
+  int64_t rows, cols;
+  int64_t x_stride, y_stride;            /* row pitches in elements */
+  int64_t grad_y_stride, dx_stride;      /* (backward only) */
+} ixk_row_norm_desc;
+/* gain NULL: no scale; shift NULL: none.  mean (LAYER only) and rstd, fp32 [rows], may be NULL where
+ * nothing will be differentiated. */
+int ixk_row_norm_fwd(const ixk_row_norm_desc* desc, const void* x, const void* gain, const void* shift,
+                     void* y, float* mean, float* rstd, void* cuda_stream);
+/* dgain and dshift may be NULL (not wanted); with either, workspace holds
+ * ixk_row_norm_bwd_workspace_bytes(desc) bytes, 16-byte aligned.  mean is not read for RMS. */
+int ixk_row_norm_bwd(const ixk_row_norm_desc* desc, const void* grad_y, const void* x, const void* gain,
+                     const float* mean, const float* rstd, void* dx, void* dgain, void* dshift,
+                     void* workspace, size_t workspace_bytes, void* cuda_stream);
+size_t ixk_row_norm_bwd_workspace_bytes(const ixk_row_norm_desc* desc);
+
 /* ------------------------------------------------------ all-reduce over NVLink */
 /* The exchange step of a tensor-parallel layer: the partial sums of a row-parallel projection,
  * one per GPU, summed into every GPU.  Replaces sycl_allreduce (xla/service/gpu/ccl_ops.h:40-46,

@@ -29,7 +29,7 @@ __all__ = [
     "EPILOGUES", "run_gemm_custom_call", "gemm_attrs_for", "gemm", "gemm_fp8", "gemm_workspace_bytes",
     "fmha_forward_kernel", "fmha_forward_kernel_bf16", "fmha_forward_kernel_fp16", "fmha_workspace_bytes",
     "fmha_forward_kernel_static_scratch", "STATIC_SCRATCH_BYTES",
-    "quantize_fp8",
+    "quantize_fp8", "row_norm_forward", "row_norm_backward", "row_norm_backward_workspace_bytes",
 ]
 
 # ----------------------------------------------------------------------------- ABI mirror
@@ -86,6 +86,13 @@ class _FmhaBwdDesc(ctypes.Structure):
                 ("dk_strides", ctypes.c_int64 * 3), ("dv_strides", ctypes.c_int64 * 3)]
 
 
+class _RowNormDesc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("param_dtype", ctypes.c_int32), ("kind", ctypes.c_int32), ("eps", ctypes.c_float),
+                ("gain_offset", ctypes.c_float), ("reserved", ctypes.c_int32), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64),
+                ("x_stride", ctypes.c_int64), ("y_stride", ctypes.c_int64), ("grad_y_stride", ctypes.c_int64),
+                ("dx_stride", ctypes.c_int64)]
+
+
 # the same layouts for struct, whose field order and padding they share
 _PACK_GEMM = struct.Struct("=2i4q2i4q2i4qq2f2i").pack
 _PACK_FMHA = struct.Struct("=7i2fi15q").pack
@@ -119,6 +126,9 @@ ABI_SYMBOLS = {
                                               ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _vp, _vp, _vp]),
     "ixk_row_norm_gain": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, _vp, ctypes.c_int64,
                                          _vp, ctypes.c_float, _vp, ctypes.c_int64, ctypes.c_float, _vp]),
+    "ixk_row_norm_fwd": (ctypes.c_int, [ctypes.POINTER(_RowNormDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "ixk_row_norm_bwd": (ctypes.c_int, [ctypes.POINTER(_RowNormDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ixk_row_norm_bwd_workspace_bytes": (_sz, [ctypes.POINTER(_RowNormDesc)]),
     "ixk_rotary_half": (ctypes.c_int, [ctypes.c_int, _vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                        ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _vp, _vp, _vp]),
     "ixk_kv_append": (ctypes.c_int, [ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _vp, _vp, ctypes.c_int64,
@@ -534,6 +544,88 @@ def row_norm(x: torch.Tensor, *, kind: int = NORM_LAYER, eps: float = 1e-5, out:
     _check(load_library().ixk_row_norm(_TORCH_TO_IXK[x.dtype], kind, rows, cols, x.data_ptr(), cols, out.data_ptr(),
                                        cols, eps, _stream_ptr(stream)))
     return out
+
+
+def _row_pitch(name: str, t: torch.Tensor) -> int:
+    """Elements between the rows of a tensor whose last dimension is a row: dense, or 2-D with any pitch."""
+    if t.is_contiguous():
+        return t.shape[-1]
+    if t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= t.shape[1]:
+        return t.stride(0)
+    raise IxkError(IXK_INVALID_ARGUMENT, f"{name} must be dense, or 2-D with contiguous rows that do not overlap")
+
+
+def _row_norm_desc(x: torch.Tensor, kind: int, gain, gain_offset: float, shift, eps: float) -> _RowNormDesc:
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise IxkError(IXK_INVALID_ARGUMENT, "x must have rows of at least one element")
+    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise IxkError(IXK_UNIMPLEMENTED, "x must be bfloat16, float16 or float32")
+    cols = x.shape[-1]
+    param_dtype = next((p.dtype for p in (gain, shift) if p is not None), x.dtype)
+    for name, p in (("gain", gain), ("shift", shift)):
+        if p is not None and (p.shape != (cols,) or p.dtype != param_dtype or not p.is_contiguous()):
+            raise IxkError(IXK_INVALID_ARGUMENT, f"{name} must be a dense [cols] vector; gain and shift of one type")
+    if param_dtype not in _TORCH_TO_IXK:
+        raise IxkError(IXK_UNIMPLEMENTED, "gain and shift must have x's type or be float32")
+    d = _RowNormDesc()
+    d.dtype, d.param_dtype, d.kind = _TORCH_TO_IXK[x.dtype], _TORCH_TO_IXK[param_dtype], int(kind)
+    d.eps, d.gain_offset = float(eps), float(gain_offset)
+    d.rows, d.cols = x.numel() // cols, cols
+    d.x_stride = d.y_stride = d.grad_y_stride = d.dx_stride = _row_pitch("x", x)
+    return d
+
+
+def row_norm_forward(x: torch.Tensor, *, kind: int = NORM_LAYER, eps: float = 1e-5, gain: Optional[torch.Tensor] = None,
+                     gain_offset: float = 0.0, shift: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, stream=None):
+    """(y, mean, rstd) of LayerNorm or RMSNorm over the last dimension, y = (x - mean) * rstd * (gain_offset + gain) + shift, for
+    training: the fp32 row statistics (x's shape without its last dimension; mean is None for RMS) are what
+    row_norm_backward wants.  x bfloat16, float16 or float32, dense or 2-D with a row pitch; gain and shift of x's type or
+    float32."""
+    d = _row_norm_desc(x, kind, gain, gain_offset, shift, eps)
+    _require_cuda(x, gain, shift, out)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if out.shape != x.shape or out.dtype != x.dtype:
+        raise IxkError(IXK_INVALID_ARGUMENT, "out must match x")
+    d.y_stride = _row_pitch("out", out)
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    mean = torch.empty_like(rstd) if kind == NORM_LAYER else None
+    _check(load_library().ixk_row_norm_fwd(ctypes.byref(d), _ptr(x), _ptr(gain), _ptr(shift), _ptr(out), _ptr(mean), _ptr(rstd),
+                                           _stream_ptr(stream)))
+    return out, mean, rstd
+
+
+def row_norm_backward_workspace_bytes(x: torch.Tensor, gain: Optional[torch.Tensor] = None) -> int:
+    return int(load_library().ixk_row_norm_bwd_workspace_bytes(ctypes.byref(_row_norm_desc(x, NORM_LAYER, gain, 0.0, None, 0.0))))
+
+
+def row_norm_backward(grad_out: torch.Tensor, x: torch.Tensor, mean: Optional[torch.Tensor], rstd: torch.Tensor, *,
+                      kind: int = NORM_LAYER, gain: Optional[torch.Tensor] = None, gain_offset: float = 0.0, with_shift: bool = False,
+                      grad_x: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None, stream=None):
+    """(dx, dgain, dshift) of row_norm_forward.  dgain is None without a gain, dshift unless with_shift; both have gain's
+    type (x's without one) and are sums over all rows, taken in a fixed order.  grad_x may be grad_out or x."""
+    d = _row_norm_desc(x, kind, gain, gain_offset, None, 0.0)
+    _require_cuda(grad_out, x, mean, rstd, gain, grad_x, workspace)
+    if grad_x is None:
+        grad_x = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    for name, t in (("grad_out", grad_out), ("grad_x", grad_x)):
+        if t.shape != x.shape or t.dtype != x.dtype:
+            raise IxkError(IXK_INVALID_ARGUMENT, f"{name} must have x's shape and type")
+    for name, t in (("rstd", rstd), ("mean", mean if kind == NORM_LAYER else None)):
+        if t is None and name == "mean" and kind != NORM_LAYER:
+            continue
+        if t is None or t.dtype != torch.float32 or t.shape != x.shape[:-1] or not t.is_contiguous():
+            raise IxkError(IXK_INVALID_ARGUMENT, f"{name} must be the forward's dense fp32 row statistics")
+    d.grad_y_stride, d.dx_stride = _row_pitch("grad_out", grad_out), _row_pitch("grad_x", grad_x)
+    lib = load_library()
+    param_dtype = x.dtype if gain is None else gain.dtype
+    dgain = None if gain is None else torch.empty(d.cols, dtype=param_dtype, device=x.device)
+    dshift = torch.empty(d.cols, dtype=param_dtype, device=x.device) if with_shift else None
+    if workspace is None and (dgain is not None or dshift is not None):
+        workspace = _own_scratch(lib.ixk_row_norm_bwd_workspace_bytes(ctypes.byref(d)), x.device, stream)
+    _check(lib.ixk_row_norm_bwd(ctypes.byref(d), _ptr(grad_out), _ptr(x), _ptr(gain), _ptr(mean), _ptr(rstd), _ptr(grad_x), _ptr(dgain),
+                                _ptr(dshift), _ptr(workspace), 0 if workspace is None else workspace.nbytes, _stream_ptr(stream)))
+    return grad_x, dgain, dshift
 
 
 def rotary_interleaved_(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, seq_len: int, rotary_dim: int,
