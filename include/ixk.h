@@ -394,6 +394,64 @@ int ixk_row_norm_bwd(const ixk_row_norm_desc* desc, const void* grad_y, const vo
                      void* workspace, size_t workspace_bytes, void* cuda_stream);
 size_t ixk_row_norm_bwd_workspace_bytes(const ixk_row_norm_desc* desc);
 
+/* ------------------------------------------------- losses at the vocabulary head */
+/* The end of a training step: hidden states x [rows, hidden] against a head weight [vocab, hidden]
+ * (and bias [vocab]), without the [rows, vocab] logits in memory (XLA would materialise them; the
+ * reference's fine-tuning example, example/gemma/finetune.py, ends in such a loss).
+ *
+ * Cross entropy, z = scale * (x.weight^T + bias):
+ *   lse_i = ln sum_v exp z_iv        loss_i = lse_i - z_{i, labels[i]}
+ * a row whose label is ignore_index or lies outside [0, vocab) has no target.
+ *
+ * Distillation from a teacher's top logits at temperature T (`scale` holds T):
+ *   q_i = softmax over row i's entries of teacher / T,   p_i = softmax((x.weight^T + bias) / T)
+ *   loss_i = T^2 * sum_k q_ik (ln q_ik - ln p_{i, index_ik})        lse_i of the logits over T
+ * an entry whose index lies outside [0, vocab) or whose teacher logit is -inf is absent, an index
+ * that appears twice counts twice; a row without entries has no target.
+ *
+ * Rows without a target have loss 0, lse 0 and gradient 0 and take no part in dweight and dbias,
+ * whatever x holds in them.  The backward calls take each row's grad_loss (pitch grad_loss_stride, 0
+ * for one number that all rows share) and the forward's lse, make the logits once more piece by piece,
+ * and return dx, dweight, dbias (any may be NULL: not wanted).  dtype in {BF16, F16}: x, weight, bias
+ * and their gradients.  Logits, statistics and all sums are fp32; the gradient with respect to the
+ * logits is rounded to dtype as an operand of the two products (for F16 scaled by a power of two that
+ * brings the largest row's into range), each result once.  Results do not depend on timing.
+ * x, weight: 16-byte aligned, strides multiples of 8 elements (else IXK_INVALID_ARGUMENT /
+ * IXK_UNIMPLEMENTED, as for ixk_gemm); everything else only as its elements are.  Workspace:
+ * ixk_linear_loss_workspace_bytes(desc, backward) bytes, 256-byte aligned; it grows with the rows, not
+ * with rows * vocab (the backward's piece of the logits' gradient is at most 256 MB where 256 columns
+ * fit that, beside x's size again in 16 and 32 bits and at most 64 MB for the products). */
+typedef struct ixk_linear_loss_desc {
+  int32_t dtype;          /* IXK_BF16 or IXK_F16 */
+  int32_t w_order;        /* ixk_order of weight as [vocab, hidden] */
+  int32_t dw_order;       /* of dweight */
+  int32_t index_bytes;    /* labels / index: 4 or 8 byte integers */
+  int32_t entries;        /* distillation: entries per row, at most 256; cross entropy: 0 */
+  int32_t teacher_dtype;  /* IXK_BF16, IXK_F16 or IXK_F32 */
+  float scale;            /* cross entropy: of the logits; distillation: temperature */
+  int32_t reserved;       /* must be 0 */
+  int64_t ignore_index;
+  int64_t rows, hidden, vocab;
+  int64_t x_stride, w_stride, dx_stride, dw_stride;   /* elements between rows (columns, if column-major) */
+  int64_t index_stride, teacher_stride;               /* distillation: elements between rows of entries */
+  int64_t grad_loss_stride;
+} ixk_linear_loss_desc;
+int ixk_linear_xent_fwd(const ixk_linear_loss_desc* desc, const void* x, const void* weight,
+                        const void* bias, const void* labels, float* loss, float* lse,
+                        void* workspace, size_t workspace_bytes, void* cuda_stream);
+int ixk_linear_xent_bwd(const ixk_linear_loss_desc* desc, const void* x, const void* weight,
+                        const void* bias, const void* labels, const float* lse, const float* grad_loss,
+                        void* dx, void* dweight, void* dbias, void* workspace, size_t workspace_bytes,
+                        void* cuda_stream);
+int ixk_linear_distill_fwd(const ixk_linear_loss_desc* desc, const void* x, const void* weight,
+                           const void* bias, const void* index, const void* teacher, float* loss,
+                           float* lse, void* workspace, size_t workspace_bytes, void* cuda_stream);
+int ixk_linear_distill_bwd(const ixk_linear_loss_desc* desc, const void* x, const void* weight,
+                           const void* bias, const void* index, const void* teacher, const float* lse,
+                           const float* grad_loss, void* dx, void* dweight, void* dbias,
+                           void* workspace, size_t workspace_bytes, void* cuda_stream);
+size_t ixk_linear_loss_workspace_bytes(const ixk_linear_loss_desc* desc, int backward);
+
 /* ------------------------------------------------------ all-reduce over NVLink */
 /* The exchange step of a tensor-parallel layer: the partial sums of a row-parallel projection,
  * one per GPU, summed into every GPU.  Replaces sycl_allreduce (xla/service/gpu/ccl_ops.h:40-46,

@@ -30,6 +30,8 @@ __all__ = [
     "fmha_forward_kernel", "fmha_forward_kernel_bf16", "fmha_forward_kernel_fp16", "fmha_workspace_bytes",
     "fmha_forward_kernel_static_scratch", "STATIC_SCRATCH_BYTES",
     "quantize_fp8", "row_norm_forward", "row_norm_backward", "row_norm_backward_workspace_bytes",
+    "linear_cross_entropy", "linear_cross_entropy_backward", "linear_distillation", "linear_distillation_backward",
+    "linear_loss_workspace_bytes",
 ]
 
 # ----------------------------------------------------------------------------- ABI mirror
@@ -93,6 +95,14 @@ class _RowNormDesc(ctypes.Structure):
                 ("dx_stride", ctypes.c_int64)]
 
 
+class _LinearLossDesc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("w_order", ctypes.c_int32), ("dw_order", ctypes.c_int32), ("index_bytes", ctypes.c_int32),
+                ("entries", ctypes.c_int32), ("teacher_dtype", ctypes.c_int32), ("scale", ctypes.c_float), ("reserved", ctypes.c_int32),
+                ("ignore_index", ctypes.c_int64), ("rows", ctypes.c_int64), ("hidden", ctypes.c_int64), ("vocab", ctypes.c_int64),
+                ("x_stride", ctypes.c_int64), ("w_stride", ctypes.c_int64), ("dx_stride", ctypes.c_int64), ("dw_stride", ctypes.c_int64),
+                ("index_stride", ctypes.c_int64), ("teacher_stride", ctypes.c_int64), ("grad_loss_stride", ctypes.c_int64)]
+
+
 # the same layouts for struct, whose field order and padding they share
 _PACK_GEMM = struct.Struct("=2i4q2i4q2i4qq2f2i").pack
 _PACK_FMHA = struct.Struct("=7i2fi15q").pack
@@ -129,6 +139,12 @@ ABI_SYMBOLS = {
     "ixk_row_norm_fwd": (ctypes.c_int, [ctypes.POINTER(_RowNormDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "ixk_row_norm_bwd": (ctypes.c_int, [ctypes.POINTER(_RowNormDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "ixk_row_norm_bwd_workspace_bytes": (_sz, [ctypes.POINTER(_RowNormDesc)]),
+    "ixk_linear_xent_fwd": (ctypes.c_int, [ctypes.POINTER(_LinearLossDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ixk_linear_xent_bwd": (ctypes.c_int, [ctypes.POINTER(_LinearLossDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ixk_linear_distill_fwd": (ctypes.c_int, [ctypes.POINTER(_LinearLossDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ixk_linear_distill_bwd": (ctypes.c_int, [ctypes.POINTER(_LinearLossDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
+                                              _vp]),
+    "ixk_linear_loss_workspace_bytes": (_sz, [ctypes.POINTER(_LinearLossDesc), ctypes.c_int]),
     "ixk_rotary_half": (ctypes.c_int, [ctypes.c_int, _vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                        ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _vp, _vp, _vp]),
     "ixk_kv_append": (ctypes.c_int, [ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _vp, _vp, ctypes.c_int64,
@@ -700,6 +716,143 @@ def residual_add(x: torch.Tensor, partial: torch.Tensor, bias: Optional[torch.Te
                                            bias.data_ptr() if bias is not None else None, out.data_ptr(),
                                            _stream_ptr(stream)))
     return out
+
+
+# ----------------------------------------------------------------------------- losses at the vocabulary head
+
+def _head_matrix(name: str, t: torch.Tensor) -> tuple:
+    """(order, stride) of a [vocab, hidden] view."""
+    order, _, _, _, _, ld = _matrix_layout(name, t)
+    return order, ld
+
+
+def _linear_loss_desc(x, weight, bias, index, teacher, scale: float, ignore_index: int) -> _LinearLossDesc:
+    if x.dim() != 2 or weight.dim() != 2 or weight.shape[1] != x.shape[1]:
+        raise IxkError(IXK_INVALID_ARGUMENT, "x must be [rows, hidden] and weight [vocab, hidden]")
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise IxkError(IXK_UNIMPLEMENTED, "x must be bfloat16 or float16")
+    if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
+        raise IxkError(IXK_INVALID_ARGUMENT, "x, weight and bias must have one element type")
+    rows, hidden, vocab = x.shape[0], x.shape[1], weight.shape[0]
+    if x.stride(1) != 1 and hidden > 1:
+        raise IxkError(IXK_INVALID_ARGUMENT, "x must be row-major")
+    if bias is not None and (bias.shape != (vocab,) or not bias.is_contiguous()):
+        raise IxkError(IXK_INVALID_ARGUMENT, "bias must be a dense [vocab] vector")
+    if index.dtype not in (torch.int32, torch.int64):
+        raise IxkError(IXK_INVALID_ARGUMENT, "labels and indices must be int32 or int64")
+    d = _LinearLossDesc()
+    if teacher is None:
+        if index.shape != (rows,) or not index.is_contiguous():
+            raise IxkError(IXK_INVALID_ARGUMENT, "labels must be a dense [rows] vector")
+    else:
+        if index.dim() != 2 or index.shape[0] != rows or teacher.shape != index.shape or index.shape[1] < 1:
+            raise IxkError(IXK_INVALID_ARGUMENT, "teacher_index and teacher_logits must be [rows, entries] with at least one entry")
+        if teacher.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+            raise IxkError(IXK_UNIMPLEMENTED, "teacher_logits must be bfloat16, float16 or float32")
+        d.entries, d.teacher_dtype = index.shape[1], _TORCH_TO_IXK[teacher.dtype]
+        d.index_stride, d.teacher_stride = _row_pitch("teacher_index", index), _row_pitch("teacher_logits", teacher)
+    d.dtype, d.index_bytes = _TORCH_TO_IXK[x.dtype], index.element_size()
+    d.scale, d.ignore_index = float(scale), int(ignore_index)
+    d.rows, d.hidden, d.vocab = rows, hidden, vocab
+    d.x_stride = x.stride(0) if rows > 1 else max(x.stride(0), (hidden + 7) // 8 * 8)
+    d.w_order, d.w_stride = _head_matrix("weight", weight)
+    d.dw_order, d.dw_stride, d.dx_stride = d.w_order, d.w_stride, hidden
+    return d
+
+
+def linear_loss_workspace_bytes(x: torch.Tensor, weight: torch.Tensor, entries: int = 0, backward: bool = False) -> int:
+    """Scratch bytes of linear_cross_entropy (entries = 0) or linear_distillation, or of their backward passes."""
+    d = _LinearLossDesc()
+    d.rows, d.hidden, d.vocab, d.entries = x.shape[0], x.shape[1], weight.shape[0], entries
+    return int(load_library().ixk_linear_loss_workspace_bytes(ctypes.byref(d), 1 if backward else 0))
+
+
+def _linear_loss_forward(x, weight, bias, index, teacher, scale, ignore_index, workspace, stream):
+    d = _linear_loss_desc(x, weight, bias, index, teacher, scale, ignore_index)
+    _require_cuda(x, weight, bias, index, teacher, workspace)
+    lib = load_library()
+    loss = torch.empty(d.rows, dtype=torch.float32, device=x.device)
+    lse = torch.empty_like(loss)
+    if workspace is None:
+        workspace = _own_scratch(lib.ixk_linear_loss_workspace_bytes(ctypes.byref(d), 0), x.device, stream)
+    tail = (_ptr(loss), _ptr(lse), _ptr(workspace), workspace.nbytes, _stream_ptr(stream))
+    if teacher is None:
+        _check(lib.ixk_linear_xent_fwd(ctypes.byref(d), _ptr(x), _ptr(weight), _ptr(bias), _ptr(index), *tail))
+    else:
+        _check(lib.ixk_linear_distill_fwd(ctypes.byref(d), _ptr(x), _ptr(weight), _ptr(bias), _ptr(index), _ptr(teacher), *tail))
+    return loss, lse
+
+
+def _linear_loss_backward(x, weight, bias, index, teacher, lse, grad_loss, scale, ignore_index, grad_x, grad_weight, weight_grad, workspace,
+                          stream):
+    d = _linear_loss_desc(x, weight, bias, index, teacher, scale, ignore_index)
+    _require_cuda(x, weight, bias, index, teacher, lse, grad_loss, grad_x, grad_weight, workspace)
+    if lse.shape != (d.rows,) or lse.dtype != torch.float32 or not lse.is_contiguous():
+        raise IxkError(IXK_INVALID_ARGUMENT, "lse must be the forward's dense fp32 [rows] vector")
+    if grad_loss.dtype != torch.float32 or grad_loss.shape not in ((d.rows,), ()):
+        raise IxkError(IXK_INVALID_ARGUMENT, "grad_loss must be fp32: one number per row, or one for all of them")
+    d.grad_loss_stride = grad_loss.stride(0) if grad_loss.dim() else 0
+    if grad_x is None:
+        grad_x = torch.empty(d.rows, d.hidden, dtype=x.dtype, device=x.device)
+    if grad_x.shape != x.shape or grad_x.dtype != x.dtype:
+        raise IxkError(IXK_INVALID_ARGUMENT, "grad_x must have x's shape and type")
+    d.dx_stride = _row_pitch("grad_x", grad_x)
+    if grad_weight is None and weight_grad:
+        grad_weight = (torch.empty(d.vocab, d.hidden, dtype=x.dtype, device=x.device) if d.w_order == ROW_MAJOR
+                       else torch.empty(d.hidden, d.vocab, dtype=x.dtype, device=x.device).t())
+    if grad_weight is not None:
+        if grad_weight.shape != weight.shape or grad_weight.dtype != x.dtype:
+            raise IxkError(IXK_INVALID_ARGUMENT, "grad_weight must have weight's shape and type")
+        d.dw_order, d.dw_stride = _head_matrix("grad_weight", grad_weight)
+    grad_bias = torch.empty_like(bias) if bias is not None and weight_grad else None
+    lib = load_library()
+    if workspace is None:
+        workspace = _own_scratch(lib.ixk_linear_loss_workspace_bytes(ctypes.byref(d), 1), x.device, stream)
+    tail = (_ptr(lse), _ptr(grad_loss), _ptr(grad_x), _ptr(grad_weight), _ptr(grad_bias), _ptr(workspace), workspace.nbytes,
+            _stream_ptr(stream))
+    if teacher is None:
+        _check(lib.ixk_linear_xent_bwd(ctypes.byref(d), _ptr(x), _ptr(weight), _ptr(bias), _ptr(index), *tail))
+    else:
+        _check(lib.ixk_linear_distill_bwd(ctypes.byref(d), _ptr(x), _ptr(weight), _ptr(bias), _ptr(index), _ptr(teacher), *tail))
+    return grad_x, grad_weight, grad_bias
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, *, bias: Optional[torch.Tensor] = None,
+                         logit_scale: float = 1.0, ignore_index: int = -100, workspace: Optional[torch.Tensor] = None, stream=None):
+    """(loss, lse), fp32 [rows]: softmax cross entropy of logits = logit_scale * (x @ weight.T + bias) against labels, the logits
+    never in memory.  x [rows, hidden] and weight [vocab, hidden] (any mix of row- and column-major weight) bfloat16 or
+    float16; labels int32 or int64.  A row whose label is ignore_index or outside the vocabulary has loss and lse 0."""
+    return _linear_loss_forward(x, weight, bias, labels, None, logit_scale, ignore_index, workspace, stream)
+
+
+def linear_cross_entropy_backward(x: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, lse: torch.Tensor, grad_loss: torch.Tensor,
+                                  *, bias: Optional[torch.Tensor] = None, logit_scale: float = 1.0, ignore_index: int = -100,
+                                  grad_x: Optional[torch.Tensor] = None, grad_weight: Optional[torch.Tensor] = None,
+                                  weight_grad: bool = True, workspace: Optional[torch.Tensor] = None, stream=None):
+    """(dx, dweight, dbias) of linear_cross_entropy from its lse and the rows' grad_loss (fp32 [rows], or a scalar tensor for
+    all).  dweight is laid out like weight; weight_grad=False leaves it and dbias out (a frozen head)."""
+    return _linear_loss_backward(x, weight, bias, labels, None, lse, grad_loss, logit_scale, ignore_index, grad_x, grad_weight, weight_grad,
+                                 workspace, stream)
+
+
+def linear_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_index: torch.Tensor, teacher_logits: torch.Tensor, *,
+                        bias: Optional[torch.Tensor] = None, temperature: float = 1.0, workspace: Optional[torch.Tensor] = None,
+                        stream=None):
+    """(loss, lse), fp32 [rows]: temperature^2 times the divergence of softmax((x @ weight.T + bias) / temperature) over the
+    vocabulary from the teacher's softmax over its entries, teacher_logits / temperature at teacher_index, both [rows, entries]
+    with up to 256 entries in any order.  An entry whose index is outside the vocabulary (-1 for padding) or whose logit is
+    -inf is absent; a row without entries has loss and lse 0."""
+    return _linear_loss_forward(x, weight, bias, teacher_index, teacher_logits, temperature, 0, workspace, stream)
+
+
+def linear_distillation_backward(x: torch.Tensor, weight: torch.Tensor, teacher_index: torch.Tensor, teacher_logits: torch.Tensor,
+                                 lse: torch.Tensor, grad_loss: torch.Tensor, *, bias: Optional[torch.Tensor] = None,
+                                 temperature: float = 1.0, grad_x: Optional[torch.Tensor] = None,
+                                 grad_weight: Optional[torch.Tensor] = None, weight_grad: bool = True,
+                                 workspace: Optional[torch.Tensor] = None, stream=None):
+    """(dx, dweight, dbias) of linear_distillation: see linear_cross_entropy_backward.  The teacher has no gradient."""
+    return _linear_loss_backward(x, weight, bias, teacher_index, teacher_logits, lse, grad_loss, temperature, 0, grad_x, grad_weight,
+                                 weight_grad, workspace, stream)
 
 
 # ----------------------------------------------------------------------------- attention

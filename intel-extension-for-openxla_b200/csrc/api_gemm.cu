@@ -9,6 +9,38 @@
 #include "gemm_sm100.h"
 
 namespace ixk {
+
+namespace gemm {
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+int run_problem(const Problem& p, void* workspace, size_t workspace_bytes, const DeviceInfo& dev, cudaStream_t stream) {
+  const int es = p.kind == kKindF16 ? 2 : p.kind == kKindTf32 ? 4 : 1;
+  // Skinny problems are cut along K as far as the caller handed over scratch for the partials;
+  // without it they run un-split (same result, fewer SMs busy).
+  if (stream_applies(p)) {
+    const int splits = stream_splits(p.M, p.N, p.K, es, workspace != nullptr && aligned16(workspace) ? workspace_bytes : 0);
+    if (splits > 1) return launch_split_k(p, splits, workspace, dev, stream);
+    return stream_alone(p) ? launch_stream(p, 1, nullptr, dev, stream)
+                                 : launch(p, dev, stream);
+  }
+  int splits = (p.force_block_n > 0 || p.aux != nullptr) ? 1 : split_k_factor(p.M, p.N, p.K, p.batch, p.fp8);
+  if (splits <= 1 && p.force_block_n == 0 && p.aux == nullptr && (p.kind == kKindF16 || p.kind == kKindF8))
+    splits = tiled_splits(p.M, p.N, p.K, p.batch, es, workspace != nullptr && aligned16(workspace) ? workspace_bytes : 0);
+  if (splits > 1 && workspace != nullptr && aligned16(workspace) &&
+      workspace_bytes >= split_k_workspace_bytes(p.M, p.N, splits))
+    return launch_split_k(p, splits, workspace, dev, stream);
+  return launch(p, dev, stream);
+}
+
+size_t problem_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  const size_t tiled = split_k_workspace_bytes(M, N, split_k_factor(M, N, K, 1, false));
+  const int more = stream_takes(M) ? stream_splits(M, N, K, 2, SIZE_MAX / 4) : tiled_splits(M, N, K, 1, 2, SIZE_MAX / 4);
+  return std::max(tiled, split_k_workspace_bytes(M, N, more));
+}
+
+}  // namespace gemm
+
 namespace {
 
 // MatrixDescriptor of the reference (xla/service/gpu/matrix_descriptor.h:31-47): storage is
@@ -247,21 +279,7 @@ int run(const ixk_gemm_desc* desc, const void* a, const void* b, const void* c, 
 
   DeviceInfo dev;
   if ((rc = get_device_info(&dev)) != IXK_OK) return rc;
-  // Skinny problems are cut along K as far as the caller handed over scratch for the partials;
-  // without it they run un-split (same result, fewer SMs busy).
-  if (gemm::stream_applies(p)) {
-    const int splits = gemm::stream_splits(p.M, p.N, p.K, es, workspace != nullptr && aligned16(workspace) ? workspace_bytes : 0);
-    if (splits > 1) return gemm::launch_split_k(p, splits, workspace, dev, static_cast<cudaStream_t>(stream));
-    return gemm::stream_alone(p) ? gemm::launch_stream(p, 1, nullptr, dev, static_cast<cudaStream_t>(stream))
-                                 : gemm::launch(p, dev, static_cast<cudaStream_t>(stream));
-  }
-  int splits = (p.force_block_n > 0 || p.aux != nullptr) ? 1 : gemm::split_k_factor(p.M, p.N, p.K, p.batch, p.fp8);
-  if (splits <= 1 && p.force_block_n == 0 && p.aux == nullptr && (p.kind == gemm::kKindF16 || p.kind == gemm::kKindF8))
-    splits = gemm::tiled_splits(p.M, p.N, p.K, p.batch, es, workspace != nullptr && aligned16(workspace) ? workspace_bytes : 0);
-  if (splits > 1 && workspace != nullptr && aligned16(workspace) &&
-      workspace_bytes >= gemm::split_k_workspace_bytes(p.M, p.N, splits))
-    return gemm::launch_split_k(p, splits, workspace, dev, static_cast<cudaStream_t>(stream));
-  return gemm::launch(p, dev, static_cast<cudaStream_t>(stream));
+  return gemm::run_problem(p, workspace, workspace_bytes, dev, static_cast<cudaStream_t>(stream));
 }
 
 // Three projections of one input: out_i = A . B_i (+ bias_i), i = 0..2, with the three [K,N]

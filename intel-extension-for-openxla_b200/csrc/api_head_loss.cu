@@ -1,0 +1,749 @@
+// Losses at the vocabulary head: softmax cross entropy against labels, and distillation from a teacher's top logits, with
+// their gradients.  The tensor-core kernel that makes the logits is in head_loss_sm100.cu; here are the entry points and
+// the short kernels around it.
+//
+//   forward    [lists: a row's teacher entries sorted, their softmax]   (distillation)
+//              [gather: rows with a target side by side]                 (more than one row block)
+//              statistics of every row's logits -> loss: partials to lse and loss
+//   backward   [lists], gather, then per piece of the vocabulary: G = dloss/dlogits in 16 bits, dw = G^T x, dx += G w (the
+//              framework's GEMM, fp32 accumulator across the pieces), [dbias = sums of G]; scatter: dx to its rows
+//
+// Rows without a target cost nothing beyond the gather's copy: their number is known on the GPU only, and the kernels take
+// their row count from there.  Their hidden states are never multiplied, so nothing that they hold reaches a result.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+
+#include "gemm_sm100.h"
+#include "head_loss.h"
+#include "ptx.cuh"
+
+namespace ixk {
+namespace head {
+
+namespace {
+
+constexpr int kMaxEntries = 256;
+constexpr int64_t kDirectRows = 128;             // up to one row block there are no tiles to save: no gather
+constexpr size_t kPieceBytes = size_t(256) << 20;  // of G
+constexpr size_t kSplitBytes = size_t(64) << 20;   // of the GEMMs' K chunks
+constexpr int kSlabRows = 64;                    // rows that the product along the rows reads at a time
+constexpr float kLn2 = 0.6931471805599453f;
+
+int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// ------------------------------------------------------------------------------------------------ lists
+
+struct Lists {
+  const void *index, *teacher;
+  int64_t index_stride, teacher_stride;
+  int wide, teacher_dtype, rows, entries, vocab;
+  float inv_temperature;
+  int* column;       // [rows][entries] ascending
+  float* weight;
+  int* has;          // [rows]: any entry
+};
+
+__device__ __forceinline__ float load_as_float(const void* p, int64_t i, int dtype) {
+  if (dtype == IXK_F32) return static_cast<const float*>(p)[i];
+  if (dtype == IXK_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(static_cast<const __half*>(p)[i]);
+}
+
+constexpr int kListWarps = 4, kListPer = kMaxEntries / 32;
+
+// One warp per row: softmax over the entries that are there (index inside the vocabulary, logit above -inf), and their
+// ranks by index, ties by position, as their places in the list.
+__global__ void __launch_bounds__(32 * kListWarps) lists_kernel(const Lists a) {
+  __shared__ int columns[kListWarps][kMaxEntries];
+  ptx::grid_dependency_sync();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kListWarps + warp; row < a.rows; row += static_cast<int64_t>(gridDim.x) * kListWarps) {
+    int col[kListPer];
+    float t[kListPer];
+    float top = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < kListPer; ++e) {
+      const int k = lane + 32 * e;
+      col[e] = kNoColumn;
+      t[e] = -INFINITY;
+      if (k < a.entries) {
+        const int64_t at = row * a.index_stride + k;
+        const int64_t c = a.wide ? static_cast<const int64_t*>(a.index)[at] : static_cast<const int*>(a.index)[at];
+        const float logit = load_as_float(a.teacher, row * a.teacher_stride + k, a.teacher_dtype) * a.inv_temperature;
+        if (c >= 0 && c < a.vocab && logit != -INFINITY) {
+          col[e] = static_cast<int>(c);
+          t[e] = logit;
+          top = fmaxf(top, logit);
+        }
+        columns[warp][k] = col[e];
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < kListPer; ++e) {
+      t[e] = col[e] != kNoColumn ? expf(t[e] - top) : 0.0f;
+      sum += t[e];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const bool any = __any_sync(0xffffffffu, [&] {
+      bool here = false;
+#pragma unroll
+      for (int e = 0; e < kListPer; ++e) here |= col[e] != kNoColumn;
+      return here;
+    }());
+    __syncwarp();
+    int rank[kListPer];
+#pragma unroll
+    for (int e = 0; e < kListPer; ++e) rank[e] = 0;
+    for (int k = 0; k < a.entries; ++k) {
+      const int c = columns[warp][k];
+#pragma unroll
+      for (int e = 0; e < kListPer; ++e) rank[e] += c < col[e] || (c == col[e] && k < lane + 32 * e);
+    }
+#pragma unroll
+    for (int e = 0; e < kListPer; ++e) {
+      if (lane + 32 * e < a.entries) {
+        a.column[row * a.entries + rank[e]] = col[e];
+        a.weight[row * a.entries + rank[e]] = col[e] != kNoColumn ? t[e] / sum : 0.0f;
+      }
+    }
+    if (lane == 0) a.has[row] = any ? 1 : 0;
+    __syncwarp();
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ gather
+
+struct HasTarget {
+  const void* labels;
+  const int* has;
+  int wide, vocab;
+  int64_t ignore_index;
+  __device__ __forceinline__ bool operator()(int64_t row) const {
+    if (labels == nullptr) return has[row] != 0;
+    const int64_t l = wide ? static_cast<const int64_t*>(labels)[row] : static_cast<const int*>(labels)[row];
+    return l != ignore_index && l >= 0 && l < vocab;
+  }
+};
+
+struct Gather {
+  HasTarget has;
+  const uint16_t* x;
+  uint16_t* packed;            // the rows with a target, pitch ldp
+  int64_t ldx, ldp;
+  int rows, hidden, rows_per_cta;
+  int *active, *row_map, *inverse;   // inverse may be nullptr
+  float *loss, *lse;           // zeroed where there is no target; may be nullptr
+  const float* grad_loss;      // with range: the power of two that brings the largest row's gradient to 2^13 .. 2^14
+  int64_t grad_stride;
+  float factor;
+  float* range;                // [2]: it and its inverse; may be nullptr
+};
+
+constexpr int kGatherThreads = 256;
+
+__global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Gather a) {
+  __shared__ int warp_count[kGatherThreads / 32];
+  __shared__ int source[kGatherThreads];
+  __shared__ float warp_top[kGatherThreads / 32];
+  ptx::grid_dependency_sync();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int first = blockIdx.x * a.rows_per_cta, end = min(first + a.rows_per_cta, a.rows);
+  auto block_sum = [&](int v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if (lane == 0) warp_count[warp] = v;
+    __syncthreads();
+    int t = 0;
+    for (int w = 0; w < kGatherThreads / 32; ++w) t += warp_count[w];
+    return t;
+  };
+  // every CTA counts the rows in front of its own
+  int before = 0;
+  for (int i = threadIdx.x; i < first; i += kGatherThreads) before += a.has(i);
+  before = block_sum(before);
+  const int row = first + threadIdx.x;
+  const bool mine = static_cast<int>(threadIdx.x) < a.rows_per_cta && row < end;
+  const bool keep = mine && a.has(row);
+  const unsigned ballot = __ballot_sync(0xffffffffu, keep);
+  const int here = block_sum(lane == 0 ? __popc(ballot) : 0);
+  if (mine) {
+    int at = __popc(ballot & ((1u << lane) - 1u));
+    for (int w = 0; w < warp; ++w) at += warp_count[w];
+    if (keep) {
+      source[at] = row;
+      a.row_map[before + at] = row;
+    } else if (a.loss != nullptr) {
+      a.loss[row] = 0.0f;
+      a.lse[row] = 0.0f;
+    }
+    if (a.inverse != nullptr) a.inverse[row] = keep ? before + at : -1;
+  }
+  __syncthreads();
+  const int whole = a.hidden / 8;
+  for (int i = warp; i < here; i += kGatherThreads / 32) {
+    const uint16_t* src = a.x + source[i] * a.ldx;
+    uint16_t* dst = a.packed + (before + i) * a.ldp;
+    for (int v = lane; v < whole; v += 32) reinterpret_cast<uint4*>(dst)[v] = reinterpret_cast<const uint4*>(src)[v];
+    for (int c = whole * 8 + lane; c < a.hidden; c += 32) dst[c] = src[c];
+  }
+  if (end != a.rows) return;
+  // the last CTA: how many there are, zeros behind them up to the end of a slab, and the gradient's range
+  const int total = before + here;
+  if (threadIdx.x == 0) *a.active = total;
+  const int zero_end = min((total + kSlabRows - 1) / kSlabRows * kSlabRows, a.rows);
+  for (int i = total + warp; i < zero_end; i += kGatherThreads / 32)
+    for (int c = lane; c < a.hidden; c += 32) a.packed[i * a.ldp + c] = 0;
+  if (a.range != nullptr) {
+    float top = 0.0f;
+    for (int i = threadIdx.x; i < a.rows; i += kGatherThreads)
+      if (a.has(i)) top = fmaxf(top, fabsf(a.grad_loss[i * a.grad_stride] * a.factor));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) warp_top[warp] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 0; w < kGatherThreads / 32; ++w) top = fmaxf(top, warp_top[w]);
+      int e = 0;
+      if (top >= FLT_MIN && top <= FLT_MAX) e = min(13 - ilogbf(top), 126);
+      a.range[0] = scalbnf(1.0f, e);
+      a.range[1] = scalbnf(1.0f, -e);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ loss
+
+struct Loss {
+  HasTarget has;               // (without a gather)
+  const float2* partial;       // [slots][rows]
+  const float* at_target;      // [batch rows][entries]
+  const float* weight;         // [batch rows][entries]; nullptr: one label of weight 1
+  const int *active, *row_map; // nullptr: all rows, in place
+  int rows, slots, entries;
+  float factor;
+  float *loss, *lse;
+};
+
+constexpr int kLossThreads = 256;
+
+// kRows rows per CTA, side by side in memory; their partials dealt out over the remaining threads.
+template <int kRows>
+__global__ void __launch_bounds__(kLossThreads) loss_kernel(const Loss a) {
+  constexpr int kParts = kLossThreads / kRows;
+  __shared__ float2 stat[kParts][kRows];
+  __shared__ float row_lse[kRows], share[kParts][kRows];
+  ptx::grid_dependency_sync();
+  const int r = threadIdx.x % kRows, part = threadIdx.x / kRows;
+  const int row = blockIdx.x * kRows + r;
+  const bool there = row < (a.active != nullptr ? *a.active : a.rows);
+  const int64_t orig = !there ? 0 : a.row_map != nullptr ? a.row_map[row] : row;
+  auto join = [](float2 p, float2 q) {
+    const float top = fmaxf(p.x, q.x);
+    return make_float2(top, p.y * exp2f(p.x - top) + q.y * exp2f(q.x - top));
+  };
+  float2 s = make_float2(-FLT_MAX, 0.0f);
+  if (there) {
+#pragma unroll 4
+    for (int i = part; i < a.slots; i += kParts) s = join(s, a.partial[static_cast<int64_t>(i) * a.rows + row]);
+  }
+  stat[part][r] = s;
+  __syncthreads();
+  for (int n = kParts / 2; n > 0; n /= 2) {
+    if (part < n) stat[part][r] = join(stat[part][r], stat[part + n][r]);
+    __syncthreads();
+  }
+  if (part == 0) row_lse[r] = fmaf(stat[0][r].x, kLn2, logf(stat[0][r].y));
+  __syncthreads();
+  const float lse = row_lse[r];
+  float t = 0.0f;
+  if (there) {
+    for (int k = part; k < a.entries; k += kParts) {
+      const float q = a.weight != nullptr ? a.weight[orig * a.entries + k] : 1.0f;
+      if (q != 0.0f) t += q * (logf(q) + (lse - a.at_target[orig * a.entries + k]));   // (0 ln 0 = 0; NaN goes on)
+    }
+  }
+  share[part][r] = t;
+  __syncthreads();
+  for (int n = kParts / 2; n > 0; n /= 2) {
+    if (part < n) share[part][r] += share[part + n][r];
+    __syncthreads();
+  }
+  if (part == 0 && there) {
+    const bool counts = a.active != nullptr || a.has(orig);
+    a.loss[orig] = counts ? share[0][r] * a.factor : 0.0f;
+    a.lse[orig] = counts ? lse : 0.0f;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ behind the products
+
+template <bool kBf16>
+__device__ __forceinline__ float from16(uint32_t bits) {
+  if constexpr (kBf16) return __uint_as_float(bits << 16);
+  else return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+}
+template <bool kBf16>
+__device__ __forceinline__ uint32_t to16(float f) {
+  if constexpr (kBf16) return __bfloat16_as_ushort(__float2bfloat16_rn(f));
+  else return __half_as_ushort(__float2half_rn(f));
+}
+
+// dbias of a piece: the sums of G's columns.  256 columns per CTA, 32 warps that take rows in turn.
+constexpr int kBiasCols = 256, kBiasGroups = 32;
+template <bool kBf16>
+__global__ void __launch_bounds__(32 * kBiasGroups) bias_kernel(const uint16_t* g, int64_t ldg, const int* active, int count, const float* range,
+                                                              uint16_t* out) {
+  __shared__ float sums[kBiasGroups][kBiasCols];
+  ptx::grid_dependency_sync();
+  const int group = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = *active;
+  const int c0 = blockIdx.x * kBiasCols + lane * 8;
+  float t[8] = {};
+  if (c0 < count) {      // (G's pitch is whole vectors)
+    const uint16_t* p = g + c0;
+#pragma unroll 4
+    for (int row = group; row < rows; row += kBiasGroups) {
+      const uint4 w = *reinterpret_cast<const uint4*>(p + row * ldg);
+      const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        t[2 * j] += from16<kBf16>(words[j] & 0xffffu);
+        t[2 * j + 1] += from16<kBf16>(words[j] >> 16);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sums[group][lane * 8 + j] = t[j];
+  __syncthreads();
+  const int c = blockIdx.x * kBiasCols + threadIdx.x;
+  if (threadIdx.x < kBiasCols && c < count) {
+    float s = 0.0f;
+    for (int i = 0; i < kBiasGroups; ++i) s += sums[i][threadIdx.x];
+    out[c] = static_cast<uint16_t>(to16<kBf16>(range != nullptr ? s * range[1] : s));
+  }
+}
+
+// dx: the accumulator's rows back to where they came from, rounded once; zeros where there was no target.
+template <bool kBf16>
+__global__ void __launch_bounds__(256) scatter_kernel(const float* acc, int64_t ld_acc, const int* inverse, const float* range, int hidden,
+                                                      int vec, uint16_t* dx, int64_t ld) {
+  ptx::grid_dependency_sync();
+  const int64_t row = blockIdx.x;
+  const int from = inverse[row];
+  const float scale = range != nullptr ? range[1] : 1.0f;
+  const float* src = acc + from * ld_acc;
+  uint16_t* dst = dx + row * ld;
+  const int vecs = vec ? hidden / 8 : 0;
+  for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (from >= 0) {
+      const float4 a = reinterpret_cast<const float4*>(src)[2 * v], b = reinterpret_cast<const float4*>(src)[2 * v + 1];
+      w.x = to16<kBf16>(a.x * scale) | to16<kBf16>(a.y * scale) << 16;
+      w.y = to16<kBf16>(a.z * scale) | to16<kBf16>(a.w * scale) << 16;
+      w.z = to16<kBf16>(b.x * scale) | to16<kBf16>(b.y * scale) << 16;
+      w.w = to16<kBf16>(b.z * scale) | to16<kBf16>(b.w * scale) << 16;
+    }
+    reinterpret_cast<uint4*>(dst)[v] = w;
+  }
+  for (int c = vecs * 8 + threadIdx.x; c < hidden; c += blockDim.x)
+    dst[c] = from >= 0 ? static_cast<uint16_t>(to16<kBf16>(src[c] * scale)) : static_cast<uint16_t>(0);
+}
+
+// ------------------------------------------------------------------------------------------------ host
+
+bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// Where everything lies in the workspace.
+struct Space {
+  size_t total = 0;
+  size_t take(size_t bytes) {
+    const size_t at = total;
+    total += (bytes + 255) / 256 * 256;
+    return at;
+  }
+};
+
+struct Layout {
+  Space space;
+  size_t active, row_map, column, weight, has, packed, at_target, partial;      // forward
+  size_t inverse, grad, acc, split, split_bytes;                               // backward
+  int64_t ldp, slots, piece, ldg, ld_acc;
+  bool gathered;
+};
+
+Layout layout_for(const ixk_linear_loss_desc& d, bool backward) {
+  Layout l{};
+  const int64_t N = d.rows, D = d.hidden, V = d.vocab, K = std::max<int64_t>(d.entries, 1);
+  l.gathered = backward || N > kDirectRows;
+  l.active = l.space.take(256);      // (and the range)
+  l.row_map = l.space.take(4 * N);
+  if (d.entries > 0) {
+    l.column = l.space.take(4 * N * K);
+    l.weight = l.space.take(4 * N * K);
+    l.has = l.space.take(4 * N);
+  }
+  l.ldp = round_up(D, 8);
+  if (l.gathered) l.packed = l.space.take(2 * N * l.ldp);
+  if (!backward) {
+    l.at_target = l.space.take(4 * N * K);
+    l.slots = stat_slots(N, V);
+    l.partial = l.space.take(sizeof(float2) * l.slots * N);
+    return l;
+  }
+  l.inverse = l.space.take(4 * N);
+  // pieces of equal size, as few as the bytes allow
+  const int64_t rows = round_up(N, 256), most = std::max<int64_t>(kPieceBytes / (2 * rows) / kPieceUnit * kPieceUnit, kPieceUnit);
+  const int64_t pieces = (V + most - 1) / most;
+  l.piece = std::min(round_up((V + pieces - 1) / pieces, kPieceUnit), round_up(V, 8));
+  l.ldg = round_up(l.piece, 8);
+  l.grad = l.space.take(2 * rows * l.ldg);
+  l.ld_acc = round_up(D, 4);
+  l.acc = l.space.take(4 * N * l.ld_acc);
+  l.split_bytes = std::min(std::max(gemm::problem_workspace_bytes(N, D, l.piece), gemm::problem_workspace_bytes(D, l.piece, N)), kSplitBytes);
+  l.split = l.space.take(l.split_bytes);
+  return l;
+}
+
+int check(const ixk_linear_loss_desc* d, const char* name, bool distill, bool backward, const void* x, const void* w, const void* bias,
+          const void* index, const void* teacher) {
+  const std::string who = std::string(name) + ": ";
+  if (d == nullptr) return fail(IXK_INVALID_ARGUMENT, who + "desc is NULL");
+  if (d->reserved != 0) return fail(IXK_INVALID_ARGUMENT, who + "desc.reserved must be 0");
+  if (d->dtype != IXK_BF16 && d->dtype != IXK_F16) return fail(IXK_UNIMPLEMENTED, who + "dtype must be BF16 or F16");
+  if (d->rows < 0 || d->hidden <= 0 || d->vocab <= 0) return fail(IXK_INVALID_ARGUMENT, who + "negative rows, or no hidden size or vocabulary");
+  if (d->rows > (1 << 24) || d->hidden > (1 << 20) || d->vocab > (1 << 24))
+    return fail(IXK_UNIMPLEMENTED, who + "more than 2^24 rows or columns, or a hidden size above 2^20");
+  for (int order : {d->w_order, d->dw_order})
+    if (order != IXK_ROW_MAJOR && order != IXK_COL_MAJOR)
+      return fail(IXK_INVALID_ARGUMENT, who + "w_order and dw_order must be 0 (row-major) or 1 (column-major)");
+  if (d->index_bytes != 4 && d->index_bytes != 8) return fail(IXK_INVALID_ARGUMENT, who + "index_bytes must be 4 or 8");
+  if (!(d->scale > 0.0f) || !std::isfinite(d->scale))
+    return fail(IXK_INVALID_ARGUMENT, who + (distill ? "temperature must be positive and finite" : "the logits' scale must be positive and finite"));
+  const int64_t w_inner = d->w_order == IXK_ROW_MAJOR ? d->hidden : d->vocab, dw_inner = d->dw_order == IXK_ROW_MAJOR ? d->hidden : d->vocab;
+  if (d->x_stride < d->hidden || d->w_stride < w_inner || (backward && (d->dx_stride < d->hidden || d->dw_stride < dw_inner)))
+    return fail(IXK_INVALID_ARGUMENT, who + "a stride is smaller than the contiguous dimension");
+  if (distill) {
+    if (d->entries < 1) return fail(IXK_INVALID_ARGUMENT, who + "entries must be at least 1");
+    if (d->entries > kMaxEntries) return fail(IXK_UNIMPLEMENTED, who + "more than 256 entries per row");
+    if (d->teacher_dtype != IXK_BF16 && d->teacher_dtype != IXK_F16 && d->teacher_dtype != IXK_F32)
+      return fail(IXK_UNIMPLEMENTED, who + "teacher_dtype must be BF16, F16 or F32");
+    if (d->index_stride < d->entries || d->teacher_stride < d->entries)
+      return fail(IXK_INVALID_ARGUMENT, who + "a row of entries is longer than its stride");
+  } else if (d->entries != 0) {
+    return fail(IXK_INVALID_ARGUMENT, who + "entries must be 0");
+  }
+  if (d->rows > 0 && (x == nullptr || w == nullptr || index == nullptr || (distill && teacher == nullptr)))
+    return fail(IXK_INVALID_ARGUMENT, who + "a required pointer is NULL");
+  if (!aligned(x, 16) || !aligned(w, 16)) return fail(IXK_INVALID_ARGUMENT, who + "x and weight must be 16-byte aligned (TMA)");
+  if (d->x_stride % 8 != 0 || d->w_stride % 8 != 0)
+    return fail(IXK_UNIMPLEMENTED, who + "the strides of x and weight must be multiples of 8 elements (TMA)");
+  if (!aligned(bias, 2) || !aligned(index, d->index_bytes) || (distill && !aligned(teacher, d->teacher_dtype == IXK_F32 ? 4 : 2)))
+    return fail(IXK_INVALID_ARGUMENT, who + "a pointer is not aligned to its element size");
+  return IXK_OK;
+}
+
+int check_space(const char* name, const Layout& l, const void* workspace, size_t bytes) {
+  if (workspace == nullptr || !aligned(workspace, 256) || bytes < l.space.total)
+    return fail(IXK_WORKSPACE_TOO_SMALL, std::string(name) + ": need " + std::to_string(l.space.total) + " bytes of 256-byte aligned scratch");
+  return IXK_OK;
+}
+
+// Logits' scale, gradient factor and loss factor: z = s (x w^T + b); cross entropy is that of softmax(z); distillation at
+// temperature T is T^2 times the divergence at s = 1 / T.
+struct Scales {
+  float logits, grad, loss;
+};
+Scales scales_of(const ixk_linear_loss_desc& d, bool distill) {
+  if (!distill) return Scales{d.scale, d.scale, 1.0f};
+  return Scales{1.0f / d.scale, d.scale, d.scale * d.scale};
+}
+
+// The targets as the kernels take them; distillation's lists are made here.
+int targets_of(const ixk_linear_loss_desc& d, const Layout& l, char* ws, const void* index, const void* teacher, cudaStream_t stream,
+               Targets* t, HasTarget* has) {
+  t->wide = d.index_bytes == 8;
+  t->ignore_index = d.ignore_index;
+  has->wide = t->wide;
+  has->vocab = static_cast<int>(d.vocab);
+  has->ignore_index = d.ignore_index;
+  if (teacher == nullptr) {
+    t->labels = has->labels = index;
+    t->entries = 1;
+    return IXK_OK;
+  }
+  t->entries = d.entries;
+  Lists a{};
+  a.index = index;
+  a.teacher = teacher;
+  a.index_stride = d.index_stride;
+  a.teacher_stride = d.teacher_stride;
+  a.wide = t->wide;
+  a.teacher_dtype = d.teacher_dtype;
+  a.rows = static_cast<int>(d.rows);
+  a.entries = d.entries;
+  a.vocab = static_cast<int>(d.vocab);
+  a.inv_temperature = 1.0f / d.scale;
+  t->column = a.column = reinterpret_cast<int*>(ws + l.column);
+  t->weight = a.weight = reinterpret_cast<float*>(ws + l.weight);
+  has->has = a.has = reinterpret_cast<int*>(ws + l.has);
+  const int64_t ctas = std::min<int64_t>((d.rows + kListWarps - 1) / kListWarps, 148 * 16);
+  return launch_overlapped(lists_kernel, dim3(static_cast<unsigned>(ctas)), dim3(32 * kListWarps), 0, stream, a);
+}
+
+int gather(const ixk_linear_loss_desc& d, const Layout& l, char* ws, const HasTarget& has, const void* x, float* loss, float* lse,
+           const float* grad_loss, float factor, bool range, cudaStream_t stream) {
+  Gather g{};
+  g.has = has;
+  g.x = static_cast<const uint16_t*>(x);
+  g.packed = reinterpret_cast<uint16_t*>(ws + l.packed);
+  g.ldx = d.x_stride;
+  g.ldp = l.ldp;
+  g.rows = static_cast<int>(d.rows);
+  g.hidden = static_cast<int>(d.hidden);
+  // (each CTA counts the rows in front of it: at most 512 CTAs while a CTA's rows fit its threads)
+  g.rows_per_cta = static_cast<int>(std::min<int64_t>(std::max<int64_t>(16, (d.rows + 511) / 512), kGatherThreads));
+  g.active = reinterpret_cast<int*>(ws + l.active);
+  g.row_map = reinterpret_cast<int*>(ws + l.row_map);
+  g.inverse = loss == nullptr ? reinterpret_cast<int*>(ws + l.inverse) : nullptr;
+  g.loss = loss;
+  g.lse = lse;
+  g.grad_loss = grad_loss;
+  g.grad_stride = d.grad_loss_stride;
+  g.factor = factor;
+  g.range = range ? reinterpret_cast<float*>(ws + l.active + 16) : nullptr;
+  const int64_t ctas = (d.rows + g.rows_per_cta - 1) / g.rows_per_cta;
+  return launch_overlapped(gather_kernel, dim3(static_cast<unsigned>(ctas)), dim3(kGatherThreads), 0, stream, g);
+}
+
+Pass pass_of(const ixk_linear_loss_desc& d, const Scales& s, const void* x, int64_t ldx, const void* w, const void* bias, const Targets& t) {
+  Pass p{};
+  p.dtype = d.dtype;
+  p.w_column_major = d.w_order == IXK_COL_MAJOR;
+  p.rows = d.rows;
+  p.hidden = d.hidden;
+  p.vocab = d.vocab;
+  p.x = x;
+  p.ldx = ldx;
+  p.w = w;
+  p.ldw = d.w_stride;
+  p.bias = bias;
+  p.scale = s.logits;
+  p.first = 0;
+  p.count = d.vocab;
+  p.targets = t;
+  return p;
+}
+
+int forward(const char* name, const ixk_linear_loss_desc* d, bool distill, const void* x, const void* w, const void* bias,
+            const void* index, const void* teacher, float* loss, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check(d, name, distill, false, x, w, bias, index, teacher);
+  if (rc != IXK_OK) return rc;
+  if (d->rows > 0 && (loss == nullptr || lse == nullptr)) return fail(IXK_INVALID_ARGUMENT, std::string(name) + ": loss and lse must be non-NULL");
+  if (!aligned(loss, 4) || !aligned(lse, 4)) return fail(IXK_INVALID_ARGUMENT, std::string(name) + ": loss and lse must be 4-byte aligned");
+  if (d->rows == 0) return IXK_OK;
+  const Layout l = layout_for(*d, false);
+  if ((rc = check_space(name, l, workspace, workspace_bytes)) != IXK_OK) return rc;
+  DeviceInfo dev;
+  if ((rc = get_device_info(&dev)) != IXK_OK) return rc;
+  auto s = static_cast<cudaStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  const Scales scales = scales_of(*d, distill);
+  Targets t{};
+  HasTarget has{};
+  if ((rc = targets_of(*d, l, ws, index, teacher, s, &t, &has)) != IXK_OK) return rc;
+  Pass p = pass_of(*d, scales, x, d->x_stride, w, bias, t);
+  if (l.gathered) {
+    if ((rc = gather(*d, l, ws, has, x, loss, lse, nullptr, 0.0f, false, s)) != IXK_OK) return rc;
+    p.x = ws + l.packed;
+    p.ldx = l.ldp;
+    p.active_rows = reinterpret_cast<const int*>(ws + l.active);
+    p.row_map = reinterpret_cast<const int*>(ws + l.row_map);
+  }
+  p.partial = reinterpret_cast<float2*>(ws + l.partial);
+  p.at_target = reinterpret_cast<float*>(ws + l.at_target);
+  if ((rc = launch_stats(p, dev, s)) != IXK_OK) return rc;
+  Loss a{};
+  a.has = has;
+  a.partial = p.partial;
+  a.at_target = p.at_target;
+  a.weight = t.weight;
+  a.active = p.active_rows;
+  a.row_map = p.row_map;
+  a.rows = static_cast<int>(d->rows);
+  a.slots = static_cast<int>(l.slots);
+  a.entries = t.entries;
+  a.factor = scales.loss;
+  a.loss = loss;
+  a.lse = lse;
+  auto go = [&](auto rows) -> int {
+    constexpr int kRows = decltype(rows)::value;
+    return launch_overlapped(loss_kernel<kRows>, dim3(static_cast<unsigned>((d->rows + kRows - 1) / kRows)), dim3(kLossThreads), 0, s, a);
+  };
+  // (rows side by side are one read of up to 256 bytes; few rows want a CTA each)
+  if (d->rows >= 4096) return go(std::integral_constant<int, 32>{});
+  if (d->rows >= 512) return go(std::integral_constant<int, 8>{});
+  return go(std::integral_constant<int, 1>{});
+}
+
+int backward(const char* name, const ixk_linear_loss_desc* d, bool distill, const void* x, const void* w, const void* bias,
+             const void* index, const void* teacher, const float* lse, const float* grad_loss, void* dx, void* dw, void* dbias,
+             void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check(d, name, distill, true, x, w, bias, index, teacher);
+  if (rc != IXK_OK) return rc;
+  const std::string who = std::string(name) + ": ";
+  if (d->rows > 0 && (lse == nullptr || grad_loss == nullptr)) return fail(IXK_INVALID_ARGUMENT, who + "lse and grad_loss must be non-NULL");
+  if (dbias != nullptr && bias == nullptr) return fail(IXK_INVALID_ARGUMENT, who + "dbias without a bias");
+  if (!aligned(lse, 4) || !aligned(grad_loss, 4) || !aligned(dx, 2) || !aligned(dw, 2) || !aligned(dbias, 2))
+    return fail(IXK_INVALID_ARGUMENT, who + "a pointer is not aligned to its element size");
+  if (d->grad_loss_stride < 0) return fail(IXK_INVALID_ARGUMENT, who + "grad_loss_stride must not be negative");
+  DeviceInfo dev;
+  auto s = static_cast<cudaStream_t>(stream);
+  if (d->rows == 0) {      // sums over no rows
+    if ((rc = get_device_info(&dev)) != IXK_OK) return rc;
+    const bool row_major = d->dw_order == IXK_ROW_MAJOR;
+    if (dw != nullptr)
+      IXK_CUDA_OK(cudaMemset2DAsync(dw, d->dw_stride * 2, 0, (row_major ? d->hidden : d->vocab) * 2, row_major ? d->vocab : d->hidden, s));
+    if (dbias != nullptr) IXK_CUDA_OK(cudaMemsetAsync(dbias, 0, d->vocab * 2, s));
+    return IXK_OK;
+  }
+  const Layout l = layout_for(*d, true);
+  if ((rc = check_space(name, l, workspace, workspace_bytes)) != IXK_OK) return rc;
+  if ((rc = get_device_info(&dev)) != IXK_OK) return rc;
+  char* ws = static_cast<char*>(workspace);
+  const Scales scales = scales_of(*d, distill);
+  const bool bf16 = d->dtype == IXK_BF16;
+  Targets t{};
+  HasTarget has{};
+  if ((rc = targets_of(*d, l, ws, index, teacher, s, &t, &has)) != IXK_OK) return rc;
+  // fp16: G = g (p - q) with g = 1 / tokens and p = 1 / vocabulary would be lost below its smallest numbers
+  const bool ranged = !bf16;
+  if ((rc = gather(*d, l, ws, has, x, nullptr, nullptr, grad_loss, scales.grad, ranged, s)) != IXK_OK) return rc;
+  Pass p = pass_of(*d, scales, ws + l.packed, l.ldp, w, bias, t);
+  p.active_rows = reinterpret_cast<const int*>(ws + l.active);
+  p.row_map = reinterpret_cast<const int*>(ws + l.row_map);
+  p.lse = lse;
+  p.grad_loss = grad_loss;
+  p.grad_stride = d->grad_loss_stride;
+  p.factor = scales.grad;
+  p.range = ranged ? reinterpret_cast<const float*>(ws + l.active + 16) : nullptr;
+  p.grad = ws + l.grad;
+  p.ldg = l.ldg;
+  float* acc = reinterpret_cast<float*>(ws + l.acc);
+
+  gemm::Problem common;
+  common.kind = gemm::kKindF16;
+  common.ab_dtype = d->dtype;
+  common.a_fmt = common.b_fmt = bf16 ? 1u : 0u;
+  common.bias_dtype = d->dtype;
+  for (int64_t first = 0; first < d->vocab; first += l.piece) {
+    p.first = first;
+    p.count = std::min(l.piece, d->vocab - first);
+    if ((rc = launch_grad(p, dev, s)) != IXK_OK) return rc;
+    if (dw != nullptr) {       // dw[v, :] = sum over rows of G[row, v] x[row, :], or its transpose
+      gemm::Problem g = common;
+      const bool row_major = d->dw_order == IXK_ROW_MAJOR;
+      g.M = row_major ? p.count : d->hidden;
+      g.N = row_major ? d->hidden : p.count;
+      g.K = d->rows;
+      g.k_limit = p.active_rows;
+      g.a = row_major ? p.grad : p.x;
+      g.lda = row_major ? l.ldg : l.ldp;
+      g.b = row_major ? p.x : p.grad;
+      g.ldb = row_major ? l.ldp : l.ldg;
+      g.a_mn_major = g.b_mn_major = true;
+      g.d = static_cast<uint16_t*>(dw) + (row_major ? first * d->dw_stride : first);
+      g.ldd = g.ldc = d->dw_stride;
+      g.out_dtype = d->dtype;
+      g.acc_scale_dev = p.range != nullptr ? p.range + 1 : nullptr;
+      if ((rc = gemm::run_problem(g, ws + l.split, l.split_bytes, dev, s)) != IXK_OK) return rc;
+    }
+    if (dx != nullptr) {       // dx += G w
+      gemm::Problem g = common;
+      g.M = d->rows;
+      g.N = d->hidden;
+      g.K = p.count;
+      // (the kernels for few rows take all of them: what comes of G's rows behind the active ones is not read)
+      if (d->rows > kDirectRows) g.m_limit = p.active_rows;
+      g.a = p.grad;
+      g.lda = l.ldg;
+      const bool row_major = d->w_order == IXK_ROW_MAJOR;
+      g.b = static_cast<const uint16_t*>(w) + (row_major ? first * d->w_stride : first);
+      g.ldb = d->w_stride;
+      g.b_mn_major = row_major;
+      g.d = acc;
+      g.c = acc;
+      g.ldd = g.ldc = l.ld_acc;
+      g.out_dtype = IXK_F32;
+      g.beta = first == 0 ? 0.0f : 1.0f;
+      if ((rc = gemm::run_problem(g, ws + l.split, l.split_bytes, dev, s)) != IXK_OK) return rc;
+    }
+    if (dbias != nullptr) {
+      auto* fn = bf16 ? bias_kernel<true> : bias_kernel<false>;
+      rc = launch_overlapped(fn, dim3(static_cast<unsigned>((p.count + kBiasCols - 1) / kBiasCols)), dim3(32 * kBiasGroups), 0, s,
+                             static_cast<const uint16_t*>(p.grad), l.ldg, p.active_rows, static_cast<int>(p.count), p.range,
+                             static_cast<uint16_t*>(dbias) + first);
+      if (rc != IXK_OK) return rc;
+    }
+  }
+  if (dx == nullptr) return IXK_OK;
+  const int vec = aligned(dx, 16) && d->dx_stride % 8 == 0;
+  auto* fn = bf16 ? scatter_kernel<true> : scatter_kernel<false>;
+  return launch_overlapped(fn, dim3(static_cast<unsigned>(d->rows)), dim3(256), 0, s, static_cast<const float*>(acc), l.ld_acc,
+                           reinterpret_cast<const int*>(ws + l.inverse), p.range, static_cast<int>(d->hidden), vec, static_cast<uint16_t*>(dx),
+                           d->dx_stride);
+}
+
+}  // namespace
+}  // namespace head
+}  // namespace ixk
+
+extern "C" {
+
+int ixk_linear_xent_fwd(const ixk_linear_loss_desc* desc, const void* x, const void* weight, const void* bias, const void* labels,
+                        float* loss, float* lse, void* workspace, size_t workspace_bytes, void* cuda_stream) {
+  IXK_API_RANGE("ixk_linear_xent_fwd");
+  ixk::clear_error();
+  return ixk::head::forward("linear_xent_fwd", desc, false, x, weight, bias, labels, nullptr, loss, lse, workspace, workspace_bytes, cuda_stream);
+}
+
+int ixk_linear_xent_bwd(const ixk_linear_loss_desc* desc, const void* x, const void* weight, const void* bias, const void* labels,
+                        const float* lse, const float* grad_loss, void* dx, void* dweight, void* dbias, void* workspace,
+                        size_t workspace_bytes, void* cuda_stream) {
+  IXK_API_RANGE("ixk_linear_xent_bwd");
+  ixk::clear_error();
+  return ixk::head::backward("linear_xent_bwd", desc, false, x, weight, bias, labels, nullptr, lse, grad_loss, dx, dweight, dbias, workspace,
+                             workspace_bytes, cuda_stream);
+}
+
+int ixk_linear_distill_fwd(const ixk_linear_loss_desc* desc, const void* x, const void* weight, const void* bias, const void* index,
+                           const void* teacher, float* loss, float* lse, void* workspace, size_t workspace_bytes, void* cuda_stream) {
+  IXK_API_RANGE("ixk_linear_distill_fwd");
+  ixk::clear_error();
+  return ixk::head::forward("linear_distill_fwd", desc, true, x, weight, bias, index, teacher, loss, lse, workspace, workspace_bytes, cuda_stream);
+}
+
+int ixk_linear_distill_bwd(const ixk_linear_loss_desc* desc, const void* x, const void* weight, const void* bias, const void* index,
+                           const void* teacher, const float* lse, const float* grad_loss, void* dx, void* dweight, void* dbias,
+                           void* workspace, size_t workspace_bytes, void* cuda_stream) {
+  IXK_API_RANGE("ixk_linear_distill_bwd");
+  ixk::clear_error();
+  return ixk::head::backward("linear_distill_bwd", desc, true, x, weight, bias, index, teacher, lse, grad_loss, dx, dweight, dbias, workspace,
+                             workspace_bytes, cuda_stream);
+}
+
+size_t ixk_linear_loss_workspace_bytes(const ixk_linear_loss_desc* desc, int backward) {
+  if (desc == nullptr || desc->rows <= 0 || desc->hidden <= 0 || desc->vocab <= 0 || desc->entries < 0 || desc->rows > (1 << 24) ||
+      desc->hidden > (1 << 20) || desc->vocab > (1 << 24) || desc->entries > ixk::head::kMaxEntries)
+    return 0;
+  return ixk::head::layout_for(*desc, backward != 0).space.total;
+}
+
+}  // extern "C"

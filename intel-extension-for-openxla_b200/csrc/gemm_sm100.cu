@@ -205,6 +205,7 @@ __device__ __forceinline__ void epilogue_tile(const KernelArgs& args, const CUte
   const bool vec_d = args.d_vec_ok != 0;
   const bool vec_c = args.c_vec_ok != 0;
   const bool vec_bias = args.bias_vec_ok != 0;
+  const float acc_scale = args.acc_scale_dev != nullptr ? args.acc_scale * *args.acc_scale_dev : args.acc_scale;
       const int m = bm * kBlockM + row_in_tile;
     const bool row_ok = m < args.M;
     const int64_t d_row = bz * args.d_batch_stride + static_cast<int64_t>(m) * args.ldd;
@@ -220,7 +221,7 @@ __device__ __forceinline__ void epilogue_tile(const KernelArgs& args, const CUte
         return;
       }
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) * args.acc_scale;
+      for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) * acc_scale;
       if (args.bias != nullptr) {
         float b[32];
         load_row16(args.bias, bz * args.bias_batch_stride + n, args.bias_dtype, count, vec_bias, b);
@@ -360,7 +361,18 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
   ptx::grid_dependency_sync();   // (set-up above overlaps the kernel before this one, see launch_one)
 
   const int num_kb = (args.K + kSlabElems - 1) / kSlabElems;
-  const int num_tiles = args.tiles_m * args.tiles_n * args.batch;
+  const int tiles_m = args.m_limit != nullptr ? (min(*args.m_limit, args.M) + kBlockM - 1) / kBlockM : args.tiles_m;
+  const int num_tiles = tiles_m * args.tiles_n * args.batch;
+  // A tile's slabs of K, all or chunk bz of them.  A chunk behind *k_limit is one slab behind K, which TMA fills with zeros.
+  const int end_kb = args.k_limit != nullptr ? min((*args.k_limit + kSlabElems - 1) / kSlabElems, num_kb) : num_kb;
+  auto slabs_of = [&](int bz, int& kb0, int& kb1) {
+    kb0 = args.k_chunk * bz;                                                  // (0 without chunks)
+    kb1 = args.k_chunk > 0 ? min(end_kb, kb0 + args.k_chunk) : end_kb;
+    if (kb1 <= kb0) {
+      kb0 = num_kb;
+      kb1 = num_kb + 1;
+    }
+  };
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
@@ -371,13 +383,13 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
       bool alive = true;
       for (int t = blockIdx.x; t < num_tiles && alive; t += gridDim.x) {
         int bz, bm, bn;
-        tile_coords(t, args.tiles_m, args.tiles_n, bz, bm, bn);
+        tile_coords(t, tiles_m, args.tiles_n, bz, bm, bn);
         const int m0 = bm * kBlockM;
         const int n0 = bn * kBlockN;
         const int az = args.a_broadcast || args.k_chunk > 0 ? 0 : bz;
         const int zb = args.k_chunk > 0 ? 0 : bz;
-        const int kb0 = args.k_chunk * bz;                                                  // (0 without chunks)
-        const int kb1 = args.k_chunk > 0 ? min(num_kb, kb0 + args.k_chunk) : num_kb;
+        int kb0, kb1;
+        slabs_of(bz, kb0, kb1);
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!ptx::mbar_wait(empty_bar(stage), phase ^ 1u, ctl, kSiteProducer)) {
             alive = false;
@@ -439,8 +451,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
         if (!ptx::mbar_wait(acc_empty_bar(buf), acc_phase ^ 1u, ctl, kSiteMmaAcc)) break;
         ptx::tc_fence_after_sync();
         const uint32_t d_tmem = tmem_base + buf * kBlockN;
-        const int chunk0 = args.k_chunk * (t / (args.tiles_m * args.tiles_n));
-        const int count = args.k_chunk > 0 ? min(num_kb - chunk0, args.k_chunk) : num_kb;
+        int kb0, kb1;
+        slabs_of(t / (tiles_m * args.tiles_n), kb0, kb1);
+        const int count = kb1 - kb0;
         for (int kb = 0; kb < count; ++kb) {
           if (!ptx::mbar_wait(full_bar(stage), phase, ctl, kSiteMmaFull)) {
             alive = false;
@@ -475,7 +488,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
     uint32_t n_store = 0;  // TMA stores issued by this warp (alternating between its two boxes)
     for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
       int bz, bm, bn;
-      tile_coords(t, args.tiles_m, args.tiles_n, bz, bm, bn);
+      tile_coords(t, tiles_m, args.tiles_n, bz, bm, bn);
       if (!ptx::mbar_wait(acc_full_bar(buf), acc_phase, ctl, kSiteEpilogue)) break;
       ptx::tc_fence_after_sync();
       epilogue_tile<kBlockN>(args, &tmap_d, tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * kBlockN, stage_smem,
@@ -518,6 +531,13 @@ struct PairCfg {
   static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
 constexpr int kMaxTailParts = 4;  // pieces of a tile of the last round
+// The tiles beyond the last full round of pairs are cut into 2 or 4 narrower ones where the idle pairs
+// can take the pieces: the round then takes about 1/2 or 1/3 of its time.  Returns the first tile that is cut.
+__host__ __device__ inline int tail_split(int64_t tiles, int pairs, bool may_cut, int& parts) {
+  const int tail = may_cut ? static_cast<int>(tiles % pairs) : 0;
+  parts = tail == 0 ? 1 : tail * kMaxTailParts <= pairs ? kMaxTailParts : tail * 2 <= pairs ? 2 : 1;
+  return static_cast<int>(tiles - tail);
+}
 enum : int { kSitePairFull = 111, kSitePairPeer = 112, kSitePairAcc = 113, kSitePairForward = 114 };
 
 // The tensor maps of D: one, or one per destination of a scattered output (rows of D dealt out
@@ -592,13 +612,25 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
   const uint32_t tmem_base = *tmem_slot;
   ptx::grid_dependency_sync();
 
-  const int num_kb = (args.K + kSlabElems - 1) / kSlabElems;
-  const int tiles_m2 = (args.tiles_m + 1) / 2;  // pair tiles along M
+  int num_kb = (args.K + kSlabElems - 1) / kSlabElems, first_kb = 0;
+  if (args.k_limit != nullptr) {
+    const int end_kb = min((*args.k_limit + kSlabElems - 1) / kSlabElems, num_kb);
+    first_kb = end_kb > 0 ? 0 : num_kb;       // (none: one slab behind K, which TMA fills with zeros)
+    num_kb = end_kb > 0 ? end_kb : 1;
+  }
+  int tiles_m2 = (args.tiles_m + 1) / 2;  // pair tiles along M
   const int pair_id = blockIdx.x >> 1;
   const int num_pairs = gridDim.x >> 1;
   // Units of work: whole tiles, then the tiles of the last round cut into tail_parts narrower ones.
-  const int num_units = args.tail_from + (tiles_m2 * args.tiles_n * args.batch - args.tail_from) * args.tail_parts;
-  const int tail_width = kBlockN / args.tail_parts;
+  int tail_from = args.tail_from, tail_parts = args.tail_parts;
+  uint32_t idesc_tail = args.idesc_tail;
+  if (args.m_limit != nullptr) {              // the last round of the rows that there are
+    tiles_m2 = (min(*args.m_limit, args.M) + 2 * kBlockM - 1) / (2 * kBlockM);
+    tail_from = tail_split(tiles_m2 * args.tiles_n, args.round_pairs, args.b_mn_major != 0, tail_parts);
+    idesc_tail = (args.idesc & ~(0x3fu << 17)) | static_cast<uint32_t>((kBlockN / tail_parts) >> 3) << 17;
+  }
+  const int num_units = tail_from + (tiles_m2 * args.tiles_n * args.batch - tail_from) * tail_parts;
+  const int tail_width = kBlockN / tail_parts;
   struct Unit {
     int bz, bm2, n_first, width;
   };
@@ -606,9 +638,9 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
     Unit x;
     int t = u, part = 0, bn;
     x.width = kBlockN;
-    if (u >= args.tail_from) {
-      t = args.tail_from + (u - args.tail_from) / args.tail_parts;
-      part = (u - args.tail_from) % args.tail_parts;
+    if (u >= tail_from) {
+      t = tail_from + (u - tail_from) / tail_parts;
+      part = (u - tail_from) % tail_parts;
       x.width = tail_width;
     }
     tile_coords(t, tiles_m2, args.tiles_n, x.bz, x.bm2, bn);
@@ -630,7 +662,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
       const int az = args.a_broadcast ? 0 : bz;
       const int b_boxes = (half_n + kSlabElems - 1) / kSlabElems;   // MN-major: boxes of one swizzle span of columns
       const uint32_t stage_bytes = kATileBytes + (args.b_mn_major ? b_boxes * kSlabElems : half_n) * kSlabBytes;
-      const CUtensorMap* map_b = t < args.tail_from ? &tmap_b : &tmap_b_tail;
+      const CUtensorMap* map_b = t < tail_from ? &tmap_b : &tmap_b_tail;
       for (int kb = 0; kb < num_kb; ++kb) {
         if (!ptx::mbar_wait(empty_bar(stage), phase ^ 1u, ctl, kSiteProducer)) {
           alive = false;
@@ -640,7 +672,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
         const uint32_t b_dst = a_dst + kATileBytes;
         // both CTAs' copies are counted on the EVEN CTA's barrier, which its issuer waits on
         const uint32_t bar = ptx::map_to_cta(full_bar(stage), 0);
-        const int k0 = kb * kSlabElems;
+        const int k0 = (first_kb + kb) * kSlabElems;
         if (ptx::elect_one()) {
           if (rank == 0) ptx::mbar_expect_tx(full_bar(stage), 2 * stage_bytes);
           if (args.a_mn_major) {
@@ -684,7 +716,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
     for (int t = pair_id; t < num_units && alive; t += num_pairs) {
       if (!ptx::mbar_wait(acc_empty_bar(buf), acc_phase ^ 1u, ctl, kSitePairAcc)) break;
       ptx::tc_fence_after_sync();
-      const uint32_t idesc = t < args.tail_from ? args.idesc : args.idesc_tail;
+      const uint32_t idesc = t < tail_from ? args.idesc : idesc_tail;
       const uint32_t d_tmem = tmem_base + buf * kBlockN;
       for (int kb = 0; kb < num_kb; ++kb) {
         if (!ptx::mbar_wait(full_bar(stage), phase, ctl, kSitePairFull)) {
@@ -831,11 +863,8 @@ int launch(const Problem& p, const DeviceInfo& dev, cudaStream_t stream) {
   bool pair = bn == 256 && tiles_m_all >= 2 && p.k_chunk == 0 && pair_tiles >= dev.sm_count / 2;
   if (const char* env = std::getenv("IXK_GEMM_PAIR")) pair = pair && std::atoi(env) != 0;
   const int b_box_rows = pair ? 128 : bn;
-  // The tiles beyond the last full round of pairs are cut into 2 or 4 narrower ones where the idle pairs
-  // can take the pieces: the round then takes about 1/2 or 1/3 of its time.
-  const int64_t pairs_all = dev.sm_count / 2;
-  const int64_t tail_tiles = pair && p.scatter_world == 0 ? pair_tiles % pairs_all : 0;
-  const int tail_parts = tail_tiles == 0 ? 1 : tail_tiles * kMaxTailParts <= pairs_all ? kMaxTailParts : tail_tiles * 2 <= pairs_all ? 2 : 1;
+  int tail_parts = 1;
+  const int tail_from = tail_split(pair_tiles, dev.sm_count / 2, pair && p.scatter_world == 0, tail_parts);
   if (p.scatter_world > 0) {
     // Only the kernel that large projections run on stores to several destinations, and only
     // whole row blocks of one CTA.
@@ -905,7 +934,7 @@ int launch(const Problem& p, const DeviceInfo& dev, cudaStream_t stream) {
   k.b_mn_major = p.b_mn_major;
   k.idesc = ptx::umma_idesc(p.a_fmt, p.b_fmt, p.a_mn_major ? 1 : 0, p.b_mn_major ? 1 : 0, pair ? 2 * kBlockM : kBlockM, bn,
                             p.kind == ptx::kKindI8 ? 2u : 1u);
-  k.tail_from = static_cast<int>(pair_tiles - tail_tiles);
+  k.tail_from = tail_from;
   k.tail_parts = tail_parts;
   k.idesc_tail = ptx::umma_idesc(p.a_fmt, p.b_fmt, p.a_mn_major ? 1 : 0, p.b_mn_major ? 1 : 0, 2 * kBlockM, PairCfg::kBlockN / tail_parts,
                                  p.kind == ptx::kKindI8 ? 2u : 1u);
@@ -921,6 +950,10 @@ int launch(const Problem& p, const DeviceInfo& dev, cudaStream_t stream) {
   k.act = p.act;
   k.acc_scale = p.acc_scale;
   k.beta = p.beta;
+  k.m_limit = p.m_limit;
+  k.k_limit = p.k_limit;
+  k.acc_scale_dev = p.acc_scale_dev;
+  k.round_pairs = dev.sm_count / 2;
   k.status_word = dev.status_word;
   const int out_es = (p.out_dtype == IXK_F32 || p.out_dtype == IXK_S32) ? 4 : 2;
   const int bias_es = p.bias_dtype == IXK_F32 ? 4 : 2;

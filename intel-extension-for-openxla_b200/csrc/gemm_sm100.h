@@ -38,6 +38,12 @@ struct Problem {
   int act = kActNone;
   float acc_scale = 1.0f;
   float beta = 0.0f;
+  // Sizes and a factor that only the GPU knows (the rows of a batch that count), nullptr: none.  D's rows from *m_limit
+  // on are not computed; K ends at *k_limit (at most K; the operands hold zeros from there to a multiple of 64);
+  // acc_scale is multiplied by *acc_scale_dev.  16-bit operands, batch 1, no scattered output.
+  const int* m_limit = nullptr;
+  const int* k_limit = nullptr;
+  const float* acc_scale_dev = nullptr;
   int force_block_n = 0;  // tuning override; 0 = heuristic
   int k_chunk = 0;        // > 0: the batches are chunks of K, this many slabs each (the last one what is left), of one A and B
   // Scattered output (row-parallel projection feeding an all-reduce): row block o of D, rows
@@ -56,12 +62,15 @@ struct KernelArgs {
   uint32_t idesc;
   uint32_t idesc_tail;         // CTA-pair kernel: the narrower tiles of the last round
   int tail_from, tail_parts;   // tiles from here on are cut into this many (1: none is)
+  int round_pairs;             // CTA pairs of a full round
   const void* bias;
   const void* c;
   void* d;
   int64_t ldd, ldc, d_batch_stride, c_batch_stride;
   int out_dtype, bias_dtype, act;
   float acc_scale, beta;
+  const int *m_limit, *k_limit;   // see Problem
+  const float* acc_scale_dev;
   int d_vec_ok, c_vec_ok, bias_vec_ok;
   int d_tma;  // 16-bit D with 16-byte-aligned rows: stored through shared memory + TMA
   int a_broadcast;
@@ -72,6 +81,11 @@ struct KernelArgs {
   int scatter_rows;  // rows per destination of a scattered output; 0 = one destination
   int* status_word;
 };
+
+// D by whichever kernel suits the problem, K cut as far as the scratch goes.
+int run_problem(const Problem& p, void* workspace, size_t workspace_bytes, const DeviceInfo& dev, cudaStream_t stream);
+// Scratch that run_problem can use for a 16-bit problem of one batch.
+size_t problem_workspace_bytes(int64_t M, int64_t N, int64_t K);
 
 int pick_block_n(int64_t M, int64_t N, int64_t batch, int sm_count);
 int launch(const Problem& p, const DeviceInfo& dev, cudaStream_t stream);

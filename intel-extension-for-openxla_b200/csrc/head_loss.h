@@ -1,0 +1,55 @@
+// Interface between the losses at the vocabulary head (api_head_loss.cu) and their tensor-core kernel (head_loss_sm100.cu).
+#pragma once
+
+#include "host_common.h"
+
+namespace ixk {
+namespace head {
+
+constexpr int kNoColumn = 0x7fffffff;
+
+// What a row of the batch is measured against: one label, or a list of columns in ascending order with their weights.
+struct Targets {
+  const void* labels;       // cross entropy: [rows], int32 or int64; nullptr: lists
+  int wide;                 // 64-bit labels
+  int64_t ignore_index;
+  const int* column;        // distillation: [rows][entries] ascending, kNoColumn behind the last one
+  const float* weight;      // [rows][entries]
+  int entries;              // 1 for labels
+};
+
+// One pass over columns [first, first + count) of the logits x w^T + bias, tile by tile.
+struct Pass {
+  int dtype;
+  bool w_column_major;      // [hidden, vocab] in memory
+  int64_t rows, hidden, vocab;
+  const void *x, *w, *bias;
+  int64_t ldx, ldw;
+  float scale;              // of the logits
+  const int* active_rows;   // device: rows of x that there are, nullptr: all
+  const int* row_map;       // device: row of the batch that a row of x is, nullptr: the same
+  int64_t first, count;
+  Targets targets;
+  // statistics
+  float2* partial;          // [slots][rows]: maximum and sum of exponentials, base 2
+  float* at_target;         // [batch rows][entries]: scaled logits at the targets
+  // gradient
+  const float* lse;         // [batch rows]
+  const float* grad_loss;   // [batch rows], pitch grad_stride
+  int64_t grad_stride;
+  float factor;             // of the gradient, scale included
+  const float* range;       // device: power of two that keeps fp16 in range, nullptr: 1
+  void* grad;               // [rows up to a multiple of 256][count] of dtype, pitch ldg
+  int64_t ldg;
+};
+
+// Rows of `partial` that a statistics pass fills.
+int stat_slots(int64_t rows, int64_t vocab);
+// Columns that a piece of the gradient had best be a multiple of.
+constexpr int kPieceUnit = 256;
+
+int launch_stats(const Pass& p, const DeviceInfo& dev, cudaStream_t stream);
+int launch_grad(const Pass& p, const DeviceInfo& dev, cudaStream_t stream);
+
+}  // namespace head
+}  // namespace ixk
