@@ -5,8 +5,8 @@
 //   forward    [lists: a row's teacher entries sorted, their softmax]   (distillation)
 //              [gather: rows with a target side by side]                 (more than one row block)
 //              statistics of every row's logits -> loss: partials to lse and loss
-//   backward   [lists], gather, then per piece of the vocabulary: G = dloss/dlogits in 16 bits, dw = G^T x, dx += G w (the
-//              framework's GEMM, fp32 accumulator across the pieces), [dbias = sums of G]; scatter: dx to its rows
+//   backward   [lists], gather, then per piece of the vocabulary: G = dloss/dlogits in 16 bits, dw = G^T x and dx += G w (the
+//              framework's GEMM kernels, both in one launch; fp32 accumulator across the pieces), [dbias = sums of G]; scatter: dx to its rows
 //
 // Rows without a target cost nothing beyond the gather's copy: their number is known on the GPU only, and the kernels take
 // their row count from there.  Their hidden states are never multiplied, so nothing that they hold reaches a result.
@@ -27,9 +27,10 @@ namespace head {
 namespace {
 
 constexpr int kMaxEntries = 256;
-constexpr int64_t kDirectRows = 128;             // up to one row block there are no tiles to save: no gather
 constexpr size_t kPieceBytes = size_t(256) << 20;  // of G
-constexpr size_t kSplitBytes = size_t(64) << 20;   // of the GEMMs' K chunks
+constexpr size_t kSplitBytes = size_t(64) << 20;   // of the GEMMs' K chunks, for few rows
+constexpr size_t kPlaneBytes = size_t(128) << 20;  // of dx's planes, for more
+constexpr int kMaxPlanes = 16;
 constexpr int kSlabRows = 64;                    // rows that the product along the rows reads at a time
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -133,18 +134,31 @@ struct HasTarget {
   }
 };
 
+// Numbers that the GPU finds out and later kernels read.
+struct Control {
+  int active;          // rows with a target
+  int plane_slabs;     // slabs of the vocabulary's piece per plane of dx (gemm::two_plan), and the planes
+  int planes;
+  int pad;
+  float range[2];      // power of two for fp16's gradient, and its inverse
+};
+
 struct Gather {
   HasTarget has;
   const uint16_t* x;
   uint16_t* packed;            // the rows with a target, pitch ldp
   int64_t ldx, ldp;
   int rows, hidden, rows_per_cta;
-  int *active, *row_map, *inverse;   // inverse may be nullptr
+  Control* control;
+  int *row_map, *inverse;      // inverse may be nullptr
   float *loss, *lse;           // zeroed where there is no target; may be nullptr
-  const float* grad_loss;      // with range: the power of two that brings the largest row's gradient to 2^13 .. 2^14
+  // backward: control's range is the power of two that brings the largest row's gradient to 2^13 .. 2^14
+  const float* grad_loss;
   int64_t grad_stride;
   float factor;
-  float* range;                // [2]: it and its inverse; may be nullptr
+  int ranged;
+  // and the products' plan: tiles of a row block of dx, of dw; slabs of a piece
+  int dx_tiles_n, piece_slabs, dw_tiles, pairs, max_planes;
 };
 
 constexpr int kGatherThreads = 256;
@@ -196,13 +210,21 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Gather a) 
     for (int c = whole * 8 + lane; c < a.hidden; c += 32) dst[c] = src[c];
   }
   if (end != a.rows) return;
-  // the last CTA: how many there are, zeros behind them up to the end of a slab, and the gradient's range
+  // the last CTA: how many there are, zeros behind them as far as the products read, and the gradient's range
   const int total = before + here;
-  if (threadIdx.x == 0) *a.active = total;
-  const int zero_end = min((total + kSlabRows - 1) / kSlabRows * kSlabRows, a.rows);
+  if (threadIdx.x == 0) {
+    a.control->active = total;
+    if (a.dx_tiles_n > 0) {
+      const int64_t tiles = (static_cast<int64_t>(total) + gemm::kTwoTile - 1) / gemm::kTwoTile * a.dx_tiles_n;
+      const int slabs = gemm::two_plan(tiles, a.piece_slabs, a.dw_tiles, max((total + kSlabRows - 1) / kSlabRows, 1), a.pairs, a.max_planes);
+      a.control->plane_slabs = slabs;
+      a.control->planes = (a.piece_slabs + slabs - 1) / slabs;
+    }
+  }
+  const int zero_end = a.rows <= kDirectRows ? a.rows : min((total + kSlabRows - 1) / kSlabRows * kSlabRows, a.rows);
   for (int i = total + warp; i < zero_end; i += kGatherThreads / 32)
     for (int c = lane; c < a.hidden; c += 32) a.packed[i * a.ldp + c] = 0;
-  if (a.range != nullptr) {
+  if (a.ranged) {
     float top = 0.0f;
     for (int i = threadIdx.x; i < a.rows; i += kGatherThreads)
       if (a.has(i)) top = fmaxf(top, fabsf(a.grad_loss[i * a.grad_stride] * a.factor));
@@ -214,8 +236,8 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Gather a) 
       for (int w = 0; w < kGatherThreads / 32; ++w) top = fmaxf(top, warp_top[w]);
       int e = 0;
       if (top >= FLT_MIN && top <= FLT_MAX) e = min(13 - ilogbf(top), 126);
-      a.range[0] = scalbnf(1.0f, e);
-      a.range[1] = scalbnf(1.0f, -e);
+      a.control->range[0] = scalbnf(1.0f, e);
+      a.control->range[1] = scalbnf(1.0f, -e);
     }
   }
 }
@@ -300,11 +322,10 @@ __device__ __forceinline__ uint32_t to16(float f) {
 // dbias of a piece: the sums of G's columns.  256 columns per CTA, 32 warps that take rows in turn.
 constexpr int kBiasCols = 256, kBiasGroups = 32;
 template <bool kBf16>
-__global__ void __launch_bounds__(32 * kBiasGroups) bias_kernel(const uint16_t* g, int64_t ldg, const int* active, int count, const float* range,
-                                                              uint16_t* out) {
+__global__ void __launch_bounds__(32 * kBiasGroups) bias_kernel(const uint16_t* g, int64_t ldg, const Control* control, int count, uint16_t* out) {
   __shared__ float sums[kBiasGroups][kBiasCols];
   ptx::grid_dependency_sync();
-  const int group = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = *active;
+  const int group = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = control->active;
   const int c0 = blockIdx.x * kBiasCols + lane * 8;
   float t[8] = {};
   if (c0 < count) {      // (G's pitch is whole vectors)
@@ -327,25 +348,31 @@ __global__ void __launch_bounds__(32 * kBiasGroups) bias_kernel(const uint16_t* 
   if (threadIdx.x < kBiasCols && c < count) {
     float s = 0.0f;
     for (int i = 0; i < kBiasGroups; ++i) s += sums[i][threadIdx.x];
-    out[c] = static_cast<uint16_t>(to16<kBf16>(range != nullptr ? s * range[1] : s));
+    out[c] = static_cast<uint16_t>(to16<kBf16>(kBf16 ? s : s * control->range[1]));
   }
 }
 
-// dx: the accumulator's rows back to where they came from, rounded once; zeros where there was no target.
+// dx: the accumulator's rows, their planes added up, back to where they came from, rounded once; zeros where there was no
+// target.
 template <bool kBf16>
-__global__ void __launch_bounds__(256) scatter_kernel(const float* acc, int64_t ld_acc, const int* inverse, const float* range, int hidden,
-                                                      int vec, uint16_t* dx, int64_t ld) {
+__global__ void __launch_bounds__(256) scatter_kernel(const float* acc, int64_t ld_acc, int64_t plane, const int* inverse, const Control* control,
+                                                      int hidden, int vec, uint16_t* dx, int64_t ld) {
   ptx::grid_dependency_sync();
   const int64_t row = blockIdx.x;
-  const int from = inverse[row];
-  const float scale = range != nullptr ? range[1] : 1.0f;
+  const int from = inverse[row], planes = plane > 0 ? control->planes : 1;
+  const float scale = kBf16 ? 1.0f : control->range[1];
   const float* src = acc + from * ld_acc;
   uint16_t* dst = dx + row * ld;
   const int vecs = vec ? hidden / 8 : 0;
   for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
     uint4 w = make_uint4(0, 0, 0, 0);
     if (from >= 0) {
-      const float4 a = reinterpret_cast<const float4*>(src)[2 * v], b = reinterpret_cast<const float4*>(src)[2 * v + 1];
+      float4 a = reinterpret_cast<const float4*>(src)[2 * v], b = reinterpret_cast<const float4*>(src)[2 * v + 1];
+      for (int i = 1; i < planes; ++i) {
+        const float4 c = reinterpret_cast<const float4*>(src + i * plane)[2 * v], d = reinterpret_cast<const float4*>(src + i * plane)[2 * v + 1];
+        a = make_float4(a.x + c.x, a.y + c.y, a.z + c.z, a.w + c.w);
+        b = make_float4(b.x + d.x, b.y + d.y, b.z + d.z, b.w + d.w);
+      }
       w.x = to16<kBf16>(a.x * scale) | to16<kBf16>(a.y * scale) << 16;
       w.y = to16<kBf16>(a.z * scale) | to16<kBf16>(a.w * scale) << 16;
       w.z = to16<kBf16>(b.x * scale) | to16<kBf16>(b.y * scale) << 16;
@@ -353,8 +380,12 @@ __global__ void __launch_bounds__(256) scatter_kernel(const float* acc, int64_t 
     }
     reinterpret_cast<uint4*>(dst)[v] = w;
   }
-  for (int c = vecs * 8 + threadIdx.x; c < hidden; c += blockDim.x)
-    dst[c] = from >= 0 ? static_cast<uint16_t>(to16<kBf16>(src[c] * scale)) : static_cast<uint16_t>(0);
+  for (int c = vecs * 8 + threadIdx.x; c < hidden; c += blockDim.x) {
+    float t = 0.0f;
+    if (from >= 0)
+      for (int i = 0; i < planes; ++i) t += src[i * plane + c];
+    dst[c] = static_cast<uint16_t>(to16<kBf16>(t * scale));
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -373,9 +404,10 @@ struct Space {
 
 struct Layout {
   Space space;
-  size_t active, row_map, column, weight, has, packed, at_target, partial;      // forward
+  size_t control, row_map, column, weight, has, packed, at_target, partial;      // forward
   size_t inverse, grad, acc, split, split_bytes;                               // backward
-  int64_t ldp, slots, piece, ldg, ld_acc;
+  int64_t ldp, slots, piece, ldg, ld_acc, plane;      // plane 0: dx is not cut into planes
+  int planes;
   bool gathered;
 };
 
@@ -383,7 +415,7 @@ Layout layout_for(const ixk_linear_loss_desc& d, bool backward) {
   Layout l{};
   const int64_t N = d.rows, D = d.hidden, V = d.vocab, K = std::max<int64_t>(d.entries, 1);
   l.gathered = backward || N > kDirectRows;
-  l.active = l.space.take(256);      // (and the range)
+  l.control = l.space.take(sizeof(Control));
   l.row_map = l.space.take(4 * N);
   if (d.entries > 0) {
     l.column = l.space.take(4 * N * K);
@@ -406,9 +438,15 @@ Layout layout_for(const ixk_linear_loss_desc& d, bool backward) {
   l.ldg = round_up(l.piece, 8);
   l.grad = l.space.take(2 * rows * l.ldg);
   l.ld_acc = round_up(D, 4);
-  l.acc = l.space.take(4 * N * l.ld_acc);
-  l.split_bytes = std::min(std::max(gemm::problem_workspace_bytes(N, D, l.piece), gemm::problem_workspace_bytes(D, l.piece, N)), kSplitBytes);
-  l.split = l.space.take(l.split_bytes);
+  if (N > kDirectRows) {
+    l.plane = N * l.ld_acc;
+    l.planes = static_cast<int>(std::clamp<int64_t>(kPlaneBytes / (4 * l.plane), 1, kMaxPlanes));
+    l.acc = l.space.take(4 * l.plane * l.planes);
+  } else {
+    l.acc = l.space.take(4 * N * l.ld_acc);
+    l.split_bytes = std::min(std::max(gemm::problem_workspace_bytes(N, D, l.piece), gemm::problem_workspace_bytes(l.piece, D, N)), kSplitBytes);
+    l.split = l.space.take(l.split_bytes);
+  }
   return l;
 }
 
@@ -499,7 +537,8 @@ int targets_of(const ixk_linear_loss_desc& d, const Layout& l, char* ws, const v
 }
 
 int gather(const ixk_linear_loss_desc& d, const Layout& l, char* ws, const HasTarget& has, const void* x, float* loss, float* lse,
-           const float* grad_loss, float factor, bool range, cudaStream_t stream) {
+           const float* grad_loss, float factor, bool want_dw, int sm_count, cudaStream_t stream) {
+  const bool backward = loss == nullptr;
   Gather g{};
   g.has = has;
   g.x = static_cast<const uint16_t*>(x);
@@ -510,15 +549,22 @@ int gather(const ixk_linear_loss_desc& d, const Layout& l, char* ws, const HasTa
   g.hidden = static_cast<int>(d.hidden);
   // (each CTA counts the rows in front of it: at most 512 CTAs while a CTA's rows fit its threads)
   g.rows_per_cta = static_cast<int>(std::min<int64_t>(std::max<int64_t>(16, (d.rows + 511) / 512), kGatherThreads));
-  g.active = reinterpret_cast<int*>(ws + l.active);
+  g.control = reinterpret_cast<Control*>(ws + l.control);
   g.row_map = reinterpret_cast<int*>(ws + l.row_map);
-  g.inverse = loss == nullptr ? reinterpret_cast<int*>(ws + l.inverse) : nullptr;
+  g.inverse = backward ? reinterpret_cast<int*>(ws + l.inverse) : nullptr;
   g.loss = loss;
   g.lse = lse;
   g.grad_loss = grad_loss;
   g.grad_stride = d.grad_loss_stride;
   g.factor = factor;
-  g.range = range ? reinterpret_cast<float*>(ws + l.active + 16) : nullptr;
+  g.ranged = backward && d.dtype == IXK_F16;
+  if (backward && l.plane > 0) {
+    g.dx_tiles_n = static_cast<int>((d.hidden + gemm::kTwoTile - 1) / gemm::kTwoTile);
+    g.piece_slabs = static_cast<int>((l.piece + kSlabRows - 1) / kSlabRows);
+    g.dw_tiles = want_dw ? g.dx_tiles_n * static_cast<int>((l.piece + gemm::kTwoTile - 1) / gemm::kTwoTile) : 0;
+    g.pairs = sm_count / 2;
+    g.max_planes = l.planes;
+  }
   const int64_t ctas = (d.rows + g.rows_per_cta - 1) / g.rows_per_cta;
   return launch_overlapped(gather_kernel, dim3(static_cast<unsigned>(ctas)), dim3(kGatherThreads), 0, stream, g);
 }
@@ -561,10 +607,10 @@ int forward(const char* name, const ixk_linear_loss_desc* d, bool distill, const
   if ((rc = targets_of(*d, l, ws, index, teacher, s, &t, &has)) != IXK_OK) return rc;
   Pass p = pass_of(*d, scales, x, d->x_stride, w, bias, t);
   if (l.gathered) {
-    if ((rc = gather(*d, l, ws, has, x, loss, lse, nullptr, 0.0f, false, s)) != IXK_OK) return rc;
+    if ((rc = gather(*d, l, ws, has, x, loss, lse, nullptr, 0.0f, false, dev.sm_count, s)) != IXK_OK) return rc;
     p.x = ws + l.packed;
     p.ldx = l.ldp;
-    p.active_rows = reinterpret_cast<const int*>(ws + l.active);
+    p.active_rows = &reinterpret_cast<const Control*>(ws + l.control)->active;
     p.row_map = reinterpret_cast<const int*>(ws + l.row_map);
   }
   p.partial = reinterpret_cast<float2*>(ws + l.partial);
@@ -624,16 +670,16 @@ int backward(const char* name, const ixk_linear_loss_desc* d, bool distill, cons
   HasTarget has{};
   if ((rc = targets_of(*d, l, ws, index, teacher, s, &t, &has)) != IXK_OK) return rc;
   // fp16: G = g (p - q) with g = 1 / tokens and p = 1 / vocabulary would be lost below its smallest numbers
-  const bool ranged = !bf16;
-  if ((rc = gather(*d, l, ws, has, x, nullptr, nullptr, grad_loss, scales.grad, ranged, s)) != IXK_OK) return rc;
+  if ((rc = gather(*d, l, ws, has, x, nullptr, nullptr, grad_loss, scales.grad, dw != nullptr, dev.sm_count, s)) != IXK_OK) return rc;
   Pass p = pass_of(*d, scales, ws + l.packed, l.ldp, w, bias, t);
-  p.active_rows = reinterpret_cast<const int*>(ws + l.active);
+  const Control* control = reinterpret_cast<const Control*>(ws + l.control);
+  p.active_rows = &control->active;
   p.row_map = reinterpret_cast<const int*>(ws + l.row_map);
   p.lse = lse;
   p.grad_loss = grad_loss;
   p.grad_stride = d->grad_loss_stride;
   p.factor = scales.grad;
-  p.range = ranged ? reinterpret_cast<const float*>(ws + l.active + 16) : nullptr;
+  p.range = bf16 ? nullptr : control->range;
   p.grad = ws + l.grad;
   p.ldg = l.ldg;
   float* acc = reinterpret_cast<float*>(ws + l.acc);
@@ -647,31 +693,12 @@ int backward(const char* name, const ixk_linear_loss_desc* d, bool distill, cons
     p.first = first;
     p.count = std::min(l.piece, d->vocab - first);
     if ((rc = launch_grad(p, dev, s)) != IXK_OK) return rc;
-    if (dw != nullptr) {       // dw[v, :] = sum over rows of G[row, v] x[row, :], or its transpose
-      gemm::Problem g = common;
-      const bool row_major = d->dw_order == IXK_ROW_MAJOR;
-      g.M = row_major ? p.count : d->hidden;
-      g.N = row_major ? d->hidden : p.count;
-      g.K = d->rows;
-      g.k_limit = p.active_rows;
-      g.a = row_major ? p.grad : p.x;
-      g.lda = row_major ? l.ldg : l.ldp;
-      g.b = row_major ? p.x : p.grad;
-      g.ldb = row_major ? l.ldp : l.ldg;
-      g.a_mn_major = g.b_mn_major = true;
-      g.d = static_cast<uint16_t*>(dw) + (row_major ? first * d->dw_stride : first);
-      g.ldd = g.ldc = d->dw_stride;
-      g.out_dtype = d->dtype;
-      g.acc_scale_dev = p.range != nullptr ? p.range + 1 : nullptr;
-      if ((rc = gemm::run_problem(g, ws + l.split, l.split_bytes, dev, s)) != IXK_OK) return rc;
-    }
+    gemm::Problem both[2] = {common, common};
     if (dx != nullptr) {       // dx += G w
-      gemm::Problem g = common;
+      gemm::Problem& g = both[0];
       g.M = d->rows;
       g.N = d->hidden;
       g.K = p.count;
-      // (the kernels for few rows take all of them: what comes of G's rows behind the active ones is not read)
-      if (d->rows > kDirectRows) g.m_limit = p.active_rows;
       g.a = p.grad;
       g.lda = l.ldg;
       const bool row_major = d->w_order == IXK_ROW_MAJOR;
@@ -681,14 +708,38 @@ int backward(const char* name, const ixk_linear_loss_desc* d, bool distill, cons
       g.d = acc;
       g.c = acc;
       g.ldd = g.ldc = l.ld_acc;
+      g.d_batch_stride = g.c_batch_stride = l.plane;
       g.out_dtype = IXK_F32;
       g.beta = first == 0 ? 0.0f : 1.0f;
-      if ((rc = gemm::run_problem(g, ws + l.split, l.split_bytes, dev, s)) != IXK_OK) return rc;
+    }
+    if (dw != nullptr) {       // dw[v, :] = sum over rows of G[row, v] x[row, :], or its transpose
+      gemm::Problem& g = both[1];
+      const bool row_major = d->dw_order == IXK_ROW_MAJOR;
+      g.M = row_major ? p.count : d->hidden;
+      g.N = row_major ? d->hidden : p.count;
+      g.K = d->rows;
+      g.a = row_major ? p.grad : p.x;
+      g.lda = row_major ? l.ldg : l.ldp;
+      g.b = row_major ? p.x : p.grad;
+      g.ldb = row_major ? l.ldp : l.ldg;
+      g.a_mn_major = g.b_mn_major = true;
+      g.d = static_cast<uint16_t*>(dw) + (row_major ? first * d->dw_stride : first);
+      g.ldd = g.ldc = d->dw_stride;
+      g.out_dtype = d->dtype;
+      g.acc_scale_dev = p.range != nullptr ? p.range + 1 : nullptr;
+    }
+    if (l.plane > 0) {
+      both[0].m_limit = both[0].M > 0 ? p.active_rows : nullptr;
+      both[1].k_limit = both[1].M > 0 ? p.active_rows : nullptr;
+      if ((rc = gemm::launch_two(both, &control->plane_slabs, dev, s)) != IXK_OK) return rc;
+    } else {      // (one row block: both are streams of weights; G's rows and x's behind the active ones are zeros)
+      for (const gemm::Problem& g : both)
+        if (g.M > 0 && (rc = gemm::run_problem(g, ws + l.split, l.split_bytes, dev, s)) != IXK_OK) return rc;
     }
     if (dbias != nullptr) {
       auto* fn = bf16 ? bias_kernel<true> : bias_kernel<false>;
       rc = launch_overlapped(fn, dim3(static_cast<unsigned>((p.count + kBiasCols - 1) / kBiasCols)), dim3(32 * kBiasGroups), 0, s,
-                             static_cast<const uint16_t*>(p.grad), l.ldg, p.active_rows, static_cast<int>(p.count), p.range,
+                             static_cast<const uint16_t*>(p.grad), l.ldg, control, static_cast<int>(p.count),
                              static_cast<uint16_t*>(dbias) + first);
       if (rc != IXK_OK) return rc;
     }
@@ -696,8 +747,8 @@ int backward(const char* name, const ixk_linear_loss_desc* d, bool distill, cons
   if (dx == nullptr) return IXK_OK;
   const int vec = aligned(dx, 16) && d->dx_stride % 8 == 0;
   auto* fn = bf16 ? scatter_kernel<true> : scatter_kernel<false>;
-  return launch_overlapped(fn, dim3(static_cast<unsigned>(d->rows)), dim3(256), 0, s, static_cast<const float*>(acc), l.ld_acc,
-                           reinterpret_cast<const int*>(ws + l.inverse), p.range, static_cast<int>(d->hidden), vec, static_cast<uint16_t*>(dx),
+  return launch_overlapped(fn, dim3(static_cast<unsigned>(d->rows)), dim3(256), 0, s, static_cast<const float*>(acc), l.ld_acc, l.plane,
+                           reinterpret_cast<const int*>(ws + l.inverse), control, static_cast<int>(d->hidden), vec, static_cast<uint16_t*>(dx),
                            d->dx_stride);
 }
 

@@ -361,18 +361,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
   ptx::grid_dependency_sync();   // (set-up above overlaps the kernel before this one, see launch_one)
 
   const int num_kb = (args.K + kSlabElems - 1) / kSlabElems;
-  const int tiles_m = args.m_limit != nullptr ? (min(*args.m_limit, args.M) + kBlockM - 1) / kBlockM : args.tiles_m;
-  const int num_tiles = tiles_m * args.tiles_n * args.batch;
-  // A tile's slabs of K, all or chunk bz of them.  A chunk behind *k_limit is one slab behind K, which TMA fills with zeros.
-  const int end_kb = args.k_limit != nullptr ? min((*args.k_limit + kSlabElems - 1) / kSlabElems, num_kb) : num_kb;
-  auto slabs_of = [&](int bz, int& kb0, int& kb1) {
-    kb0 = args.k_chunk * bz;                                                  // (0 without chunks)
-    kb1 = args.k_chunk > 0 ? min(end_kb, kb0 + args.k_chunk) : end_kb;
-    if (kb1 <= kb0) {
-      kb0 = num_kb;
-      kb1 = num_kb + 1;
-    }
-  };
+  const int num_tiles = args.tiles_m * args.tiles_n * args.batch;
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
@@ -383,13 +372,13 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
       bool alive = true;
       for (int t = blockIdx.x; t < num_tiles && alive; t += gridDim.x) {
         int bz, bm, bn;
-        tile_coords(t, tiles_m, args.tiles_n, bz, bm, bn);
+        tile_coords(t, args.tiles_m, args.tiles_n, bz, bm, bn);
         const int m0 = bm * kBlockM;
         const int n0 = bn * kBlockN;
         const int az = args.a_broadcast || args.k_chunk > 0 ? 0 : bz;
         const int zb = args.k_chunk > 0 ? 0 : bz;
-        int kb0, kb1;
-        slabs_of(bz, kb0, kb1);
+        const int kb0 = args.k_chunk * bz;                                                  // (0 without chunks)
+        const int kb1 = args.k_chunk > 0 ? min(num_kb, kb0 + args.k_chunk) : num_kb;
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!ptx::mbar_wait(empty_bar(stage), phase ^ 1u, ctl, kSiteProducer)) {
             alive = false;
@@ -451,9 +440,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
         if (!ptx::mbar_wait(acc_empty_bar(buf), acc_phase ^ 1u, ctl, kSiteMmaAcc)) break;
         ptx::tc_fence_after_sync();
         const uint32_t d_tmem = tmem_base + buf * kBlockN;
-        int kb0, kb1;
-        slabs_of(t / (tiles_m * args.tiles_n), kb0, kb1);
-        const int count = kb1 - kb0;
+        const int chunk0 = args.k_chunk * (t / (args.tiles_m * args.tiles_n));
+        const int count = args.k_chunk > 0 ? min(num_kb - chunk0, args.k_chunk) : num_kb;
         for (int kb = 0; kb < count; ++kb) {
           if (!ptx::mbar_wait(full_bar(stage), phase, ctl, kSiteMmaFull)) {
             alive = false;
@@ -488,7 +476,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
     uint32_t n_store = 0;  // TMA stores issued by this warp (alternating between its two boxes)
     for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
       int bz, bm, bn;
-      tile_coords(t, tiles_m, args.tiles_n, bz, bm, bn);
+      tile_coords(t, args.tiles_m, args.tiles_n, bz, bm, bn);
       if (!ptx::mbar_wait(acc_full_bar(buf), acc_phase, ctl, kSiteEpilogue)) break;
       ptx::tc_fence_after_sync();
       epilogue_tile<kBlockN>(args, &tmap_d, tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * kBlockN, stage_smem,
@@ -531,13 +519,6 @@ struct PairCfg {
   static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
 constexpr int kMaxTailParts = 4;  // pieces of a tile of the last round
-// The tiles beyond the last full round of pairs are cut into 2 or 4 narrower ones where the idle pairs
-// can take the pieces: the round then takes about 1/2 or 1/3 of its time.  Returns the first tile that is cut.
-__host__ __device__ inline int tail_split(int64_t tiles, int pairs, bool may_cut, int& parts) {
-  const int tail = may_cut ? static_cast<int>(tiles % pairs) : 0;
-  parts = tail == 0 ? 1 : tail * kMaxTailParts <= pairs ? kMaxTailParts : tail * 2 <= pairs ? 2 : 1;
-  return static_cast<int>(tiles - tail);
-}
 enum : int { kSitePairFull = 111, kSitePairPeer = 112, kSitePairAcc = 113, kSitePairForward = 114 };
 
 // The tensor maps of D: one, or one per destination of a scattered output (rows of D dealt out
@@ -612,25 +593,13 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
   const uint32_t tmem_base = *tmem_slot;
   ptx::grid_dependency_sync();
 
-  int num_kb = (args.K + kSlabElems - 1) / kSlabElems, first_kb = 0;
-  if (args.k_limit != nullptr) {
-    const int end_kb = min((*args.k_limit + kSlabElems - 1) / kSlabElems, num_kb);
-    first_kb = end_kb > 0 ? 0 : num_kb;       // (none: one slab behind K, which TMA fills with zeros)
-    num_kb = end_kb > 0 ? end_kb : 1;
-  }
-  int tiles_m2 = (args.tiles_m + 1) / 2;  // pair tiles along M
+  const int num_kb = (args.K + kSlabElems - 1) / kSlabElems;
+  const int tiles_m2 = (args.tiles_m + 1) / 2;  // pair tiles along M
   const int pair_id = blockIdx.x >> 1;
   const int num_pairs = gridDim.x >> 1;
   // Units of work: whole tiles, then the tiles of the last round cut into tail_parts narrower ones.
-  int tail_from = args.tail_from, tail_parts = args.tail_parts;
-  uint32_t idesc_tail = args.idesc_tail;
-  if (args.m_limit != nullptr) {              // the last round of the rows that there are
-    tiles_m2 = (min(*args.m_limit, args.M) + 2 * kBlockM - 1) / (2 * kBlockM);
-    tail_from = tail_split(tiles_m2 * args.tiles_n, args.round_pairs, args.b_mn_major != 0, tail_parts);
-    idesc_tail = (args.idesc & ~(0x3fu << 17)) | static_cast<uint32_t>((kBlockN / tail_parts) >> 3) << 17;
-  }
-  const int num_units = tail_from + (tiles_m2 * args.tiles_n * args.batch - tail_from) * tail_parts;
-  const int tail_width = kBlockN / tail_parts;
+  const int num_units = args.tail_from + (tiles_m2 * args.tiles_n * args.batch - args.tail_from) * args.tail_parts;
+  const int tail_width = kBlockN / args.tail_parts;
   struct Unit {
     int bz, bm2, n_first, width;
   };
@@ -638,9 +607,9 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
     Unit x;
     int t = u, part = 0, bn;
     x.width = kBlockN;
-    if (u >= tail_from) {
-      t = tail_from + (u - tail_from) / tail_parts;
-      part = (u - tail_from) % tail_parts;
+    if (u >= args.tail_from) {
+      t = args.tail_from + (u - args.tail_from) / args.tail_parts;
+      part = (u - args.tail_from) % args.tail_parts;
       x.width = tail_width;
     }
     tile_coords(t, tiles_m2, args.tiles_n, x.bz, x.bm2, bn);
@@ -662,7 +631,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
       const int az = args.a_broadcast ? 0 : bz;
       const int b_boxes = (half_n + kSlabElems - 1) / kSlabElems;   // MN-major: boxes of one swizzle span of columns
       const uint32_t stage_bytes = kATileBytes + (args.b_mn_major ? b_boxes * kSlabElems : half_n) * kSlabBytes;
-      const CUtensorMap* map_b = t < tail_from ? &tmap_b : &tmap_b_tail;
+      const CUtensorMap* map_b = t < args.tail_from ? &tmap_b : &tmap_b_tail;
       for (int kb = 0; kb < num_kb; ++kb) {
         if (!ptx::mbar_wait(empty_bar(stage), phase ^ 1u, ctl, kSiteProducer)) {
           alive = false;
@@ -672,7 +641,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
         const uint32_t b_dst = a_dst + kATileBytes;
         // both CTAs' copies are counted on the EVEN CTA's barrier, which its issuer waits on
         const uint32_t bar = ptx::map_to_cta(full_bar(stage), 0);
-        const int k0 = (first_kb + kb) * kSlabElems;
+        const int k0 = kb * kSlabElems;
         if (ptx::elect_one()) {
           if (rank == 0) ptx::mbar_expect_tx(full_bar(stage), 2 * stage_bytes);
           if (args.a_mn_major) {
@@ -716,7 +685,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
     for (int t = pair_id; t < num_units && alive; t += num_pairs) {
       if (!ptx::mbar_wait(acc_empty_bar(buf), acc_phase ^ 1u, ctl, kSitePairAcc)) break;
       ptx::tc_fence_after_sync();
-      const uint32_t idesc = t < tail_from ? args.idesc : idesc_tail;
+      const uint32_t idesc = t < args.tail_from ? args.idesc : args.idesc_tail;
       const uint32_t d_tmem = tmem_base + buf * kBlockN;
       for (int kb = 0; kb < num_kb; ++kb) {
         if (!ptx::mbar_wait(full_bar(stage), phase, ctl, kSitePairFull)) {
@@ -779,6 +748,226 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
 
   // Teardown: neither CTA may leave while its partner can still read its shared memory or arrive
   // on its barriers.
+  if (*abort_flag != 0) __nanosleep(2000000);
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  ptx::cluster_sync_all();
+  if (warp == 1) {
+    ptx::tc_fence_after_sync();
+    ptx::tmem_dealloc_pair(tmem_base, C::kTmemCols);
+  }
+  ptx::cluster_sync_all();
+}
+
+// Two products in one launch of CTA pairs (see launch_two in gemm_sm100.h).  The kernel above with a unit list of two parts:
+// pair i takes units i, i + pairs, ... of the long product (planes x tiles, all tiles of a plane side by side, so that pairs
+// walk K together and share slabs in L2), then tiles of the other, in an order that a round of all pairs at work at the time
+// takes neighbouring tiles: the pairs with one long unit less run `ahead` rounds among themselves first.
+struct TwoArgs {
+  KernelArgs p[2];
+  const int* plan;
+  int pairs;
+};
+
+__global__ void __launch_bounds__(kThreads, 1)
+gemm_two_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_constant__ CUtensorMap tmap_b0,
+                const __grid_constant__ CUtensorMap tmap_a1, const __grid_constant__ CUtensorMap tmap_b1,
+                const __grid_constant__ CUtensorMap tmap_d1, const __grid_constant__ TwoArgs args) {
+  using C = PairCfg;
+  constexpr int kStages = C::kStages;
+  constexpr int kBlockN = C::kBlockN;
+  constexpr int kSlabElems = kSlabBytes / 2;
+  constexpr int kUmmaK = 16;
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem_gen = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
+  const uint32_t stage_smem = smem_base + kStages * C::kStageBytes;
+  const uint32_t bar_base = stage_smem + C::kStagingBytes;
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](int s) { return bar_base + 8u * (kStages + s); };
+  auto acc_full_bar = [&](int b) { return bar_base + 8u * (2 * kStages + b); };
+  auto acc_empty_bar = [&](int b) { return bar_base + 8u * (2 * kStages + 2 + b); };
+  uint8_t* tail = smem_gen + kStages * C::kStageBytes + C::kStagingBytes + 8 * (2 * kStages + 4);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(tail);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 4);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = ptx::cluster_ctarank();
+  ptx::AbortCtl ctl{abort_flag, args.p[0].status_word};
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < kStages; ++s) {
+      ptx::mbar_init(full_bar(s), 1);
+      ptx::mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      ptx::mbar_init(acc_full_bar(b), 1);
+      ptx::mbar_init(acc_empty_bar(b), 256);
+    }
+    ptx::fence_mbar_init();
+    ptx::prefetch_tmap(&tmap_a0);
+    ptx::prefetch_tmap(&tmap_b0);
+    ptx::prefetch_tmap(&tmap_a1);
+    ptx::prefetch_tmap(&tmap_b1);
+    if (args.p[1].d_tma) ptx::prefetch_tmap(&tmap_d1);
+  }
+  __syncthreads();
+  ptx::cluster_sync_all();
+  if (warp == 1) {
+    ptx::tmem_alloc_pair(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), C::kTmemCols);
+    ptx::tmem_relinquish_pair();
+  }
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  ptx::cluster_sync_all();
+  ptx::tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  ptx::grid_dependency_sync();
+
+  const KernelArgs &p0 = args.p[0], &p1 = args.p[1];
+  const int pairs = args.pairs, pair_id = blockIdx.x >> 1;
+  const int num_kb0 = (p0.K + kSlabElems - 1) / kSlabElems, num_kb1 = (p1.K + kSlabElems - 1) / kSlabElems;
+  const int rows0 = p0.m_limit != nullptr ? min(*p0.m_limit, p0.M) : p0.M;
+  const int end_kb1 = p1.k_limit != nullptr ? min((*p1.k_limit + kSlabElems - 1) / kSlabElems, num_kb1) : num_kb1;
+  const int tiles_m0 = (rows0 + 2 * kBlockM - 1) / (2 * kBlockM), tiles0 = tiles_m0 * p0.tiles_n;
+  const int tiles_m1 = (p1.tiles_m + 1) / 2, tiles1 = tiles_m1 * p1.tiles_n;
+  const int plane_slabs = *args.plan, units0 = tiles0 * ((num_kb0 + plane_slabs - 1) / plane_slabs);
+  // (a tile of few slabs costs about two more for its results)
+  const int heavy = units0 % pairs, light = pairs - heavy;
+  const int ahead = heavy > 0 ? (plane_slabs + max(end_kb1, 1) / 2) / (max(end_kb1, 1) + 2) : 0;
+  struct Unit {
+    int which, bz, bm2, bn, kb0, count;
+  };
+  const int mine0 = units0 / pairs + (pair_id < heavy ? 1 : 0);
+  auto unit_at = [&](int i, Unit& x) {       // the pair's i-th unit; false behind the last
+    if (i < mine0) {
+      const int u = pair_id + i * pairs;
+      x.which = 0;
+      x.bz = u / tiles0;
+      int bz;
+      tile_coords(u - x.bz * tiles0, tiles_m0, p0.tiles_n, bz, x.bm2, x.bn);
+      x.kb0 = x.bz * plane_slabs;
+      x.count = min(plane_slabs, num_kb0 - x.kb0);
+      return true;
+    }
+    const int j = i - mine0;
+    int t;
+    if (pair_id < heavy) t = ahead * light + j * pairs + pair_id;
+    else if (j < ahead) t = j * light + pair_id - heavy;
+    else t = ahead * light + (j - ahead) * pairs + pair_id;
+    if (t >= tiles1) return false;
+    x.which = 1;
+    tile_coords(t, tiles_m1, p1.tiles_n, x.bz, x.bm2, x.bn);
+    x.kb0 = end_kb1 > 0 ? 0 : num_kb1;       // (no rows: one slab behind K, which TMA fills with zeros)
+    x.count = end_kb1 > 0 ? end_kb1 : 1;
+    return true;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    int stage = 0;
+    uint32_t phase = 0;
+    bool alive = true;
+    Unit x;
+    for (int i = 0; alive && unit_at(i, x); ++i) {
+      const KernelArgs& p = args.p[x.which];
+      const CUtensorMap* map_a = x.which == 0 ? &tmap_a0 : &tmap_a1;
+      const CUtensorMap* map_b = x.which == 0 ? &tmap_b0 : &tmap_b1;
+      const int m0 = (x.bm2 * 2 + static_cast<int>(rank)) * kBlockM, n0 = x.bn * kBlockN + static_cast<int>(rank) * 128;
+      for (int kb = 0; kb < x.count; ++kb) {
+        if (!ptx::mbar_wait(empty_bar(stage), phase ^ 1u, ctl, kSiteProducer)) {
+          alive = false;
+          break;
+        }
+        const uint32_t a_dst = smem_base + stage * C::kStageBytes, b_dst = a_dst + kATileBytes;
+        const uint32_t bar = ptx::map_to_cta(full_bar(stage), 0);
+        const int k0 = (x.kb0 + kb) * kSlabElems;
+        if (ptx::elect_one()) {
+          if (rank == 0) ptx::mbar_expect_tx(full_bar(stage), 2 * C::kStageBytes);
+          if (p.a_mn_major) {
+#pragma unroll
+            for (int j = 0; j < kBlockM / kSlabElems; ++j)
+              ptx::tma_load_3d_pair(a_dst + j * (kSlabElems * kSlabBytes), map_a, bar, m0 + j * kSlabElems, k0, 0);
+          } else {
+            ptx::tma_load_3d_pair(a_dst, map_a, bar, k0, m0, 0);
+          }
+          if (p.b_mn_major) {
+#pragma unroll
+            for (int j = 0; j < 128 / kSlabElems; ++j)
+              ptx::tma_load_3d_pair(b_dst + j * (kSlabElems * kSlabBytes), map_b, bar, n0 + j * kSlabElems, k0, 0);
+          } else {
+            ptx::tma_load_3d_pair(b_dst, map_b, bar, k0, n0, 0);
+          }
+        }
+        __syncwarp();
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  } else if (warp == 1 && rank == 0) {
+    // ------------------------------------------------------------ even CTA: MMA issuer for the pair
+    int stage = 0, buf = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    bool alive = true;
+    Unit x;
+    for (int i = 0; alive && unit_at(i, x); ++i) {
+      const KernelArgs& p = args.p[x.which];
+      const uint32_t a_lbo = p.a_mn_major ? kSlabElems * kSlabBytes : 16, b_lbo = p.b_mn_major ? kSlabElems * kSlabBytes : 16;
+      const uint32_t a_kstep = p.a_mn_major ? kUmmaK * kSlabBytes : 32, b_kstep = p.b_mn_major ? kUmmaK * kSlabBytes : 32;
+      const uint32_t idesc = p.idesc;
+      if (!ptx::mbar_wait(acc_empty_bar(buf), acc_phase ^ 1u, ctl, kSitePairAcc)) break;
+      ptx::tc_fence_after_sync();
+      const uint32_t d_tmem = tmem_base + buf * kBlockN;
+      for (int kb = 0; kb < x.count; ++kb) {
+        if (!ptx::mbar_wait(full_bar(stage), phase, ctl, kSitePairFull)) {
+          alive = false;
+          break;
+        }
+        ptx::tc_fence_after_sync();
+        const uint32_t a_src = smem_base + stage * C::kStageBytes, b_src = a_src + kATileBytes;
+#pragma unroll
+        for (int ks = 0; ks < kSlabElems / kUmmaK; ++ks) {
+          const uint64_t da = ptx::umma_smem_desc(a_src + ks * a_kstep, a_lbo, 1024);
+          const uint64_t db = ptx::umma_smem_desc(b_src + ks * b_kstep, b_lbo, 1024);
+          ptx::umma_ss_pair_elect<ptx::kKindF16>(d_tmem, da, db, idesc, (kb | ks) != 0 ? 1u : 0u);
+        }
+        ptx::umma_commit_pair_elect(empty_bar(stage));
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!alive) break;
+      ptx::umma_commit_pair_elect(acc_full_bar(buf));
+      buf ^= 1;
+      if (buf == 0) acc_phase ^= 1u;
+    }
+  } else if (warp >= 2) {
+    // ------------------------------------------------------------ epilogue (each CTA: its 128 rows)
+    const int quarter = warp & 3;
+    int buf = 0;
+    uint32_t acc_phase = 0;
+    uint32_t n_store = 0;
+    Unit x;
+    for (int i = 0; unit_at(i, x); ++i) {
+      if (!ptx::mbar_wait(acc_full_bar(buf), acc_phase, ctl, kSiteEpilogue)) break;
+      ptx::tc_fence_after_sync();
+      epilogue_tile<kBlockN>(args.p[x.which], &tmap_d1, tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * kBlockN, stage_smem,
+                             x.bz, x.bm2 * 2 + static_cast<int>(rank), x.bn * kBlockN, quarter, lane, n_store);
+      ptx::tc_fence_before_sync();
+      if (rank == 0) ptx::mbar_arrive(acc_empty_bar(buf));
+      else ptx::mbar_arrive_cluster_tmem(acc_empty_bar(buf), 0);
+      buf ^= 1;
+      if (buf == 0) acc_phase ^= 1u;
+    }
+    if (lane == 0) ptx::bulk_wait_group<0>();
+  }
+
   if (*abort_flag != 0) __nanosleep(2000000);
   ptx::tc_fence_before_sync();
   __syncthreads();
@@ -863,8 +1052,11 @@ int launch(const Problem& p, const DeviceInfo& dev, cudaStream_t stream) {
   bool pair = bn == 256 && tiles_m_all >= 2 && p.k_chunk == 0 && pair_tiles >= dev.sm_count / 2;
   if (const char* env = std::getenv("IXK_GEMM_PAIR")) pair = pair && std::atoi(env) != 0;
   const int b_box_rows = pair ? 128 : bn;
-  int tail_parts = 1;
-  const int tail_from = tail_split(pair_tiles, dev.sm_count / 2, pair && p.scatter_world == 0, tail_parts);
+  // The tiles beyond the last full round of pairs are cut into 2 or 4 narrower ones where the idle pairs
+  // can take the pieces: the round then takes about 1/2 or 1/3 of its time.
+  const int64_t pairs_all = dev.sm_count / 2;
+  const int64_t tail_tiles = pair && p.scatter_world == 0 ? pair_tiles % pairs_all : 0;
+  const int tail_parts = tail_tiles == 0 ? 1 : tail_tiles * kMaxTailParts <= pairs_all ? kMaxTailParts : tail_tiles * 2 <= pairs_all ? 2 : 1;
   if (p.scatter_world > 0) {
     // Only the kernel that large projections run on stores to several destinations, and only
     // whole row blocks of one CTA.
@@ -934,7 +1126,7 @@ int launch(const Problem& p, const DeviceInfo& dev, cudaStream_t stream) {
   k.b_mn_major = p.b_mn_major;
   k.idesc = ptx::umma_idesc(p.a_fmt, p.b_fmt, p.a_mn_major ? 1 : 0, p.b_mn_major ? 1 : 0, pair ? 2 * kBlockM : kBlockM, bn,
                             p.kind == ptx::kKindI8 ? 2u : 1u);
-  k.tail_from = tail_from;
+  k.tail_from = static_cast<int>(pair_tiles - tail_tiles);
   k.tail_parts = tail_parts;
   k.idesc_tail = ptx::umma_idesc(p.a_fmt, p.b_fmt, p.a_mn_major ? 1 : 0, p.b_mn_major ? 1 : 0, 2 * kBlockM, PairCfg::kBlockN / tail_parts,
                                  p.kind == ptx::kKindI8 ? 2u : 1u);
@@ -950,10 +1142,7 @@ int launch(const Problem& p, const DeviceInfo& dev, cudaStream_t stream) {
   k.act = p.act;
   k.acc_scale = p.acc_scale;
   k.beta = p.beta;
-  k.m_limit = p.m_limit;
-  k.k_limit = p.k_limit;
   k.acc_scale_dev = p.acc_scale_dev;
-  k.round_pairs = dev.sm_count / 2;
   k.status_word = dev.status_word;
   const int out_es = (p.out_dtype == IXK_F32 || p.out_dtype == IXK_S32) ? 4 : 2;
   const int bias_es = p.bias_dtype == IXK_F32 ? 4 : 2;
@@ -1030,6 +1219,104 @@ int launch(const Problem& p, const DeviceInfo& dev, cudaStream_t stream) {
     case ptx::kKindI8: return dispatch(std::integral_constant<int, ptx::kKindI8>{});
     default: return dispatch(std::integral_constant<int, ptx::kKindF16>{});
   }
+}
+
+int launch_two(const Problem (&p)[2], const int* plan, const DeviceInfo& dev, cudaStream_t stream) {
+  if (p[0].M == 0 && p[1].M == 0) return IXK_OK;
+  CUtensorMap a[2], b[2], d1;
+  TwoArgs args{};
+  auto aligned16 = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; };
+  for (int i = 0; i < 2; ++i) {
+    const Problem& q = p[i].M != 0 ? p[i] : p[1 - i];      // (an absent product's maps are never used)
+    auto map = [&](CUtensorMap* out, const void* base, bool mn_major, int64_t mn, int64_t ld) {
+      TmapSpec s{};
+      s.dtype = q.ab_dtype == IXK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+      s.rank = 3;
+      s.swizzle128 = true;
+      s.dims[0] = mn_major ? mn : q.K;
+      s.dims[1] = mn_major ? q.K : mn;
+      s.dims[2] = 1;
+      s.box[0] = kSlabBytes / 2;
+      s.box[1] = mn_major ? kSlabBytes / 2 : 128;
+      s.box[2] = 1;
+      s.strides_bytes[0] = static_cast<uint64_t>(ld) * 2;
+      s.strides_bytes[1] = s.strides_bytes[0] * s.dims[1];
+      return encode_tmap(out, base, s);
+    };
+    int rc = map(&a[i], q.a, q.a_mn_major, q.M, q.lda);
+    if (rc != IXK_OK) return rc;
+    if ((rc = map(&b[i], q.b, q.b_mn_major, q.N, q.ldb)) != IXK_OK) return rc;
+    KernelArgs& k = args.p[i];
+    k.M = static_cast<int>(p[i].M);
+    k.N = static_cast<int>(p[i].N);
+    k.K = static_cast<int>(p[i].K);
+    k.batch = 1;
+    k.tiles_m = static_cast<int>((p[i].M + kBlockM - 1) / kBlockM);
+    k.tiles_n = p[i].M != 0 ? static_cast<int>((p[i].N + PairCfg::kBlockN - 1) / PairCfg::kBlockN) : 0;
+    k.a_mn_major = q.a_mn_major;
+    k.b_mn_major = q.b_mn_major;
+    k.idesc = ptx::umma_idesc(q.a_fmt, q.b_fmt, q.a_mn_major ? 1 : 0, q.b_mn_major ? 1 : 0, 2 * kBlockM, PairCfg::kBlockN);
+    k.tail_parts = 1;
+    k.c = p[i].beta != 0.0f ? p[i].c : nullptr;
+    k.d = p[i].d;
+    k.ldd = p[i].ldd;
+    k.ldc = p[i].ldc;
+    k.d_batch_stride = p[i].d_batch_stride;
+    k.c_batch_stride = p[i].c_batch_stride;
+    k.out_dtype = p[i].out_dtype;
+    k.bias_dtype = p[i].bias_dtype;
+    k.act = kActNone;
+    k.acc_scale = p[i].acc_scale;
+    k.beta = p[i].beta;
+    k.m_limit = p[i].m_limit;
+    k.k_limit = p[i].k_limit;
+    k.acc_scale_dev = p[i].acc_scale_dev;
+    k.status_word = dev.status_word;
+    const int es = p[i].out_dtype == IXK_F32 ? 4 : 2;
+    k.d_vec_ok = aligned16(p[i].d) && (p[i].ldd * es) % 16 == 0 && (p[i].d_batch_stride * es) % 16 == 0;
+    k.c_vec_ok = k.c != nullptr && aligned16(p[i].c) && (p[i].ldc * es) % 16 == 0 && (p[i].c_batch_stride * es) % 16 == 0;
+  }
+  d1 = a[1];
+  if (p[1].M != 0 && args.p[1].d_vec_ok && p[1].out_dtype != IXK_F32) {
+    args.p[1].d_tma = 1;
+    TmapSpec s{};
+    s.dtype = p[1].out_dtype == IXK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    s.rank = 3;
+    s.swizzle128 = true;
+    s.dims[0] = p[1].N;
+    s.dims[1] = p[1].M;
+    s.dims[2] = 1;
+    s.box[0] = 64;
+    s.box[1] = 32;
+    s.box[2] = 1;
+    s.strides_bytes[0] = static_cast<uint64_t>(p[1].ldd) * 2;
+    s.strides_bytes[1] = s.strides_bytes[0] * s.dims[1];
+    if (int rc = encode_tmap(&d1, p[1].d, s)) return rc;
+  }
+  args.plan = plan;
+  args.pairs = dev.sm_count / 2;      // (all of them, whatever the tiles: which tile is whose follows from it)
+  static thread_local int configured_device = -1;
+  if (configured_device != dev.device) {
+    IXK_CUDA_OK(cudaFuncSetAttribute(gemm_two_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg::kSmemBytes));
+    configured_device = dev.device;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * args.pairs);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = PairCfg::kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  IXK_CUDA_OK(cudaLaunchKernelEx(&cfg, gemm_two_kernel, a[0], b[0], a[1], b[1], d1, args));
+  count_launch();
+  return IXK_OK;
 }
 
 }  // namespace gemm

@@ -38,9 +38,8 @@ struct Problem {
   int act = kActNone;
   float acc_scale = 1.0f;
   float beta = 0.0f;
-  // Sizes and a factor that only the GPU knows (the rows of a batch that count), nullptr: none.  D's rows from *m_limit
-  // on are not computed; K ends at *k_limit (at most K; the operands hold zeros from there to a multiple of 64);
-  // acc_scale is multiplied by *acc_scale_dev.  16-bit operands, batch 1, no scattered output.
+  // What only the GPU knows, nullptr: nothing.  acc_scale is multiplied by *acc_scale_dev.  launch_two only: D's rows from
+  // *m_limit on are not computed; K ends at *k_limit (at most K; the operands hold zeros from there to a multiple of 64).
   const int* m_limit = nullptr;
   const int* k_limit = nullptr;
   const float* acc_scale_dev = nullptr;
@@ -62,7 +61,6 @@ struct KernelArgs {
   uint32_t idesc;
   uint32_t idesc_tail;         // CTA-pair kernel: the narrower tiles of the last round
   int tail_from, tail_parts;   // tiles from here on are cut into this many (1: none is)
-  int round_pairs;             // CTA pairs of a full round
   const void* bias;
   const void* c;
   void* d;
@@ -86,6 +84,34 @@ struct KernelArgs {
 int run_problem(const Problem& p, void* workspace, size_t workspace_bytes, const DeviceInfo& dev, cudaStream_t stream);
 // Scratch that run_problem can use for a 16-bit problem of one batch.
 size_t problem_workspace_bytes(int64_t M, int64_t N, int64_t K);
+
+// Two products in one launch, for the gradients of a layer whose weight is much longer one way than the other:
+//   p[0]  D0 (+)= A0.B0, fp32, few tiles and a long K: cut along K into planes, d_batch_stride elements apart, which the
+//         caller adds up; beta 0 or 1 with c = d
+//   p[1]  D1 = A1.B1, many tiles and a short K
+// Either may be absent (M = 0).  The pairs of CTAs that have one unit less of the long product begin with the other's tiles,
+// so that all end together.  `plan` (device): the slabs of K per plane, from two_plan.  16-bit operands; p[0].m_limit and
+// p[1].k_limit hold the same number.
+int launch_two(const Problem (&p)[2], const int* plan, const DeviceInfo& dev, cudaStream_t stream);
+constexpr int kTwoTile = 256;    // of either product
+
+// Slabs of 64 of the long product's K per plane: as few planes as let the longest pair's share of it end with the whole.
+// tiles and slabs: of the long product (0), of the other (1).
+__host__ __device__ inline int two_plan(int64_t tiles0, int slabs0, int64_t tiles1, int slabs1, int pairs, int max_planes) {
+  const int64_t share = (tiles0 * slabs0 + tiles1 * slabs1 + pairs - 1) / pairs;
+  int best = slabs0;
+  int64_t best_time = 0;
+  for (int s = 1; s <= max_planes && (s == 1 || slabs0 / s >= 16); ++s) {
+    const int chunk = (slabs0 + s - 1) / s, planes = (slabs0 + chunk - 1) / chunk;
+    const int64_t longest = (tiles0 * planes + pairs - 1) / pairs * chunk, time = longest > share ? longest : share;
+    if (s == 1 || time * 100 < best_time * 97) {    // (a further plane is written, read and added up)
+      best = chunk;
+      best_time = time;
+    }
+    if (best_time * 100 <= share * 102) break;
+  }
+  return best;
+}
 
 int pick_block_n(int64_t M, int64_t N, int64_t batch, int sm_count);
 int launch(const Problem& p, const DeviceInfo& dev, cudaStream_t stream);

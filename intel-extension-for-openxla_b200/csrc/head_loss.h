@@ -7,6 +7,7 @@ namespace ixk {
 namespace head {
 
 constexpr int kNoColumn = 0x7fffffff;
+constexpr int64_t kDirectRows = 128;    // one row block: no tiles to save, the forward pass takes x as it is
 
 // What a row of the batch is measured against: one label, or a list of columns in ascending order with their weights.
 struct Targets {

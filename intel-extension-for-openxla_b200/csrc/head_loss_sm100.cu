@@ -358,8 +358,9 @@ head_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
           if (args.range != nullptr) coef *= *args.range;
         }
       }
-      // (the gradient's rows up to the end of a slab are read by the product along the rows: zeros)
-      const bool work = kGrad ? warp_row < (active_rows + kSlabElems - 1) / kSlabElems * kSlabElems : warp_row < active_rows;
+      // (the products read the gradient's rows up to the end of a slab, or of the only row block: zeros)
+      const bool work = !kGrad ? warp_row < active_rows
+                               : args.rows <= kDirectRows || warp_row < (active_rows + kSlabElems - 1) / kSlabElems * kSlabElems;
       for (int n = n_begin; n < n_end; ++n) {
         const int n0 = n * args.tile_n, limit = min(args.tile_n, args.count - n0);
         if (!ptx::mbar_wait(acc_full_bar(buf), acc_phase, ctl, kSiteEpilogue)) {
