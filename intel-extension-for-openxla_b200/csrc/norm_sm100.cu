@@ -31,7 +31,7 @@ constexpr int kMaxElems = 16;             // elements of a row per thread
 constexpr int64_t kMaxCols = kMaxThreads * kMaxElems;
 constexpr int kAssumedSms = 148;          // (the workspace query runs without a device)
 constexpr int kThreadsPerSm = 1024;       // what 64 registers a thread leave room for
-constexpr int kSumCols = 32, kSumParts = 32;
+constexpr int kSumCols = 8, kSumParts = 64;
 
 // kVec elements of type T as they lie in memory.
 template <typename T, int kVec>
@@ -63,6 +63,11 @@ __device__ __forceinline__ Raw<T, kVec> pack(const float (&f)[kVec]) {
   for (int j = 0; j < kVec; ++j) e[j] = from_float<T>(f[j]);
   return raw;
 }
+// The compiler may not keep what it unpacked of `raw` beyond this point: registers hold the row as it lies in memory, not
+// twice as many floats (bf16 at 16 vectors a lane: 164 registers with, 255 and spills without at 32).
+__device__ __forceinline__ void forget(uint4& raw) { asm volatile("" : "+r"(raw.x), "+r"(raw.y), "+r"(raw.z), "+r"(raw.w)); }
+__device__ __forceinline__ void forget(uint32_t& raw) { asm volatile("" : "+r"(raw)); }
+__device__ __forceinline__ void forget(uint16_t& raw) { asm volatile("" : "+h"(raw)); }
 __device__ __forceinline__ float load_param(const void* p, int64_t i, int dtype) {
   if (dtype == IXK_F32) return static_cast<const float*>(p)[i];
   if (dtype == IXK_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
@@ -77,6 +82,9 @@ struct Args {
   int64_t rows, ldx, ldg, ldo;
   int cols, rms, param_dtype;
   float eps, gain_offset, inv_cols;
+  int gain_vec, shift_vec;      // gain and shift start on 16 bytes
+  int stages;                   // of the ring
+  int* status_word;
 };
 
 // The sums of kCount values over the row's threads, in every one of them.  kWarp: the row is a warp's; else a CTA's, and
@@ -295,31 +303,608 @@ __global__ void __launch_bounds__(kWarp ? 256 : kMaxThreads, 1) row_norm_bwd_ker
   }
 }
 
-// dgain (blockIdx.y 0) and dshift (1): the CTAs' rows of partials added up, 32 columns per CTA.
+// Whole vectors are worked on as pairs of fp32 (fma.rn.f32x2 and its kin: half of the instructions, which bound these
+// kernels, not memory, when every element is its own: 27 a element forward and 45 backward).
+template <typename T>
+constexpr int kPairs = 8 / sizeof(T);     // of a 16-byte vector
+template <typename T>
+__device__ __forceinline__ void unpack_pairs(const uint4& raw, uint64_t (&p)[kPairs<T>]) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int j = 0; j < kPairs<T>; ++j) {
+    if constexpr (std::is_same_v<T, float>) {
+      p[j] = ptx::f32x2(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1]));
+    } else if constexpr (std::is_same_v<T, __half>) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+      p[j] = ptx::f32x2(f.x, f.y);
+    } else {
+      p[j] = ptx::f32x2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack_pairs(const uint64_t (&p)[kPairs<T>]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < kPairs<T>; ++j) {
+    float lo, hi;
+    ptx::f32x2_split(p[j], lo, hi);
+    if constexpr (std::is_same_v<T, float>) {
+      w[2 * j] = __float_as_uint(lo);
+      w[2 * j + 1] = __float_as_uint(hi);
+    } else if constexpr (std::is_same_v<T, __half>) {
+      const __half2 h = __floats2half2_rn(lo, hi);
+      w[j] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+      w[j] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ float pair_sum(uint64_t p) {
+  float lo, hi;
+  ptx::f32x2_split(p, lo, hi);
+  return lo + hi;
+}
+// offset + parameters of type P, as pairs: the kN pairs from column c on (`none` without a parameter).
+template <typename P, int kN>
+__device__ __forceinline__ void load_params(const void* p, int c, bool vec, float offset, float none, uint64_t (&out)[kN]) {
+  const uint64_t off = ptx::f32x2(offset, offset);
+  if (p == nullptr) {
+#pragma unroll
+    for (int j = 0; j < kN; ++j) out[j] = ptx::f32x2(none, none);
+  } else if (vec) {      // (as many bytes as the parameters of a vector of columns have: 16 or 32)
+    const P* at = static_cast<const P*>(p) + c;
+#pragma unroll
+    for (int j = 0; j < kN; j += kPairs<P>) {
+      uint64_t part[kPairs<P>];
+      unpack_pairs<P>(*reinterpret_cast<const uint4*>(at + 2 * j), part);
+#pragma unroll
+      for (int i = 0; i < kPairs<P>; ++i) out[j + i] = ptx::add2(part[i], off);
+    }
+  } else {
+    const P* at = static_cast<const P*>(p) + c;
+#pragma unroll
+    for (int j = 0; j < kN; ++j) out[j] = ptx::add2(ptx::f32x2(to_float<P>(at[2 * j]), to_float<P>(at[2 * j + 1])), off);
+  }
+}
+// The warp's sums of kCount values (a power of two), in every lane.  Halves of the lanes first take over halves of the values,
+// so that 8 values take 9 shuffles and 8 to hand the sums back instead of 40.
+template <int kCount>
+__device__ __forceinline__ int value_of_lane(int lane) {
+  return kCount == 8 ? lane >> 2 : kCount == 4 ? lane >> 3 : kCount == 2 ? lane >> 4 : 0;
+}
+template <int kCount>
+__device__ __forceinline__ float warp_sum_of_lane(float (&v)[kCount]) {     // of value value_of_lane
+  const int lane = threadIdx.x & 31;
+  int o = 16;
+#pragma unroll
+  for (int n = kCount; n > 1; n /= 2, o /= 2) {
+    const bool upper = (lane & o) != 0;
+#pragma unroll
+    for (int i = 0; i < n / 2; ++i) {
+      const float keep = upper ? v[i + n / 2] : v[i], give = upper ? v[i] : v[i + n / 2];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    }
+  }
+#pragma unroll
+  for (; o > 0; o /= 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+  return v[0];
+}
+template <int kCount>
+__device__ __forceinline__ void warp_sums(float (&v)[kCount]) {
+  const float t = warp_sum_of_lane<kCount>(v);
+#pragma unroll
+  for (int c = 0; c < kCount; ++c) v[c] = __shfl_sync(0xffffffffu, t, c * (32 / kCount));
+}
+// The same over a CTA of at most 16 warps; `scratch` is not the one of the call before.
+template <int kCount>
+__device__ __forceinline__ void cta_sums(float (&v)[kCount], float (&scratch)[kCount][16]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  constexpr int kLanes = 32 / kCount;      // per value
+  const float t = warp_sum_of_lane<kCount>(v);
+  const int c = value_of_lane<kCount>(lane), at = lane % kLanes;
+  if (at == 0) scratch[c][warp] = t;
+  __syncthreads();
+  float u = at < warps ? scratch[c][at] : 0.0f;
+  if (kLanes < 16 && at + kLanes < warps) u += scratch[c][at + kLanes];
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o /= 2) u += __shfl_xor_sync(0xffffffffu, u, o);
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) v[i] = __shfl_sync(0xffffffffu, u, i * kLanes);
+}
+
+// Forward, short rows (up to eight elements a lane): a warp has kRows rows at a time, all of their loads out at once and no
+// barrier between warps.
+template <typename T, typename P, int kPer, int kRows>
+__global__ void __launch_bounds__(128) row_norm_fwd_rows_kernel(const Args a) {
+  constexpr int kVec = 16 / sizeof(T), kN = kPairs<T>;
+  ptx::grid_dependency_sync();
+  const int lane = threadIdx.x & 31, nvec = a.cols / kVec;
+  const int64_t warps = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
+  for (int64_t first = (static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5)) * kRows; first < a.rows; first += warps * kRows) {
+    uint4 raw[kRows][kPer];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + (first + r) * a.ldx);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int v = lane + 32 * i;
+        raw[r][i] = first + r < a.rows && v < nvec ? x[v] : make_uint4(0, 0, 0, 0);
+      }
+    }
+    float mean[kRows], s[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) mean[r] = 0.0f;
+    if (!a.rms) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        uint64_t t = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          uint64_t f[kN];
+          unpack_pairs<T>(raw[r][i], f);
+#pragma unroll
+          for (int j = 0; j < kN; ++j) t = ptx::add2(t, f[j]);
+        }
+        mean[r] = pair_sum(t);
+      }
+      warp_sums<kRows>(mean);
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) mean[r] *= a.inv_cols;
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const uint64_t minus = ptx::f32x2(-mean[r], -mean[r]);
+      uint64_t t = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        forget(raw[r][i]);
+        if (lane + 32 * i < nvec) {
+          uint64_t f[kN];
+          unpack_pairs<T>(raw[r][i], f);
+#pragma unroll
+          for (int j = 0; j < kN; ++j) {
+            f[j] = ptx::add2(f[j], minus);
+            t = ptx::fma2(f[j], f[j], t);
+          }
+        }
+      }
+      s[r] = pair_sum(t);
+    }
+    warp_sums<kRows>(s);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) s[r] = rsqrtf(fmaf(s[r], a.inv_cols, a.eps));
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int v = lane + 32 * i;
+      if (v < nvec) {
+        uint64_t scale[kN], shift[kN];
+        load_params<P, kN>(a.gain, v * kVec, a.gain_vec, a.gain_offset, 1.0f, scale);
+        load_params<P, kN>(a.shift, v * kVec, a.shift_vec, 0.0f, 0.0f, shift);
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          if (first + r < a.rows) {
+            const uint64_t minus = ptx::f32x2(-mean[r], -mean[r]), rstd = ptx::f32x2(s[r], s[r]);
+            uint64_t f[kN];
+            forget(raw[r][i]);
+            unpack_pairs<T>(raw[r][i], f);
+#pragma unroll
+            for (int j = 0; j < kN; ++j) f[j] = ptx::fma2(ptx::mul2(ptx::add2(f[j], minus), rstd), scale[j], shift[j]);
+            reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (first + r) * a.ldo)[v] = pack_pairs<T>(f);
+          }
+        }
+      }
+    }
+    if (lane < kRows && first + lane < a.rows) {
+      float m = mean[0], q = s[0];
+#pragma unroll
+      for (int r = 1; r < kRows; ++r) {
+        if (lane == r) {
+          m = mean[r];
+          q = s[r];
+        }
+      }
+      if (a.mean != nullptr) a.mean[first + lane] = m;
+      if (a.rstd != nullptr) a.rstd[first + lane] = q;
+    }
+  }
+}
+
+// What a vector of columns adds to a row's two sums, mean(h xh) and mean(h), and to the columns' own.
+template <typename T, int kN>
+__device__ __forceinline__ void bwd_sums(const uint4& xr, const uint4& gr, float mean, float rstd, const uint64_t (&scale)[kN], uint64_t (&dgain)[kN],
+                                         uint64_t (&dshift)[kN], uint64_t& hx, uint64_t& hs) {
+  const uint64_t minus = ptx::f32x2(-mean, -mean), r2 = ptx::f32x2(rstd, rstd);
+  uint64_t x[kN], g[kN];
+  unpack_pairs<T>(xr, x);
+  unpack_pairs<T>(gr, g);
+#pragma unroll
+  for (int j = 0; j < kN; ++j) {
+    const uint64_t xh = ptx::mul2(ptx::add2(x[j], minus), r2), h = ptx::mul2(g[j], scale[j]);
+    dgain[j] = ptx::fma2(g[j], xh, dgain[j]);
+    dshift[j] = ptx::add2(dshift[j], g[j]);
+    hx = ptx::fma2(h, xh, hx);
+    hs = ptx::add2(hs, h);
+  }
+}
+// dx of a vector: rstd (h - c0 - xh c1).
+template <typename T, int kN>
+__device__ __forceinline__ uint4 bwd_dx(uint4& xr, uint4& gr, float mean, float rstd, const uint64_t (&scale)[kN], float c1, float c0) {
+  forget(xr);
+  forget(gr);
+  const uint64_t minus = ptx::f32x2(-mean, -mean), r2 = ptx::f32x2(rstd, rstd), m1 = ptx::f32x2(-c1, -c1), m0 = ptx::f32x2(-c0, -c0);
+  uint64_t x[kN], g[kN];
+  unpack_pairs<T>(xr, x);
+  unpack_pairs<T>(gr, g);
+#pragma unroll
+  for (int j = 0; j < kN; ++j) {
+    const uint64_t xh = ptx::mul2(ptx::add2(x[j], minus), r2);
+    x[j] = ptx::mul2(ptx::fma2(xh, m1, ptx::fma2(g[j], scale[j], m0)), r2);
+  }
+  return pack_pairs<T>(x);
+}
+template <int kN>
+__device__ __forceinline__ void put_pairs(float* out, const uint64_t (&p)[kN], bool add) {
+#pragma unroll
+  for (int j = 0; j < kN; ++j) {
+    float lo, hi;
+    ptx::f32x2_split(p[j], lo, hi);
+    out[2 * j] = add ? out[2 * j] + lo : lo;
+    out[2 * j + 1] = add ? out[2 * j + 1] + hi : hi;
+  }
+}
+
+// Backward, short rows (up to eight elements a lane): a warp has kRows rows at a time, a lane kPer vectors of columns and
+// their sums.
+template <typename T, typename P, int kPer, int kRows>
+__global__ void __launch_bounds__(256) row_norm_bwd_rows_kernel(const Args a) {
+  constexpr int kVec = 16 / sizeof(T), kN = kPairs<T>;
+  extern __shared__ float sums[];    // [2][cols]
+  ptx::grid_dependency_sync();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nvec = a.cols / kVec;
+  const int64_t warps = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
+  uint64_t scale[kPer][kN], dgain[kPer][kN], dshift[kPer][kN];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int v = lane + 32 * i;
+    if (v < nvec) load_params<P, kN>(a.gain, v * kVec, a.gain_vec, a.gain_offset, 1.0f, scale[i]);
+#pragma unroll
+    for (int j = 0; j < kN; ++j) dgain[i][j] = dshift[i][j] = 0;
+  }
+  for (int64_t first = (static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + warp) * kRows; first < a.rows; first += warps * kRows) {
+    uint4 xr[kRows][kPer], gr[kRows][kPer];
+    float mean[kRows], rstd[kRows], s[2 * kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const bool there = first + r < a.rows;
+      const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + (first + r) * a.ldx);
+      const uint4* g = reinterpret_cast<const uint4*>(static_cast<const T*>(a.gy) + (first + r) * a.ldg);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int v = lane + 32 * i;
+        const bool in = there && v < nvec;
+        xr[r][i] = in ? x[v] : make_uint4(0, 0, 0, 0);
+        gr[r][i] = in ? g[v] : make_uint4(0, 0, 0, 0);
+      }
+      mean[r] = there && !a.rms ? a.mean[first + r] : 0.0f;
+      rstd[r] = there ? a.rstd[first + r] : 0.0f;
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      uint64_t hx = 0, hs = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (lane + 32 * i < nvec) bwd_sums<T, kN>(xr[r][i], gr[r][i], mean[r], rstd[r], scale[i], dgain[i], dshift[i], hx, hs);
+      s[2 * r] = pair_sum(hx);
+      s[2 * r + 1] = pair_sum(hs);
+    }
+    warp_sums<2 * kRows>(s);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const float c1 = s[2 * r] * a.inv_cols, c0 = a.rms ? 0.0f : s[2 * r + 1] * a.inv_cols;
+      uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (first + r) * a.ldo);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int v = lane + 32 * i;
+        if (first + r < a.rows && v < nvec) out[v] = bwd_dx<T, kN>(xr[r][i], gr[r][i], mean[r], rstd[r], scale[i], c1, c0);
+      }
+    }
+  }
+  if (a.part_gain == nullptr && a.part_shift == nullptr) return;
+  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) {     // the CTA's warps add up one after the other
+    if (warp == w) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int v = lane + 32 * i;
+        if (v < nvec) {
+          put_pairs<kN>(sums + v * kVec, dgain[i], w > 0);
+          put_pairs<kN>(sums + a.cols + v * kVec, dshift[i], w > 0);
+        }
+      }
+    }
+    __syncthreads();
+  }
+  for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
+    if (a.part_gain != nullptr) a.part_gain[static_cast<int64_t>(blockIdx.x) * a.cols + c] = sums[c];
+    if (a.part_shift != nullptr) a.part_shift[static_cast<int64_t>(blockIdx.x) * a.cols + c] = sums[a.cols + c];
+  }
+}
+
+// Longer rows of whole vectors: a CTA takes kRows rows at a time out of a ring in shared memory that bulk copies keep full
+// (about 190 KB under way an SM, which registers could not hold beside the parameters and the columns' sums), and one barrier
+// serves the sums of all of them.  A thread has 16 columns: with eight, the sums across threads were a third of all
+// instructions.
+enum : int { kSiteRing = 701 };
+constexpr int kRingBytes = 190 * 1024;
+constexpr int kRingThreads = 512, kRingElems = 16;
+constexpr int kMaxStages = 16;
+
+// The ring of kTensors tensors' rows: stage s holds batch blockIdx + s * gridDim, then every stages-th one after it.
+template <typename T, int kRows, int kTensors>
+struct Ring {
+  uint8_t* data;        // [stages][kRows][kTensors][row]
+  uint64_t* full;
+  int* abort_flag;
+  const void* from[kTensors];
+  int64_t ld[kTensors], rows, batches;
+  uint32_t row_bytes;
+  int stages, stage;
+  uint32_t phase;
+  bool alive;
+  int* status_word;
+
+  __device__ __forceinline__ uint32_t stage_bytes() const { return kTensors * kRows * row_bytes; }
+  __device__ __forceinline__ void fetch(int64_t batch, int s) {      // one thread
+    const int n = static_cast<int>(min(static_cast<int64_t>(kRows), rows - batch * kRows));
+    const uint32_t bar = ptx::smem_u32(&full[s]);
+    uint32_t dst = ptx::smem_u32(data) + s * stage_bytes();
+    ptx::mbar_expect_tx(bar, kTensors * n * row_bytes);
+    for (int r = 0; r < n; ++r) {
+#pragma unroll
+      for (int t = 0; t < kTensors; ++t) {
+        ptx::bulk_load_1d(dst, static_cast<const T*>(from[t]) + (batch * kRows + r) * ld[t], row_bytes, bar);
+        dst += row_bytes;
+      }
+    }
+  }
+  __device__ __forceinline__ void init() {
+    if (threadIdx.x == 0) {
+      *abort_flag = 0;
+      for (int s = 0; s < stages; ++s) ptx::mbar_init(ptx::smem_u32(&full[s]), 1);
+      ptx::fence_mbar_init();
+    }
+    __syncthreads();
+  }
+  __device__ __forceinline__ void start() {
+    stage = 0;
+    phase = 0;
+    alive = true;
+    if (threadIdx.x == 0)
+      for (int s = 0; s < stages; ++s)
+        if (blockIdx.x + static_cast<int64_t>(s) * gridDim.x < batches) fetch(blockIdx.x + static_cast<int64_t>(s) * gridDim.x, s);
+  }
+  // (a wait that gave up is not tried again: the loop runs out with what is in the ring)
+  __device__ __forceinline__ const uint8_t* wait() {
+    if (alive) alive = ptx::mbar_wait(ptx::smem_u32(&full[stage]), phase, ptx::AbortCtl{abort_flag, status_word}, kSiteRing);
+    return data + stage * stage_bytes();
+  }
+  // Behind a barrier that every thread reached after its reads of the stage and a fence_proxy_async_smem.
+  __device__ __forceinline__ void refill(int64_t batch) {
+    const int64_t next = batch + static_cast<int64_t>(stages) * gridDim.x;
+    if (threadIdx.x == 0 && next < batches) fetch(next, stage);
+    if (++stage == stages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+  __device__ __forceinline__ void finish() const {
+    if (*abort_flag != 0) __nanosleep(2000000);      // copies still in flight land before their shared memory is released
+  }
+};
+
+template <typename T, typename P, int kRows>
+__global__ void __launch_bounds__(kRingThreads, 1) row_norm_fwd_ring_kernel(const Args a) {
+  constexpr int kVec = 16 / sizeof(T), kN = kPairs<T>, kPer = kRingElems / kVec;
+  extern __shared__ __align__(16) uint8_t data[];
+  __shared__ alignas(8) uint64_t full[kMaxStages];
+  __shared__ float scratch[2][kRows][16];
+  __shared__ int abort_flag;
+  Ring<T, kRows, 1> ring{data, full, &abort_flag, {a.x}, {a.ldx}, a.rows, (a.rows + kRows - 1) / kRows, static_cast<uint32_t>(a.cols * sizeof(T)), a.stages};
+  ring.status_word = a.status_word;
+  ring.init();
+  ptx::grid_dependency_sync();
+  ring.start();
+  const int nvec = a.cols / kVec;
+  uint64_t scale[kPer][kN], shift[kPer][kN];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int v = threadIdx.x + i * blockDim.x;
+    if (v < nvec) {
+      load_params<P, kN>(a.gain, v * kVec, a.gain_vec, a.gain_offset, 1.0f, scale[i]);
+      load_params<P, kN>(a.shift, v * kVec, a.shift_vec, 0.0f, 0.0f, shift[i]);
+    }
+  }
+  int turn = 0;
+  for (int64_t batch = blockIdx.x; batch < ring.batches; batch += gridDim.x) {
+    const uint8_t* at = ring.wait();
+    uint64_t x[kRows][kPer][kN];
+    float mean[kRows], s[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      uint64_t t = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int v = threadIdx.x + i * blockDim.x;
+        if (v < nvec && batch * kRows + r < a.rows) {
+          unpack_pairs<T>(reinterpret_cast<const uint4*>(at + r * ring.row_bytes)[v], x[r][i]);
+#pragma unroll
+          for (int j = 0; j < kN; ++j) t = ptx::add2(t, x[r][i][j]);
+        }
+      }
+      mean[r] = pair_sum(t);
+    }
+    ptx::fence_proxy_async_smem();      // the reads above come before the copy that overwrites them
+    if (a.rms) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) mean[r] = 0.0f;
+    } else {
+      cta_sums<kRows>(mean, scratch[turn ^ 1]);
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) mean[r] *= a.inv_cols;
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const uint64_t minus = ptx::f32x2(-mean[r], -mean[r]);
+      uint64_t t = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        if (threadIdx.x + i * blockDim.x < nvec && batch * kRows + r < a.rows) {
+#pragma unroll
+          for (int j = 0; j < kN; ++j) {
+            x[r][i][j] = ptx::add2(x[r][i][j], minus);
+            t = ptx::fma2(x[r][i][j], x[r][i][j], t);
+          }
+        }
+      }
+      s[r] = pair_sum(t);
+    }
+    cta_sums<kRows>(s, scratch[turn]);
+    turn ^= a.rms;      // (LayerNorm's two sums alternate by themselves)
+    ring.refill(batch);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const int64_t row = batch * kRows + r;
+      const float rstd = rsqrtf(fmaf(s[r], a.inv_cols, a.eps));
+      const uint64_t r2 = ptx::f32x2(rstd, rstd);
+      uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * a.ldo);
+      if (row < a.rows) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const int v = threadIdx.x + i * blockDim.x;
+          if (v < nvec) {
+#pragma unroll
+            for (int j = 0; j < kN; ++j) x[r][i][j] = ptx::fma2(ptx::mul2(x[r][i][j], r2), scale[i][j], shift[i][j]);
+            out[v] = pack_pairs<T>(x[r][i]);
+          }
+        }
+        if (threadIdx.x == 0) {
+          if (a.mean != nullptr) a.mean[row] = mean[r];
+          if (a.rstd != nullptr) a.rstd[row] = rstd;
+        }
+      }
+    }
+  }
+  ring.finish();
+}
+
+template <typename T, typename P, int kRows>
+__global__ void __launch_bounds__(kRingThreads, 1) row_norm_bwd_ring_kernel(const Args a) {
+  constexpr int kVec = 16 / sizeof(T), kN = kPairs<T>, kPer = kRingElems / kVec;
+  extern __shared__ __align__(16) uint8_t data[];
+  __shared__ alignas(8) uint64_t full[kMaxStages];
+  __shared__ float scratch[2][2 * kRows][16];
+  __shared__ int abort_flag;
+  Ring<T, kRows, 2> ring{data, full, &abort_flag, {a.x, a.gy}, {a.ldx, a.ldg}, a.rows, (a.rows + kRows - 1) / kRows, static_cast<uint32_t>(a.cols * sizeof(T)), a.stages};
+  ring.status_word = a.status_word;
+  ring.init();
+  ptx::grid_dependency_sync();
+  ring.start();
+  const int nvec = a.cols / kVec;
+  uint64_t scale[kPer][kN], dgain[kPer][kN], dshift[kPer][kN];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int v = threadIdx.x + i * blockDim.x;
+    if (v < nvec) load_params<P, kN>(a.gain, v * kVec, a.gain_vec, a.gain_offset, 1.0f, scale[i]);
+#pragma unroll
+    for (int j = 0; j < kN; ++j) dgain[i][j] = dshift[i][j] = 0;
+  }
+  float mean[kRows], rstd[kRows];
+  auto stats = [&](int64_t batch) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const int64_t row = batch * kRows + r;
+      mean[r] = row < a.rows && !a.rms ? a.mean[row] : 0.0f;
+      rstd[r] = row < a.rows ? a.rstd[row] : 0.0f;
+    }
+  };
+  stats(blockIdx.x);
+  int turn = 0;
+  for (int64_t batch = blockIdx.x; batch < ring.batches; batch += gridDim.x) {
+    const uint8_t* at = ring.wait();
+    uint4 xr[kRows][kPer], gr[kRows][kPer];
+    float s[2 * kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      uint64_t hx = 0, hs = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int v = threadIdx.x + i * blockDim.x;
+        if (v < nvec && batch * kRows + r < a.rows) {
+          xr[r][i] = reinterpret_cast<const uint4*>(at + 2 * r * ring.row_bytes)[v];
+          gr[r][i] = reinterpret_cast<const uint4*>(at + (2 * r + 1) * ring.row_bytes)[v];
+          bwd_sums<T, kN>(xr[r][i], gr[r][i], mean[r], rstd[r], scale[i], dgain[i], dshift[i], hx, hs);
+        }
+      }
+      s[2 * r] = pair_sum(hx);
+      s[2 * r + 1] = pair_sum(hs);
+    }
+    ptx::fence_proxy_async_smem();      // the reads above come before the copy that overwrites them
+    cta_sums<2 * kRows>(s, scratch[turn]);
+    turn ^= 1;
+    ring.refill(batch);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const float c1 = s[2 * r] * a.inv_cols, c0 = a.rms ? 0.0f : s[2 * r + 1] * a.inv_cols;
+      uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (batch * kRows + r) * a.ldo);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int v = threadIdx.x + i * blockDim.x;
+        if (batch * kRows + r < a.rows && v < nvec) out[v] = bwd_dx<T, kN>(xr[r][i], gr[r][i], mean[r], rstd[r], scale[i], c1, c0);
+      }
+    }
+    stats(batch + gridDim.x);
+  }
+  ring.finish();
+  if (a.part_gain == nullptr && a.part_shift == nullptr) return;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int v = threadIdx.x + i * blockDim.x;
+    if (v < nvec) {
+      const int64_t at = static_cast<int64_t>(blockIdx.x) * a.cols + v * kVec;
+      if (a.part_gain != nullptr) put_pairs<kN>(a.part_gain + at, dgain[i], false);
+      if (a.part_shift != nullptr) put_pairs<kN>(a.part_shift + at, dshift[i], false);
+    }
+  }
+}
+
+// dgain (blockIdx.y 0) and dshift (1): the CTAs' rows of partials added up, kSumCols columns (a 32-byte sector) per CTA.
 __global__ void __launch_bounds__(kSumCols* kSumParts) row_norm_sum_kernel(const float* part_gain, const float* part_shift, int parts,
                                                                           int cols, void* dgain, void* dshift, int dtype) {
   ptx::grid_dependency_sync();
-  __shared__ float s[kSumParts][kSumCols + 1];
+  __shared__ float s[kSumParts][kSumCols];
   const float* part = blockIdx.y == 0 ? part_gain : part_shift;
   void* out = blockIdx.y == 0 ? dgain : dshift;
   if (out == nullptr) return;
   const int lane = threadIdx.x % kSumCols, p0 = threadIdx.x / kSumCols, c = blockIdx.x * kSumCols + lane;
   float t = 0.0f;
   if (c < cols) {
-#pragma unroll 4
+#pragma unroll 8
     for (int p = p0; p < parts; p += kSumParts) t += part[static_cast<int64_t>(p) * cols + c];
   }
   s[p0][lane] = t;
   __syncthreads();
-  // (column p0 now, its partial sums across the lanes)
-  t = s[lane][p0];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-  const int col = blockIdx.x * kSumCols + p0;
-  if (lane == 0 && col < cols) {
-    if (dtype == IXK_F32) static_cast<float*>(out)[col] = t;
-    else if (dtype == IXK_BF16) static_cast<__nv_bfloat16*>(out)[col] = __float2bfloat16_rn(t);
-    else static_cast<__half*>(out)[col] = __float2half_rn(t);
+  for (int n = kSumParts / 2; n > 0; n /= 2) {
+    if (p0 < n) s[p0][lane] += s[p0 + n][lane];
+    __syncthreads();
+  }
+  if (p0 == 0 && c < cols) {
+    t = s[0][lane];
+    if (dtype == IXK_F32) static_cast<float*>(out)[c] = t;
+    else if (dtype == IXK_BF16) static_cast<__nv_bfloat16*>(out)[c] = __float2bfloat16_rn(t);
+    else static_cast<__half*>(out)[c] = __float2half_rn(t);
   }
 }
 
@@ -351,6 +936,24 @@ Plan plan_for(int64_t cols, int elem_bytes, bool aligned) {
   p.per = per;
   return p;
 }
+// Rows of whole vectors: a warp's (up to eight elements a lane), or a ring's.
+bool short_rows(int64_t cols) { return cols <= 32 * 8; }
+bool vec_takes(int64_t cols) { return cols <= kRingThreads * kRingElems; }
+int ring_threads(int64_t cols) { return static_cast<int>((cols + kRingElems - 1) / kRingElems + 31) / 32 * 32; }
+int ring_ctas_per_sm(int threads) { return std::clamp(kRingThreads / threads, 1, 8); }
+// Two rows a batch where every CTA gets some and the ring holds two batches of them.
+int ring_rows(int64_t cols, int64_t rows, int elem_bytes, bool bwd) {
+  const int ctas = ring_ctas_per_sm(ring_threads(cols));
+  return rows >= 2 * kAssumedSms * ctas && 2 * (bwd ? 4 : 2) * cols * elem_bytes <= kRingBytes / ctas ? 2 : 1;
+}
+int64_t vec_ctas(int64_t cols, int64_t rows, int elem_bytes, bool bwd) {
+  if (short_rows(cols)) {
+    const int64_t warps = (rows + 3) / 4;      // (four rows of 16-bit elements a warp, or more)
+    return bwd ? std::min<int64_t>((warps + 7) / 8, kAssumedSms * 2) : std::min<int64_t>((warps + 3) / 4, kAssumedSms * 8);
+  }
+  const int batch = ring_rows(cols, rows, elem_bytes, bwd);
+  return std::min<int64_t>((rows + batch - 1) / batch, static_cast<int64_t>(kAssumedSms) * ring_ctas_per_sm(ring_threads(cols)));
+}
 int64_t ctas_for(const Plan& p, int64_t rows) {
   const int64_t want = (rows + p.groups_per_cta - 1) / p.groups_per_cta;
   return std::min<int64_t>(want, static_cast<int64_t>(kAssumedSms) * std::max(1, kThreadsPerSm / p.threads));
@@ -368,19 +971,51 @@ int launch(const Plan& p, const Args& a, int64_t ctas, cudaStream_t stream) {
   constexpr int kFull = 16 / sizeof(T);
 #define IXK_NORM_CASE(V, P, W) \
   if (p.vec == V && p.per == P && p.warp == W) return go(std::integral_constant<int, V>{}, std::integral_constant<int, P>{}, std::bool_constant<W>{});
-  IXK_NORM_CASE(kFull, 1, true)
-  if constexpr (kFull == 4) { IXK_NORM_CASE(kFull, 2, true) }
+  IXK_NORM_CASE(kFull, 16 / kFull, false)
   IXK_NORM_CASE(1, 1, true)
   IXK_NORM_CASE(1, 2, true)
   IXK_NORM_CASE(1, 4, true)
   IXK_NORM_CASE(1, 8, true)
-  if constexpr (kFull == 8) { IXK_NORM_CASE(kFull, 1, false) }
-  IXK_NORM_CASE(kFull, 2, false)
-  if constexpr (kFull == 4) { IXK_NORM_CASE(kFull, 4, false) }
   IXK_NORM_CASE(1, 8, false)
   IXK_NORM_CASE(1, 16, false)
 #undef IXK_NORM_CASE
   return fail(IXK_UNIMPLEMENTED, "row_norm: no kernel for this row");
+}
+
+// Whole vectors: warps for short rows, rings for longer ones; kRows to a batch while that leaves every CTA one.
+template <typename T, typename P, bool kBwd>
+int launch_vec(Args a, int64_t ctas, cudaStream_t stream) {
+  if (short_rows(a.cols)) {
+    constexpr int kPer = sizeof(T) / 2;
+    if constexpr (kBwd)
+      return launch_overlapped(row_norm_bwd_rows_kernel<T, P, kPer, 4 / kPer>, dim3(static_cast<unsigned>(ctas)), dim3(256), 2 * sizeof(float) * a.cols, stream, a);
+    else
+      return launch_overlapped(row_norm_fwd_rows_kernel<T, P, kPer, 8 / kPer>, dim3(static_cast<unsigned>(ctas)), dim3(128), 0, stream, a);
+  }
+  auto go = [&](auto rows_tag) -> int {
+    constexpr int kRows = decltype(rows_tag)::value;
+    auto* fn = &row_norm_fwd_ring_kernel<T, P, kRows>;
+    if constexpr (kBwd) fn = &row_norm_bwd_ring_kernel<T, P, kRows>;
+    const int threads = ring_threads(a.cols), stage = (kBwd ? 2 : 1) * kRows * a.cols * static_cast<int>(sizeof(T));
+    a.stages = std::min(kMaxStages, kRingBytes / ring_ctas_per_sm(threads) / stage);
+    static thread_local int configured_device = -1;
+    int dev = 0;
+    IXK_CUDA_OK(cudaGetDevice(&dev));
+    if (configured_device != dev) {
+      IXK_CUDA_OK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes));
+      configured_device = dev;
+    }
+    return launch_overlapped(fn, dim3(static_cast<unsigned>(ctas)), dim3(threads), static_cast<size_t>(a.stages) * stage, stream, a);
+  };
+  return ring_rows(a.cols, a.rows, sizeof(T), kBwd) == 2 ? go(std::integral_constant<int, 2>{}) : go(std::integral_constant<int, 1>{});
+}
+
+// call(a value of the rows' type, one of the parameters')
+template <typename Call>
+int with_types(int dtype, int param_dtype, const Call& call) {
+  if (dtype == IXK_F32) return call(float{}, float{});
+  if (dtype == IXK_BF16) return param_dtype == IXK_F32 ? call(__nv_bfloat16{}, float{}) : call(__nv_bfloat16{}, __nv_bfloat16{});
+  return param_dtype == IXK_F32 ? call(__half{}, float{}) : call(__half{}, __half{});
 }
 
 bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
@@ -432,6 +1067,13 @@ int fwd(const ixk_row_norm_desc* d, const void* x, const void* gain, const void*
   a.eps = d->eps;
   a.gain_offset = d->gain_offset;
   a.inv_cols = 1.0f / static_cast<float>(d->cols);
+  a.gain_vec = aligned(gain, 16);
+  a.shift_vec = aligned(shift, 16);
+  a.status_word = info.status_word;
+  if (wide && d->cols * es % 16 == 0 && vec_takes(d->cols))
+    return with_types(d->dtype, d->param_dtype, [&](auto t, auto pt) {
+      return launch_vec<decltype(t), decltype(pt), false>(a, vec_ctas(d->cols, d->rows, es, false), static_cast<cudaStream_t>(stream));
+    });
   const int64_t want = (d->rows + p.groups_per_cta - 1) / p.groups_per_cta;
   const int64_t ctas = std::min<int64_t>(want, static_cast<int64_t>(info.sm_count) * (2048 / p.threads));
   auto s = static_cast<cudaStream_t>(stream);
@@ -443,7 +1085,8 @@ int fwd(const ixk_row_norm_desc* d, const void* x, const void* gain, const void*
 // (the partials' CTAs must not depend on alignment, which the query does not know: the most that any plan has)
 size_t part_bytes(const ixk_row_norm_desc* d) {
   const int es = bytes_of(d->dtype);
-  const int64_t ctas = std::max(ctas_for(plan_for(d->cols, es, true), d->rows), ctas_for(plan_for(d->cols, es, false), d->rows));
+  const int64_t ctas = std::max({ctas_for(plan_for(d->cols, es, true), d->rows), ctas_for(plan_for(d->cols, es, false), d->rows),
+                                 vec_ctas(d->cols, d->rows, es, true)});
   return static_cast<size_t>(ctas) * d->cols * sizeof(float);
 }
 
@@ -470,7 +1113,8 @@ int bwd(const ixk_row_norm_desc* d, const void* gy, const void* x, const void* g
   const bool wide = aligned(x, 16) && aligned(gy, 16) && aligned(dx, 16) && d->x_stride * es % 16 == 0 &&
                     d->grad_y_stride * es % 16 == 0 && d->dx_stride * es % 16 == 0;
   const Plan p = plan_for(d->cols, es, wide);
-  const int64_t ctas = ctas_for(p, d->rows);
+  const bool vec = wide && d->cols * es % 16 == 0 && vec_takes(d->cols);
+  const int64_t ctas = vec ? vec_ctas(d->cols, d->rows, es, true) : ctas_for(p, d->rows);
   Args a{};
   a.x = x;
   a.gy = gy;
@@ -490,7 +1134,12 @@ int bwd(const ixk_row_norm_desc* d, const void* gy, const void* x, const void* g
   a.gain_offset = d->gain_offset;
   a.inv_cols = 1.0f / static_cast<float>(d->cols);
   auto s = static_cast<cudaStream_t>(stream);
-  if (d->rows > 0) {
+  a.gain_vec = aligned(gain, 16);
+  a.status_word = info.status_word;
+  if (d->rows > 0 && vec) {
+    rc = with_types(d->dtype, d->param_dtype, [&](auto t, auto pt) { return launch_vec<decltype(t), decltype(pt), true>(a, ctas, s); });
+    if (rc != IXK_OK) return rc;
+  } else if (d->rows > 0) {
     rc = d->dtype == IXK_F32 ? launch<float, true>(p, a, ctas, s)
          : d->dtype == IXK_BF16 ? launch<__nv_bfloat16, true>(p, a, ctas, s) : launch<__half, true>(p, a, ctas, s);
     if (rc != IXK_OK) return rc;
