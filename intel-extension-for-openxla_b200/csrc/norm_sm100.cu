@@ -83,7 +83,8 @@ struct Args {
   int cols, rms, param_dtype;
   float eps, gain_offset, inv_cols;
   int gain_vec, shift_vec;      // gain and shift start on 16 bytes
-  int stages;                   // of the ring
+  int stages;                   // of the ring, and a row's bytes in it
+  uint32_t row_bytes;
   int* status_word;
 };
 
@@ -342,6 +343,16 @@ __device__ __forceinline__ uint4 pack_pairs(const uint64_t (&p)[kPairs<T>]) {
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
+template <typename T, int kN>
+__device__ __forceinline__ void unpack_all(const uint4* raw, uint64_t (&p)[kN]) {
+#pragma unroll
+  for (int i = 0; i < kN / kPairs<T>; ++i) {
+    uint64_t part[kPairs<T>];
+    unpack_pairs<T>(raw[i], part);
+#pragma unroll
+    for (int j = 0; j < kPairs<T>; ++j) p[i * kPairs<T> + j] = part[j];
+  }
+}
 __device__ __forceinline__ float pair_sum(uint64_t p) {
   float lo, hi;
   ptx::f32x2_split(p, lo, hi);
@@ -512,14 +523,14 @@ __global__ void __launch_bounds__(128) row_norm_fwd_rows_kernel(const Args a) {
   }
 }
 
-// What a vector of columns adds to a row's two sums, mean(h xh) and mean(h), and to the columns' own.
+// What kN pairs of columns add to a row's two sums, mean(h xh) and mean(h), and to the columns' own.
 template <typename T, int kN>
-__device__ __forceinline__ void bwd_sums(const uint4& xr, const uint4& gr, float mean, float rstd, const uint64_t (&scale)[kN], uint64_t (&dgain)[kN],
+__device__ __forceinline__ void bwd_sums(const uint4* xr, const uint4* gr, float mean, float rstd, const uint64_t (&scale)[kN], uint64_t (&dgain)[kN],
                                          uint64_t (&dshift)[kN], uint64_t& hx, uint64_t& hs) {
   const uint64_t minus = ptx::f32x2(-mean, -mean), r2 = ptx::f32x2(rstd, rstd);
   uint64_t x[kN], g[kN];
-  unpack_pairs<T>(xr, x);
-  unpack_pairs<T>(gr, g);
+  unpack_all<T, kN>(xr, x);
+  unpack_all<T, kN>(gr, g);
 #pragma unroll
   for (int j = 0; j < kN; ++j) {
     const uint64_t xh = ptx::mul2(ptx::add2(x[j], minus), r2), h = ptx::mul2(g[j], scale[j]);
@@ -529,21 +540,24 @@ __device__ __forceinline__ void bwd_sums(const uint4& xr, const uint4& gr, float
     hs = ptx::add2(hs, h);
   }
 }
-// dx of a vector: rstd (h - c0 - xh c1).
+// dx of kN pairs: rstd (h - c0 - xh c1).
 template <typename T, int kN>
-__device__ __forceinline__ uint4 bwd_dx(uint4& xr, uint4& gr, float mean, float rstd, const uint64_t (&scale)[kN], float c1, float c0) {
-  forget(xr);
-  forget(gr);
+__device__ __forceinline__ void bwd_dx(uint4* xr, uint4* gr, float mean, float rstd, const uint64_t (&scale)[kN], float c1, float c0,
+                                       uint64_t (&x)[kN]) {
+#pragma unroll
+  for (int i = 0; i < kN / kPairs<T>; ++i) {
+    forget(xr[i]);
+    forget(gr[i]);
+  }
   const uint64_t minus = ptx::f32x2(-mean, -mean), r2 = ptx::f32x2(rstd, rstd), m1 = ptx::f32x2(-c1, -c1), m0 = ptx::f32x2(-c0, -c0);
-  uint64_t x[kN], g[kN];
-  unpack_pairs<T>(xr, x);
-  unpack_pairs<T>(gr, g);
+  uint64_t g[kN];
+  unpack_all<T, kN>(xr, x);
+  unpack_all<T, kN>(gr, g);
 #pragma unroll
   for (int j = 0; j < kN; ++j) {
     const uint64_t xh = ptx::mul2(ptx::add2(x[j], minus), r2);
     x[j] = ptx::mul2(ptx::fma2(xh, m1, ptx::fma2(g[j], scale[j], m0)), r2);
   }
-  return pack_pairs<T>(x);
 }
 template <int kN>
 __device__ __forceinline__ void put_pairs(float* out, const uint64_t (&p)[kN], bool add) {
@@ -596,7 +610,7 @@ __global__ void __launch_bounds__(256) row_norm_bwd_rows_kernel(const Args a) {
       uint64_t hx = 0, hs = 0;
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
-        if (lane + 32 * i < nvec) bwd_sums<T, kN>(xr[r][i], gr[r][i], mean[r], rstd[r], scale[i], dgain[i], dshift[i], hx, hs);
+        if (lane + 32 * i < nvec) bwd_sums<T, kN>(&xr[r][i], &gr[r][i], mean[r], rstd[r], scale[i], dgain[i], dshift[i], hx, hs);
       s[2 * r] = pair_sum(hx);
       s[2 * r + 1] = pair_sum(hs);
     }
@@ -608,7 +622,11 @@ __global__ void __launch_bounds__(256) row_norm_bwd_rows_kernel(const Args a) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const int v = lane + 32 * i;
-        if (first + r < a.rows && v < nvec) out[v] = bwd_dx<T, kN>(xr[r][i], gr[r][i], mean[r], rstd[r], scale[i], c1, c0);
+        if (first + r < a.rows && v < nvec) {
+          uint64_t dx[kN];
+          bwd_dx<T, kN>(&xr[r][i], &gr[r][i], mean[r], rstd[r], scale[i], c1, c0, dx);
+          out[v] = pack_pairs<T>(dx);
+        }
       }
     }
   }
@@ -632,40 +650,63 @@ __global__ void __launch_bounds__(256) row_norm_bwd_rows_kernel(const Args a) {
   }
 }
 
-// Longer rows of whole vectors: a CTA takes kRows rows at a time out of a ring in shared memory that bulk copies keep full
-// (about 190 KB under way an SM, which registers could not hold beside the parameters and the columns' sums), and one barrier
-// serves the sums of all of them.  A thread has 16 columns: with eight, the sums across threads were a third of all
-// instructions.
+// Longer rows: a CTA takes kRows rows at a time out of a ring in shared memory that bulk copies keep full (about 190 KB under
+// way an SM, which registers could not hold beside the parameters and the columns' sums), and one barrier serves the sums of
+// all of them.  A thread has 16 columns: with eight, the sums across threads were a third of all instructions.
+// kWhole: rows start on 16 bytes and hold whole vectors; a thread has vectors of columns.  Otherwise a row's image in the ring
+// keeps the row's place within 16 bytes, the copy brings every 16-byte piece that the row touches (of the first and the last
+// row only those that lie wholly in it: nothing outside the tensor is read, and the rest comes element by element), and a
+// thread has single columns, blockDim apart.
 enum : int { kSiteRing = 701 };
 constexpr int kRingBytes = 190 * 1024;
-constexpr int kRingThreads = 512, kRingElems = 16;
+constexpr int kRingThreads = 512, kRingElems = 16, kRingPairs = kRingElems / 2;
 constexpr int kMaxStages = 16;
 
 // The ring of kTensors tensors' rows: stage s holds batch blockIdx + s * gridDim, then every stages-th one after it.
-template <typename T, int kRows, int kTensors>
+template <typename T, int kRows, int kTensors, bool kWhole>
 struct Ring {
-  uint8_t* data;        // [stages][kRows][kTensors][row]
+  uint8_t* data;        // [stages][kRows][kTensors][row_bytes]
   uint64_t* full;
   int* abort_flag;
   const void* from[kTensors];
-  int64_t ld[kTensors], rows, batches;
-  uint32_t row_bytes;
+  int64_t ld[kTensors];
+  int rows, batches, cols;
+  uint32_t row_bytes;   // in the ring
   int stages, stage;
   uint32_t phase;
   bool alive;
   int* status_word;
 
+  __device__ __forceinline__ const T* row_of(int t, int row) const { return static_cast<const T*>(from[t]) + row * ld[t]; }
   __device__ __forceinline__ uint32_t stage_bytes() const { return kTensors * kRows * row_bytes; }
-  __device__ __forceinline__ void fetch(int64_t batch, int s) {      // one thread
-    const int n = static_cast<int>(min(static_cast<int64_t>(kRows), rows - batch * kRows));
+  __device__ __forceinline__ int rows_of(int batch) const { return min(kRows, rows - batch * kRows); }
+  // The part of a row's image that the copy brings: [begin, end), bytes from the 16-byte boundary at or in front of the row.
+  __device__ __forceinline__ void copied(int t, int row, uint32_t& begin, uint32_t& end) const {
+    const uint32_t at = reinterpret_cast<uintptr_t>(row_of(t, row)) & 15u;
+    begin = row == 0 ? (at + 15u) & ~15u : 0;
+    end = (at + cols * static_cast<uint32_t>(sizeof(T)) + (row == rows - 1 ? 0u : 15u)) & ~15u;
+  }
+  __device__ __forceinline__ void fetch(int batch, int s) {      // one thread
+    const int n = rows_of(batch);
     const uint32_t bar = ptx::smem_u32(&full[s]);
-    uint32_t dst = ptx::smem_u32(data) + s * stage_bytes();
-    ptx::mbar_expect_tx(bar, kTensors * n * row_bytes);
+    const uint32_t dst = ptx::smem_u32(data) + s * stage_bytes();
+    uint32_t bytes = kTensors * n * row_bytes, begin = 0, end = row_bytes;
+    if constexpr (!kWhole) {
+      bytes = 0;
+      for (int i = 0; i < n * kTensors; ++i) {
+        copied(i % kTensors, batch * kRows + i / kTensors, begin, end);
+        bytes += end > begin ? end - begin : 0;
+      }
+    }
+    ptx::mbar_expect_tx(bar, bytes);
     for (int r = 0; r < n; ++r) {
 #pragma unroll
       for (int t = 0; t < kTensors; ++t) {
-        ptx::bulk_load_1d(dst, static_cast<const T*>(from[t]) + (batch * kRows + r) * ld[t], row_bytes, bar);
-        dst += row_bytes;
+        const T* row = row_of(t, batch * kRows + r);
+        if constexpr (!kWhole) copied(t, batch * kRows + r, begin, end);
+        if (kWhole || end > begin)
+          ptx::bulk_load_1d(dst + (r * kTensors + t) * row_bytes + begin,
+                            reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(row) & ~uintptr_t(15)) + begin, end - begin, bar);
       }
     }
   }
@@ -683,17 +724,59 @@ struct Ring {
     alive = true;
     if (threadIdx.x == 0)
       for (int s = 0; s < stages; ++s)
-        if (blockIdx.x + static_cast<int64_t>(s) * gridDim.x < batches) fetch(blockIdx.x + static_cast<int64_t>(s) * gridDim.x, s);
+        if (batches - static_cast<int>(blockIdx.x) > s * static_cast<int>(gridDim.x)) fetch(blockIdx.x + s * gridDim.x, s);
   }
   // (a wait that gave up is not tried again: the loop runs out with what is in the ring)
-  __device__ __forceinline__ const uint8_t* wait() {
+  __device__ __forceinline__ const uint8_t* wait(int batch) {
     if (alive) alive = ptx::mbar_wait(ptx::smem_u32(&full[stage]), phase, ptx::AbortCtl{abort_flag, status_word}, kSiteRing);
-    return data + stage * stage_bytes();
+    uint8_t* at = data + stage * stage_bytes();
+    const int first = batch * kRows, last = first + rows_of(batch) - 1;
+    if (!kWhole && (first == 0 || last == rows - 1)) {      // what the copies left out of the first and the last row
+      for (int i = 0; i < 2 * kTensors; ++i) {
+        const int t = i >> 1, row = i & 1 ? rows - 1 : 0;
+        if (row < first || row > last) continue;
+        uint32_t begin, end;
+        copied(t, row, begin, end);
+        const uint32_t start = reinterpret_cast<uintptr_t>(row_of(t, row)) & 15u;
+        uint8_t* image = at + ((row - first) * kTensors + t) * row_bytes;
+        for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+          const uint32_t p = start + c * static_cast<uint32_t>(sizeof(T));
+          if (p < begin || p >= end) *reinterpret_cast<Raw<T, 1>*>(image + p) = reinterpret_cast<const volatile Raw<T, 1>*>(row_of(t, row))[c];
+        }
+      }
+      __syncthreads();
+    }
+    return at;
+  }
+  // This thread's 16 columns of a row, zeros where there are none.
+  __device__ __forceinline__ void read(const uint8_t* at, int t, int r, int batch, uint4 (&raw)[kRingPairs / kPairs<T>]) const {
+    const uint8_t* image = at + (r * kTensors + t) * row_bytes;
+    constexpr int kVec = 2 * kPairs<T>, kCount = kRingPairs / kPairs<T>;
+    if constexpr (kWhole) {
+#pragma unroll
+      for (int i = 0; i < kCount; ++i) {
+        const int v = threadIdx.x + i * blockDim.x;
+        raw[i] = v * kVec < cols ? reinterpret_cast<const uint4*>(image)[v] : make_uint4(0, 0, 0, 0);
+      }
+    } else {
+      const Raw<T, 1>* row = reinterpret_cast<const Raw<T, 1>*>(image + (reinterpret_cast<uintptr_t>(row_of(t, batch * kRows + r)) & 15u));
+      uint32_t words[kCount * 4];
+#pragma unroll
+      for (int e = 0; e < kRingElems; ++e) {
+        const int c = threadIdx.x + e * blockDim.x;
+        const uint32_t bits = c < cols ? row[c] : 0;
+        if constexpr (sizeof(T) == 4) words[e] = bits;
+        else if (e & 1) words[e / 2] |= bits << 16;
+        else words[e / 2] = bits;
+      }
+#pragma unroll
+      for (int i = 0; i < kCount; ++i) raw[i] = make_uint4(words[4 * i], words[4 * i + 1], words[4 * i + 2], words[4 * i + 3]);
+    }
   }
   // Behind a barrier that every thread reached after its reads of the stage and a fence_proxy_async_smem.
-  __device__ __forceinline__ void refill(int64_t batch) {
-    const int64_t next = batch + static_cast<int64_t>(stages) * gridDim.x;
-    if (threadIdx.x == 0 && next < batches) fetch(next, stage);
+  __device__ __forceinline__ void refill(int batch) {
+    const int ahead = stages * gridDim.x;
+    if (threadIdx.x == 0 && ahead < batches - batch) fetch(batch + ahead, stage);
     if (++stage == stages) {
       stage = 0;
       phase ^= 1u;
@@ -704,44 +787,89 @@ struct Ring {
   }
 };
 
-template <typename T, typename P, int kRows>
+// The column of a thread's element e (pair e / 2): kWhole, element e % kVec of vector thread + (e / kVec) * threads.
+template <typename T, bool kWhole>
+__device__ __forceinline__ int column_of(int e) {
+  constexpr int kVec = 2 * kPairs<T>;
+  return kWhole ? (threadIdx.x + e / kVec * blockDim.x) * kVec + e % kVec : threadIdx.x + e * blockDim.x;
+}
+template <typename T, bool kWhole>
+__device__ __forceinline__ void write_row(T* row, int cols, const uint64_t (&p)[kRingPairs]) {
+  constexpr int kN = kPairs<T>;
+  if constexpr (kWhole) {
+#pragma unroll
+    for (int i = 0; i < kRingPairs / kN; ++i) {
+      uint64_t part[kN];
+#pragma unroll
+      for (int j = 0; j < kN; ++j) part[j] = p[i * kN + j];
+      const int v = threadIdx.x + i * blockDim.x;
+      if (v * 2 * kN < cols) reinterpret_cast<uint4*>(row)[v] = pack_pairs<T>(part);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kRingPairs; ++j) {
+      float f[2];
+      ptx::f32x2_split(p[j], f[0], f[1]);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int c = column_of<T, false>(2 * j + k);
+        if (c < cols) row[c] = from_float<T>(f[k]);
+      }
+    }
+  }
+}
+template <typename T, typename P, bool kWhole>
+__device__ __forceinline__ void ring_params(const void* p, int cols, bool vec, float offset, float none, uint64_t (&out)[kRingPairs]) {
+  constexpr int kN = kPairs<T>;
+  if constexpr (kWhole) {
+#pragma unroll
+    for (int i = 0; i < kRingPairs / kN; ++i) {
+      uint64_t part[kN] = {};
+      const int c = column_of<T, true>(2 * kN * i);
+      if (c < cols) load_params<P, kN>(p, c, vec, offset, none, part);
+#pragma unroll
+      for (int j = 0; j < kN; ++j) out[i * kN + j] = part[j];
+    }
+  } else {
+    const P* at = static_cast<const P*>(p);
+#pragma unroll
+    for (int j = 0; j < kRingPairs; ++j) {      // (a column behind the last one is never used)
+      const int c = min(column_of<T, false>(2 * j), cols - 1), d = min(column_of<T, false>(2 * j + 1), cols - 1);
+      out[j] = p == nullptr ? ptx::f32x2(none, none) : ptx::f32x2(offset + to_float<P>(at[c]), offset + to_float<P>(at[d]));
+    }
+  }
+}
+
+template <typename T, typename P, int kRows, bool kWhole>
 __global__ void __launch_bounds__(kRingThreads, 1) row_norm_fwd_ring_kernel(const Args a) {
-  constexpr int kVec = 16 / sizeof(T), kN = kPairs<T>, kPer = kRingElems / kVec;
   extern __shared__ __align__(16) uint8_t data[];
   __shared__ alignas(8) uint64_t full[kMaxStages];
   __shared__ float scratch[2][kRows][16];
   __shared__ int abort_flag;
-  Ring<T, kRows, 1> ring{data, full, &abort_flag, {a.x}, {a.ldx}, a.rows, (a.rows + kRows - 1) / kRows, static_cast<uint32_t>(a.cols * sizeof(T)), a.stages};
+  Ring<T, kRows, 1, kWhole> ring{data, full, &abort_flag, {a.x}, {a.ldx}, static_cast<int>(a.rows), static_cast<int>((a.rows + kRows - 1) / kRows),
+                                 a.cols, a.row_bytes, a.stages};
   ring.status_word = a.status_word;
   ring.init();
   ptx::grid_dependency_sync();
   ring.start();
-  const int nvec = a.cols / kVec;
-  uint64_t scale[kPer][kN], shift[kPer][kN];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int v = threadIdx.x + i * blockDim.x;
-    if (v < nvec) {
-      load_params<P, kN>(a.gain, v * kVec, a.gain_vec, a.gain_offset, 1.0f, scale[i]);
-      load_params<P, kN>(a.shift, v * kVec, a.shift_vec, 0.0f, 0.0f, shift[i]);
-    }
-  }
+  uint64_t scale[kRingPairs], shift[kRingPairs];
+  ring_params<T, P, kWhole>(a.gain, a.cols, a.gain_vec, a.gain_offset, 1.0f, scale);
+  ring_params<T, P, kWhole>(a.shift, a.cols, a.shift_vec, 0.0f, 0.0f, shift);
   int turn = 0;
-  for (int64_t batch = blockIdx.x; batch < ring.batches; batch += gridDim.x) {
-    const uint8_t* at = ring.wait();
-    uint64_t x[kRows][kPer][kN];
+  for (int batch = blockIdx.x; batch < ring.batches; batch += gridDim.x) {      // (rows + gridDim * stages fits an int: check())
+    const int there = ring.rows_of(batch);
+    const uint8_t* at = ring.wait(batch);
+    uint64_t x[kRows][kRingPairs];
     float mean[kRows], s[kRows];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       uint64_t t = 0;
+      if (r < there) {
+        uint4 raw[kRingPairs / kPairs<T>];
+        ring.read(at, 0, r, batch, raw);
+        unpack_all<T, kRingPairs>(raw, x[r]);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int v = threadIdx.x + i * blockDim.x;
-        if (v < nvec && batch * kRows + r < a.rows) {
-          unpack_pairs<T>(reinterpret_cast<const uint4*>(at + r * ring.row_bytes)[v], x[r][i]);
-#pragma unroll
-          for (int j = 0; j < kN; ++j) t = ptx::add2(t, x[r][i][j]);
-        }
+        for (int j = 0; j < kRingPairs; ++j) t = ptx::add2(t, x[r][j]);
       }
       mean[r] = pair_sum(t);
     }
@@ -756,15 +884,19 @@ __global__ void __launch_bounds__(kRingThreads, 1) row_norm_fwd_ring_kernel(cons
     }
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const uint64_t minus = ptx::f32x2(-mean[r], -mean[r]);
       uint64_t t = 0;
+      if (r < there) {
+        const uint64_t minus = ptx::f32x2(-mean[r], -mean[r]);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        if (threadIdx.x + i * blockDim.x < nvec && batch * kRows + r < a.rows) {
-#pragma unroll
-          for (int j = 0; j < kN; ++j) {
-            x[r][i][j] = ptx::add2(x[r][i][j], minus);
-            t = ptx::fma2(x[r][i][j], x[r][i][j], t);
+        for (int j = 0; j < kRingPairs; ++j) {
+          x[r][j] = ptx::add2(x[r][j], minus);
+          // (columns behind the row's end count nothing; whole vectors end together)
+          if (kWhole ? column_of<T, true>(2 * j) < a.cols : column_of<T, false>(2 * j + 1) < a.cols) {
+            t = ptx::fma2(x[r][j], x[r][j], t);
+          } else if (!kWhole && column_of<T, false>(2 * j) < a.cols) {
+            float lo, hi;
+            ptx::f32x2_split(x[r][j], lo, hi);
+            t = ptx::add2(t, ptx::f32x2(lo * lo, 0.0f));
           }
         }
       }
@@ -775,20 +907,13 @@ __global__ void __launch_bounds__(kRingThreads, 1) row_norm_fwd_ring_kernel(cons
     ring.refill(batch);
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const int64_t row = batch * kRows + r;
-      const float rstd = rsqrtf(fmaf(s[r], a.inv_cols, a.eps));
-      const uint64_t r2 = ptx::f32x2(rstd, rstd);
-      uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * a.ldo);
-      if (row < a.rows) {
+      if (r < there) {
+        const int64_t row = static_cast<int64_t>(batch) * kRows + r;
+        const float rstd = rsqrtf(fmaf(s[r], a.inv_cols, a.eps));
+        const uint64_t r2 = ptx::f32x2(rstd, rstd);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          const int v = threadIdx.x + i * blockDim.x;
-          if (v < nvec) {
-#pragma unroll
-            for (int j = 0; j < kN; ++j) x[r][i][j] = ptx::fma2(ptx::mul2(x[r][i][j], r2), scale[i][j], shift[i][j]);
-            out[v] = pack_pairs<T>(x[r][i]);
-          }
-        }
+        for (int j = 0; j < kRingPairs; ++j) x[r][j] = ptx::fma2(ptx::mul2(x[r][j], r2), scale[j], shift[j]);
+        write_row<T, kWhole>(static_cast<T*>(a.out) + row * a.ldo, a.cols, x[r]);
         if (threadIdx.x == 0) {
           if (a.mean != nullptr) a.mean[row] = mean[r];
           if (a.rstd != nullptr) a.rstd[row] = rstd;
@@ -799,53 +924,53 @@ __global__ void __launch_bounds__(kRingThreads, 1) row_norm_fwd_ring_kernel(cons
   ring.finish();
 }
 
-template <typename T, typename P, int kRows>
+template <typename T, typename P, int kRows, bool kWhole>
 __global__ void __launch_bounds__(kRingThreads, 1) row_norm_bwd_ring_kernel(const Args a) {
-  constexpr int kVec = 16 / sizeof(T), kN = kPairs<T>, kPer = kRingElems / kVec;
+  constexpr int kCount = kRingPairs / kPairs<T>;
   extern __shared__ __align__(16) uint8_t data[];
   __shared__ alignas(8) uint64_t full[kMaxStages];
   __shared__ float scratch[2][2 * kRows][16];
   __shared__ int abort_flag;
-  Ring<T, kRows, 2> ring{data, full, &abort_flag, {a.x, a.gy}, {a.ldx, a.ldg}, a.rows, (a.rows + kRows - 1) / kRows, static_cast<uint32_t>(a.cols * sizeof(T)), a.stages};
+  Ring<T, kRows, 2, kWhole> ring{data, full, &abort_flag, {a.x, a.gy}, {a.ldx, a.ldg}, static_cast<int>(a.rows), static_cast<int>((a.rows + kRows - 1) / kRows),
+                                 a.cols, a.row_bytes, a.stages};
   ring.status_word = a.status_word;
   ring.init();
   ptx::grid_dependency_sync();
   ring.start();
-  const int nvec = a.cols / kVec;
-  uint64_t scale[kPer][kN], dgain[kPer][kN], dshift[kPer][kN];
+  uint64_t scale[kRingPairs], dgain[kRingPairs], dshift[kRingPairs];
+  ring_params<T, P, kWhole>(a.gain, a.cols, a.gain_vec, a.gain_offset, 1.0f, scale);
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int v = threadIdx.x + i * blockDim.x;
-    if (v < nvec) load_params<P, kN>(a.gain, v * kVec, a.gain_vec, a.gain_offset, 1.0f, scale[i]);
-#pragma unroll
-    for (int j = 0; j < kN; ++j) dgain[i][j] = dshift[i][j] = 0;
-  }
-  float mean[kRows], rstd[kRows];
-  auto stats = [&](int64_t batch) {
+  for (int j = 0; j < kRingPairs; ++j) dgain[j] = dshift[j] = 0;
+  float next_mean[kRows], next_rstd[kRows];
+  auto stats = [&](int batch) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const int64_t row = batch * kRows + r;
-      mean[r] = row < a.rows && !a.rms ? a.mean[row] : 0.0f;
-      rstd[r] = row < a.rows ? a.rstd[row] : 0.0f;
+      const bool is = batch < ring.batches && r < ring.rows_of(batch);
+      next_mean[r] = is && !a.rms ? a.mean[batch * kRows + r] : 0.0f;
+      next_rstd[r] = is ? a.rstd[batch * kRows + r] : 0.0f;
     }
   };
   stats(blockIdx.x);
   int turn = 0;
-  for (int64_t batch = blockIdx.x; batch < ring.batches; batch += gridDim.x) {
-    const uint8_t* at = ring.wait();
-    uint4 xr[kRows][kPer], gr[kRows][kPer];
+  for (int batch = blockIdx.x; batch < ring.batches; batch += gridDim.x) {      // (rows + gridDim * stages fits an int: check())
+    const int there = ring.rows_of(batch);
+    float mean[kRows], rstd[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      mean[r] = next_mean[r];
+      rstd[r] = next_rstd[r];
+    }
+    stats(batch + gridDim.x);
+    const uint8_t* at = ring.wait(batch);
+    uint4 xr[kRows][kCount], gr[kRows][kCount];
     float s[2 * kRows];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       uint64_t hx = 0, hs = 0;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int v = threadIdx.x + i * blockDim.x;
-        if (v < nvec && batch * kRows + r < a.rows) {
-          xr[r][i] = reinterpret_cast<const uint4*>(at + 2 * r * ring.row_bytes)[v];
-          gr[r][i] = reinterpret_cast<const uint4*>(at + (2 * r + 1) * ring.row_bytes)[v];
-          bwd_sums<T, kN>(xr[r][i], gr[r][i], mean[r], rstd[r], scale[i], dgain[i], dshift[i], hx, hs);
-        }
+      if (r < there) {      // (behind the row's end grad_y reads 0)
+        ring.read(at, 0, r, batch, xr[r]);
+        ring.read(at, 1, r, batch, gr[r]);
+        bwd_sums<T, kRingPairs>(xr[r], gr[r], mean[r], rstd[r], scale, dgain, dshift, hx, hs);
       }
       s[2 * r] = pair_sum(hx);
       s[2 * r + 1] = pair_sum(hs);
@@ -856,25 +981,30 @@ __global__ void __launch_bounds__(kRingThreads, 1) row_norm_bwd_ring_kernel(cons
     ring.refill(batch);
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const float c1 = s[2 * r] * a.inv_cols, c0 = a.rms ? 0.0f : s[2 * r + 1] * a.inv_cols;
-      uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (batch * kRows + r) * a.ldo);
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int v = threadIdx.x + i * blockDim.x;
-        if (batch * kRows + r < a.rows && v < nvec) out[v] = bwd_dx<T, kN>(xr[r][i], gr[r][i], mean[r], rstd[r], scale[i], c1, c0);
+      if (r < there) {
+        const float c1 = s[2 * r] * a.inv_cols, c0 = a.rms ? 0.0f : s[2 * r + 1] * a.inv_cols;
+        uint64_t dx[kRingPairs];
+        bwd_dx<T, kRingPairs>(xr[r], gr[r], mean[r], rstd[r], scale, c1, c0, dx);
+        write_row<T, kWhole>(static_cast<T*>(a.out) + static_cast<int64_t>(batch * kRows + r) * a.ldo, a.cols, dx);
       }
     }
-    stats(batch + gridDim.x);
   }
   ring.finish();
-  if (a.part_gain == nullptr && a.part_shift == nullptr) return;
+  float* parts[2] = {a.part_gain, a.part_shift};
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int v = threadIdx.x + i * blockDim.x;
-    if (v < nvec) {
-      const int64_t at = static_cast<int64_t>(blockIdx.x) * a.cols + v * kVec;
-      if (a.part_gain != nullptr) put_pairs<kN>(a.part_gain + at, dgain[i], false);
-      if (a.part_shift != nullptr) put_pairs<kN>(a.part_shift + at, dshift[i], false);
+  for (int t = 0; t < 2; ++t) {
+    if (parts[t] != nullptr) {
+      float* out = parts[t] + static_cast<int64_t>(blockIdx.x) * a.cols;
+#pragma unroll
+      for (int j = 0; j < kRingPairs; ++j) {
+        float f[2];
+        ptx::f32x2_split(t == 0 ? dgain[j] : dshift[j], f[0], f[1]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int c = column_of<T, kWhole>(2 * j + k);
+          if (c < a.cols) out[c] = f[k];
+        }
+      }
     }
   }
 }
@@ -936,15 +1066,17 @@ Plan plan_for(int64_t cols, int elem_bytes, bool aligned) {
   p.per = per;
   return p;
 }
-// Rows of whole vectors: a warp's (up to eight elements a lane), or a ring's.
+// Short rows (up to eight elements a lane of a warp) and those that the ring takes.
 bool short_rows(int64_t cols) { return cols <= 32 * 8; }
-bool vec_takes(int64_t cols) { return cols <= kRingThreads * kRingElems; }
+bool vec_takes(int64_t cols, bool whole) { return cols <= kRingThreads * kRingElems && (whole || !short_rows(cols)); }
 int ring_threads(int64_t cols) { return static_cast<int>((cols + kRingElems - 1) / kRingElems + 31) / 32 * 32; }
 int ring_ctas_per_sm(int threads) { return std::clamp(kRingThreads / threads, 1, 8); }
-// Two rows a batch where every CTA gets some and the ring holds two batches of them.
+// (a row that is not whole vectors keeps its place within 16 bytes)
+int64_t ring_row_bytes(int64_t cols, int elem_bytes, bool whole) { return whole ? cols * elem_bytes : (cols * elem_bytes + 15) / 16 * 16 + 16; }
+// Two rows a batch where every CTA gets two batches and the ring holds two batches of them.
 int ring_rows(int64_t cols, int64_t rows, int elem_bytes, bool bwd) {
   const int ctas = ring_ctas_per_sm(ring_threads(cols));
-  return rows >= 2 * kAssumedSms * ctas && 2 * (bwd ? 4 : 2) * cols * elem_bytes <= kRingBytes / ctas ? 2 : 1;
+  return rows >= 4 * kAssumedSms * ctas && 2 * (bwd ? 4 : 2) * ring_row_bytes(cols, elem_bytes, false) <= kRingBytes / ctas ? 2 : 1;
 }
 int64_t vec_ctas(int64_t cols, int64_t rows, int elem_bytes, bool bwd) {
   if (short_rows(cols)) {
@@ -976,15 +1108,14 @@ int launch(const Plan& p, const Args& a, int64_t ctas, cudaStream_t stream) {
   IXK_NORM_CASE(1, 2, true)
   IXK_NORM_CASE(1, 4, true)
   IXK_NORM_CASE(1, 8, true)
-  IXK_NORM_CASE(1, 8, false)
   IXK_NORM_CASE(1, 16, false)
 #undef IXK_NORM_CASE
   return fail(IXK_UNIMPLEMENTED, "row_norm: no kernel for this row");
 }
 
-// Whole vectors: warps for short rows, rings for longer ones; kRows to a batch while that leaves every CTA one.
+// Short rows of whole vectors by the warp, longer rows of any kind by the ring.
 template <typename T, typename P, bool kBwd>
-int launch_vec(Args a, int64_t ctas, cudaStream_t stream) {
+int launch_vec(Args a, bool whole, int64_t ctas, cudaStream_t stream) {
   if (short_rows(a.cols)) {
     constexpr int kPer = sizeof(T) / 2;
     if constexpr (kBwd)
@@ -992,11 +1123,13 @@ int launch_vec(Args a, int64_t ctas, cudaStream_t stream) {
     else
       return launch_overlapped(row_norm_fwd_rows_kernel<T, P, kPer, 8 / kPer>, dim3(static_cast<unsigned>(ctas)), dim3(128), 0, stream, a);
   }
-  auto go = [&](auto rows_tag) -> int {
+  auto go = [&](auto rows_tag, auto whole_tag) -> int {
     constexpr int kRows = decltype(rows_tag)::value;
-    auto* fn = &row_norm_fwd_ring_kernel<T, P, kRows>;
-    if constexpr (kBwd) fn = &row_norm_bwd_ring_kernel<T, P, kRows>;
-    const int threads = ring_threads(a.cols), stage = (kBwd ? 2 : 1) * kRows * a.cols * static_cast<int>(sizeof(T));
+    constexpr bool kWhole = decltype(whole_tag)::value;
+    auto* fn = &row_norm_fwd_ring_kernel<T, P, kRows, kWhole>;
+    if constexpr (kBwd) fn = &row_norm_bwd_ring_kernel<T, P, kRows, kWhole>;
+    a.row_bytes = static_cast<uint32_t>(ring_row_bytes(a.cols, sizeof(T), kWhole));
+    const int threads = ring_threads(a.cols), stage = (kBwd ? 2 : 1) * kRows * static_cast<int>(a.row_bytes);
     a.stages = std::min(kMaxStages, kRingBytes / ring_ctas_per_sm(threads) / stage);
     static thread_local int configured_device = -1;
     int dev = 0;
@@ -1007,7 +1140,11 @@ int launch_vec(Args a, int64_t ctas, cudaStream_t stream) {
     }
     return launch_overlapped(fn, dim3(static_cast<unsigned>(ctas)), dim3(threads), static_cast<size_t>(a.stages) * stage, stream, a);
   };
-  return ring_rows(a.cols, a.rows, sizeof(T), kBwd) == 2 ? go(std::integral_constant<int, 2>{}) : go(std::integral_constant<int, 1>{});
+  const bool two = ring_rows(a.cols, a.rows, sizeof(T), kBwd) == 2;
+  constexpr std::integral_constant<int, 1> kOne;
+  constexpr std::integral_constant<int, 2> kTwo;
+  if (whole) return two ? go(kTwo, std::true_type{}) : go(kOne, std::true_type{});
+  return two ? go(kTwo, std::false_type{}) : go(kOne, std::false_type{});
 }
 
 // call(a value of the rows' type, one of the parameters')
@@ -1032,7 +1169,7 @@ int check(const ixk_row_norm_desc* d, const char* name) {
   if (d->reserved != 0) return fail(IXK_INVALID_ARGUMENT, who + "desc.reserved must be 0");
   if (d->rows < 0 || d->cols <= 0) return fail(IXK_INVALID_ARGUMENT, who + "negative rows or no columns");
   if (d->cols > kMaxCols) return fail(IXK_UNIMPLEMENTED, who + "rows longer than 16384 elements");
-  if (d->rows > 0x7fffffff) return fail(IXK_UNIMPLEMENTED, who + "more than 2^31-1 rows");
+  if (d->rows > (1 << 30)) return fail(IXK_UNIMPLEMENTED, who + "more than 2^30 rows");
   if (!(d->eps >= 0.0f)) return fail(IXK_INVALID_ARGUMENT, who + "eps must not be negative");
   return IXK_OK;
 }
@@ -1070,9 +1207,10 @@ int fwd(const ixk_row_norm_desc* d, const void* x, const void* gain, const void*
   a.gain_vec = aligned(gain, 16);
   a.shift_vec = aligned(shift, 16);
   a.status_word = info.status_word;
-  if (wide && d->cols * es % 16 == 0 && vec_takes(d->cols))
+  const bool whole = wide && d->cols * es % 16 == 0;
+  if (vec_takes(d->cols, whole))
     return with_types(d->dtype, d->param_dtype, [&](auto t, auto pt) {
-      return launch_vec<decltype(t), decltype(pt), false>(a, vec_ctas(d->cols, d->rows, es, false), static_cast<cudaStream_t>(stream));
+      return launch_vec<decltype(t), decltype(pt), false>(a, whole, vec_ctas(d->cols, d->rows, es, false), static_cast<cudaStream_t>(stream));
     });
   const int64_t want = (d->rows + p.groups_per_cta - 1) / p.groups_per_cta;
   const int64_t ctas = std::min<int64_t>(want, static_cast<int64_t>(info.sm_count) * (2048 / p.threads));
@@ -1113,7 +1251,7 @@ int bwd(const ixk_row_norm_desc* d, const void* gy, const void* x, const void* g
   const bool wide = aligned(x, 16) && aligned(gy, 16) && aligned(dx, 16) && d->x_stride * es % 16 == 0 &&
                     d->grad_y_stride * es % 16 == 0 && d->dx_stride * es % 16 == 0;
   const Plan p = plan_for(d->cols, es, wide);
-  const bool vec = wide && d->cols * es % 16 == 0 && vec_takes(d->cols);
+  const bool whole = wide && d->cols * es % 16 == 0, vec = vec_takes(d->cols, whole);
   const int64_t ctas = vec ? vec_ctas(d->cols, d->rows, es, true) : ctas_for(p, d->rows);
   Args a{};
   a.x = x;
@@ -1137,7 +1275,7 @@ int bwd(const ixk_row_norm_desc* d, const void* gy, const void* x, const void* g
   a.gain_vec = aligned(gain, 16);
   a.status_word = info.status_word;
   if (d->rows > 0 && vec) {
-    rc = with_types(d->dtype, d->param_dtype, [&](auto t, auto pt) { return launch_vec<decltype(t), decltype(pt), true>(a, ctas, s); });
+    rc = with_types(d->dtype, d->param_dtype, [&](auto t, auto pt) { return launch_vec<decltype(t), decltype(pt), true>(a, whole, ctas, s); });
     if (rc != IXK_OK) return rc;
   } else if (d->rows > 0) {
     rc = d->dtype == IXK_F32 ? launch<float, true>(p, a, ctas, s)
