@@ -381,6 +381,12 @@ __device__ __forceinline__ uint32_t ld_shared_cluster_u32(uint32_t local_addr, u
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
   return v;
 }
+// Four floats at a shared::cluster address (see map_to_cta), 16-byte aligned.
+__device__ __forceinline__ float4 ld_shared_cluster_f32x4(uint32_t addr_cluster) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr_cluster) : "memory");
+  return v;
+}
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t smem_dst, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_dst), "r"(ncols)
                : "memory");
