@@ -218,7 +218,7 @@ def _bind_native(lib) -> None:
 
 
 def _native_result(r):
-    """A native call's answer that is not None: the result tensor, or a status."""
+    """A native call's answer that is not None: the result tensor or tensors, or a status."""
     if type(r) is int:
         _check(r)
     return r
@@ -597,6 +597,10 @@ def row_norm_forward(x: torch.Tensor, *, kind: int = NORM_LAYER, eps: float = 1e
     training: the fp32 row statistics (x's shape without its last dimension; mean is None for RMS) are what
     row_norm_backward wants.  x bfloat16, float16 or float32, dense or 2-D with a row pitch; gain and shift of x's type or
     float32."""
+    if _NATIVE is not None:
+        r = _NATIVE.row_norm_forward(x, kind, eps, gain, gain_offset, shift, out, stream)
+        if r is not None:
+            return _native_result(r)
     d = _row_norm_desc(x, kind, gain, gain_offset, shift, eps)
     _require_cuda(x, gain, shift, out)
     if out is None:
@@ -620,6 +624,10 @@ def row_norm_backward(grad_out: torch.Tensor, x: torch.Tensor, mean: Optional[to
                       grad_x: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None, stream=None):
     """(dx, dgain, dshift) of row_norm_forward.  dgain is None without a gain, dshift unless with_shift; both have gain's
     type (x's without one) and are sums over all rows, taken in a fixed order.  grad_x may be grad_out or x."""
+    if _NATIVE is not None:
+        r = _NATIVE.row_norm_backward(grad_out, x, mean, rstd, kind, gain, gain_offset, with_shift, grad_x, workspace, stream)
+        if r is not None:
+            return _native_result(r)
     d = _row_norm_desc(x, kind, gain, gain_offset, None, 0.0)
     _require_cuda(grad_out, x, mean, rstd, gain, grad_x, workspace)
     if grad_x is None:
@@ -768,6 +776,10 @@ def linear_loss_workspace_bytes(x: torch.Tensor, weight: torch.Tensor, entries: 
 
 
 def _linear_loss_forward(x, weight, bias, index, teacher, scale, ignore_index, workspace, stream):
+    if _NATIVE is not None:
+        r = _NATIVE.linear_loss_forward(x, weight, bias, index, teacher, scale, ignore_index, workspace, stream)
+        if r is not None:
+            return _native_result(r)
     d = _linear_loss_desc(x, weight, bias, index, teacher, scale, ignore_index)
     _require_cuda(x, weight, bias, index, teacher, workspace)
     lib = load_library()
@@ -785,6 +797,11 @@ def _linear_loss_forward(x, weight, bias, index, teacher, scale, ignore_index, w
 
 def _linear_loss_backward(x, weight, bias, index, teacher, lse, grad_loss, scale, ignore_index, grad_x, grad_weight, weight_grad, workspace,
                           stream):
+    if _NATIVE is not None:
+        r = _NATIVE.linear_loss_backward(x, weight, bias, index, teacher, lse, grad_loss, scale, ignore_index, grad_x, grad_weight, weight_grad,
+                                         workspace, stream)
+        if r is not None:
+            return _native_result(r)
     d = _linear_loss_desc(x, weight, bias, index, teacher, scale, ignore_index)
     _require_cuda(x, weight, bias, index, teacher, lse, grad_loss, grad_x, grad_weight, workspace)
     if lse.shape != (d.rows,) or lse.dtype != torch.float32 or not lse.is_contiguous():

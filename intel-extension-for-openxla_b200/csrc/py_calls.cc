@@ -33,6 +33,14 @@ decltype(&ixk_row_norm_gain) g_row_norm_gain;
 decltype(&ixk_rotary_interleaved) g_rotary, g_rotary_half;
 decltype(&ixk_kv_append) g_kv_append;
 decltype(&ixk_residual_add) g_residual_add;
+decltype(&ixk_row_norm_fwd) g_norm_fwd;
+decltype(&ixk_row_norm_bwd) g_norm_bwd;
+decltype(&ixk_row_norm_bwd_workspace_bytes) g_norm_bwd_bytes;
+decltype(&ixk_linear_xent_fwd) g_xent_fwd;
+decltype(&ixk_linear_xent_bwd) g_xent_bwd;
+decltype(&ixk_linear_distill_fwd) g_distill_fwd;
+decltype(&ixk_linear_distill_bwd) g_distill_bwd;
+decltype(&ixk_linear_loss_workspace_bytes) g_loss_bytes;
 
 // A plain CUDA tensor, nullptr for anything else (None included; see `optional`).
 const at::Tensor* tensor(PyObject* o) {
@@ -405,6 +413,242 @@ IXK_PY_FUNCTION(py_residual_add, 5)
 IXK_PY_END
 
 // bind(name -> address): the entry points of the library that the package has loaded
+// ------------------------------------------------------------------------------------------------ training
+
+at::Tensor like(const at::Tensor& t, at::IntArrayRef sizes, at::ScalarType type) {
+  return at::empty(sizes, at::TensorOptions().device(t.device()).dtype(type));
+}
+PyObject* wrap(const at::Tensor& t) {
+  if (!t.defined()) Py_RETURN_NONE;
+  return THPVariable_Wrap(t);
+}
+// (given or made, ...); the status where it is not OK.
+PyObject* results(int st, std::initializer_list<std::pair<PyObject*, const at::Tensor*>> items) {
+  if (st != IXK_OK) return status(st);
+  PyObject* t = PyTuple_New(static_cast<Py_ssize_t>(items.size()));
+  Py_ssize_t i = 0;
+  for (const auto& [given, made] : items) {
+    PyObject* o = given;
+    if (o != nullptr) Py_INCREF(o);
+    else o = wrap(*made);
+    if (o == nullptr) {
+      Py_DECREF(t);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(t, i++, o);
+  }
+  return t;
+}
+// _row_pitch
+bool row_pitch(const at::Tensor& t, int64_t* pitch) {
+  const int64_t d = t.dim();
+  if (d < 1) return false;
+  if (t.is_contiguous()) *pitch = t.size(d - 1);
+  else if (d == 2 && (t.stride(1) == 1 || t.size(1) == 1) && t.stride(0) >= t.size(1)) *pitch = t.stride(0);
+  else return false;
+  return true;
+}
+bool param(const at::Tensor* p, int64_t cols, const at::Tensor& x) {
+  return p == nullptr || (p->dim() == 1 && p->size(0) == cols && p->is_contiguous() && (p->scalar_type() == x.scalar_type() || p->scalar_type() == at::kFloat));
+}
+bool float_type(const at::Tensor& t, bool with_fp32) {
+  return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf || (with_fp32 && t.scalar_type() == at::kFloat);
+}
+
+// _row_norm_desc
+bool norm_desc(const at::Tensor& x, int64_t kind, const at::Tensor* gain, double offset, const at::Tensor* shift, double eps, ixk_row_norm_desc* d) {
+  if (x.dim() < 1 || x.size(x.dim() - 1) < 1 || !float_type(x, true)) return false;
+  const int64_t cols = x.size(x.dim() - 1);
+  if (!param(gain, cols, x) || !param(shift, cols, x) || (gain != nullptr && shift != nullptr && gain->scalar_type() != shift->scalar_type())) return false;
+  *d = ixk_row_norm_desc{};
+  d->dtype = dtype_of(x);
+  d->param_dtype = dtype_of(gain != nullptr ? *gain : shift != nullptr ? *shift : x);
+  d->kind = static_cast<int32_t>(kind);
+  d->eps = static_cast<float>(eps);
+  d->gain_offset = static_cast<float>(offset);
+  d->rows = x.numel() / cols;
+  d->cols = cols;
+  if (!row_pitch(x, &d->x_stride)) return false;
+  d->y_stride = d->grad_y_stride = d->dx_stride = d->x_stride;
+  return true;
+}
+
+// x, kind, eps, gain, gain_offset, shift, out, stream
+IXK_PY_FUNCTION(py_row_norm_forward, 8)
+  const at::Tensor *x = tensor(a[0]), *gain, *shift, *out;
+  int64_t kind;
+  double eps, offset;
+  void* stream;
+  ixk_row_norm_desc d;
+  if (x == nullptr || !integer(a[1], &kind) || !number(a[2], &eps) || !optional(a[3], &gain) || !number(a[4], &offset) ||
+      !optional(a[5], &shift) || !optional(a[6], &out) || !stream_arg(a[7], &stream) || (kind != IXK_NORM_LAYER && kind != IXK_NORM_RMS) ||
+      !norm_desc(*x, kind, gain, offset, shift, eps, &d))
+    Py_RETURN_NONE;
+  if (out != nullptr && (out->sizes() != x->sizes() || out->scalar_type() != x->scalar_type() || !row_pitch(*out, &d.y_stride))) Py_RETURN_NONE;
+  at::Tensor made, mean, rstd = like(*x, x->sizes().slice(0, x->dim() - 1), at::kFloat);
+  if (out == nullptr) {
+    made = like(*x, x->sizes(), x->scalar_type());
+    out = &made;
+    d.y_stride = d.cols;
+  }
+  if (kind == IXK_NORM_LAYER) mean = like(*x, x->sizes().slice(0, x->dim() - 1), at::kFloat);
+  void *px = ptr(x), *pg = ptr(gain), *ps = ptr(shift), *po = ptr(out), *pr = ptr(&rstd), *pm = mean.defined() ? ptr(&mean) : nullptr;
+  const int st = unlocked([&] { return g_norm_fwd(&d, px, pg, ps, po, static_cast<float*>(pm), static_cast<float*>(pr), stream); });
+  return results(st, {{a[6] == Py_None ? nullptr : a[6], &made}, {nullptr, &mean}, {nullptr, &rstd}});
+IXK_PY_END
+
+// grad_out, x, mean, rstd, kind, gain, gain_offset, with_shift, grad_x, workspace, stream
+IXK_PY_FUNCTION(py_row_norm_backward, 11)
+  const at::Tensor *gy = tensor(a[0]), *x = tensor(a[1]), *mean, *rstd = tensor(a[3]), *gain, *dx, *ws;
+  int64_t kind;
+  double offset;
+  void* stream;
+  ixk_row_norm_desc d;
+  if (gy == nullptr || x == nullptr || !optional(a[2], &mean) || rstd == nullptr || !integer(a[4], &kind) || !optional(a[5], &gain) ||
+      !number(a[6], &offset) || !PyBool_Check(a[7]) || !optional(a[8], &dx) || !optional(a[9], &ws) || !stream_arg(a[10], &stream) ||
+      (kind != IXK_NORM_LAYER && kind != IXK_NORM_RMS) || !norm_desc(*x, kind, gain, offset, nullptr, 0.0, &d))
+    Py_RETURN_NONE;
+  const at::IntArrayRef rows = x->sizes().slice(0, x->dim() - 1);
+  auto stats = [&](const at::Tensor* t) { return t != nullptr && t->scalar_type() == at::kFloat && t->sizes() == rows && t->is_contiguous(); };
+  if (!stats(rstd) || (kind == IXK_NORM_LAYER && !stats(mean))) Py_RETURN_NONE;
+  auto fits = [&](const at::Tensor& t, int64_t* pitch) { return t.sizes() == x->sizes() && t.scalar_type() == x->scalar_type() && row_pitch(t, pitch); };
+  if (!fits(*gy, &d.grad_y_stride) || (dx != nullptr && !fits(*dx, &d.dx_stride))) Py_RETURN_NONE;
+  const bool with_shift = a[7] == Py_True;
+  if (ws == nullptr && (gain != nullptr || with_shift) && a[10] != Py_None) Py_RETURN_NONE;   // (the twin allocates in that stream's pool)
+  at::Tensor made, dgain, dshift, scratch;
+  if (dx == nullptr) {
+    made = like(*x, x->sizes(), x->scalar_type());
+    dx = &made;
+    d.dx_stride = d.cols;
+  }
+  const at::ScalarType type = gain != nullptr ? gain->scalar_type() : x->scalar_type();
+  if (gain != nullptr) dgain = like(*x, {d.cols}, type);
+  if (with_shift) dshift = like(*x, {d.cols}, type);
+  if (ws == nullptr && (gain != nullptr || with_shift)) {
+    scratch = like(*x, {static_cast<int64_t>(g_norm_bwd_bytes(&d))}, at::kByte);
+    ws = &scratch;
+  }
+  void *pgy = ptr(gy), *px = ptr(x), *pg = ptr(gain), *pm = ptr(mean), *pr = ptr(rstd), *pdx = ptr(dx), *pw = ptr(ws);
+  void *pdg = dgain.defined() ? ptr(&dgain) : nullptr, *pds = dshift.defined() ? ptr(&dshift) : nullptr;
+  const size_t bytes = size_of(ws);
+  const int st = unlocked([&] {
+    return g_norm_bwd(&d, pgy, px, pg, static_cast<float*>(pm), static_cast<float*>(pr), pdx, pdg, pds, pw, bytes, stream);
+  });
+  return results(st, {{a[8] == Py_None ? nullptr : a[8], &made}, {nullptr, &dgain}, {nullptr, &dshift}});
+IXK_PY_END
+
+// _linear_loss_desc
+bool loss_desc(const at::Tensor& x, const at::Tensor& w, const at::Tensor* bias, const at::Tensor& index, const at::Tensor* teacher, double scale,
+               int64_t ignore, ixk_linear_loss_desc* d) {
+  if (x.dim() != 2 || w.dim() != 2 || w.size(1) != x.size(1) || !float_type(x, false) || w.scalar_type() != x.scalar_type()) return false;
+  const int64_t rows = x.size(0), hidden = x.size(1), vocab = w.size(0);
+  if (hidden > 1 && x.stride(1) != 1) return false;
+  if (bias != nullptr && (bias->scalar_type() != x.scalar_type() || bias->dim() != 1 || bias->size(0) != vocab || !bias->is_contiguous())) return false;
+  if (index.scalar_type() != at::kInt && index.scalar_type() != at::kLong) return false;
+  *d = ixk_linear_loss_desc{};
+  if (teacher == nullptr) {
+    if (index.dim() != 1 || index.size(0) != rows || !index.is_contiguous()) return false;
+  } else {
+    if (index.dim() != 2 || index.size(0) != rows || teacher->sizes() != index.sizes() || index.size(1) < 1 || index.size(1) > INT32_MAX ||
+        !float_type(*teacher, true) || !row_pitch(index, &d->index_stride) || !row_pitch(*teacher, &d->teacher_stride))
+      return false;
+    d->entries = static_cast<int32_t>(index.size(1));
+    d->teacher_dtype = dtype_of(*teacher);
+  }
+  ixk_matrix_layout l;
+  if (!layout(w, &l)) return false;
+  d->dtype = dtype_of(x);
+  d->index_bytes = index.scalar_type() == at::kLong ? 8 : 4;
+  d->scale = static_cast<float>(scale);
+  d->ignore_index = ignore;
+  d->rows = rows;
+  d->hidden = hidden;
+  d->vocab = vocab;
+  d->x_stride = rows > 1 ? x.stride(0) : std::max(x.stride(0), (hidden + 7) / 8 * 8);
+  d->w_order = d->dw_order = l.order;
+  d->w_stride = d->dw_stride = l.leading_dim_stride;
+  d->dx_stride = hidden;
+  return true;
+}
+
+// x, weight, bias, labels or index, None or teacher, scale, ignore_index, workspace, stream
+IXK_PY_FUNCTION(py_linear_loss_forward, 9)
+  const at::Tensor *x = tensor(a[0]), *w = tensor(a[1]), *bias, *index = tensor(a[3]), *teacher, *ws;
+  double scale;
+  int64_t ignore;
+  void* stream;
+  ixk_linear_loss_desc d;
+  if (x == nullptr || w == nullptr || !optional(a[2], &bias) || index == nullptr || !optional(a[4], &teacher) || !number(a[5], &scale) ||
+      !integer(a[6], &ignore) || !optional(a[7], &ws) || !stream_arg(a[8], &stream) || !loss_desc(*x, *w, bias, *index, teacher, scale, ignore, &d))
+    Py_RETURN_NONE;
+  if (ws == nullptr && a[8] != Py_None) Py_RETURN_NONE;
+  at::Tensor loss = like(*x, {d.rows}, at::kFloat), lse = like(*x, {d.rows}, at::kFloat), scratch;
+  if (ws == nullptr) {
+    scratch = like(*x, {static_cast<int64_t>(g_loss_bytes(&d, 0))}, at::kByte);
+    ws = &scratch;
+  }
+  void *px = ptr(x), *pw = ptr(w), *pb = ptr(bias), *pi = ptr(index), *pt = ptr(teacher), *pws = ptr(ws);
+  float *pl = static_cast<float*>(ptr(&loss)), *pe = static_cast<float*>(ptr(&lse));
+  const size_t bytes = size_of(ws);
+  const int st = unlocked([&] {
+    return teacher == nullptr ? g_xent_fwd(&d, px, pw, pb, pi, pl, pe, pws, bytes, stream)
+                              : g_distill_fwd(&d, px, pw, pb, pi, pt, pl, pe, pws, bytes, stream);
+  });
+  return results(st, {{nullptr, &loss}, {nullptr, &lse}});
+IXK_PY_END
+
+// x, weight, bias, labels or index, None or teacher, lse, grad_loss, scale, ignore_index, grad_x, grad_weight, weight_grad, workspace, stream
+IXK_PY_FUNCTION(py_linear_loss_backward, 14)
+  const at::Tensor *x = tensor(a[0]), *w = tensor(a[1]), *bias, *index = tensor(a[3]), *teacher, *lse = tensor(a[5]), *g = tensor(a[6]), *dx, *dw, *ws;
+  double scale;
+  int64_t ignore;
+  void* stream;
+  ixk_linear_loss_desc d;
+  if (x == nullptr || w == nullptr || !optional(a[2], &bias) || index == nullptr || !optional(a[4], &teacher) || lse == nullptr || g == nullptr ||
+      !number(a[7], &scale) || !integer(a[8], &ignore) || !optional(a[9], &dx) || !optional(a[10], &dw) || !PyBool_Check(a[11]) ||
+      !optional(a[12], &ws) || !stream_arg(a[13], &stream) || !loss_desc(*x, *w, bias, *index, teacher, scale, ignore, &d))
+    Py_RETURN_NONE;
+  if (lse->dim() != 1 || lse->size(0) != d.rows || lse->scalar_type() != at::kFloat || !lse->is_contiguous()) Py_RETURN_NONE;
+  if (g->scalar_type() != at::kFloat || g->dim() > 1 || (g->dim() == 1 && g->size(0) != d.rows)) Py_RETURN_NONE;
+  if (ws == nullptr && a[13] != Py_None) Py_RETURN_NONE;
+  d.grad_loss_stride = g->dim() == 1 ? g->stride(0) : 0;
+  if (dx != nullptr && (dx->sizes() != x->sizes() || dx->scalar_type() != x->scalar_type() || !row_pitch(*dx, &d.dx_stride))) Py_RETURN_NONE;
+  if (dw != nullptr) {
+    ixk_matrix_layout l;
+    if (dw->sizes() != w->sizes() || dw->scalar_type() != x->scalar_type() || !layout(*dw, &l)) Py_RETURN_NONE;
+    d.dw_order = l.order;
+    d.dw_stride = l.leading_dim_stride;
+  }
+  const bool weight_grad = a[11] == Py_True;
+  at::Tensor made_dx, made_dw, dbias, scratch;
+  if (dx == nullptr) {
+    made_dx = like(*x, {d.rows, d.hidden}, x->scalar_type());
+    dx = &made_dx;
+  }
+  if (dw == nullptr && weight_grad) {
+    made_dw = d.w_order == IXK_ROW_MAJOR ? like(*x, {d.vocab, d.hidden}, x->scalar_type()) : like(*x, {d.hidden, d.vocab}, x->scalar_type()).t();
+    dw = &made_dw;
+    ixk_matrix_layout l;
+    if (!layout(made_dw, &l)) Py_RETURN_NONE;
+    d.dw_order = l.order;
+    d.dw_stride = l.leading_dim_stride;
+  }
+  if (bias != nullptr && weight_grad) dbias = like(*x, {d.vocab}, x->scalar_type());
+  if (ws == nullptr) {
+    scratch = like(*x, {static_cast<int64_t>(g_loss_bytes(&d, 1))}, at::kByte);
+    ws = &scratch;
+  }
+  void *px = ptr(x), *pw = ptr(w), *pb = ptr(bias), *pi = ptr(index), *pt = ptr(teacher), *pws = ptr(ws), *pdx = ptr(dx), *pdw = ptr(dw);
+  void* pdb = dbias.defined() ? ptr(&dbias) : nullptr;
+  const float *pe = static_cast<const float*>(ptr(lse)), *pg = static_cast<const float*>(ptr(g));
+  const size_t bytes = size_of(ws);
+  const int st = unlocked([&] {
+    return teacher == nullptr ? g_xent_bwd(&d, px, pw, pb, pi, pe, pg, pdx, pdw, pdb, pws, bytes, stream)
+                              : g_distill_bwd(&d, px, pw, pb, pi, pt, pe, pg, pdx, pdw, pdb, pws, bytes, stream);
+  });
+  return results(st, {{a[9] == Py_None ? nullptr : a[9], &made_dx}, {a[10] == Py_None ? nullptr : a[10], &made_dw}, {nullptr, &dbias}});
+IXK_PY_END
+
 PyObject* py_bind(PyObject*, PyObject* table) {
   struct Entry {
     const char* name;
@@ -425,6 +669,14 @@ PyObject* py_bind(PyObject*, PyObject* table) {
       {"ixk_rotary_half", reinterpret_cast<void**>(&g_rotary_half)},
       {"ixk_kv_append", reinterpret_cast<void**>(&g_kv_append)},
       {"ixk_residual_add", reinterpret_cast<void**>(&g_residual_add)},
+      {"ixk_row_norm_fwd", reinterpret_cast<void**>(&g_norm_fwd)},
+      {"ixk_row_norm_bwd", reinterpret_cast<void**>(&g_norm_bwd)},
+      {"ixk_row_norm_bwd_workspace_bytes", reinterpret_cast<void**>(&g_norm_bwd_bytes)},
+      {"ixk_linear_xent_fwd", reinterpret_cast<void**>(&g_xent_fwd)},
+      {"ixk_linear_xent_bwd", reinterpret_cast<void**>(&g_xent_bwd)},
+      {"ixk_linear_distill_fwd", reinterpret_cast<void**>(&g_distill_fwd)},
+      {"ixk_linear_distill_bwd", reinterpret_cast<void**>(&g_distill_bwd)},
+      {"ixk_linear_loss_workspace_bytes", reinterpret_cast<void**>(&g_loss_bytes)},
   };
   for (const Entry& e : entries) {
     PyObject* address = PyDict_GetItemString(table, e.name);   // borrowed
@@ -449,6 +701,10 @@ PyMethodDef methods[] = {
     IXK_METHOD("rotary", py_rotary),
     IXK_METHOD("kv_append", py_kv_append),
     IXK_METHOD("residual_add", py_residual_add),
+    IXK_METHOD("row_norm_forward", py_row_norm_forward),
+    IXK_METHOD("row_norm_backward", py_row_norm_backward),
+    IXK_METHOD("linear_loss_forward", py_linear_loss_forward),
+    IXK_METHOD("linear_loss_backward", py_linear_loss_backward),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "ixk_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
