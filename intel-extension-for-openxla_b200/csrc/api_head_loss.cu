@@ -31,6 +31,7 @@ constexpr size_t kPieceBytes = size_t(256) << 20;  // of G
 constexpr size_t kSplitBytes = size_t(64) << 20;   // of the GEMMs' K chunks, for few rows
 constexpr size_t kPlaneBytes = size_t(128) << 20;  // of dx's planes, for more
 constexpr int kMaxPlanes = 16;
+constexpr int64_t kPitchUnit = 64;               // rows of whole 128-byte lines: a box that straddles lines reads one more of each
 constexpr int kSlabRows = 64;                    // rows that the product along the rows reads at a time
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -162,6 +163,7 @@ struct Gather {
 };
 
 constexpr int kGatherThreads = 256;
+constexpr int kCopyVecs = 8;
 
 __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Gather a) {
   __shared__ int warp_count[kGatherThreads / 32];
@@ -180,13 +182,14 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Gather a) 
     for (int w = 0; w < kGatherThreads / 32; ++w) t += warp_count[w];
     return t;
   };
-  // every CTA counts the rows in front of its own
-  int before = 0;
-  for (int i = threadIdx.x; i < first; i += kGatherThreads) before += a.has(i);
-  before = block_sum(before);
   const int row = first + threadIdx.x;
   const bool mine = static_cast<int>(threadIdx.x) < a.rows_per_cta && row < end;
   const bool keep = mine && a.has(row);
+  // every CTA counts the rows in front of its own
+  int before = 0;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < first; i += kGatherThreads) before += a.has(i);
+  before = block_sum(before);
   const unsigned ballot = __ballot_sync(0xffffffffu, keep);
   const int here = block_sum(lane == 0 ? __popc(ballot) : 0);
   if (mine) {
@@ -206,7 +209,15 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Gather a) 
   for (int i = warp; i < here; i += kGatherThreads / 32) {
     const uint16_t* src = a.x + source[i] * a.ldx;
     uint16_t* dst = a.packed + (before + i) * a.ldp;
-    for (int v = lane; v < whole; v += 32) reinterpret_cast<uint4*>(dst)[v] = reinterpret_cast<const uint4*>(src)[v];
+    for (int v0 = lane; v0 < whole; v0 += 32 * kCopyVecs) {
+      uint4 w[kCopyVecs];      // (all loads out before the first store)
+#pragma unroll
+      for (int j = 0; j < kCopyVecs; ++j)
+        if (v0 + 32 * j < whole) w[j] = reinterpret_cast<const uint4*>(src)[v0 + 32 * j];
+#pragma unroll
+      for (int j = 0; j < kCopyVecs; ++j)
+        if (v0 + 32 * j < whole) reinterpret_cast<uint4*>(dst)[v0 + 32 * j] = w[j];
+    }
     for (int c = whole * 8 + lane; c < a.hidden; c += 32) dst[c] = src[c];
   }
   if (end != a.rows) return;
@@ -422,7 +433,7 @@ Layout layout_for(const ixk_linear_loss_desc& d, bool backward) {
     l.weight = l.space.take(4 * N * K);
     l.has = l.space.take(4 * N);
   }
-  l.ldp = round_up(D, 8);
+  l.ldp = round_up(D, kPitchUnit);
   if (l.gathered) l.packed = l.space.take(2 * N * l.ldp);
   if (!backward) {
     l.at_target = l.space.take(4 * N * K);
@@ -435,9 +446,9 @@ Layout layout_for(const ixk_linear_loss_desc& d, bool backward) {
   const int64_t rows = round_up(N, 256), most = std::max<int64_t>(kPieceBytes / (2 * rows) / kPieceUnit * kPieceUnit, kPieceUnit);
   const int64_t pieces = (V + most - 1) / most;
   l.piece = std::min(round_up((V + pieces - 1) / pieces, kPieceUnit), round_up(V, 8));
-  l.ldg = round_up(l.piece, 8);
+  l.ldg = round_up(l.piece, kPitchUnit);
   l.grad = l.space.take(2 * rows * l.ldg);
-  l.ld_acc = round_up(D, 4);
+  l.ld_acc = round_up(D, kPitchUnit / 2);
   if (N > kDirectRows) {
     l.plane = N * l.ld_acc;
     l.planes = static_cast<int>(std::clamp<int64_t>(kPlaneBytes / (4 * l.plane), 1, kMaxPlanes));
@@ -547,8 +558,8 @@ int gather(const ixk_linear_loss_desc& d, const Layout& l, char* ws, const HasTa
   g.ldp = l.ldp;
   g.rows = static_cast<int>(d.rows);
   g.hidden = static_cast<int>(d.hidden);
-  // (each CTA counts the rows in front of it: at most 512 CTAs while a CTA's rows fit its threads)
-  g.rows_per_cta = static_cast<int>(std::min<int64_t>(std::max<int64_t>(16, (d.rows + 511) / 512), kGatherThreads));
+  // (each CTA counts the rows in front of it: at most 1024 CTAs while a CTA's rows fit its threads)
+  g.rows_per_cta = static_cast<int>(std::min<int64_t>(std::max<int64_t>(8, (d.rows + 1023) / 1024), kGatherThreads));
   g.control = reinterpret_cast<Control*>(ws + l.control);
   g.row_map = reinterpret_cast<int*>(ws + l.row_map);
   g.inverse = backward ? reinterpret_cast<int*>(ws + l.inverse) : nullptr;
