@@ -55,12 +55,13 @@ __device__ __forceinline__ float load_as_float(const void* p, int64_t i, int dty
   return __half2float(static_cast<const __half*>(p)[i]);
 }
 
-constexpr int kListWarps = 4, kListPer = kMaxEntries / 32;
+constexpr int kListWarps = 4;
 
 // One warp per row: softmax over the entries that are there (index inside the vocabulary, logit above -inf), and their
-// ranks by index, ties by position, as their places in the list.
+// ranks by index, ties by position, as their places in the list.  kListPer entries a lane.
+template <int kListPer>
 __global__ void __launch_bounds__(32 * kListWarps) lists_kernel(const Lists a) {
-  __shared__ int columns[kListWarps][kMaxEntries];
+  __shared__ int columns[kListWarps][32 * kListPer];
   ptx::grid_dependency_sync();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * kListWarps + warp; row < a.rows; row += static_cast<int64_t>(gridDim.x) * kListWarps) {
@@ -330,10 +331,12 @@ __device__ __forceinline__ uint32_t to16(float f) {
   else return __half_as_ushort(__float2half_rn(f));
 }
 
-// dbias of a piece: the sums of G's columns.  256 columns per CTA, 32 warps that take rows in turn.
-constexpr int kBiasCols = 256, kBiasGroups = 32;
+// dbias of a piece: the sums of G's columns.  256 columns per CTA, 32 warps that take rows in turn; where the columns alone
+// leave SMs idle the rows are dealt out to gridDim.y CTAs, which leave partial sums for bias_sum_kernel.
+constexpr int kBiasCols = 256, kBiasGroups = 32, kBiasParts = 32;
 template <bool kBf16>
-__global__ void __launch_bounds__(32 * kBiasGroups) bias_kernel(const uint16_t* g, int64_t ldg, const Control* control, int count, uint16_t* out) {
+__global__ void __launch_bounds__(32 * kBiasGroups) bias_kernel(const uint16_t* g, int64_t ldg, const Control* control, int count, float* partial,
+                                                              uint16_t* out) {
   __shared__ float sums[kBiasGroups][kBiasCols];
   ptx::grid_dependency_sync();
   const int group = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = control->active;
@@ -342,7 +345,7 @@ __global__ void __launch_bounds__(32 * kBiasGroups) bias_kernel(const uint16_t* 
   if (c0 < count) {      // (G's pitch is whole vectors)
     const uint16_t* p = g + c0;
 #pragma unroll 4
-    for (int row = group; row < rows; row += kBiasGroups) {
+    for (int row = blockIdx.y * kBiasGroups + group; row < rows; row += gridDim.y * kBiasGroups) {
       const uint4 w = *reinterpret_cast<const uint4*>(p + row * ldg);
       const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -359,18 +362,29 @@ __global__ void __launch_bounds__(32 * kBiasGroups) bias_kernel(const uint16_t* 
   if (threadIdx.x < kBiasCols && c < count) {
     float s = 0.0f;
     for (int i = 0; i < kBiasGroups; ++i) s += sums[i][threadIdx.x];
-    out[c] = static_cast<uint16_t>(to16<kBf16>(kBf16 ? s : s * control->range[1]));
+    if (gridDim.y > 1) partial[static_cast<int64_t>(blockIdx.y) * count + c] = s;
+    else out[c] = static_cast<uint16_t>(to16<kBf16>(kBf16 ? s : s * control->range[1]));
   }
+}
+template <bool kBf16>
+__global__ void __launch_bounds__(128) bias_sum_kernel(const float* partial, int parts, const Control* control, int count, uint16_t* out) {
+  ptx::grid_dependency_sync();
+  const int c = blockIdx.x * 128 + threadIdx.x;
+  if (c >= count) return;
+  float s = 0.0f;
+#pragma unroll 8
+  for (int i = 0; i < parts; ++i) s += partial[static_cast<int64_t>(i) * count + c];
+  out[c] = static_cast<uint16_t>(to16<kBf16>(kBf16 ? s : s * control->range[1]));
 }
 
 // dx: the accumulator's rows, their planes added up, back to where they came from, rounded once; zeros where there was no
 // target.
 template <bool kBf16>
-__global__ void __launch_bounds__(256) scatter_kernel(const float* acc, int64_t ld_acc, int64_t plane, const int* inverse, const Control* control,
+__global__ void __launch_bounds__(256) scatter_kernel(const float* acc, int64_t ld_acc, int64_t plane, int known_planes, const int* inverse, const Control* control,
                                                       int hidden, int vec, uint16_t* dx, int64_t ld) {
   ptx::grid_dependency_sync();
   const int64_t row = blockIdx.x;
-  const int from = inverse[row], planes = plane > 0 ? control->planes : 1;
+  const int from = inverse[row], planes = known_planes > 0 ? known_planes : control->planes;
   const float scale = kBf16 ? 1.0f : control->range[1];
   const float* src = acc + from * ld_acc;
   uint16_t* dst = dx + row * ld;
@@ -416,11 +430,17 @@ struct Space {
 struct Layout {
   Space space;
   size_t control, row_map, column, weight, has, packed, at_target, partial;      // forward
-  size_t inverse, grad, acc, split, split_bytes;                               // backward
+  size_t inverse, grad, bias, acc, split, split_bytes;                               // backward
   int64_t ldp, slots, piece, ldg, ld_acc, plane;      // plane 0: dx is not cut into planes
   int planes;
   bool gathered;
 };
+
+// CTAs along the rows for the sums of a piece's columns: as many as give the SMs one each, with four rows a warp or more.
+int64_t bias_parts(int64_t columns, int64_t rows) {
+  const int64_t blocks = (columns + kBiasCols - 1) / kBiasCols;
+  return std::clamp<int64_t>(std::min<int64_t>(148 / blocks, rows / (4 * kBiasGroups)), 1, kBiasParts);
+}
 
 Layout layout_for(const ixk_linear_loss_desc& d, bool backward) {
   Layout l{};
@@ -448,14 +468,20 @@ Layout layout_for(const ixk_linear_loss_desc& d, bool backward) {
   l.piece = std::min(round_up((V + pieces - 1) / pieces, kPieceUnit), round_up(V, 8));
   l.ldg = round_up(l.piece, kPitchUnit);
   l.grad = l.space.take(2 * rows * l.ldg);
+  l.bias = l.space.take(4 * bias_parts(std::min(l.piece, V), N) * l.piece);
   l.ld_acc = round_up(D, kPitchUnit / 2);
   if (N > kDirectRows) {
     l.plane = N * l.ld_acc;
     l.planes = static_cast<int>(std::clamp<int64_t>(kPlaneBytes / (4 * l.plane), 1, kMaxPlanes));
     l.acc = l.space.take(4 * l.plane * l.planes);
+  } else if (pieces == 1) {      // (planes of the kernel for few rows: dense)
+    l.ld_acc = D;
+    l.plane = N * D;
+    l.planes = gemm::stream_splits(N, D, V, 2, kSplitBytes);
+    l.acc = l.space.take(4 * l.plane * l.planes);
   } else {
     l.acc = l.space.take(4 * N * l.ld_acc);
-    l.split_bytes = std::min(std::max(gemm::problem_workspace_bytes(N, D, l.piece), gemm::problem_workspace_bytes(l.piece, D, N)), kSplitBytes);
+    l.split_bytes = std::min(gemm::problem_workspace_bytes(N, D, l.piece), kSplitBytes);
     l.split = l.space.take(l.split_bytes);
   }
   return l;
@@ -544,7 +570,8 @@ int targets_of(const ixk_linear_loss_desc& d, const Layout& l, char* ws, const v
   t->weight = a.weight = reinterpret_cast<float*>(ws + l.weight);
   has->has = a.has = reinterpret_cast<int*>(ws + l.has);
   const int64_t ctas = std::min<int64_t>((d.rows + kListWarps - 1) / kListWarps, 148 * 16);
-  return launch_overlapped(lists_kernel, dim3(static_cast<unsigned>(ctas)), dim3(32 * kListWarps), 0, stream, a);
+  auto* fn = d.entries <= 32 ? lists_kernel<1> : d.entries <= 64 ? lists_kernel<2> : d.entries <= 128 ? lists_kernel<4> : lists_kernel<8>;
+  return launch_overlapped(fn, dim3(static_cast<unsigned>(ctas)), dim3(32 * kListWarps), 0, stream, a);
 }
 
 int gather(const ixk_linear_loss_desc& d, const Layout& l, char* ws, const HasTarget& has, const void* x, float* loss, float* lse,
@@ -569,7 +596,7 @@ int gather(const ixk_linear_loss_desc& d, const Layout& l, char* ws, const HasTa
   g.grad_stride = d.grad_loss_stride;
   g.factor = factor;
   g.ranged = backward && d.dtype == IXK_F16;
-  if (backward && l.plane > 0) {
+  if (backward && d.rows > kDirectRows) {
     g.dx_tiles_n = static_cast<int>((d.hidden + gemm::kTwoTile - 1) / gemm::kTwoTile);
     g.piece_slabs = static_cast<int>((l.piece + kSlabRows - 1) / kSlabRows);
     g.dw_tiles = want_dw ? g.dx_tiles_n * static_cast<int>((l.piece + gemm::kTwoTile - 1) / gemm::kTwoTile) : 0;
@@ -739,27 +766,33 @@ int backward(const char* name, const ixk_linear_loss_desc* d, bool distill, cons
       g.out_dtype = d->dtype;
       g.acc_scale_dev = p.range != nullptr ? p.range + 1 : nullptr;
     }
-    if (l.plane > 0) {
-      both[0].m_limit = both[0].M > 0 ? p.active_rows : nullptr;
-      both[1].k_limit = both[1].M > 0 ? p.active_rows : nullptr;
-      if ((rc = gemm::launch_two(both, &control->plane_slabs, dev, s)) != IXK_OK) return rc;
-    } else {      // (one row block: both are streams of weights; G's rows and x's behind the active ones are zeros)
-      for (const gemm::Problem& g : both)
-        if (g.M > 0 && (rc = gemm::run_problem(g, ws + l.split, l.split_bytes, dev, s)) != IXK_OK) return rc;
+    if (both[1].M > 0) both[1].k_limit = p.active_rows;
+    if (d->rows <= kDirectRows && both[0].M > 0) {      // one row block: dx is a stream of the weights
+      const gemm::Problem& g = both[0];
+      rc = l.plane == 0 ? gemm::run_problem(g, ws + l.split, l.split_bytes, dev, s)
+                        : gemm::launch_stream(g, l.planes, l.planes > 1 ? acc : nullptr, dev, s);
+      if (rc != IXK_OK) return rc;
+      both[0].M = 0;
     }
+    if (both[0].M > 0) both[0].m_limit = p.active_rows;
+    if ((rc = gemm::launch_two(both, &control->plane_slabs, dev, s)) != IXK_OK) return rc;
     if (dbias != nullptr) {
-      auto* fn = bf16 ? bias_kernel<true> : bias_kernel<false>;
-      rc = launch_overlapped(fn, dim3(static_cast<unsigned>((p.count + kBiasCols - 1) / kBiasCols)), dim3(32 * kBiasGroups), 0, s,
-                             static_cast<const uint16_t*>(p.grad), l.ldg, control, static_cast<int>(p.count),
-                             static_cast<uint16_t*>(dbias) + first);
+      const unsigned blocks = static_cast<unsigned>((p.count + kBiasCols - 1) / kBiasCols), parts = static_cast<unsigned>(bias_parts(p.count, d->rows));
+      float* partial = reinterpret_cast<float*>(ws + l.bias);
+      auto* out = static_cast<uint16_t*>(dbias) + first;
+      rc = launch_overlapped(bf16 ? bias_kernel<true> : bias_kernel<false>, dim3(blocks, parts), dim3(32 * kBiasGroups), 0, s,
+                             static_cast<const uint16_t*>(p.grad), l.ldg, control, static_cast<int>(p.count), partial, out);
+      if (rc == IXK_OK && parts > 1)
+        rc = launch_overlapped(bf16 ? bias_sum_kernel<true> : bias_sum_kernel<false>, dim3(static_cast<unsigned>((p.count + 127) / 128)), dim3(128), 0, s,
+                               static_cast<const float*>(partial), static_cast<int>(parts), control, static_cast<int>(p.count), out);
       if (rc != IXK_OK) return rc;
     }
   }
   if (dx == nullptr) return IXK_OK;
-  const int vec = aligned(dx, 16) && d->dx_stride % 8 == 0;
+  const int vec = aligned(dx, 16) && d->dx_stride % 8 == 0 && l.ld_acc % 4 == 0;
   auto* fn = bf16 ? scatter_kernel<true> : scatter_kernel<false>;
   return launch_overlapped(fn, dim3(static_cast<unsigned>(d->rows)), dim3(256), 0, s, static_cast<const float*>(acc), l.ld_acc, l.plane,
-                           reinterpret_cast<const int*>(ws + l.inverse), control, static_cast<int>(d->hidden), vec, static_cast<uint16_t*>(dx),
+                           d->rows > kDirectRows ? 0 : std::max(l.planes, 1), reinterpret_cast<const int*>(ws + l.inverse), control, static_cast<int>(d->hidden), vec, static_cast<uint16_t*>(dx),
                            d->dx_stride);
 }
 

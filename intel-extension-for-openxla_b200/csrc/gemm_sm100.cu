@@ -195,9 +195,10 @@ __device__ __forceinline__ void tile_coords(int t, int tiles_m, int tiles_n, int
 
 // One tile's epilogue for the calling warp (TMEM lanes [32 quarter, 32 quarter + 32) of the
 // accumulator at tmem_acc, `width` columns that start at column n_first of D): scale, bias, residual, activation, one rounding, store.
-template <int kBlockN>
+// `boxes`: the warp's kBoxes staging boxes.
+template <int kBlockN, int kBoxes = 2>
 __device__ __forceinline__ void epilogue_tile(const KernelArgs& args, const CUtensorMap* tmap_d_ptr, uint32_t tmem_acc,
-                                              uint32_t stage_smem, int bz, int bm, int n_first, int quarter, int lane,
+                                              uint32_t boxes, int bz, int bm, int n_first, int quarter, int lane,
                                               uint32_t& n_store, int width = kBlockN, int d_row_shift = 0) {
   const CUtensorMap& tmap_d = *tmap_d_ptr;
   if (bm * kBlockM >= args.M) return;  // a CTA pair's second half past the last row block
@@ -276,8 +277,8 @@ __device__ __forceinline__ void epilogue_tile(const KernelArgs& args, const CUte
           }
         }
         if (plain) break;   // (the row's last box)
-        const uint32_t box = stage_smem + static_cast<uint32_t>((quarter * 2 + (n_store & 1)) * 4096);
-        if (lane == 0) ptx::bulk_wait_group_read<1>();
+        const uint32_t box = boxes + static_cast<uint32_t>(n_store % kBoxes * 4096);
+        if (lane == 0) ptx::bulk_wait_group_read<kBoxes - 1>();
         __syncwarp();
 #pragma unroll
         for (int g = 0; g < 8; ++g) {
@@ -479,8 +480,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
       tile_coords(t, args.tiles_m, args.tiles_n, bz, bm, bn);
       if (!ptx::mbar_wait(acc_full_bar(buf), acc_phase, ctl, kSiteEpilogue)) break;
       ptx::tc_fence_after_sync();
-      epilogue_tile<kBlockN>(args, &tmap_d, tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * kBlockN, stage_smem,
-                             bz, bm, bn * kBlockN, quarter, lane, n_store);
+      epilogue_tile<kBlockN>(args, &tmap_d, tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * kBlockN,
+                             stage_smem + quarter * 8192, bz, bm, bn * kBlockN, quarter, lane, n_store);
       ptx::tc_fence_before_sync();
       ptx::mbar_arrive(acc_empty_bar(buf));
       buf ^= 1;
@@ -726,7 +727,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
       // scattered output: this row block's destination and the row that destination starts at
       const int dest = kDests > 1 ? (bm * kBlockM) / args.scatter_rows : 0;
       epilogue_tile<kBlockN>(args, &tmaps_d.m[dest], tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * kBlockN,
-                             stage_smem, unit.bz, bm, unit.n_first, quarter, lane, n_store, unit.width,
+                             stage_smem + quarter * 8192, unit.bz, bm, unit.n_first, quarter, lane, n_store, unit.width,
                              kDests > 1 ? dest * args.scatter_rows : 0);
       ptx::tc_fence_before_sync();
       if (rank == 0) {
@@ -763,13 +764,15 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
 // pair i takes units i, i + pairs, ... of the long product (planes x tiles, all tiles of a plane side by side, so that pairs
 // walk K together and share slabs in L2), then tiles of the other, in an order that a round of all pairs at work at the time
 // takes neighbouring tiles: the pairs with one long unit less run `ahead` rounds among themselves first.
+constexpr int kTwoEpilogueWarps = 8, kTwoThreads = 32 * (2 + kTwoEpilogueWarps);
+static_assert(kTwoEpilogueWarps * 4096 <= PairCfg::kStagingBytes, "staging boxes");
 struct TwoArgs {
   KernelArgs p[2];
   const int* plan;
   int pairs;
 };
 
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kTwoThreads, 1)
 gemm_two_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_constant__ CUtensorMap tmap_b0,
                 const __grid_constant__ CUtensorMap tmap_a1, const __grid_constant__ CUtensorMap tmap_b1,
                 const __grid_constant__ CUtensorMap tmap_d1, const __grid_constant__ TwoArgs args) {
@@ -805,7 +808,7 @@ gemm_two_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_consta
     }
     for (int b = 0; b < 2; ++b) {
       ptx::mbar_init(acc_full_bar(b), 1);
-      ptx::mbar_init(acc_empty_bar(b), 256);
+      ptx::mbar_init(acc_empty_bar(b), 2 * 32 * kTwoEpilogueWarps);
     }
     ptx::fence_mbar_init();
     ptx::prefetch_tmap(&tmap_a0);
@@ -834,7 +837,7 @@ gemm_two_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_consta
   const int end_kb1 = p1.k_limit != nullptr ? min((*p1.k_limit + kSlabElems - 1) / kSlabElems, num_kb1) : num_kb1;
   const int tiles_m0 = (rows0 + 2 * kBlockM - 1) / (2 * kBlockM), tiles0 = tiles_m0 * p0.tiles_n;
   const int tiles_m1 = (p1.tiles_m + 1) / 2, tiles1 = tiles_m1 * p1.tiles_n;
-  const int plane_slabs = *args.plan, units0 = tiles0 * ((num_kb0 + plane_slabs - 1) / plane_slabs);
+  const int plane_slabs = tiles0 > 0 ? *args.plan : 1, units0 = tiles0 * ((num_kb0 + plane_slabs - 1) / plane_slabs);
   // (a tile of few slabs costs about two more for its results)
   const int heavy = units0 % pairs, light = pairs - heavy;
   const int ahead = heavy > 0 ? (plane_slabs + max(end_kb1, 1) / 2) / (max(end_kb1, 1) + 2) : 0;
@@ -949,7 +952,9 @@ gemm_two_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_consta
     }
   } else if (warp >= 2) {
     // ------------------------------------------------------------ epilogue (each CTA: its 128 rows)
-    const int quarter = warp & 3;
+    // (two warps per 32 rows, half of the columns each, one box each: with four warps a tile of K up to 600 waited for them)
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t box = stage_smem + (warp - 2) * 4096;
     int buf = 0;
     uint32_t acc_phase = 0;
     uint32_t n_store = 0;
@@ -957,8 +962,9 @@ gemm_two_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_consta
     for (int i = 0; unit_at(i, x); ++i) {
       if (!ptx::mbar_wait(acc_full_bar(buf), acc_phase, ctl, kSiteEpilogue)) break;
       ptx::tc_fence_after_sync();
-      epilogue_tile<kBlockN>(args.p[x.which], &tmap_d1, tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * kBlockN, stage_smem,
-                             x.bz, x.bm2 * 2 + static_cast<int>(rank), x.bn * kBlockN, quarter, lane, n_store);
+      epilogue_tile<kBlockN, 1>(args.p[x.which], &tmap_d1, tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * kBlockN + half * (kBlockN / 2),
+                                box, x.bz, x.bm2 * 2 + static_cast<int>(rank), x.bn * kBlockN + half * (kBlockN / 2), quarter, lane, n_store,
+                                kBlockN / 2);
       ptx::tc_fence_before_sync();
       if (rank == 0) ptx::mbar_arrive(acc_empty_bar(buf));
       else ptx::mbar_arrive_cluster_tmem(acc_empty_bar(buf), 0);
@@ -1302,7 +1308,7 @@ int launch_two(const Problem (&p)[2], const int* plan, const DeviceInfo& dev, cu
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * args.pairs);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kTwoThreads);
   cfg.dynamicSmemBytes = PairCfg::kSmemBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];

@@ -38,7 +38,7 @@ constexpr int kEpilogueWarps = 8;
 constexpr int kThreads = 32 * (2 + kEpilogueWarps);
 constexpr int kTmemCols = 2 * kMaxTileN;
 constexpr int kRingBytes = 192 * 1024;
-constexpr int kMaxStages = 16;
+constexpr int kMaxStages = 32;
 constexpr int kBoxBytes = 32 * 128;                       // a warp's 32 rows x 64 16-bit (or 32 fp32) columns
 constexpr int kBarrierBytes = 8 * (2 * kMaxStages + 4) + 8;
 constexpr int kSmemBytes = kRingBytes + kEpilogueWarps * kBoxBytes + kBarrierBytes + 1024;
@@ -135,14 +135,15 @@ __device__ __forceinline__ void box_write(uint32_t addr, float f) {
 // A row's walk through its targets in ascending order.
 struct Walk {
   const int* column;
-  int entries, at, next;     // next: the column of target `at`
+  int entries, at, next, after;     // the columns of targets `at` and at + 1 (asked for a step ahead of its use)
   __device__ __forceinline__ void step() {
     ++at;
-    next = at < entries ? column[at] : kNoColumn;
+    next = after;
+    after = at + 1 < entries ? column[at + 1] : kNoColumn;
   }
 };
 __device__ __forceinline__ Walk start_walk(const Targets& t, int64_t row, bool active, int from) {
-  Walk w{nullptr, 1, 0, kNoColumn};
+  Walk w{nullptr, 1, 0, kNoColumn, kNoColumn};
   if (!active) return w;
   if (t.labels != nullptr) {
     const int64_t label = t.wide ? static_cast<const int64_t*>(t.labels)[row] : static_cast<const int*>(t.labels)[row];
@@ -158,8 +159,9 @@ __device__ __forceinline__ Walk start_walk(const Targets& t, int64_t row, bool a
     if (w.column[mid] < from) lo = mid + 1;
     else hi = mid;
   }
-  w.at = lo - 1;
-  w.step();
+  w.at = lo;
+  w.next = lo < t.entries ? w.column[lo] : kNoColumn;
+  w.after = lo + 1 < t.entries ? w.column[lo + 1] : kNoColumn;
   return w;
 }
 
