@@ -33,7 +33,7 @@ constexpr size_t kPlaneBytes = size_t(128) << 20;  // of dx's planes, for more
 constexpr int kMaxPlanes = 16;
 constexpr int64_t kPitchUnit = 64;               // rows of whole 128-byte lines: a box that straddles lines reads one more of each
 constexpr int kSlabRows = 64;                    // rows that the product along the rows reads at a time
-constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kLn2 = 0.6931471805599453f, kLog2E = 1.4426950408889634f;
 
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
@@ -46,6 +46,8 @@ struct Lists {
   float inv_temperature;
   int* column;       // [rows][entries] ascending
   float* weight;
+  uint16_t* start;   // [rows][starts]: the first entry at or behind column i * kStartUnit
+  int starts;
   int* has;          // [rows]: any entry
 };
 
@@ -61,7 +63,7 @@ constexpr int kListWarps = 4;
 // ranks by index, ties by position, as their places in the list.  kListPer entries a lane.
 template <int kListPer>
 __global__ void __launch_bounds__(32 * kListWarps) lists_kernel(const Lists a) {
-  __shared__ int columns[kListWarps][32 * kListPer];
+  __shared__ int columns[kListWarps][32 * kListPer], sorted[kListWarps][32 * kListPer];
   ptx::grid_dependency_sync();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * kListWarps + warp; row < a.rows; row += static_cast<int64_t>(gridDim.x) * kListWarps) {
@@ -114,10 +116,18 @@ __global__ void __launch_bounds__(32 * kListWarps) lists_kernel(const Lists a) {
     for (int e = 0; e < kListPer; ++e) {
       if (lane + 32 * e < a.entries) {
         a.column[row * a.entries + rank[e]] = col[e];
+        sorted[warp][rank[e]] = col[e];
         a.weight[row * a.entries + rank[e]] = col[e] != kNoColumn ? t[e] / sum : 0.0f;
       }
     }
     if (lane == 0) a.has[row] = any ? 1 : 0;
+    __syncwarp();
+    // entry k is the first of the units behind the one before it, up to its own; behind the last entry there is none
+    for (int k = lane; k <= a.entries; k += 32) {
+      const int from = k == 0 ? 0 : min(sorted[warp][k - 1] / kStartUnit + 1, a.starts);
+      const int to = k == a.entries ? a.starts : min(sorted[warp][k] / kStartUnit + 1, a.starts);
+      for (int i = from; i < to; ++i) a.start[row * a.starts + i] = static_cast<uint16_t>(k);
+    }
     __syncwarp();
   }
 }
@@ -133,6 +143,9 @@ struct HasTarget {
     if (labels == nullptr) return has[row] != 0;
     const int64_t l = wide ? static_cast<const int64_t*>(labels)[row] : static_cast<const int*>(labels)[row];
     return l != ignore_index && l >= 0 && l < vocab;
+  }
+  __device__ __forceinline__ int label(int64_t row) const {      // of a row that has one
+    return wide ? static_cast<int>(static_cast<const int64_t*>(labels)[row]) : static_cast<const int*>(labels)[row];
   }
 };
 
@@ -152,10 +165,11 @@ struct Gather {
   int64_t ldx, ldp;
   int rows, hidden, rows_per_cta;
   Control* control;
-  int *row_map, *inverse;      // inverse may be nullptr
+  RowInfo* info;
+  int* inverse;                // may be nullptr
   float *loss, *lse;           // zeroed where there is no target; may be nullptr
   // backward: control's range is the power of two that brings the largest row's gradient to 2^13 .. 2^14
-  const float* grad_loss;
+  const float *lse_in, *grad_loss;
   int64_t grad_stride;
   float factor;
   int ranged;
@@ -198,7 +212,13 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Gather a) 
     for (int w = 0; w < warp; ++w) at += warp_count[w];
     if (keep) {
       source[at] = row;
-      a.row_map[before + at] = row;
+      RowInfo info{row, kNoColumn, 0.0f, 0.0f};
+      if (a.has.labels != nullptr) info.label = a.has.label(row);
+      if (a.grad_loss != nullptr) {
+        info.lse2 = a.lse_in[row] * kLog2E;
+        info.coef = a.grad_loss[row * a.grad_stride] * a.factor;
+      }
+      a.info[before + at] = info;
     } else if (a.loss != nullptr) {
       a.loss[row] = 0.0f;
       a.lse[row] = 0.0f;
@@ -261,7 +281,8 @@ struct Loss {
   const float2* partial;       // [slots][rows]
   const float* at_target;      // [batch rows][entries]
   const float* weight;         // [batch rows][entries]; nullptr: one label of weight 1
-  const int *active, *row_map; // nullptr: all rows, in place
+  const int* active;           // nullptr: all rows, in place
+  const RowInfo* info;
   int rows, slots, entries;
   float factor;
   float *loss, *lse;
@@ -279,7 +300,7 @@ __global__ void __launch_bounds__(kLossThreads) loss_kernel(const Loss a) {
   const int r = threadIdx.x % kRows, part = threadIdx.x / kRows;
   const int row = blockIdx.x * kRows + r;
   const bool there = row < (a.active != nullptr ? *a.active : a.rows);
-  const int64_t orig = !there ? 0 : a.row_map != nullptr ? a.row_map[row] : row;
+  const int64_t orig = !there ? 0 : a.info != nullptr ? a.info[row].row : row;
   auto join = [](float2 p, float2 q) {
     const float top = fmaxf(p.x, q.x);
     return make_float2(top, p.y * exp2f(p.x - top) + q.y * exp2f(q.x - top));
@@ -429,7 +450,7 @@ struct Space {
 
 struct Layout {
   Space space;
-  size_t control, row_map, column, weight, has, packed, at_target, partial;      // forward
+  size_t control, info, column, weight, start, has, packed, at_target, partial;      // forward
   size_t inverse, grad, bias, acc, split, split_bytes;                               // backward
   int64_t ldp, slots, piece, ldg, ld_acc, plane;      // plane 0: dx is not cut into planes
   int planes;
@@ -442,19 +463,24 @@ int64_t bias_parts(int64_t columns, int64_t rows) {
   return std::clamp<int64_t>(std::min<int64_t>(148 / blocks, rows / (4 * kBiasGroups)), 1, kBiasParts);
 }
 
+int64_t starts_of(int64_t vocab) { return (vocab + kStartUnit - 1) / kStartUnit; }
+
 Layout layout_for(const ixk_linear_loss_desc& d, bool backward) {
   Layout l{};
   const int64_t N = d.rows, D = d.hidden, V = d.vocab, K = std::max<int64_t>(d.entries, 1);
   l.gathered = backward || N > kDirectRows;
   l.control = l.space.take(sizeof(Control));
-  l.row_map = l.space.take(4 * N);
   if (d.entries > 0) {
     l.column = l.space.take(4 * N * K);
     l.weight = l.space.take(4 * N * K);
+    l.start = l.space.take(sizeof(uint16_t) * N * starts_of(V));
     l.has = l.space.take(4 * N);
   }
   l.ldp = round_up(D, kPitchUnit);
-  if (l.gathered) l.packed = l.space.take(2 * N * l.ldp);
+  if (l.gathered) {
+    l.info = l.space.take(sizeof(RowInfo) * N);
+    l.packed = l.space.take(2 * N * l.ldp);
+  }
   if (!backward) {
     l.at_target = l.space.take(4 * N * K);
     l.slots = stat_slots(N, V);
@@ -568,6 +594,8 @@ int targets_of(const ixk_linear_loss_desc& d, const Layout& l, char* ws, const v
   a.inv_temperature = 1.0f / d.scale;
   t->column = a.column = reinterpret_cast<int*>(ws + l.column);
   t->weight = a.weight = reinterpret_cast<float*>(ws + l.weight);
+  t->start = a.start = reinterpret_cast<uint16_t*>(ws + l.start);
+  t->starts = a.starts = static_cast<int>(starts_of(d.vocab));
   has->has = a.has = reinterpret_cast<int*>(ws + l.has);
   const int64_t ctas = std::min<int64_t>((d.rows + kListWarps - 1) / kListWarps, 148 * 16);
   auto* fn = d.entries <= 32 ? lists_kernel<1> : d.entries <= 64 ? lists_kernel<2> : d.entries <= 128 ? lists_kernel<4> : lists_kernel<8>;
@@ -575,7 +603,7 @@ int targets_of(const ixk_linear_loss_desc& d, const Layout& l, char* ws, const v
 }
 
 int gather(const ixk_linear_loss_desc& d, const Layout& l, char* ws, const HasTarget& has, const void* x, float* loss, float* lse,
-           const float* grad_loss, float factor, bool want_dw, int sm_count, cudaStream_t stream) {
+           const float* lse_in, const float* grad_loss, float factor, bool want_dw, int sm_count, cudaStream_t stream) {
   const bool backward = loss == nullptr;
   Gather g{};
   g.has = has;
@@ -588,10 +616,11 @@ int gather(const ixk_linear_loss_desc& d, const Layout& l, char* ws, const HasTa
   // (each CTA counts the rows in front of it: at most 1024 CTAs while a CTA's rows fit its threads)
   g.rows_per_cta = static_cast<int>(std::min<int64_t>(std::max<int64_t>(8, (d.rows + 1023) / 1024), kGatherThreads));
   g.control = reinterpret_cast<Control*>(ws + l.control);
-  g.row_map = reinterpret_cast<int*>(ws + l.row_map);
+  g.info = reinterpret_cast<RowInfo*>(ws + l.info);
   g.inverse = backward ? reinterpret_cast<int*>(ws + l.inverse) : nullptr;
   g.loss = loss;
   g.lse = lse;
+  g.lse_in = lse_in;
   g.grad_loss = grad_loss;
   g.grad_stride = d.grad_loss_stride;
   g.factor = factor;
@@ -645,11 +674,11 @@ int forward(const char* name, const ixk_linear_loss_desc* d, bool distill, const
   if ((rc = targets_of(*d, l, ws, index, teacher, s, &t, &has)) != IXK_OK) return rc;
   Pass p = pass_of(*d, scales, x, d->x_stride, w, bias, t);
   if (l.gathered) {
-    if ((rc = gather(*d, l, ws, has, x, loss, lse, nullptr, 0.0f, false, dev.sm_count, s)) != IXK_OK) return rc;
+    if ((rc = gather(*d, l, ws, has, x, loss, lse, nullptr, nullptr, 0.0f, false, dev.sm_count, s)) != IXK_OK) return rc;
     p.x = ws + l.packed;
     p.ldx = l.ldp;
     p.active_rows = &reinterpret_cast<const Control*>(ws + l.control)->active;
-    p.row_map = reinterpret_cast<const int*>(ws + l.row_map);
+    p.info = reinterpret_cast<const RowInfo*>(ws + l.info);
   }
   p.partial = reinterpret_cast<float2*>(ws + l.partial);
   p.at_target = reinterpret_cast<float*>(ws + l.at_target);
@@ -660,7 +689,7 @@ int forward(const char* name, const ixk_linear_loss_desc* d, bool distill, const
   a.at_target = p.at_target;
   a.weight = t.weight;
   a.active = p.active_rows;
-  a.row_map = p.row_map;
+  a.info = p.info;
   a.rows = static_cast<int>(d->rows);
   a.slots = static_cast<int>(l.slots);
   a.entries = t.entries;
@@ -708,15 +737,11 @@ int backward(const char* name, const ixk_linear_loss_desc* d, bool distill, cons
   HasTarget has{};
   if ((rc = targets_of(*d, l, ws, index, teacher, s, &t, &has)) != IXK_OK) return rc;
   // fp16: G = g (p - q) with g = 1 / tokens and p = 1 / vocabulary would be lost below its smallest numbers
-  if ((rc = gather(*d, l, ws, has, x, nullptr, nullptr, grad_loss, scales.grad, dw != nullptr, dev.sm_count, s)) != IXK_OK) return rc;
+  if ((rc = gather(*d, l, ws, has, x, nullptr, nullptr, lse, grad_loss, scales.grad, dw != nullptr, dev.sm_count, s)) != IXK_OK) return rc;
   Pass p = pass_of(*d, scales, ws + l.packed, l.ldp, w, bias, t);
   const Control* control = reinterpret_cast<const Control*>(ws + l.control);
   p.active_rows = &control->active;
-  p.row_map = reinterpret_cast<const int*>(ws + l.row_map);
-  p.lse = lse;
-  p.grad_loss = grad_loss;
-  p.grad_stride = d->grad_loss_stride;
-  p.factor = scales.grad;
+  p.info = reinterpret_cast<const RowInfo*>(ws + l.info);
   p.range = bf16 ? nullptr : control->range;
   p.grad = ws + l.grad;
   p.ldg = l.ldg;

@@ -845,13 +845,27 @@ gemm_two_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_consta
     int which, bz, bm2, bn, kb0, count;
   };
   const int mine0 = units0 / pairs + (pair_id < heavy ? 1 : 0);
+  // Tiles go down bands of kBand row blocks (as tile_coords), column by column.
+  constexpr int kBand = 8;
+  const ptx::FastDiv by_tiles0(max(tiles0, 1)), by_band0(kBand * max(p0.tiles_n, 1)), by_band1(kBand * max(p1.tiles_n, 1));
+  const ptx::FastDiv by_last0((max(tiles_m0, 1) - 1) % kBand + 1), by_last1((max(tiles_m1, 1) - 1) % kBand + 1);
+  auto place = [](int t, int tiles_m, const ptx::FastDiv& by_band, const ptx::FastDiv& by_last, Unit& x) {
+    int r, in;
+    const int first = by_band.div(t, r) * kBand;
+    if (tiles_m - first >= kBand) {
+      x.bn = r / kBand;
+      in = r % kBand;
+    } else {
+      x.bn = by_last.div(r, in);
+    }
+    x.bm2 = first + in;
+  };
   auto unit_at = [&](int i, Unit& x) {       // the pair's i-th unit; false behind the last
     if (i < mine0) {
-      const int u = pair_id + i * pairs;
+      int t;
       x.which = 0;
-      x.bz = u / tiles0;
-      int bz;
-      tile_coords(u - x.bz * tiles0, tiles_m0, p0.tiles_n, bz, x.bm2, x.bn);
+      x.bz = by_tiles0.div(pair_id + i * pairs, t);
+      place(t, tiles_m0, by_band0, by_last0, x);
       x.kb0 = x.bz * plane_slabs;
       x.count = min(plane_slabs, num_kb0 - x.kb0);
       return true;
@@ -863,7 +877,8 @@ gemm_two_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_consta
     else t = ahead * light + (j - ahead) * pairs + pair_id;
     if (t >= tiles1) return false;
     x.which = 1;
-    tile_coords(t, tiles_m1, p1.tiles_n, x.bz, x.bm2, x.bn);
+    x.bz = 0;
+    place(t, tiles_m1, by_band1, by_last1, x);
     x.kb0 = end_kb1 > 0 ? 0 : num_kb1;       // (no rows: one slab behind K, which TMA fills with zeros)
     x.count = end_kb1 > 0 ? end_kb1 : 1;
     return true;

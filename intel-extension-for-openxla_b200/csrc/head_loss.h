@@ -16,7 +16,17 @@ struct Targets {
   int64_t ignore_index;
   const int* column;        // distillation: [rows][entries] ascending, kNoColumn behind the last one
   const float* weight;      // [rows][entries]
+  const uint16_t* start;    // [rows][starts]: the first entry at or behind column i * kStartUnit
+  int starts;
   int entries;              // 1 for labels
+};
+constexpr int kStartUnit = 256;
+
+// What the tiles' epilogue needs to know of a row, one 16-byte load.
+struct alignas(16) RowInfo {
+  int row;                  // of the batch
+  int label;                // cross entropy; kNoColumn: none
+  float lse2, coef;         // gradient: log-sum-exp, base 2; grad_loss times the logits' and the loss's factors
 };
 
 // One pass over columns [first, first + count) of the logits x w^T + bias, tile by tile.
@@ -28,17 +38,13 @@ struct Pass {
   int64_t ldx, ldw;
   float scale;              // of the logits
   const int* active_rows;   // device: rows of x that there are, nullptr: all
-  const int* row_map;       // device: row of the batch that a row of x is, nullptr: the same
+  const RowInfo* info;      // device, of x's rows; nullptr (statistics only): the batch's rows as they are
   int64_t first, count;
   Targets targets;
   // statistics
   float2* partial;          // [slots][rows]: maximum and sum of exponentials, base 2
   float* at_target;         // [batch rows][entries]: scaled logits at the targets
   // gradient
-  const float* lse;         // [batch rows]
-  const float* grad_loss;   // [batch rows], pitch grad_stride
-  int64_t grad_stride;
-  float factor;             // of the gradient, scale included
   const float* range;       // device: power of two that keeps fp16 in range, nullptr: 1
   void* grad;               // [rows up to a multiple of 256][count] of dtype, pitch ldg
   int64_t ldg;

@@ -55,16 +55,15 @@ struct Args {
   int stages, stage_bytes, a_bytes, b_boxes;
   int w_mn_major;
   uint32_t idesc;
-  const int *active_rows, *row_map;
+  const int* active_rows;
+  const RowInfo* info;
   const void* bias;
   int bf16, bias_vec_ok;
   float scale, scale2;                  // of the logits; times log2 e
   Targets targets;
   float2* partial;
   float* at_target;
-  const float *lse, *grad_loss, *range;
-  int64_t grad_stride;
-  float factor;
+  const float* range;
   int* status_word;
 };
 
@@ -142,26 +141,19 @@ struct Walk {
     after = at + 1 < entries ? column[at + 1] : kNoColumn;
   }
 };
-__device__ __forceinline__ Walk start_walk(const Targets& t, int64_t row, bool active, int from) {
+__device__ __forceinline__ Walk start_walk(const Targets& t, const RowInfo& info, bool active, int from) {
   Walk w{nullptr, 1, 0, kNoColumn, kNoColumn};
   if (!active) return w;
   if (t.labels != nullptr) {
-    const int64_t label = t.wide ? static_cast<const int64_t*>(t.labels)[row] : static_cast<const int*>(t.labels)[row];
-    // (a label outside the vocabulary is in no tile)
-    if (label != t.ignore_index && label >= from && label < kNoColumn) w.next = static_cast<int>(label);
+    if (info.label >= from) w.next = info.label;
     return w;
   }
-  w.column = t.column + row * t.entries;
+  w.column = t.column + static_cast<int64_t>(info.row) * t.entries;
   w.entries = t.entries;
-  int lo = 0, hi = t.entries;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (w.column[mid] < from) lo = mid + 1;
-    else hi = mid;
-  }
-  w.at = lo;
-  w.next = lo < t.entries ? w.column[lo] : kNoColumn;
-  w.after = lo + 1 < t.entries ? w.column[lo + 1] : kNoColumn;
+  w.at = t.start[static_cast<int64_t>(info.row) * t.starts + from / kStartUnit];
+  w.next = w.at < t.entries ? w.column[w.at] : kNoColumn;
+  w.after = w.at + 1 < t.entries ? w.column[w.at + 1] : kNoColumn;
+  while (w.next < from) w.step();
   return w;
 }
 
@@ -228,11 +220,18 @@ head_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
   const int num_units = tiles_m * args.strips;
   const int worker = kPair ? blockIdx.x >> 1 : blockIdx.x, workers = kPair ? gridDim.x >> 1 : gridDim.x;
   // Units of a band of row blocks, strip by strip: the CTAs at work share few strips of w and few blocks of x in L2.
+  const ptx::FastDiv by_band(kGroupM * args.strips), by_last((tiles_m - 1) % kGroupM + 1);
   auto unit_at = [&](int u, int& bm, int& n_begin, int& n_end) {
-    const int band = kGroupM * args.strips, g = u / band, first_m = g * kGroupM;
-    const int in_band = min(tiles_m - first_m, kGroupM), r = u - g * band;
-    bm = first_m + r % in_band;
-    n_begin = (r / in_band) * args.strip;
+    int r, in, strip;
+    const int first_m = by_band.div(u, r) * kGroupM;
+    if (tiles_m - first_m >= kGroupM) {
+      strip = r / kGroupM;
+      in = r % kGroupM;
+    } else {
+      strip = by_last.div(r, in);
+    }
+    bm = first_m + in;
+    n_begin = strip * args.strip;
     n_end = min(n_begin + args.strip, args.tiles_n);
   };
 
@@ -344,22 +343,39 @@ head_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
     int buf = 0;
     uint32_t acc_phase = 0;
     bool alive = true;
-    for (int u = worker; u < num_units && alive; u += workers) {
-      int bm, n_begin, n_end;
-      unit_at(u, bm, n_begin, n_end);
-      const int warp_row = (kPair ? bm * 2 + static_cast<int>(rank) : bm) * kBlockM + quarter * 32, row = warp_row + lane;
-      const bool active = row < active_rows;
-      const int64_t orig = active ? (args.row_map != nullptr ? args.row_map[row] : row) : 0;
-      Walk walk = start_walk(args.targets, orig, active, args.first + n_begin * args.tile_n);
-      float top = -FLT_MAX, sum = 0.0f;     // statistics so far: t <= top, sum of 2^(t - top)
-      float lse2 = 0.0f, coef = 0.0f;
-      if constexpr (kGrad) {
-        if (active) {
-          lse2 = args.lse[orig] * kLog2E;
-          coef = args.grad_loss[orig * args.grad_stride] * args.factor;
-          if (args.range != nullptr) coef *= *args.range;
+    const float range = kGrad && args.range != nullptr ? *args.range : 1.0f;
+    int warp_row = 0, n_begin = 0, n_end = 0;
+    RowInfo info{0, kNoColumn, 0.0f, 0.0f};
+    // a unit's place, and what is to be known of this thread's row (asked for a unit ahead of its use)
+    auto look = [&](int u, int& first_row, int& from, int& to, RowInfo& i) {
+      int bm;
+      unit_at(u, bm, from, to);
+      first_row = (kPair ? bm * 2 + static_cast<int>(rank) : bm) * kBlockM + quarter * 32;
+      const int row = first_row + lane;
+      if (row >= active_rows) return;
+      if (args.info != nullptr) {
+        const int4 v = *reinterpret_cast<const int4*>(args.info + row);
+        i = RowInfo{v.x, v.y, __int_as_float(v.z), __int_as_float(v.w)};
+      } else {
+        i.row = row;
+        if (args.targets.labels != nullptr) {
+          const int64_t label = args.targets.wide ? static_cast<const int64_t*>(args.targets.labels)[row] : static_cast<const int*>(args.targets.labels)[row];
+          // (a label outside the vocabulary is in no tile)
+          i.label = label != args.targets.ignore_index && label >= 0 && label < kNoColumn ? static_cast<int>(label) : kNoColumn;
         }
       }
+    };
+    if (worker < num_units) look(worker, warp_row, n_begin, n_end, info);
+    int next_row = 0, next_begin = 0, next_end = 0;
+    RowInfo next_info = info;
+    for (int u = worker; u < num_units && alive; u += workers, warp_row = next_row, n_begin = next_begin, n_end = next_end, info = next_info) {
+      if (u + workers < num_units) look(u + workers, next_row, next_begin, next_end, next_info);
+      const int row = warp_row + lane;
+      const bool active = row < active_rows;
+      const int64_t orig = info.row;
+      Walk walk = start_walk(args.targets, info, active, args.first + n_begin * args.tile_n);
+      float top = -FLT_MAX, sum = 0.0f;     // statistics so far: t <= top, sum of 2^(t - top)
+      const float lse2 = info.lse2, coef = info.coef * range;
       // (the products read the gradient's rows up to the end of a slab, or of the only row block: zeros)
       const bool work = !kGrad ? warp_row < active_rows
                                : args.rows <= kDirectRows || warp_row < (active_rows + kSlabElems - 1) / kSlabElems * kSlabElems;
@@ -583,7 +599,7 @@ int launch(const Pass& p, const DeviceInfo& dev, cudaStream_t stream) {
   const uint32_t fmt = p.dtype == IXK_BF16 ? 1u : 0u;
   a.idesc = ptx::umma_idesc(fmt, fmt, 0, a.w_mn_major, t.pair ? 2 * kBlockM : kBlockM, t.tile_n);
   a.active_rows = p.active_rows;
-  a.row_map = p.row_map;
+  a.info = p.info;
   a.bias = p.bias;
   a.bf16 = p.dtype == IXK_BF16 ? 1 : 0;
   a.bias_vec_ok = p.bias != nullptr && (reinterpret_cast<uintptr_t>(p.bias) & 15u) == 0;
@@ -592,11 +608,7 @@ int launch(const Pass& p, const DeviceInfo& dev, cudaStream_t stream) {
   a.targets = p.targets;
   a.partial = p.partial;
   a.at_target = p.at_target;
-  a.lse = p.lse;
-  a.grad_loss = p.grad_loss;
   a.range = p.range;
-  a.grad_stride = p.grad_stride;
-  a.factor = p.factor;
   a.status_word = dev.status_word;
 
   const int64_t tile_rows = t.pair ? 2 * kBlockM : kBlockM;

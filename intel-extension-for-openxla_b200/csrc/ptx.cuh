@@ -646,6 +646,26 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // ---------------------------------------------------------------- misc math
+// Division of small numbers that a kernel divides by again and again: an estimate in fp32 (within one of the quotient below
+// 2^23) and its correction, 6 instructions instead of 40.
+struct FastDiv {
+  int d;
+  float inverse;
+  __device__ __forceinline__ explicit FastDiv(int divisor) : d(divisor), inverse(1.0f / static_cast<float>(divisor)) {}
+  __device__ __forceinline__ int div(int n, int& rest) const {      // 0 <= n, rest = n % d
+    int q = static_cast<int>(static_cast<float>(n) * inverse);
+    rest = n - q * d;
+    while (rest < 0) {
+      --q;
+      rest += d;
+    }
+    while (rest >= d) {
+      ++q;
+      rest -= d;
+    }
+    return q;
+  }
+};
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
