@@ -764,6 +764,54 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
 // pair i takes units i, i + pairs, ... of the long product (planes x tiles, all tiles of a plane side by side, so that pairs
 // walk K together and share slabs in L2), then tiles of the other, in an order that a round of all pairs at work at the time
 // takes neighbouring tiles: the pairs with one long unit less run `ahead` rounds among themselves first.
+// A warp's 32 rows x 128 columns of a 16-bit result without bias or activation: scaled, rounded, stored through its box.
+__device__ __forceinline__ void store_half_tile(const KernelArgs& args, const CUtensorMap* tmap_d, uint32_t tmem_acc, uint32_t box, int row,
+                                                int n_first, int lane) {
+  const float scale = args.acc_scale_dev != nullptr ? args.acc_scale * *args.acc_scale_dev : args.acc_scale;
+  const bool bf16 = args.out_dtype == IXK_BF16, odd_end = (args.N & 7) != 0;
+  if (n_first >= args.N) return;
+  uint32_t r[32];
+  ptx::tmem_ld_32x32(tmem_acc, r);
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const int n = n_first + 64 * g;
+    if (n >= args.N) break;
+    const bool plain = odd_end && n + 64 > args.N;      // (see epilogue_tile)
+    uint32_t words[32];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      // (tensor memory hands out 16 bytes a cycle and quarter: a chunk is asked for while the one before it is worked on)
+      ptx::tmem_ld_wait_for(r);
+      float v[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) * scale;
+      if (g == 0 || h == 0) ptx::tmem_ld_32x32(tmem_acc + 64 * g + 32 * (h + 1), r);
+      pack_row16(v, bf16 ? IXK_BF16 : IXK_F16, &words[16 * h]);
+      const int nh = n + 32 * h;
+      if (plain && row + lane < args.M && nh < args.N)
+        store_row(args.d, static_cast<int64_t>(row + lane) * args.ldd + nh, args.out_dtype, min(32, args.N - nh), args.d_vec_ok != 0, v);
+    }
+    if (plain) break;
+    if (lane == 0) ptx::bulk_wait_group_read<0>();
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t addr = box + static_cast<uint32_t>(lane * 128 + ((i ^ (lane & 7)) << 4));
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(words[4 * i]), "r"(words[4 * i + 1]), "r"(words[4 * i + 2]),
+                   "r"(words[4 * i + 3])
+                   : "memory");
+    }
+    ptx::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      ptx::tma_store_3d(tmap_d, box, n, row, 0);
+      ptx::bulk_commit_group();
+    }
+  }
+  // (a chunk behind N may still be on its way into registers)
+  ptx::tmem_ld_wait_for(r);
+}
+
 constexpr int kTwoEpilogueWarps = 8, kTwoThreads = 32 * (2 + kTwoEpilogueWarps);
 static_assert(kTwoEpilogueWarps * 4096 <= PairCfg::kStagingBytes, "staging boxes");
 struct TwoArgs {
@@ -977,9 +1025,13 @@ gemm_two_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_consta
     for (int i = 0; unit_at(i, x); ++i) {
       if (!ptx::mbar_wait(acc_full_bar(buf), acc_phase, ctl, kSiteEpilogue)) break;
       ptx::tc_fence_after_sync();
-      epilogue_tile<kBlockN, 1>(args.p[x.which], &tmap_d1, tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * kBlockN + half * (kBlockN / 2),
-                                box, x.bz, x.bm2 * 2 + static_cast<int>(rank), x.bn * kBlockN + half * (kBlockN / 2), quarter, lane, n_store,
-                                kBlockN / 2);
+      const uint32_t acc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * kBlockN + half * (kBlockN / 2);
+      const int bm = x.bm2 * 2 + static_cast<int>(rank), n_first = x.bn * kBlockN + half * (kBlockN / 2);
+      if (x.which == 1 && p1.d_tma) {
+        if (bm * kBlockM < p1.M) store_half_tile(p1, &tmap_d1, acc, box, bm * kBlockM + quarter * 32, n_first, lane);
+      } else {
+        epilogue_tile<kBlockN, 1>(args.p[x.which], &tmap_d1, acc, box, x.bz, bm, n_first, quarter, lane, n_store, kBlockN / 2);
+      }
       ptx::tc_fence_before_sync();
       if (rank == 0) ptx::mbar_arrive(acc_empty_bar(buf));
       else ptx::mbar_arrive_cluster_tmem(acc_empty_bar(buf), 0);
