@@ -288,12 +288,11 @@ struct Loss {
   float *loss, *lse;
 };
 
-constexpr int kLossThreads = 256;
 
 // kRows rows per CTA, side by side in memory; their partials dealt out over the remaining threads.
-template <int kRows>
-__global__ void __launch_bounds__(kLossThreads) loss_kernel(const Loss a) {
-  constexpr int kParts = kLossThreads / kRows;
+template <int kRows, int kThreads>
+__global__ void __launch_bounds__(kThreads) loss_kernel(const Loss a) {
+  constexpr int kParts = kThreads / kRows;
   __shared__ float2 stat[kParts][kRows];
   __shared__ float row_lse[kRows], share[kParts][kRows];
   ptx::grid_dependency_sync();
@@ -307,7 +306,7 @@ __global__ void __launch_bounds__(kLossThreads) loss_kernel(const Loss a) {
   };
   float2 s = make_float2(-FLT_MAX, 0.0f);
   if (there) {
-#pragma unroll 4
+#pragma unroll 8
     for (int i = part; i < a.slots; i += kParts) s = join(s, a.partial[static_cast<int64_t>(i) * a.rows + row]);
   }
   stat[part][r] = s;
@@ -352,21 +351,22 @@ __device__ __forceinline__ uint32_t to16(float f) {
   else return __half_as_ushort(__float2half_rn(f));
 }
 
-// dbias of a piece: the sums of G's columns.  256 columns per CTA, 32 warps that take rows in turn; where the columns alone
+// dbias of a piece: the sums of G's columns.  256 columns per CTA, kGroups warps that take rows in turn; where the columns alone
 // leave SMs idle the rows are dealt out to gridDim.y CTAs, which leave partial sums for bias_sum_kernel.
-constexpr int kBiasCols = 256, kBiasGroups = 32, kBiasParts = 32;
-template <bool kBf16>
-__global__ void __launch_bounds__(32 * kBiasGroups) bias_kernel(const uint16_t* g, int64_t ldg, const Control* control, int count, float* partial,
+constexpr int kBiasCols = 256, kBiasGroups = 32, kFewGroups = 4, kBiasParts = 32;
+constexpr int64_t kFewBiasRows = 32;      // 5 x 176783: 6.9 us with 32 warps, 4.3 with four; 76 x 99763: 7.7 and 13
+template <bool kBf16, int kGroups>
+__global__ void __launch_bounds__(32 * kGroups) bias_kernel(const uint16_t* g, int64_t ldg, const Control* control, int count, float* partial,
                                                               uint16_t* out) {
-  __shared__ float sums[kBiasGroups][kBiasCols];
+  __shared__ float sums[kGroups][kBiasCols];
   ptx::grid_dependency_sync();
   const int group = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = control->active;
   const int c0 = blockIdx.x * kBiasCols + lane * 8;
   float t[8] = {};
   if (c0 < count) {      // (G's pitch is whole vectors)
     const uint16_t* p = g + c0;
-#pragma unroll 4
-    for (int row = blockIdx.y * kBiasGroups + group; row < rows; row += gridDim.y * kBiasGroups) {
+#pragma unroll 8
+    for (int row = blockIdx.y * kGroups + group; row < rows; row += gridDim.y * kGroups) {
       const uint4 w = *reinterpret_cast<const uint4*>(p + row * ldg);
       const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -379,10 +379,12 @@ __global__ void __launch_bounds__(32 * kBiasGroups) bias_kernel(const uint16_t* 
 #pragma unroll
   for (int j = 0; j < 8; ++j) sums[group][lane * 8 + j] = t[j];
   __syncthreads();
-  const int c = blockIdx.x * kBiasCols + threadIdx.x;
-  if (threadIdx.x < kBiasCols && c < count) {
+  for (int col = threadIdx.x; col < kBiasCols; col += 32 * kGroups) {
+    const int c = blockIdx.x * kBiasCols + col;
+    if (c >= count) return;
     float s = 0.0f;
-    for (int i = 0; i < kBiasGroups; ++i) s += sums[i][threadIdx.x];
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) s += sums[i][col];
     if (gridDim.y > 1) partial[static_cast<int64_t>(blockIdx.y) * count + c] = s;
     else out[c] = static_cast<uint16_t>(to16<kBf16>(kBf16 ? s : s * control->range[1]));
   }
@@ -401,11 +403,11 @@ __global__ void __launch_bounds__(128) bias_sum_kernel(const float* partial, int
 // dx: the accumulator's rows, their planes added up, back to where they came from, rounded once; zeros where there was no
 // target.
 template <bool kBf16>
-__global__ void __launch_bounds__(256) scatter_kernel(const float* acc, int64_t ld_acc, int64_t plane, int known_planes, const int* inverse, const Control* control,
+__global__ void __launch_bounds__(256) scatter_kernel(const float* acc, int64_t ld_acc, int64_t plane, const int* inverse, const Control* control,
                                                       int hidden, int vec, uint16_t* dx, int64_t ld) {
   ptx::grid_dependency_sync();
   const int64_t row = blockIdx.x;
-  const int from = inverse[row], planes = known_planes > 0 ? known_planes : control->planes;
+  const int from = inverse[row], planes = control->planes;
   const float scale = kBf16 ? 1.0f : control->range[1];
   const float* src = acc + from * ld_acc;
   uint16_t* dst = dx + row * ld;
@@ -414,6 +416,7 @@ __global__ void __launch_bounds__(256) scatter_kernel(const float* acc, int64_t 
     uint4 w = make_uint4(0, 0, 0, 0);
     if (from >= 0) {
       float4 a = reinterpret_cast<const float4*>(src)[2 * v], b = reinterpret_cast<const float4*>(src)[2 * v + 1];
+#pragma unroll 8
       for (int i = 1; i < planes; ++i) {
         const float4 c = reinterpret_cast<const float4*>(src + i * plane)[2 * v], d = reinterpret_cast<const float4*>(src + i * plane)[2 * v + 1];
         a = make_float4(a.x + c.x, a.y + c.y, a.z + c.z, a.w + c.w);
@@ -428,10 +431,44 @@ __global__ void __launch_bounds__(256) scatter_kernel(const float* acc, int64_t 
   }
   for (int c = vecs * 8 + threadIdx.x; c < hidden; c += blockDim.x) {
     float t = 0.0f;
-    if (from >= 0)
+    if (from >= 0) {
+#pragma unroll 8
       for (int i = 0; i < planes; ++i) t += src[i * plane + c];
+    }
     dst[c] = static_cast<uint16_t>(to16<kBf16>(t * scale));
   }
+}
+
+// The same for few rows in many planes: 256 columns per CTA, eight groups of threads that take planes in turn.
+constexpr int kFewCols = 256, kFewPlaneGroups = 8;
+template <bool kBf16>
+__global__ void __launch_bounds__(32 * kFewPlaneGroups) scatter_few_kernel(const float* acc, int64_t ld_acc, int64_t plane, int planes, const int* inverse,
+                                                                         const Control* control, int hidden, uint16_t* dx, int64_t ld) {
+  __shared__ float sums[kFewPlaneGroups][kFewCols];
+  ptx::grid_dependency_sync();
+  const int64_t row = blockIdx.x;
+  const int from = inverse[row], lane = threadIdx.x & 31, group = threadIdx.x >> 5, c0 = blockIdx.y * kFewCols;
+  if (from >= 0) {
+    const float* src = acc + from * ld_acc + c0;
+    float t[8] = {};
+#pragma unroll 4
+    for (int i = group; i < planes; i += kFewPlaneGroups) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c0 + lane + 32 * j < hidden) t[j] += src[i * plane + lane + 32 * j];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sums[group][lane + 32 * j] = t[j];
+  }
+  __syncthreads();
+  const int c = c0 + threadIdx.x;
+  if (c >= hidden) return;
+  float s = 0.0f;
+  if (from >= 0) {
+#pragma unroll
+    for (int i = 0; i < kFewPlaneGroups; ++i) s += sums[i][threadIdx.x];
+  }
+  dx[row * ld + c] = static_cast<uint16_t>(to16<kBf16>(kBf16 ? s : s * control->range[1]));
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -696,14 +733,15 @@ int forward(const char* name, const ixk_linear_loss_desc* d, bool distill, const
   a.factor = scales.loss;
   a.loss = loss;
   a.lse = lse;
-  auto go = [&](auto rows) -> int {
-    constexpr int kRows = decltype(rows)::value;
-    return launch_overlapped(loss_kernel<kRows>, dim3(static_cast<unsigned>((d->rows + kRows - 1) / kRows)), dim3(kLossThreads), 0, s, a);
+  auto go = [&](auto rows, auto threads) -> int {
+    constexpr int kRows = decltype(rows)::value, kThreads = decltype(threads)::value;
+    return launch_overlapped(loss_kernel<kRows, kThreads>, dim3(static_cast<unsigned>((d->rows + kRows - 1) / kRows)), dim3(kThreads), 0, s, a);
   };
   // (rows side by side are one read of up to 256 bytes; few rows want a CTA each)
-  if (d->rows >= 4096) return go(std::integral_constant<int, 32>{});
-  if (d->rows >= 512) return go(std::integral_constant<int, 8>{});
-  return go(std::integral_constant<int, 1>{});
+  using std::integral_constant;
+  if (d->rows >= 4096) return go(integral_constant<int, 32>{}, integral_constant<int, 1024>{});
+  if (d->rows >= 512) return go(integral_constant<int, 8>{}, integral_constant<int, 1024>{});
+  return go(integral_constant<int, 1>{}, integral_constant<int, 256>{});
 }
 
 int backward(const char* name, const ixk_linear_loss_desc* d, bool distill, const void* x, const void* w, const void* bias,
@@ -805,7 +843,10 @@ int backward(const char* name, const ixk_linear_loss_desc* d, bool distill, cons
       const unsigned blocks = static_cast<unsigned>((p.count + kBiasCols - 1) / kBiasCols), parts = static_cast<unsigned>(bias_parts(p.count, d->rows));
       float* partial = reinterpret_cast<float*>(ws + l.bias);
       auto* out = static_cast<uint16_t*>(dbias) + first;
-      rc = launch_overlapped(bf16 ? bias_kernel<true> : bias_kernel<false>, dim3(blocks, parts), dim3(32 * kBiasGroups), 0, s,
+      const bool few = d->rows <= kFewBiasRows;
+      auto* fn = few ? (bf16 ? bias_kernel<true, kFewGroups> : bias_kernel<false, kFewGroups>)
+                     : (bf16 ? bias_kernel<true, kBiasGroups> : bias_kernel<false, kBiasGroups>);
+      rc = launch_overlapped(fn, dim3(blocks, parts), dim3(32 * (few ? kFewGroups : kBiasGroups)), 0, s,
                              static_cast<const uint16_t*>(p.grad), l.ldg, control, static_cast<int>(p.count), partial, out);
       if (rc == IXK_OK && parts > 1)
         rc = launch_overlapped(bf16 ? bias_sum_kernel<true> : bias_sum_kernel<false>, dim3(static_cast<unsigned>((p.count + 127) / 128)), dim3(128), 0, s,
@@ -814,11 +855,16 @@ int backward(const char* name, const ixk_linear_loss_desc* d, bool distill, cons
     }
   }
   if (dx == nullptr) return IXK_OK;
-  const int vec = aligned(dx, 16) && d->dx_stride % 8 == 0 && l.ld_acc % 4 == 0;
-  auto* fn = bf16 ? scatter_kernel<true> : scatter_kernel<false>;
-  return launch_overlapped(fn, dim3(static_cast<unsigned>(d->rows)), dim3(256), 0, s, static_cast<const float*>(acc), l.ld_acc, l.plane,
-                           d->rows > kDirectRows ? 0 : std::max(l.planes, 1), reinterpret_cast<const int*>(ws + l.inverse), control, static_cast<int>(d->hidden), vec, static_cast<uint16_t*>(dx),
-                           d->dx_stride);
+  const int* inverse = reinterpret_cast<const int*>(ws + l.inverse);
+  if (d->rows <= kDirectRows)
+    return launch_overlapped(bf16 ? scatter_few_kernel<true> : scatter_few_kernel<false>,
+                             dim3(static_cast<unsigned>(d->rows), static_cast<unsigned>((d->hidden + kFewCols - 1) / kFewCols)), dim3(32 * kFewPlaneGroups), 0, s,
+                             static_cast<const float*>(acc), l.ld_acc, l.plane, std::max(l.planes, 1), inverse, control, static_cast<int>(d->hidden),
+                             static_cast<uint16_t*>(dx), d->dx_stride);
+  const int vec = aligned(dx, 16) && d->dx_stride % 8 == 0;
+  return launch_overlapped(bf16 ? scatter_kernel<true> : scatter_kernel<false>, dim3(static_cast<unsigned>(d->rows)), dim3(256), 0, s,
+                           static_cast<const float*>(acc), l.ld_acc, l.plane, inverse, control, static_cast<int>(d->hidden), vec,
+                           static_cast<uint16_t*>(dx), d->dx_stride);
 }
 
 }  // namespace

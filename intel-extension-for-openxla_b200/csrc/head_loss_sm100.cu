@@ -240,13 +240,13 @@ head_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
     int stage = 0;
     uint32_t phase = 0;
     bool alive = true;
-    const uint32_t cta_bytes = static_cast<uint32_t>(args.a_bytes + (args.w_mn_major ? args.b_boxes * kSlabElems : kPair ? 128 : args.tile_n) * kSlabBytes);
+    const uint32_t cta_bytes = static_cast<uint32_t>(args.a_bytes + (args.w_mn_major ? args.b_boxes * kSlabElems : kPair ? args.tile_n / 2 : args.tile_n) * kSlabBytes);
     for (int u = worker; u < num_units && alive; u += workers) {
       int bm, n_begin, n_end;
       unit_at(u, bm, n_begin, n_end);
       const int m0 = (kPair ? bm * 2 + static_cast<int>(rank) : bm) * kBlockM;
       for (int n = n_begin; n < n_end && alive; ++n) {
-        const int v0 = args.first + n * args.tile_n + (kPair ? static_cast<int>(rank) * 128 : 0);
+        const int v0 = args.first + n * args.tile_n + (kPair ? static_cast<int>(rank) * (args.tile_n / 2) : 0);
         for (int kb = 0; kb < args.slabs; ++kb) {
           if (!ptx::mbar_wait(empty_bar(stage), phase ^ 1u, ctl, kSiteProducer)) {
             alive = false;
@@ -522,7 +522,7 @@ struct Tiling {
   int tile_n, tiles_n, strip, strips;
 };
 
-// 256 x 256 tiles on CTA pairs once every pair has one; else row blocks of 128 and column tiles that are as wide as a whole
+// 256 x 256 tiles on CTA pairs once every pair has one (narrower ones where that fills the last of few rounds); else row blocks of 128 and column tiles that are as wide as a whole
 // number of rounds of all SMs allows, in steps of `unit` columns.
 Tiling tiling_for(int64_t rows, int64_t columns, int unit) {
   Tiling t{};
@@ -530,7 +530,12 @@ Tiling tiling_for(int64_t rows, int64_t columns, int unit) {
   t.pair = rows > kBlockM && pair_rows * wide >= pairs;
   t.strip = 1;
   if (t.pair) {
+    // (a tile of w columns takes about w + 16 columns' time; the gradient's boxes are 64 columns, a CTA's half 16)
     t.tile_n = kMaxTileN;
+    auto time = [&](int w) { return (pair_rows * ((columns + w - 1) / w) + pairs - 1) / pairs * (w + 16); };
+    for (int w = kMaxTileN; w >= 192; w -= std::max(unit, 32))
+      if (time(w) * 100 < time(t.tile_n) * 98) t.tile_n = w;
+    const int64_t wide = (columns + t.tile_n - 1) / t.tile_n;
     t.tiles_n = static_cast<int>(wide);
     // the longest strip that does not lengthen the longest pair's share by more than 1 %
     auto rounds = [&](int strip) { return (pair_rows * ((wide + strip - 1) / strip) + pairs - 1) / pairs * strip; };
@@ -554,7 +559,7 @@ template <bool kGrad>
 int launch(const Pass& p, const DeviceInfo& dev, cudaStream_t stream) {
   const Tiling t = tiling_for(p.rows, p.count, kGrad ? kGradUnit : kStatUnit);
   const int a_rows = t.pair ? kBlockM : static_cast<int>(std::min<int64_t>(kBlockM, (p.rows + 7) / 8 * 8));
-  const int b_rows = t.pair ? 128 : t.tile_n;
+  const int b_rows = t.pair ? t.tile_n / 2 : t.tile_n;
   const CUtensorMapDataType dt = p.dtype == IXK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   auto map = [&](CUtensorMap* out, const void* base, int64_t inner, int64_t outer, int64_t ld, int box_inner, int box_outer) {
     TmapSpec s{};
