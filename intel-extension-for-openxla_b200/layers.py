@@ -77,6 +77,28 @@ class KernelOps:
     def kv_append_(self, k_cache, v_cache, k_new, v_new, position):
         self.pkg.kv_append_(k_cache, v_cache, k_new, v_new, position)
 
+    def norm_forward(self, x, kind, eps, gain, gain_offset, shift):
+        return self.pkg.row_norm_forward(x, kind=self._kind(kind), eps=eps, gain=gain, gain_offset=gain_offset, shift=shift)
+
+    def norm_backward(self, grad, x, mean, rstd, kind, gain, gain_offset, with_shift):
+        return self.pkg.row_norm_backward(grad, x, mean, rstd, kind=self._kind(kind), gain=gain, gain_offset=gain_offset,
+                                          with_shift=with_shift)
+
+    def _kind(self, kind):
+        return self.pkg.NORM_LAYER if kind == "layer" else self.pkg.NORM_RMS
+
+    def head_loss(self, h, weight, bias, target, temperature):
+        """`target`: labels, or a teacher's (indices, logits)."""
+        if isinstance(target, tuple):
+            return self.pkg.linear_distillation(h, weight, *target, bias=bias, temperature=temperature)
+        return self.pkg.linear_cross_entropy(h, weight, target, bias=bias)
+
+    def head_loss_backward(self, h, weight, bias, target, temperature, lse, grad_loss, weight_grad):
+        if isinstance(target, tuple):
+            return self.pkg.linear_distillation_backward(h, weight, *target, lse, grad_loss, bias=bias, temperature=temperature,
+                                                         weight_grad=weight_grad)
+        return self.pkg.linear_cross_entropy_backward(h, weight, target, lse, grad_loss, bias=bias, weight_grad=weight_grad)
+
 
 def _glue(ops, name, fallback):
     return getattr(ops, name, None) or fallback
@@ -354,3 +376,113 @@ def gemma_decode_bytes(B, T, hidden=3072, heads=16, head_dim=256, ffn=24576, ele
     attn = 2.0 * B * heads * T * head_dim * elem + 2.0 * B * heads * head_dim * elem
     weights = (hidden * 3 * heads * head_dim + heads * head_dim * hidden + 2 * hidden * ffn + ffn * hidden) * elem
     return attn + weights
+
+
+# ----------------------------------------------------------------------------- the end of a training step
+
+def _norm_forward_torch(x, kind, eps, gain, gain_offset, shift):
+    xf = x.float()
+    mean = xf.mean(-1) if kind == "layer" else None
+    xc = xf if mean is None else xf - mean[..., None]
+    rstd = torch.rsqrt(xc.pow(2).mean(-1) + eps)
+    y = xc * rstd[..., None]
+    y = y if gain is None else y * (gain_offset + gain.float())
+    return (y if shift is None else y + shift.float()).to(x.dtype), mean, rstd
+
+
+def _norm_backward_torch(grad, x, mean, rstd, kind, gain, gain_offset, with_shift):
+    g, xc = grad.float(), x.float() if mean is None else x.float() - mean[..., None]
+    xh = xc * rstd[..., None]
+    h = g if gain is None else g * (gain_offset + gain.float())
+    dx = h - xh * (h * xh).mean(-1, keepdim=True) - (h.mean(-1, keepdim=True) if kind == "layer" else 0)
+    over = tuple(range(x.dim() - 1))
+    like = x if gain is None else gain
+    return ((dx * rstd[..., None]).to(x.dtype), None if gain is None else (g * xh).sum(over).to(like.dtype),
+            g.sum(over).to(like.dtype) if with_shift else None)
+
+
+def _head_targets(h, weight, target, temperature):
+    """(columns, weights, rows that count): one column of weight 1 per label, or the teacher's softmax over its entries."""
+    vocab = weight.shape[0]
+    if not isinstance(target, tuple):
+        ok = (target >= 0) & (target < vocab)
+        return torch.where(ok, target, 0)[:, None].long(), ok[:, None].float(), ok
+    index, logits = target
+    ok = (index >= 0) & (index < vocab) & (logits > -math.inf)
+    t = torch.where(ok, logits.float() / temperature, -math.inf)
+    rows = ok.any(1)
+    return torch.where(ok, index, 0).long(), torch.where(ok, torch.softmax(torch.where(rows[:, None], t, 0.0), 1), 0.0), rows
+
+
+def _head_logits(h, weight, bias, rows, scale):
+    z = torch.where(rows[:, None], h.float(), 0.0) @ weight.float().t()
+    return (z if bias is None else z + bias.float()) * scale
+
+
+def _head_loss_torch(h, weight, bias, target, temperature):
+    columns, q, rows = _head_targets(h, weight, target, temperature)
+    scale = 1.0 / temperature if isinstance(target, tuple) else 1.0
+    z = _head_logits(h, weight, bias, rows, scale)
+    lse = torch.logsumexp(z, 1)
+    loss = (torch.special.xlogy(q, q) + q * (lse[:, None] - z.gather(1, columns))).sum(1) / (scale * scale)
+    return torch.where(rows, loss, 0.0), torch.where(rows, lse, 0.0)
+
+
+def _head_loss_backward_torch(h, weight, bias, target, temperature, lse, grad_loss, weight_grad):
+    columns, q, rows = _head_targets(h, weight, target, temperature)
+    scale = 1.0 / temperature if isinstance(target, tuple) else 1.0
+    p = torch.exp(_head_logits(h, weight, bias, rows, scale) - lse[:, None])
+    g = torch.where(rows, grad_loss.float().expand(rows.shape), 0.0)[:, None] * p.scatter_add_(1, columns, -q) / scale
+    dh = (g @ weight.float()).to(h.dtype)
+    if not weight_grad:
+        return dh, None, None
+    x = torch.where(rows[:, None], h.float(), 0.0)
+    return dh, (g.t() @ x).to(weight.dtype), None if bias is None else g.sum(0).to(bias.dtype)
+
+
+@dataclass
+class LmHeadWeights:
+    """The final norm and the vocabulary head: RMSNorm with the (1 + w) scale (Gemma) or LayerNorm with gain and shift (GPT-J, whose
+    head has a bias).  weight [vocab, hidden] (the token embedding, where the two are tied)."""
+    weight: torch.Tensor
+    gain: torch.Tensor
+    kind: str = "rms"                       # "rms" or "layer"
+    shift: Optional[torch.Tensor] = None
+    bias: Optional[torch.Tensor] = None
+    eps: float = 1e-6
+
+
+@dataclass
+class LmHeadGradients:
+    x: torch.Tensor
+    gain: torch.Tensor
+    shift: Optional[torch.Tensor]
+    weight: Optional[torch.Tensor]
+    bias: Optional[torch.Tensor]
+
+
+def lm_head_training_pass(x: torch.Tensor, w: LmHeadWeights, ops, *, labels: Optional[torch.Tensor] = None, teacher=None,
+                          temperature: float = 1.0, loss_scale: float = 1.0, weight_grad: bool = True):
+    """The end of a decoder's training step (the loss of the reference's fine-tuning example, example/gemma/finetune.py): final
+    norm, vocabulary head and loss, and back to the hidden states x [..., hidden].  `labels` (x's shape without its last
+    dimension; -100, or anything else outside the vocabulary, for tokens that carry no loss), or `teacher` = (indices, logits)
+    [..., entries] to distil from.  Returns (mean loss over the tokens that count, gradients of loss_scale times it).  The
+    [tokens, vocab] logits are in memory at no time; nothing here waits for the GPU."""
+    hidden = x.shape[-1]
+    rows = x.reshape(-1, hidden)
+    if (labels is None) == (teacher is None):
+        raise ValueError("either labels or a teacher")
+    offset = 1.0 if w.kind == "rms" else 0.0
+    if teacher is None:
+        target = labels.reshape(-1)
+        counts = (target >= 0) & (target < w.weight.shape[0])
+    else:
+        target = tuple(t.reshape(-1, t.shape[-1]) for t in teacher)
+        counts = ((target[0] >= 0) & (target[0] < w.weight.shape[0]) & (target[1] > -math.inf)).any(1)
+    h, mean, rstd = _glue(ops, "norm_forward", _norm_forward_torch)(rows, w.kind, w.eps, w.gain, offset, w.shift)
+    loss, lse = _glue(ops, "head_loss", _head_loss_torch)(h, w.weight, w.bias, target, temperature)
+    count = counts.sum().clamp(min=1).float()
+    dh, dweight, dbias = _glue(ops, "head_loss_backward", _head_loss_backward_torch)(
+        h, w.weight, w.bias, target, temperature, lse, loss_scale / count, weight_grad)
+    dx, dgain, dshift = _glue(ops, "norm_backward", _norm_backward_torch)(dh, rows, mean, rstd, w.kind, w.gain, offset, w.shift is not None)
+    return loss.sum() / count, LmHeadGradients(x=dx.view(x.shape), gain=dgain, shift=dshift, weight=dweight, bias=dbias)
