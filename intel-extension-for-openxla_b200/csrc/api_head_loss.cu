@@ -37,6 +37,17 @@ constexpr float kLn2 = 0.6931471805599453f, kLog2E = 1.4426950408889634f;
 
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
+template <bool kBf16>
+__device__ __forceinline__ float from16(uint32_t bits) {
+  if constexpr (kBf16) return __uint_as_float(bits << 16);
+  else return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+}
+template <bool kBf16>
+__device__ __forceinline__ uint32_t to16(float f) {
+  if constexpr (kBf16) return __bfloat16_as_ushort(__float2bfloat16_rn(f));
+  else return __half_as_ushort(__float2half_rn(f));
+}
+
 // ------------------------------------------------------------------------------------------------ lists
 
 struct Lists {
@@ -286,19 +297,66 @@ struct Loss {
   int rows, slots, entries;
   float factor;
   float *loss, *lse;
+  // labels: the label's logit, scale (x . w[label] + bias[label]), is made here (and left out of the partials)
+  const uint16_t *x, *w, *bias;
+  int64_t ldx, ldw;
+  int hidden, w_column_major;
+  float scale;
 };
 
 
-// kRows rows per CTA, side by side in memory; their partials dealt out over the remaining threads.
-template <int kRows, int kThreads>
+// A lane's share of x . w[label]: every step-th vector from `first` on (w row-major), or element.
+template <bool kBf16>
+__device__ __forceinline__ float dot_share(const Loss& a, int64_t row, int label, int first, int step) {
+  const uint16_t* x = a.x + row * a.ldx;
+  float t = 0.0f;
+  if (a.w_column_major) {
+    const uint16_t* w = a.w + label;
+#pragma unroll 8
+    for (int c = first; c < a.hidden; c += step) t = fmaf(from16<kBf16>(x[c]), from16<kBf16>(w[c * a.ldw]), t);
+    return t;
+  }
+  const uint16_t* w = a.w + label * a.ldw;
+  const int whole = a.hidden / 8;
+#pragma unroll 4
+  for (int v = first; v < whole; v += step) {
+    const uint4 p = reinterpret_cast<const uint4*>(x)[v], q = reinterpret_cast<const uint4*>(w)[v];
+    const uint32_t pw[4] = {p.x, p.y, p.z, p.w}, qw[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      t = fmaf(from16<kBf16>(pw[j] & 0xffffu), from16<kBf16>(qw[j] & 0xffffu), t);
+      t = fmaf(from16<kBf16>(pw[j] >> 16), from16<kBf16>(qw[j] >> 16), t);
+    }
+  }
+  for (int c = whole * 8 + first; c < a.hidden; c += step) t = fmaf(from16<kBf16>(x[c]), from16<kBf16>(w[c]), t);
+  return t;
+}
+
+// kRows rows per CTA, side by side in memory; their partials dealt out over the remaining threads, their labels' logits over
+// the warps.
+template <int kRows, int kThreads, bool kBf16>
 __global__ void __launch_bounds__(kThreads) loss_kernel(const Loss a) {
   constexpr int kParts = kThreads / kRows;
   __shared__ float2 stat[kParts][kRows];
-  __shared__ float row_lse[kRows], share[kParts][kRows];
+  __shared__ float row_lse[kRows], share[kParts][kRows], logit[kThreads / 32 / kRows][kRows];
   ptx::grid_dependency_sync();
+  const int active_rows = a.active != nullptr ? *a.active : a.rows;
+  if (a.weight == nullptr) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wr = warp % kRows, wrow = blockIdx.x * kRows + wr;
+    constexpr int kShares = kThreads / 32 / kRows;
+    int label = kNoColumn;
+    if (wrow < active_rows) {
+      if (a.info != nullptr) label = a.info[wrow].label;
+      else if (a.has(wrow)) label = a.has.label(wrow);
+    }
+    float t = label != kNoColumn ? dot_share<kBf16>(a, wrow, label, warp / kRows * 32 + lane, kShares * 32) : 0.0f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    if (lane == 0) logit[warp / kRows][wr] = warp < kRows && a.bias != nullptr && label != kNoColumn ? t + from16<kBf16>(a.bias[label]) : t;
+  }
   const int r = threadIdx.x % kRows, part = threadIdx.x / kRows;
   const int row = blockIdx.x * kRows + r;
-  const bool there = row < (a.active != nullptr ? *a.active : a.rows);
+  const bool there = row < active_rows;
   const int64_t orig = !there ? 0 : a.info != nullptr ? a.info[row].row : row;
   auto join = [](float2 p, float2 q) {
     const float top = fmaxf(p.x, q.x);
@@ -315,13 +373,27 @@ __global__ void __launch_bounds__(kThreads) loss_kernel(const Loss a) {
     if (part < n) stat[part][r] = join(stat[part][r], stat[part + n][r]);
     __syncthreads();
   }
-  if (part == 0) row_lse[r] = fmaf(stat[0][r].x, kLn2, logf(stat[0][r].y));
+  float own = 0.0f;      // the label's logit
+  if (part == 0) {
+    float2 all = stat[0][r];
+    if (a.weight == nullptr) {
+#pragma unroll
+      for (int i = 0; i < kThreads / 32 / kRows; ++i) own += logit[i][r];
+      own *= a.scale;
+      // (an infinite logit has to make the sum infinite, not undefined)
+      const float t2 = own * kLog2E;
+      all = t2 == INFINITY ? make_float2(FLT_MAX, INFINITY) : t2 == -INFINITY ? all : join(all, make_float2(t2, 1.0f));
+    }
+    row_lse[r] = fmaf(all.x, kLn2, logf(all.y));
+  }
   __syncthreads();
   const float lse = row_lse[r];
   float t = 0.0f;
-  if (there) {
+  if (a.weight == nullptr) {
+    if (part == 0) t = lse - own;
+  } else if (there) {
     for (int k = part; k < a.entries; k += kParts) {
-      const float q = a.weight != nullptr ? a.weight[orig * a.entries + k] : 1.0f;
+      const float q = a.weight[orig * a.entries + k];
       if (q != 0.0f) t += q * (logf(q) + (lse - a.at_target[orig * a.entries + k]));   // (0 ln 0 = 0; NaN goes on)
     }
   }
@@ -339,17 +411,6 @@ __global__ void __launch_bounds__(kThreads) loss_kernel(const Loss a) {
 }
 
 // ------------------------------------------------------------------------------------------------ behind the products
-
-template <bool kBf16>
-__device__ __forceinline__ float from16(uint32_t bits) {
-  if constexpr (kBf16) return __uint_as_float(bits << 16);
-  else return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
-}
-template <bool kBf16>
-__device__ __forceinline__ uint32_t to16(float f) {
-  if constexpr (kBf16) return __bfloat16_as_ushort(__float2bfloat16_rn(f));
-  else return __half_as_ushort(__float2half_rn(f));
-}
 
 // dbias of a piece: the sums of G's columns.  256 columns per CTA, kGroups warps that take rows in turn; where the columns alone
 // leave SMs idle the rows are dealt out to gridDim.y CTAs, which leave partial sums for bias_sum_kernel.
@@ -519,7 +580,7 @@ Layout layout_for(const ixk_linear_loss_desc& d, bool backward) {
     l.packed = l.space.take(2 * N * l.ldp);
   }
   if (!backward) {
-    l.at_target = l.space.take(4 * N * K);
+    if (d.entries > 0) l.at_target = l.space.take(4 * N * K);
     l.slots = stat_slots(N, V);
     l.partial = l.space.take(sizeof(float2) * l.slots * N);
     return l;
@@ -733,9 +794,18 @@ int forward(const char* name, const ixk_linear_loss_desc* d, bool distill, const
   a.factor = scales.loss;
   a.loss = loss;
   a.lse = lse;
+  a.x = static_cast<const uint16_t*>(p.x);
+  a.ldx = p.ldx;
+  a.w = static_cast<const uint16_t*>(w);
+  a.ldw = d->w_stride;
+  a.w_column_major = p.w_column_major ? 1 : 0;
+  a.bias = static_cast<const uint16_t*>(bias);
+  a.hidden = static_cast<int>(d->hidden);
+  a.scale = scales.logits;
   auto go = [&](auto rows, auto threads) -> int {
     constexpr int kRows = decltype(rows)::value, kThreads = decltype(threads)::value;
-    return launch_overlapped(loss_kernel<kRows, kThreads>, dim3(static_cast<unsigned>((d->rows + kRows - 1) / kRows)), dim3(kThreads), 0, s, a);
+    auto* fn = d->dtype == IXK_BF16 ? loss_kernel<kRows, kThreads, true> : loss_kernel<kRows, kThreads, false>;
+    return launch_overlapped(fn, dim3(static_cast<unsigned>((d->rows + kRows - 1) / kRows)), dim3(kThreads), 0, s, a);
   };
   // (rows side by side are one read of up to 256 bytes; few rows want a CTA each)
   using std::integral_constant;

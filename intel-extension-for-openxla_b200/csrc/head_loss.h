@@ -43,7 +43,7 @@ struct Pass {
   Targets targets;
   // statistics
   float2* partial;          // [slots][rows]: maximum and sum of exponentials, base 2
-  float* at_target;         // [batch rows][entries]: scaled logits at the targets
+  float* at_target;         // lists: [batch rows][entries]: scaled logits at the targets
   // gradient
   const float* range;       // device: power of two that keeps fp16 in range, nullptr: 1
   void* grad;               // [rows up to a multiple of 256][count] of dtype, pitch ldg

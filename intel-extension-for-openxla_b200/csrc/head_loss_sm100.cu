@@ -2,7 +2,9 @@
 // is turned, where it lies in tensor memory, into what the loss or its gradient needs of it.
 //
 //   statistics   per row the running maximum and sum of exponentials (base 2: t = z log2 e, one fused multiply-add), and
-//                z at the row's targets
+//                z at the columns of a teacher's list; a label's column is left out (the tensor cores cut what an addition
+//                shifts out instead of rounding it: a logit of 10 loses 4e-5 over 4096 products, and the label's is the one
+//                that the loss is made of, so the loss kernel makes it again in fp32)
 //   gradient     G = g (softmax(z) - target weights), rounded once to the 16-bit operand of the two products that
 //                follow (dx = G w, dw = G^T x): a rounding error of 2^-9 or 2^-12 of each entry, as of any activation
 //                gradient, independent from entry to entry
@@ -412,10 +414,15 @@ head_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
                   if (hit) {
                     box_put(box, lane, v);
                     while (walk.next < col_end) {
-                      if (walk.next >= col)
-                        args.at_target[orig * walk.entries + walk.at] = box_read(box_addr(box, lane, walk.next - col)) * args.scale;
+                      if (walk.next >= col) {
+                        const uint32_t addr = box_addr(box, lane, walk.next - col);
+                        // (a label's logit stays out of the sum: the loss adds it, from a product of its own)
+                        if (args.targets.labels != nullptr) box_write(addr, -INFINITY);
+                        else args.at_target[orig * walk.entries + walk.at] = box_read(addr) * args.scale;
+                      }
                       walk.step();
                     }
+                    if (args.targets.labels != nullptr) box_get(box, lane, v);
                   }
                   if (count < 32) {
 #pragma unroll
