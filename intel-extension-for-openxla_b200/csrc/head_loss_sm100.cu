@@ -49,12 +49,18 @@ constexpr int kGroupM = 8;      // row blocks that share a column strip in L2
 constexpr int kAssumedSms = 148;
 constexpr int kMaxStrip = 8;
 constexpr float kLog2E = 1.4426950408889634f;
+// Slabs of K that the tensor cores add up before the statistics' warps take over: their sums cut what an addition shifts out
+// (4e-6 of a logit over K = 4096, always towards zero), the warps' fp32 additions round.  Every chunk is read out of tensor
+// memory, which holds up the next one's products (16 slabs cost 3 % of 4096 x 32768 x 4096, 661 -> 685 us); where the time is
+// that of w's stream, up to one row block, they are shorter.  A tile's chunks are of equal length, at most these.
+constexpr int kChunkSlabs = 24, kShortChunkSlabs = 8;
+enum class Mode { kStats, kStatsChunks, kGrad };     // statistics of one chunk, of several; gradient
 enum : int { kSiteProducer = 601, kSiteFull = 602, kSiteAcc = 603, kSiteEpilogue = 604 };
 
 struct Args {
   int rows, slabs, first, count;        // columns [first, first + count)
   int tiles_n, tile_n, strip, strips;
-  int stages, stage_bytes, a_bytes, b_boxes;
+  int stages, stage_bytes, a_bytes, b_boxes, chunk_slabs;
   int w_mn_major;
   uint32_t idesc;
   const int* active_rows;
@@ -159,10 +165,11 @@ __device__ __forceinline__ Walk start_walk(const Targets& t, const RowInfo& info
   return w;
 }
 
-template <bool kPair, bool kGrad>
+template <bool kPair, Mode kMode>
 __global__ void __launch_bounds__(kThreads, 1)
 head_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
             const __grid_constant__ CUtensorMap tmap_g, const Args args) {
+  constexpr bool kGrad = kMode == Mode::kGrad, kChunks = kMode == Mode::kStatsChunks;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
@@ -298,14 +305,17 @@ head_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
     for (int u = worker; u < num_units && alive; u += workers) {
       int bm, n_begin, n_end;
       unit_at(u, bm, n_begin, n_end);
-      for (int n = n_begin; n < n_end && alive; ++n) {
+      // (accumulators are handed over tile by tile, or chunk by chunk of one)
+      const int chunks = kChunks ? (args.slabs + args.chunk_slabs - 1) / args.chunk_slabs : 1;
+      for (int i = 0; i < (n_end - n_begin) * chunks && alive; ++i) {
         if (!ptx::mbar_wait(acc_empty_bar(buf), acc_phase ^ 1u, ctl, kSiteAcc)) {
           alive = false;
           break;
         }
         ptx::tc_fence_after_sync();
         const uint32_t d_tmem = tmem_base + buf * kMaxTileN;
-        for (int kb = 0; kb < args.slabs; ++kb) {
+        const int slabs = kChunks ? min(args.chunk_slabs, args.slabs - i % chunks * args.chunk_slabs) : args.slabs;
+        for (int kb = 0; kb < slabs; ++kb) {
           if (!ptx::mbar_wait(full_bar(stage), phase, ctl, kSiteFull)) {
             alive = false;
             break;
@@ -381,8 +391,95 @@ head_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
       // (the products read the gradient's rows up to the end of a slab, or of the only row block: zeros)
       const bool work = !kGrad ? warp_row < active_rows
                                : args.rows <= kDirectRows || warp_row < (active_rows + kSlabElems - 1) / kSlabElems * kSlabElems;
+      // 32 columns of the tile from c0 on, `count` of them in the vocabulary, into the row's statistics
+      auto take = [&](float (&v)[32], int col, int count) {
+        const int col_end = col + count;
+        if (args.bias != nullptr) add_bias(args, col, count, v);
+        const bool hit = __any_sync(0xffffffffu, walk.next < col_end);
+        if (hit) {
+          box_put(box, lane, v);
+          while (walk.next < col_end) {
+            if (walk.next >= col) {
+              const uint32_t addr = box_addr(box, lane, walk.next - col);
+              // (a label's logit stays out of the sum: the loss adds it, from a product of its own)
+              if (args.targets.labels != nullptr) box_write(addr, -INFINITY);
+              else args.at_target[orig * walk.entries + walk.at] = box_read(addr) * args.scale;
+            }
+            walk.step();
+          }
+          if (args.targets.labels != nullptr) box_get(box, lane, v);
+        }
+        if (count < 32) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (i >= count) v[i] = -INFINITY;
+        }
+        float m = v[0];
+#pragma unroll
+        for (int i = 1; i < 31; i += 2) m = ptx::max3(m, v[i], v[i + 1]);
+        m = fmaxf(m, v[31]);
+        // (finite, whatever the logits: an infinite one makes the sum infinite, not undefined)
+        const float new_top = fminf(fmaxf(top, m * s2), FLT_MAX);
+        sum *= ptx::ex2_approx(top - new_top);
+        top = new_top;
+        const uint64_t scale_pair = ptx::f32x2(s2, s2), top_pair = ptx::f32x2(-top, -top);
+        uint64_t part0 = ptx::f32x2(0.0f, 0.0f), part1 = part0;
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          float e0, e1, e2, e3;
+          ptx::f32x2_split(ptx::fma2(ptx::f32x2(v[i], v[i + 1]), scale_pair, top_pair), e0, e1);
+          ptx::f32x2_split(ptx::fma2(ptx::f32x2(v[i + 2], v[i + 3]), scale_pair, top_pair), e2, e3);
+          part0 = ptx::add2(part0, ptx::f32x2(ptx::ex2_approx(e0), ptx::ex2_approx(e1)));
+          part1 = ptx::add2(part1, ptx::f32x2(ptx::ex2_approx(e2), ptx::ex2_approx(e3)));
+        }
+        float a, b;
+        ptx::f32x2_split(ptx::add2(part0, part1), a, b);
+        sum += a + b;
+      };
       for (int n = n_begin; n < n_end; ++n) {
         const int n0 = n * args.tile_n, limit = min(args.tile_n, args.count - n0);
+        if constexpr (kChunks) {
+          // the tile's logits chunk of K by chunk, in registers: this warp's two groups of 64 columns
+          float acc[2][64];
+          for (int first = 0; first < args.slabs && alive; first += args.chunk_slabs) {
+            alive = ptx::mbar_wait(acc_full_bar(buf), acc_phase, ctl, kSiteEpilogue);
+            if (!alive) break;
+            ptx::tc_fence_after_sync();
+            if (work) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const int c0 = half * 64 + (q >> 1) * 128 + (q & 1) * 32;
+                if (c0 < limit) {      // warp-uniform
+                  uint32_t r[32];
+                  ptx::tmem_ld_32x32(acc_lane + buf * kMaxTileN + c0, r);
+                  ptx::tmem_ld_wait();
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) {
+                    float& sum_of = acc[q >> 1][(q & 1) * 32 + i];
+                    sum_of = __uint_as_float(r[i]) + (first == 0 ? 0.0f : sum_of);
+                  }
+                }
+              }
+            }
+            ptx::tc_fence_before_sync();
+            if (kPair && rank == 1) ptx::mbar_arrive_cluster_tmem(acc_empty_bar(buf), 0);
+            else ptx::mbar_arrive(acc_empty_bar(buf));
+            buf ^= 1;
+            if (buf == 0) acc_phase ^= 1u;
+          }
+          if (!alive) break;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int c0 = half * 64 + (q >> 1) * 128 + (q & 1) * 32;
+            if (work && c0 < limit) {
+              float v[32];
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = acc[q >> 1][(q & 1) * 32 + i];
+              take(v, args.first + n0 + c0, min(32, limit - c0));
+            }
+          }
+          continue;
+        }
         if (!ptx::mbar_wait(acc_full_bar(buf), acc_phase, ctl, kSiteEpilogue)) {
           alive = false;
           break;
@@ -408,49 +505,11 @@ head_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
                 ptx::tmem_ld_wait();
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-                if (args.bias != nullptr) add_bias(args, col, count, v);
-                const bool hit = __any_sync(0xffffffffu, walk.next < col_end);
                 if constexpr (!kGrad) {
-                  if (hit) {
-                    box_put(box, lane, v);
-                    while (walk.next < col_end) {
-                      if (walk.next >= col) {
-                        const uint32_t addr = box_addr(box, lane, walk.next - col);
-                        // (a label's logit stays out of the sum: the loss adds it, from a product of its own)
-                        if (args.targets.labels != nullptr) box_write(addr, -INFINITY);
-                        else args.at_target[orig * walk.entries + walk.at] = box_read(addr) * args.scale;
-                      }
-                      walk.step();
-                    }
-                    if (args.targets.labels != nullptr) box_get(box, lane, v);
-                  }
-                  if (count < 32) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                      if (i >= count) v[i] = -INFINITY;
-                  }
-                  float m = v[0];
-#pragma unroll
-                  for (int i = 1; i < 31; i += 2) m = ptx::max3(m, v[i], v[i + 1]);
-                  m = fmaxf(m, v[31]);
-                  // (finite, whatever the logits: an infinite one makes the sum infinite, not undefined)
-                  const float new_top = fminf(fmaxf(top, m * s2), FLT_MAX);
-                  sum *= ptx::ex2_approx(top - new_top);
-                  top = new_top;
-                  const uint64_t scale_pair = ptx::f32x2(s2, s2), top_pair = ptx::f32x2(-top, -top);
-                  uint64_t part0 = ptx::f32x2(0.0f, 0.0f), part1 = part0;
-#pragma unroll
-                  for (int i = 0; i < 32; i += 4) {
-                    float e0, e1, e2, e3;
-                    ptx::f32x2_split(ptx::fma2(ptx::f32x2(v[i], v[i + 1]), scale_pair, top_pair), e0, e1);
-                    ptx::f32x2_split(ptx::fma2(ptx::f32x2(v[i + 2], v[i + 3]), scale_pair, top_pair), e2, e3);
-                    part0 = ptx::add2(part0, ptx::f32x2(ptx::ex2_approx(e0), ptx::ex2_approx(e1)));
-                    part1 = ptx::add2(part1, ptx::f32x2(ptx::ex2_approx(e2), ptx::ex2_approx(e3)));
-                  }
-                  float a, b;
-                  ptx::f32x2_split(ptx::add2(part0, part1), a, b);
-                  sum += a + b;
+                  take(v, col, count);
                 } else {
+                  if (args.bias != nullptr) add_bias(args, col, count, v);
+                  const bool hit = __any_sync(0xffffffffu, walk.next < col_end);
                   const uint64_t scale_pair = ptx::f32x2(s2, s2), lse_pair = ptx::f32x2(-lse2, -lse2);
 #pragma unroll
                   for (int i = 0; i < 32; i += 2) {
@@ -595,6 +654,8 @@ int launch(const Pass& p, const DeviceInfo& dev, cudaStream_t stream) {
   Args a{};
   a.rows = static_cast<int>(p.rows);
   a.slabs = static_cast<int>((p.hidden + kSlabElems - 1) / kSlabElems);
+  const int most = p.rows <= kDirectRows ? kShortChunkSlabs : kChunkSlabs, chunks = (a.slabs + most - 1) / most;
+  a.chunk_slabs = (a.slabs + chunks - 1) / chunks;
   a.first = static_cast<int>(p.first);
   a.count = static_cast<int>(p.count);
   a.tiles_n = t.tiles_n;
@@ -625,9 +686,10 @@ int launch(const Pass& p, const DeviceInfo& dev, cudaStream_t stream) {
 
   const int64_t tile_rows = t.pair ? 2 * kBlockM : kBlockM;
   const int64_t units = (p.rows + tile_rows - 1) / tile_rows * t.strips;
-  auto go = [&](auto pair_tag) -> int {
+  auto go = [&](auto pair_tag, auto mode_tag) -> int {
     constexpr bool kPair = decltype(pair_tag)::value;
-    auto* fn = &head_kernel<kPair, kGrad>;
+    constexpr Mode kMode = decltype(mode_tag)::value;
+    auto* fn = &head_kernel<kPair, kMode>;
     static thread_local int configured_device = -1;
     if (configured_device != dev.device) {
       IXK_CUDA_OK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
@@ -652,7 +714,13 @@ int launch(const Pass& p, const DeviceInfo& dev, cudaStream_t stream) {
     count_launch();
     return IXK_OK;
   };
-  return t.pair ? go(std::true_type{}) : go(std::false_type{});
+  using std::integral_constant;
+  constexpr integral_constant<Mode, kGrad ? Mode::kGrad : Mode::kStats> kOne;
+  if constexpr (!kGrad) {
+    constexpr integral_constant<Mode, Mode::kStatsChunks> kMany;
+    if (a.slabs > a.chunk_slabs) return t.pair ? go(std::true_type{}, kMany) : go(std::false_type{}, kMany);
+  }
+  return t.pair ? go(std::true_type{}, kOne) : go(std::false_type{}, kOne);
 }
 
 }  // namespace

@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kWarp ? 256 : kMaxThreads, 1) row_norm_fwd_ker
       }
     }
     row_sums<kWarp, 1>(s, scratch, turn);
-    const float rstd = rsqrtf(fmaf(s[0], a.inv_cols, a.eps));
+    const float rstd = __frsqrt_rn(fmaf(s[0], a.inv_cols, a.eps));
     T* out = static_cast<T*>(a.out) + row * a.ldo;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(128) row_norm_fwd_rows_kernel(const Args a) {
     }
     warp_sums<kRows>(s);
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) s[r] = rsqrtf(fmaf(s[r], a.inv_cols, a.eps));
+    for (int r = 0; r < kRows; ++r) s[r] = __frsqrt_rn(fmaf(s[r], a.inv_cols, a.eps));
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int v = lane + 32 * i;
@@ -910,7 +910,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) row_norm_fwd_ring_kernel(cons
     for (int r = 0; r < kRows; ++r) {
       if (r < there) {
         const int64_t row = static_cast<int64_t>(batch) * kRows + r;
-        const float rstd = rsqrtf(fmaf(s[r], a.inv_cols, a.eps));
+        const float rstd = __frsqrt_rn(fmaf(s[r], a.inv_cols, a.eps));
         const uint64_t r2 = ptx::f32x2(rstd, rstd);
 #pragma unroll
         for (int j = 0; j < kRingPairs; ++j) x[r][j] = ptx::fma2(ptx::mul2(x[r][j], r2), scale[j], shift[j]);
