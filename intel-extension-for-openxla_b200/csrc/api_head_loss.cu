@@ -297,7 +297,8 @@ struct Loss {
   int rows, slots, entries;
   float factor;
   float *loss, *lse;
-  // labels: the label's logit, scale (x . w[label] + bias[label]), is made here (and left out of the partials)
+  // labels apart: the label's logit, scale (x . w[label] + bias[label]), is made here (and left out of the partials)
+  int apart;
   const uint16_t *x, *w, *bias;
   int64_t ldx, ldw;
   int hidden, w_column_major;
@@ -341,7 +342,7 @@ __global__ void __launch_bounds__(kThreads) loss_kernel(const Loss a) {
   __shared__ float row_lse[kRows], share[kParts][kRows], logit[kThreads / 32 / kRows][kRows];
   ptx::grid_dependency_sync();
   const int active_rows = a.active != nullptr ? *a.active : a.rows;
-  if (a.weight == nullptr) {
+  if (a.apart) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wr = warp % kRows, wrow = blockIdx.x * kRows + wr;
     constexpr int kShares = kThreads / 32 / kRows;
     int label = kNoColumn;
@@ -376,7 +377,7 @@ __global__ void __launch_bounds__(kThreads) loss_kernel(const Loss a) {
   float own = 0.0f;      // the label's logit
   if (part == 0) {
     float2 all = stat[0][r];
-    if (a.weight == nullptr) {
+    if (a.apart) {
 #pragma unroll
       for (int i = 0; i < kThreads / 32 / kRows; ++i) own += logit[i][r];
       own *= a.scale;
@@ -389,11 +390,11 @@ __global__ void __launch_bounds__(kThreads) loss_kernel(const Loss a) {
   __syncthreads();
   const float lse = row_lse[r];
   float t = 0.0f;
-  if (a.weight == nullptr) {
+  if (a.apart) {
     if (part == 0) t = lse - own;
   } else if (there) {
     for (int k = part; k < a.entries; k += kParts) {
-      const float q = a.weight[orig * a.entries + k];
+      const float q = a.weight != nullptr ? a.weight[orig * a.entries + k] : 1.0f;
       if (q != 0.0f) t += q * (logf(q) + (lse - a.at_target[orig * a.entries + k]));   // (0 ln 0 = 0; NaN goes on)
     }
   }
@@ -561,6 +562,9 @@ int64_t bias_parts(int64_t columns, int64_t rows) {
   return std::clamp<int64_t>(std::min<int64_t>(148 / blocks, rows / (4 * kBiasGroups)), 1, kBiasParts);
 }
 
+// Whether the label's logit is a product of its own: one row of w each, or, column-major, a 32-byte sector an element, which
+// only few rows can pay (7355 x 3520 x 8144: 270 of 1700 us).
+bool labels_apart(const ixk_linear_loss_desc& d) { return d.w_order == IXK_ROW_MAJOR || d.rows <= kDirectRows; }
 int64_t starts_of(int64_t vocab) { return (vocab + kStartUnit - 1) / kStartUnit; }
 
 Layout layout_for(const ixk_linear_loss_desc& d, bool backward) {
@@ -580,7 +584,7 @@ Layout layout_for(const ixk_linear_loss_desc& d, bool backward) {
     l.packed = l.space.take(2 * N * l.ldp);
   }
   if (!backward) {
-    if (d.entries > 0) l.at_target = l.space.take(4 * N * K);
+    if (d.entries > 0 || !labels_apart(d)) l.at_target = l.space.take(4 * N * K);
     l.slots = stat_slots(N, V);
     l.partial = l.space.take(sizeof(float2) * l.slots * N);
     return l;
@@ -675,6 +679,7 @@ int targets_of(const ixk_linear_loss_desc& d, const Layout& l, char* ws, const v
   has->ignore_index = d.ignore_index;
   if (teacher == nullptr) {
     t->labels = has->labels = index;
+    t->apart = labels_apart(d) ? 1 : 0;
     t->entries = 1;
     return IXK_OK;
   }
@@ -794,6 +799,7 @@ int forward(const char* name, const ixk_linear_loss_desc* d, bool distill, const
   a.factor = scales.loss;
   a.loss = loss;
   a.lse = lse;
+  a.apart = t.apart;
   a.x = static_cast<const uint16_t*>(p.x);
   a.ldx = p.ldx;
   a.w = static_cast<const uint16_t*>(w);

@@ -14,6 +14,7 @@ struct Targets {
   const void* labels;       // cross entropy: [rows], int32 or int64; nullptr: lists
   int wide;                 // 64-bit labels
   int64_t ignore_index;
+  int apart;                // statistics: the label's column is left out of the sum, the caller makes its logit
   const int* column;        // distillation: [rows][entries] ascending, kNoColumn behind the last one
   const float* weight;      // [rows][entries]
   const uint16_t* start;    // [rows][starts]: the first entry at or behind column i * kStartUnit
@@ -43,7 +44,7 @@ struct Pass {
   Targets targets;
   // statistics
   float2* partial;          // [slots][rows]: maximum and sum of exponentials, base 2
-  float* at_target;         // lists: [batch rows][entries]: scaled logits at the targets
+  float* at_target;         // [batch rows][entries]: scaled logits at the targets (not of labels apart)
   // gradient
   const float* range;       // device: power of two that keeps fp16 in range, nullptr: 1
   void* grad;               // [rows up to a multiple of 256][count] of dtype, pitch ldg

@@ -2,9 +2,9 @@
 // is turned, where it lies in tensor memory, into what the loss or its gradient needs of it.
 //
 //   statistics   per row the running maximum and sum of exponentials (base 2: t = z log2 e, one fused multiply-add), and
-//                z at the columns of a teacher's list; a label's column is left out (the tensor cores cut what an addition
-//                shifts out instead of rounding it: a logit of 10 loses 4e-5 over 4096 products, and the label's is the one
-//                that the loss is made of, so the loss kernel makes it again in fp32)
+//                z at the row's targets; a label's column can be left out (the tensor cores cut what an addition shifts out
+//                instead of rounding it: a logit of 10 loses 4e-5 over 4096 products, and the label's is the one that the
+//                loss is made of, so the loss kernel makes it again in fp32 where that is a row of w to read)
 //   gradient     G = g (softmax(z) - target weights), rounded once to the 16-bit operand of the two products that
 //                follow (dx = G w, dw = G^T x): a rounding error of 2^-9 or 2^-12 of each entry, as of any activation
 //                gradient, independent from entry to entry
@@ -51,9 +51,9 @@ constexpr int kMaxStrip = 8;
 constexpr float kLog2E = 1.4426950408889634f;
 // Slabs of K that the tensor cores add up before the statistics' warps take over: their sums cut what an addition shifts out
 // (4e-6 of a logit over K = 4096, always towards zero), the warps' fp32 additions round.  Every chunk is read out of tensor
-// memory, which holds up the next one's products (16 slabs cost 3 % of 4096 x 32768 x 4096, 661 -> 685 us); where the time is
-// that of w's stream, up to one row block, they are shorter.  A tile's chunks are of equal length, at most these.
-constexpr int kChunkSlabs = 24, kShortChunkSlabs = 8;
+// memory, which holds up the next one's products (16 slabs cost 3 % of 4096 x 32768 x 4096, 661 -> 685 us).  A tile's chunks are
+// of equal length, at most this.
+constexpr int kChunkSlabs = 24;
 enum class Mode { kStats, kStatsChunks, kGrad };     // statistics of one chunk, of several; gradient
 enum : int { kSiteProducer = 601, kSiteFull = 602, kSiteAcc = 603, kSiteEpilogue = 604 };
 
@@ -401,13 +401,13 @@ head_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
           while (walk.next < col_end) {
             if (walk.next >= col) {
               const uint32_t addr = box_addr(box, lane, walk.next - col);
-              // (a label's logit stays out of the sum: the loss adds it, from a product of its own)
-              if (args.targets.labels != nullptr) box_write(addr, -INFINITY);
+              // (a label apart stays out of the sum: the loss adds it, from a product of its own)
+              if (args.targets.apart) box_write(addr, -INFINITY);
               else args.at_target[orig * walk.entries + walk.at] = box_read(addr) * args.scale;
             }
             walk.step();
           }
-          if (args.targets.labels != nullptr) box_get(box, lane, v);
+          if (args.targets.apart) box_get(box, lane, v);
         }
         if (count < 32) {
 #pragma unroll
@@ -654,7 +654,7 @@ int launch(const Pass& p, const DeviceInfo& dev, cudaStream_t stream) {
   Args a{};
   a.rows = static_cast<int>(p.rows);
   a.slabs = static_cast<int>((p.hidden + kSlabElems - 1) / kSlabElems);
-  const int most = p.rows <= kDirectRows ? kShortChunkSlabs : kChunkSlabs, chunks = (a.slabs + most - 1) / most;
+  const int chunks = (a.slabs + kChunkSlabs - 1) / kChunkSlabs;
   a.chunk_slabs = (a.slabs + chunks - 1) / chunks;
   a.first = static_cast<int>(p.first);
   a.count = static_cast<int>(p.count);
