@@ -166,7 +166,7 @@ struct Control {
   int plane_slabs;     // slabs of the vocabulary's piece per plane of dx (gemm::two_plan), and the planes
   int planes;
   int pad;
-  float range[2];      // power of two for fp16's gradient, and its inverse
+  float range[2];      // what G is multiplied by, and the inverse
 };
 
 struct Gather {
@@ -179,11 +179,14 @@ struct Gather {
   RowInfo* info;
   int* inverse;                // may be nullptr
   float *loss, *lse;           // zeroed where there is no target; may be nullptr
-  // backward: control's range is the power of two that brings the largest row's gradient to 2^13 .. 2^14
+  // backward: G is made of grad_loss over its largest size in the batch.  With equal grad_loss, a mean, a label's entry is then
+  // p - 1, which 16 bits hold well where p is small, and not (p - 1) / tokens, whose rounding error every row shares (3.9e-3 of
+  // the gradient in the worst case); times `top` (fp16: 2^13), as G = g (p - q) with g = 1 / tokens and p = 1 / vocabulary
+  // would be lost below fp16's smallest numbers.
   const float *lse_in, *grad_loss;
   int64_t grad_stride;
   float factor;
-  int ranged;
+  float top;                   // 0: forward
   // and the products' plan: tiles of a row block of dx, of dw; slabs of a piece
   int dx_tiles_n, piece_slabs, dw_tiles, pairs, max_planes;
 };
@@ -213,8 +216,16 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Gather a) 
   const bool keep = mine && a.has(row);
   // every CTA counts the rows in front of its own
   int before = 0;
+  float largest = 0.0f;        // (the last CTA: of grad_loss)
+  const bool ranges = a.top > 0.0f && end == a.rows;
 #pragma unroll 4
-  for (int i = threadIdx.x; i < first; i += kGatherThreads) before += a.has(i);
+  for (int i = threadIdx.x; i < first; i += kGatherThreads) {
+    const float g = ranges ? fabsf(a.grad_loss[i * a.grad_stride] * a.factor) : 0.0f;
+    if (a.has(i)) {
+      ++before;
+      largest = fmaxf(largest, g);
+    }
+  }
   before = block_sum(before);
   const unsigned ballot = __ballot_sync(0xffffffffu, keep);
   const int here = block_sum(lane == 0 ? __popc(ballot) : 0);
@@ -228,6 +239,7 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Gather a) 
       if (a.grad_loss != nullptr) {
         info.lse2 = a.lse_in[row] * kLog2E;
         info.coef = a.grad_loss[row * a.grad_stride] * a.factor;
+        largest = fmaxf(largest, fabsf(info.coef));
       }
       a.info[before + at] = info;
     } else if (a.loss != nullptr) {
@@ -267,20 +279,16 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Gather a) 
   const int zero_end = a.rows <= kDirectRows ? a.rows : min((total + kSlabRows - 1) / kSlabRows * kSlabRows, a.rows);
   for (int i = total + warp; i < zero_end; i += kGatherThreads / 32)
     for (int c = lane; c < a.hidden; c += 32) a.packed[i * a.ldp + c] = 0;
-  if (a.ranged) {
-    float top = 0.0f;
-    for (int i = threadIdx.x; i < a.rows; i += kGatherThreads)
-      if (a.has(i)) top = fmaxf(top, fabsf(a.grad_loss[i * a.grad_stride] * a.factor));
+  if (ranges) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) warp_top[warp] = top;
+    for (int o = 16; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+    if (lane == 0) warp_top[warp] = largest;
     __syncthreads();
     if (threadIdx.x == 0) {
-      for (int w = 0; w < kGatherThreads / 32; ++w) top = fmaxf(top, warp_top[w]);
-      int e = 0;
-      if (top >= FLT_MIN && top <= FLT_MAX) e = min(13 - ilogbf(top), 126);
-      a.control->range[0] = scalbnf(1.0f, e);
-      a.control->range[1] = scalbnf(1.0f, -e);
+      for (int w = 0; w < kGatherThreads / 32; ++w) largest = fmaxf(largest, warp_top[w]);
+      const bool fit = largest >= 0x1p-100f && largest <= 0x1p100f;      // (both quotients are finite)
+      a.control->range[0] = fit ? a.top / largest : 1.0f;
+      a.control->range[1] = fit ? largest / a.top : 1.0f;
     }
   }
 }
@@ -448,7 +456,7 @@ __global__ void __launch_bounds__(32 * kGroups) bias_kernel(const uint16_t* g, i
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) s += sums[i][col];
     if (gridDim.y > 1) partial[static_cast<int64_t>(blockIdx.y) * count + c] = s;
-    else out[c] = static_cast<uint16_t>(to16<kBf16>(kBf16 ? s : s * control->range[1]));
+    else out[c] = static_cast<uint16_t>(to16<kBf16>(s * control->range[1]));
   }
 }
 template <bool kBf16>
@@ -459,7 +467,7 @@ __global__ void __launch_bounds__(128) bias_sum_kernel(const float* partial, int
   float s = 0.0f;
 #pragma unroll 8
   for (int i = 0; i < parts; ++i) s += partial[static_cast<int64_t>(i) * count + c];
-  out[c] = static_cast<uint16_t>(to16<kBf16>(kBf16 ? s : s * control->range[1]));
+  out[c] = static_cast<uint16_t>(to16<kBf16>(s * control->range[1]));
 }
 
 // dx: the accumulator's rows, their planes added up, back to where they came from, rounded once; zeros where there was no
@@ -470,7 +478,7 @@ __global__ void __launch_bounds__(256) scatter_kernel(const float* acc, int64_t 
   ptx::grid_dependency_sync();
   const int64_t row = blockIdx.x;
   const int from = inverse[row], planes = control->planes;
-  const float scale = kBf16 ? 1.0f : control->range[1];
+  const float scale = control->range[1];
   const float* src = acc + from * ld_acc;
   uint16_t* dst = dx + row * ld;
   const int vecs = vec ? hidden / 8 : 0;
@@ -530,7 +538,7 @@ __global__ void __launch_bounds__(32 * kFewPlaneGroups) scatter_few_kernel(const
 #pragma unroll
     for (int i = 0; i < kFewPlaneGroups; ++i) s += sums[i][threadIdx.x];
   }
-  dx[row * ld + c] = static_cast<uint16_t>(to16<kBf16>(kBf16 ? s : s * control->range[1]));
+  dx[row * ld + c] = static_cast<uint16_t>(to16<kBf16>(s * control->range[1]));
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -727,7 +735,7 @@ int gather(const ixk_linear_loss_desc& d, const Layout& l, char* ws, const HasTa
   g.grad_loss = grad_loss;
   g.grad_stride = d.grad_loss_stride;
   g.factor = factor;
-  g.ranged = backward && d.dtype == IXK_F16;
+  g.top = !backward ? 0.0f : d.dtype == IXK_F16 ? 0x1p13f : 1.0f;
   if (backward && d.rows > kDirectRows) {
     g.dx_tiles_n = static_cast<int>((d.hidden + gemm::kTwoTile - 1) / gemm::kTwoTile);
     g.piece_slabs = static_cast<int>((l.piece + kSlabRows - 1) / kSlabRows);
@@ -850,13 +858,12 @@ int backward(const char* name, const ixk_linear_loss_desc* d, bool distill, cons
   Targets t{};
   HasTarget has{};
   if ((rc = targets_of(*d, l, ws, index, teacher, s, &t, &has)) != IXK_OK) return rc;
-  // fp16: G = g (p - q) with g = 1 / tokens and p = 1 / vocabulary would be lost below its smallest numbers
   if ((rc = gather(*d, l, ws, has, x, nullptr, nullptr, lse, grad_loss, scales.grad, dw != nullptr, dev.sm_count, s)) != IXK_OK) return rc;
   Pass p = pass_of(*d, scales, ws + l.packed, l.ldp, w, bias, t);
   const Control* control = reinterpret_cast<const Control*>(ws + l.control);
   p.active_rows = &control->active;
   p.info = reinterpret_cast<const RowInfo*>(ws + l.info);
-  p.range = bf16 ? nullptr : control->range;
+  p.range = control->range;
   p.grad = ws + l.grad;
   p.ldg = l.ldg;
   float* acc = reinterpret_cast<float*>(ws + l.acc);
@@ -903,7 +910,7 @@ int backward(const char* name, const ixk_linear_loss_desc* d, bool distill, cons
       g.d = static_cast<uint16_t*>(dw) + (row_major ? first * d->dw_stride : first);
       g.ldd = g.ldc = d->dw_stride;
       g.out_dtype = d->dtype;
-      g.acc_scale_dev = p.range != nullptr ? p.range + 1 : nullptr;
+      g.acc_scale_dev = p.range + 1;
     }
     if (both[1].M > 0) both[1].k_limit = p.active_rows;
     if (d->rows <= kDirectRows && both[0].M > 0) {      // one row block: dx is a stream of the weights

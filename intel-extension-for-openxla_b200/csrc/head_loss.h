@@ -46,7 +46,7 @@ struct Pass {
   float2* partial;          // [slots][rows]: maximum and sum of exponentials, base 2
   float* at_target;         // [batch rows][entries]: scaled logits at the targets (not of labels apart)
   // gradient
-  const float* range;       // device: power of two that keeps fp16 in range, nullptr: 1
+  const float* range;       // device: what the gradient is multiplied by
   void* grad;               // [rows up to a multiple of 256][count] of dtype, pitch ldg
   int64_t ldg;
 };

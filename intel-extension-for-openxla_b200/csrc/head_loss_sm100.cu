@@ -355,7 +355,7 @@ head_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
     int buf = 0;
     uint32_t acc_phase = 0;
     bool alive = true;
-    const float range = kGrad && args.range != nullptr ? *args.range : 1.0f;
+    const float range = kGrad ? *args.range : 1.0f;
     int warp_row = 0, n_begin = 0, n_end = 0;
     RowInfo info{0, kNoColumn, 0.0f, 0.0f};
     // a unit's place, and what is to be known of this thread's row (asked for a unit ahead of its use)

@@ -66,8 +66,6 @@ __device__ __forceinline__ Raw<T, kVec> pack(const float (&f)[kVec]) {
 // The compiler may not keep what it unpacked of `raw` beyond this point: registers hold the row as it lies in memory, not
 // twice as many floats (bf16 at 16 vectors a lane: 164 registers with, 255 and spills without at 32).
 __device__ __forceinline__ void forget(uint4& raw) { asm volatile("" : "+r"(raw.x), "+r"(raw.y), "+r"(raw.z), "+r"(raw.w)); }
-__device__ __forceinline__ void forget(uint32_t& raw) { asm volatile("" : "+r"(raw)); }
-__device__ __forceinline__ void forget(uint16_t& raw) { asm volatile("" : "+h"(raw)); }
 __device__ __forceinline__ float load_param(const void* p, int64_t i, int dtype) {
   if (dtype == IXK_F32) return static_cast<const float*>(p)[i];
   if (dtype == IXK_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);

@@ -347,3 +347,24 @@ def test_refusals(pkg, cuda):
                  lambda: pkg.linear_cross_entropy_backward(x, w, labels, lse, g, workspace=torch.empty(1024, dtype=torch.uint8, device=cuda))):
         with pytest.raises(pkg.IxkError):
             call()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("N", [100, 300])
+def test_a_mean_leaves_the_labels_entry_whole(pkg, cuda, dtype, N):
+    """With equal grad_loss a label's entry is p - 1 before its rounding, whose error is then at most p where p is small: 1 / N is
+    not rounded with it."""
+    V = 4096
+    gen, x, w, b, g = head(N, 64, V, DT[dtype], cuda)
+    x = x * 0.0625      # (p about 1 / 4096)
+    labels = torch.randint(0, V, (N,), generator=gen).to(cuda)
+    g = torch.full((N,), 1.0 / N, device=cuda)
+    loss, lse = pkg.linear_cross_entropy(x, w, labels)
+    dx, dw = pkg.linear_cross_entropy_backward(x, w, labels, lse, g)[:2]
+    r = reference(x, w, None, *one_hot_args(labels, V), 1.0, 1.0, g)
+    u = U[DT[dtype]]
+    dG = r["gg"] * (r["p"] * (2 * r["dz"][:, None] + 2.0 ** -18) + 2.0 ** -20 * r["Q"]) + u * r["gg"] * r["p"] + 2.0 ** -37 * r["gg"]
+    assert r["p"].max() < 2.0 ** -10
+    tiny = 2.0 ** -25 if dtype == "fp16" else 0.0
+    within("dx", dx, r["dx"], u * r["dx"].abs() + dG @ r["w"].abs() + (V + 64) * E * (r["G"].abs() @ r["w"].abs()) + tiny + r["gg"] * (r["p"] * r["Q"]).sum(1, keepdim=True) * r["w"].abs()[labels])
+    within("dw", dw, r["dw"], u * r["dw"].abs() + (dG + r["gg"] * r["p"] * r["Q"]).t() @ r["x"].abs() + (N + 64) * E * (r["G"].abs().t() @ r["x"].abs()) + tiny)
