@@ -150,10 +150,10 @@ struct HasTarget {
   const int* has;
   int wide, vocab;
   int64_t ignore_index;
+  __device__ __forceinline__ bool counts(int64_t l) const { return l != ignore_index && l >= 0 && l < vocab; }
   __device__ __forceinline__ bool operator()(int64_t row) const {
     if (labels == nullptr) return has[row] != 0;
-    const int64_t l = wide ? static_cast<const int64_t*>(labels)[row] : static_cast<const int*>(labels)[row];
-    return l != ignore_index && l >= 0 && l < vocab;
+    return counts(wide ? static_cast<const int64_t*>(labels)[row] : static_cast<const int*>(labels)[row]);
   }
   __device__ __forceinline__ int label(int64_t row) const {      // of a row that has one
     return wide ? static_cast<int>(static_cast<const int64_t*>(labels)[row]) : static_cast<const int*>(labels)[row];
@@ -192,7 +192,7 @@ struct Gather {
 };
 
 constexpr int kGatherThreads = 256;
-constexpr int kCopyVecs = 8;
+constexpr int kCopyVecs = 8, kCountAtOnce = 8;
 
 __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Gather a) {
   __shared__ int warp_count[kGatherThreads / 32];
@@ -218,14 +218,29 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Gather a) 
   int before = 0;
   float largest = 0.0f;        // (the last CTA: of grad_loss)
   const bool ranges = a.top > 0.0f && end == a.rows;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < first; i += kGatherThreads) {
-    const float g = ranges ? fabsf(a.grad_loss[i * a.grad_stride] * a.factor) : 0.0f;
-    if (a.has(i)) {
-      ++before;
-      largest = fmaxf(largest, g);
+  auto count = [&](const auto* targets, auto none, auto test) {
+    for (int i0 = threadIdx.x; i0 < first; i0 += kCountAtOnce * kGatherThreads) {
+      decltype(none) t[kCountAtOnce];      // (all loads out before the first test)
+      float g[kCountAtOnce];
+#pragma unroll
+      for (int j = 0; j < kCountAtOnce; ++j) {
+        const int i = i0 + j * kGatherThreads;
+        t[j] = i < first ? targets[i] : none;
+        g[j] = ranges && i < first ? a.grad_loss[i * a.grad_stride] : 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < kCountAtOnce; ++j) {
+        if (test(t[j])) {
+          ++before;
+          largest = fmaxf(largest, fabsf(g[j] * a.factor));
+        }
+      }
     }
-  }
+  };
+  const auto is_label = [&](int64_t l) { return a.has.counts(l); };
+  if (a.has.labels == nullptr) count(a.has.has, 0, [](int h) { return h != 0; });
+  else if (a.has.wide) count(static_cast<const int64_t*>(a.has.labels), int64_t(-1), is_label);
+  else count(static_cast<const int*>(a.has.labels), -1, is_label);
   before = block_sum(before);
   const unsigned ballot = __ballot_sync(0xffffffffu, keep);
   const int here = block_sum(lane == 0 ? __popc(ballot) : 0);
@@ -267,11 +282,11 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Gather a) 
   if (end != a.rows) return;
   // the last CTA: how many there are, zeros behind them as far as the products read, and the gradient's range
   const int total = before + here;
-  if (threadIdx.x == 0) {
-    a.control->active = total;
-    if (a.dx_tiles_n > 0) {
-      const int64_t tiles = (static_cast<int64_t>(total) + gemm::kTwoTile - 1) / gemm::kTwoTile * a.dx_tiles_n;
-      const int slabs = gemm::two_plan(tiles, a.piece_slabs, a.dw_tiles, max((total + kSlabRows - 1) / kSlabRows, 1), a.pairs, a.max_planes);
+  if (threadIdx.x == 0) a.control->active = total;
+  if (warp == 0 && a.dx_tiles_n > 0) {
+    const int64_t tiles = (static_cast<int64_t>(total) + gemm::kTwoTile - 1) / gemm::kTwoTile * a.dx_tiles_n;
+    const int slabs = gemm::two_plan(tiles, a.piece_slabs, a.dw_tiles, max((total + kSlabRows - 1) / kSlabRows, 1), a.pairs, a.max_planes);
+    if (lane == 0) {
       a.control->plane_slabs = slabs;
       a.control->planes = (a.piece_slabs + slabs - 1) / slabs;
     }
@@ -471,18 +486,20 @@ __global__ void __launch_bounds__(128) bias_sum_kernel(const float* partial, int
 }
 
 // dx: the accumulator's rows, their planes added up, back to where they came from, rounded once; zeros where there was no
-// target.
+// target.  `width` threads a row.
 template <bool kBf16>
 __global__ void __launch_bounds__(256) scatter_kernel(const float* acc, int64_t ld_acc, int64_t plane, const int* inverse, const Control* control,
-                                                      int hidden, int vec, uint16_t* dx, int64_t ld) {
+                                                      int rows, int hidden, int vec, int width, uint16_t* dx, int64_t ld) {
   ptx::grid_dependency_sync();
-  const int64_t row = blockIdx.x;
+  const int in = threadIdx.x / width, thread = threadIdx.x % width, per_cta = blockDim.x / width;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * per_cta + in;
+  if (in >= per_cta || row >= rows) return;
   const int from = inverse[row], planes = control->planes;
   const float scale = control->range[1];
   const float* src = acc + from * ld_acc;
   uint16_t* dst = dx + row * ld;
   const int vecs = vec ? hidden / 8 : 0;
-  for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
+  for (int v = thread; v < vecs; v += width) {
     uint4 w = make_uint4(0, 0, 0, 0);
     if (from >= 0) {
       float4 a = reinterpret_cast<const float4*>(src)[2 * v], b = reinterpret_cast<const float4*>(src)[2 * v + 1];
@@ -499,7 +516,7 @@ __global__ void __launch_bounds__(256) scatter_kernel(const float* acc, int64_t 
     }
     reinterpret_cast<uint4*>(dst)[v] = w;
   }
-  for (int c = vecs * 8 + threadIdx.x; c < hidden; c += blockDim.x) {
+  for (int c = vecs * 8 + thread; c < hidden; c += width) {
     float t = 0.0f;
     if (from >= 0) {
 #pragma unroll 8
@@ -893,6 +910,7 @@ int backward(const char* name, const ixk_linear_loss_desc* d, bool distill, cons
       g.c = acc;
       g.ldd = g.ldc = l.ld_acc;
       g.d_batch_stride = g.c_batch_stride = l.plane;
+      if (d->rows > kDirectRows) g.batch = l.planes;
       g.out_dtype = IXK_F32;
       g.beta = first == 0 ? 0.0f : 1.0f;
     }
@@ -945,9 +963,10 @@ int backward(const char* name, const ixk_linear_loss_desc* d, bool distill, cons
                              static_cast<const float*>(acc), l.ld_acc, l.plane, std::max(l.planes, 1), inverse, control, static_cast<int>(d->hidden),
                              static_cast<uint16_t*>(dx), d->dx_stride);
   const int vec = aligned(dx, 16) && d->dx_stride % 8 == 0;
-  return launch_overlapped(bf16 ? scatter_kernel<true> : scatter_kernel<false>, dim3(static_cast<unsigned>(d->rows)), dim3(256), 0, s,
-                           static_cast<const float*>(acc), l.ld_acc, l.plane, inverse, control, static_cast<int>(d->hidden), vec,
-                           static_cast<uint16_t*>(dx), d->dx_stride);
+  const int width = static_cast<int>(std::min<int64_t>(round_up(vec ? d->hidden / 8 : d->hidden, 32), 256));
+  return launch_overlapped(bf16 ? scatter_kernel<true> : scatter_kernel<false>, dim3(static_cast<unsigned>((d->rows + 256 / width - 1) / (256 / width))),
+                           dim3(256), 0, s, static_cast<const float*>(acc), l.ld_acc, l.plane, inverse, control, static_cast<int>(d->rows),
+                           static_cast<int>(d->hidden), vec, width, static_cast<uint16_t*>(dx), d->dx_stride);
 }
 
 }  // namespace

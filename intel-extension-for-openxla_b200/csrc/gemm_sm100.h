@@ -86,8 +86,8 @@ int run_problem(const Problem& p, void* workspace, size_t workspace_bytes, const
 size_t problem_workspace_bytes(int64_t M, int64_t N, int64_t K);
 
 // Two products in one launch, for the gradients of a layer whose weight is much longer one way than the other:
-//   p[0]  D0 (+)= A0.B0, fp32, few tiles and a long K: cut along K into planes, d_batch_stride elements apart, which the
-//         caller adds up; beta 0 or 1 with c = d
+//   p[0]  D0 (+)= A0.B0, fp32, unscaled, few tiles and a long K: cut along K into planes (at most `batch`), d_batch_stride
+//         elements apart, which the caller adds up; beta 0 or 1 with c = d; rows of whole 16-byte pieces
 //   p[1]  D1 = A1.B1, many tiles and a short K
 // Either may be absent (M = 0).  The pairs of CTAs that have one unit less of the long product begin with the other's tiles,
 // so that all end together.  `plan` (device): the slabs of K per plane, from two_plan.  16-bit operands; p[0].m_limit and
@@ -95,22 +95,25 @@ size_t problem_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int launch_two(const Problem (&p)[2], const int* plan, const DeviceInfo& dev, cudaStream_t stream);
 constexpr int kTwoTile = 256;    // of either product
 
-// Slabs of 64 of the long product's K per plane: as few planes as let the longest pair's share of it end with the whole.
-// tiles and slabs: of the long product (0), of the other (1).
-__host__ __device__ inline int two_plan(int64_t tiles0, int slabs0, int64_t tiles1, int slabs1, int pairs, int max_planes) {
+// Slabs of 64 of the long product's K per plane: as few planes as let the longest pair's share of it end with the whole, of 8
+// slabs or more (at least 16: 3 of 14 to 50 us more where it matters; 4: no further gain).
+// tiles and slabs: of the long product (0), of the other (1).  Called by a whole warp: a lane looks at as many planes as its
+// number says, one after the other these divisions took 2 us.
+__device__ inline int two_plan(int64_t tiles0, int slabs0, int64_t tiles1, int slabs1, int pairs, int max_planes) {
   const int64_t share = (tiles0 * slabs0 + tiles1 * slabs1 + pairs - 1) / pairs;
-  int best = slabs0;
-  int64_t best_time = 0;
-  for (int s = 1; s <= max_planes && (s == 1 || slabs0 / s >= 16); ++s) {
-    const int chunk = (slabs0 + s - 1) / s, planes = (slabs0 + chunk - 1) / chunk;
-    const int64_t longest = (tiles0 * planes + pairs - 1) / pairs * chunk, time = longest > share ? longest : share;
-    if (s == 1 || time * 100 < best_time * 97) {    // (a further plane is written, read and added up)
-      best = chunk;
-      best_time = time;
+  const int s = (threadIdx.x & 31) + 1, chunk = (slabs0 + s - 1) / s, planes = (slabs0 + chunk - 1) / chunk;
+  const int64_t longest = (tiles0 * planes + pairs - 1) / pairs * chunk, time = longest > share ? longest : share;
+  const unsigned allowed = __ballot_sync(0xffffffffu, s <= max_planes && (s == 1 || slabs0 / s >= 8));
+  int best = 0;
+  int64_t best_time = __shfl_sync(0xffffffffu, time, 0);
+  for (int i = 1; i < 32 && (allowed >> i & 1u) != 0 && best_time * 100 > share * 102; ++i) {
+    const int64_t t = __shfl_sync(0xffffffffu, time, i);
+    if (t * 100 < best_time * 97) {    // (a further plane is written, read and added up)
+      best = i;
+      best_time = t;
     }
-    if (best_time * 100 <= share * 102) break;
   }
-  return best;
+  return __shfl_sync(0xffffffffu, chunk, best);
 }
 
 int pick_block_n(int64_t M, int64_t N, int64_t batch, int sm_count);
