@@ -5,12 +5,15 @@
 //                z at the row's targets; a label's column can be left out (the tensor cores cut what an addition shifts out
 //                instead of rounding it: a logit of 10 loses 4e-5 over 4096 products, and the label's is the one that the
 //                loss is made of, so the loss kernel makes it again in fp32 where that is a row of w to read)
-//   gradient     G = g (softmax(z) - target weights), rounded once to the 16-bit operand of the two products that
-//                follow (dx = G w, dw = G^T x): a rounding error of 2^-9 or 2^-12 of each entry, as of any activation
-//                gradient, independent from entry to entry
+//   gradient     G = g (softmax(z) - target weights), g relative to the batch's largest, rounded once to the 16-bit operand
+//                of the two products that follow (dx = G w, dw = G^T x): a rounding error of at most 2^-8 or 2^-11 of each
+//                entry, as of any activation gradient, independent from entry to entry
 //
-// Both are 2 N D V flops on the tensor cores; the epilogue's V N exponentials (16 per cycle and SM) are hidden behind the
-// product from hidden sizes of about 256 on.  CTA pairs work on 256 x 256 tiles (cta_group::2: half of w's tile per CTA),
+// Both are 2 N D V flops on the tensor cores, which bound them from hidden sizes of about 600 on: 2048 x 4096 x 51200 532 and
+// 530 us alone, 1.61 PFLOP/s, and as much as the power limit leaves of that in a row of such calls.  Below, the epilogue does:
+// reading tensor memory (16 bytes a cycle and quarter of an SM) and V N exponentials (16 a cycle and SM) take 2048 cycles each
+// of a tile's 4400 at 6000 x 160 x 30000, 111 us.  Few rows are a stream of w: 16 x 4096 x 51200 72 us, 5.8 TB/s.
+// CTA pairs work on 256 x 256 tiles (cta_group::2: half of w's tile per CTA),
 // or, where that leaves pairs without one, single CTAs on 128 rows and as many columns as give every SM an equal share.
 // A unit of work is a row block and a strip of consecutive column tiles, whose statistics stay in registers.
 //
@@ -588,8 +591,8 @@ struct Tiling {
   int tile_n, tiles_n, strip, strips;
 };
 
-// 256 x 256 tiles on CTA pairs once every pair has one (narrower ones where that fills the last of few rounds); else row blocks of 128 and column tiles that are as wide as a whole
-// number of rounds of all SMs allows, in steps of `unit` columns.
+// 256 x 256 tiles on CTA pairs once every pair has one (narrower ones where that fills the last of few rounds); else row blocks
+// of 128 and column tiles that are as wide as a whole number of rounds of all SMs allows, in steps of `unit` columns.
 Tiling tiling_for(int64_t rows, int64_t columns, int unit) {
   Tiling t{};
   const int64_t pairs = kAssumedSms / 2, pair_rows = (rows + 255) / 256, wide = (columns + kMaxTileN - 1) / kMaxTileN;

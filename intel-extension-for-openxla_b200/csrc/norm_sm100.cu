@@ -10,8 +10,15 @@
 // A row belongs to a group of threads (a warp for short rows, a CTA else) and stays in their registers between its
 // statistics and its result.  CTAs are persistent: a thread has the same columns in every row, so gain and shift are read
 // once, and the columns' sums over the CTA's rows grow in its registers (fp32) instead of passing through memory.  They
-// leave as one row of partials per CTA, which a second kernel adds up in a fixed order: the result does not depend on
-// which CTA was faster.  The next row's loads are asked for before this row's statistics are waited for.
+// leave as one row of partials per CTA or pair of CTAs, which a second kernel adds up in a fixed order: the result does not
+// depend on which CTA was faster.  Statistics and sums are fp32, the variance is taken about the mean, and 1 / sqrt is the
+// correctly rounded one: its error would be shared by all elements of a row.
+//
+// Which kernel a row takes (times: forward / backward with its sums, cold caches, one call waited for):
+//   up to 256 columns, whole 16-byte vectors    row_norm_*_rows_kernel, several rows a warp      65536 x 256 bf16   22 /  32 us
+//   257 .. 8192, or whole vectors or not        row_norm_*_ring_kernel, rows through a ring      8192 x 4096 bf16   35 /  50 us
+//   up to 256 single elements, or above 8192    row_norm_*_kernel, a row a warp or a CTA         (512 threads of 16 columns are
+//                                               the ring's limit; 5461 x 12288 bf16   74 / 190 us)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -64,7 +71,7 @@ __device__ __forceinline__ Raw<T, kVec> pack(const float (&f)[kVec]) {
   return raw;
 }
 // The compiler may not keep what it unpacked of `raw` beyond this point: registers hold the row as it lies in memory, not
-// twice as many floats (bf16 at 16 vectors a lane: 164 registers with, 255 and spills without at 32).
+// twice as many floats.
 __device__ __forceinline__ void forget(uint4& raw) { asm volatile("" : "+r"(raw.x), "+r"(raw.y), "+r"(raw.z), "+r"(raw.w)); }
 __device__ __forceinline__ float load_param(const void* p, int64_t i, int dtype) {
   if (dtype == IXK_F32) return static_cast<const float*>(p)[i];
@@ -129,6 +136,7 @@ struct Piece {
   }
 };
 
+// Rows that neither of the kernels below takes: the next row's loads are asked for before this row's statistics are waited for.
 template <typename T, int kVec, int kPer, bool kWarp>
 __global__ void __launch_bounds__(kWarp ? 256 : kMaxThreads, 1) row_norm_fwd_kernel(const Args a) {
   __shared__ float scratch[2 * 2 * 32];
@@ -425,7 +433,8 @@ __device__ __forceinline__ void cta_sums(float (&v)[kCount], float (&scratch)[kC
 }
 
 // Forward, short rows (up to eight elements a lane): a warp has kRows rows at a time, all of their loads out at once and no
-// barrier between warps.
+// barrier between warps.  65536 x 256 bf16: 16 us on the device, 67 MB at 4.2 TB/s, what a copy of that size gets between its
+// start and its end (rows copied ahead into shared memory changed nothing).
 template <typename T, typename P, int kPer, int kRows>
 __global__ void __launch_bounds__(128) row_norm_fwd_rows_kernel(const Args a) {
   constexpr int kVec = 16 / sizeof(T), kN = kPairs<T>;
@@ -569,7 +578,7 @@ __device__ __forceinline__ void put_pairs(float* out, const uint64_t (&p)[kN], b
 }
 
 // Backward, short rows (up to eight elements a lane): a warp has kRows rows at a time, a lane kPer vectors of columns and
-// their sums.
+// their sums.  65536 x 256 bf16: 24 us on the device, 100 MB at 4.2 TB/s, and 5 us for the sums.
 template <typename T, typename P, int kPer, int kRows>
 __global__ void __launch_bounds__(256) row_norm_bwd_rows_kernel(const Args a) {
   constexpr int kVec = 16 / sizeof(T), kN = kPairs<T>;
@@ -650,7 +659,10 @@ __global__ void __launch_bounds__(256) row_norm_bwd_rows_kernel(const Args a) {
 
 // Longer rows: a CTA takes kRows rows at a time out of a ring in shared memory that bulk copies keep full (about 190 KB under
 // way an SM, which registers could not hold beside the parameters and the columns' sums), and one barrier serves the sums of
-// all of them.  A thread has 16 columns: with eight, the sums across threads were a third of all instructions.
+// all of them.  A thread has 16 columns: with eight, the sums across threads were a third of all instructions.  What bounds
+// it is the chain of a batch (copy's arrival, sums, barrier, result) with two batches an SM to fill the gaps: 8192 x 4096 bf16
+// LayerNorm 32 us on the device forward (134 MB at 4.2 TB/s), 43 backward (201 MB at 4.7 TB/s); three or four CTAs an SM have
+// too few registers (37 us called, not 35), one row a batch pays its barriers alone.
 // kWhole: rows start on 16 bytes and hold whole vectors; a thread has vectors of columns.  Otherwise a row's image in the ring
 // keeps the row's place within 16 bytes, the copy brings every 16-byte piece that the row touches (of the first and the last
 // row only those that lie wholly in it: nothing outside the tensor is read, and the rest comes element by element), and a
@@ -1041,7 +1053,8 @@ __global__ void __launch_bounds__(kRingThreads, 1) row_norm_bwd_ring_kernel(cons
   ptx::cluster_sync_all();      // (nobody leaves while its memory is read)
 }
 
-// dgain (blockIdx.y 0) and dshift (1): the CTAs' rows of partials added up, kSumCols columns per CTA.
+// dgain (blockIdx.y 0) and dshift (1): the CTAs' rows of partials added up, kSumCols columns per CTA, every sixteenth row by a
+// thread and the threads' sums in a tree: always the same order.  148 rows of 4096: 5 us, a launch and two reads' latency.
 __global__ void __launch_bounds__(kSumCols* kSumParts) row_norm_sum_kernel(const float* part_gain, const float* part_shift, int parts,
                                                                           int cols, void* dgain, void* dshift, int dtype) {
   ptx::grid_dependency_sync();
