@@ -73,6 +73,8 @@ __device__ __forceinline__ Raw<T, kVec> pack(const float (&f)[kVec]) {
 // The compiler may not keep what it unpacked of `raw` beyond this point: registers hold the row as it lies in memory, not
 // twice as many floats.
 __device__ __forceinline__ void forget(uint4& raw) { asm volatile("" : "+r"(raw.x), "+r"(raw.y), "+r"(raw.z), "+r"(raw.w)); }
+__device__ __forceinline__ void forget(uint32_t& raw) { asm volatile("" : "+r"(raw)); }
+__device__ __forceinline__ void forget(uint16_t& raw) { asm volatile("" : "+h"(raw)); }
 __device__ __forceinline__ float load_param(const void* p, int64_t i, int dtype) {
   if (dtype == IXK_F32) return static_cast<const float*>(p)[i];
   if (dtype == IXK_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
@@ -136,31 +138,47 @@ struct Piece {
   }
 };
 
-// Rows that neither of the kernels below takes: the next row's loads are asked for before this row's statistics are waited for.
+// Rows that neither of the kernels below takes.  kAhead: parameters in registers, the next row's loads asked for before this
+// row's statistics are waited for.  Otherwise a CTA's row, whose 1024 threads of 16 columns have 64 registers each: parameters
+// in shared memory, one row at a time.  Ahead and not: 5461 rows of 12288 16-bit elements in whole vectors, backward, 189 and
+// 202 us; of 12287, forward 275 and 214, backward 507 and 423; 3000 x 10000 fp32 in whole vectors, forward 70 and 82, backward
+// 151 and 120.
+template <typename T, int kVec, bool kWarp, bool kBwd>
+constexpr bool kAhead = kWarp || (kVec > 1 && (sizeof(T) == 2 || !kBwd));
 template <typename T, int kVec, int kPer, bool kWarp>
 __global__ void __launch_bounds__(kWarp ? 256 : kMaxThreads, 1) row_norm_fwd_kernel(const Args a) {
   __shared__ float scratch[2 * 2 * 32];
+  extern __shared__ float params[];      // not ahead: scale and shift, [2][cols]
+  constexpr bool kRegs = kAhead<T, kVec, kWarp, false>;
   const int threads = kWarp ? 32 : blockDim.x, thread = kWarp ? threadIdx.x & 31 : threadIdx.x;
   const int64_t groups = kWarp ? static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5) : gridDim.x;
   int64_t row = kWarp ? static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
   const int nvec = a.cols / kVec;
   int turn = 0;
   ptx::grid_dependency_sync();
-  float scale[kPer * kVec], shift[kPer * kVec];
+  float own_scale[kRegs ? kPer * kVec : 1], own_shift[kRegs ? kPer * kVec : 1];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
       const int c = (thread + i * threads) * kVec + j;
-      scale[i * kVec + j] = a.gain != nullptr && c < a.cols ? a.gain_offset + load_param(a.gain, c, a.param_dtype) : 1.0f;
-      shift[i * kVec + j] = a.shift != nullptr && c < a.cols ? load_param(a.shift, c, a.param_dtype) : 0.0f;
+      const float scale = a.gain != nullptr && c < a.cols ? a.gain_offset + load_param(a.gain, c, a.param_dtype) : 1.0f;
+      const float shift = a.shift != nullptr && c < a.cols ? load_param(a.shift, c, a.param_dtype) : 0.0f;
+      if constexpr (kRegs) {
+        own_scale[i * kVec + j] = scale;
+        own_shift[i * kVec + j] = shift;
+      } else if (c < a.cols) {      // (read by this thread alone)
+        params[c] = scale;
+        params[a.cols + c] = shift;
+      }
     }
   }
   Piece<T, kVec, kPer> next;
-  if (row < a.rows) next.load(a.x, row, a.ldx, thread, threads, nvec);
+  if (kRegs && row < a.rows) next.load(a.x, row, a.ldx, thread, threads, nvec);
   for (; row < a.rows; row += groups) {
-    const Piece<T, kVec, kPer> cur = next;
-    if (row + groups < a.rows) next.load(a.x, row + groups, a.ldx, thread, threads, nvec);
+    if (!kRegs) next.load(a.x, row, a.ldx, thread, threads, nvec);
+    Piece<T, kVec, kPer> cur = next;
+    if (kRegs && row + groups < a.rows) next.load(a.x, row + groups, a.ldx, thread, threads, nvec);
     float s[1] = {0.0f};
     float mean = 0.0f;
     if (!a.rms) {
@@ -186,6 +204,10 @@ __global__ void __launch_bounds__(kWarp ? 256 : kMaxThreads, 1) row_norm_fwd_ker
       }
     }
     row_sums<kWarp, 1>(s, scratch, turn);
+    if constexpr (!kRegs) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) forget(cur.raw[i]);
+    }
     const float rstd = __frsqrt_rn(fmaf(s[0], a.inv_cols, a.eps));
     T* out = static_cast<T*>(a.out) + row * a.ldo;
 #pragma unroll
@@ -195,7 +217,17 @@ __global__ void __launch_bounds__(kWarp ? 256 : kMaxThreads, 1) row_norm_fwd_ker
         float f[kVec];
         unpack<T, kVec>(cur.raw[i], f);
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) f[j] = fmaf((f[j] - mean) * rstd, scale[i * kVec + j], shift[i * kVec + j]);
+        for (int j = 0; j < kVec; ++j) {
+          float scale, shift;
+          if constexpr (kRegs) {
+            scale = own_scale[i * kVec + j];
+            shift = own_shift[i * kVec + j];
+          } else {
+            scale = params[v * kVec + j];
+            shift = params[a.cols + v * kVec + j];
+          }
+          f[j] = fmaf((f[j] - mean) * rstd, scale, shift);
+        }
         *reinterpret_cast<Raw<T, kVec>*>(out + static_cast<int64_t>(v) * kVec) = pack<T, kVec>(f);
       }
     }
@@ -209,23 +241,30 @@ __global__ void __launch_bounds__(kWarp ? 256 : kMaxThreads, 1) row_norm_fwd_ker
 template <typename T, int kVec, int kPer, bool kWarp>
 __global__ void __launch_bounds__(kWarp ? 256 : kMaxThreads, 1) row_norm_bwd_kernel(const Args a) {
   __shared__ float scratch[2 * 2 * 32];
-  extern __shared__ float sums[];    // kWarp: [2][cols]
+  extern __shared__ float sums[];    // kWarp: [2][cols]; not ahead: the scale, [cols]
   const int threads = kWarp ? 32 : blockDim.x, thread = kWarp ? threadIdx.x & 31 : threadIdx.x;
   const int64_t groups = kWarp ? static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5) : gridDim.x;
   int64_t row = kWarp ? static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
   const int nvec = a.cols / kVec;
   int turn = 0;
   ptx::grid_dependency_sync();
-  float scale[kPer * kVec], dgain[kPer * kVec], dshift[kPer * kVec];
+  constexpr bool kRegs = kAhead<T, kVec, kWarp, true>;
+  float own_scale[kRegs ? kPer * kVec : 1], dgain[kPer * kVec], dshift[kPer * kVec];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
       const int c = (thread + i * threads) * kVec + j;
-      scale[i * kVec + j] = a.gain != nullptr && c < a.cols ? a.gain_offset + load_param(a.gain, c, a.param_dtype) : 1.0f;
+      const float scale = a.gain != nullptr && c < a.cols ? a.gain_offset + load_param(a.gain, c, a.param_dtype) : 1.0f;
+      if constexpr (kRegs) own_scale[i * kVec + j] = scale;
+      else if (c < a.cols) sums[c] = scale;      // (read by this thread alone)
       dgain[i * kVec + j] = dshift[i * kVec + j] = 0.0f;
     }
   }
+  auto scale_of = [&](int i, int j) {      // (behind the row's end g is 0)
+    if constexpr (kRegs) return own_scale[i * kVec + j];
+    else return thread + i * threads < nvec ? sums[(thread + i * threads) * kVec + j] : 0.0f;
+  };
   Piece<T, kVec, kPer> next_x, next_g;
   float next_mean = 0.0f, next_rstd = 0.0f;
   auto fetch = [&](int64_t r) {
@@ -234,11 +273,12 @@ __global__ void __launch_bounds__(kWarp ? 256 : kMaxThreads, 1) row_norm_bwd_ker
     next_mean = a.rms ? 0.0f : a.mean[r];
     next_rstd = a.rstd[r];
   };
-  if (row < a.rows) fetch(row);
+  if (kRegs && row < a.rows) fetch(row);
   for (; row < a.rows; row += groups) {
-    const Piece<T, kVec, kPer> cur_x = next_x, cur_g = next_g;
+    if (!kRegs) fetch(row);
+    Piece<T, kVec, kPer> cur_x = next_x, cur_g = next_g;
     const float mean = next_mean, rstd = next_rstd;
-    if (row + groups < a.rows) fetch(row + groups);
+    if (kRegs && row + groups < a.rows) fetch(row + groups);
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -247,7 +287,7 @@ __global__ void __launch_bounds__(kWarp ? 256 : kMaxThreads, 1) row_norm_bwd_ker
       unpack<T, kVec>(cur_g.raw[i], g);
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {     // (behind the row's end g is 0)
-        const float xh = (x[j] - mean) * rstd, h = g[j] * scale[i * kVec + j];
+        const float xh = (x[j] - mean) * rstd, h = g[j] * scale_of(i, j);
         dgain[i * kVec + j] = fmaf(g[j], xh, dgain[i * kVec + j]);
         dshift[i * kVec + j] += g[j];
         s[0] = fmaf(h, xh, s[0]);
@@ -255,6 +295,13 @@ __global__ void __launch_bounds__(kWarp ? 256 : kMaxThreads, 1) row_norm_bwd_ker
       }
     }
     row_sums<kWarp, 2>(s, scratch, turn);
+    if constexpr (!kRegs) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        forget(cur_x.raw[i]);
+        forget(cur_g.raw[i]);
+      }
+    }
     const float c1 = s[0] * a.inv_cols, c0 = a.rms ? 0.0f : s[1] * a.inv_cols;
     T* out = static_cast<T*>(a.out) + row * a.ldo;
 #pragma unroll
@@ -266,7 +313,7 @@ __global__ void __launch_bounds__(kWarp ? 256 : kMaxThreads, 1) row_norm_bwd_ker
         unpack<T, kVec>(cur_g.raw[i], g);
 #pragma unroll
         for (int j = 0; j < kVec; ++j) {
-          const float xh = (x[j] - mean) * rstd, h = g[j] * scale[i * kVec + j];
+          const float xh = (x[j] - mean) * rstd, h = g[j] * scale_of(i, j);
           x[j] = rstd * (h - fmaf(xh, c1, c0));
         }
         *reinterpret_cast<Raw<T, kVec>*>(out + static_cast<int64_t>(v) * kVec) = pack<T, kVec>(x);
@@ -1139,12 +1186,23 @@ int64_t ctas_for(const Plan& p, int64_t rows) {
 
 template <typename T, bool kBwd>
 int launch(const Plan& p, const Args& a, int64_t ctas, cudaStream_t stream) {
-  const size_t smem = kBwd && p.warp ? 2 * sizeof(float) * a.cols : 0;
   auto go = [&](auto vec, auto per, auto warp) -> int {
     constexpr int kVec = decltype(vec)::value, kPer = decltype(per)::value;
     constexpr bool kWarp = decltype(warp)::value;
-    if constexpr (kBwd) return launch_overlapped(row_norm_bwd_kernel<T, kVec, kPer, kWarp>, dim3(ctas), dim3(p.threads), smem, stream, a);
-    else return launch_overlapped(row_norm_fwd_kernel<T, kVec, kPer, kWarp>, dim3(ctas), dim3(p.threads), smem, stream, a);
+    auto* fn = &row_norm_fwd_kernel<T, kVec, kPer, kWarp>;
+    if constexpr (kBwd) fn = &row_norm_bwd_kernel<T, kVec, kPer, kWarp>;
+    size_t smem = kBwd && kWarp ? 2 * sizeof(float) * a.cols : 0;
+    if constexpr (!kAhead<T, kVec, kWarp, kBwd>) {
+      smem = (kBwd ? 1 : 2) * sizeof(float) * a.cols;
+      static thread_local int configured_device = -1;
+      int dev = 0;
+      IXK_CUDA_OK(cudaGetDevice(&dev));
+      if (configured_device != dev) {
+        IXK_CUDA_OK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(2 * sizeof(float) * kMaxCols)));
+        configured_device = dev;
+      }
+    }
+    return launch_overlapped(fn, dim3(ctas), dim3(p.threads), smem, stream, a);
   };
   constexpr int kFull = 16 / sizeof(T);
 #define IXK_NORM_CASE(V, P, W) \
