@@ -1,7 +1,11 @@
 """CPU: the end of a training step (layers.lm_head_training_pass) in its plain form against autograd in 64 bits.  fp32 in, fp32
 throughout: sums of up to 400 terms, so 1e-5 of a result's own size holds them with room."""
+import ctypes
 import importlib
 import math
+import os
+import subprocess
+import tempfile
 
 import pytest
 import torch
@@ -76,3 +80,18 @@ def test_one_kind_of_target(layers):
     for kw in ({}, {"labels": labels, "teacher": teacher}):
         with pytest.raises(ValueError):
             layers.lm_head_training_pass(x, w, object(), **kw)
+
+
+def test_descriptors_are_laid_out_as_in_the_header(pkg):
+    """Every field of the two descriptors: where the C compiler puts it and where ctypes does."""
+    pairs = {"ixk_row_norm_desc": pkg._RowNormDesc, "ixk_linear_loss_desc": pkg._LinearLossDesc}
+    lines = [f'printf("%zu\\n", sizeof({c}));' + "".join(f'printf("%zu\\n", offsetof({c}, {f[0]}));' for f in s._fields_) for c, s in pairs.items()]
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    with tempfile.TemporaryDirectory() as d:
+        src, exe = os.path.join(d, "probe.c"), os.path.join(d, "probe")
+        with open(src, "w") as f:
+            f.write("#include <stdio.h>\n#include <stddef.h>\n#include \"ixk.h\"\nint main(void) {" + "\n".join(lines) + "return 0; }\n")
+        subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-I", os.path.join(root, "include"), src, "-o", exe], check=True)
+        got = [int(v) for v in subprocess.run([exe], check=True, capture_output=True, text=True).stdout.split()]
+    want = [v for s in pairs.values() for v in [ctypes.sizeof(s)] + [getattr(s, f[0]).offset for f in s._fields_]]
+    assert got == want
