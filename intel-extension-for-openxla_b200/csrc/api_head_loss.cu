@@ -19,6 +19,7 @@
 
 #include "gemm_sm100.h"
 #include "head_loss.h"
+#include "head_pieces.h"
 #include "ptx.cuh"
 
 namespace ixk {
@@ -27,15 +28,12 @@ namespace head {
 namespace {
 
 constexpr int kMaxEntries = 256;
-constexpr size_t kPieceBytes = size_t(256) << 20;  // of G
 constexpr size_t kSplitBytes = size_t(64) << 20;   // of the GEMMs' K chunks, for few rows
 constexpr size_t kPlaneBytes = size_t(128) << 20;  // of dx's planes, for more
 constexpr int kMaxPlanes = 16;
 constexpr int64_t kPitchUnit = 64;               // rows of whole 128-byte lines: a box that straddles lines reads one more of each
 constexpr int kSlabRows = 64;                    // rows that the product along the rows reads at a time
 constexpr float kLn2 = 0.6931471805599453f, kLog2E = 1.4426950408889634f;
-
-int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 template <bool kBf16>
 __device__ __forceinline__ float from16(uint32_t bits) {
@@ -441,7 +439,7 @@ __global__ void __launch_bounds__(kThreads) loss_kernel(const Loss a) {
 // dbias of a piece: the sums of G's columns, another read of G (2048 x 51200: 45 us, 4.7 TB/s; the products before it leave
 // little of a large G in L2, and the kernel that makes G has a row a thread).  256 columns per CTA, kGroups warps that take rows in turn; where the columns alone
 // leave SMs idle the rows are dealt out to gridDim.y CTAs, which leave partial sums for bias_sum_kernel.
-constexpr int kBiasCols = 256, kBiasGroups = 32, kFewGroups = 4, kBiasParts = 32;
+constexpr int kFewGroups = 4;
 constexpr int64_t kFewBiasRows = 32;      // 5 x 176783: 6.9 us with 32 warps, 4.3 with four; 76 x 99763: 7.7 and 13
 template <bool kBf16, int kGroups>
 __global__ void __launch_bounds__(32 * kGroups) bias_kernel(const uint16_t* g, int64_t ldg, const Control* control, int count, float* partial,
@@ -579,16 +577,11 @@ struct Layout {
   Space space;
   size_t control, info, column, weight, start, has, packed, at_target, partial;      // forward
   size_t inverse, grad, bias, acc, split, split_bytes;                               // backward
-  int64_t ldp, slots, piece, ldg, ld_acc, plane;      // plane 0: dx is not cut into planes
+  int64_t ldp, slots, ldg, ld_acc, plane;      // plane 0: dx is not cut into planes
+  Pieces pieces;
   int planes;
   bool gathered;
 };
-
-// CTAs along the rows for the sums of a piece's columns: as many as give the SMs one each, with four rows a warp or more.
-int64_t bias_parts(int64_t columns, int64_t rows) {
-  const int64_t blocks = (columns + kBiasCols - 1) / kBiasCols;
-  return std::clamp<int64_t>(std::min<int64_t>(148 / blocks, rows / (4 * kBiasGroups)), 1, kBiasParts);
-}
 
 // Whether the label's logit is a product of its own: one row of w each, or, column-major, a 32-byte sector an element, which
 // only few rows can pay (7355 x 3520 x 8144: 270 of 1700 us).
@@ -618,26 +611,23 @@ Layout layout_for(const ixk_linear_loss_desc& d, bool backward) {
     return l;
   }
   l.inverse = l.space.take(4 * N);
-  // pieces of equal size, as few as the bytes allow
-  const int64_t rows = round_up(N, 256), most = std::max<int64_t>(kPieceBytes / (2 * rows) / kPieceUnit * kPieceUnit, kPieceUnit);
-  const int64_t pieces = (V + most - 1) / most;
-  l.piece = std::min(round_up((V + pieces - 1) / pieces, kPieceUnit), round_up(V, 8));
-  l.ldg = round_up(l.piece, kPitchUnit);
-  l.grad = l.space.take(2 * rows * l.ldg);
-  l.bias = l.space.take(4 * bias_parts(std::min(l.piece, V), N) * l.piece);
+  l.pieces = pieces_for(N, V);
+  l.ldg = round_up(l.pieces.columns, kPitchUnit);
+  l.grad = l.space.take(2 * round_up(N, 256) * l.ldg);
+  l.bias = l.space.take(4 * l.pieces.bias_partials());
   l.ld_acc = round_up(D, kPitchUnit / 2);
   if (N > kDirectRows) {
     l.plane = N * l.ld_acc;
     l.planes = static_cast<int>(std::clamp<int64_t>(kPlaneBytes / (4 * l.plane), 1, kMaxPlanes));
     l.acc = l.space.take(4 * l.plane * l.planes);
-  } else if (pieces == 1) {      // (planes of the kernel for few rows: dense)
+  } else if (l.pieces.count == 1) {      // (planes of the kernel for few rows: dense)
     l.ld_acc = D;
     l.plane = N * D;
     l.planes = gemm::stream_splits(N, D, V, 2, kSplitBytes);
     l.acc = l.space.take(4 * l.plane * l.planes);
   } else {
     l.acc = l.space.take(4 * N * l.ld_acc);
-    l.split_bytes = std::min(gemm::problem_workspace_bytes(N, D, l.piece), kSplitBytes);
+    l.split_bytes = std::min(gemm::problem_workspace_bytes(N, D, l.pieces.columns), kSplitBytes);
     l.split = l.space.take(l.split_bytes);
   }
   return l;
@@ -758,8 +748,8 @@ int gather(const ixk_linear_loss_desc& d, const Layout& l, char* ws, const HasTa
   g.top = !backward ? 0.0f : d.dtype == IXK_F16 ? 0x1p13f : 1.0f;
   if (backward && d.rows > kDirectRows) {
     g.dx_tiles_n = static_cast<int>((d.hidden + gemm::kTwoTile - 1) / gemm::kTwoTile);
-    g.piece_slabs = static_cast<int>((l.piece + kSlabRows - 1) / kSlabRows);
-    g.dw_tiles = want_dw ? g.dx_tiles_n * static_cast<int>((l.piece + gemm::kTwoTile - 1) / gemm::kTwoTile) : 0;
+    g.piece_slabs = static_cast<int>((l.pieces.columns + kSlabRows - 1) / kSlabRows);
+    g.dw_tiles = want_dw ? g.dx_tiles_n * static_cast<int>((l.pieces.columns + gemm::kTwoTile - 1) / gemm::kTwoTile) : 0;
     g.pairs = sm_count / 2;
     g.max_planes = l.planes;
   }
@@ -893,9 +883,9 @@ int backward(const char* name, const ixk_linear_loss_desc* d, bool distill, cons
   common.ab_dtype = d->dtype;
   common.a_fmt = common.b_fmt = bf16 ? 1u : 0u;
   common.bias_dtype = d->dtype;
-  for (int64_t first = 0; first < d->vocab; first += l.piece) {
+  for (int64_t first = 0; first < d->vocab; first += l.pieces.columns) {
     p.first = first;
-    p.count = std::min(l.piece, d->vocab - first);
+    p.count = l.pieces.columns_of(first);
     if ((rc = launch_grad(p, dev, s)) != IXK_OK) return rc;
     gemm::Problem both[2] = {common, common};
     if (dx != nullptr) {       // dx += G w
@@ -944,7 +934,7 @@ int backward(const char* name, const ixk_linear_loss_desc* d, bool distill, cons
     if (both[0].M > 0) both[0].m_limit = p.active_rows;
     if ((rc = gemm::launch_two(both, &control->plane_slabs, dev, s)) != IXK_OK) return rc;
     if (dbias != nullptr) {
-      const unsigned blocks = static_cast<unsigned>((p.count + kBiasCols - 1) / kBiasCols), parts = static_cast<unsigned>(bias_parts(p.count, d->rows));
+      const unsigned blocks = static_cast<unsigned>((p.count + kBiasCols - 1) / kBiasCols), parts = static_cast<unsigned>(l.pieces.bias_parts);
       float* partial = reinterpret_cast<float*>(ws + l.bias);
       auto* out = static_cast<uint16_t*>(dbias) + first;
       const bool few = d->rows <= kFewBiasRows;

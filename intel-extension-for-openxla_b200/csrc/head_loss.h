@@ -53,8 +53,6 @@ struct Pass {
 
 // Rows of `partial` that a statistics pass fills.
 int stat_slots(int64_t rows, int64_t vocab);
-// Columns that a piece of the gradient had best be a multiple of.
-constexpr int kPieceUnit = 256;
 
 int launch_stats(const Pass& p, const DeviceInfo& dev, cudaStream_t stream);
 int launch_grad(const Pass& p, const DeviceInfo& dev, cudaStream_t stream);
