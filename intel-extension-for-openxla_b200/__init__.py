@@ -769,8 +769,10 @@ def _linear_loss_desc(x, weight, bias, index, teacher, scale: float, ignore_inde
 
 
 def linear_loss_workspace_bytes(x: torch.Tensor, weight: torch.Tensor, entries: int = 0, backward: bool = False) -> int:
-    """Scratch bytes of linear_cross_entropy (entries = 0) or linear_distillation, or of their backward passes."""
+    """Scratch bytes of linear_cross_entropy (entries = 0) or linear_distillation with this weight (its layout counts), or of
+    their backward passes."""
     d = _LinearLossDesc()
+    d.w_order, d.w_stride = _head_matrix("weight", weight)
     d.rows, d.hidden, d.vocab, d.entries = x.shape[0], x.shape[1], weight.shape[0], entries
     return int(load_library().ixk_linear_loss_workspace_bytes(ctypes.byref(d), 1 if backward else 0))
 

@@ -1,7 +1,11 @@
 """CPU: what the host decides for the losses at the vocabulary head: the pieces of the vocabulary, scratch, the workspace query."""
+import ctypes
 import os
 import subprocess
 import tempfile
+
+import pytest
+import torch
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "intel-extension-for-openxla_b200", "csrc")
@@ -49,3 +53,17 @@ def test_every_piece_of_the_vocabulary_fits_its_scratch():
         assert 2 * ((r + 255) // 256 * 256) * columns <= (256 << 20) or columns <= 256, (r, v)
         several += count > 1
     assert several > 500
+
+
+@pytest.mark.parametrize("rows", [1, 128, 129, 5000])
+@pytest.mark.parametrize("entries", [0, 9])
+def test_the_workspace_query_knows_the_weights_layout(pkg, rows, entries):
+    """What Python tells is what the call with this weight will ask for."""
+    lib = pkg.load_library()
+    x, row_major, column_major = torch.empty(rows, 512), torch.empty(4000, 512), torch.empty(512, 4000).t()
+    for backward in (False, True):
+        for w, order in ((row_major, pkg.ROW_MAJOR), (column_major, pkg.COL_MAJOR)):
+            d = pkg._LinearLossDesc()
+            d.rows, d.hidden, d.vocab, d.entries, d.w_order = rows, 512, 4000, entries, order
+            want = lib.ixk_linear_loss_workspace_bytes(ctypes.byref(d), int(backward))
+            assert pkg.linear_loss_workspace_bytes(x, w, entries, backward) == want > 0
