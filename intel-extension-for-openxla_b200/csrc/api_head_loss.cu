@@ -956,7 +956,8 @@ int backward(const char* name, const ixk_linear_loss_desc* d, bool distill, cons
                              static_cast<const float*>(acc), l.ld_acc, l.plane, std::max(l.planes, 1), inverse, control, static_cast<int>(d->hidden),
                              static_cast<uint16_t*>(dx), d->dx_stride);
   const int vec = aligned(dx, 16) && d->dx_stride % 8 == 0;
-  const int width = static_cast<int>(std::min<int64_t>(round_up(vec ? d->hidden / 8 : d->hidden, 32), 256));
+  // (a row of less than one vector has a warp too, for its single elements)
+  const int width = static_cast<int>(std::clamp<int64_t>(round_up(vec ? d->hidden / 8 : d->hidden, 32), 32, 256));
   return launch_overlapped(bf16 ? scatter_kernel<true> : scatter_kernel<false>, dim3(static_cast<unsigned>((d->rows + 256 / width - 1) / (256 / width))),
                            dim3(256), 0, s, static_cast<const float*>(acc), l.ld_acc, l.plane, inverse, control, static_cast<int>(d->rows),
                            static_cast<int>(d->hidden), vec, width, static_cast<uint16_t*>(dx), d->dx_stride);
