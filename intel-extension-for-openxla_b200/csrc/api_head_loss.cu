@@ -186,14 +186,46 @@ struct Gather {
   int64_t grad_stride;
   float factor;
   float top;                   // 0: forward
+  // labels apart: the label's p - 1, from its fp32 logit and lse.  What the products over all of K lose of a logit of 15 is 6e-5, as
+  // much as 1 - p of a token that the model is sure of.
+  float* gap;
+  const uint16_t *w, *bias;
+  int64_t ldw;
+  int w_column_major;
+  float scale;
   // and the products' plan: tiles of a row block of dx, of dw; slabs of a piece
   int dx_tiles_n, piece_slabs, dw_tiles, pairs, max_planes;
 };
+
+// The label's logit of a row, scale (x . w[label] + bias[label]) in fp32, is made by a CTA of the loss kernel that has kShares warps
+// for it, and again by one warp of the gather in front of the gradient.  Both add up in the same order, so that what the sum's
+// rounding does to the logit is in lse as well and p - 1 does not see it: share i takes every kShares-th group of 32 vectors (w
+// row-major) or elements, the lanes' sums meet in a butterfly, the shares' in ascending order.
+template <bool kBf16>
+__device__ __forceinline__ float dot_vec(const uint4& p, const uint4& q, float t) {
+  const uint32_t pw[4] = {p.x, p.y, p.z, p.w}, qw[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    t = fmaf(from16<kBf16>(pw[j] & 0xffffu), from16<kBf16>(qw[j] & 0xffffu), t);
+    t = fmaf(from16<kBf16>(pw[j] >> 16), from16<kBf16>(qw[j] >> 16), t);
+  }
+  return t;
+}
+// call(rows, threads of a CTA of the loss kernel): rows side by side are one read of up to 256 bytes; few rows want a CTA each.
+template <typename Call>
+int loss_shape(int64_t rows, const Call& call) {
+  using std::integral_constant;
+  if (rows >= 4096) return call(integral_constant<int, 32>{}, integral_constant<int, 1024>{});
+  if (rows >= 512) return call(integral_constant<int, 8>{}, integral_constant<int, 1024>{});
+  return call(integral_constant<int, 1>{}, integral_constant<int, 256>{});
+}
 
 // 2048 x 4096: 8 us, 34 MB moved; every CTA first counts the rows with a target in front of its own, which saves a launch.
 constexpr int kGatherThreads = 256;
 constexpr int kCopyVecs = 8, kCountAtOnce = 8;
 
+// kShares: of the label's logit, 0: it is not wanted.
+template <bool kBf16, int kShares>
 __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Gather a) {
   __shared__ int warp_count[kGatherThreads / 32];
   __shared__ int source[kGatherThreads];
@@ -268,16 +300,73 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Gather a) 
   for (int i = warp; i < here; i += kGatherThreads / 32) {
     const uint16_t* src = a.x + source[i] * a.ldx;
     uint16_t* dst = a.packed + (before + i) * a.ldp;
-    for (int v0 = lane; v0 < whole; v0 += 32 * kCopyVecs) {
-      uint4 w[kCopyVecs];      // (all loads out before the first store)
+    constexpr bool kLogit = kShares > 0;
+    const int label = kLogit ? a.has.label(source[i]) : 0;
+    // (with more than kDirectRows rows, a column-major weight's labels are not apart)
+    constexpr bool kByColumn = kShares == 8;
+    const bool by_row = kLogit && !(kByColumn && a.w_column_major);
+    const uint16_t* of_label = !kLogit ? nullptr : by_row ? a.w + label * a.ldw : a.w + label;
+    float share[kLogit ? kShares : 1] = {};
+    float lse = 0.0f, bias = 0.0f;
+    if constexpr (kLogit) {
+      lse = a.lse_in[source[i]];
+      if (a.bias != nullptr) bias = from16<kBf16>(a.bias[label]);
+      static_assert(kCopyVecs % kShares == 0, "a lane's vectors belong to the shares in turn");
+      if (kByColumn && !by_row) {
+        constexpr int kAtOnce = 16;
+        for (int c0 = lane; c0 < a.hidden; c0 += 32 * kAtOnce) {
+          uint16_t p[kAtOnce], q[kAtOnce];
 #pragma unroll
-      for (int j = 0; j < kCopyVecs; ++j)
-        if (v0 + 32 * j < whole) w[j] = reinterpret_cast<const uint4*>(src)[v0 + 32 * j];
+          for (int j = 0; j < kAtOnce; ++j) {
+            const int c = c0 + 32 * j;
+            p[j] = c < a.hidden ? src[c] : 0;
+            q[j] = c < a.hidden ? of_label[c * a.ldw] : 0;
+          }
 #pragma unroll
-      for (int j = 0; j < kCopyVecs; ++j)
-        if (v0 + 32 * j < whole) reinterpret_cast<uint4*>(dst)[v0 + 32 * j] = w[j];
+          for (int j = 0; j < kAtOnce; ++j)
+            if (c0 + 32 * j < a.hidden) share[j % kShares] = fmaf(from16<kBf16>(p[j]), from16<kBf16>(q[j]), share[j % kShares]);
+        }
+      }
     }
-    for (int c = whole * 8 + lane; c < a.hidden; c += 32) dst[c] = src[c];
+    for (int v0 = lane; v0 < whole; v0 += 32 * kCopyVecs) {
+      uint4 w[kCopyVecs], q[kLogit ? kCopyVecs : 1];      // (all loads out before the first store)
+#pragma unroll
+      for (int j = 0; j < kCopyVecs; ++j) {
+        if (v0 + 32 * j < whole) {
+          w[j] = reinterpret_cast<const uint4*>(src)[v0 + 32 * j];
+          if constexpr (kLogit)
+            if (by_row) q[j] = reinterpret_cast<const uint4*>(of_label)[v0 + 32 * j];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kCopyVecs; ++j) {
+        if (v0 + 32 * j < whole) {
+          reinterpret_cast<uint4*>(dst)[v0 + 32 * j] = w[j];
+          if constexpr (kLogit)
+            if (by_row) share[j % kShares] = dot_vec<kBf16>(w[j], q[j], share[j % kShares]);
+        }
+      }
+    }
+    for (int c = whole * 8 + lane; c < a.hidden; c += 32) {
+      dst[c] = src[c];
+      if constexpr (kLogit)
+        if (by_row) share[0] = fmaf(from16<kBf16>(src[c]), from16<kBf16>(of_label[c]), share[0]);
+    }
+    if constexpr (kLogit) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+        for (int j = 0; j < kShares; ++j) share[j] += __shfl_xor_sync(0xffffffffu, share[j], o);
+      }
+      share[0] += bias;
+      float own = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kShares; ++j) own += share[j];
+      own *= a.scale;
+      // (no probability is above 1, however lse was rounded; NaN stays)
+      const float gap = expm1f(own - lse);
+      if (lane == 0) a.gap[before + i] = gap > 0.0f ? 0.0f : gap;
+    }
   }
   if (end != a.rows) return;
   // the last CTA: how many there are, zeros behind them as far as the products read, and the gradient's range
@@ -343,15 +432,7 @@ __device__ __forceinline__ float dot_share(const Loss& a, int64_t row, int label
   const uint16_t* w = a.w + label * a.ldw;
   const int whole = a.hidden / 8;
 #pragma unroll 4
-  for (int v = first; v < whole; v += step) {
-    const uint4 p = reinterpret_cast<const uint4*>(x)[v], q = reinterpret_cast<const uint4*>(w)[v];
-    const uint32_t pw[4] = {p.x, p.y, p.z, p.w}, qw[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      t = fmaf(from16<kBf16>(pw[j] & 0xffffu), from16<kBf16>(qw[j] & 0xffffu), t);
-      t = fmaf(from16<kBf16>(pw[j] >> 16), from16<kBf16>(qw[j] >> 16), t);
-    }
-  }
+  for (int v = first; v < whole; v += step) t = dot_vec<kBf16>(reinterpret_cast<const uint4*>(x)[v], reinterpret_cast<const uint4*>(w)[v], t);
   for (int c = whole * 8 + first; c < a.hidden; c += step) t = fmaf(from16<kBf16>(x[c]), from16<kBf16>(w[c]), t);
   return t;
 }
@@ -576,7 +657,7 @@ struct Space {
 struct Layout {
   Space space;
   size_t control, info, column, weight, start, has, packed, at_target, partial;      // forward
-  size_t inverse, grad, bias, acc, split, split_bytes;                               // backward
+  size_t gap, inverse, grad, bias, acc, split, split_bytes;                          // backward
   int64_t ldp, slots, ldg, ld_acc, plane;      // plane 0: dx is not cut into planes
   Pieces pieces;
   int planes;
@@ -610,6 +691,7 @@ Layout layout_for(const ixk_linear_loss_desc& d, bool backward) {
     l.partial = l.space.take(sizeof(float2) * l.slots * N);
     return l;
   }
+  if (d.entries == 0 && labels_apart(d)) l.gap = l.space.take(4 * N);
   l.inverse = l.space.take(4 * N);
   l.pieces = pieces_for(N, V);
   l.ldg = round_up(l.pieces.columns, kPitchUnit);
@@ -723,8 +805,10 @@ int targets_of(const ixk_linear_loss_desc& d, const Layout& l, char* ws, const v
   return launch_overlapped(fn, dim3(static_cast<unsigned>(ctas)), dim3(32 * kListWarps), 0, stream, a);
 }
 
+// (w and bias: backward with labels apart, else nullptr)
 int gather(const ixk_linear_loss_desc& d, const Layout& l, char* ws, const HasTarget& has, const void* x, float* loss, float* lse,
-           const float* lse_in, const float* grad_loss, float factor, bool want_dw, int sm_count, cudaStream_t stream) {
+           const void* w, const void* bias, const float* lse_in, const float* grad_loss, const Scales& scales, bool want_dw, int sm_count,
+           cudaStream_t stream) {
   const bool backward = loss == nullptr;
   Gather g{};
   g.has = has;
@@ -744,7 +828,7 @@ int gather(const ixk_linear_loss_desc& d, const Layout& l, char* ws, const HasTa
   g.lse_in = lse_in;
   g.grad_loss = grad_loss;
   g.grad_stride = d.grad_loss_stride;
-  g.factor = factor;
+  g.factor = scales.grad;
   g.top = !backward ? 0.0f : d.dtype == IXK_F16 ? 0x1p13f : 1.0f;
   if (backward && d.rows > kDirectRows) {
     g.dx_tiles_n = static_cast<int>((d.hidden + gemm::kTwoTile - 1) / gemm::kTwoTile);
@@ -754,7 +838,18 @@ int gather(const ixk_linear_loss_desc& d, const Layout& l, char* ws, const HasTa
     g.max_planes = l.planes;
   }
   const int64_t ctas = (d.rows + g.rows_per_cta - 1) / g.rows_per_cta;
-  return launch_overlapped(gather_kernel, dim3(static_cast<unsigned>(ctas)), dim3(kGatherThreads), 0, stream, g);
+  auto go = [&](auto* fn) { return launch_overlapped(fn, dim3(static_cast<unsigned>(ctas)), dim3(kGatherThreads), 0, stream, g); };
+  if (w == nullptr) return go(gather_kernel<false, 0>);
+  g.gap = reinterpret_cast<float*>(ws + l.gap);
+  g.w = static_cast<const uint16_t*>(w);
+  g.bias = static_cast<const uint16_t*>(bias);
+  g.ldw = d.w_stride;
+  g.w_column_major = d.w_order == IXK_COL_MAJOR ? 1 : 0;
+  g.scale = scales.logits;
+  return loss_shape(d.rows, [&](auto rows, auto threads) {
+    constexpr int kShares = decltype(threads)::value / 32 / decltype(rows)::value;
+    return go(d.dtype == IXK_BF16 ? gather_kernel<true, kShares> : gather_kernel<false, kShares>);
+  });
 }
 
 Pass pass_of(const ixk_linear_loss_desc& d, const Scales& s, const void* x, int64_t ldx, const void* w, const void* bias, const Targets& t) {
@@ -795,7 +890,7 @@ int forward(const char* name, const ixk_linear_loss_desc* d, bool distill, const
   if ((rc = targets_of(*d, l, ws, index, teacher, s, &t, &has)) != IXK_OK) return rc;
   Pass p = pass_of(*d, scales, x, d->x_stride, w, bias, t);
   if (l.gathered) {
-    if ((rc = gather(*d, l, ws, has, x, loss, lse, nullptr, nullptr, 0.0f, false, dev.sm_count, s)) != IXK_OK) return rc;
+    if ((rc = gather(*d, l, ws, has, x, loss, lse, nullptr, nullptr, nullptr, nullptr, scales, false, dev.sm_count, s)) != IXK_OK) return rc;
     p.x = ws + l.packed;
     p.ldx = l.ldp;
     p.active_rows = &reinterpret_cast<const Control*>(ws + l.control)->active;
@@ -826,16 +921,11 @@ int forward(const char* name, const ixk_linear_loss_desc* d, bool distill, const
   a.bias = static_cast<const uint16_t*>(bias);
   a.hidden = static_cast<int>(d->hidden);
   a.scale = scales.logits;
-  auto go = [&](auto rows, auto threads) -> int {
+  return loss_shape(d->rows, [&](auto rows, auto threads) -> int {
     constexpr int kRows = decltype(rows)::value, kThreads = decltype(threads)::value;
     auto* fn = d->dtype == IXK_BF16 ? loss_kernel<kRows, kThreads, true> : loss_kernel<kRows, kThreads, false>;
     return launch_overlapped(fn, dim3(static_cast<unsigned>((d->rows + kRows - 1) / kRows)), dim3(kThreads), 0, s, a);
-  };
-  // (rows side by side are one read of up to 256 bytes; few rows want a CTA each)
-  using std::integral_constant;
-  if (d->rows >= 4096) return go(integral_constant<int, 32>{}, integral_constant<int, 1024>{});
-  if (d->rows >= 512) return go(integral_constant<int, 8>{}, integral_constant<int, 1024>{});
-  return go(integral_constant<int, 1>{}, integral_constant<int, 256>{});
+  });
 }
 
 int backward(const char* name, const ixk_linear_loss_desc* d, bool distill, const void* x, const void* w, const void* bias,
@@ -868,7 +958,9 @@ int backward(const char* name, const ixk_linear_loss_desc* d, bool distill, cons
   Targets t{};
   HasTarget has{};
   if ((rc = targets_of(*d, l, ws, index, teacher, s, &t, &has)) != IXK_OK) return rc;
-  if ((rc = gather(*d, l, ws, has, x, nullptr, nullptr, lse, grad_loss, scales.grad, dw != nullptr, dev.sm_count, s)) != IXK_OK) return rc;
+  if ((rc = gather(*d, l, ws, has, x, nullptr, nullptr, t.apart ? w : nullptr, bias, lse, grad_loss, scales, dw != nullptr, dev.sm_count, s)) != IXK_OK)
+    return rc;
+  if (t.apart) t.gap = reinterpret_cast<const float*>(ws + l.gap);
   Pass p = pass_of(*d, scales, ws + l.packed, l.ldp, w, bias, t);
   const Control* control = reinterpret_cast<const Control*>(ws + l.control);
   p.active_rows = &control->active;

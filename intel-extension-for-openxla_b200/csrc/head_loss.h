@@ -15,6 +15,7 @@ struct Targets {
   int wide;                 // 64-bit labels
   int64_t ignore_index;
   int apart;                // statistics: the label's column is left out of the sum, the caller makes its logit
+  const float* gap;         // labels apart, gradient: of x's rows, the label's p - 1
   const int* column;        // distillation: [rows][entries] ascending, kNoColumn behind the last one
   const float* weight;      // [rows][entries]
   const uint16_t* start;    // [rows][starts]: the first entry at or behind column i * kStartUnit

@@ -7,7 +7,9 @@
 //                loss is made of, so the loss kernel makes it again in fp32 where that is a row of w to read)
 //   gradient     G = g (softmax(z) - target weights), g relative to the batch's largest, rounded once to the 16-bit operand
 //                of the two products that follow (dx = G w, dw = G^T x): a rounding error of at most 2^-8 or 2^-11 of each
-//                entry, as of any activation gradient, independent from entry to entry
+//                entry, as of any activation gradient, independent from entry to entry.  p - 1 of a label apart is handed in, made
+//                of the same fp32 logit as lse; the other targets' p - q is made of the logits that lse was made of, chunk of K by
+//                chunk: where the model is sure of a token, or agrees with its teacher, the logit's own error would be as large
 //
 // Both are 2 N D V flops on the tensor cores, which bound them from hidden sizes of about 600 on: 2048 x 4096 x 51200 532 and
 // 530 us alone, 1.61 PFLOP/s, and as much as the power limit leaves of that in a row of such calls.  Below, the epilogue does:
@@ -57,7 +59,9 @@ constexpr float kLog2E = 1.4426950408889634f;
 // memory, which holds up the next one's products (16 slabs cost 3 % of 4096 x 32768 x 4096, 661 -> 685 us).  A tile's chunks are
 // of equal length, at most this.
 constexpr int kChunkSlabs = 24;
-enum class Mode { kStats, kStatsChunks, kGrad };     // statistics of one chunk, of several; gradient
+// The gradient takes the same chunks where its targets' entries come from the tile (7355 x 3520 x 8144 column-major, forward and
+// backward: 1224 -> 1253 us).
+enum class Mode { kStats, kStatsChunks, kGrad, kGradChunks };     // statistics of one chunk, of several; gradient the same
 enum : int { kSiteProducer = 601, kSiteFull = 602, kSiteAcc = 603, kSiteEpilogue = 604 };
 
 struct Args {
@@ -172,7 +176,7 @@ template <bool kPair, Mode kMode>
 __global__ void __launch_bounds__(kThreads, 1)
 head_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
             const __grid_constant__ CUtensorMap tmap_g, const Args args) {
-  constexpr bool kGrad = kMode == Mode::kGrad, kChunks = kMode == Mode::kStatsChunks;
+  constexpr bool kGrad = kMode == Mode::kGrad || kMode == Mode::kGradChunks, kChunks = kMode == Mode::kStatsChunks || kMode == Mode::kGradChunks;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
@@ -439,6 +443,58 @@ head_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
         ptx::f32x2_split(ptx::add2(part0, part1), a, b);
         sum += a + b;
       };
+      // the same columns as 16-bit entries of the gradient
+      auto gradient = [&](float (&v)[32], int col, int count, uint32_t* words) {
+        const int col_end = col + count;
+        if (args.bias != nullptr) add_bias(args, col, count, v);
+        const bool hit = __any_sync(0xffffffffu, walk.next < col_end);
+        const uint64_t scale_pair = ptx::f32x2(s2, s2), lse_pair = ptx::f32x2(-lse2, -lse2);
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          float e0, e1;
+          ptx::f32x2_split(ptx::fma2(ptx::f32x2(v[i], v[i + 1]), scale_pair, lse_pair), e0, e1);
+          v[i] = ptx::ex2_approx(e0) * coef;
+          v[i + 1] = ptx::ex2_approx(e1) * coef;
+        }
+        if (hit) {
+          box_put(box, lane, v);
+          while (walk.next < col_end) {
+            if (walk.next >= col) {
+              const uint32_t addr = box_addr(box, lane, walk.next - col);
+              if (args.targets.apart) {
+                box_write(addr, coef * args.targets.gap[row]);
+              } else {
+                const float weight = args.targets.labels != nullptr ? 1.0f : args.targets.weight[orig * walk.entries + walk.at];
+                box_write(addr, box_read(addr) - coef * weight);
+              }
+            }
+            walk.step();
+          }
+          box_get(box, lane, v);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) words[i] = active ? pack2(v[2 * i], v[2 * i + 1], bf16) : 0u;
+      };
+      // 64 columns of them on their way, through this warp's box
+      auto box_free = [&] {      // (the store before this one has read it)
+        if (lane == 0) ptx::bulk_wait_group_read<0>();
+        __syncwarp();
+      };
+      auto leave = [&](const uint32_t (&words)[32], int column) {
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+          const uint32_t addr = box + static_cast<uint32_t>(lane * 128 + ((g ^ (lane & 7)) << 4));
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(words[4 * g]), "r"(words[4 * g + 1]),
+                       "r"(words[4 * g + 2]), "r"(words[4 * g + 3])
+                       : "memory");
+        }
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          ptx::tma_store_3d(&tmap_g, box, column, warp_row, 0);
+          ptx::bulk_commit_group();
+        }
+      };
       for (int n = n_begin; n < n_end; ++n) {
         const int n0 = n * args.tile_n, limit = min(args.tile_n, args.count - n0);
         if constexpr (kChunks) {
@@ -472,14 +528,29 @@ head_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
           }
           if (!alive) break;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int c0 = half * 64 + (q >> 1) * 128 + (q & 1) * 32;
-            if (work && c0 < limit) {
+          for (int g = 0; g < 2; ++g) {
+            const int g0 = half * 64 + g * 128;
+            if (!work || g0 >= limit) continue;
+            uint32_t words[32];
+            if constexpr (kGrad) box_free();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int c0 = g0 + 32 * h, count = min(32, limit - c0);
               float v[32];
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = acc[q >> 1][(q & 1) * 32 + i];
-              take(v, args.first + n0 + c0, min(32, limit - c0));
+              for (int i = 0; i < 32; ++i) v[i] = acc[g][32 * h + i];
+              if constexpr (kGrad) {
+                if (count > 0) {
+                  gradient(v, args.first + n0 + c0, count, words + 16 * h);
+                } else {
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) words[16 * h + i] = 0u;
+                }
+              } else if (count > 0) {
+                take(v, args.first + n0 + c0, count);
+              }
             }
+            if constexpr (kGrad) leave(words, n0 + g0);
           }
           continue;
         }
@@ -493,69 +564,25 @@ head_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ 
 #pragma unroll 1
           for (int g0 = half * 64; g0 < limit; g0 += 128) {
             uint32_t words[32];
-            if constexpr (kGrad) {     // the store before this one has read the box
-              if (lane == 0) ptx::bulk_wait_group_read<0>();
-              __syncwarp();
-            }
+            if constexpr (kGrad) box_free();
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const int c0 = g0 + 32 * h, count = min(32, limit - c0);
               if (count > 0) {           // warp-uniform
-                const int col = args.first + n0 + c0, col_end = col + count;
                 uint32_t r[32];
                 float v[32];
                 ptx::tmem_ld_32x32(acc + c0, r);
                 ptx::tmem_ld_wait();
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-                if constexpr (!kGrad) {
-                  take(v, col, count);
-                } else {
-                  if (args.bias != nullptr) add_bias(args, col, count, v);
-                  const bool hit = __any_sync(0xffffffffu, walk.next < col_end);
-                  const uint64_t scale_pair = ptx::f32x2(s2, s2), lse_pair = ptx::f32x2(-lse2, -lse2);
-#pragma unroll
-                  for (int i = 0; i < 32; i += 2) {
-                    float e0, e1;
-                    ptx::f32x2_split(ptx::fma2(ptx::f32x2(v[i], v[i + 1]), scale_pair, lse_pair), e0, e1);
-                    v[i] = ptx::ex2_approx(e0) * coef;
-                    v[i + 1] = ptx::ex2_approx(e1) * coef;
-                  }
-                  if (hit) {
-                    box_put(box, lane, v);
-                    while (walk.next < col_end) {
-                      if (walk.next >= col) {
-                        const uint32_t addr = box_addr(box, lane, walk.next - col);
-                        const float weight = args.targets.labels != nullptr ? 1.0f : args.targets.weight[orig * walk.entries + walk.at];
-                        box_write(addr, box_read(addr) - coef * weight);
-                      }
-                      walk.step();
-                    }
-                    box_get(box, lane, v);
-                  }
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) words[16 * h + i] = active ? pack2(v[2 * i], v[2 * i + 1], bf16) : 0u;
-                }
+                if constexpr (!kGrad) take(v, args.first + n0 + c0, count);
+                else gradient(v, args.first + n0 + c0, count, words + 16 * h);
               } else if constexpr (kGrad) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) words[16 * h + i] = 0u;
               }
             }
-            if constexpr (kGrad) {
-#pragma unroll
-              for (int g = 0; g < 8; ++g) {
-                const uint32_t addr = box + static_cast<uint32_t>(lane * 128 + ((g ^ (lane & 7)) << 4));
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(words[4 * g]), "r"(words[4 * g + 1]),
-                             "r"(words[4 * g + 2]), "r"(words[4 * g + 3])
-                             : "memory");
-              }
-              ptx::fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) {
-                ptx::tma_store_3d(&tmap_g, box, n0 + g0, warp_row, 0);
-                ptx::bulk_commit_group();
-              }
-            }
+            if constexpr (kGrad) leave(words, n0 + g0);
           }
         }
         ptx::tc_fence_before_sync();
@@ -719,10 +746,9 @@ int launch(const Pass& p, const DeviceInfo& dev, cudaStream_t stream) {
   };
   using std::integral_constant;
   constexpr integral_constant<Mode, kGrad ? Mode::kGrad : Mode::kStats> kOne;
-  if constexpr (!kGrad) {
-    constexpr integral_constant<Mode, Mode::kStatsChunks> kMany;
-    if (a.slabs > a.chunk_slabs) return t.pair ? go(std::true_type{}, kMany) : go(std::false_type{}, kMany);
-  }
+  constexpr integral_constant<Mode, kGrad ? Mode::kGradChunks : Mode::kStatsChunks> kMany;
+  // (a gradient with labels apart has its small differences from elsewhere)
+  if (a.slabs > a.chunk_slabs && !(kGrad && a.targets.apart)) return t.pair ? go(std::true_type{}, kMany) : go(std::false_type{}, kMany);
   return t.pair ? go(std::true_type{}, kOne) : go(std::false_type{}, kOne);
 }
 
