@@ -478,24 +478,35 @@ __global__ void __launch_bounds__(kThreads) loss_kernel(const Loss a) {
     if (part < n) stat[part][r] = join(stat[part][r], stat[part + n][r]);
     __syncthreads();
   }
-  float own = 0.0f;      // the label's logit
+  float of_label = 0.0f;      // labels apart: the loss
   if (part == 0) {
     float2 all = stat[0][r];
     if (a.apart) {
+      float own = 0.0f;       // the label's logit
 #pragma unroll
       for (int i = 0; i < kThreads / 32 / kRows; ++i) own += logit[i][r];
       own *= a.scale;
-      // (an infinite logit has to make the sum infinite, not undefined)
       const float t2 = own * kLog2E;
-      all = t2 == INFINITY ? make_float2(FLT_MAX, INFINITY) : t2 == -INFINITY ? all : join(all, make_float2(t2, 1.0f));
+      if (t2 < INFINITY && all.x <= t2) {
+        // at least as large as all others: ln(1 + their sum over its exponential), as small as it may be
+        of_label = log1pf(all.y * exp2f(all.x - t2));
+        row_lse[r] = own + of_label;
+      } else {
+        // (an infinite logit has to make the sum infinite, not undefined)
+        all = t2 == INFINITY ? make_float2(FLT_MAX, INFINITY) : t2 == -INFINITY ? all : join(all, make_float2(t2, 1.0f));
+        const float lse = fmaf(all.x, kLn2, logf(all.y));
+        of_label = lse - own;
+        row_lse[r] = lse;
+      }
+    } else {
+      row_lse[r] = fmaf(all.x, kLn2, logf(all.y));
     }
-    row_lse[r] = fmaf(all.x, kLn2, logf(all.y));
   }
   __syncthreads();
   const float lse = row_lse[r];
   float t = 0.0f;
   if (a.apart) {
-    if (part == 0) t = lse - own;
+    t = of_label;
   } else if (there) {
     for (int k = part; k < a.entries; k += kParts) {
       const float q = a.weight != nullptr ? a.weight[orig * a.entries + k] : 1.0f;
@@ -510,7 +521,10 @@ __global__ void __launch_bounds__(kThreads) loss_kernel(const Loss a) {
   }
   if (part == 0 && there) {
     const bool counts = a.active != nullptr || a.has(orig);
-    a.loss[orig] = counts ? share[0][r] * a.factor : 0.0f;
+    // (lse - logit of a label that is all there is may come out below 0 by a rounding; a divergence from entries that appear
+    // twice is below 0 by its definition)
+    const float sum = a.weight == nullptr && share[0][r] < 0.0f ? 0.0f : share[0][r];
+    a.loss[orig] = counts ? sum * a.factor : 0.0f;
     a.lse[orig] = counts ? lse : 0.0f;
   }
 }

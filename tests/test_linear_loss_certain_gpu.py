@@ -77,3 +77,25 @@ def test_distillation_from_a_teacher_that_agrees(pkg, cuda, dtype, N):
     grads = pkg.linear_distillation_backward(x, w, index, logits, lse, g, bias=b)
     r = reference(x, w, b, *teacher_args(index, logits, 1.0, V), 1.0, 1.0, g)
     check(r, x.dtype, loss, grads, 1.0)
+
+
+@pytest.mark.parametrize("order", ["vd", "dv"])
+@pytest.mark.parametrize("N", [60, 300, 700, 4200])
+def test_losses_next_to_zero(pkg, cuda, order, N):
+    """1 - p from 1e-3 down to 1e-9: no loss is below 0, and where the label's logit is a product of its own (row-major, or up to
+    128 rows) a loss is right to 2^-12 of itself: its terms' logits are off by up to 6e-5 each way, their exponentials by 2^-21."""
+    gen = torch.Generator().manual_seed(N)
+    d, v = 1024, 1000
+    w = (torch.randn(v, d, generator=gen) * 0.04).bfloat16().to(cuda)
+    labels = torch.randint(0, v, (N,), generator=gen).to(cuda)
+    lift = (15.0 + 15.0 * torch.rand(N, 1, generator=gen)).to(cuda) / (0.0016 * d)
+    x = ((torch.randn(N, d, generator=gen) * 0.5).to(cuda) + lift * w[labels].float()).bfloat16()
+    z = x.to(D64) @ w.to(D64).t()
+    rest = torch.logsumexp(z.scatter(1, labels[:, None], -torch.inf), 1) - z.gather(1, labels[:, None])[:, 0]
+    want = torch.log1p(torch.exp(rest))
+    assert want.min() < 1e-7 and want.max() > 1e-4
+    loss, lse = pkg.linear_cross_entropy(x, w if order == "vd" else w.t().contiguous().t(), labels)
+    assert (loss >= 0).all()
+    assert (lse.to(D64) - torch.logsumexp(z, 1)).abs().max() < 2.0 ** -13
+    if order == "vd" or N <= 128:
+        assert ((loss.to(D64) - want).abs() <= 2.0 ** -12 * want).all()
