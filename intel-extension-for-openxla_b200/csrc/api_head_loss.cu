@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(32 * kListWarps) lists_kernel(const Lists a) {
       if (k < a.entries) {
         const int64_t at = row * a.index_stride + k;
         const int64_t c = a.wide ? static_cast<const int64_t*>(a.index)[at] : static_cast<const int*>(a.index)[at];
-        const float logit = load_as_float(a.teacher, row * a.teacher_stride + k, a.teacher_dtype) * a.inv_temperature;
+        const float logit = load_as_float(a.teacher, row * a.teacher_stride + k, a.teacher_dtype);
         if (c >= 0 && c < a.vocab && logit != -INFINITY) {
           col[e] = static_cast<int>(c);
           t[e] = logit;
@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(32 * kListWarps) lists_kernel(const Lists a) {
     float sum = 0.0f;
 #pragma unroll
     for (int e = 0; e < kListPer; ++e) {
-      t[e] = col[e] != kNoColumn ? expf(t[e] - top) : 0.0f;
+      t[e] = col[e] != kNoColumn ? expf((t[e] - top) * a.inv_temperature) : 0.0f;   // (a logit over T may be infinite)
       sum += t[e];
     }
 #pragma unroll

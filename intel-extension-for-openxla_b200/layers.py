@@ -409,8 +409,10 @@ def _head_targets(h, weight, target, temperature):
         return torch.where(ok, target, 0)[:, None].long(), ok[:, None].float(), ok
     index, logits = target
     ok = (index >= 0) & (index < vocab) & (logits > -math.inf)
-    t = torch.where(ok, logits.float() / temperature, -math.inf)
+    t = torch.where(ok, logits.float(), -math.inf)
     rows = ok.any(1)
+    # (differences first: a logit over the temperature may be infinite)
+    t = (t - torch.where(rows, t.amax(1), 0.0)[:, None]) / temperature
     return torch.where(ok, index, 0).long(), torch.where(ok, torch.softmax(torch.where(rows[:, None], t, 0.0), 1), 0.0), rows
 
 

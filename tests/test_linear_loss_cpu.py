@@ -1,5 +1,7 @@
 """CPU: what the host decides for the losses at the vocabulary head: the pieces of the vocabulary, scratch, the workspace query."""
 import ctypes
+import importlib
+import math
 import os
 import subprocess
 import tempfile
@@ -67,3 +69,17 @@ def test_the_workspace_query_knows_the_weights_layout(pkg, rows, entries):
             d.rows, d.hidden, d.vocab, d.entries, d.w_order = rows, 512, 4000, entries, order
             want = lib.ixk_linear_loss_workspace_bytes(ctypes.byref(d), int(backward))
             assert pkg.linear_loss_workspace_bytes(x, w, entries, backward) == want > 0
+
+
+def test_plain_form_with_teacher_logits_at_the_ends_of_the_type(pkg):
+    """Entries masked by the type's lowest number are there: alone they weigh alike, beside others nothing."""
+    layers = importlib.import_module(pkg.__name__ + ".layers")
+    low = torch.finfo(torch.float32).min
+    logits = torch.tensor([[low, low, low, low], [1.0, 2.0, low, low], [-low, 0.0, -low, low], [1.0, -math.inf, 3.0, 2.0]])
+    index = torch.tensor([[1, 2, 3, 4]] * 4)
+    _, q, rows = layers._head_targets(None, torch.empty(10, 8), (index, logits), 0.25)
+    e = [math.exp(-4.0), math.exp(-8.0)]
+    want = torch.tensor([[0.25] * 4, [e[0] / (1 + e[0]), 1 / (1 + e[0]), 0, 0], [0.5, 0, 0.5, 0],
+                         [e[1] / (1 + e[0] + e[1]), 0, 1 / (1 + e[0] + e[1]), e[0] / (1 + e[0] + e[1])]])
+    assert rows.all()
+    assert (q - want).abs().max() < 1e-6
