@@ -243,9 +243,6 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Gather a) 
     for (int w = 0; w < kGatherThreads / 32; ++w) t += warp_count[w];
     return t;
   };
-  const int row = first + threadIdx.x;
-  const bool mine = static_cast<int>(threadIdx.x) < a.rows_per_cta && row < end;
-  const bool keep = mine && a.has(row);
   // every CTA counts the rows in front of its own
   int before = 0;
   float largest = 0.0f;        // (the last CTA: of grad_loss)
@@ -274,103 +271,109 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const Gather a) 
   else if (a.has.wide) count(static_cast<const int64_t*>(a.has.labels), int64_t(-1), is_label);
   else count(static_cast<const int*>(a.has.labels), -1, is_label);
   before = block_sum(before);
-  const unsigned ballot = __ballot_sync(0xffffffffu, keep);
-  const int here = block_sum(lane == 0 ? __popc(ballot) : 0);
-  if (mine) {
-    int at = __popc(ballot & ((1u << lane) - 1u));
-    for (int w = 0; w < warp; ++w) at += warp_count[w];
-    if (keep) {
-      source[at] = row;
-      RowInfo info{row, kNoColumn, 0.0f, 0.0f};
-      if (a.has.labels != nullptr) info.label = a.has.label(row);
-      if (a.grad_loss != nullptr) {
-        info.lse2 = a.lse_in[row] * kLog2E;
-        info.coef = a.grad_loss[row * a.grad_stride] * a.factor;
-        largest = fmaxf(largest, fabsf(info.coef));
-      }
-      a.info[before + at] = info;
-    } else if (a.loss != nullptr) {
-      a.loss[row] = 0.0f;
-      a.lse[row] = 0.0f;
-    }
-    if (a.inverse != nullptr) a.inverse[row] = keep ? before + at : -1;
-  }
-  __syncthreads();
   const int whole = a.hidden / 8;
-  for (int i = warp; i < here; i += kGatherThreads / 32) {
-    const uint16_t* src = a.x + source[i] * a.ldx;
-    uint16_t* dst = a.packed + (before + i) * a.ldp;
-    constexpr bool kLogit = kShares > 0;
-    const int label = kLogit ? a.has.label(source[i]) : 0;
-    // (with more than kDirectRows rows, a column-major weight's labels are not apart)
-    constexpr bool kByColumn = kShares == 8;
-    const bool by_row = kLogit && !(kByColumn && a.w_column_major);
-    const uint16_t* of_label = !kLogit ? nullptr : by_row ? a.w + label * a.ldw : a.w + label;
-    float share[kLogit ? kShares : 1] = {};
-    float lse = 0.0f, bias = 0.0f;
-    if constexpr (kLogit) {
-      lse = a.lse_in[source[i]];
-      if (a.bias != nullptr) bias = from16<kBf16>(a.bias[label]);
-      static_assert(kCopyVecs % kShares == 0, "a lane's vectors belong to the shares in turn");
-      if (kByColumn && !by_row) {
-        constexpr int kAtOnce = 16;
-        for (int c0 = lane; c0 < a.hidden; c0 += 32 * kAtOnce) {
-          uint16_t p[kAtOnce], q[kAtOnce];
+  for (int from = first; from < end; from += kGatherThreads) {      // (a row a thread; block_sum's barriers part the rounds)
+    const int row = from + threadIdx.x;
+    const bool mine = row < end;
+    const bool keep = mine && a.has(row);
+    const unsigned ballot = __ballot_sync(0xffffffffu, keep);
+    const int here = block_sum(lane == 0 ? __popc(ballot) : 0);
+    if (mine) {
+      int at = __popc(ballot & ((1u << lane) - 1u));
+      for (int w = 0; w < warp; ++w) at += warp_count[w];
+      if (keep) {
+        source[at] = row;
+        RowInfo info{row, kNoColumn, 0.0f, 0.0f};
+        if (a.has.labels != nullptr) info.label = a.has.label(row);
+        if (a.grad_loss != nullptr) {
+          info.lse2 = a.lse_in[row] * kLog2E;
+          info.coef = a.grad_loss[row * a.grad_stride] * a.factor;
+          largest = fmaxf(largest, fabsf(info.coef));
+        }
+        a.info[before + at] = info;
+      } else if (a.loss != nullptr) {
+        a.loss[row] = 0.0f;
+        a.lse[row] = 0.0f;
+      }
+      if (a.inverse != nullptr) a.inverse[row] = keep ? before + at : -1;
+    }
+    __syncthreads();
+    for (int i = warp; i < here; i += kGatherThreads / 32) {
+      const uint16_t* src = a.x + source[i] * a.ldx;
+      uint16_t* dst = a.packed + (before + i) * a.ldp;
+      constexpr bool kLogit = kShares > 0;
+      const int label = kLogit ? a.has.label(source[i]) : 0;
+      // (with more than kDirectRows rows, a column-major weight's labels are not apart)
+      constexpr bool kByColumn = kShares == 8;
+      const bool by_row = kLogit && !(kByColumn && a.w_column_major);
+      const uint16_t* of_label = !kLogit ? nullptr : by_row ? a.w + label * a.ldw : a.w + label;
+      float share[kLogit ? kShares : 1] = {};
+      float lse = 0.0f, bias = 0.0f;
+      if constexpr (kLogit) {
+        lse = a.lse_in[source[i]];
+        if (a.bias != nullptr) bias = from16<kBf16>(a.bias[label]);
+        static_assert(kCopyVecs % kShares == 0, "a lane's vectors belong to the shares in turn");
+        if (kByColumn && !by_row) {
+          constexpr int kAtOnce = 16;
+          for (int c0 = lane; c0 < a.hidden; c0 += 32 * kAtOnce) {
+            uint16_t p[kAtOnce], q[kAtOnce];
 #pragma unroll
-          for (int j = 0; j < kAtOnce; ++j) {
-            const int c = c0 + 32 * j;
-            p[j] = c < a.hidden ? src[c] : 0;
-            q[j] = c < a.hidden ? of_label[c * a.ldw] : 0;
+            for (int j = 0; j < kAtOnce; ++j) {
+              const int c = c0 + 32 * j;
+              p[j] = c < a.hidden ? src[c] : 0;
+              q[j] = c < a.hidden ? of_label[c * a.ldw] : 0;
+            }
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j)
+              if (c0 + 32 * j < a.hidden) share[j % kShares] = fmaf(from16<kBf16>(p[j]), from16<kBf16>(q[j]), share[j % kShares]);
           }
-#pragma unroll
-          for (int j = 0; j < kAtOnce; ++j)
-            if (c0 + 32 * j < a.hidden) share[j % kShares] = fmaf(from16<kBf16>(p[j]), from16<kBf16>(q[j]), share[j % kShares]);
         }
       }
-    }
-    for (int v0 = lane; v0 < whole; v0 += 32 * kCopyVecs) {
-      uint4 w[kCopyVecs], q[kLogit ? kCopyVecs : 1];      // (all loads out before the first store)
+      for (int v0 = lane; v0 < whole; v0 += 32 * kCopyVecs) {
+        uint4 w[kCopyVecs], q[kLogit ? kCopyVecs : 1];      // (all loads out before the first store)
 #pragma unroll
-      for (int j = 0; j < kCopyVecs; ++j) {
-        if (v0 + 32 * j < whole) {
-          w[j] = reinterpret_cast<const uint4*>(src)[v0 + 32 * j];
-          if constexpr (kLogit)
-            if (by_row) q[j] = reinterpret_cast<const uint4*>(of_label)[v0 + 32 * j];
+        for (int j = 0; j < kCopyVecs; ++j) {
+          if (v0 + 32 * j < whole) {
+            w[j] = reinterpret_cast<const uint4*>(src)[v0 + 32 * j];
+            if constexpr (kLogit)
+              if (by_row) q[j] = reinterpret_cast<const uint4*>(of_label)[v0 + 32 * j];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kCopyVecs; ++j) {
+          if (v0 + 32 * j < whole) {
+            reinterpret_cast<uint4*>(dst)[v0 + 32 * j] = w[j];
+            if constexpr (kLogit)
+              if (by_row) share[j % kShares] = dot_vec<kBf16>(w[j], q[j], share[j % kShares]);
+          }
         }
       }
+      for (int c = whole * 8 + lane; c < a.hidden; c += 32) {
+        dst[c] = src[c];
+        if constexpr (kLogit)
+          if (by_row) share[0] = fmaf(from16<kBf16>(src[c]), from16<kBf16>(of_label[c]), share[0]);
+      }
+      if constexpr (kLogit) {
 #pragma unroll
-      for (int j = 0; j < kCopyVecs; ++j) {
-        if (v0 + 32 * j < whole) {
-          reinterpret_cast<uint4*>(dst)[v0 + 32 * j] = w[j];
-          if constexpr (kLogit)
-            if (by_row) share[j % kShares] = dot_vec<kBf16>(w[j], q[j], share[j % kShares]);
+        for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+          for (int j = 0; j < kShares; ++j) share[j] += __shfl_xor_sync(0xffffffffu, share[j], o);
         }
+        share[0] += bias;
+        float own = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kShares; ++j) own += share[j];
+        own *= a.scale;
+        // (no probability is above 1, however lse was rounded; NaN stays)
+        const float gap = expm1f(own - lse);
+        if (lane == 0) a.gap[before + i] = gap > 0.0f ? 0.0f : gap;
       }
     }
-    for (int c = whole * 8 + lane; c < a.hidden; c += 32) {
-      dst[c] = src[c];
-      if constexpr (kLogit)
-        if (by_row) share[0] = fmaf(from16<kBf16>(src[c]), from16<kBf16>(of_label[c]), share[0]);
-    }
-    if constexpr (kLogit) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-#pragma unroll
-        for (int j = 0; j < kShares; ++j) share[j] += __shfl_xor_sync(0xffffffffu, share[j], o);
-      }
-      share[0] += bias;
-      float own = 0.0f;
-#pragma unroll
-      for (int j = 0; j < kShares; ++j) own += share[j];
-      own *= a.scale;
-      // (no probability is above 1, however lse was rounded; NaN stays)
-      const float gap = expm1f(own - lse);
-      if (lane == 0) a.gap[before + i] = gap > 0.0f ? 0.0f : gap;
-    }
+    before += here;
   }
   if (end != a.rows) return;
   // the last CTA: how many there are, zeros behind them as far as the products read, and the gradient's range
-  const int total = before + here;
+  const int total = before;
   if (threadIdx.x == 0) a.control->active = total;
   if (warp == 0 && a.dx_tiles_n > 0) {
     const int64_t tiles = (static_cast<int64_t>(total) + gemm::kTwoTile - 1) / gemm::kTwoTile * a.dx_tiles_n;
@@ -832,8 +835,8 @@ int gather(const ixk_linear_loss_desc& d, const Layout& l, char* ws, const HasTa
   g.ldp = l.ldp;
   g.rows = static_cast<int>(d.rows);
   g.hidden = static_cast<int>(d.hidden);
-  // (each CTA counts the rows in front of it: at most 1024 CTAs while a CTA's rows fit its threads)
-  g.rows_per_cta = static_cast<int>(std::min<int64_t>(std::max<int64_t>(8, (d.rows + 1023) / 1024), kGatherThreads));
+  // (each CTA counts the rows in front of it: at most 1024 CTAs, or their number would count twice)
+  g.rows_per_cta = static_cast<int>(std::max<int64_t>(8, (d.rows + 1023) / 1024));
   g.control = reinterpret_cast<Control*>(ws + l.control);
   g.info = reinterpret_cast<RowInfo*>(ws + l.info);
   g.inverse = backward ? reinterpret_cast<int*>(ws + l.inverse) : nullptr;
