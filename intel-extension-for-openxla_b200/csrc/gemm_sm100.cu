@@ -1155,6 +1155,7 @@ int pick_block_n(int64_t M, int64_t N, int64_t batch, int sm_count) {
 }
 
 int launch(const Problem& p, const DeviceInfo& dev, cudaStream_t stream) {
+  if (p.needs_two()) return fail(IXK_INVALID_ARGUMENT, "gemm: limits or a scale on the GPU outside launch_two");
   const int es = p.kind == ptx::kKindF16 ? 2 : (p.kind == ptx::kKindTf32 ? 4 : 1);
   const int slab_elems = kSlabBytes / es;
   int bn = p.force_block_n > 0 ? p.force_block_n : pick_block_n(p.M, p.N, p.batch, dev.sm_count);
@@ -1259,7 +1260,6 @@ int launch(const Problem& p, const DeviceInfo& dev, cudaStream_t stream) {
   k.act = p.act;
   k.acc_scale = p.acc_scale;
   k.beta = p.beta;
-  k.acc_scale_dev = p.acc_scale_dev;
   k.status_word = dev.status_word;
   const int out_es = (p.out_dtype == IXK_F32 || p.out_dtype == IXK_S32) ? 4 : 2;
   const int bias_es = p.bias_dtype == IXK_F32 ? 4 : 2;

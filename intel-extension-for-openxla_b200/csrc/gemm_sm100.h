@@ -38,11 +38,13 @@ struct Problem {
   int act = kActNone;
   float acc_scale = 1.0f;
   float beta = 0.0f;
-  // What only the GPU knows, nullptr: nothing.  acc_scale is multiplied by *acc_scale_dev.  launch_two only: D's rows from
-  // *m_limit on are not computed; K ends at *k_limit (at most K; the operands hold zeros from there to a multiple of 64).
+  // What only the GPU knows, nullptr: nothing.  launch_two only, the other launches refuse it: acc_scale is multiplied by
+  // *acc_scale_dev; D's rows from *m_limit on are not computed; K ends at *k_limit (at most K; the operands hold zeros from there
+  // to a multiple of 64).
   const int* m_limit = nullptr;
   const int* k_limit = nullptr;
   const float* acc_scale_dev = nullptr;
+  bool needs_two() const { return m_limit != nullptr || k_limit != nullptr || acc_scale_dev != nullptr; }
   int force_block_n = 0;  // tuning override; 0 = heuristic
   int k_chunk = 0;        // > 0: the batches are chunks of K, this many slabs each (the last one what is left), of one A and B
   // Scattered output (row-parallel projection feeding an all-reduce): row block o of D, rows

@@ -349,6 +349,7 @@ int stream_splits(int64_t M, int64_t N, int64_t K, int elem_bytes, size_t worksp
 
 // `partial`: nullptr (one chunk, D finished here) or scratch for splits x M x N floats.
 int launch_stream(const Problem& p, int splits, float* partial, const DeviceInfo& dev, cudaStream_t stream) {
+  if (p.needs_two()) return fail(IXK_INVALID_ARGUMENT, "gemm: limits or a scale on the GPU outside launch_two");
   const int es = p.kind == kKindF16 ? 2 : 1;
   const int slab_elems = kSlabBytes / es;
   const int rows = static_cast<int>((p.M + 15) / 16) * 16;
