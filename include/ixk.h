@@ -413,14 +413,20 @@ size_t ixk_row_norm_bwd_workspace_bytes(const ixk_row_norm_desc* desc);
  * whatever x holds in them.  The backward calls take each row's grad_loss (pitch grad_loss_stride, 0
  * for one number that all rows share) and the forward's lse, make the logits once more piece by piece,
  * and return dx, dweight, dbias (any may be NULL: not wanted).  dtype in {BF16, F16}: x, weight, bias
- * and their gradients.  Logits, statistics and all sums are fp32; the gradient with respect to the
- * logits is rounded to dtype as an operand of the two products (for F16 scaled by a power of two that
- * brings the largest row's into range), each result once.  Results do not depend on timing.
+ * and their gradients.  Logits, statistics and all sums are fp32 (the tensor cores' own additions cut
+ * what they shift out; a label's logit is a sum of rounded ones, except with a column-major weight and
+ * more than 128 rows).  The gradient with respect to the logits, divided by the batch's largest
+ * |grad_loss| (F16: and times 2^13, so that entries down to 2^-37 of the largest row's count), is
+ * rounded to dtype as an operand of the two products; dbias is the sum of the same rounded entries.
+ * Each result is rounded once.  Results do not depend on timing.
  * x, weight: 16-byte aligned, strides multiples of 8 elements (else IXK_INVALID_ARGUMENT /
  * IXK_UNIMPLEMENTED, as for ixk_gemm); everything else only as its elements are.  Workspace:
- * ixk_linear_loss_workspace_bytes(desc, backward) bytes, 256-byte aligned; it grows with the rows, not
- * with rows * vocab (the backward's piece of the logits' gradient is at most 256 MB where 256 columns
- * fit that, beside x's size again in 16 and 32 bits and at most 64 MB for the products). */
+ * ixk_linear_loss_workspace_bytes(desc, backward) bytes, 256-byte aligned (of desc, the sizes, entries
+ * and w_order count).  Forward: x's size again (above 128 rows) and 8 bytes a row and half strip of
+ * columns (a strip is 32 to 2048 columns: 3.3 MB for 2048 rows and 51200 columns).  Backward: a piece of the
+ * logits' gradient, at most 256 MB where 256 columns fit that; x's size again; dx in fp32, up to 16
+ * times where that fits 128 MB; up to 128 rows 64 MB at most for the products' partial sums.
+ * Distillation: 8 bytes an entry (forward 12), and 2 bytes a row and 256 columns. */
 typedef struct ixk_linear_loss_desc {
   int32_t dtype;          /* IXK_BF16 or IXK_F16 */
   int32_t w_order;        /* ixk_order of weight as [vocab, hidden] */
