@@ -360,6 +360,138 @@ int ixk_residual_add(int dtype, int64_t rows, int64_t cols, const void* x,
                      const void* partial, const void* bias, void* out,
                      void* cuda_stream);
 
+/* ------------------------------------------------------ a paged key/value cache */
+/* A decoding step over a cache in pages, for requests of different lengths (the reference's Gemma
+ * example keeps one dense cache, example/gemma/keras_nlp.patch:6-63, as ixk_kv_append and ixk_fmha_fwd
+ * do).  K and V are arrays of pages of page_size tokens; request b's tokens [i * page_size,
+ * (i + 1) * page_size) live in page page_table[b][i].  A token's slot is page * page_size + its place in
+ * the page.  Everything that varies from step to step (lengths, tables, maps, counts) lives on the GPU
+ * as int32, so a step needs nothing from the host and can be captured once and replayed:
+ *   ixk_paged_extend            pages for the new tokens, and their request, position and slot
+ *   ixk_qk_norm_rotary_fwd      per layer: q and k normed and rotated, k and v into their slots
+ *   ixk_fmha_paged_fwd          per layer: attention over the pages
+ *   ixk_paged_keep              after verification: accepted drafts close up, lengths grow, pages return
+ * Between steps request b holds exactly the ceil(lengths[b] / page_size) first places of its table row.
+ * Numbers on the GPU are checked there: whatever they are, no call reads or writes outside its buffers. */
+typedef struct ixk_page_pool {
+  int32_t page_size;      /* tokens of a page, >= 1 */
+  int32_t pages;          /* pages of the cache, = capacity of free_pages; pages * page_size < 2^31 */
+  int32_t requests;       /* B, at most 16384 */
+  int32_t columns;        /* places of a page table row; columns * page_size < 2^31 */
+  int64_t table_stride;   /* elements between rows of page_table */
+} ixk_page_pool;
+/* Request b has lengths[b] tokens in the cache and gets new_tokens[b] more.  Its rows of a packed batch
+ * are row_start[b] .. row_start[b + 1] (row_start: [B + 1], the sums of max(new_tokens, 0), cut at
+ * `rows`, the capacity of the maps).  Pages are taken from the end of free_pages[0, *free_count) in the
+ * order of the requests.  A request whose new tokens do not fit into its table row or into the maps, or that
+ * needs pages when, together with all that fit before it, more are needed than there are, is not
+ * served: granted[b] = 0, no page is taken, its rows' maps are -1.  Otherwise granted[b] =
+ * new_tokens[b], and row r = row_start[b] + j has request[r] = b, position[r] = lengths[b] + j and slot[r].  Rows
+ * behind the last request are -1 as well.  *free_count_out = pages left (may be free_count itself; no
+ * other output may be one of the inputs).  lengths is left as it is until ixk_paged_keep. */
+int ixk_paged_extend(const ixk_page_pool* pool, const int32_t* lengths, const int32_t* new_tokens,
+                     int32_t* page_table, const int32_t* free_pages, const int32_t* free_count,
+                     int32_t* free_count_out, int32_t* granted, int32_t* row_start, int64_t rows,
+                     int32_t* request, int32_t* position, int32_t* slot, void* cuda_stream);
+
+typedef struct ixk_paged_cache {
+  int32_t dtype;          /* IXK_BF16 or IXK_F16 */
+  int32_t page_size;
+  int32_t pages;
+  int32_t heads;          /* key/value heads */
+  int32_t head_size;
+  int32_t layers;         /* ixk_paged_keep: caches of several layers at once; elsewhere 1 */
+  int64_t k_strides[4];   /* layer, page, token, head (elements; multiples of 8) */
+  int64_t v_strides[4];
+} ixk_paged_cache;
+/* Of request b's granted[b] drafts (positions lengths[b] ...) kept[b] stay.  path [B, path_columns] (pitch
+ * path_stride) lists them, in ascending order: the K and V of position lengths[b] + path[b][j] move
+ * to lengths[b] + j, in every layer; an entry that is not above the one before it, or not below
+ * granted[b], ends the path.  path NULL: the first kept[b] stay where they are.  Then lengths_out[b] = lengths[b]
+ * + kept, and the pages above go back to the end of free_pages in the order of the requests.  kept[b] < 0
+ * ends the request: lengths_out[b] = 0 and all of its pages go back.  lengths_out may be lengths,
+ * free_count_out free_count.  The table itself is not written.  cache, k, v: NULL with path NULL.
+ * path_columns at most 1024; K and V 16-byte aligned. */
+int ixk_paged_keep(const ixk_page_pool* pool, const int32_t* lengths, const int32_t* granted,
+                   const int32_t* kept, const int32_t* path, int64_t path_columns, int64_t path_stride,
+                   const int32_t* page_table, int32_t* free_pages, const int32_t* free_count,
+                   int32_t* free_count_out, int32_t* lengths_out, const ixk_paged_cache* cache, void* k,
+                   void* v, void* cuda_stream);
+
+/* Norm of every query and key head and its rotation, in one pass.  With a position p and table rows
+ * cos[p], sin[p] ([places, rotary_dim / 2] fp32, dense):
+ *   r = 1 / sqrt(mean(x^2) + eps)     u = x * r * (gain_offset + gain)      y = u with its first
+ *   rotary_dim elements rotated in pairs: (i, i + rotary_dim / 2), or (2 i, 2 i + 1) where interleaved
+ * rounded once.  q [tokens, heads, head_size], k and v [tokens, kv_heads, head_size] by token and head
+ * strides (they may be slices of one projection).  positions NULL: token t sits at t % places.  A token
+ * whose position is outside [0, places) is left out: nothing of it is written, its gradient is 0, and
+ * it takes no part in the gains' gradients.  Keys go to k_out, or, with `cache`, to their slots, and
+ * values with them; a slot outside the cache is not written.  y may be x.
+ * dtype in {BF16, F16, F32} (with a cache its type); gains NULL (1) or [head_size] of dtype or F32.
+ * head_size a multiple of 8 up to 256, rotary_dim a multiple of 16 (interleaved: 8); strides multiples of 8
+ * elements, pointers 16-byte aligned (positions and slots: as their elements are). */
+typedef struct ixk_qk_desc {
+  int32_t dtype;
+  int32_t param_dtype;
+  int32_t heads, kv_heads, head_size, rotary_dim;
+  int32_t interleaved;
+  int32_t position_bytes;   /* 4 or 8 */
+  float eps, gain_offset;
+  int64_t tokens, places;
+  int64_t q_strides[2], k_strides[2], v_strides[2];   /* token, head */
+  int64_t q_out_strides[2], k_out_strides[2];         /* (backward: of dq and dk) */
+  int64_t gq_strides[2], gk_strides[2];               /* (backward: of the gradients that come in) */
+} ixk_qk_desc;
+int ixk_qk_norm_rotary_fwd(const ixk_qk_desc* desc, const void* q, const void* k, const void* v,
+                           const void* q_gain, const void* k_gain, const float* cos_table,
+                           const float* sin_table, const void* positions, void* q_out, void* k_out,
+                           const ixk_paged_cache* cache, const int32_t* slots, void* k_pages,
+                           void* v_pages, void* cuda_stream);
+/* dq, dk from the gradients of the rotated heads and the forward's inputs; dq_gain, dk_gain (NULL: not
+ * wanted) [head_size] of param_dtype, the sums over tokens and heads in fp32 and in a fixed order: with
+ * either, workspace holds ixk_qk_norm_rotary_bwd_workspace_bytes(desc) bytes, 16-byte aligned.  dq may
+ * be q or grad_q, dk likewise. */
+int ixk_qk_norm_rotary_bwd(const ixk_qk_desc* desc, const void* grad_q, const void* grad_k,
+                           const void* q, const void* k, const void* q_gain, const void* k_gain,
+                           const float* cos_table, const float* sin_table, const void* positions,
+                           void* dq, void* dk, void* dq_gain, void* dk_gain, void* workspace,
+                           size_t workspace_bytes, void* cuda_stream);
+size_t ixk_qk_norm_rotary_bwd_workspace_bytes(const ixk_qk_desc* desc);
+
+/* Attention of packed rows over the pages.  Row j of request b (q, out: row row_start[b] + j; j <
+ * granted[b], which may be smaller than the row_start differences) sees the keys of positions t <
+ * lengths[b], and of the drafts at lengths[b] + i (i < granted[b]) those whose bit i of its mask is set (mask
+ * [rows, mask_words] int32 with pitch mask_stride, bit i % 32 of word i / 32; drafts behind the last word
+ * are not seen); mask NULL: i <= j.  heads is a multiple of the cache's heads: query heads
+ * [g * h, g * (h + 1)) read key head h, g = heads / cache heads, at most 128.
+ *   out = sum p v / sum p,  p = exp(head_scale * q.k)      lse = ln sum p     (fp32 [rows, heads], or NULL)
+ * A row that sees nothing gets out 0 and lse -inf.  Rows that belong to no request are left as they
+ * were.  Values that a row does not see do not reach it, whatever they are (NaN, infinities; anything at
+ * all behind the last token).  A page number outside the cache reads as zeros; positions beyond the
+ * table row are not read.  Scores, statistics and sums are fp32; p is rounded to dtype (to nearest) as an operand
+ * of the second product, and out is divided by the sum of the rounded p (lse: of the fp32 ones).  Results depend on
+ * the lengths and sizes alone, not on timing.
+ * page_size in {8, 16, 32, 64, 128, 256}; head_size a multiple of 8 up to 256; q, out, K and V 16-byte aligned
+ * with strides that are multiples of 8 elements; workspace: ixk_fmha_paged_fwd_workspace_bytes(desc, cache)
+ * bytes, 16-byte aligned. */
+typedef struct ixk_fmha_paged_desc {
+  int32_t heads;
+  int32_t requests;
+  int32_t columns;          /* places of a page table row */
+  int32_t mask_words;
+  float head_scale;
+  int32_t reserved;         /* must be 0 */
+  int64_t rows;             /* capacity of q, out, lse and mask */
+  int64_t table_stride, mask_stride;
+  int64_t q_strides[2], o_strides[2];   /* row, head */
+} ixk_fmha_paged_desc;
+int ixk_fmha_paged_fwd(const ixk_fmha_paged_desc* desc, const ixk_paged_cache* cache, const void* q,
+                       const void* k_pages, const void* v_pages, const int32_t* page_table,
+                       const int32_t* lengths, const int32_t* row_start, const int32_t* granted,
+                       const int32_t* mask, void* out, float* lse, void* workspace,
+                       size_t workspace_bytes, void* cuda_stream);
+size_t ixk_fmha_paged_fwd_workspace_bytes(const ixk_fmha_paged_desc* desc, const ixk_paged_cache* cache);
+
 /* --------------------------------------------------------- row norms, training */
 /* LayerNorm and RMSNorm with gain and shift, the row statistics kept for the backward pass (XLA
  * compiles both from the model's own expressions; the reference has no custom call for them).  Per

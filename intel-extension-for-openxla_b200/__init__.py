@@ -18,7 +18,7 @@ import importlib.machinery
 import importlib.util
 import os
 import struct
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -32,6 +32,8 @@ __all__ = [
     "quantize_fp8", "row_norm_forward", "row_norm_backward", "row_norm_backward_workspace_bytes",
     "linear_cross_entropy", "linear_cross_entropy_backward", "linear_distillation", "linear_distillation_backward",
     "linear_loss_workspace_bytes",
+    "PagedRows", "paged_extend", "paged_keep", "qk_norm_rotary_forward", "qk_norm_rotary_backward",
+    "qk_norm_rotary_backward_workspace_bytes", "fmha_paged_forward", "fmha_paged_workspace_bytes",
 ]
 
 # ----------------------------------------------------------------------------- ABI mirror
@@ -103,6 +105,31 @@ class _LinearLossDesc(ctypes.Structure):
                 ("index_stride", ctypes.c_int64), ("teacher_stride", ctypes.c_int64), ("grad_loss_stride", ctypes.c_int64)]
 
 
+class _PagePool(ctypes.Structure):
+    _fields_ = [("page_size", ctypes.c_int32), ("pages", ctypes.c_int32), ("requests", ctypes.c_int32), ("columns", ctypes.c_int32),
+                ("table_stride", ctypes.c_int64)]
+
+
+class _PagedCache(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("page_size", ctypes.c_int32), ("pages", ctypes.c_int32), ("heads", ctypes.c_int32),
+                ("head_size", ctypes.c_int32), ("layers", ctypes.c_int32), ("k_strides", ctypes.c_int64 * 4), ("v_strides", ctypes.c_int64 * 4)]
+
+
+class _QkDesc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("param_dtype", ctypes.c_int32), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_size", ctypes.c_int32), ("rotary_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("position_bytes", ctypes.c_int32), ("eps", ctypes.c_float), ("gain_offset", ctypes.c_float), ("tokens", ctypes.c_int64),
+                ("places", ctypes.c_int64), ("q_strides", ctypes.c_int64 * 2), ("k_strides", ctypes.c_int64 * 2),
+                ("v_strides", ctypes.c_int64 * 2), ("q_out_strides", ctypes.c_int64 * 2), ("k_out_strides", ctypes.c_int64 * 2),
+                ("gq_strides", ctypes.c_int64 * 2), ("gk_strides", ctypes.c_int64 * 2)]
+
+
+class _FmhaPagedDesc(ctypes.Structure):
+    _fields_ = [("heads", ctypes.c_int32), ("requests", ctypes.c_int32), ("columns", ctypes.c_int32), ("mask_words", ctypes.c_int32),
+                ("head_scale", ctypes.c_float), ("reserved", ctypes.c_int32), ("rows", ctypes.c_int64), ("table_stride", ctypes.c_int64),
+                ("mask_stride", ctypes.c_int64), ("q_strides", ctypes.c_int64 * 2), ("o_strides", ctypes.c_int64 * 2)]
+
+
 # the same layouts for struct, whose field order and padding they share
 _PACK_GEMM = struct.Struct("=2i4q2i4q2i4qq2f2i").pack
 _PACK_FMHA = struct.Struct("=7i2fi15q").pack
@@ -145,6 +172,17 @@ ABI_SYMBOLS = {
     "ixk_linear_distill_bwd": (ctypes.c_int, [ctypes.POINTER(_LinearLossDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
                                               _vp]),
     "ixk_linear_loss_workspace_bytes": (_sz, [ctypes.POINTER(_LinearLossDesc), ctypes.c_int]),
+    "ixk_paged_extend": (ctypes.c_int, [ctypes.POINTER(_PagePool), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_int64, _vp, _vp, _vp, _vp]),
+    "ixk_paged_keep": (ctypes.c_int, [ctypes.POINTER(_PagePool), _vp, _vp, _vp, _vp, ctypes.c_int64, ctypes.c_int64, _vp, _vp, _vp, _vp, _vp,
+                                      ctypes.POINTER(_PagedCache), _vp, _vp, _vp]),
+    "ixk_qk_norm_rotary_fwd": (ctypes.c_int, [ctypes.POINTER(_QkDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                              ctypes.POINTER(_PagedCache), _vp, _vp, _vp, _vp]),
+    "ixk_qk_norm_rotary_bwd": (ctypes.c_int, [ctypes.POINTER(_QkDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
+                                              _vp]),
+    "ixk_qk_norm_rotary_bwd_workspace_bytes": (_sz, [ctypes.POINTER(_QkDesc)]),
+    "ixk_fmha_paged_fwd": (ctypes.c_int, [ctypes.POINTER(_FmhaPagedDesc), ctypes.POINTER(_PagedCache), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                          _vp, _vp, _vp, _sz, _vp]),
+    "ixk_fmha_paged_fwd_workspace_bytes": (_sz, [ctypes.POINTER(_FmhaPagedDesc), ctypes.POINTER(_PagedCache)]),
     "ixk_rotary_half": (ctypes.c_int, [ctypes.c_int, _vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                        ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _vp, _vp, _vp]),
     "ixk_kv_append": (ctypes.c_int, [ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _vp, _vp, ctypes.c_int64,
@@ -1006,6 +1044,317 @@ def fmha_backward_kernel(stream, query: torch.Tensor, key: torch.Tensor, value: 
                           _ptr(activation), _ptr(grad_query), _ptr(grad_key), _ptr(grad_value), _ptr(workspace),
                           ws_bytes, _stream_ptr(stream))
     _check(st)
+
+
+# ----------------------------------------------------------------------------- a paged key/value cache
+
+class PagedRows(NamedTuple):
+    """What paged_extend says of a step's packed rows, all int32 on the GPU: row_start [B + 1] and granted [B] by request;
+    request, position and slot [rows] by row (-1 where a row has none); free_count [1], the pages left."""
+    row_start: torch.Tensor
+    granted: torch.Tensor
+    request: torch.Tensor
+    position: torch.Tensor
+    slot: torch.Tensor
+    free_count: torch.Tensor
+
+
+def _require_here(*tensors) -> None:
+    """CUDA tensors of the current device: kernels are launched there."""
+    _require_cuda(*tensors)
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != here:
+            raise IxkError(IXK_INVALID_ARGUMENT, f"operands must be on the current device ({here}), one is on {t.device}")
+
+
+def _empty(shape, dtype, device, stream) -> torch.Tensor:
+    """A result, from the pool of the stream that writes it."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with _on_stream(stream, device):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _int32(name: str, t: torch.Tensor, *shape) -> None:
+    if t.dtype != torch.int32 or not t.is_contiguous() or (t.numel() != 1 if shape == (1,) else t.shape != shape):
+        raise IxkError(IXK_INVALID_ARGUMENT, f"{name} must be a dense int32 tensor [{', '.join(map(str, shape))}]")
+
+
+def _page_pool(page_table, lengths, free_pages, free_count, page_size) -> _PagePool:
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise IxkError(IXK_INVALID_ARGUMENT, "page_table must be int32 [requests, columns] with contiguous rows")
+    d = _PagePool()
+    d.page_size, d.pages = int(page_size), free_pages.numel()
+    d.requests, d.columns = page_table.shape
+    d.table_stride = page_table.stride(0)
+    _int32("lengths", lengths, d.requests)
+    _int32("free_pages", free_pages, d.pages)
+    _int32("free_count", free_count, 1)
+    return d
+
+
+def paged_extend(page_table: torch.Tensor, lengths: torch.Tensor, new_tokens: torch.Tensor, free_pages: torch.Tensor,
+                 free_count: torch.Tensor, *, rows: int, page_size: int, out: Optional[PagedRows] = None, stream=None) -> PagedRows:
+    """Pages for new_tokens[b] more tokens of every request, taken from the end of free_pages[:free_count] and entered into
+    page_table [B, columns] in place, and the maps of the step's packed rows, of which there is room for `rows`.
+    lengths [B] holds the tokens that are in the cache, free_count [1] the free pages; all int32.  A request that does not
+    fit (the free pages, its table row, `rows`) is granted nothing and its rows are -1.  `out`: the results' tensors, as an
+    earlier call returned them; its free_count may be the one that goes in.  Nothing else of `out` may be an input."""
+    if _NATIVE is not None:
+        r = _NATIVE.paged_extend(page_table, lengths, new_tokens, free_pages, free_count, rows, page_size, out, stream)
+        if r is not None:
+            return PagedRows(*_native_result(r))
+    _require_here(page_table, lengths, new_tokens, free_pages, free_count, *(out or ()))
+    d = _page_pool(page_table, lengths, free_pages, free_count, page_size)
+    _int32("new_tokens", new_tokens, d.requests)
+    rows = int(rows)
+    if rows < 0:
+        raise IxkError(IXK_INVALID_ARGUMENT, "rows must not be negative")
+    shapes = ((d.requests + 1,), (d.requests,), (rows,), (rows,), (rows,), (1,))
+    if out is None:
+        out = PagedRows(*(_empty(s, torch.int32, lengths.device, stream) for s in shapes))
+    for name, t, s in zip(PagedRows._fields, out, shapes):
+        _int32(f"out.{name}", t, *s)
+    _check(load_library().ixk_paged_extend(ctypes.byref(d), _ptr(lengths), _ptr(new_tokens), _ptr(page_table), _ptr(free_pages),
+                                           _ptr(free_count), _ptr(out.free_count), _ptr(out.granted), _ptr(out.row_start), rows,
+                                           _ptr(out.request), _ptr(out.position), _ptr(out.slot), _stream_ptr(stream)))
+    return out
+
+
+def _paged_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, layers: bool = False) -> _PagedCache:
+    """k_pages / v_pages [pages, page_size, heads, head_size], or with `layers` also [layers, ...], any strides but the last."""
+    dims = k_pages.dim()
+    if dims != 4 and not (layers and dims == 5):
+        raise IxkError(IXK_INVALID_ARGUMENT, "k_pages must be [pages, page_size, heads, head_size]" + (", or that by layers" if layers else ""))
+    if v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
+        raise IxkError(IXK_INVALID_ARGUMENT, "v_pages must have k_pages's shape and type")
+    if k_pages.dtype not in (torch.bfloat16, torch.float16):
+        raise IxkError(IXK_UNIMPLEMENTED, "the cache must be bfloat16 or float16")
+    if k_pages.numel() == 0 or max(k_pages.shape) > 0x7fffffff:
+        raise IxkError(IXK_INVALID_ARGUMENT, "the cache must have pages, and fewer than 2^31 of anything")
+    if k_pages.stride(-1) != 1 or v_pages.stride(-1) != 1:
+        raise IxkError(IXK_INVALID_ARGUMENT, "the cache's last dimension must be contiguous")
+    c = _PagedCache()
+    c.dtype = _TORCH_TO_IXK[k_pages.dtype]
+    c.pages, c.page_size, c.heads, c.head_size = k_pages.shape[-4:]
+    c.layers = k_pages.shape[0] if dims == 5 else 1
+    for strides, t in ((c.k_strides, k_pages), (c.v_strides, v_pages)):
+        strides[:] = t.stride()[:4] if dims == 5 else (0, *t.stride()[:3])
+        for i, n in enumerate((c.layers, c.pages, c.page_size, c.heads)):
+            if n == 1:
+                strides[i] = 0       # (never used)
+    return c
+
+
+def paged_keep(page_table: torch.Tensor, lengths: torch.Tensor, granted: torch.Tensor, kept: torch.Tensor, free_pages: torch.Tensor,
+               free_count: torch.Tensor, *, page_size: int, path: Optional[torch.Tensor] = None, k_pages: Optional[torch.Tensor] = None,
+               v_pages: Optional[torch.Tensor] = None, lengths_out: Optional[torch.Tensor] = None,
+               free_count_out: Optional[torch.Tensor] = None, stream=None):
+    """After a verification: kept[b] of request b's granted[b] drafts stay, those that path[b, :kept[b]] lists in ascending
+    order (None: the first ones).  Their keys and values in k_pages / v_pages ([pages, page_size, heads, head_size], or
+    [layers, pages, ...]: all layers at once) move together behind the committed ones, lengths grow, pages that are no longer
+    needed go back to free_pages.  kept[b] < 0 ends the request.  Returns (lengths, free_count): new tensors, or lengths_out
+    and free_count_out, which may be the ones that go in."""
+    if _NATIVE is not None:
+        r = _NATIVE.paged_keep(page_table, lengths, granted, kept, free_pages, free_count, page_size, path, k_pages, v_pages, lengths_out,
+                               free_count_out, stream)
+        if r is not None:
+            return _native_result(r)
+    _require_here(page_table, lengths, granted, kept, free_pages, free_count, path, k_pages, v_pages, lengths_out, free_count_out)
+    d = _page_pool(page_table, lengths, free_pages, free_count, page_size)
+    _int32("granted", granted, d.requests)
+    _int32("kept", kept, d.requests)
+    cache, columns, stride = None, 0, 0
+    if path is not None:
+        if k_pages is None or v_pages is None:
+            raise IxkError(IXK_INVALID_ARGUMENT, "a path needs k_pages and v_pages, whose tokens move")
+        if path.dim() != 2 or path.dtype != torch.int32 or path.shape[0] != d.requests or (path.shape[1] > 1 and path.stride(1) != 1):
+            raise IxkError(IXK_INVALID_ARGUMENT, "path must be int32 [requests, most drafts] with contiguous rows")
+        cache, columns, stride = _paged_cache(k_pages, v_pages, True), path.shape[1], path.stride(0)
+    elif k_pages is not None or v_pages is not None:
+        raise IxkError(IXK_INVALID_ARGUMENT, "without a path nothing moves: no k_pages and v_pages")
+    if lengths_out is None:
+        lengths_out = _empty((d.requests,), torch.int32, lengths.device, stream)
+    if free_count_out is None:
+        free_count_out = _empty((1,), torch.int32, lengths.device, stream)
+    _int32("lengths_out", lengths_out, d.requests)
+    _int32("free_count_out", free_count_out, 1)
+    _check(load_library().ixk_paged_keep(ctypes.byref(d), _ptr(lengths), _ptr(granted), _ptr(kept), _ptr(path), columns, stride,
+                                         _ptr(page_table), _ptr(free_pages), _ptr(free_count), _ptr(free_count_out), _ptr(lengths_out),
+                                         None if cache is None else ctypes.byref(cache), _ptr(k_pages), _ptr(v_pages), _stream_ptr(stream)))
+    return lengths_out, free_count_out
+
+
+def _heads_view(name: str, t: torch.Tensor, shape, dtype, strides) -> None:
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or (shape[2] > 1 and t.stride(2) != 1):
+        raise IxkError(IXK_INVALID_ARGUMENT, f"{name} must be [{', '.join(map(str, shape))}] of q's type with contiguous heads")
+    # (the stride of a dimension of one entry is never used)
+    strides[:] = [0 if n == 1 else s for n, s in zip(shape[:2], t.stride()[:2])]
+
+
+def _qk_desc(q, k, q_gain, k_gain, gain_offset, eps, cos, sin, positions, half_split) -> _QkDesc:
+    if q.dim() != 3 or k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or k.dtype != q.dtype:
+        raise IxkError(IXK_INVALID_ARGUMENT, "q must be [tokens, heads, head_size], k [tokens, kv_heads, head_size] of the same type")
+    if q.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise IxkError(IXK_UNIMPLEMENTED, "q and k must be bfloat16, float16 or float32")
+    d = _QkDesc()
+    d.tokens, d.heads, d.head_size = q.shape
+    d.kv_heads = k.shape[1]
+    param_dtype = next((g.dtype for g in (q_gain, k_gain) if g is not None), q.dtype)
+    for name, g in (("q_gain", q_gain), ("k_gain", k_gain)):
+        if g is not None and (g.shape != (d.head_size,) or g.dtype != param_dtype or not g.is_contiguous()):
+            raise IxkError(IXK_INVALID_ARGUMENT, f"{name} must be a dense [head_size] vector; both gains of one type")
+    if param_dtype not in (q.dtype, torch.float32):
+        raise IxkError(IXK_UNIMPLEMENTED, "gains must have q's type or be float32")
+    for name, t in (("cos", cos), ("sin", sin)):
+        if t.dim() != 2 or t.dtype != torch.float32 or t.shape != cos.shape or not t.is_contiguous():
+            raise IxkError(IXK_INVALID_ARGUMENT, f"{name} must be a dense float32 [places, rotary_dim / 2] table")
+    if positions is not None and (positions.dtype not in (torch.int32, torch.int64) or positions.shape != (d.tokens,) or not positions.is_contiguous()):
+        raise IxkError(IXK_INVALID_ARGUMENT, "positions must be a dense int32 or int64 vector, one for each token")
+    d.dtype, d.param_dtype = _TORCH_TO_IXK[q.dtype], _TORCH_TO_IXK[param_dtype]
+    d.rotary_dim, d.places, d.interleaved = 2 * cos.shape[1], cos.shape[0], 0 if half_split else 1
+    d.position_bytes = 8 if positions is not None and positions.dtype == torch.int64 else 4
+    d.eps, d.gain_offset = float(eps), float(gain_offset)
+    _heads_view("q", q, q.shape, q.dtype, d.q_strides)
+    _heads_view("k", k, k.shape, q.dtype, d.k_strides)
+    return d
+
+
+def qk_norm_rotary_forward(q: torch.Tensor, k: torch.Tensor, *, q_gain: Optional[torch.Tensor] = None, k_gain: Optional[torch.Tensor] = None,
+                           gain_offset: float = 0.0, eps: float = 1e-6, cos: torch.Tensor, sin: torch.Tensor,
+                           positions: Optional[torch.Tensor] = None, half_split: bool = True, v: Optional[torch.Tensor] = None,
+                           slots: Optional[torch.Tensor] = None, k_pages: Optional[torch.Tensor] = None,
+                           v_pages: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None,
+                           k_out: Optional[torch.Tensor] = None, stream=None):
+    """RMSNorm of every head of q [tokens, heads, head_size] and k [tokens, kv_heads, head_size] (views with any token and head
+    strides), scaled by gain_offset + gain [head_size], and the rotation of its first elements by the angles cos / sin [places,
+    rotary_dim / 2] of the token's position (None: t % places), in one pass with one rounding.  half_split: element i pairs
+    with i + rotary_dim / 2, otherwise 2 i with 2 i + 1.  Returns (q, k); with slots, k_pages and v_pages (see paged_extend) the
+    keys, and v as it is, go into the cache instead, and k is None.  A token whose position is outside the tables is left
+    out, a slot outside the cache is not written.  q_out and k_out may be q and k."""
+    if _NATIVE is not None:
+        r = _NATIVE.qk_forward(q, k, q_gain, k_gain, gain_offset, eps, cos, sin, positions, half_split, v, slots, k_pages, v_pages, q_out, k_out,
+                               stream)
+        if r is not None:
+            return _native_result(r)
+    _require_here(q, k, q_gain, k_gain, cos, sin, positions, v, slots, k_pages, v_pages, q_out, k_out)
+    d = _qk_desc(q, k, q_gain, k_gain, gain_offset, eps, cos, sin, positions, half_split)
+    cache = None
+    paged = [t is not None for t in (v, slots, k_pages, v_pages)]
+    if any(paged):
+        if not all(paged) or k_out is not None:
+            raise IxkError(IXK_INVALID_ARGUMENT, "into a cache: v, slots, k_pages and v_pages together, and no k_out")
+        _int32("slots", slots, d.tokens)
+        _heads_view("v", v, k.shape, q.dtype, d.v_strides)
+        cache = _paged_cache(k_pages, v_pages)
+    elif k_out is None:
+        k_out = _empty(k.shape, k.dtype, k.device, stream)
+    if q_out is None:
+        q_out = _empty(q.shape, q.dtype, q.device, stream)
+    _heads_view("q_out", q_out, q.shape, q.dtype, d.q_out_strides)
+    if k_out is not None:
+        _heads_view("k_out", k_out, k.shape, q.dtype, d.k_out_strides)
+    _check(load_library().ixk_qk_norm_rotary_fwd(ctypes.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(q_gain), _ptr(k_gain), _ptr(cos), _ptr(sin),
+                                                 _ptr(positions), _ptr(q_out), _ptr(k_out), None if cache is None else ctypes.byref(cache),
+                                                 _ptr(slots), _ptr(k_pages), _ptr(v_pages), _stream_ptr(stream)))
+    return q_out, k_out
+
+
+def qk_norm_rotary_backward_workspace_bytes(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor) -> int:
+    return int(load_library().ixk_qk_norm_rotary_bwd_workspace_bytes(
+        ctypes.byref(_qk_desc(q, k, None, None, 0.0, 0.0, cos, cos, None, 2 * cos.shape[1] % 16 == 0))))
+
+
+def qk_norm_rotary_backward(grad_q: torch.Tensor, grad_k: torch.Tensor, q: torch.Tensor, k: torch.Tensor, *,
+                            q_gain: Optional[torch.Tensor] = None, k_gain: Optional[torch.Tensor] = None, gain_offset: float = 0.0,
+                            eps: float = 1e-6, cos: torch.Tensor, sin: torch.Tensor, positions: Optional[torch.Tensor] = None,
+                            half_split: bool = True, dq: Optional[torch.Tensor] = None, dk: Optional[torch.Tensor] = None,
+                            workspace: Optional[torch.Tensor] = None, stream=None):
+    """The gradients of qk_norm_rotary_forward's inputs from those of its results and the inputs themselves: (dq, dk, dq_gain,
+    dk_gain), the last two None where there is no gain, otherwise of the gains' type.  Tokens that the forward left out have
+    gradient 0.  dq may be q or grad_q, dk likewise."""
+    if _NATIVE is not None:
+        r = _NATIVE.qk_backward(grad_q, grad_k, q, k, q_gain, k_gain, gain_offset, eps, cos, sin, positions, half_split, dq, dk, workspace,
+                                stream)
+        if r is not None:
+            return _native_result(r)
+    _require_here(grad_q, grad_k, q, k, q_gain, k_gain, cos, sin, positions, dq, dk, workspace)
+    d = _qk_desc(q, k, q_gain, k_gain, gain_offset, eps, cos, sin, positions, half_split)
+    _heads_view("grad_q", grad_q, q.shape, q.dtype, d.gq_strides)
+    _heads_view("grad_k", grad_k, k.shape, q.dtype, d.gk_strides)
+    dq = _empty(q.shape, q.dtype, q.device, stream) if dq is None else dq
+    dk = _empty(k.shape, k.dtype, k.device, stream) if dk is None else dk
+    _heads_view("dq", dq, q.shape, q.dtype, d.q_out_strides)
+    _heads_view("dk", dk, k.shape, q.dtype, d.k_out_strides)
+    dq_gain, dk_gain = (None if g is None else _empty(g.shape, g.dtype, g.device, stream) for g in (q_gain, k_gain))
+    lib = load_library()
+    if workspace is None and (dq_gain is not None or dk_gain is not None):
+        workspace = _own_scratch(lib.ixk_qk_norm_rotary_bwd_workspace_bytes(ctypes.byref(d)), q.device, stream)
+    _check(lib.ixk_qk_norm_rotary_bwd(ctypes.byref(d), _ptr(grad_q), _ptr(grad_k), _ptr(q), _ptr(k), _ptr(q_gain), _ptr(k_gain), _ptr(cos),
+                                      _ptr(sin), _ptr(positions), _ptr(dq), _ptr(dk), _ptr(dq_gain), _ptr(dk_gain), _ptr(workspace),
+                                      0 if workspace is None else workspace.nbytes, _stream_ptr(stream)))
+    return dq, dk, dq_gain, dk_gain
+
+
+def _fmha_paged_desc(q, k_pages, v_pages, page_table, lengths, row_start, granted, scale, mask, out):
+    c = _paged_cache(k_pages, v_pages)
+    if q.dim() != 3 or q.dtype != k_pages.dtype or q.shape[2] != c.head_size:
+        raise IxkError(IXK_INVALID_ARGUMENT, "q must be [rows, heads, head_size] of the cache's type and head_size")
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise IxkError(IXK_INVALID_ARGUMENT, "page_table must be int32 [requests, columns] with contiguous rows")
+    d = _FmhaPagedDesc()
+    d.rows, d.heads = q.shape[:2]
+    d.requests, d.columns = page_table.shape
+    d.table_stride = page_table.stride(0)
+    d.head_scale = float(scale)
+    _int32("lengths", lengths, d.requests)
+    _int32("row_start", row_start, d.requests + 1)
+    _int32("granted", granted, d.requests)
+    if mask is not None:
+        if mask.dim() != 2 or mask.dtype != torch.int32 or mask.shape[0] != d.rows or mask.shape[1] < 1 or \
+                (mask.shape[1] > 1 and mask.stride(1) != 1):
+            raise IxkError(IXK_INVALID_ARGUMENT, "mask must be int32 [rows, words] with contiguous rows of a word at least")
+        d.mask_words, d.mask_stride = mask.shape[1], mask.stride(0)
+    _heads_view("q", q, q.shape, q.dtype, d.q_strides)
+    _heads_view("out", out, q.shape, q.dtype, d.o_strides)
+    return d, c
+
+
+def fmha_paged_workspace_bytes(q: torch.Tensor, k_pages: torch.Tensor) -> int:
+    """Scratch bytes of fmha_paged_forward (they depend on q's rows and heads and on the cache's heads alone)."""
+    d, c = _FmhaPagedDesc(), _paged_cache(k_pages, k_pages)
+    d.rows, d.heads, d.columns = q.shape[0], q.shape[1], 1
+    return int(load_library().ixk_fmha_paged_fwd_workspace_bytes(ctypes.byref(d), ctypes.byref(c)))
+
+
+def fmha_paged_forward(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                       row_start: torch.Tensor, granted: torch.Tensor, *, scale: float, mask: Optional[torch.Tensor] = None,
+                       out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, with_lse: bool = False,
+                       workspace: Optional[torch.Tensor] = None, stream=None):
+    """Attention of a step's packed rows q [rows, heads, head_size] over a paged cache (see paged_extend, whose lengths,
+    row_start and granted these are; the new tokens' keys and values are in their slots).  heads is a multiple of the cache's.
+    A row sees its request's committed tokens and of the new ones those whose bits its row of mask [rows, words] (int32, bit
+    i % 32 of word i / 32) sets; without a mask, those up to itself.  Returns (out, lse): out like q, rows that belong to no
+    request left as they were; lse [rows, heads] fp32 with `with_lse` or given, otherwise None."""
+    if _NATIVE is not None:
+        r = _NATIVE.fmha_paged(q, k_pages, v_pages, page_table, lengths, row_start, granted, scale, mask, out, lse, with_lse, workspace, stream)
+        if r is not None:
+            return _native_result(r)
+    _require_here(q, k_pages, v_pages, page_table, lengths, row_start, granted, mask, out, lse, workspace)
+    out = _empty(q.shape, q.dtype, q.device, stream) if out is None else out
+    d, c = _fmha_paged_desc(q, k_pages, v_pages, page_table, lengths, row_start, granted, scale, mask, out)
+    if lse is None and with_lse:
+        lse = _empty((d.rows, d.heads), torch.float32, q.device, stream)
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous()):
+        raise IxkError(IXK_INVALID_ARGUMENT, "lse must be a dense float32 [rows, heads] tensor")
+    lib = load_library()
+    if workspace is None:
+        workspace = _own_scratch(lib.ixk_fmha_paged_fwd_workspace_bytes(ctypes.byref(d), ctypes.byref(c)), q.device, stream)
+    _check(lib.ixk_fmha_paged_fwd(ctypes.byref(d), ctypes.byref(c), _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(page_table), _ptr(lengths),
+                                  _ptr(row_start), _ptr(granted), _ptr(mask), _ptr(out), _ptr(lse), _ptr(workspace), workspace.nbytes,
+                                  _stream_ptr(stream)))
+    return out, lse
 
 
 STATIC_SCRATCH_BYTES = 4 << 20  # IXK_STATIC_SCRATCH_BYTES in include/ixk.h

@@ -1,0 +1,927 @@
+// Attention of a step's new rows (a tree of drafted tokens, a chain, or one token a request) over a paged key/value cache.
+//
+//   o = sum_t p_t v_t / sum_t p_t,   p_t = exp(head_scale q.k_t)   over the keys that a row sees
+//
+// The G query heads of a key head and a request's new tokens are the rows of one tile of 128: every key and value is read
+// once for all of them.  A unit of work is 64 keys of one tile (request, key head, block of tokens); all units of the call, in
+// that order, are cut into equal runs, one for every worker, whatever the requests' lengths are.  A worker is a CTA; up to head
+// size 128 there are two on an SM, so that one's products run beside the other's exponentials.
+//
+//   warps 0-3   softmax: a thread owns a row (a lane of tensor memory); then the row's result
+//   warp 4      copies: Q, K_0, K_1, V_0, K_2, V_1 ... of the run through a ring of 64-key slots, page by page
+//   warp 5      tcgen05.mma: S_g = Q K_g^T two units ahead into one of two buffers, O += P_g V_g (P from tensor memory)
+//
+// Bound by HBM: 64 keys of K and V take H * 256 bytes, 1340 cycles of an SM's share of the bandwidth at H = 128, the two products
+// 640 (the tile is padded to 128 rows), the softmax about 1000 and beside those of the other worker.
+// The running maximum is raised when it has moved by more than 2^8, so O is seldom rescaled.  P is rounded to nearest, and the
+// row is divided by the sum of the rounded values, so that a row with one large weight loses nothing; the log-sum-exp is
+// taken of the sum of the fp32 ones.
+//
+// A tile whose units all lie in one run is written out; otherwise its parts go to scratch in fp32, and the second kernel joins
+// them.  A worker has at most two: the end of a tile that an earlier worker began, and the beginning of one that goes on.
+//
+// Units that reach behind a request's committed tokens see masks, bit by bit, and the stale rest of its last page.  There the
+// softmax warps go through V in shared memory first: rows behind the end become zeros, and of drafts every NaN and infinity, since
+// 0 * NaN would reach rows that do not see the draft; rows that do see it get them back at the end (`odd_values`).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "paged.h"
+#include "ptx.cuh"
+
+namespace ixk {
+namespace fmha_paged {
+
+namespace {
+
+constexpr int kRows = 128;            // rows of a tile (= TMEM lanes)
+constexpr int kKeys = 64;             // keys of a unit
+constexpr int kChunkElems = 64;       // 16-bit elements of a 128-byte swizzle row
+constexpr int kThreads = 192;
+constexpr int kCopyWarp = 4;
+constexpr int kMmaWarp = 5;
+constexpr int kSoftmaxThreads = 128;
+constexpr int kTable = 40;            // requests whose numbers a worker holds in shared memory
+constexpr int kMinUnits = 2;          // shortest run: below that, joining parts costs more than it saves
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kRescaleThreshold = 8.0f;   // log2 units
+
+enum : int { kSiteLoadQ = 801, kSiteLoadKV = 802, kSiteMmaQ = 803, kSiteMmaKV = 804, kSiteMmaP = 805, kSiteMmaO = 806, kSiteSoftmaxS = 807,
+             kSiteSoftmaxO = 808, kSiteSoftmaxV = 809, kSiteAlign = 810 };
+
+template <int kHeadDim>
+struct Cfg {
+  static constexpr int kChunks = kHeadDim / kChunkElems;
+  static constexpr int kQChunkBytes = kRows * 128;
+  static constexpr int kKvChunkBytes = kKeys * 128;
+  static constexpr int kQBytes = kChunks * kQChunkBytes;
+  static constexpr int kSlotBytes = kChunks * kKvChunkBytes;
+  static constexpr int kWorkers = kHeadDim <= 128 ? 2 : 1;        // on an SM
+  static constexpr int kSlots = kHeadDim == 64 ? 8 : 5;
+  static constexpr int kTmemColumns = kHeadDim <= 128 ? 256 : 512;
+  static constexpr int kTmemO = 2 * kKeys;                        // S in two buffers of 64 columns
+  static constexpr int kTailBytes = 8 * (10 + 2 * kSlots) + 32 + 8 * 8 + kTable * 12;
+  static constexpr int kSmemBytes = kQBytes + kSlots * kSlotBytes + kTailBytes;
+  static_assert(kSmemBytes <= (kWorkers == 2 ? 115712 : 232448), "shared memory budget");
+  static_assert(kTmemO + kHeadDim <= kTmemColumns, "TMEM budget");
+};
+
+struct Args {
+  int requests, heads, kv_heads, group, head_size;
+  int block_tokens;           // tokens of a tile: 128 / group
+  int rows_in;                // rows of q
+  int columns, page_shift, pages;
+  int cap;                    // keys that a table row can hold
+  int is_bf16;
+  float scale_log2;
+  int64_t table_stride, mask_stride;
+  int mask_words;
+  const int *table, *lengths, *row_start, *granted, *mask;
+  const uint16_t* v;          // (odd values of drafts)
+  int64_t v_strides[3];       // page, token, head
+  uint16_t* out;
+  int64_t o_strides[2];
+  float* lse;
+  int* status_word;
+  int part_rows;              // rows of a part in scratch
+  int4* meta;                 // [workers] the tile that a worker began and did not finish: request, key head, block, parts
+  float* part_o;              // [2 * workers][part_rows][kHeadDim]
+  float4* part_stat;          // [2 * workers][part_rows]: maximum (log2), sum, sum of rounded weights
+};
+
+// A request's numbers, cut to what its buffers hold.
+struct Request {
+  int length, rows, row0;     // committed tokens, new rows, first row
+};
+__device__ __forceinline__ Request load_request(const Args& a, int b) {
+  Request r;
+  const int start = a.row_start[b], n = a.granted[b];
+  r.length = min(max(a.lengths[b], 0), a.cap);
+  r.row0 = start;
+  r.rows = start < 0 || start >= a.rows_in ? 0 : max(min(n, a.rows_in - start), 0);
+  return r;
+}
+// Keys and 64-key units of the block of tokens that starts at token t0.
+__device__ __forceinline__ int block_keys(const Args& a, const Request& r, int t0) {
+  const int seen = a.mask != nullptr ? r.rows : min(r.rows, t0 + a.block_tokens);
+  return static_cast<int>(min(static_cast<long long>(r.length) + seen, static_cast<long long>(a.cap)));
+}
+__device__ __forceinline__ int block_units(const Args& a, const Request& r, int t0) { return (block_keys(a, r, t0) + kKeys - 1) / kKeys; }
+// Units of one key head of a request.
+__device__ __forceinline__ long long head_units(const Args& a, const Request& r) {
+  long long sum = 0;
+  for (int t0 = 0; t0 < r.rows; t0 += a.block_tokens) sum += block_units(a, r, t0);
+  return sum;
+}
+
+// A worker's walk over its run of units.
+struct Walk {
+  int b, kv_head, t0;
+  Request req;
+  int unit, units;            // of the tile
+  int first;                  // the first unit of the tile in this run
+  long long left;             // units left in the run, this one included
+  const int* table;           // the run's first requests in shared memory
+  int table_base, table_count;
+
+  __device__ __forceinline__ Request request(const Args& a, int i) const {
+    const int k = i - table_base;
+    if (k < table_count) return Request{table[3 * k], table[3 * k + 1], table[3 * k + 2]};
+    return load_request(a, i);
+  }
+  __device__ __forceinline__ void begin(const Args& a, int start_b, long long offset, long long count, const int* shared, int shared_count) {
+    table = shared;
+    table_base = start_b;
+    table_count = shared_count;
+    b = start_b;
+    left = count;
+    if (left <= 0) return;
+    req = request(a, b);
+    const long long per_head = head_units(a, req);
+    kv_head = static_cast<int>(offset / per_head);
+    long long rest = offset - kv_head * per_head;
+    t0 = 0;
+    while (rest >= (units = block_units(a, req, t0))) {
+      rest -= units;
+      t0 += a.block_tokens;
+    }
+    unit = first = static_cast<int>(rest);
+  }
+  __device__ __forceinline__ bool done() const { return left <= 0; }
+  __device__ __forceinline__ bool starts() const { return unit == first; }
+  __device__ __forceinline__ bool ends() const { return unit + 1 == units || left == 1; }      // the tile's last unit of this run
+  __device__ __forceinline__ void next(const Args& a) {
+    if (--left <= 0) return;
+    if (++unit < units) return;
+    unit = first = 0;
+    t0 += a.block_tokens;
+    if (t0 >= req.rows) {
+      t0 = 0;
+      if (++kv_head == a.kv_heads) {
+        kv_head = 0;
+        do req = request(a, ++b);       // (units are left, so a request with rows follows)
+        while (req.rows == 0);
+      }
+    }
+    units = block_units(a, req, t0);
+  }
+};
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, bool bf16) {
+  if (bf16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack2(uint32_t w, bool bf16) {
+  if (bf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// Issued by one elected lane of a converged warp; descriptors as (lo, hi) halves, the high one a constant.
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, e;\n\t"
+      ".reg .b64 da, db;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "mov.b64 da, {%1, %2};\n\t"
+      "mov.b64 db, {%3, %4};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t"
+      "}\n" ::"r"(d_tmem),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, e;\n\t"
+      ".reg .b64 db;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t"
+      "}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Which of keys [k0, k0 + 64) a row sees, as bits: committed ones, and drafts by its mask or, without one, up to itself.
+__device__ __forceinline__ uint64_t visible_keys(const Args& a, const Request& r, int row, int token, int k0) {
+  auto below = [](long long n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1ull; };
+  const long long committed = static_cast<long long>(r.length) - k0;
+  uint64_t bits = below(committed);
+  const long long end = min(static_cast<long long>(r.length) + r.rows, static_cast<long long>(a.cap)) - k0;
+  if (a.mask == nullptr) {
+    bits |= below(min(committed + token + 1, end));
+  } else {
+    // drafts d0 .. d0 + 63 stand at keys k0 .. (d0 < 0: the first of them at key k0 - d0)
+    const int* words = a.mask + row * a.mask_stride;
+    const long long d0 = -committed;
+    const long long w0 = d0 >= 0 ? d0 >> 5 : -((-d0 + 31) >> 5);
+    const int shift = static_cast<int>(d0 - (w0 << 5));
+    auto word = [&](long long w) { return w >= 0 && w < a.mask_words ? static_cast<uint32_t>(words[w]) : 0u; };
+    const uint32_t x = word(w0), y = word(w0 + 1), z = word(w0 + 2);
+    const uint32_t lo = __funnelshift_r(x, y, shift), hi = __funnelshift_r(y, z, shift);
+    bits |= (static_cast<uint64_t>(hi) << 32 | lo) & below(end);
+  }
+  return bits;
+}
+
+template <int kHeadDim>
+__global__ void __launch_bounds__(kThreads, Cfg<kHeadDim>::kWorkers)
+fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                  const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ Args args) {
+  using C = Cfg<kHeadDim>;
+  constexpr int kSlots = C::kSlots;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t q_smem = ptx::smem_u32(smem);
+  const uint32_t kv_smem = q_smem + C::kQBytes;
+  const uint32_t bar_base = kv_smem + kSlots * C::kSlotBytes;
+  const uint32_t q_full = bar_base, q_empty = bar_base + 8, o_free = bar_base + 16;
+  // (by buffer: what a thread waits for is then never two phases ahead of what it knows to have passed)
+  auto s_full = [&](int i) { return bar_base + 8u * (3 + i); };
+  auto p_full = [&](int i) { return bar_base + 8u * (5 + i); };
+  auto pv_done = [&](int i) { return bar_base + 8u * (7 + i); };
+  auto kv_full = [&](int s) { return bar_base + 8u * (9 + s); };
+  auto kv_empty = [&](int s) { return bar_base + 8u * (9 + kSlots + s); };
+  uint8_t* tail = smem + C::kQBytes + kSlots * C::kSlotBytes + 8 * (10 + 2 * kSlots);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(tail);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 4);
+  volatile int* odd_values = reinterpret_cast<volatile int*>(tail + 8);      // [3] by tile
+  int* start_request = reinterpret_cast<int*>(tail + 20);
+  long long* start_offset = reinterpret_cast<long long*>(tail + 24);
+  long long* sums = reinterpret_cast<long long*>(tail + 32);                 // [6 + 1]
+  int* table = reinterpret_cast<int*>(tail + 32 + 8 * 8);                    // [kTable][3]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  ptx::AbortCtl ctl{abort_flag, args.status_word};
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    odd_values[0] = odd_values[1] = odd_values[2] = 0;
+    ptx::mbar_init(q_full, 1);
+    ptx::mbar_init(q_empty, 1);
+    ptx::mbar_init(o_free, kSoftmaxThreads);
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(s_full(i), 1);
+      ptx::mbar_init(p_full(i), kSoftmaxThreads);
+      ptx::mbar_init(pv_done(i), 1);
+    }
+    for (int s = 0; s < kSlots; ++s) {
+      ptx::mbar_init(kv_full(s), 1);
+      ptx::mbar_init(kv_empty(s), 1);
+    }
+    ptx::fence_mbar_init();
+    ptx::prefetch_tmap(&tmap_q);
+    ptx::prefetch_tmap(&tmap_k);
+    ptx::prefetch_tmap(&tmap_v);
+  }
+  if (warp == kMmaWarp) {
+    ptx::tmem_alloc(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), C::kTmemColumns);
+    ptx::tmem_relinquish();
+  }
+  ptx::grid_dependency_sync();
+
+  // ---- the run: its length from the units of all requests, its start by a second walk over the sums
+  auto units_of = [&](int b) -> long long {
+    if (b >= args.requests) return 0;
+    return head_units(args, load_request(args, b)) * args.kv_heads;
+  };
+  const long long mine = units_of(threadIdx.x);
+  long long sum = mine;
+  for (int b = threadIdx.x + kThreads; b < args.requests; b += kThreads) sum += units_of(b);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) sums[warp] = sum;
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  ptx::tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  long long total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) total += sums[w];
+  const long long run = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(kMinUnits));
+  const long long start = run * blockIdx.x;
+  const long long count = max(min(run, total - start), 0LL);
+  if (count > 0) {
+    long long before = 0;
+    for (int b0 = 0; b0 < args.requests; b0 += kThreads) {
+      const long long u = b0 == 0 ? mine : units_of(b0 + threadIdx.x);
+      long long upto = u;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      __syncthreads();
+      if (lane == 31) sums[warp] = upto;
+      __syncthreads();
+      long long all = 0;
+#pragma unroll
+      for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) upto += sums[w];
+        all += sums[w];
+      }
+      upto += before;
+      if (start >= upto - u && start < upto) {
+        *start_request = b0 + threadIdx.x;
+        *start_offset = start - (upto - u);
+      }
+      before += all;
+      if (before > start) break;
+    }
+    __syncthreads();
+    const int b = *start_request;
+    const int i = b + static_cast<int>(threadIdx.x);
+    if (threadIdx.x < kTable && i < args.requests) {
+      const Request r = load_request(args, i);
+      table[3 * threadIdx.x] = r.length;
+      table[3 * threadIdx.x + 1] = r.rows;
+      table[3 * threadIdx.x + 2] = r.row0;
+    }
+    __syncthreads();
+  }
+  const bool aligned = (q_smem & 1023u) == 0;
+  if (!aligned && threadIdx.x == 0) atomicCAS(args.status_word, 0, kSiteAlign);
+  Walk walk;
+  walk.begin(args, count > 0 ? *start_request : 0, count > 0 ? *start_offset : 0, aligned ? count : 0, table,
+             count > 0 ? min(kTable, args.requests - *start_request) : 0);
+
+  if (warp == kCopyWarp) {
+    // ------------------------------------------------------------------ copies: a lane takes one page's 64 columns
+    const int box_keys = min(kKeys, 1 << args.page_shift);
+    const int pieces = kKeys / box_keys;
+    const int piece = lane / C::kChunks, chunk = lane - piece * C::kChunks;
+    const bool copies = piece < pieces;
+    uint32_t load = 0;          // place in the sequence K_0, K_1, V_0, K_2, V_1 ...
+    bool alive = true;
+    auto wait = [&](uint32_t bar, uint32_t parity, int site) {
+      if (alive && !ptx::mbar_wait(bar, parity, ctl, site)) alive = false;
+      alive = __all_sync(0xffffffffu, alive);
+      return alive;
+    };
+    auto load_unit = [&](const Walk& at, const CUtensorMap* map) {
+      const int slot = load % kSlots;
+      if (!wait(kv_empty(slot), ((load / kSlots) & 1u) ^ 1u, kSiteLoadKV)) return;
+      ++load;
+      if (lane == 0) ptx::mbar_expect_tx(kv_full(slot), C::kSlotBytes);
+      __syncwarp();
+      if (copies) {
+        const int k0 = at.unit * kKeys + piece * box_keys;
+        // (pages behind the last key are not looked up: their rows are zeros, as those of a page number outside the cache)
+        int page = args.pages;
+        if (k0 < static_cast<int>(min(static_cast<long long>(at.req.length) + at.req.rows, static_cast<long long>(args.cap)))) {
+          page = args.table[at.b * args.table_stride + (k0 >> args.page_shift)];
+          if (static_cast<unsigned>(page) >= static_cast<unsigned>(args.pages)) page = args.pages;
+        }
+        ptx::tma_load_4d(kv_smem + slot * C::kSlotBytes + chunk * C::kKvChunkBytes + piece * box_keys * 128, map, kv_full(slot),
+                         chunk * kChunkElems, at.kv_head, k0 & ((1 << args.page_shift) - 1), page);
+      }
+    };
+    Walk k_walk = walk, v_walk = walk;
+    uint32_t tiles = 0;
+    auto load_k = [&]() {
+      if (k_walk.starts()) {       // a new tile: Q, once the products of the one before have read theirs
+        if (!wait(q_empty, (tiles & 1u) ^ 1u, kSiteLoadQ)) return;
+        ++tiles;
+        if (lane == 0) {
+          ptx::mbar_expect_tx(q_full, static_cast<uint32_t>(C::kChunks * args.group * args.block_tokens * 128));
+#pragma unroll
+          for (int c = 0; c < C::kChunks; ++c)
+            ptx::tma_load_3d(q_smem + c * C::kQChunkBytes, &tmap_q, q_full, c * kChunkElems, k_walk.kv_head * args.group,
+                             k_walk.req.row0 + k_walk.t0);
+        }
+        __syncwarp();
+      }
+      load_unit(k_walk, &tmap_k);
+      k_walk.next(args);
+    };
+    if (!k_walk.done()) load_k();
+    while (alive && !v_walk.done()) {
+      if (!k_walk.done()) load_k();
+      if (!alive) break;
+      load_unit(v_walk, &tmap_v);
+      v_walk.next(args);
+    }
+  } else if (warp == kMmaWarp) {
+    // ------------------------------------------------------------------ products (all lanes; one elected per instruction)
+    const uint32_t fmt = args.is_bf16 ? 1u : 0u;
+    const uint32_t idesc_s = ptx::umma_idesc(fmt, fmt, 0, 0, kRows, kKeys);
+    const uint32_t idesc_o = ptx::umma_idesc(fmt, fmt, 0, 1, kRows, kHeadDim);
+    const uint64_t kmajor = ptx::umma_smem_desc(0, 16, 1024);
+    const uint64_t mnmajor = ptx::umma_smem_desc(0, C::kKvChunkBytes, 1024);
+    const uint32_t k_lo = static_cast<uint32_t>(kmajor), k_hi = static_cast<uint32_t>(kmajor >> 32);
+    const uint32_t v_lo = static_cast<uint32_t>(mnmajor), v_hi = static_cast<uint32_t>(mnmajor >> 32);
+    bool alive = true;
+    auto wait = [&](uint32_t bar, uint32_t parity, int site) {
+      if (alive && !ptx::mbar_wait(bar, parity, ctl, site)) alive = false;
+      alive = __all_sync(0xffffffffu, alive);
+      return alive;
+    };
+    uint32_t slot = 0, slot_parity = 0;
+    auto advance = [&]() {
+      if (++slot == static_cast<uint32_t>(kSlots)) {
+        slot = 0;
+        slot_parity ^= 1u;
+      }
+    };
+    Walk s_walk = walk, o_walk = walk;
+    uint32_t s_units = 0, o_units = 0, q_parity = 0, o_parity = 1;
+    auto issue_s = [&]() {
+      if (s_walk.starts()) {
+        if (!wait(q_full, q_parity, kSiteMmaQ)) return;
+        q_parity ^= 1u;
+      }
+      if (!wait(kv_full(slot), slot_parity, kSiteMmaKV)) return;
+      ptx::tc_fence_after_sync();
+      const uint32_t d = tmem_base + (s_units & 1u) * kKeys;
+      const uint32_t qa = k_lo + (q_smem >> 4), kb = k_lo + ((kv_smem + slot * C::kSlotBytes) >> 4);
+#pragma unroll
+      for (int ks = 0; ks < kHeadDim / 16; ++ks)
+        mma_ss(d, qa + (((ks >> 2) * C::kQChunkBytes + (ks & 3) * 32) >> 4), k_hi, kb + (((ks >> 2) * C::kKvChunkBytes + (ks & 3) * 32) >> 4), k_hi,
+               idesc_s, ks != 0 ? 1u : 0u);
+      ptx::umma_commit_elect(s_full(s_units & 1u));
+      ptx::umma_commit_elect(kv_empty(slot));
+      if (s_walk.ends()) ptx::umma_commit_elect(q_empty);
+      advance();
+      ++s_units;
+      s_walk.next(args);
+    };
+    if (!s_walk.done()) issue_s();
+    while (alive && !o_walk.done()) {
+      if (!s_walk.done()) issue_s();
+      if (!alive) break;
+      // O of the tile before must have been read out
+      if (o_walk.starts()) {
+        if (!wait(o_free, o_parity, kSiteMmaO)) break;
+        o_parity ^= 1u;
+      }
+      if (!wait(kv_full(slot), slot_parity, kSiteMmaKV)) break;
+      if (!wait(p_full(o_units & 1u), (o_units >> 1) & 1u, kSiteMmaP)) break;
+      ptx::tc_fence_after_sync();
+      const uint32_t a = tmem_base + (o_units & 1u) * kKeys, d = tmem_base + C::kTmemO;
+      const uint32_t vb = v_lo + ((kv_smem + slot * C::kSlotBytes) >> 4);
+#pragma unroll
+      for (int ks = 0; ks < kKeys / 16; ++ks)
+        mma_ts(d, a + ks * 8, vb + ((ks * 2048) >> 4), v_hi, idesc_o, (!o_walk.starts() || ks != 0) ? 1u : 0u);
+      ptx::umma_commit_elect(pv_done(o_units & 1u));
+      ptx::umma_commit_elect(kv_empty(slot));
+      advance();
+      ++o_units;
+      o_walk.next(args);
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax and results
+    const bool bf16 = args.is_bf16 != 0;
+    const int row = warp * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(warp * 32) << 16;
+    const uint32_t o_addr = tmem_base + lane_addr + C::kTmemO;
+    const int row_token = row / args.group, row_head = row - row_token * args.group;
+    const long long all_units = count;
+    uint32_t g = 0, tiles = 0;
+    bool alive = true;
+    int4 begun = make_int4(0, 0, 0, 0);       // the tile that this worker leaves to others: none
+    while (alive && !walk.done()) {
+      const Request req = walk.req;
+      const int token = walk.t0 + row_token;
+      const bool row_ok = row_token < args.block_tokens && token < req.rows;
+      const bool warp_ok = __any_sync(0xffffffffu, row_ok);
+      const int q_row = req.row0 + token;
+      const int keys_end = static_cast<int>(min(static_cast<long long>(req.length) + req.rows, static_cast<long long>(args.cap)));
+      const int first_unit = walk.unit;
+      float m_run = -INFINITY, l_run = 0.0f, r_run = 0.0f;     // maximum, sum, sum of the rounded weights
+      bool more = true;
+      for (; more; ++g) {
+        const int buf = g & 1u;
+        const int k0 = walk.unit * kKeys;
+        const bool masked = k0 + kKeys > req.length;
+        const uint32_t s_addr = tmem_base + lane_addr + buf * kKeys;
+        if (!ptx::mbar_wait(s_full(buf), (g >> 1) & 1u, ctl, kSiteSoftmaxS)) {
+          alive = false;
+          break;
+        }
+        ptx::tc_fence_after_sync();
+        if (warp_ok) {
+          uint32_t r[2][32];
+          ptx::tmem_ld_32x32(s_addr, r[0]);
+          ptx::tmem_ld_32x32(s_addr + 32, r[1]);
+          ptx::tmem_ld_wait();
+          float mult = args.scale_log2;
+          if (!(mult > 0.0f)) {       // (so that the maximum can be taken of r)
+#pragma unroll
+            for (int i = 0; i < 64; ++i) r[i >> 5][i & 31] = __float_as_uint(__uint_as_float(r[i >> 5][i & 31]) * mult);
+            mult = 1.0f;
+          }
+          if (masked) {
+            const uint64_t bits = row_ok ? visible_keys(args, req, q_row, token, k0) : 0ull;
+            const uint32_t lo = static_cast<uint32_t>(bits), hi = static_cast<uint32_t>(bits >> 32);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              if (!(lo >> i & 1u)) r[0][i] = 0xff800000u;
+              if (!(hi >> i & 1u)) r[1][i] = 0xff800000u;
+            }
+          }
+          float mx[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) mx[e] = ptx::max3(__uint_as_float(r[0][2 * e]), __uint_as_float(r[0][2 * e + 1]), __uint_as_float(r[0][16 + 2 * e]));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            mx[e] = ptx::max3(mx[e], __uint_as_float(r[0][17 + 2 * e]), __uint_as_float(r[1][2 * e]));
+            mx[e] = ptx::max3(mx[e], __uint_as_float(r[1][2 * e + 1]), __uint_as_float(r[1][16 + 2 * e]));
+            mx[e] = fmaxf(mx[e], __uint_as_float(r[1][17 + 2 * e]));
+          }
+          const float top = fmaxf(fmaxf(ptx::max3(mx[0], mx[1], mx[2]), mx[3]), fmaxf(ptx::max3(mx[4], mx[5], mx[6]), mx[7])) * mult;
+          float alpha = 1.0f;
+          if (row_ok && top - m_run > kRescaleThreshold) {     // also where the row has seen nothing so far
+            alpha = ptx::ex2_approx(m_run - top);
+            m_run = top;
+          }
+          if (walk.unit != first_unit && __any_sync(0xffffffffu, alpha != 1.0f)) {
+            // (S of this unit was issued behind P.V of the unit before the last: only the last one's may still run)
+            if (!ptx::mbar_wait(pv_done((g - 1) & 1u), ((g - 1) >> 1) & 1u, ctl, kSiteSoftmaxO)) {
+              alive = false;
+              break;
+            }
+            ptx::tc_fence_after_sync();
+#pragma unroll 1
+            for (int c = 0; c < kHeadDim / 32; ++c) {
+              uint32_t o[32];
+              ptx::tmem_ld_32x32(o_addr + c * 32, o);
+              ptx::tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              ptx::tmem_st_32x32(o_addr + c * 32, o);
+            }
+          }
+          const float m_use = m_run == -INFINITY ? 0.0f : m_run;
+          const uint64_t mult2 = ptx::f32x2(mult, mult), minus2 = ptx::f32x2(-m_use, -m_use);
+          uint64_t total2 = ptx::f32x2(0.0f, 0.0f), round2 = total2;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t packed[16];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float x0, x1;
+              ptx::f32x2_split(ptx::fma2(ptx::f32x2(__uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1])), mult2, minus2), x0, x1);
+              x0 = ptx::ex2_approx(x0);
+              x1 = ptx::ex2_approx(x1);
+              total2 = ptx::add2(total2, ptx::f32x2(x0, x1));
+              packed[i >> 1] = pack2(x0, x1, bf16);
+              const float2 rounded = unpack2(packed[i >> 1], bf16);
+              round2 = ptx::add2(round2, ptx::f32x2(rounded.x, rounded.y));
+            }
+            ptx::tmem_st_32x16(s_addr + c * 16, packed);
+          }
+          float t0, t1;
+          ptx::f32x2_split(total2, t0, t1);
+          l_run = l_run * alpha + (t0 + t1);
+          ptx::f32x2_split(round2, t0, t1);
+          r_run = r_run * alpha + (t0 + t1);
+          ptx::tmem_st_wait();
+        }
+        if (masked) {
+          // V behind the last key, and values of drafts that are no numbers
+          const uint32_t load = static_cast<long long>(g) < all_units - 1 ? 2 * g + 2 : 2 * g + 1;
+          if (!ptx::mbar_wait(kv_full(load % kSlots), (load / kSlots) & 1u, ctl, kSiteSoftmaxV)) {
+            alive = false;
+            break;
+          }
+          uint4* v = reinterpret_cast<uint4*>(smem + C::kQBytes + (load % kSlots) * C::kSlotBytes);
+          const uint32_t expo = bf16 ? 0x7f80u : 0x7c00u;
+          bool odd = false;
+#pragma unroll 4
+          for (int i = row; i < kKeys * 8 * C::kChunks; i += kSoftmaxThreads) {    // (16-byte pieces; a key is 8 of them in each chunk)
+            const int key = k0 + ((i >> 3) & (kKeys - 1));
+            if (key < req.length) continue;
+            uint4 w = v[i];
+            if (key >= keys_end) {
+              w = make_uint4(0, 0, 0, 0);
+              v[i] = w;
+              continue;
+            }
+            uint32_t words[4] = {w.x, w.y, w.z, w.w};
+            bool changed = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if ((words[e] & expo) == expo) {
+                words[e] &= 0xffff0000u;
+                changed = true;
+              }
+              if ((words[e] >> 16 & expo) == expo) {
+                words[e] &= 0x0000ffffu;
+                changed = true;
+              }
+            }
+            if (changed) {
+              v[i] = make_uint4(words[0], words[1], words[2], words[3]);
+              odd = true;
+            }
+          }
+          if (odd) odd_values[tiles % 3] = 1;
+          ptx::fence_proxy_async_smem();
+        }
+        more = !walk.ends();
+        // The flag of the tile after this one: last used two tiles ago, by nobody any more once all threads are in this one.
+        if (!more && row == 0) odd_values[(tiles + 1) % 3] = 0;
+        ptx::tc_fence_before_sync();
+        ptx::mbar_arrive(p_full(buf));
+        if (more) walk.next(args);
+      }
+      if (!alive) break;
+      if (!ptx::mbar_wait(pv_done((g - 1) & 1u), ((g - 1) >> 1) & 1u, ctl, kSiteSoftmaxO)) break;
+      ptx::tc_fence_after_sync();
+      const bool odd = odd_values[tiles % 3] != 0;
+      ++tiles;
+      const bool whole = first_unit == 0 && walk.unit + 1 == walk.units;
+      const int head = walk.kv_head * args.group + row_head;
+      int64_t part = 2 * static_cast<int64_t>(blockIdx.x);
+      if (!whole && first_unit == 0) {
+        ++part;
+        // (the tile's units start at start + g - (units of it so far); the workers behind this one have runs of `run`)
+        const long long after = walk.units - (walk.unit + 1);
+        begun = make_int4(walk.b, walk.kv_head, walk.t0, static_cast<int>((after + run - 1) / run) + 1);
+      }
+      if (warp_ok) {
+        const float inv_l = 1.0f / r_run;
+        uint16_t* out_row = args.out + q_row * args.o_strides[0] + head * args.o_strides[1];
+        float* part_row = args.part_o + (part * args.part_rows + row) * kHeadDim;
+#pragma unroll 1
+        for (int c = 0; c < kHeadDim / 32; ++c) {
+          uint32_t o[32];
+          ptx::tmem_ld_32x32(o_addr + c * 32, o);
+          ptx::tmem_ld_wait();
+          if (!row_ok || c * 32 >= args.head_size) continue;
+          if (odd) {
+            // the odd values of the drafts that this row sees, out of memory again
+            const int d0 = max(first_unit * kKeys - req.length, 0), d1 = min((walk.unit + 1) * kKeys, keys_end) - req.length;
+            for (int d = d0; d < d1; ++d) {
+              const int k = req.length + d;
+              if (!(visible_keys(args, req, q_row, token, k) & 1ull)) continue;
+              const int page = args.table[walk.b * args.table_stride + (k >> args.page_shift)];
+              if (static_cast<unsigned>(page) >= static_cast<unsigned>(args.pages)) continue;
+              const uint16_t* v = args.v + page * args.v_strides[0] + (k & ((1 << args.page_shift) - 1)) * args.v_strides[1] +
+                                  walk.kv_head * args.v_strides[2] + c * 32;
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                if (c * 32 + i >= args.head_size) break;
+                const float x = bf16 ? __uint_as_float(static_cast<uint32_t>(v[i]) << 16) : __half2float(__ushort_as_half(v[i]));
+                if (!(fabsf(x) < INFINITY)) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
+              }
+            }
+          }
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (c * 32 + e * 8 >= args.head_size) break;
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int at = e * 8 + i * 2;
+                w[i] = r_run == 0.0f ? 0u : pack2(__uint_as_float(o[at]) * inv_l, __uint_as_float(o[at + 1]) * inv_l, bf16);
+              }
+              reinterpret_cast<uint4*>(out_row + c * 32)[e] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              reinterpret_cast<uint4*>(part_row + c * 32)[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
+        }
+        if (row_ok) {
+          if (!whole) args.part_stat[part * args.part_rows + row] = make_float4(m_run, l_run, r_run, 0.0f);
+          else if (args.lse != nullptr)
+            args.lse[static_cast<int64_t>(q_row) * args.heads + head] = l_run == 0.0f ? -INFINITY : (m_run + log2f(l_run)) * kLn2;
+        }
+      }
+      ptx::tc_fence_before_sync();
+      ptx::mbar_arrive(o_free);
+      walk.next(args);
+    }
+    if (threadIdx.x == 0) args.meta[blockIdx.x] = begun;
+  }
+
+  if (*abort_flag != 0) __nanosleep(2000000);
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    ptx::tc_fence_after_sync();
+    ptx::tmem_dealloc(tmem_base, C::kTmemColumns);
+  }
+}
+
+// Joins the parts of the tiles that several workers did: a warp a row.  With the parts' maxima m_i and sums l_i, M = max m_i:
+//   o = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i
+// Worker w's own part is at 2 w + 1, those of the workers behind it at 2 (w + i).
+constexpr int kJoinWarps = 8;
+template <int kHeadDim>
+__global__ void __launch_bounds__(kJoinWarps * 32) fmha_paged_join_kernel(const __grid_constant__ Args a) {
+  ptx::grid_dependency_sync();
+  const int4 tile = a.meta[blockIdx.x];
+  if (tile.w == 0) return;
+  const Request req = load_request(a, tile.x);
+  const int lane = threadIdx.x & 31;
+  const int rows = min(a.block_tokens, req.rows - tile.z) * a.group;
+  const bool bf16 = a.is_bf16 != 0;
+  constexpr int kPer = kHeadDim / 32;
+  for (int row = blockIdx.y * kJoinWarps + (threadIdx.x >> 5); row < rows; row += gridDim.y * kJoinWarps) {
+    auto part_of = [&](int i) { return 2 * (static_cast<int64_t>(blockIdx.x) + i) + (i == 0 ? 1 : 0); };
+    float top = -INFINITY, mine_m = 0.0f, mine_l = 0.0f, mine_r = 0.0f, sum = 0.0f, rounded = 0.0f;
+    // a lane a part, 32 parts at a time
+    for (int i0 = 0; i0 < tile.w; i0 += 32) {
+      float m = -INFINITY;
+      if (i0 + lane < tile.w) m = a.part_stat[part_of(i0 + lane) * a.part_rows + row].x;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      top = fmaxf(top, m);
+    }
+    const float use = top == -INFINITY ? 0.0f : top;
+    float o[kPer];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) o[e] = 0.0f;
+    for (int i0 = 0; i0 < tile.w; i0 += 32) {
+      if (i0 + lane < tile.w) {
+        const float4 s = a.part_stat[part_of(i0 + lane) * a.part_rows + row];
+        mine_m = ptx::ex2_approx(s.x - use);
+        mine_l = s.y;
+        mine_r = s.z;
+      }
+      const int n = min(32, tile.w - i0);
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const float weight = __shfl_sync(0xffffffffu, mine_m, i);
+        sum = fmaf(weight, __shfl_sync(0xffffffffu, mine_l, i), sum);
+        rounded = fmaf(weight, __shfl_sync(0xffffffffu, mine_r, i), rounded);
+        const float* src = a.part_o + (part_of(i0 + i) * a.part_rows + row) * kHeadDim + lane * kPer;
+        // (a part that saw nothing has weight 0, and nothing in it)
+#pragma unroll
+        for (int e = 0; e < kPer; e += 2) {
+          const float2 v = *reinterpret_cast<const float2*>(src + e);
+          o[e] = fmaf(weight, v.x, o[e]);
+          o[e + 1] = fmaf(weight, v.y, o[e + 1]);
+        }
+      }
+    }
+    const int q_row = req.row0 + tile.z + row / a.group, head = tile.y * a.group + row % a.group;
+    const float inv = 1.0f / rounded;
+    uint16_t* out = a.out + q_row * a.o_strides[0] + head * a.o_strides[1];
+#pragma unroll
+    for (int e = 0; e < kPer; e += 2)
+      if (lane * kPer + e < a.head_size)
+        *reinterpret_cast<uint32_t*>(out + lane * kPer + e) = rounded == 0.0f ? 0u : pack2(o[e] * inv, o[e + 1] * inv, bf16);
+    if (lane == 0 && a.lse != nullptr)
+      a.lse[static_cast<int64_t>(q_row) * a.heads + head] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+  }
+}
+
+int head_dim(int head_size) { return head_size <= 64 ? 64 : head_size <= 128 ? 128 : 256; }
+int workers(int dim, int sm_count) { return sm_count * (dim <= 128 ? 2 : 1); }
+
+struct Scratch {
+  size_t meta, stat, o, total;
+  int part_rows;
+};
+Scratch scratch_of(const ixk_fmha_paged_desc* d, const ixk_paged_cache* c, int sm_count) {
+  const int dim = head_dim(c->head_size), w = workers(dim, sm_count);
+  const int group = std::max(d->heads / std::max(c->heads, 1), 1);
+  const int64_t tokens = std::max<int64_t>(std::min<int64_t>(std::max(kRows / group, 1), d->rows), 0);
+  Scratch s;
+  s.part_rows = static_cast<int>(tokens * group);
+  s.meta = 0;
+  s.stat = (static_cast<size_t>(w) * sizeof(int4) + 255) / 256 * 256;
+  s.o = s.stat + (static_cast<size_t>(2 * w) * s.part_rows * sizeof(float4) + 255) / 256 * 256;
+  s.total = s.o + static_cast<size_t>(2 * w) * s.part_rows * dim * sizeof(float);
+  return s;
+}
+
+int check(const ixk_fmha_paged_desc* d, const ixk_paged_cache* c) {
+  if (d == nullptr || c == nullptr) return fail(IXK_INVALID_ARGUMENT, "fmha_paged: desc or cache is NULL");
+  if (d->reserved != 0) return fail(IXK_INVALID_ARGUMENT, "fmha_paged: desc.reserved must be 0");
+  if (d->requests < 0 || d->rows < 0 || d->columns < 1 || d->heads < 1 || c->heads < 1 || d->mask_words < 0)
+    return fail(IXK_INVALID_ARGUMENT, "fmha_paged: negative size, or no heads or table columns");
+  if (c->head_size < 8 || c->head_size % 8 != 0 || c->head_size > 256)
+    return fail(IXK_UNIMPLEMENTED, "fmha_paged: head_size must be a multiple of 8, at most 256");
+  if (d->heads % c->heads != 0) return fail(IXK_INVALID_ARGUMENT, "fmha_paged: heads must be a multiple of the cache's heads");
+  if (d->heads / c->heads > kRows) return fail(IXK_UNIMPLEMENTED, "fmha_paged: more than 128 query heads to a key head");
+  if (c->page_size < 8 || c->page_size > 256 || (c->page_size & (c->page_size - 1)) != 0)
+    return fail(IXK_UNIMPLEMENTED, "fmha_paged: page_size must be 8, 16, 32, 64, 128 or 256");
+  if (!std::isfinite(d->head_scale)) return fail(IXK_INVALID_ARGUMENT, "fmha_paged: head_scale is not finite");
+  if (d->rows > 0x7fffffff - 256 || static_cast<int64_t>(d->columns) * c->page_size > 0x7fffffff - 256)
+    return fail(IXK_UNIMPLEMENTED, "fmha_paged: 2^31 rows, or keys of a request, or more");
+  return IXK_OK;
+}
+
+template <int kHeadDim>
+int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const Args& a, int sm_count, cudaStream_t stream) {
+  using C = Cfg<kHeadDim>;
+  IXK_CUDA_OK(cudaFuncSetAttribute(fmha_paged_kernel<kHeadDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
+  const int w = workers(kHeadDim, sm_count);
+  if (int st = launch_overlapped(fmha_paged_kernel<kHeadDim>, dim3(w), dim3(kThreads), C::kSmemBytes, stream, q, k, v, a)) return st;
+  const unsigned blocks = static_cast<unsigned>(std::max(1, std::min((a.part_rows + kJoinWarps - 1) / kJoinWarps, 8)));
+  return launch_overlapped(fmha_paged_join_kernel<kHeadDim>, dim3(w, blocks), dim3(kJoinWarps * 32), 0, stream, a);
+}
+
+}  // namespace
+}  // namespace fmha_paged
+}  // namespace ixk
+
+using namespace ixk;
+
+extern "C" {
+
+size_t ixk_fmha_paged_fwd_workspace_bytes(const ixk_fmha_paged_desc* desc, const ixk_paged_cache* cache) {
+  if (fmha_paged::check(desc, cache) != IXK_OK) return 0;
+  return fmha_paged::scratch_of(desc, cache, 148).total;
+}
+
+int ixk_fmha_paged_fwd(const ixk_fmha_paged_desc* d, const ixk_paged_cache* c, const void* q, const void* k_pages, const void* v_pages,
+                       const int32_t* page_table, const int32_t* lengths, const int32_t* row_start, const int32_t* granted,
+                       const int32_t* mask, void* out, float* lse, void* workspace, size_t workspace_bytes, void* cuda_stream) {
+  IXK_API_RANGE("ixk_fmha_paged_fwd");
+  clear_error();
+  if (int st = fmha_paged::check(d, c)) return st;
+  if (int st = paged::check_cache(c, k_pages, v_pages, "fmha_paged")) return st;
+  if (d->requests > 0 && d->rows > 0 &&
+      (q == nullptr || out == nullptr || page_table == nullptr || lengths == nullptr || row_start == nullptr || granted == nullptr))
+    return fail(IXK_INVALID_ARGUMENT, "fmha_paged: null argument");
+  if (!paged::aligned16(q) || !paged::aligned16(out) || !paged::aligned16(workspace))
+    return fail(IXK_INVALID_ARGUMENT, "fmha_paged: q, out and workspace must be 16-byte aligned");
+  if (d->requests > 1 && d->table_stride < d->columns) return fail(IXK_INVALID_ARGUMENT, "fmha_paged: rows of the page table overlap");
+  if (mask != nullptr && (d->mask_words < 1 || (d->rows > 1 && d->mask_stride < d->mask_words)))
+    return fail(IXK_INVALID_ARGUMENT, "fmha_paged: mask must have words, and rows that do not overlap");
+  for (int i = 0; i < 2; ++i) {
+    const int64_t extent = i == 0 ? d->rows : d->heads;
+    if (d->q_strides[i] % 8 != 0 || d->o_strides[i] % 8 != 0)
+      return fail(IXK_UNIMPLEMENTED, "fmha_paged: q and out strides must be multiples of 8 elements (16 bytes)");
+    if (extent > 1 && (d->q_strides[i] < c->head_size || d->o_strides[i] < c->head_size))
+      return fail(IXK_INVALID_ARGUMENT, "fmha_paged: rows of q or out overlap");
+  }
+  DeviceInfo info;
+  if (int st = get_device_info(&info)) return st;
+  if (d->requests == 0 || d->rows == 0) return IXK_OK;
+  if (info.sm_count > 148) info.sm_count = 148;        // (what the workspace was asked for)
+  const fmha_paged::Scratch scratch = fmha_paged::scratch_of(d, c, info.sm_count);
+  if (workspace == nullptr || workspace_bytes < scratch.total)
+    return fail(IXK_WORKSPACE_TOO_SMALL, "fmha_paged: workspace_bytes is below ixk_fmha_paged_fwd_workspace_bytes");
+
+  fmha_paged::Args a{};
+  a.requests = d->requests;
+  a.heads = d->heads;
+  a.kv_heads = c->heads;
+  a.group = d->heads / c->heads;
+  a.head_size = c->head_size;
+  a.block_tokens = fmha_paged::kRows / a.group;
+  a.rows_in = static_cast<int>(d->rows);
+  a.columns = d->columns;
+  a.page_shift = __builtin_ctz(static_cast<unsigned>(c->page_size));
+  a.pages = c->pages;
+  a.cap = d->columns * c->page_size;
+  a.is_bf16 = c->dtype == IXK_BF16;
+  a.scale_log2 = d->head_scale * fmha_paged::kLog2e;
+  a.table_stride = d->table_stride;
+  a.mask_stride = d->mask_stride;
+  a.mask_words = d->mask_words;
+  a.table = page_table, a.lengths = lengths, a.row_start = row_start, a.granted = granted, a.mask = mask;
+  a.v = static_cast<const uint16_t*>(v_pages);
+  for (int i = 0; i < 3; ++i) a.v_strides[i] = c->v_strides[i + 1];
+  a.out = static_cast<uint16_t*>(out);
+  for (int i = 0; i < 2; ++i) a.o_strides[i] = d->o_strides[i];
+  a.lse = lse;
+  a.status_word = info.status_word;
+  a.part_rows = scratch.part_rows;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  a.meta = reinterpret_cast<int4*>(ws + scratch.meta);
+  a.part_stat = reinterpret_cast<float4*>(ws + scratch.stat);
+  a.part_o = reinterpret_cast<float*>(ws + scratch.o);
+
+  const CUtensorMapDataType type = a.is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  // (the stride of a dimension of one entry is never used: any that a map takes)
+  auto bytes = [](int64_t stride, int64_t extent) { return static_cast<uint64_t>(extent > 1 ? stride * 2 : 512); };
+  CUtensorMap mq, mk, mv;
+  TmapSpec sq{type, 3, {static_cast<uint64_t>(c->head_size), static_cast<uint64_t>(d->heads), static_cast<uint64_t>(d->rows)},
+              {bytes(d->q_strides[1], d->heads), bytes(d->q_strides[0], d->rows)},
+              {fmha_paged::kChunkElems, static_cast<uint32_t>(a.group), static_cast<uint32_t>(a.block_tokens)}, true};
+  if (int st = encode_tmap(&mq, q, sq)) return st;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t* s = i == 0 ? c->k_strides : c->v_strides;
+    TmapSpec sk{type, 4,
+                {static_cast<uint64_t>(c->head_size), static_cast<uint64_t>(c->heads), static_cast<uint64_t>(c->page_size), static_cast<uint64_t>(c->pages)},
+                {bytes(s[3], c->heads), bytes(s[2], c->page_size), bytes(s[1], c->pages)},
+                {fmha_paged::kChunkElems, 1, static_cast<uint32_t>(std::min(c->page_size, fmha_paged::kKeys)), 1}, true};
+    if (int st = encode_tmap(i == 0 ? &mk : &mv, i == 0 ? k_pages : v_pages, sk)) return st;
+  }
+  auto s = static_cast<cudaStream_t>(cuda_stream);
+  const int dim = fmha_paged::head_dim(c->head_size);
+  if (dim == 64) return fmha_paged::launch<64>(mq, mk, mv, a, info.sm_count, s);
+  if (dim == 128) return fmha_paged::launch<128>(mq, mk, mv, a, info.sm_count, s);
+  return fmha_paged::launch<256>(mq, mk, mv, a, info.sm_count, s);
+}
+
+}  // extern "C"

@@ -11,6 +11,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/DispatchKeySet.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
@@ -41,6 +42,13 @@ decltype(&ixk_linear_xent_bwd) g_xent_bwd;
 decltype(&ixk_linear_distill_fwd) g_distill_fwd;
 decltype(&ixk_linear_distill_bwd) g_distill_bwd;
 decltype(&ixk_linear_loss_workspace_bytes) g_loss_bytes;
+decltype(&ixk_paged_extend) g_extend;
+decltype(&ixk_paged_keep) g_keep;
+decltype(&ixk_qk_norm_rotary_fwd) g_qk_fwd;
+decltype(&ixk_qk_norm_rotary_bwd) g_qk_bwd;
+decltype(&ixk_qk_norm_rotary_bwd_workspace_bytes) g_qk_bwd_bytes;
+decltype(&ixk_fmha_paged_fwd) g_paged_fwd;
+decltype(&ixk_fmha_paged_fwd_workspace_bytes) g_paged_fwd_bytes;
 
 // A plain CUDA tensor, nullptr for anything else (None included; see `optional`).
 const at::Tensor* tensor(PyObject* o) {
@@ -649,6 +657,287 @@ IXK_PY_FUNCTION(py_linear_loss_backward, 14)
   return results(st, {{a[9] == Py_None ? nullptr : a[9], &made_dx}, {a[10] == Py_None ? nullptr : a[10], &made_dw}, {nullptr, &dbias}});
 IXK_PY_END
 
+// ------------------------------------------------------------------------------------------------ a paged cache
+
+// _require_here: given tensors are on the current device.
+bool here(std::initializer_list<const at::Tensor*> tensors) {
+  const auto device = c10::cuda::current_device();
+  for (const at::Tensor* t : tensors)
+    if (t != nullptr && t->device().index() != device) return false;
+  return true;
+}
+// _int32
+bool ints(const at::Tensor* t, int64_t n) {
+  return t != nullptr && t->scalar_type() == at::kInt && t->is_contiguous() && (n == 1 ? t->numel() == 1 : t->dim() == 1 && t->size(0) == n);
+}
+int32_t* ip(const at::Tensor* t) { return static_cast<int32_t*>(ptr(t)); }
+bool int_rows(const at::Tensor* t) { return t != nullptr && t->dim() == 2 && t->scalar_type() == at::kInt && (t->size(1) <= 1 || t->stride(1) == 1); }
+
+// _page_pool
+bool page_pool(const at::Tensor* table, const at::Tensor* lengths, const at::Tensor* free_pages, const at::Tensor* free_count, int64_t page_size,
+               ixk_page_pool* d) {
+  if (!int_rows(table) || free_pages == nullptr || free_pages->dim() != 1) return false;
+  const int64_t B = table->size(0), columns = table->size(1), pages = free_pages->size(0);
+  if (B > INT32_MAX || columns > INT32_MAX || pages > INT32_MAX || page_size > INT32_MAX || page_size < 1) return false;
+  *d = ixk_page_pool{static_cast<int32_t>(page_size), static_cast<int32_t>(pages), static_cast<int32_t>(B), static_cast<int32_t>(columns), table->stride(0)};
+  return ints(lengths, B) && ints(free_pages, pages) && ints(free_count, 1);
+}
+
+// _paged_cache
+bool paged_cache(const at::Tensor* k, const at::Tensor* v, bool layers, ixk_paged_cache* c) {
+  if (k == nullptr || v == nullptr) return false;
+  const int64_t dims = k->dim();
+  if ((dims != 4 && !(layers && dims == 5)) || v->sizes() != k->sizes() || v->scalar_type() != k->scalar_type() || !float_type(*k, false) ||
+      k->numel() == 0 || k->stride(dims - 1) != 1 || v->stride(dims - 1) != 1)
+    return false;
+  const int64_t at = dims - 4;
+  for (int64_t i = 0; i < dims; ++i)
+    if (k->size(i) > INT32_MAX) return false;
+  c->dtype = dtype_of(*k);
+  c->pages = static_cast<int32_t>(k->size(at));
+  c->page_size = static_cast<int32_t>(k->size(at + 1));
+  c->heads = static_cast<int32_t>(k->size(at + 2));
+  c->head_size = static_cast<int32_t>(k->size(at + 3));
+  c->layers = at == 1 ? static_cast<int32_t>(k->size(0)) : 1;
+  for (int i = 0; i < 4; ++i) {
+    const int64_t dim = i - 1 + at;
+    const bool used = dim >= 0 && k->size(dim) != 1;
+    c->k_strides[i] = used ? k->stride(dim) : 0;
+    c->v_strides[i] = used ? v->stride(dim) : 0;
+  }
+  return true;
+}
+
+// page_table, lengths, new_tokens, free_pages, free_count, rows, page_size, out, stream
+IXK_PY_FUNCTION(py_paged_extend, 9)
+  const at::Tensor *table = tensor(a[0]), *lengths = tensor(a[1]), *fresh = tensor(a[2]), *pages = tensor(a[3]), *count = tensor(a[4]);
+  int64_t rows, page_size;
+  void* stream;
+  ixk_page_pool d;
+  if (!integer(a[5], &rows) || !integer(a[6], &page_size) || rows < 0 || !stream_arg(a[8], &stream) ||
+      !page_pool(table, lengths, pages, count, page_size, &d) || !ints(fresh, d.requests) || !here({table, lengths, fresh, pages, count}))
+    Py_RETURN_NONE;
+  const int64_t shapes[6] = {d.requests + 1, d.requests, rows, rows, rows, 1};
+  at::Tensor made[6];
+  const at::Tensor* o[6];
+  PyObject* given[6] = {nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
+  if (a[7] == Py_None) {
+    if (a[8] != Py_None) Py_RETURN_NONE;    // (the twin allocates in that stream's pool)
+    for (int i = 0; i < 6; ++i) {
+      made[i] = like(*lengths, {shapes[i]}, at::kInt);
+      o[i] = &made[i];
+    }
+  } else {
+    if (!PyTuple_Check(a[7]) || PyTuple_GET_SIZE(a[7]) != 6) Py_RETURN_NONE;
+    for (int i = 0; i < 6; ++i) {
+      given[i] = PyTuple_GET_ITEM(a[7], i);
+      o[i] = tensor(given[i]);
+      if (!ints(o[i], shapes[i]) || !here({o[i]})) Py_RETURN_NONE;
+    }
+  }
+  int32_t *pt = ip(table), *pl = ip(lengths), *pn = ip(fresh), *pp = ip(pages), *pc = ip(count), *r[6];
+  for (int i = 0; i < 6; ++i) r[i] = ip(o[i]);
+  const int st = unlocked([&] { return g_extend(&d, pl, pn, pt, pp, pc, r[5], r[1], r[0], rows, r[2], r[3], r[4], stream); });
+  return results(st, {{given[0], &made[0]}, {given[1], &made[1]}, {given[2], &made[2]}, {given[3], &made[3]}, {given[4], &made[4]}, {given[5], &made[5]}});
+IXK_PY_END
+
+// page_table, lengths, granted, kept, free_pages, free_count, page_size, path, k_pages, v_pages, lengths_out, free_count_out, stream
+IXK_PY_FUNCTION(py_paged_keep, 13)
+  const at::Tensor *table = tensor(a[0]), *lengths = tensor(a[1]), *granted = tensor(a[2]), *kept = tensor(a[3]), *pages = tensor(a[4]),
+                   *count = tensor(a[5]), *path, *k, *v, *lengths_out, *count_out;
+  int64_t page_size;
+  void* stream;
+  ixk_page_pool d;
+  ixk_paged_cache c;
+  if (!integer(a[6], &page_size) || !optional(a[7], &path) || !optional(a[8], &k) || !optional(a[9], &v) || !optional(a[10], &lengths_out) ||
+      !optional(a[11], &count_out) || !stream_arg(a[12], &stream) || !page_pool(table, lengths, pages, count, page_size, &d) ||
+      !ints(granted, d.requests) || !ints(kept, d.requests) ||
+      !here({table, lengths, granted, kept, pages, count, path, k, v, lengths_out, count_out}))
+    Py_RETURN_NONE;
+  if (path != nullptr ? !int_rows(path) || path->size(0) != d.requests || !paged_cache(k, v, true, &c) : k != nullptr || v != nullptr) Py_RETURN_NONE;
+  if ((lengths_out == nullptr || count_out == nullptr) && a[12] != Py_None) Py_RETURN_NONE;
+  at::Tensor made_lengths, made_count;
+  if (lengths_out == nullptr) {
+    made_lengths = like(*lengths, {d.requests}, at::kInt);
+    lengths_out = &made_lengths;
+  }
+  if (count_out == nullptr) {
+    made_count = like(*lengths, {1}, at::kInt);
+    count_out = &made_count;
+  }
+  if (!ints(lengths_out, d.requests) || !ints(count_out, 1)) Py_RETURN_NONE;
+  int32_t *pt = ip(table), *pl = ip(lengths), *pg = ip(granted), *pk = ip(kept), *pp = ip(pages), *pc = ip(count), *ppath = ip(path),
+          *plo = ip(lengths_out), *pco = ip(count_out);
+  void *kp = ptr(k), *vp = ptr(v);
+  const int64_t columns = path != nullptr ? path->size(1) : 0, stride = path != nullptr ? path->stride(0) : 0;
+  const ixk_paged_cache* cache = path != nullptr ? &c : nullptr;
+  const int st = unlocked([&] { return g_keep(&d, pl, pg, pk, ppath, columns, stride, pt, pp, pc, pco, plo, cache, kp, vp, stream); });
+  return results(st, {{a[10] == Py_None ? nullptr : a[10], &made_lengths}, {a[11] == Py_None ? nullptr : a[11], &made_count}});
+IXK_PY_END
+
+// _heads_view
+bool heads_view(const at::Tensor* t, at::IntArrayRef sizes, at::ScalarType type, int64_t* strides) {
+  if (t == nullptr || t->dim() != 3 || t->sizes() != sizes || t->scalar_type() != type || (t->size(2) > 1 && t->stride(2) != 1)) return false;
+  for (int i = 0; i < 2; ++i) strides[i] = t->size(i) == 1 ? 0 : t->stride(i);
+  return true;
+}
+// _qk_desc
+bool qk_desc(const at::Tensor* q, const at::Tensor* k, const at::Tensor* q_gain, const at::Tensor* k_gain, double offset, double eps,
+             const at::Tensor* cos, const at::Tensor* sin, const at::Tensor* positions, bool half_split, ixk_qk_desc* d) {
+  if (q == nullptr || k == nullptr || cos == nullptr || sin == nullptr || q->dim() != 3 || k->dim() != 3 || k->size(0) != q->size(0) ||
+      k->size(2) != q->size(2) || !float_type(*q, true) || q->size(1) > INT32_MAX || k->size(1) > INT32_MAX || q->size(2) > INT32_MAX)
+    return false;
+  *d = ixk_qk_desc{};
+  if (!heads_view(q, q->sizes(), q->scalar_type(), d->q_strides) || !heads_view(k, k->sizes(), q->scalar_type(), d->k_strides)) return false;
+  if (!param(q_gain, q->size(2), *q) || !param(k_gain, q->size(2), *q) ||
+      (q_gain != nullptr && k_gain != nullptr && q_gain->scalar_type() != k_gain->scalar_type()))
+    return false;
+  for (const at::Tensor* t : {cos, sin})
+    if (t->dim() != 2 || t->scalar_type() != at::kFloat || t->sizes() != cos->sizes() || !t->is_contiguous() || t->size(1) > INT32_MAX / 2) return false;
+  if (positions != nullptr && ((positions->scalar_type() != at::kInt && positions->scalar_type() != at::kLong) || positions->dim() != 1 ||
+                               positions->size(0) != q->size(0) || !positions->is_contiguous()))
+    return false;
+  const at::Tensor& gained = q_gain != nullptr ? *q_gain : k_gain != nullptr ? *k_gain : *q;
+  d->dtype = dtype_of(*q);
+  d->param_dtype = dtype_of(gained);
+  d->tokens = q->size(0);
+  d->heads = static_cast<int32_t>(q->size(1));
+  d->kv_heads = static_cast<int32_t>(k->size(1));
+  d->head_size = static_cast<int32_t>(q->size(2));
+  d->rotary_dim = static_cast<int32_t>(2 * cos->size(1));
+  d->places = cos->size(0);
+  d->interleaved = half_split ? 0 : 1;
+  d->position_bytes = positions != nullptr && positions->scalar_type() == at::kLong ? 8 : 4;
+  d->eps = static_cast<float>(eps);
+  d->gain_offset = static_cast<float>(offset);
+  return true;
+}
+
+// q, k, q_gain, k_gain, gain_offset, eps, cos, sin, positions, half_split, v, slots, k_pages, v_pages, q_out, k_out, stream
+IXK_PY_FUNCTION(py_qk_forward, 17)
+  const at::Tensor *q = tensor(a[0]), *k = tensor(a[1]), *qg, *kg, *cos = tensor(a[6]), *sin = tensor(a[7]), *pos, *v, *slots, *kp, *vp, *qo, *ko;
+  double offset, eps;
+  void* stream;
+  ixk_qk_desc d;
+  ixk_paged_cache c;
+  if (!optional(a[2], &qg) || !optional(a[3], &kg) || !number(a[4], &offset) || !number(a[5], &eps) || !optional(a[8], &pos) ||
+      !PyBool_Check(a[9]) || !optional(a[10], &v) || !optional(a[11], &slots) || !optional(a[12], &kp) || !optional(a[13], &vp) ||
+      !optional(a[14], &qo) || !optional(a[15], &ko) || !stream_arg(a[16], &stream) ||
+      !qk_desc(q, k, qg, kg, offset, eps, cos, sin, pos, a[9] == Py_True, &d) || !here({q, k, qg, kg, cos, sin, pos, v, slots, kp, vp, qo, ko}))
+    Py_RETURN_NONE;
+  const bool paged = v != nullptr || slots != nullptr || kp != nullptr || vp != nullptr;
+  if (paged && (ko != nullptr || !ints(slots, d.tokens) || !heads_view(v, k->sizes(), q->scalar_type(), d.v_strides) || !paged_cache(kp, vp, false, &c)))
+    Py_RETURN_NONE;
+  if (a[16] != Py_None && (qo == nullptr || (!paged && ko == nullptr))) Py_RETURN_NONE;
+  at::Tensor made_q, made_k;
+  if (qo == nullptr) {
+    made_q = like(*q, q->sizes(), q->scalar_type());
+    qo = &made_q;
+  }
+  if (!paged && ko == nullptr) {
+    made_k = like(*k, k->sizes(), k->scalar_type());
+    ko = &made_k;
+  }
+  if (!heads_view(qo, q->sizes(), q->scalar_type(), d.q_out_strides) || (ko != nullptr && !heads_view(ko, k->sizes(), q->scalar_type(), d.k_out_strides)))
+    Py_RETURN_NONE;
+  void *pq = ptr(q), *pk = ptr(k), *pv = ptr(v), *pqg = ptr(qg), *pkg = ptr(kg), *ppos = ptr(pos), *pqo = ptr(qo), *pko = ptr(ko), *pkp = ptr(kp),
+       *pvp = ptr(vp);
+  const float *pc = static_cast<const float*>(ptr(cos)), *ps = static_cast<const float*>(ptr(sin));
+  const int32_t* psl = ip(slots);
+  const int st = unlocked([&] { return g_qk_fwd(&d, pq, pk, pv, pqg, pkg, pc, ps, ppos, pqo, pko, paged ? &c : nullptr, psl, pkp, pvp, stream); });
+  return results(st, {{a[14] == Py_None ? nullptr : a[14], &made_q}, {a[15] == Py_None ? nullptr : a[15], &made_k}});
+IXK_PY_END
+
+// grad_q, grad_k, q, k, q_gain, k_gain, gain_offset, eps, cos, sin, positions, half_split, dq, dk, workspace, stream
+IXK_PY_FUNCTION(py_qk_backward, 16)
+  const at::Tensor *gq = tensor(a[0]), *gk = tensor(a[1]), *q = tensor(a[2]), *k = tensor(a[3]), *qg, *kg, *cos = tensor(a[8]), *sin = tensor(a[9]),
+                   *pos, *dq, *dk, *ws;
+  double offset, eps;
+  void* stream;
+  ixk_qk_desc d;
+  if (!optional(a[4], &qg) || !optional(a[5], &kg) || !number(a[6], &offset) || !number(a[7], &eps) || !optional(a[10], &pos) ||
+      !PyBool_Check(a[11]) || !optional(a[12], &dq) || !optional(a[13], &dk) || !optional(a[14], &ws) || !stream_arg(a[15], &stream) ||
+      !qk_desc(q, k, qg, kg, offset, eps, cos, sin, pos, a[11] == Py_True, &d) || !heads_view(gq, q->sizes(), q->scalar_type(), d.gq_strides) ||
+      !heads_view(gk, k->sizes(), q->scalar_type(), d.gk_strides) || !here({gq, gk, q, k, qg, kg, cos, sin, pos, dq, dk, ws}))
+    Py_RETURN_NONE;
+  const bool gains = qg != nullptr || kg != nullptr;
+  if (a[15] != Py_None && (dq == nullptr || dk == nullptr || gains)) Py_RETURN_NONE;
+  at::Tensor made_q, made_k, dqg, dkg, scratch;
+  if (dq == nullptr) {
+    made_q = like(*q, q->sizes(), q->scalar_type());
+    dq = &made_q;
+  }
+  if (dk == nullptr) {
+    made_k = like(*k, k->sizes(), k->scalar_type());
+    dk = &made_k;
+  }
+  if (!heads_view(dq, q->sizes(), q->scalar_type(), d.q_out_strides) || !heads_view(dk, k->sizes(), q->scalar_type(), d.k_out_strides)) Py_RETURN_NONE;
+  if (qg != nullptr) dqg = like(*q, qg->sizes(), qg->scalar_type());
+  if (kg != nullptr) dkg = like(*q, kg->sizes(), kg->scalar_type());
+  if (gains && ws == nullptr) {
+    scratch = like(*q, {static_cast<int64_t>(g_qk_bwd_bytes(&d))}, at::kByte);
+    ws = &scratch;
+  }
+  void *pgq = ptr(gq), *pgk = ptr(gk), *pq = ptr(q), *pk = ptr(k), *pqg = ptr(qg), *pkg = ptr(kg), *ppos = ptr(pos), *pdq = ptr(dq), *pdk = ptr(dk),
+       *pw = ptr(ws), *pdqg = dqg.defined() ? ptr(&dqg) : nullptr, *pdkg = dkg.defined() ? ptr(&dkg) : nullptr;
+  const float *pc = static_cast<const float*>(ptr(cos)), *ps = static_cast<const float*>(ptr(sin));
+  const size_t bytes = size_of(ws);
+  const int st = unlocked([&] { return g_qk_bwd(&d, pgq, pgk, pq, pk, pqg, pkg, pc, ps, ppos, pdq, pdk, pdqg, pdkg, pw, bytes, stream); });
+  return results(st, {{a[12] == Py_None ? nullptr : a[12], &made_q}, {a[13] == Py_None ? nullptr : a[13], &made_k}, {nullptr, &dqg}, {nullptr, &dkg}});
+IXK_PY_END
+
+// q, k_pages, v_pages, page_table, lengths, row_start, granted, scale, mask, out, lse, with_lse, workspace, stream
+IXK_PY_FUNCTION(py_fmha_paged, 14)
+  const at::Tensor *q = tensor(a[0]), *k = tensor(a[1]), *v = tensor(a[2]), *table = tensor(a[3]), *lengths = tensor(a[4]), *start = tensor(a[5]),
+                   *granted = tensor(a[6]), *mask, *out, *lse, *ws;
+  double scale;
+  void* stream;
+  ixk_fmha_paged_desc d{};
+  ixk_paged_cache c;
+  if (q == nullptr || !number(a[7], &scale) || !optional(a[8], &mask) || !optional(a[9], &out) || !optional(a[10], &lse) || !PyBool_Check(a[11]) ||
+      !optional(a[12], &ws) || !stream_arg(a[13], &stream) || !paged_cache(k, v, false, &c) || !int_rows(table) ||
+      !here({q, k, v, table, lengths, start, granted, mask, out, lse, ws}))
+    Py_RETURN_NONE;
+  const int64_t B = table->size(0);
+  if (q->dim() != 3 || q->scalar_type() != k->scalar_type() || q->size(2) != c.head_size || q->size(1) > INT32_MAX || B > INT32_MAX - 1 ||
+      table->size(1) > INT32_MAX || !ints(lengths, B) || !ints(start, B + 1) || !ints(granted, B) ||
+      (mask != nullptr && (!int_rows(mask) || mask->size(0) != q->size(0) || mask->size(1) < 1 || mask->size(1) > INT32_MAX)))
+    Py_RETURN_NONE;
+  const bool want_lse = lse != nullptr || a[11] == Py_True;
+  if (a[13] != Py_None && (out == nullptr || (want_lse && lse == nullptr) || ws == nullptr)) Py_RETURN_NONE;
+  at::Tensor made, made_lse, scratch;
+  if (out == nullptr) {
+    made = like(*q, q->sizes(), q->scalar_type());
+    out = &made;
+  }
+  d.rows = q->size(0);
+  d.heads = static_cast<int32_t>(q->size(1));
+  d.requests = static_cast<int32_t>(B);
+  d.columns = static_cast<int32_t>(table->size(1));
+  d.table_stride = table->stride(0);
+  d.head_scale = static_cast<float>(scale);
+  if (mask != nullptr) {
+    d.mask_words = static_cast<int32_t>(mask->size(1));
+    d.mask_stride = mask->stride(0);
+  }
+  if (!heads_view(q, q->sizes(), q->scalar_type(), d.q_strides) || !heads_view(out, q->sizes(), q->scalar_type(), d.o_strides)) Py_RETURN_NONE;
+  if (lse == nullptr && want_lse) {
+    made_lse = like(*q, {d.rows, q->size(1)}, at::kFloat);
+    lse = &made_lse;
+  }
+  if (lse != nullptr && (lse->scalar_type() != at::kFloat || lse->sizes() != q->sizes().slice(0, 2) || !lse->is_contiguous())) Py_RETURN_NONE;
+  if (ws == nullptr) {
+    scratch = like(*q, {static_cast<int64_t>(g_paged_fwd_bytes(&d, &c))}, at::kByte);
+    ws = &scratch;
+  }
+  void *pq = ptr(q), *pk = ptr(k), *pv = ptr(v), *po = ptr(out), *pw = ptr(ws);
+  int32_t *pt = ip(table), *pl = ip(lengths), *ps = ip(start), *pg = ip(granted), *pm = ip(mask);
+  float* ple = static_cast<float*>(ptr(lse));
+  const size_t bytes = size_of(ws);
+  const int st = unlocked([&] { return g_paged_fwd(&d, &c, pq, pk, pv, pt, pl, ps, pg, pm, po, ple, pw, bytes, stream); });
+  return results(st, {{a[9] == Py_None ? nullptr : a[9], &made}, {a[10] == Py_None ? nullptr : a[10], &made_lse}});
+IXK_PY_END
+
 PyObject* py_bind(PyObject*, PyObject* table) {
   struct Entry {
     const char* name;
@@ -677,6 +966,13 @@ PyObject* py_bind(PyObject*, PyObject* table) {
       {"ixk_linear_distill_fwd", reinterpret_cast<void**>(&g_distill_fwd)},
       {"ixk_linear_distill_bwd", reinterpret_cast<void**>(&g_distill_bwd)},
       {"ixk_linear_loss_workspace_bytes", reinterpret_cast<void**>(&g_loss_bytes)},
+      {"ixk_paged_extend", reinterpret_cast<void**>(&g_extend)},
+      {"ixk_paged_keep", reinterpret_cast<void**>(&g_keep)},
+      {"ixk_qk_norm_rotary_fwd", reinterpret_cast<void**>(&g_qk_fwd)},
+      {"ixk_qk_norm_rotary_bwd", reinterpret_cast<void**>(&g_qk_bwd)},
+      {"ixk_qk_norm_rotary_bwd_workspace_bytes", reinterpret_cast<void**>(&g_qk_bwd_bytes)},
+      {"ixk_fmha_paged_fwd", reinterpret_cast<void**>(&g_paged_fwd)},
+      {"ixk_fmha_paged_fwd_workspace_bytes", reinterpret_cast<void**>(&g_paged_fwd_bytes)},
   };
   for (const Entry& e : entries) {
     PyObject* address = PyDict_GetItemString(table, e.name);   // borrowed
@@ -705,6 +1001,11 @@ PyMethodDef methods[] = {
     IXK_METHOD("row_norm_backward", py_row_norm_backward),
     IXK_METHOD("linear_loss_forward", py_linear_loss_forward),
     IXK_METHOD("linear_loss_backward", py_linear_loss_backward),
+    IXK_METHOD("paged_extend", py_paged_extend),
+    IXK_METHOD("paged_keep", py_paged_keep),
+    IXK_METHOD("qk_forward", py_qk_forward),
+    IXK_METHOD("qk_backward", py_qk_backward),
+    IXK_METHOD("fmha_paged", py_fmha_paged),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "ixk_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
