@@ -44,7 +44,8 @@ constexpr int kThreads = 192;
 constexpr int kCopyWarp = 4;
 constexpr int kMmaWarp = 5;
 constexpr int kSoftmaxThreads = 128;
-constexpr int kTable = 40;            // requests whose numbers a worker holds in shared memory
+constexpr int kTable = 56;            // requests whose numbers a worker holds in shared memory
+constexpr int kTileCost = 1;          // what a tile costs beside its units (Q, masks, results)
 constexpr int kMinUnits = 2;          // shortest run: below that, joining parts costs more than it saves
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -64,7 +65,7 @@ struct Cfg {
   static constexpr int kSlots = kHeadDim == 64 ? 8 : 5;
   static constexpr int kTmemColumns = kHeadDim <= 128 ? 256 : 512;
   static constexpr int kTmemO = 2 * kKeys;                        // S in two buffers of 64 columns
-  static constexpr int kTailBytes = 8 * (10 + 2 * kSlots) + 32 + 8 * 8 + kTable * 12;
+  static constexpr int kTailBytes = 8 * (10 + 2 * kSlots) + 32 + 8 * 12 + kTable * 12;
   static constexpr int kSmemBytes = kQBytes + kSlots * kSlotBytes + kTailBytes;
   static_assert(kSmemBytes <= (kWorkers == 2 ? 115712 : 232448), "shared memory budget");
   static_assert(kTmemO + kHeadDim <= kTmemColumns, "TMEM budget");
@@ -85,10 +86,11 @@ struct Args {
   int64_t v_strides[3];       // page, token, head
   uint16_t* out;
   int64_t o_strides[2];
+  int out_sectors;            // out's rows start on 32-byte boundaries and hold whole 32-byte sectors
   float* lse;
   int* status_word;
   int part_rows;              // rows of a part in scratch
-  int4* meta;                 // [workers] the tile that a worker began and did not finish: request, key head, block, parts
+  int4* meta;                 // [workers] the tile that a worker began and did not finish: first row, first head, rows, parts
   float* part_o;              // [2 * workers][part_rows][kHeadDim]
   float4* part_stat;          // [2 * workers][part_rows]: maximum (log2), sum, sum of rounded weights
 };
@@ -111,63 +113,83 @@ __device__ __forceinline__ int block_keys(const Args& a, const Request& r, int t
   return static_cast<int>(min(static_cast<long long>(r.length) + seen, static_cast<long long>(a.cap)));
 }
 __device__ __forceinline__ int block_units(const Args& a, const Request& r, int t0) { return (block_keys(a, r, t0) + kKeys - 1) / kKeys; }
-// Units of one key head of a request.
-__device__ __forceinline__ long long head_units(const Args& a, const Request& r) {
+// What one key head of a request costs: its units, and kTileCost for every tile.
+__device__ __forceinline__ long long head_cost(const Args& a, const Request& r) {
+  if (r.rows <= 0) return 0;
+  if (r.rows <= a.block_tokens) return block_units(a, r, 0) + kTileCost;
   long long sum = 0;
-  for (int t0 = 0; t0 < r.rows; t0 += a.block_tokens) sum += block_units(a, r, t0);
+  for (int t0 = 0; t0 < r.rows; t0 += a.block_tokens) sum += block_units(a, r, t0) + kTileCost;
   return sum;
 }
 
-// A worker's walk over its run of units.
+// A worker's walk over its run, a stretch of the costs of all tiles one behind the other.  A tile's costs begin with kTileCost
+// that stand for its start and end; the worker in whose run these end begins it.
 struct Walk {
   int b, kv_head, t0;
   Request req;
-  int unit, units;            // of the tile
-  int first;                  // the first unit of the tile in this run
-  long long left;             // units left in the run, this one included
+  int first, unit, end;       // units of the tile: the run's first, the present one, behind the run's last
+  int units;                  // of the whole tile
+  long long budget;           // the run's end, from the tile's start on
+  bool live;
   const int* table;           // the run's first requests in shared memory
   int table_base, table_count;
 
   __device__ __forceinline__ Request request(const Args& a, int i) const {
     const int k = i - table_base;
-    if (k < table_count) return Request{table[3 * k], table[3 * k + 1], table[3 * k + 2]};
+    if (k >= 0 && k < table_count) return Request{table[3 * k], table[3 * k + 1], table[3 * k + 2]};
     return load_request(a, i);
   }
-  __device__ __forceinline__ void begin(const Args& a, int start_b, long long offset, long long count, const int* shared, int shared_count) {
-    table = shared;
-    table_base = start_b;
-    table_count = shared_count;
-    b = start_b;
-    left = count;
-    if (left <= 0) return;
-    req = request(a, b);
-    const long long per_head = head_units(a, req);
-    kv_head = static_cast<int>(offset / per_head);
-    long long rest = offset - kv_head * per_head;
-    t0 = 0;
-    while (rest >= (units = block_units(a, req, t0))) {
-      rest -= units;
-      t0 += a.block_tokens;
-    }
-    unit = first = static_cast<int>(rest);
+  // The tile at (b, kv_head, t0), whose first `from` costs lie before the run.
+  __device__ __forceinline__ void enter(const Args& a, int from) {
+    units = block_units(a, req, t0);
+    first = unit = max(from - kTileCost, 0);
+    end = static_cast<int>(max(min(static_cast<long long>(units), budget - kTileCost), 0LL));
   }
-  __device__ __forceinline__ bool done() const { return left <= 0; }
-  __device__ __forceinline__ bool starts() const { return unit == first; }
-  __device__ __forceinline__ bool ends() const { return unit + 1 == units || left == 1; }      // the tile's last unit of this run
-  __device__ __forceinline__ void next(const Args& a) {
-    if (--left <= 0) return;
-    if (++unit < units) return;
-    unit = first = 0;
+  __device__ __forceinline__ void next_tile(const Args& a) {
+    budget -= units + kTileCost;
+    if (budget <= kTileCost) {        // (the next tile's first unit is another worker's, or there is none)
+      live = false;
+      return;
+    }
     t0 += a.block_tokens;
     if (t0 >= req.rows) {
       t0 = 0;
       if (++kv_head == a.kv_heads) {
         kv_head = 0;
-        do req = request(a, ++b);       // (units are left, so a request with rows follows)
-        while (req.rows == 0);
+        do {
+          if (++b >= a.requests) {
+            live = false;
+            return;
+          }
+          req = request(a, b);
+        } while (req.rows == 0);
       }
     }
-    units = block_units(a, req, t0);
+    enter(a, 0);
+  }
+  // `offset`: of the run's start in request start_b; `count`: its costs
+  __device__ __forceinline__ void begin(const Args& a, int start_b, long long offset, long long count) {
+    b = start_b;
+    live = count > 0;
+    if (!live) return;
+    req = request(a, b);
+    const long long per_head = head_cost(a, req);
+    kv_head = offset < per_head ? 0
+              : (offset >> 31) == 0 ? static_cast<int>(static_cast<unsigned>(offset) / static_cast<unsigned>(per_head))
+                                    : static_cast<int>(offset / per_head);
+    long long rest = offset - kv_head * per_head;
+    t0 = 0;
+    for (long long cost; rest >= (cost = block_units(a, req, t0) + kTileCost); t0 += a.block_tokens) rest -= cost;
+    budget = rest + count;
+    enter(a, static_cast<int>(rest));
+    if (unit >= end) next_tile(a);
+  }
+  __device__ __forceinline__ bool done() const { return !live; }
+  __device__ __forceinline__ bool starts() const { return unit == first; }
+  __device__ __forceinline__ bool ends() const { return unit + 1 == end; }                     // the tile's last unit of this run
+  __device__ __forceinline__ bool last() const { return ends() && budget - (units + kTileCost) <= kTileCost; }
+  __device__ __forceinline__ void next(const Args& a) {
+    if (++unit >= end) next_tile(a);
   }
 };
 
@@ -178,6 +200,12 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, bool bf16) {
   }
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+// 32 bytes, 32-byte aligned: a whole sector, where a lane's 16 would be half of one.
+__device__ __forceinline__ void store_sector(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+               "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
 }
 __device__ __forceinline__ float2 unpack2(uint32_t w, bool bf16) {
   if (bf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
@@ -259,8 +287,9 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   volatile int* odd_values = reinterpret_cast<volatile int*>(tail + 8);      // [3] by tile
   int* start_request = reinterpret_cast<int*>(tail + 20);
   long long* start_offset = reinterpret_cast<long long*>(tail + 24);
-  long long* sums = reinterpret_cast<long long*>(tail + 32);                 // [6 + 1]
-  int* table = reinterpret_cast<int*>(tail + 32 + 8 * 8);                    // [kTable][3]
+  long long* sums = reinterpret_cast<long long*>(tail + 32);                 // [6]
+  long long* other_sums = sums + 6;                                          // [6]
+  int* table = reinterpret_cast<int*>(tail + 32 + 8 * 12);                   // [kTable][3]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   ptx::AbortCtl ctl{abort_flag, args.status_word};
@@ -290,70 +319,88 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   }
   ptx::grid_dependency_sync();
 
-  // ---- the run: its length from the units of all requests, its start by a second walk over the sums
-  auto units_of = [&](int b) -> long long {
-    if (b >= args.requests) return 0;
-    return head_units(args, load_request(args, b)) * args.kv_heads;
-  };
-  const long long mine = units_of(threadIdx.x);
-  long long sum = mine;
-  for (int b = threadIdx.x + kThreads; b < args.requests; b += kThreads) sum += units_of(b);
+  // ---- the run: its length from the costs of all requests, its start from their sums
+  Request mine{0, 0, 0};
+  auto cost_of = [&](const Request& r) { return head_cost(args, r) * args.kv_heads; };
+  if (static_cast<int>(threadIdx.x) < args.requests) mine = load_request(args, threadIdx.x);
+  const long long my_cost = cost_of(mine);
+  auto prefix = [&](long long v) {     // inclusive, in the warp; the warp's sum to `sums`
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) sums[warp] = sum;
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += up;
+    }
+    if (lane == 31) sums[warp] = v;
+    return v;
+  };
+  long long upto = prefix(my_cost);
+  long long others = 0;                // of the requests behind the first kThreads
+  for (int b = threadIdx.x + kThreads; b < args.requests; b += kThreads) others += cost_of(load_request(args, b));
+  if (args.requests > kThreads) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) others += __shfl_xor_sync(0xffffffffu, others, o);
+    if (lane == 0) other_sums[warp] = others;
+  }
+  auto keep = [&](int i, const Request& r) {
+    table[3 * i] = r.length;
+    table[3 * i + 1] = r.rows;
+    table[3 * i + 2] = r.row0;
+  };
+  const bool few = args.requests <= kTable;
+  if (few && static_cast<int>(threadIdx.x) < args.requests) keep(threadIdx.x, mine);
   ptx::tc_fence_before_sync();
   __syncthreads();
   ptx::tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
   long long total = 0;
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) total += sums[w];
-  const long long run = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(kMinUnits));
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) upto += sums[w];
+    total += sums[w];
+  }
+  long long before = total;            // costs of the requests that the scan has been over
+  if (args.requests > kThreads)
+    for (int w = 0; w < kThreads / 32; ++w) total += other_sums[w];
+  const unsigned grid = gridDim.x;
+  long long run = (total >> 31) == 0 ? (static_cast<unsigned>(total) + grid - 1u) / grid : (total + grid - 1) / grid;
+  run = max(run, static_cast<long long>(kMinUnits + kTileCost));
   const long long start = run * blockIdx.x;
-  const long long count = max(min(run, total - start), 0LL);
+  const bool aligned = (q_smem & 1023u) == 0;
+  if (!aligned && threadIdx.x == 0) atomicCAS(args.status_word, 0, kSiteAlign);
+  const long long count = aligned ? max(min(run, total - start), 0LL) : 0LL;
   if (count > 0) {
-    long long before = 0;
-    for (int b0 = 0; b0 < args.requests; b0 += kThreads) {
-      const long long u = b0 == 0 ? mine : units_of(b0 + threadIdx.x);
-      long long upto = u;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
-      }
+    if (start >= upto - my_cost && start < upto) {
+      *start_request = threadIdx.x;
+      *start_offset = start - (upto - my_cost);
+    }
+    for (int b0 = kThreads; before <= start; b0 += kThreads) {      // (the same in all threads; start < total)
+      const int b = b0 + static_cast<int>(threadIdx.x);
+      const long long cost = b < args.requests ? cost_of(load_request(args, b)) : 0;
       __syncthreads();
-      if (lane == 31) sums[warp] = upto;
+      upto = prefix(cost) + before;
       __syncthreads();
-      long long all = 0;
 #pragma unroll
       for (int w = 0; w < kThreads / 32; ++w) {
         if (w < warp) upto += sums[w];
-        all += sums[w];
+        before += sums[w];
       }
-      upto += before;
-      if (start >= upto - u && start < upto) {
-        *start_request = b0 + threadIdx.x;
-        *start_offset = start - (upto - u);
+      if (start >= upto - cost && start < upto) {
+        *start_request = b;
+        *start_offset = start - (upto - cost);
       }
-      before += all;
-      if (before > start) break;
     }
     __syncthreads();
-    const int b = *start_request;
-    const int i = b + static_cast<int>(threadIdx.x);
-    if (threadIdx.x < kTable && i < args.requests) {
-      const Request r = load_request(args, i);
-      table[3 * threadIdx.x] = r.length;
-      table[3 * threadIdx.x + 1] = r.rows;
-      table[3 * threadIdx.x + 2] = r.row0;
+    if (!few) {
+      const int i = *start_request + static_cast<int>(threadIdx.x);
+      if (threadIdx.x < kTable && i < args.requests) keep(threadIdx.x, load_request(args, i));
+      __syncthreads();
     }
-    __syncthreads();
   }
-  const bool aligned = (q_smem & 1023u) == 0;
-  if (!aligned && threadIdx.x == 0) atomicCAS(args.status_word, 0, kSiteAlign);
   Walk walk;
-  walk.begin(args, count > 0 ? *start_request : 0, count > 0 ? *start_offset : 0, aligned ? count : 0, table,
-             count > 0 ? min(kTable, args.requests - *start_request) : 0);
+  walk.table = table;
+  walk.table_base = count > 0 && !few ? *start_request : 0;
+  walk.table_count = min(kTable, args.requests - walk.table_base);
+  walk.begin(args, count > 0 ? *start_request : 0, count > 0 ? *start_offset : 0, count);
 
   if (warp == kCopyWarp) {
     // ------------------------------------------------------------------ copies: a lane takes one page's 64 columns
@@ -485,10 +532,9 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     const uint32_t lane_addr = static_cast<uint32_t>(warp * 32) << 16;
     const uint32_t o_addr = tmem_base + lane_addr + C::kTmemO;
     const int row_token = row / args.group, row_head = row - row_token * args.group;
-    const long long all_units = count;
     uint32_t g = 0, tiles = 0;
     bool alive = true;
-    int4 begun = make_int4(0, 0, 0, 0);       // the tile that this worker leaves to others: none
+    int4 begun = make_int4(0, 0, 0, 0);       // the tile that this worker leaves to others: none so far
     while (alive && !walk.done()) {
       const Request req = walk.req;
       const int token = walk.t0 + row_token;
@@ -589,7 +635,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         }
         if (masked) {
           // V behind the last key, and values of drafts that are no numbers
-          const uint32_t load = static_cast<long long>(g) < all_units - 1 ? 2 * g + 2 : 2 * g + 1;
+          const uint32_t load = walk.last() ? 2 * g + 1 : 2 * g + 2;
           if (!ptx::mbar_wait(kv_full(load % kSlots), (load / kSlots) & 1u, ctl, kSiteSoftmaxV)) {
             alive = false;
             break;
@@ -640,14 +686,15 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       ptx::tc_fence_after_sync();
       const bool odd = odd_values[tiles % 3] != 0;
       ++tiles;
-      const bool whole = first_unit == 0 && walk.unit + 1 == walk.units;
+      const bool whole = first_unit == 0 && walk.end == walk.units;
       const int head = walk.kv_head * args.group + row_head;
       int64_t part = 2 * static_cast<int64_t>(blockIdx.x);
       if (!whole && first_unit == 0) {
         ++part;
-        // (the tile's units start at start + g - (units of it so far); the workers behind this one have runs of `run`)
-        const long long after = walk.units - (walk.unit + 1);
-        begun = make_int4(walk.b, walk.kv_head, walk.t0, static_cast<int>((after + run - 1) / run) + 1);
+        // (the workers behind this one have runs of `run`)
+        const long long after = walk.units + kTileCost - walk.budget;
+        begun = make_int4(req.row0 + walk.t0, walk.kv_head * args.group, min(args.block_tokens, req.rows - walk.t0) * args.group,
+                          static_cast<int>((after + run - 1) / run) + 1);
       }
       if (warp_ok) {
         const float inv_l = 1.0f / r_run;
@@ -678,21 +725,27 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             }
           }
           if (whole) {
+            uint32_t w[16];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if (c * 32 + e * 8 >= args.head_size) break;
-              uint32_t w[4];
+            for (int i = 0; i < 16; ++i)
+              w[i] = r_run == 0.0f ? 0u : pack2(__uint_as_float(o[2 * i]) * inv_l, __uint_as_float(o[2 * i + 1]) * inv_l, bf16);
+            if (args.out_sectors) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int at = e * 8 + i * 2;
-                w[i] = r_run == 0.0f ? 0u : pack2(__uint_as_float(o[at]) * inv_l, __uint_as_float(o[at + 1]) * inv_l, bf16);
-              }
-              reinterpret_cast<uint4*>(out_row + c * 32)[e] = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int e = 0; e < 2; ++e)
+                if (c * 32 + e * 16 < args.head_size)
+                  store_sector(out_row + c * 32 + e * 16, {w[8 * e], w[8 * e + 1], w[8 * e + 2], w[8 * e + 3], w[8 * e + 4], w[8 * e + 5], w[8 * e + 6],
+                                                           w[8 * e + 7]});
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (c * 32 + e * 8 < args.head_size)
+                  reinterpret_cast<uint4*>(out_row + c * 32)[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
             }
           } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              reinterpret_cast<uint4*>(part_row + c * 32)[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            for (int e = 0; e < 4; ++e)
+              store_sector(part_row + c * 32 + e * 8, {o[8 * e], o[8 * e + 1], o[8 * e + 2], o[8 * e + 3], o[8 * e + 4], o[8 * e + 5], o[8 * e + 6],
+                                                       o[8 * e + 7]});
           }
         }
         if (row_ok) {
@@ -720,64 +773,70 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 // Joins the parts of the tiles that several workers did: a warp a row.  With the parts' maxima m_i and sums l_i, M = max m_i:
 //   o = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i
 // Worker w's own part is at 2 w + 1, those of the workers behind it at 2 (w + i).
+// Bound by trips to memory: what it needs of the tile is one load, then all parts' numbers and values are asked for together,
+// four parts at a time.
 constexpr int kJoinWarps = 8;
+constexpr int kJoinParts = 4;
 template <int kHeadDim>
 __global__ void __launch_bounds__(kJoinWarps * 32) fmha_paged_join_kernel(const __grid_constant__ Args a) {
   ptx::grid_dependency_sync();
-  const int4 tile = a.meta[blockIdx.x];
-  if (tile.w == 0) return;
-  const Request req = load_request(a, tile.x);
+  const int4 tile = a.meta[blockIdx.x];        // first row, first head, rows, parts
   const int lane = threadIdx.x & 31;
-  const int rows = min(a.block_tokens, req.rows - tile.z) * a.group;
   const bool bf16 = a.is_bf16 != 0;
   constexpr int kPer = kHeadDim / 32;
-  for (int row = blockIdx.y * kJoinWarps + (threadIdx.x >> 5); row < rows; row += gridDim.y * kJoinWarps) {
-    auto part_of = [&](int i) { return 2 * (static_cast<int64_t>(blockIdx.x) + i) + (i == 0 ? 1 : 0); };
-    float top = -INFINITY, mine_m = 0.0f, mine_l = 0.0f, mine_r = 0.0f, sum = 0.0f, rounded = 0.0f;
-    // a lane a part, 32 parts at a time
-    for (int i0 = 0; i0 < tile.w; i0 += 32) {
-      float m = -INFINITY;
-      if (i0 + lane < tile.w) m = a.part_stat[part_of(i0 + lane) * a.part_rows + row].x;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      top = fmaxf(top, m);
-    }
-    const float use = top == -INFINITY ? 0.0f : top;
+  for (int row = blockIdx.y * kJoinWarps + (threadIdx.x >> 5); row < tile.z; row += gridDim.y * kJoinWarps) {
+    auto part_of = [&](int i) { return (2 * (static_cast<int64_t>(blockIdx.x) + i) + (i == 0 ? 1 : 0)) * a.part_rows + row; };
+    float top = -INFINITY, sum = 0.0f, rounded = 0.0f;
     float o[kPer];
 #pragma unroll
     for (int e = 0; e < kPer; ++e) o[e] = 0.0f;
-    for (int i0 = 0; i0 < tile.w; i0 += 32) {
-      if (i0 + lane < tile.w) {
-        const float4 s = a.part_stat[part_of(i0 + lane) * a.part_rows + row];
-        mine_m = ptx::ex2_approx(s.x - use);
-        mine_l = s.y;
-        mine_r = s.z;
-      }
-      const int n = min(32, tile.w - i0);
-#pragma unroll 4
-      for (int i = 0; i < n; ++i) {
-        const float weight = __shfl_sync(0xffffffffu, mine_m, i);
-        sum = fmaf(weight, __shfl_sync(0xffffffffu, mine_l, i), sum);
-        rounded = fmaf(weight, __shfl_sync(0xffffffffu, mine_r, i), rounded);
-        const float* src = a.part_o + (part_of(i0 + i) * a.part_rows + row) * kHeadDim + lane * kPer;
-        // (a part that saw nothing has weight 0, and nothing in it)
+    for (int i0 = 0; i0 < tile.w; i0 += kJoinParts) {
+      float4 stat[kJoinParts];
+      float2 v[kJoinParts][kPer / 2];
 #pragma unroll
-        for (int e = 0; e < kPer; e += 2) {
-          const float2 v = *reinterpret_cast<const float2*>(src + e);
-          o[e] = fmaf(weight, v.x, o[e]);
-          o[e + 1] = fmaf(weight, v.y, o[e + 1]);
+      for (int i = 0; i < kJoinParts; ++i) {
+        stat[i] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+        if (i0 + i < tile.w) {
+          const int64_t p = part_of(i0 + i);
+          stat[i] = a.part_stat[p];
+          const float2* src = reinterpret_cast<const float2*>(a.part_o + p * kHeadDim) + lane * (kPer / 2);
+#pragma unroll
+          for (int e = 0; e < kPer / 2; ++e) v[i][e] = src[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < kPer / 2; ++e) v[i][e] = make_float2(0.0f, 0.0f);
+        }
+      }
+      float m = top;
+#pragma unroll
+      for (int i = 0; i < kJoinParts; ++i) m = fmaxf(m, stat[i].x);
+      const float use = m == -INFINITY ? 0.0f : m;
+      const float old = ptx::ex2_approx(top - use);       // (top - use: -inf, or a number)
+      top = m;
+      sum *= old;
+      rounded *= old;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) o[e] *= old;
+#pragma unroll
+      for (int i = 0; i < kJoinParts; ++i) {
+        const float weight = ptx::ex2_approx(stat[i].x - use);      // a part that saw nothing: 0, and nothing in it
+        sum = fmaf(weight, stat[i].y, sum);
+        rounded = fmaf(weight, stat[i].z, rounded);
+#pragma unroll
+        for (int e = 0; e < kPer / 2; ++e) {
+          o[2 * e] = fmaf(weight, v[i][e].x, o[2 * e]);
+          o[2 * e + 1] = fmaf(weight, v[i][e].y, o[2 * e + 1]);
         }
       }
     }
-    const int q_row = req.row0 + tile.z + row / a.group, head = tile.y * a.group + row % a.group;
+    const int token = row / a.group;
+    const int64_t q_row = tile.x + token, head = tile.y + row - token * a.group;
     const float inv = 1.0f / rounded;
-    uint16_t* out = a.out + q_row * a.o_strides[0] + head * a.o_strides[1];
+    uint16_t* out = a.out + q_row * a.o_strides[0] + head * a.o_strides[1] + lane * kPer;
 #pragma unroll
     for (int e = 0; e < kPer; e += 2)
-      if (lane * kPer + e < a.head_size)
-        *reinterpret_cast<uint32_t*>(out + lane * kPer + e) = rounded == 0.0f ? 0u : pack2(o[e] * inv, o[e + 1] * inv, bf16);
-    if (lane == 0 && a.lse != nullptr)
-      a.lse[static_cast<int64_t>(q_row) * a.heads + head] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+      if (lane * kPer + e < a.head_size) *reinterpret_cast<uint32_t*>(out + e) = rounded == 0.0f ? 0u : pack2(o[e] * inv, o[e + 1] * inv, bf16);
+    if (lane == 0 && a.lse != nullptr) a.lse[q_row * a.heads + head] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
   }
 }
 
@@ -893,6 +952,7 @@ int ixk_fmha_paged_fwd(const ixk_fmha_paged_desc* d, const ixk_paged_cache* c, c
   for (int i = 0; i < 3; ++i) a.v_strides[i] = c->v_strides[i + 1];
   a.out = static_cast<uint16_t*>(out);
   for (int i = 0; i < 2; ++i) a.o_strides[i] = d->o_strides[i];
+  a.out_sectors = (reinterpret_cast<uintptr_t>(out) & 31u) == 0 && c->head_size % 16 == 0 && d->o_strides[0] % 16 == 0 && d->o_strides[1] % 16 == 0;
   a.lse = lse;
   a.status_word = info.status_word;
   a.part_rows = scratch.part_rows;
