@@ -40,12 +40,13 @@ namespace {
 constexpr int kRows = 128;            // rows of a tile (= TMEM lanes)
 constexpr int kKeys = 64;             // keys of a unit
 constexpr int kChunkElems = 64;       // 16-bit elements of a 128-byte swizzle row
-constexpr int kThreads = 192;
+constexpr int kThreads = 192;         // 224 where V has a copy warp of its own
 constexpr int kCopyWarp = 4;
 constexpr int kMmaWarp = 5;
+constexpr int kCopyVWarp = 6;
 constexpr int kSoftmaxThreads = 128;
 constexpr int kTable = 56;            // requests whose numbers a worker holds in shared memory
-constexpr int kTileCost = 1;          // what a tile costs beside its units (Q, masks, results)
+constexpr int kTileCost = 3;          // what a tile costs beside its units (Q, masks, results)
 constexpr int kMinUnits = 2;          // shortest run: below that, joining parts costs more than it saves
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -62,6 +63,10 @@ struct Cfg {
   static constexpr int kQBytes = kChunks * kQChunkBytes;
   static constexpr int kSlotBytes = kChunks * kKvChunkBytes;
   static constexpr int kWorkers = kHeadDim <= 128 ? 2 : 1;        // on an SM
+  // A copy of a page's 64 columns costs its warp about 100 cycles: 32 a unit at head size 256 and 16-token pages, more than the
+  // 2700 that the unit's bytes take.
+  static constexpr bool kTwoCopyWarps = kHeadDim == 256;
+  static constexpr int kAllThreads = kTwoCopyWarps ? kThreads + 32 : kThreads;
   static constexpr int kSlots = kHeadDim == 64 ? 8 : 5;
   static constexpr int kTmemColumns = kHeadDim <= 128 ? 256 : 512;
   static constexpr int kTmemO = 2 * kKeys;                        // S in two buffers of 64 columns
@@ -91,7 +96,7 @@ struct Args {
   int* status_word;
   int part_rows;              // rows of a part in scratch
   int4* meta;                 // [workers] the tile that a worker began and did not finish: first row, first head, rows, parts
-  float* part_o;              // [2 * workers][part_rows][kHeadDim]
+  float* part_o;              // [2 * workers][kHeadDim / 4][part_rows][4]: a warp's rows side by side
   float4* part_stat;          // [2 * workers][part_rows]: maximum (log2), sum, sum of rounded weights
 };
 
@@ -242,21 +247,23 @@ __device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_
       : "memory");
 }
 
-// Which of keys [k0, k0 + 64) a row sees, as bits: committed ones, and drafts by its mask or, without one, up to itself.
-__device__ __forceinline__ uint64_t visible_keys(const Args& a, const Request& r, int row, int token, int k0) {
-  auto below = [](long long n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1ull; };
-  const long long committed = static_cast<long long>(r.length) - k0;
+// Which of keys [k0, k0 + 64) a row sees, as bits: committed ones, and drafts by its mask or, without one, up to itself.  Of a unit
+// with keys behind the committed ones (length - k0 < 64).  `words`: the row's mask, its first two words in m0 and m1.
+__device__ __forceinline__ uint64_t visible_keys(const Args& a, const Request& r, const int* words, uint32_t m0, uint32_t m1, int token, int k0) {
+  auto below = [](int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1ull; };
+  const int committed = r.length - k0, end = min(r.rows, a.cap - r.length) + committed;
   uint64_t bits = below(committed);
-  const long long end = min(static_cast<long long>(r.length) + r.rows, static_cast<long long>(a.cap)) - k0;
-  if (a.mask == nullptr) {
+  if (words == nullptr) {
     bits |= below(min(committed + token + 1, end));
   } else {
     // drafts d0 .. d0 + 63 stand at keys k0 .. (d0 < 0: the first of them at key k0 - d0)
-    const int* words = a.mask + row * a.mask_stride;
-    const long long d0 = -committed;
-    const long long w0 = d0 >= 0 ? d0 >> 5 : -((-d0 + 31) >> 5);
-    const int shift = static_cast<int>(d0 - (w0 << 5));
-    auto word = [&](long long w) { return w >= 0 && w < a.mask_words ? static_cast<uint32_t>(words[w]) : 0u; };
+    const int d0 = -committed;
+    const int w0 = d0 >> 5, shift = d0 & 31;       // (rounded down)
+    auto word = [&](int w) {
+      if (w == 0) return m0;
+      if (w == 1) return m1;
+      return w > 1 && w < a.mask_words ? static_cast<uint32_t>(words[w]) : 0u;
+    };
     const uint32_t x = word(w0), y = word(w0 + 1), z = word(w0 + 2);
     const uint32_t lo = __funnelshift_r(x, y, shift), hi = __funnelshift_r(y, z, shift);
     bits |= (static_cast<uint64_t>(hi) << 32 | lo) & below(end);
@@ -264,8 +271,54 @@ __device__ __forceinline__ uint64_t visible_keys(const Args& a, const Request& r
   return bits;
 }
 
+// 0 as long as all numbers were finite: each times 0, added up.
+__device__ __forceinline__ uint32_t finite_test(uint32_t acc, uint32_t w, bool bf16) {
+  if (bf16) {
+    const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w), __floats2bfloat162_rn(0.0f, 0.0f), *reinterpret_cast<const __nv_bfloat162*>(&acc));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&w), __floats2half2_rn(0.0f, 0.0f), *reinterpret_cast<const __half2*>(&acc));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// The rare case, kept out of the way: a stretch of V in shared memory with its NaN and infinities made zeros.
+__device__ __noinline__ void clear_odd_values(uint4* v, int pieces, int stride, int first, uint32_t expo) {
+  for (int i = first; i < pieces; i += stride) {
+    const uint4 w = v[i];
+    uint32_t words[4] = {w.x, w.y, w.z, w.w};
+    for (int e = 0; e < 4; ++e) {
+      if ((words[e] & expo) == expo) words[e] &= 0xffff0000u;
+      if ((words[e] >> 16 & expo) == expo) words[e] &= 0x0000ffffu;
+    }
+    v[i] = make_uint4(words[0], words[1], words[2], words[3]);
+  }
+}
+// ... and the other end of it: a row that was written without them gets the odd values of the drafts [d0, d1) that it sees, out of
+// memory again.  `out`: the row itself, or `part`: its part in scratch.
+__device__ __noinline__ void add_odd_values(const Args& a, int length, int b, int kv_head, int token, int q_row, int d0, int d1, uint16_t* out,
+                                            float* part, int64_t part_pitch) {
+  const int* words = a.mask != nullptr ? a.mask + q_row * a.mask_stride : nullptr;
+  const bool bf16 = a.is_bf16 != 0;
+  for (int d = d0; d < d1; ++d) {
+    if (words == nullptr ? d > token : (d >> 5) >= a.mask_words || !(static_cast<uint32_t>(words[d >> 5]) >> (d & 31) & 1u)) continue;
+    const int k = length + d;
+    const int page = a.table[b * a.table_stride + (k >> a.page_shift)];
+    if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.pages)) continue;
+    const uint16_t* v = a.v + page * a.v_strides[0] + (k & ((1 << a.page_shift) - 1)) * a.v_strides[1] + kv_head * a.v_strides[2];
+    for (int i = 0; i < a.head_size; ++i) {
+      const float x = bf16 ? __uint_as_float(static_cast<uint32_t>(v[i]) << 16) : __half2float(__ushort_as_half(v[i]));
+      if (fabsf(x) < INFINITY) continue;
+      if (part != nullptr) {
+        part[(i >> 2) * part_pitch + (i & 3)] += x;
+      } else {
+        const float y = bf16 ? __uint_as_float(static_cast<uint32_t>(out[i]) << 16) : __half2float(__ushort_as_half(out[i]));
+        out[i] = static_cast<uint16_t>(pack2(y + x, 0.0f, bf16) & 0xffffu);
+      }
+    }
+  }
+}
+
 template <int kHeadDim>
-__global__ void __launch_bounds__(kThreads, Cfg<kHeadDim>::kWorkers)
+__global__ void __launch_bounds__(Cfg<kHeadDim>::kAllThreads, Cfg<kHeadDim>::kWorkers)
 fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                   const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ Args args) {
   using C = Cfg<kHeadDim>;
@@ -319,10 +372,17 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   }
   ptx::grid_dependency_sync();
 
+  // (the page table on its way to L2, a line a thread: who reads which of it is not known yet)
+  {
+    const int64_t lines = ((args.requests - 1) * args.table_stride + args.columns + 31) / 32;
+    const int64_t line = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+    if (line < lines) asm volatile("prefetch.global.L2 [%0];" ::"l"(args.table + min(line * 32, (args.requests - 1) * args.table_stride + args.columns - 1)));
+  }
   // ---- the run: its length from the costs of all requests, its start from their sums
   Request mine{0, 0, 0};
   auto cost_of = [&](const Request& r) { return head_cost(args, r) * args.kv_heads; };
-  if (static_cast<int>(threadIdx.x) < args.requests) mine = load_request(args, threadIdx.x);
+  const bool scans = threadIdx.x < kThreads;
+  if (scans && static_cast<int>(threadIdx.x) < args.requests) mine = load_request(args, threadIdx.x);
   const long long my_cost = cost_of(mine);
   auto prefix = [&](long long v) {     // inclusive, in the warp; the warp's sum to `sums`
 #pragma unroll
@@ -330,16 +390,16 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       const long long up = __shfl_up_sync(0xffffffffu, v, o);
       if (lane >= o) v += up;
     }
-    if (lane == 31) sums[warp] = v;
+    if (lane == 31 && scans) sums[warp] = v;
     return v;
   };
   long long upto = prefix(my_cost);
   long long others = 0;                // of the requests behind the first kThreads
-  for (int b = threadIdx.x + kThreads; b < args.requests; b += kThreads) others += cost_of(load_request(args, b));
+  for (int b = threadIdx.x + kThreads; scans && b < args.requests; b += kThreads) others += cost_of(load_request(args, b));
   if (args.requests > kThreads) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) others += __shfl_xor_sync(0xffffffffu, others, o);
-    if (lane == 0) other_sums[warp] = others;
+    if (lane == 0 && scans) other_sums[warp] = others;
   }
   auto keep = [&](int i, const Request& r) {
     table[3 * i] = r.length;
@@ -375,7 +435,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     }
     for (int b0 = kThreads; before <= start; b0 += kThreads) {      // (the same in all threads; start < total)
       const int b = b0 + static_cast<int>(threadIdx.x);
-      const long long cost = b < args.requests ? cost_of(load_request(args, b)) : 0;
+      const long long cost = scans && b < args.requests ? cost_of(load_request(args, b)) : 0;
       __syncthreads();
       upto = prefix(cost) + before;
       __syncthreads();
@@ -402,39 +462,41 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   walk.table_count = min(kTable, args.requests - walk.table_base);
   walk.begin(args, count > 0 ? *start_request : 0, count > 0 ? *start_offset : 0, count);
 
-  if (warp == kCopyWarp) {
-    // ------------------------------------------------------------------ copies: a lane takes one page's 64 columns
+  if (warp == kCopyWarp || (C::kTwoCopyWarps && warp == kCopyVWarp)) {
+    // ------------------------------------------------------------------ copies: a page's 64 columns at a time
     const int box_keys = min(kKeys, 1 << args.page_shift);
     const int pieces = kKeys / box_keys;
     const int piece = lane / C::kChunks, chunk = lane - piece * C::kChunks;
-    const bool copies = piece < pieces;
-    uint32_t load = 0;          // place in the sequence K_0, K_1, V_0, K_2, V_1 ...
     bool alive = true;
     auto wait = [&](uint32_t bar, uint32_t parity, int site) {
       if (alive && !ptx::mbar_wait(bar, parity, ctl, site)) alive = false;
       alive = __all_sync(0xffffffffu, alive);
       return alive;
     };
-    auto load_unit = [&](const Walk& at, const CUtensorMap* map) {
+    // A unit's page numbers, a lane each.  (Pages behind the last key are not looked up: their rows are zeros, as those of a page
+    // number outside the cache.)
+    auto pages_of = [&](const Walk& at) {
+      const int k0 = at.unit * kKeys + piece * box_keys;
+      int page = args.pages;
+      if (piece < pieces && k0 < at.req.length + min(at.req.rows, args.cap - at.req.length)) {
+        page = args.table[at.b * args.table_stride + (k0 >> args.page_shift)];
+        if (static_cast<unsigned>(page) >= static_cast<unsigned>(args.pages)) page = args.pages;
+      }
+      return page;
+    };
+    // `load`: its place in the sequence K_0, K_1, V_0, K_2, V_1 ...
+    auto load_unit = [&](const Walk& at, uint32_t load, int page, const CUtensorMap* map) {
       const int slot = load % kSlots;
       if (!wait(kv_empty(slot), ((load / kSlots) & 1u) ^ 1u, kSiteLoadKV)) return;
-      ++load;
       if (lane == 0) ptx::mbar_expect_tx(kv_full(slot), C::kSlotBytes);
       __syncwarp();
-      if (copies) {
-        const int k0 = at.unit * kKeys + piece * box_keys;
-        // (pages behind the last key are not looked up: their rows are zeros, as those of a page number outside the cache)
-        int page = args.pages;
-        if (k0 < static_cast<int>(min(static_cast<long long>(at.req.length) + at.req.rows, static_cast<long long>(args.cap)))) {
-          page = args.table[at.b * args.table_stride + (k0 >> args.page_shift)];
-          if (static_cast<unsigned>(page) >= static_cast<unsigned>(args.pages)) page = args.pages;
-        }
-        ptx::tma_load_4d(kv_smem + slot * C::kSlotBytes + chunk * C::kKvChunkBytes + piece * box_keys * 128, map, kv_full(slot),
-                         chunk * kChunkElems, at.kv_head, k0 & ((1 << args.page_shift) - 1), page);
-      }
+      if (piece < pieces)
+        ptx::tma_load_4d(kv_smem + slot * C::kSlotBytes + chunk * C::kKvChunkBytes + piece * box_keys * 128, map, kv_full(slot), chunk * kChunkElems,
+                         at.kv_head, (at.unit * kKeys) & ((1 << args.page_shift) - 1), page);
     };
     Walk k_walk = walk, v_walk = walk;
-    uint32_t tiles = 0;
+    uint32_t tiles = 0, k_units = 0, v_units = 0;
+    int next_pages = 0, pages0 = 0, pages1 = 0;
     auto load_k = [&]() {
       if (k_walk.starts()) {       // a new tile: Q, once the products of the one before have read theirs
         if (!wait(q_empty, (tiles & 1u) ^ 1u, kSiteLoadQ)) return;
@@ -448,15 +510,34 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         }
         __syncwarp();
       }
-      load_unit(k_walk, &tmap_k);
+      load_unit(k_walk, k_units < 2 ? k_units : 2 * k_units - 1, next_pages, &tmap_k);
+      // (in one warp V follows K by two units at most)
+      if (k_units == v_units) pages0 = next_pages;
+      else pages1 = next_pages;
+      ++k_units;
       k_walk.next(args);
+      if (!k_walk.done()) next_pages = pages_of(k_walk);     // on its way while the ring is full
     };
-    if (!k_walk.done()) load_k();
-    while (alive && !v_walk.done()) {
-      if (!k_walk.done()) load_k();
-      if (!alive) break;
-      load_unit(v_walk, &tmap_v);
+    auto load_v = [&](int page) {
+      load_unit(v_walk, v_walk.last() ? 2 * v_units + 1 : 2 * v_units + 2, page, &tmap_v);
+      ++v_units;
       v_walk.next(args);
+    };
+    if (!walk.done()) pages0 = next_pages = pages_of(walk);
+    if (C::kTwoCopyWarps && warp == kCopyVWarp) {
+      while (alive && !v_walk.done()) {
+        load_v(pages0);
+        if (!v_walk.done()) pages0 = pages_of(v_walk);
+      }
+    } else {
+      if (!k_walk.done()) load_k();
+      while (alive && (C::kTwoCopyWarps ? !k_walk.done() : !v_walk.done())) {
+        if (!k_walk.done()) load_k();
+        if (!C::kTwoCopyWarps && alive) {
+          load_v(pages0);
+          pages0 = pages1;
+        }
+      }
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------------ products (all lanes; one elected per instruction)
@@ -541,8 +622,15 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       const bool row_ok = row_token < args.block_tokens && token < req.rows;
       const bool warp_ok = __any_sync(0xffffffffu, row_ok);
       const int q_row = req.row0 + token;
-      const int keys_end = static_cast<int>(min(static_cast<long long>(req.length) + req.rows, static_cast<long long>(args.cap)));
+      const int keys_end = req.length + min(req.rows, args.cap - req.length);
       const int first_unit = walk.unit;
+      // the row's mask, asked for long before it is needed
+      const int* words = args.mask != nullptr ? args.mask + q_row * args.mask_stride : nullptr;
+      uint32_t m0 = 0, m1 = 0;
+      if (words != nullptr && row_ok) {
+        m0 = words[0];
+        if (args.mask_words > 1) m1 = words[1];
+      }
       float m_run = -INFINITY, l_run = 0.0f, r_run = 0.0f;     // maximum, sum, sum of the rounded weights
       bool more = true;
       for (; more; ++g) {
@@ -567,7 +655,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             mult = 1.0f;
           }
           if (masked) {
-            const uint64_t bits = row_ok ? visible_keys(args, req, q_row, token, k0) : 0ull;
+            const uint64_t bits = row_ok ? visible_keys(args, req, words, m0, m1, token, k0) : 0ull;
             const uint32_t lo = static_cast<uint32_t>(bits), hi = static_cast<uint32_t>(bits >> 32);
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
@@ -640,38 +728,28 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             alive = false;
             break;
           }
-          uint4* v = reinterpret_cast<uint4*>(smem + C::kQBytes + (load % kSlots) * C::kSlotBytes);
-          const uint32_t expo = bf16 ? 0x7f80u : 0x7c00u;
-          bool odd = false;
-#pragma unroll 4
-          for (int i = row; i < kKeys * 8 * C::kChunks; i += kSoftmaxThreads) {    // (16-byte pieces; a key is 8 of them in each chunk)
-            const int key = k0 + ((i >> 3) & (kKeys - 1));
-            if (key < req.length) continue;
-            uint4 w = v[i];
-            if (key >= keys_end) {
-              w = make_uint4(0, 0, 0, 0);
-              v[i] = w;
-              continue;
-            }
-            uint32_t words[4] = {w.x, w.y, w.z, w.w};
-            bool changed = false;
+          uint4* v = reinterpret_cast<uint4*>(smem + C::kQBytes + (load % kSlots) * C::kSlotBytes);     // (16-byte pieces: a key is 8 in a chunk)
+          const int d0 = max(req.length - k0, 0), d1 = min(keys_end - k0, kKeys);
+          // (whole pages behind the last key were never copied: zeros already)
+          const int stale = (min(((keys_end - 1) >> args.page_shift << args.page_shift) + (1 << args.page_shift) - k0, kKeys) - d1) * 8;
+          const int drafts = (d1 - d0) * 8;
+          uint32_t test = 0;
+#pragma unroll 2
+          for (int i = row; i < drafts; i += kSoftmaxThreads) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if ((words[e] & expo) == expo) {
-                words[e] &= 0xffff0000u;
-                changed = true;
-              }
-              if ((words[e] >> 16 & expo) == expo) {
-                words[e] &= 0x0000ffffu;
-                changed = true;
-              }
-            }
-            if (changed) {
-              v[i] = make_uint4(words[0], words[1], words[2], words[3]);
-              odd = true;
+            for (int c = 0; c < C::kChunks; ++c) {
+              const uint4 w = v[c * kKeys * 8 + d0 * 8 + i];
+              test = finite_test(finite_test(finite_test(finite_test(test, w.x, bf16), w.y, bf16), w.z, bf16), w.w, bf16);
             }
           }
-          if (odd) odd_values[tiles % 3] = 1;
+          for (int i = row; i < stale; i += kSoftmaxThreads) {
+#pragma unroll
+            for (int c = 0; c < C::kChunks; ++c) v[c * kKeys * 8 + d1 * 8 + i] = make_uint4(0, 0, 0, 0);
+          }
+          if ((test & 0x7fff7fffu) != 0) {      // (this thread's own pieces)
+            for (int c = 0; c < C::kChunks; ++c) clear_odd_values(v + c * kKeys * 8 + d0 * 8, drafts, kSoftmaxThreads, row, bf16 ? 0x7f80u : 0x7c00u);
+            odd_values[tiles % 3] = 1;
+          }
           ptx::fence_proxy_async_smem();
         }
         more = !walk.ends();
@@ -699,59 +777,44 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       if (warp_ok) {
         const float inv_l = 1.0f / r_run;
         uint16_t* out_row = args.out + q_row * args.o_strides[0] + head * args.o_strides[1];
-        float* part_row = args.part_o + (part * args.part_rows + row) * kHeadDim;
+        float* part_row = args.part_o + (part * (kHeadDim / 4) * args.part_rows + row) * 4;
+        const int64_t part_pitch = static_cast<int64_t>(args.part_rows) * 4;
 #pragma unroll 1
-        for (int c = 0; c < kHeadDim / 32; ++c) {
-          uint32_t o[32];
-          ptx::tmem_ld_32x32(o_addr + c * 32, o);
+        for (int c0 = 0; c0 < kHeadDim; c0 += 64) {
+          uint32_t o[64];
+          ptx::tmem_ld_32x32(o_addr + c0, *reinterpret_cast<uint32_t(*)[32]>(o));
+          ptx::tmem_ld_32x32(o_addr + c0 + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
           ptx::tmem_ld_wait();
-          if (!row_ok || c * 32 >= args.head_size) continue;
-          if (odd) {
-            // the odd values of the drafts that this row sees, out of memory again
-            const int d0 = max(first_unit * kKeys - req.length, 0), d1 = min((walk.unit + 1) * kKeys, keys_end) - req.length;
-            for (int d = d0; d < d1; ++d) {
-              const int k = req.length + d;
-              if (!(visible_keys(args, req, q_row, token, k) & 1ull)) continue;
-              const int page = args.table[walk.b * args.table_stride + (k >> args.page_shift)];
-              if (static_cast<unsigned>(page) >= static_cast<unsigned>(args.pages)) continue;
-              const uint16_t* v = args.v + page * args.v_strides[0] + (k & ((1 << args.page_shift) - 1)) * args.v_strides[1] +
-                                  walk.kv_head * args.v_strides[2] + c * 32;
-#pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                if (c * 32 + i >= args.head_size) break;
-                const float x = bf16 ? __uint_as_float(static_cast<uint32_t>(v[i]) << 16) : __half2float(__ushort_as_half(v[i]));
-                if (!(fabsf(x) < INFINITY)) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
-              }
-            }
-          }
+          if (!row_ok) continue;
           if (whole) {
-            uint32_t w[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              w[i] = r_run == 0.0f ? 0u : pack2(__uint_as_float(o[2 * i]) * inv_l, __uint_as_float(o[2 * i + 1]) * inv_l, bf16);
+            for (int i = 0; i < 32; ++i)
+              o[i] = r_run == 0.0f ? 0u : pack2(__uint_as_float(o[2 * i]) * inv_l, __uint_as_float(o[2 * i + 1]) * inv_l, bf16);
             if (args.out_sectors) {
 #pragma unroll
-              for (int e = 0; e < 2; ++e)
-                if (c * 32 + e * 16 < args.head_size)
-                  store_sector(out_row + c * 32 + e * 16, {w[8 * e], w[8 * e + 1], w[8 * e + 2], w[8 * e + 3], w[8 * e + 4], w[8 * e + 5], w[8 * e + 6],
-                                                           w[8 * e + 7]});
+              for (int e = 0; e < 4; ++e)
+                if (c0 + e * 16 < args.head_size)
+                  store_sector(out_row + c0 + e * 16, {o[8 * e], o[8 * e + 1], o[8 * e + 2], o[8 * e + 3], o[8 * e + 4], o[8 * e + 5], o[8 * e + 6],
+                                                       o[8 * e + 7]});
             } else {
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (c * 32 + e * 8 < args.head_size)
-                  reinterpret_cast<uint4*>(out_row + c * 32)[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+              for (int e = 0; e < 8; ++e)
+                if (c0 + e * 8 < args.head_size)
+                  reinterpret_cast<uint4*>(out_row + c0)[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
             }
           } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              store_sector(part_row + c * 32 + e * 8, {o[8 * e], o[8 * e + 1], o[8 * e + 2], o[8 * e + 3], o[8 * e + 4], o[8 * e + 5], o[8 * e + 6],
-                                                       o[8 * e + 7]});
+            for (int e = 0; e < 16; ++e)
+              *reinterpret_cast<uint4*>(part_row + (c0 / 4 + e) * part_pitch) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           }
         }
         if (row_ok) {
           if (!whole) args.part_stat[part * args.part_rows + row] = make_float4(m_run, l_run, r_run, 0.0f);
           else if (args.lse != nullptr)
             args.lse[static_cast<int64_t>(q_row) * args.heads + head] = l_run == 0.0f ? -INFINITY : (m_run + log2f(l_run)) * kLn2;
+          if (odd)
+            add_odd_values(args, req.length, walk.b, walk.kv_head, token, q_row, max(first_unit * kKeys - req.length, 0),
+                           min(walk.end * kKeys, keys_end) - req.length, out_row, whole ? nullptr : part_row, part_pitch);
         }
       }
       ptx::tc_fence_before_sync();
@@ -770,74 +833,79 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   }
 }
 
-// Joins the parts of the tiles that several workers did: a warp a row.  With the parts' maxima m_i and sums l_i, M = max m_i:
+// Joins the parts of the tiles that several workers did.  With the parts' maxima m_i and sums l_i, M = max m_i:
 //   o = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i
-// Worker w's own part is at 2 w + 1, those of the workers behind it at 2 (w + i).
-// Bound by trips to memory: what it needs of the tile is one load, then all parts' numbers and values are asked for together,
-// four parts at a time.
-constexpr int kJoinWarps = 8;
-constexpr int kJoinParts = 4;
+// Worker w's own part is at 2 w + 1, those of the workers behind it at 2 (w + i).  A thread takes 16 columns of a row, a warp 32 rows
+// of these columns, as the parts lie in memory.  Bound by trips to memory: what it needs of the tile is one load, then
+// two parts' numbers and values at a time are asked for together.
+constexpr int kJoinRows = 32;
+constexpr int kJoinParts = 2;
 template <int kHeadDim>
-__global__ void __launch_bounds__(kJoinWarps * 32) fmha_paged_join_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kHeadDim * 2) fmha_paged_join_kernel(const __grid_constant__ Args a) {
   ptx::grid_dependency_sync();
   const int4 tile = a.meta[blockIdx.x];        // first row, first head, rows, parts
-  const int lane = threadIdx.x & 31;
+  const int row = blockIdx.y * kJoinRows + (threadIdx.x & 31), column = (threadIdx.x >> 5) * 16;
+  if (tile.w == 0 || row >= tile.z || column >= a.head_size) return;
   const bool bf16 = a.is_bf16 != 0;
-  constexpr int kPer = kHeadDim / 32;
-  for (int row = blockIdx.y * kJoinWarps + (threadIdx.x >> 5); row < tile.z; row += gridDim.y * kJoinWarps) {
-    auto part_of = [&](int i) { return (2 * (static_cast<int64_t>(blockIdx.x) + i) + (i == 0 ? 1 : 0)) * a.part_rows + row; };
-    float top = -INFINITY, sum = 0.0f, rounded = 0.0f;
-    float o[kPer];
+  const int64_t pitch = static_cast<int64_t>(a.part_rows) * 4;
+  auto part_of = [&](int i) { return 2 * (static_cast<int64_t>(blockIdx.x) + i) + (i == 0 ? 1 : 0); };
+  float top = -INFINITY, sum = 0.0f, rounded = 0.0f;
+  float o[16];
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) o[e] = 0.0f;
-    for (int i0 = 0; i0 < tile.w; i0 += kJoinParts) {
-      float4 stat[kJoinParts];
-      float2 v[kJoinParts][kPer / 2];
+  for (int e = 0; e < 16; ++e) o[e] = 0.0f;
+  for (int i0 = 0; i0 < tile.w; i0 += kJoinParts) {
+    float4 stat[kJoinParts], v[kJoinParts][4];
 #pragma unroll
-      for (int i = 0; i < kJoinParts; ++i) {
-        stat[i] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
-        if (i0 + i < tile.w) {
-          const int64_t p = part_of(i0 + i);
-          stat[i] = a.part_stat[p];
-          const float2* src = reinterpret_cast<const float2*>(a.part_o + p * kHeadDim) + lane * (kPer / 2);
+    for (int i = 0; i < kJoinParts; ++i) {
+      stat[i] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-          for (int e = 0; e < kPer / 2; ++e) v[i][e] = src[e];
-        } else {
+      for (int e = 0; e < 4; ++e) v[i][e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (i0 + i < tile.w) {
+        const int64_t p = part_of(i0 + i);
+        stat[i] = a.part_stat[p * a.part_rows + row];
+        const float* src = a.part_o + (p * (kHeadDim / 4) * a.part_rows + row) * 4;
 #pragma unroll
-          for (int e = 0; e < kPer / 2; ++e) v[i][e] = make_float2(0.0f, 0.0f);
-        }
-      }
-      float m = top;
-#pragma unroll
-      for (int i = 0; i < kJoinParts; ++i) m = fmaxf(m, stat[i].x);
-      const float use = m == -INFINITY ? 0.0f : m;
-      const float old = ptx::ex2_approx(top - use);       // (top - use: -inf, or a number)
-      top = m;
-      sum *= old;
-      rounded *= old;
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) o[e] *= old;
-#pragma unroll
-      for (int i = 0; i < kJoinParts; ++i) {
-        const float weight = ptx::ex2_approx(stat[i].x - use);      // a part that saw nothing: 0, and nothing in it
-        sum = fmaf(weight, stat[i].y, sum);
-        rounded = fmaf(weight, stat[i].z, rounded);
-#pragma unroll
-        for (int e = 0; e < kPer / 2; ++e) {
-          o[2 * e] = fmaf(weight, v[i][e].x, o[2 * e]);
-          o[2 * e + 1] = fmaf(weight, v[i][e].y, o[2 * e + 1]);
-        }
+        for (int e = 0; e < 4; ++e) v[i][e] = *reinterpret_cast<const float4*>(src + (column / 4 + e) * pitch);
       }
     }
-    const int token = row / a.group;
-    const int64_t q_row = tile.x + token, head = tile.y + row - token * a.group;
-    const float inv = 1.0f / rounded;
-    uint16_t* out = a.out + q_row * a.o_strides[0] + head * a.o_strides[1] + lane * kPer;
+    float m = top;
 #pragma unroll
-    for (int e = 0; e < kPer; e += 2)
-      if (lane * kPer + e < a.head_size) *reinterpret_cast<uint32_t*>(out + e) = rounded == 0.0f ? 0u : pack2(o[e] * inv, o[e + 1] * inv, bf16);
-    if (lane == 0 && a.lse != nullptr) a.lse[q_row * a.heads + head] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+    for (int i = 0; i < kJoinParts; ++i) m = fmaxf(m, stat[i].x);
+    const float use = m == -INFINITY ? 0.0f : m;
+    const float old = ptx::ex2_approx(top - use);       // (0 before the first part that saw anything)
+    top = m;
+    sum *= old;
+    rounded *= old;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[e] *= old;
+#pragma unroll
+    for (int i = 0; i < kJoinParts; ++i) {
+      const float weight = ptx::ex2_approx(stat[i].x - use);      // a part that saw nothing: 0, and nothing in it
+      sum = fmaf(weight, stat[i].y, sum);
+      rounded = fmaf(weight, stat[i].z, rounded);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        o[4 * e] = fmaf(weight, v[i][e].x, o[4 * e]);
+        o[4 * e + 1] = fmaf(weight, v[i][e].y, o[4 * e + 1]);
+        o[4 * e + 2] = fmaf(weight, v[i][e].z, o[4 * e + 2]);
+        o[4 * e + 3] = fmaf(weight, v[i][e].w, o[4 * e + 3]);
+      }
+    }
   }
+  const int token = row / a.group;
+  const int64_t q_row = tile.x + token, head = tile.y + row - token * a.group;
+  const float inv = 1.0f / rounded;
+  uint16_t* out = a.out + q_row * a.o_strides[0] + head * a.o_strides[1] + column;
+  uint32_t w[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = rounded == 0.0f ? 0u : pack2(o[2 * e] * inv, o[2 * e + 1] * inv, bf16);
+  if (a.out_sectors) {
+    store_sector(out, w);
+  } else {
+    reinterpret_cast<uint4*>(out)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    if (column + 8 < a.head_size) reinterpret_cast<uint4*>(out)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+  if (column == 0 && a.lse != nullptr) a.lse[q_row * a.heads + head] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
 int head_dim(int head_size) { return head_size <= 64 ? 64 : head_size <= 128 ? 128 : 256; }
@@ -882,9 +950,9 @@ int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, con
   using C = Cfg<kHeadDim>;
   IXK_CUDA_OK(cudaFuncSetAttribute(fmha_paged_kernel<kHeadDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
   const int w = workers(kHeadDim, sm_count);
-  if (int st = launch_overlapped(fmha_paged_kernel<kHeadDim>, dim3(w), dim3(kThreads), C::kSmemBytes, stream, q, k, v, a)) return st;
-  const unsigned blocks = static_cast<unsigned>(std::max(1, std::min((a.part_rows + kJoinWarps - 1) / kJoinWarps, 8)));
-  return launch_overlapped(fmha_paged_join_kernel<kHeadDim>, dim3(w, blocks), dim3(kJoinWarps * 32), 0, stream, a);
+  if (int st = launch_overlapped(fmha_paged_kernel<kHeadDim>, dim3(w), dim3(C::kAllThreads), C::kSmemBytes, stream, q, k, v, a)) return st;
+  const unsigned blocks = static_cast<unsigned>((a.part_rows + kJoinRows - 1) / kJoinRows);
+  return launch_overlapped(fmha_paged_join_kernel<kHeadDim>, dim3(w, blocks), dim3(kHeadDim * 2), 0, stream, a);
 }
 
 }  // namespace
