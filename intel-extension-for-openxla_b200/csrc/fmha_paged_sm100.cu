@@ -423,7 +423,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     for (int w = 0; w < kThreads / 32; ++w) total += other_sums[w];
   const unsigned grid = gridDim.x;
   long long run = (total >> 31) == 0 ? (static_cast<unsigned>(total) + grid - 1u) / grid : (total + grid - 1) / grid;
-  run = max(run, static_cast<long long>(kMinUnits + kTileCost));
+  run = max(run, static_cast<long long>(kMinUnits));
   const long long start = run * blockIdx.x;
   const bool aligned = (q_smem & 1023u) == 0;
   if (!aligned && threadIdx.x == 0) atomicCAS(args.status_word, 0, kSiteAlign);

@@ -1,14 +1,16 @@
 // RMSNorm of every query and key head and the position rotation in one pass, into a dense tensor or into the pages of a
 // key/value cache, and the gradient.
 //
-// A head's H elements lie in G lanes of 8 (G = 8, 16 or 32), a warp holds 32 / G heads.  With r = 1 / sqrt(mean(x^2) + eps),
-// w = gain_offset + gain and R the rotation by the token's angles:
-//   y = R (x r w).  An element's pair lies in the same lane (interleaved) or in the lane H_rot / 16 away (half-split), whose
-//   unscaled x comes by shuffle.  r is the head's, so y_i = r (a_i x_i + b_i x_pair), with a = w cos and b = -+ w_pair sin the
-//   same for all heads of a token: made once per warp.
+// A head's H elements lie in G lanes of 16 (G = 4, 8 or 16), a warp holds 32 / G heads.  A lane has two chunks of 8 that turn into
+// each other (half-split), or any two (interleaved pairs lie inside a chunk; what does not turn), so no element is needed by two
+// lanes.  With r = 1 / sqrt(mean(x^2) + eps), w = gain_offset + gain and R the rotation by the token's angles:
+//   y = R (x r w):  y_i = r (a_i x_i + b_i x_pair), with a = w cos and b = -+ w_pair sin the same for all heads of a token.
 //   backward: g~ = R^T g, h = g~ w, dx = r (h - x r^2 mean(h x)), dgain = sum of g~ x r.
-// Bound by HBM: every head read and written once (64 lanes' worth of arithmetic per 16 bytes stays under the memory's time).
 // r is made again from x in the backward pass, which reads x anyway: nothing is kept.
+//
+// Bound by HBM: every head read and written once.  A warp takes a token (or, where tokens are few, a part of its heads), a few heads a
+// lane at a time, and asks for the next ones before it computes those it has; what a token needs once (angles, slot, addresses)
+// is shared by all of its heads.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -22,9 +24,15 @@ namespace qk {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMaxBwdCtas = 148 * 4;
+constexpr int kForwardCtas = 4;       // on an SM: 128 registers a thread
+constexpr int kBackwardCtas = 3;      // 168
+constexpr int kMaxBwdCtas = 148 * kBackwardCtas;
+// Heads of a lane at a time.
+template <typename T>
+constexpr int kForwardHeads = sizeof(T) == 2 ? 2 : 1;
+constexpr int kBackwardHeads = 1;
 
 struct Args {
   int heads, kv_heads, rotary_chunks;   // 8-element chunks of a head that rotate
@@ -40,12 +48,61 @@ struct Args {
   void *qo, *ko;                        // outputs, or dq and dk
   paged::CacheArgs cache;
   const int* slots;                     // nullptr: k to ko
-  int q_segments, kv_segments, v_segments, rows_per_warp;   // forward: a warp's share of a token's heads
+  int q_segments, kv_segments, segments;     // stretches of a token's heads: queries, then keys, then values
+  int parts;                            // warps that share a token's segments
   float* partial;                       // backward: [CTA][2][256]
   int with_gains;
 };
 
-// Eight elements of a head as floats, and back with one rounding.
+// Eight elements of a head as four pairs of floats (two operations an instruction on a pair), and back with one rounding.
+struct Pairs {
+  uint64_t v[4];
+};
+__device__ __forceinline__ Pairs mul(const Pairs& a, const Pairs& b) {
+  Pairs r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.v[i] = ptx::mul2(a.v[i], b.v[i]);
+  return r;
+}
+__device__ __forceinline__ Pairs mul(const Pairs& a, float b) {
+  Pairs r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.v[i] = ptx::mul2(a.v[i], ptx::f32x2(b, b));
+  return r;
+}
+__device__ __forceinline__ Pairs fma(const Pairs& a, const Pairs& b, const Pairs& c) {
+  Pairs r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.v[i] = ptx::fma2(a.v[i], b.v[i], c.v[i]);
+  return r;
+}
+__device__ __forceinline__ Pairs fma(const Pairs& a, float b, const Pairs& c) {
+  Pairs r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.v[i] = ptx::fma2(a.v[i], ptx::f32x2(b, b), c.v[i]);
+  return r;
+}
+// The sum of the products.
+__device__ __forceinline__ float dot(const Pairs& a, const Pairs& b) {
+  uint64_t s = ptx::mul2(a.v[0], b.v[0]);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) s = ptx::fma2(a.v[i], b.v[i], s);
+  float lo, hi;
+  ptx::f32x2_split(s, lo, hi);
+  return lo + hi;
+}
+// Every element's neighbour.
+__device__ __forceinline__ Pairs swapped(const Pairs& a) {
+  Pairs r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float lo, hi;
+    ptx::f32x2_split(a.v[i], lo, hi);
+    r.v[i] = ptx::f32x2(hi, lo);
+  }
+  return r;
+}
+
 template <typename T>
 struct Vec;
 template <>
@@ -54,56 +111,47 @@ struct Vec<__nv_bfloat16> {
   __device__ __forceinline__ void load(const void* base, int64_t element) { w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + element); }
   __device__ __forceinline__ void store(void* base, int64_t element) const { *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + element) = w; }
   __device__ __forceinline__ void zero() { w = make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
+  __device__ __forceinline__ Pairs get() const {
     const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+    Pairs r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[2 * i] = __uint_as_float(words[i] << 16);
-      f[2 * i + 1] = __uint_as_float(words[i] & 0xffff0000u);
-    }
+    for (int i = 0; i < 4; ++i) r.v[i] = ptx::f32x2(__uint_as_float(words[i] << 16), __uint_as_float(words[i] & 0xffff0000u));
+    return r;
   }
-  __device__ __forceinline__ void set(const float (&f)[8]) {
+  __device__ __forceinline__ void set(const Pairs& f) {
     uint32_t words[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      float lo, hi;
+      ptx::f32x2_split(f.v[i], lo, hi);
+      const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
       words[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
     w = make_uint4(words[0], words[1], words[2], words[3]);
-  }
-  __device__ __forceinline__ Vec from_lane(int lane) const {
-    Vec v;
-    v.w.x = __shfl_sync(0xffffffffu, w.x, lane);
-    v.w.y = __shfl_sync(0xffffffffu, w.y, lane);
-    v.w.z = __shfl_sync(0xffffffffu, w.z, lane);
-    v.w.w = __shfl_sync(0xffffffffu, w.w, lane);
-    return v;
   }
 };
 template <>
 struct Vec<__half> : Vec<__nv_bfloat16> {
-  __device__ __forceinline__ void get(float (&f)[8]) const {
+  __device__ __forceinline__ Pairs get() const {
     const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+    Pairs r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&words[i]));
-      f[2 * i] = p.x;
-      f[2 * i + 1] = p.y;
+      r.v[i] = ptx::f32x2(p.x, p.y);
     }
+    return r;
   }
-  __device__ __forceinline__ void set(const float (&f)[8]) {
+  __device__ __forceinline__ void set(const Pairs& f) {
     uint32_t words[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      float lo, hi;
+      ptx::f32x2_split(f.v[i], lo, hi);
+      const __half2 h = __floats2half2_rn(lo, hi);
       words[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
     w = make_uint4(words[0], words[1], words[2], words[3]);
-  }
-  __device__ __forceinline__ Vec from_lane(int lane) const {
-    Vec v;
-    static_cast<Vec<__nv_bfloat16>&>(v) = Vec<__nv_bfloat16>::from_lane(lane);
-    return v;
   }
 };
 template <>
@@ -123,93 +171,117 @@ struct Vec<float> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = 0.0f;
   }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
+  __device__ __forceinline__ Pairs get() const {
+    Pairs r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = v[i];
-  }
-  __device__ __forceinline__ void set(const float (&f)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = f[i];
-  }
-  __device__ __forceinline__ Vec from_lane(int lane) const {
-    Vec r;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r.v[i] = __shfl_sync(0xffffffffu, v[i], lane);
+    for (int i = 0; i < 4; ++i) r.v[i] = ptx::f32x2(v[2 * i], v[2 * i + 1]);
     return r;
   }
+  __device__ __forceinline__ void set(const Pairs& f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ptx::f32x2_split(f.v[i], v[2 * i], v[2 * i + 1]);
+  }
 };
+
+// gain_offset + gain of eight columns, 1 without a gain
+template <typename T>
+__device__ __forceinline__ Pairs load_weights(const Args& a, const void* gain, int first, bool there) {
+  Pairs w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w.v[i] = ptx::f32x2(1.0f, 1.0f);
+  if (gain == nullptr || !there) return w;
+  if (a.param_fp32) {
+    Vec<float> v;
+    v.load(gain, first);
+    w = v.get();
+  } else {
+    Vec<T> v;
+    v.load(gain, first);
+    w = v.get();
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w.v[i] = ptx::add2(w.v[i], ptx::f32x2(a.gain_offset, a.gain_offset));
+  return w;
+}
+
+// A lane's place in its head: its two chunks (behind the head's last: none), and whether they turn.
+struct Place {
+  int a, b;          // first elements
+  bool has_a, has_b, turns;
+  int angles;        // of the first chunk's elements in a table row
+};
+template <int kLanes>
+__device__ __forceinline__ Place place_of(const Args& a, int lane) {
+  const int i = lane & (kLanes - 1), half = a.rotary_chunks >> 1;
+  Place p;
+  p.turns = a.interleaved ? 2 * i < a.rotary_chunks : i < half;
+  const bool across = !a.interleaved && p.turns;
+  const int first = across ? i : 2 * i, second = across ? i + half : 2 * i + 1;       // (half-split: what does not turn begins at 2 half)
+  p.a = first * 8;
+  p.b = second * 8;
+  p.has_a = first < a.head_chunks;
+  p.has_b = second < a.head_chunks;
+  p.angles = (a.interleaved ? first * 4 : first * 8);
+  return p;
+}
 
 __device__ __forceinline__ int64_t position_of(const Args& a, int64_t token) {
   if (a.positions == nullptr) return token % a.places;
   return a.wide_positions ? static_cast<const int64_t*>(a.positions)[token] : static_cast<const int*>(a.positions)[token];
 }
-
-// gain_offset + gain of a lane's eight columns (chunk < head_chunks)
-template <typename T>
-__device__ __forceinline__ void load_weights(const Args& a, const void* gain, int chunk, bool there, float (&w)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = 1.0f;
-  if (gain == nullptr || !there) return;
-  if (a.param_fp32) {
-    Vec<float> v;
-    v.load(gain, chunk * 8);
-    v.get(w);
-  } else {
-    Vec<T> v;
-    v.load(gain, chunk * 8);
-    v.get(w);
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] += a.gain_offset;
-}
-
-// A lane's place in its head and the angles of its elements.
-struct Turn {
-  bool there;        // the lane holds elements of the head
-  bool turns, second;   // they rotate; half-split: they are second of their pairs
-  int pair_lane;     // half-split: where the others are (the lane itself where nothing rotates)
-  int chunk;
+// A lane's cosines and sines: half-split, of its eight pairs; interleaved, of the four pairs of each of its chunks.  What does not
+// turn has 1 and 0.
+struct Angles {
+  float c[8], s[8];
 };
-template <int kLanes>
-__device__ __forceinline__ Turn turn_of(const Args& a, int lane) {
-  Turn t;
-  t.chunk = lane & (kLanes - 1);
-  t.there = t.chunk < a.head_chunks;
-  t.turns = t.chunk < a.rotary_chunks;
-  const int half = a.rotary_chunks >> 1;
-  t.second = !a.interleaved && t.turns && t.chunk >= half;
-  t.pair_lane = a.interleaved || !t.turns ? lane : t.second ? lane - half : lane + half;
-  return t;
-}
-// c and s of the lane's eight elements: y_i = c_i u_i + s_i u_pair(i).  (Interleaved: the pair is the neighbour.)
-__device__ __forceinline__ void load_angles(const Args& a, const Turn& t, int64_t place, float (&c)[8], float (&s)[8]) {
+template <bool kHalf>
+__device__ __forceinline__ Angles load_angles(const Args& a, const Place& p, int64_t place) {
+  Angles g;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    c[i] = 1.0f;
-    s[i] = 0.0f;
+    g.c[i] = 1.0f;
+    g.s[i] = 0.0f;
   }
-  if (!t.turns) return;
-  const int half = a.rotary_chunks >> 1;
-  if (a.interleaved) {
-    const int64_t at = (place * a.rotary_chunks + t.chunk) * 4;
-    const float4 cs = *reinterpret_cast<const float4*>(a.cos_t + at), sn = *reinterpret_cast<const float4*>(a.sin_t + at);
-    const float cv[4] = {cs.x, cs.y, cs.z, cs.w}, sv[4] = {sn.x, sn.y, sn.z, sn.w};
+  if (!p.turns) return g;
+  const float* c = a.cos_t + place * (a.rotary_chunks * 4) + p.angles;
+  const float* s = a.sin_t + place * (a.rotary_chunks * 4) + p.angles;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      c[2 * i] = c[2 * i + 1] = cv[i];
-      s[2 * i] = -sv[i];
-      s[2 * i + 1] = sv[i];
+  for (int i = 0; i < 8; i += 4) {
+    if (!kHalf && i == 4 && p.b >= a.rotary_chunks * 8) break;      // (the second chunk lies behind the last that turns)
+    const float4 cv = *reinterpret_cast<const float4*>(c + i), sv = *reinterpret_cast<const float4*>(s + i);
+    g.c[i] = cv.x, g.c[i + 1] = cv.y, g.c[i + 2] = cv.z, g.c[i + 3] = cv.w;
+    g.s[i] = sv.x, g.s[i + 1] = sv.y, g.s[i + 2] = sv.z, g.s[i + 3] = sv.w;
+  }
+  return g;
+}
+// What a lane's elements are multiplied with: y_i = c_i u_i + s_i u_pair(i).
+struct Turn {
+  Pairs ca, sa, cb, sb;
+};
+template <bool kHalf, bool kBack>
+__device__ __forceinline__ Turn turn_of(const Angles& g) {
+  Turn t;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (kHalf) {
+      const float s0 = kBack ? -g.s[2 * i] : g.s[2 * i], s1 = kBack ? -g.s[2 * i + 1] : g.s[2 * i + 1];
+      t.ca.v[i] = t.cb.v[i] = ptx::f32x2(g.c[2 * i], g.c[2 * i + 1]);
+      t.sa.v[i] = ptx::f32x2(-s0, -s1);
+      t.sb.v[i] = ptx::f32x2(s0, s1);
+    } else {
+      const float s0 = kBack ? -g.s[i] : g.s[i], s1 = kBack ? -g.s[4 + i] : g.s[4 + i];
+      t.ca.v[i] = ptx::f32x2(g.c[i], g.c[i]);
+      t.sa.v[i] = ptx::f32x2(-s0, s0);
+      t.cb.v[i] = ptx::f32x2(g.c[4 + i], g.c[4 + i]);
+      t.sb.v[i] = ptx::f32x2(-s1, s1);
     }
-  } else {
-    const int64_t at = (place * half + (t.second ? t.chunk - half : t.chunk)) * 8;
-    Vec<float> cv, sv;
-    cv.load(a.cos_t, at);
-    sv.load(a.sin_t, at);
-    cv.get(c);
-    sv.get(s);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] = t.second ? s[i] : -s[i];
   }
+  return t;
+}
+template <bool kHalf>
+__device__ __forceinline__ void turn(const Turn& t, const Pairs& xa, const Pairs& xb, Pairs* ya, Pairs* yb) {
+  *ya = fma(xa, t.ca, mul(kHalf ? xb : swapped(xa), t.sa));
+  *yb = fma(xb, t.cb, mul(kHalf ? xa : swapped(xb), t.sb));
 }
 
 template <int kLanes>
@@ -219,211 +291,218 @@ __device__ __forceinline__ float head_sum(float v) {
   return v;
 }
 
-// The elements that pair with a lane's eight.
-template <typename T>
-__device__ __forceinline__ void pairs_of(const Args& a, const Vec<T>& v, const float (&x)[8], int pair_lane, float (&p)[8]) {
-  if (a.interleaved) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = x[i ^ 1];
-  } else {
-    v.from_lane(pair_lane).get(p);
-  }
+// A warp's tokens, and which of their segments it takes.
+struct Share {
+  int64_t token, step;
+  int seg0, seg1;
+};
+__device__ __forceinline__ Share share_of(const Args& a) {
+  const unsigned warp = blockIdx.x * kWarps + (threadIdx.x >> 5), parts = a.parts;      // (a token's warps are neighbours)
+  const int part = static_cast<int>(warp % parts);
+  Share s;
+  s.step = gridDim.x * kWarps / parts;
+  s.token = warp < s.step * parts ? warp / parts : a.tokens;
+  s.seg0 = part * a.segments / a.parts;
+  s.seg1 = (part + 1) * a.segments / a.parts;
+  return s;
 }
 
-constexpr int kUnroll = 4;   // heads of a lane in flight
-
-template <typename T, int kLanes>
-__global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant__ Args a) {
-  ptx::grid_dependency_sync();
-  constexpr int kGroups = 32 / kLanes;
+// All tokens' heads of one kind: a warp walks over its tokens and their segments [seg0, seg1) of this kind, the next segment's heads
+// (the next token's, behind the last) on their way while the present ones are computed.
+enum : int { kQueries = 0, kKeys = 1, kValues = 2 };
+template <typename T, int kLanes, bool kHalf, int kKind>
+__device__ __forceinline__ void forward_kind(const Args& a, const Place& p, const Share& share, int seg0, int seg1) {
+  if (seg0 >= seg1 || share.token >= a.tokens) return;
+  constexpr int kGroups = 32 / kLanes, kHeads = kForwardHeads<T>, kRows = kGroups * kHeads;
   const int lane = threadIdx.x & 31;
-  const int segments = a.q_segments + a.kv_segments + a.v_segments;
-  const int64_t w = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  const int64_t token = w / segments;
-  if (token >= a.tokens) return;
-  int segment = static_cast<int>(w - token * segments);
-  const int64_t place = position_of(a, token);
-  if (place < 0 || place >= a.places) return;
-  const bool is_q = segment < a.q_segments;
-  const bool is_v = segment >= a.q_segments + a.kv_segments;
-  if (!is_q) segment -= is_v ? a.q_segments + a.kv_segments : a.q_segments;
-  const int heads = is_q ? a.heads : a.kv_heads;
-  const int head0 = segment * a.rows_per_warp, head1 = min(head0 + a.rows_per_warp, heads);
-  const Turn t = turn_of<kLanes>(a, lane);
-
-  const void* in = is_q ? a.q : is_v ? a.v : a.k;
-  const int64_t in_head = is_q ? a.q_strides[1] : is_v ? a.v_strides[1] : a.k_strides[1];
-  const int64_t in_at = token * (is_q ? a.q_strides[0] : is_v ? a.v_strides[0] : a.k_strides[0]) + t.chunk * 8;
-  void* out;
-  int64_t out_head, out_at;
-  if (is_q || a.slots == nullptr) {
-    out = is_q ? a.qo : a.ko;
-    out_head = is_q ? a.qo_strides[1] : a.ko_strides[1];
-    out_at = token * (is_q ? a.qo_strides[0] : a.ko_strides[0]) + t.chunk * 8;
-  } else {
-    const int slot = a.slots[token];
-    const unsigned page = static_cast<unsigned>(slot) / static_cast<unsigned>(a.cache.page_size);
-    if (slot < 0 || page >= static_cast<unsigned>(a.cache.pages)) return;
-    const int in_page = slot - static_cast<int>(page) * a.cache.page_size;
-    const paged::CacheArgs& c = a.cache;
-    out = is_v ? c.v : c.k;
-    out_head = (is_v ? c.v_head : c.k_head) * 8;
-    out_at = (is_v ? page * c.v_page + in_page * c.v_token : page * c.k_page + in_page * c.k_token) * 8 + t.chunk * 8;
-  }
-  if (is_v) {
-    for (int h0 = head0 + lane / kLanes; h0 < head1; h0 += kGroups * kUnroll) {
-      Vec<T> x[kUnroll];
+  const T* in = static_cast<const T*>(kKind == kQueries ? a.q : kKind == kKeys ? a.k : a.v);
+  const int64_t* strides = kKind == kQueries ? a.q_strides : kKind == kKeys ? a.k_strides : a.v_strides;
+  const int heads = kKind == kQueries ? a.heads : a.kv_heads;
+  const int64_t x_step = kGroups * strides[1];
+  Vec<T> xa[kHeads], xb[kHeads];
+  auto load = [&](Vec<T> (&va)[kHeads], Vec<T> (&vb)[kHeads], int64_t token, int seg) {
+    const int head = seg * kRows + lane / kLanes;
+    const T* x = in + token * strides[0] + head * strides[1];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (h0 + u * kGroups < head1 && t.there) x[u].load(in, in_at + (h0 + u * kGroups) * in_head);
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (h0 + u * kGroups < head1 && t.there) x[u].store(out, out_at + (h0 + u * kGroups) * out_head);
-    }
-    return;
-  }
-  float c[8], s[8];
-  load_angles(a, t, place, c, s);
-  {
-    float g[8], gp[8];
-    load_weights<T>(a, is_q ? a.q_gain : a.k_gain, t.chunk, t.there, g);
-    if (a.interleaved) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) gp[i] = g[i ^ 1];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) gp[i] = __shfl_sync(0xffffffffu, g[i], t.pair_lane);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      c[i] *= g[i];
-      s[i] *= gp[i];
-    }
-  }
-  for (int h0 = head0; h0 < head1; h0 += kGroups * kUnroll) {     // (uniform in the warp: shuffles)
-    const int mine = h0 + lane / kLanes;
-    Vec<T> x[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      x[u].zero();
-      if (mine + u * kGroups < head1 && t.there) x[u].load(in, in_at + (mine + u * kGroups) * in_head);
-    }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      if (h0 + u * kGroups >= head1) break;
-      float f[8], p[8];
-      x[u].get(f);
-      float sq = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sq = fmaf(f[i], f[i], sq);
-      const float r = rsqrtf(head_sum<kLanes>(sq) * a.inv_size + a.eps);
-      pairs_of<T>(a, x[u], f, t.pair_lane, p);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = r * fmaf(f[i], c[i], t.turns ? p[i] * s[i] : 0.0f);
-      if (mine + u * kGroups < head1 && t.there) {
-        x[u].set(f);
-        x[u].store(out, out_at + (mine + u * kGroups) * out_head);
-      }
-    }
-  }
-}
-
-// A CTA's warps walk the tokens; each lane sums the gains' gradients of its eight columns in registers, q's and k's apart,
-// then the CTA's lanes of the same columns are added in order and leave as one row of partial sums.
-template <typename T, int kLanes>
-__global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constant__ Args a) {
-  ptx::grid_dependency_sync();
-  constexpr int kGroups = 32 / kLanes;
-  constexpr int kUnroll = 2;
-  __shared__ float sums[kWarps * kGroups][kLanes * 8 + 4];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Turn t = turn_of<kLanes>(a, lane);
-  float acc[2][8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) acc[0][i] = acc[1][i] = 0.0f;
-  const int segments = a.q_segments + a.kv_segments;
-  const int64_t units = a.tokens * segments;
-  auto heads_of = [&](auto k_tag, int64_t token, int segment, const float (&c)[8], const float (&s)[8], bool valid) {
-    constexpr int which = decltype(k_tag)::value;
-    const void* x_in = which ? a.k : a.q;
-    const void* g_in = which ? a.gk : a.gq;
-    void* out = which ? a.ko : a.qo;
-    const int64_t* xs = which ? a.k_strides : a.q_strides;
-    const int64_t* gs = which ? a.gk_strides : a.gq_strides;
-    const int64_t* os = which ? a.ko_strides : a.qo_strides;
-    const int heads = which ? a.kv_heads : a.heads;
-    const int head0 = segment * a.rows_per_warp, head1 = min(head0 + a.rows_per_warp, heads);
-    const int64_t x_at = token * xs[0] + t.chunk * 8, g_at = token * gs[0] + t.chunk * 8, o_at = token * os[0] + t.chunk * 8;
-    float wgt[8];
-    load_weights<T>(a, which ? a.k_gain : a.q_gain, t.chunk, t.there, wgt);
-    for (int h0 = head0; h0 < head1; h0 += kGroups * kUnroll) {
-      const int mine = h0 + lane / kLanes;
-      Vec<T> x[kUnroll], g[kUnroll];
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        x[u].zero();
-        g[u].zero();
-        if (valid && mine + u * kGroups < head1 && t.there) {
-          x[u].load(x_in, x_at + (mine + u * kGroups) * xs[1]);
-          g[u].load(g_in, g_at + (mine + u * kGroups) * gs[1]);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        if (h0 + u * kGroups >= head1) break;
-        const bool mine_there = mine + u * kGroups < head1 && t.there;
-        float f[8], h[8], p[8];
-        x[u].get(f);
-        g[u].get(h);
-        pairs_of<T>(a, g[u], h, t.pair_lane, p);
-        float sq = 0.0f, hx = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          h[i] = fmaf(h[i], c[i], t.turns ? -p[i] * s[i] : 0.0f);      // turned back
-          sq = fmaf(f[i], f[i], sq);
-          hx = fmaf(h[i] * wgt[i], f[i], hx);
-        }
-        const float square = head_sum<kLanes>(sq);
-        // (0 for a row that is left out: with eps 0 its root would be infinite)
-        const float r = valid && mine + u * kGroups < head1 ? rsqrtf(square * a.inv_size + a.eps) : 0.0f;
-        const float m = head_sum<kLanes>(hx) * a.inv_size * r * r;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          acc[which][i] = fmaf(h[i] * r, f[i], acc[which][i]);
-          h[i] = r * (h[i] * wgt[i] - f[i] * m);
-        }
-        if (mine_there) {
-          g[u].set(h);
-          g[u].store(out, o_at + (mine + u * kGroups) * os[1]);
-        }
+    for (int i = 0; i < kHeads; ++i, x += x_step) {
+      va[i].zero();
+      vb[i].zero();
+      if (head + i * kGroups < heads) {
+        if (p.has_a) va[i].load(x, p.a);
+        if (p.has_b) vb[i].load(x, p.b);
       }
     }
   };
-  for (int64_t unit = static_cast<int64_t>(blockIdx.x) * kWarps + warp; unit < units; unit += static_cast<int64_t>(gridDim.x) * kWarps) {
-    const int64_t token = unit / segments;
-    const int segment = static_cast<int>(unit - token * segments);
-    const int64_t place = position_of(a, token);
+  load(xa, xb, share.token, seg0);
+  int64_t place = position_of(a, share.token);
+  for (int64_t token = share.token; token < a.tokens; token += share.step) {
+    const int64_t next_token = token + share.step;
     const bool valid = place >= 0 && place < a.places;
-    float c[8], s[8];
-    load_angles(a, t, valid ? place : 0, c, s);
-    if (segment < a.q_segments) heads_of(std::integral_constant<int, 0>{}, token, segment, c, s, valid);
-    else heads_of(std::integral_constant<int, 1>{}, token, segment - a.q_segments, c, s, valid);
-  }
-  if (!a.with_gains) return;
+    const int slot = kKind != kQueries && a.slots != nullptr ? a.slots[token] : 0;
+    Turn t;
+    if (kKind != kValues) {
+      t = turn_of<kHalf, false>(load_angles<kHalf>(a, p, valid ? place : 0));
+      const void* gain = kKind == kQueries ? a.q_gain : a.k_gain;
+      const Pairs wa = load_weights<T>(a, gain, p.a, p.has_a), wb = load_weights<T>(a, gain, p.b, p.has_b);
+      t.ca = mul(t.ca, wa);
+      t.cb = mul(t.cb, wb);
+      t.sa = mul(t.sa, kHalf ? wb : swapped(wa));
+      t.sb = mul(t.sb, kHalf ? wa : swapped(wb));
+    }
+    if (next_token < a.tokens) place = position_of(a, next_token);
+    T* y = static_cast<T*>(kKind == kQueries ? a.qo : a.ko);
+    int64_t y_head = kKind == kQueries ? a.qo_strides[1] : a.ko_strides[1], y_token = token * (kKind == kQueries ? a.qo_strides[0] : a.ko_strides[0]);
+    bool written = valid;
+    if (kKind != kQueries && a.slots != nullptr) {
+      const paged::CacheArgs& c = a.cache;
+      const unsigned page = static_cast<unsigned>(slot) / static_cast<unsigned>(c.page_size);
+      const int in_page = slot - static_cast<int>(page) * c.page_size;
+      written = valid && slot >= 0 && page < static_cast<unsigned>(c.pages);
+      y = reinterpret_cast<T*>(kKind == kKeys ? c.k : c.v);
+      y_head = (kKind == kKeys ? c.k_head : c.v_head) * 8;
+      y_token = (kKind == kKeys ? page * c.k_page + in_page * c.k_token : page * c.v_page + in_page * c.v_token) * 8;
+    }
+    int head = seg0 * kRows + lane / kLanes;
+    y += y_token + head * y_head;
+    y_head *= kGroups;
+    for (int seg = seg0; seg < seg1; ++seg, head += kRows) {
+      Vec<T> na[kHeads], nb[kHeads];
+      if (seg + 1 < seg1) load(na, nb, token, seg + 1);
+      else if (next_token < a.tokens) load(na, nb, next_token, seg0);
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    __syncthreads();
-    float* row = sums[warp * kGroups + lane / kLanes] + t.chunk * 8;
+      for (int i = 0; i < kHeads; ++i, y += y_head) {
+        if (seg * kRows + i * kGroups >= heads) break;       // (uniform in the warp: shuffles)
+        if (kKind != kValues) {
+          const Pairs fa = xa[i].get(), fb = xb[i].get();
+          const float r = rsqrtf(head_sum<kLanes>(dot(fa, fa) + dot(fb, fb)) * a.inv_size + a.eps);
+          Pairs ya, yb;
+          turn<kHalf>(t, fa, fb, &ya, &yb);
+          xa[i].set(mul(ya, r));
+          xb[i].set(mul(yb, r));
+        }
+        if (written && head + i * kGroups < heads) {
+          if (p.has_a) xa[i].store(y, p.a);
+          if (p.has_b) xb[i].store(y, p.b);
+        }
+      }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) row[i] = acc[which][i];
-    __syncthreads();
-    if (threadIdx.x < kLanes * 8) {
-      float v = 0.0f;
-#pragma unroll 4
-      for (int i = 0; i < kWarps * kGroups; ++i) v += sums[i][threadIdx.x];
-      a.partial[(static_cast<int64_t>(blockIdx.x) * 2 + which) * 256 + threadIdx.x] = v;
+      for (int i = 0; i < kHeads; ++i) xa[i] = na[i], xb[i] = nb[i];
     }
   }
+}
+template <typename T, int kLanes, bool kHalf>
+__global__ void __launch_bounds__(kThreads, kForwardCtas) forward_kernel(const __grid_constant__ Args a) {
+  ptx::grid_dependency_sync();
+  const Place p = place_of<kLanes>(a, threadIdx.x & 31);
+  const Share share = share_of(a);
+  const int first_k = a.q_segments, first_v = first_k + a.kv_segments;
+  forward_kind<T, kLanes, kHalf, kQueries>(a, p, share, share.seg0, min(share.seg1, first_k));
+  forward_kind<T, kLanes, kHalf, kKeys>(a, p, share, max(share.seg0 - first_k, 0), min(share.seg1, first_v) - first_k);
+  forward_kind<T, kLanes, kHalf, kValues>(a, p, share, max(share.seg0 - first_v, 0), share.seg1 - first_v);
+}
+
+// The same for the gradients; each lane sums the gains' gradients of its columns in registers over all tokens of its warp, then the
+// CTA's lanes of the same columns are added in order and leave as one row of partial sums.
+template <typename T, int kLanes, bool kHalf, int kKind>
+__device__ __forceinline__ void backward_kind(const Args& a, const Place& p, const Share& share, int seg0, int seg1, float (*sums)[kLanes * 16 + 4]) {
+  constexpr int kGroups = 32 / kLanes, kHeads = kBackwardHeads, kRows = kGroups * kHeads;
+  const int lane = threadIdx.x & 31;
+  Pairs acc_a, acc_b;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc_a.v[i] = acc_b.v[i] = 0;
+  if (seg0 < seg1 && share.token < a.tokens) {
+    const T* x_in = static_cast<const T*>(kKind == kQueries ? a.q : a.k);
+    const T* g_in = static_cast<const T*>(kKind == kQueries ? a.gq : a.gk);
+    T* out = static_cast<T*>(kKind == kQueries ? a.qo : a.ko);
+    const int64_t* xs = kKind == kQueries ? a.q_strides : a.k_strides;
+    const int64_t* gs = kKind == kQueries ? a.gq_strides : a.gk_strides;
+    const int64_t* os = kKind == kQueries ? a.qo_strides : a.ko_strides;
+    const int heads = kKind == kQueries ? a.heads : a.kv_heads;
+    const int64_t x_step = kGroups * xs[1], g_step = kGroups * gs[1], o_step = kGroups * os[1];
+    struct Heads {
+      Vec<T> xa, xb, ga, gb;
+    };
+    Heads now[kHeads];
+    auto load = [&](Heads (&v)[kHeads], int64_t token, int seg) {
+      const int head = seg * kRows + lane / kLanes;
+      const T* x = x_in + token * xs[0] + head * xs[1];
+      const T* g = g_in + token * gs[0] + head * gs[1];
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i, x += x_step, g += g_step) {
+        v[i].xa.zero(), v[i].xb.zero(), v[i].ga.zero(), v[i].gb.zero();
+        if (head + i * kGroups < heads) {
+          if (p.has_a) v[i].xa.load(x, p.a), v[i].ga.load(g, p.a);
+          if (p.has_b) v[i].xb.load(x, p.b), v[i].gb.load(g, p.b);
+        }
+      }
+    };
+    load(now, share.token, seg0);
+    const void* gain = kKind == kQueries ? a.q_gain : a.k_gain;
+    const Pairs wa = load_weights<T>(a, gain, p.a, p.has_a), wb = load_weights<T>(a, gain, p.b, p.has_b);
+    int64_t place = position_of(a, share.token);
+    for (int64_t token = share.token; token < a.tokens; token += share.step) {
+      const int64_t next_token = token + share.step;
+      const bool valid = place >= 0 && place < a.places;
+      const Turn t = turn_of<kHalf, true>(load_angles<kHalf>(a, p, valid ? place : 0));
+      if (next_token < a.tokens) place = position_of(a, next_token);
+      int head = seg0 * kRows + lane / kLanes;
+      T* o = out + token * os[0] + head * os[1];
+      for (int seg = seg0; seg < seg1; ++seg, head += kRows) {
+        Heads next[kHeads];
+        if (seg + 1 < seg1) load(next, token, seg + 1);
+        else if (next_token < a.tokens) load(next, next_token, seg0);
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i, o += o_step) {
+          if (seg * kRows + i * kGroups >= heads) break;                  // (uniform in the warp: shuffles)
+          const Pairs fa = now[i].xa.get(), fb = now[i].xb.get();
+          Pairs ha, hb;
+          turn<kHalf>(t, now[i].ga.get(), now[i].gb.get(), &ha, &hb);
+          const Pairs ua = mul(ha, wa), ub = mul(hb, wb);
+          const float square = head_sum<kLanes>(dot(fa, fa) + dot(fb, fb)), along = head_sum<kLanes>(dot(ua, fa) + dot(ub, fb));
+          const float r = rsqrtf(square * a.inv_size + a.eps);
+          if (head + i * kGroups >= heads) continue;
+          if (valid) {
+            const float m = -along * a.inv_size * r * r;
+            acc_a = fma(mul(ha, r), fa, acc_a);
+            acc_b = fma(mul(hb, r), fb, acc_b);
+            now[i].ga.set(mul(fma(fa, m, ua), r));
+            now[i].gb.set(mul(fma(fb, m, ub), r));
+          } else {
+            now[i].ga.zero();        // (a token that was left out, whatever it holds)
+            now[i].gb.zero();
+          }
+          if (p.has_a) now[i].ga.store(o, p.a);
+          if (p.has_b) now[i].gb.store(o, p.b);
+        }
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) now[i] = next[i];
+      }
+    }
+  }
+  if (!a.with_gains) return;
+  __syncthreads();
+  float* row = sums[(threadIdx.x >> 5) * kGroups + lane / kLanes];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (p.has_a) ptx::f32x2_split(acc_a.v[i], row[p.a + 2 * i], row[p.a + 2 * i + 1]);
+    if (p.has_b) ptx::f32x2_split(acc_b.v[i], row[p.b + 2 * i], row[p.b + 2 * i + 1]);
+  }
+  __syncthreads();
+  for (int column = threadIdx.x; column < a.head_chunks * 8; column += kThreads) {
+    float v = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < kWarps * kGroups; ++i) v += sums[i][column];
+    a.partial[(static_cast<int64_t>(blockIdx.x) * 2 + kKind) * 256 + column] = v;
+  }
+}
+template <typename T, int kLanes, bool kHalf>
+__global__ void __launch_bounds__(kThreads, kBackwardCtas) backward_kernel(const __grid_constant__ Args a) {
+  ptx::grid_dependency_sync();
+  __shared__ float sums[kWarps * (32 / kLanes)][kLanes * 16 + 4];
+  const Place p = place_of<kLanes>(a, threadIdx.x & 31);
+  const Share share = share_of(a);
+  backward_kind<T, kLanes, kHalf, kQueries>(a, p, share, share.seg0, min(share.seg1, a.q_segments), sums);
+  backward_kind<T, kLanes, kHalf, kKeys>(a, p, share, max(share.seg0 - a.q_segments, 0), share.seg1 - a.q_segments, sums);
 }
 
 // The CTAs' rows of partial sums added up: 32 columns a CTA, 32 threads a column, then a tree over them.
@@ -501,28 +580,23 @@ Args base_args(const ixk_qk_desc* d) {
   return a;
 }
 
-int lanes_for(int head_size) { return head_size <= 64 ? 8 : head_size <= 128 ? 16 : 32; }
+int lanes_for(int head_size) { return head_size <= 64 ? 4 : head_size <= 128 ? 8 : 16; }
 
-// Heads that a warp takes: four loads a lane and more where there are tokens enough to fill the GPU, fewer where not.
-void split_heads(Args* a, int lanes, int sm_count) {
-  const int groups = 32 / lanes;
-  int rows = groups * 8;
-  while (rows > groups) {
-    const int64_t warps = a->tokens * ((a->heads + rows - 1) / rows + (a->kv_heads + rows - 1) / rows);
-    if (warps >= static_cast<int64_t>(sm_count) * 32) break;
-    rows /= 2;
-  }
-  a->rows_per_warp = rows;
+// The segments of a token (of `rows` heads), and over how many warps they go: one, unless tokens are too few to fill the GPU.
+void split_heads(Args* a, int rows, bool with_v, int64_t warps) {
   a->q_segments = (a->heads + rows - 1) / rows;
   a->kv_segments = (a->kv_heads + rows - 1) / rows;
-  a->v_segments = 0;
+  a->segments = a->q_segments + a->kv_segments * (with_v ? 2 : 1);
+  a->parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(a->segments, warps / std::max<int64_t>(a->tokens, 1))));
 }
+int64_t ctas_for(const Args& a, int64_t most) { return std::max<int64_t>(1, std::min((a.tokens * a.parts + kWarps - 1) / kWarps, most)); }
+int forward_heads(int dtype) { return dtype == IXK_F32 ? kForwardHeads<float> : kForwardHeads<__half>; }
 
 template <template <typename, int> class Launcher, typename... More>
 int dispatch(int dtype, int lanes, const More&... more) {
   auto with = [&](auto tag) {
     using T = decltype(tag);
-    return lanes == 8 ? Launcher<T, 8>::run(more...) : lanes == 16 ? Launcher<T, 16>::run(more...) : Launcher<T, 32>::run(more...);
+    return lanes == 4 ? Launcher<T, 4>::run(more...) : lanes == 8 ? Launcher<T, 8>::run(more...) : Launcher<T, 16>::run(more...);
   };
   if (dtype == IXK_BF16) return with(__nv_bfloat16{});
   if (dtype == IXK_F16) return with(__half{});
@@ -530,17 +604,18 @@ int dispatch(int dtype, int lanes, const More&... more) {
 }
 template <typename T, int kLanes>
 struct Forward {
-  static int run(const Args& a, unsigned grid, cudaStream_t s) { return launch_overlapped(forward_kernel<T, kLanes>, dim3(grid), dim3(kThreads), 0, s, a); }
+  static int run(const Args& a, unsigned grid, cudaStream_t s) { 
+    return a.interleaved ? launch_overlapped(forward_kernel<T, kLanes, false>, dim3(grid), dim3(kThreads), 0, s, a)
+                         : launch_overlapped(forward_kernel<T, kLanes, true>, dim3(grid), dim3(kThreads), 0, s, a);
+  }
 };
 template <typename T, int kLanes>
 struct Backward {
-  static int run(const Args& a, unsigned grid, cudaStream_t s) { return launch_overlapped(backward_kernel<T, kLanes>, dim3(grid), dim3(kThreads), 0, s, a); }
+  static int run(const Args& a, unsigned grid, cudaStream_t s) { 
+    return a.interleaved ? launch_overlapped(backward_kernel<T, kLanes, false>, dim3(grid), dim3(kThreads), 0, s, a)
+                         : launch_overlapped(backward_kernel<T, kLanes, true>, dim3(grid), dim3(kThreads), 0, s, a);
+  }
 };
-
-int64_t backward_ctas(const Args& a) {
-  const int64_t units = a.tokens * (a.q_segments + a.kv_segments);
-  return std::max<int64_t>(1, std::min<int64_t>((units + kWarps - 1) / kWarps, kMaxBwdCtas));
-}
 
 }  // namespace
 }  // namespace qk
@@ -585,23 +660,21 @@ int ixk_qk_norm_rotary_fwd(const ixk_qk_desc* d, const void* q, const void* k, c
   a.q = q, a.k = k, a.v = v, a.q_gain = q_gain, a.k_gain = k_gain, a.cos_t = cos_table, a.sin_t = sin_table, a.positions = positions;
   a.qo = q_out, a.ko = k_out;
   const int lanes = qk::lanes_for(d->head_size);
-  qk::split_heads(&a, lanes, info.sm_count);
   if (paged) {
     a.cache = paged::cache_args(cache, k_pages, v_pages);
     a.slots = slots;
-    a.v_segments = a.kv_segments;
   }
-  const int64_t warps = a.tokens * (a.q_segments + a.kv_segments + a.v_segments);
-  const int64_t grid = (warps + qk::kWarps - 1) / qk::kWarps;
-  if (grid > 0x7fffffff) return fail(IXK_UNIMPLEMENTED, "qk_norm_rotary: too many tokens and heads");
+  const int64_t most = static_cast<int64_t>(info.sm_count) * qk::kForwardCtas;
+  qk::split_heads(&a, 32 / lanes * qk::forward_heads(d->dtype), paged, most * qk::kWarps);
+  const int64_t grid = qk::ctas_for(a, most);
   return qk::dispatch<qk::Forward>(d->dtype, lanes, a, static_cast<unsigned>(grid), static_cast<cudaStream_t>(cuda_stream));
 }
 
 size_t ixk_qk_norm_rotary_bwd_workspace_bytes(const ixk_qk_desc* d) {
   if (qk::check(d, "qk_norm_rotary") != IXK_OK) return 0;
   qk::Args a = qk::base_args(d);
-  qk::split_heads(&a, qk::lanes_for(d->head_size), 148);
-  return static_cast<size_t>(qk::backward_ctas(a)) * 2 * 256 * sizeof(float);
+  qk::split_heads(&a, 32 / qk::lanes_for(d->head_size) * qk::kBackwardHeads, false, qk::kMaxBwdCtas * qk::kWarps);
+  return static_cast<size_t>(qk::ctas_for(a, qk::kMaxBwdCtas)) * 2 * 256 * sizeof(float);
 }
 
 int ixk_qk_norm_rotary_bwd(const ixk_qk_desc* d, const void* grad_q, const void* grad_k, const void* q, const void* k, const void* q_gain,
@@ -635,8 +708,8 @@ int ixk_qk_norm_rotary_bwd(const ixk_qk_desc* d, const void* grad_q, const void*
   a.partial = static_cast<float*>(workspace);
   a.with_gains = gains;
   const int lanes = qk::lanes_for(d->head_size);
-  qk::split_heads(&a, lanes, 148);
-  const int ctas = static_cast<int>(qk::backward_ctas(a));
+  qk::split_heads(&a, 32 / lanes * qk::kBackwardHeads, false, qk::kMaxBwdCtas * qk::kWarps);
+  const int ctas = static_cast<int>(qk::ctas_for(a, qk::kMaxBwdCtas));
   auto s = static_cast<cudaStream_t>(cuda_stream);
   if (int st = qk::dispatch<qk::Backward>(d->dtype, lanes, a, static_cast<unsigned>(ctas), s)) return st;
   if (!gains) return IXK_OK;
