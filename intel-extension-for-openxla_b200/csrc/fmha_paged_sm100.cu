@@ -27,6 +27,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "paged.h"
@@ -946,9 +947,14 @@ int check(const ixk_fmha_paged_desc* d, const ixk_paged_cache* c) {
 }
 
 template <int kHeadDim>
-int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const Args& a, int sm_count, cudaStream_t stream) {
+int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const Args& a, int device, int sm_count, cudaStream_t stream) {
   using C = Cfg<kHeadDim>;
-  IXK_CUDA_OK(cudaFuncSetAttribute(fmha_paged_kernel<kHeadDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
+  static std::atomic<uint64_t> allowed{0};      // devices on which the kernel may use its shared memory
+  const uint64_t bit = 1ull << (device & 63);
+  if ((allowed.load(std::memory_order_relaxed) & bit) == 0) {
+    IXK_CUDA_OK(cudaFuncSetAttribute(fmha_paged_kernel<kHeadDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
   const int w = workers(kHeadDim, sm_count);
   if (int st = launch_overlapped(fmha_paged_kernel<kHeadDim>, dim3(w), dim3(C::kAllThreads), C::kSmemBytes, stream, q, k, v, a)) return st;
   const unsigned blocks = static_cast<unsigned>((a.part_rows + kJoinRows - 1) / kJoinRows);
@@ -1047,9 +1053,9 @@ int ixk_fmha_paged_fwd(const ixk_fmha_paged_desc* d, const ixk_paged_cache* c, c
   }
   auto s = static_cast<cudaStream_t>(cuda_stream);
   const int dim = fmha_paged::head_dim(c->head_size);
-  if (dim == 64) return fmha_paged::launch<64>(mq, mk, mv, a, info.sm_count, s);
-  if (dim == 128) return fmha_paged::launch<128>(mq, mk, mv, a, info.sm_count, s);
-  return fmha_paged::launch<256>(mq, mk, mv, a, info.sm_count, s);
+  if (dim == 64) return fmha_paged::launch<64>(mq, mk, mv, a, info.device, info.sm_count, s);
+  if (dim == 128) return fmha_paged::launch<128>(mq, mk, mv, a, info.device, info.sm_count, s);
+  return fmha_paged::launch<256>(mq, mk, mv, a, info.device, info.sm_count, s);
 }
 
 }  // extern "C"

@@ -16,7 +16,8 @@ namespace paged {
 
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 1024;        // of a block that does the sums; 256 where requests and rows are few
+constexpr int kFewThreads = 256;
 constexpr int kMaxRequests = 16384;   // 9 bytes a request in shared memory
 constexpr int kMaxPath = 1024;
 
@@ -32,7 +33,7 @@ __device__ __forceinline__ long long block_scan(long long v, long long* scratch,
   __syncthreads();          // (the scratch may still be read from the scan before)
   if (lane == 31) scratch[warp] = sum;
   __syncthreads();
-  long long w = lane < kThreads / 32 ? scratch[lane] : 0;
+  long long w = lane < static_cast<int>(blockDim.x >> 5) ? scratch[lane] : 0;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const long long up = __shfl_up_sync(0xffffffffu, w, o);
@@ -60,33 +61,40 @@ __device__ __forceinline__ int pages_for(int tokens, int page_size) {
 
 struct ExtendArgs {
   int requests, page_size, pages, columns, rows;
+  int in_place;                        // the count: the CTAs are a cluster
   int64_t table_stride;
   const int *lengths, *new_tokens, *free_pages, *free_count;
   int *page_table, *free_count_out, *granted, *row_start, *request, *position, *slot;
 };
 
-// Latency-bound: 20 bytes a request and 12 a row.  One cluster of up to eight CTAs: each makes the sums over all requests for
-// itself (a few microseconds of loads less than a second launch would cost) and writes its share of rows and pages; the
-// meeting at the end lets the count be updated in place, behind everybody's read of it.
+// Latency-bound: 20 bytes a request and 12 a row.  Every CTA makes the sums over all requests for itself (a few microseconds of loads
+// less than a second launch would cost) and writes its share of rows and pages: a row a thread.  Where the count is updated in
+// place, its CTAs are one cluster, and the update waits for all of them to have read it.
 __global__ void __launch_bounds__(kThreads) extend_kernel(const __grid_constant__ ExtendArgs a) {
   extern __shared__ int smem[];
   __shared__ long long scratch[32];
+  __shared__ int taken_max[32];
   int* start = smem;                                    // [B + 1]
   int* first = smem + a.requests + 1;                   // [B + 1]
   uint8_t* fits = reinterpret_cast<uint8_t*>(first + a.requests + 1);
   ptx::grid_dependency_sync();
-  const int B = a.requests;
-  const int per = (B + kThreads - 1) / kThreads;
+  const int B = a.requests, threads = blockDim.x;
+  const int per = (B + threads - 1) / threads;
   const int b0 = min(static_cast<int>(threadIdx.x) * per, B), b1 = min(b0 + per, B);
   const int available = min(max(*a.free_count, 0), a.pages);
 
   long long rows = 0, total;
-  for (int b = b0; b < b1; ++b) rows += max(a.new_tokens[b], 0);
+  for (int b = b0; b < b1; ++b) {
+    const int n = max(a.new_tokens[b], 0);
+    start[b] = n;
+    first[b] = a.lengths[b];
+    rows += n;
+  }
   long long row = block_scan(rows, scratch, &total);
   const int total_rows = static_cast<int>(min(total, static_cast<long long>(a.rows)));
   long long need = 0;
   for (int b = b0; b < b1; ++b) {
-    const int n = max(a.new_tokens[b], 0), L = a.lengths[b];
+    const int n = start[b], L = first[b];
     start[b] = static_cast<int>(min(row, static_cast<long long>(a.rows)));
     row += n;
     const bool ok = L >= 0 && static_cast<long long>(L) + n <= static_cast<long long>(a.columns) * a.page_size && row <= a.rows;
@@ -111,14 +119,13 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(const __grid_constant_
     first[B] = static_cast<int>(min(total, 0x7fffffffLL));
   }
   // pages taken = the largest sum that was served
-  __shared__ int taken_max[32];
   int taken = __reduce_max_sync(0xffffffffu, served_pages);
   if ((threadIdx.x & 31) == 0) taken_max[threadIdx.x >> 5] = taken;
   __syncthreads();
-  taken = __reduce_max_sync(0xffffffffu, taken_max[threadIdx.x & 31]);
+  taken = __reduce_max_sync(0xffffffffu, static_cast<int>(threadIdx.x & 31) < (threads >> 5) ? taken_max[threadIdx.x & 31] : 0);
 
-  const int stride = static_cast<int>(gridDim.x) * kThreads;
-  const int me = static_cast<int>(blockIdx.x) * kThreads + static_cast<int>(threadIdx.x);
+  const int stride = static_cast<int>(gridDim.x) * threads;
+  const int me = static_cast<int>(blockIdx.x) * threads + static_cast<int>(threadIdx.x);
   for (int b = me; b <= B; b += stride) {
     a.row_start[b] = start[b];
     if (b < B) a.granted[b] = fits[b] ? max(a.new_tokens[b], 0) : 0;
@@ -144,7 +151,7 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(const __grid_constant_
     a.position[r] = position;
     a.slot[r] = slot;
   }
-  if (gridDim.x > 1) ptx::cluster_sync_all();
+  if (a.in_place && gridDim.x > 1) ptx::cluster_sync_all();
   else __syncthreads();
   if (me == 0) *a.free_count_out = available - taken;
 }
@@ -177,13 +184,13 @@ __device__ void keep_books(const KeepArgs& a, int* smem) {
   int* first = smem;                   // [B + 1]
   int* low = smem + a.requests + 1;    // [B]
   const int B = a.requests;
-  const int per = (B + kThreads - 1) / kThreads;
+  const int threads = blockDim.x, per = (B + threads - 1) / threads;
   const int b0 = min(static_cast<int>(threadIdx.x) * per, B), b1 = min(b0 + per, B);
   const int count = min(max(*a.free_count, 0), a.pages);
   long long mine = 0, total;
   if (a.path != nullptr) {             // how much of a request's path counts: a warp each, 32 entries at a time
     const int lane = threadIdx.x & 31;
-    for (int b = threadIdx.x >> 5; b < B; b += kThreads / 32) {
+    for (int b = threadIdx.x >> 5; b < B; b += threads >> 5) {
       int L, n, kept;
       keep_range(a, b, &L, &n, &kept);
       kept = min(kept, a.path_columns);
@@ -217,7 +224,7 @@ __device__ void keep_books(const KeepArgs& a, int* smem) {
   const int back = static_cast<int>(min(total, static_cast<long long>(a.pages - count)));
   if (threadIdx.x == 0) first[B] = static_cast<int>(min(total, 0x7fffffffLL));
   __syncthreads();
-  for (int i = threadIdx.x; i < back; i += kThreads) {
+  for (int i = threadIdx.x; i < back; i += threads) {
     const int b = owner(first, B, i);
     a.free_pages[count + i] = a.page_table[b * a.table_stride + low[b] + i - first[b]];
   }
@@ -225,10 +232,11 @@ __device__ void keep_books(const KeepArgs& a, int* smem) {
 }
 
 // The moves: a thread takes one 16-byte vector of a token (a layer, K or V, a head, a place in it) and walks the path in
-// order, eight entries at a time: eight loads, then eight stores.  An entry's source is never below its target, so a
+// order, four entries at a time: four loads, then four stores.  An entry's source is never below its target, so a
 // source read in its turn, or earlier, has not been written by a target before it.
 constexpr int kMoveThreads = 256;
-constexpr int kBatch = 8;
+constexpr int kMoveCtas = 6;           // on an SM
+constexpr int kBatch = 4;
 
 __device__ __forceinline__ int slot_of(const KeepArgs& a, const int* table, long long position) {
   if (position >= static_cast<long long>(a.columns) * a.page_size) return -1;
@@ -292,10 +300,13 @@ __global__ void __launch_bounds__(kThreads) keep_books_kernel(const __grid_const
   ptx::grid_dependency_sync();
   keep_books(a, smem);
 }
-__global__ void __launch_bounds__(kMoveThreads) keep_moves_kernel(const __grid_constant__ KeepArgs a) {
+// The moves, and with_books beside them, in CTA 0, the books.  (Where the new lengths go over the old ones, which the moves read,
+// the books wait for a launch of their own.)
+__global__ void __launch_bounds__(kMoveThreads, kMoveCtas) keep_moves_kernel(const __grid_constant__ KeepArgs a, int with_books) {
   extern __shared__ int smem[];
   ptx::grid_dependency_sync();
-  keep_moves(a, smem, blockIdx.x);
+  if (with_books && blockIdx.x == 0) keep_books(a, smem);
+  else keep_moves(a, smem, static_cast<int>(blockIdx.x) - with_books);
 }
 
 int check_pool(const ixk_page_pool* p, const char* who) {
@@ -337,17 +348,24 @@ int ixk_paged_extend(const ixk_page_pool* pool, const int32_t* lengths, const in
       if (out != nullptr && out == in) return fail(IXK_INVALID_ARGUMENT, "paged_extend: an output is one of the inputs");
   DeviceInfo info;
   if (int st = get_device_info(&info)) return st;
-  paged::ExtendArgs a{pool->requests, pool->page_size, pool->pages, pool->columns, static_cast<int>(rows), pool->table_stride,
+  const bool in_place = free_count_out == free_count;
+  paged::ExtendArgs a{pool->requests, pool->page_size, pool->pages, pool->columns, static_cast<int>(rows), in_place, pool->table_stride,
                       lengths, new_tokens, free_pages, free_count, page_table, free_count_out, granted, row_start, request, position, slot};
   const size_t smem = (static_cast<size_t>(pool->requests) + 1) * 8 + pool->requests;
   if (smem > 48 * 1024)
     IXK_CUDA_OK(cudaFuncSetAttribute(paged::extend_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  // two rows a thread, up to eight CTAs
-  unsigned ctas = 1;
-  while (ctas < 8 && static_cast<int64_t>(ctas) * paged::kThreads * 2 < rows) ctas *= 2;
+  const bool few = pool->requests <= paged::kFewThreads && rows <= 2 * paged::kFewThreads;
+  const int threads = few ? paged::kFewThreads : paged::kThreads;
+  // a row a thread; in place up to a cluster of eight
+  const int64_t want = std::max<int64_t>(1, (std::max<int64_t>(rows, pool->requests) + threads - 1) / threads);
+  unsigned ctas = static_cast<unsigned>(std::min<int64_t>(want, info.sm_count));
+  if (in_place) {
+    ctas = 1;
+    while (ctas < 8 && ctas < want) ctas *= 2;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(paged::kThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = static_cast<cudaStream_t>(cuda_stream);
   cudaLaunchAttribute attr[2];
@@ -357,7 +375,7 @@ int ixk_paged_extend(const ixk_page_pool* pool, const int32_t* lengths, const in
   attr[1].val.clusterDim.x = ctas;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = ctas > 1 ? 2 : 1;
+  cfg.numAttrs = in_place && ctas > 1 ? 2 : 1;
   IXK_CUDA_OK(cudaLaunchKernelEx(&cfg, paged::extend_kernel, a));
   count_launch();
   return IXK_OK;
@@ -411,15 +429,20 @@ int ixk_paged_keep(const ixk_page_pool* pool, const int32_t* lengths, const int3
     const int64_t vecs = static_cast<int64_t>(a.vecs_per_head) * a.heads * 2 * cache->layers;
     if (vecs > 0x3fffffff) return fail(IXK_UNIMPLEMENTED, "paged_keep: too many layers and heads");
     a.vecs = static_cast<int>(vecs);
-    a.chunks = static_cast<int>(std::min<int64_t>((vecs + paged::kMoveThreads - 1) / paged::kMoveThreads, 32));
-    if (int st = launch_overlapped(paged::keep_moves_kernel, dim3(static_cast<unsigned>(a.requests) * a.chunks), dim3(paged::kMoveThreads),
-                                   static_cast<size_t>(path_columns) * 8, s, a))
+    // CTAs a request: as many as are on the GPU at one time, if there is work for them
+    const int64_t resident = static_cast<int64_t>(info.sm_count) * paged::kMoveCtas;
+    a.chunks = static_cast<int>(std::max<int64_t>(1, std::min((vecs + paged::kMoveThreads - 1) / paged::kMoveThreads, resident / a.requests)));
+    const size_t for_path = static_cast<size_t>(path_columns) * 8, for_books = (static_cast<size_t>(pool->requests) * 2 + 1) * 4;
+    const int with_books = lengths_out != lengths && pool->requests <= 1024 ? 1 : 0;
+    if (int st = launch_overlapped(paged::keep_moves_kernel, dim3(static_cast<unsigned>(a.requests) * a.chunks + with_books), dim3(paged::kMoveThreads),
+                                   with_books ? std::max(for_path, for_books) : for_path, s, a, with_books))
       return st;
+    if (with_books) return IXK_OK;
   }
   const size_t smem = (static_cast<size_t>(pool->requests) * 2 + 1) * 4;
   if (smem > 48 * 1024)
     IXK_CUDA_OK(cudaFuncSetAttribute(paged::keep_books_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  return launch_overlapped(paged::keep_books_kernel, dim3(1), dim3(paged::kThreads), smem, s, a);
+  return launch_overlapped(paged::keep_books_kernel, dim3(1), dim3(pool->requests <= paged::kFewThreads ? paged::kFewThreads : paged::kThreads), smem, s, a);
 }
 
 }  // extern "C"

@@ -659,6 +659,13 @@ IXK_PY_END
 
 // ------------------------------------------------------------------------------------------------ a paged cache
 
+// A vector of `n` elements from element `at` of a tensor's memory on.
+at::Tensor piece(const at::Tensor& whole, int64_t at, int64_t n) {
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(at);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return t;
+}
 // _require_here: given tensors are on the current device.
 bool here(std::initializer_list<const at::Tensor*> tensors) {
   const auto device = c10::cuda::current_device();
@@ -718,13 +725,17 @@ IXK_PY_FUNCTION(py_paged_extend, 9)
       !page_pool(table, lengths, pages, count, page_size, &d) || !ints(fresh, d.requests) || !here({table, lengths, fresh, pages, count}))
     Py_RETURN_NONE;
   const int64_t shapes[6] = {d.requests + 1, d.requests, rows, rows, rows, 1};
-  at::Tensor made[6];
+  at::Tensor made[6], whole;
   const at::Tensor* o[6];
   PyObject* given[6] = {nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
   if (a[7] == Py_None) {
     if (a[8] != Py_None) Py_RETURN_NONE;    // (the twin allocates in that stream's pool)
+    // six small results in one piece of memory, each from a 256-byte boundary on: six allocations would cost more than the kernel
+    int64_t at[7] = {0};
+    for (int i = 0; i < 6; ++i) at[i + 1] = at[i] + (shapes[i] + 63) / 64 * 64;
+    whole = like(*lengths, {at[6]}, at::kInt);
     for (int i = 0; i < 6; ++i) {
-      made[i] = like(*lengths, {shapes[i]}, at::kInt);
+      made[i] = piece(whole, at[i], shapes[i]);
       o[i] = &made[i];
     }
   } else {
@@ -872,8 +883,12 @@ IXK_PY_FUNCTION(py_qk_backward, 16)
     dk = &made_k;
   }
   if (!heads_view(dq, q->sizes(), q->scalar_type(), d.q_out_strides) || !heads_view(dk, k->sizes(), q->scalar_type(), d.k_out_strides)) Py_RETURN_NONE;
-  if (qg != nullptr) dqg = like(*q, qg->sizes(), qg->scalar_type());
-  if (kg != nullptr) dkg = like(*q, kg->sizes(), kg->scalar_type());
+  if (gains) {      // (both in one piece of memory, 16-byte boundaries for heads of any size)
+    const int64_t n = (q->size(2) + 7) / 8 * 8;
+    const at::Tensor both = like(*q, {2 * n}, (qg != nullptr ? qg : kg)->scalar_type());
+    if (qg != nullptr) dqg = piece(both, 0, q->size(2));
+    if (kg != nullptr) dkg = piece(both, n, q->size(2));
+  }
   if (gains && ws == nullptr) {
     scratch = like(*q, {static_cast<int64_t>(g_qk_bwd_bytes(&d))}, at::kByte);
     ws = &scratch;

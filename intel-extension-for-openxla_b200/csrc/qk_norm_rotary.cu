@@ -27,12 +27,16 @@ namespace {
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kForwardCtas = 4;       // on an SM: 128 registers a thread
-constexpr int kBackwardCtas = 3;      // 168
+constexpr int kBackwardCtas = 4;
 constexpr int kMaxBwdCtas = 148 * kBackwardCtas;
 // Heads of a lane at a time.
 template <typename T>
 constexpr int kForwardHeads = sizeof(T) == 2 ? 2 : 1;
 constexpr int kBackwardHeads = 1;
+// Segments of a warp in shared memory or on their way there.
+template <typename T>
+constexpr int kBackwardStages = sizeof(T) == 2 ? 4 : 2;
+constexpr int kForwardStages = 3;
 
 struct Args {
   int heads, kv_heads, rotary_chunks;   // 8-element chunks of a head that rotate
@@ -111,6 +115,7 @@ struct Vec<__nv_bfloat16> {
   __device__ __forceinline__ void load(const void* base, int64_t element) { w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + element); }
   __device__ __forceinline__ void store(void* base, int64_t element) const { *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + element) = w; }
   __device__ __forceinline__ void zero() { w = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void from_shared(const uint4* at) { w = at[0]; }
   __device__ __forceinline__ Pairs get() const {
     const uint32_t words[4] = {w.x, w.y, w.z, w.w};
     Pairs r;
@@ -171,6 +176,13 @@ struct Vec<float> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = 0.0f;
   }
+  __device__ __forceinline__ void from_shared(const uint4* at) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint4 w = at[i * kThreads];
+      v[4 * i] = __uint_as_float(w.x), v[4 * i + 1] = __uint_as_float(w.y), v[4 * i + 2] = __uint_as_float(w.z), v[4 * i + 3] = __uint_as_float(w.w);
+    }
+  }
   __device__ __forceinline__ Pairs get() const {
     Pairs r;
 #pragma unroll
@@ -182,6 +194,22 @@ struct Vec<float> {
     for (int i = 0; i < 4; ++i) ptx::f32x2_split(f.v[i], v[2 * i], v[2 * i + 1]);
   }
 };
+
+// Eight elements on their way to a thread's own places in shared memory (zeros where it has none): nobody else reads them, so the
+// thread's own wait is all there is to wait for.
+template <typename T>
+__device__ __forceinline__ void copy_vec(uint4* to, const T* from, bool there) {
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(to + i * kThreads)), "l"(from + (there ? i * 16 / static_cast<int>(sizeof(T)) : 0)),
+                 "r"(there ? 16 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
 
 // gain_offset + gain of eight columns, 1 without a gain
 template <typename T>
@@ -307,33 +335,43 @@ __device__ __forceinline__ Share share_of(const Args& a) {
   return s;
 }
 
-// All tokens' heads of one kind: a warp walks over its tokens and their segments [seg0, seg1) of this kind, the next segment's heads
-// (the next token's, behind the last) on their way while the present ones are computed.
+// All tokens' heads of one kind: a warp walks over its tokens and their segments [seg0, seg1) of this kind, the next segments' heads
+// (the next token's, behind the last) on their way to shared memory meanwhile.
 enum : int { kQueries = 0, kKeys = 1, kValues = 2 };
 template <typename T, int kLanes, bool kHalf, int kKind>
-__device__ __forceinline__ void forward_kind(const Args& a, const Place& p, const Share& share, int seg0, int seg1) {
+__device__ __forceinline__ void forward_kind(const Args& a, const Place& p, const Share& share, int seg0, int seg1, uint4* ring) {
   if (seg0 >= seg1 || share.token >= a.tokens) return;
   constexpr int kGroups = 32 / kLanes, kHeads = kForwardHeads<T>, kRows = kGroups * kHeads;
   const int lane = threadIdx.x & 31;
   const T* in = static_cast<const T*>(kKind == kQueries ? a.q : kKind == kKeys ? a.k : a.v);
   const int64_t* strides = kKind == kQueries ? a.q_strides : kKind == kKeys ? a.k_strides : a.v_strides;
   const int heads = kKind == kQueries ? a.heads : a.kv_heads;
-  const int64_t x_step = kGroups * strides[1];
-  Vec<T> xa[kHeads], xb[kHeads];
-  auto load = [&](Vec<T> (&va)[kHeads], Vec<T> (&vb)[kHeads], int64_t token, int seg) {
-    const int head = seg * kRows + lane / kLanes;
-    const T* x = in + token * strides[0] + head * strides[1];
+  constexpr int kVec = sizeof(T) / 2 * kThreads;        // places of eight elements
+  // the segment that is asked for next, and its stage
+  int64_t ahead_token = share.token;
+  int ahead_seg = seg0, ahead = 0;
+  auto ask = [&]() {
+    if (ahead_token < a.tokens) {
+      const int head = ahead_seg * kRows + lane / kLanes;
+      const T* x = in + ahead_token * strides[0] + head * strides[1];
+      uint4* to = ring + ahead * (2 * kHeads * kVec);
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i, x += x_step) {
-      va[i].zero();
-      vb[i].zero();
-      if (head + i * kGroups < heads) {
-        if (p.has_a) va[i].load(x, p.a);
-        if (p.has_b) vb[i].load(x, p.b);
+      for (int i = 0; i < kHeads; ++i, x += kGroups * strides[1]) {
+        const bool there = head + i * kGroups < heads;
+        copy_vec(to + (2 * i) * kVec, there && p.has_a ? x + p.a : in, there && p.has_a);
+        copy_vec(to + (2 * i + 1) * kVec, there && p.has_b ? x + p.b : in, there && p.has_b);
+      }
+      if (++ahead_seg == seg1) {
+        ahead_seg = seg0;
+        ahead_token += share.step;
       }
     }
+    copies_commit();
+    if (++ahead == kForwardStages) ahead = 0;
   };
-  load(xa, xb, share.token, seg0);
+#pragma unroll
+  for (int i = 0; i < kForwardStages - 1; ++i) ask();
+  int stage = 0;
   int64_t place = position_of(a, share.token);
   for (int64_t token = share.token; token < a.tokens; token += share.step) {
     const int64_t next_token = token + share.step;
@@ -366,9 +404,15 @@ __device__ __forceinline__ void forward_kind(const Args& a, const Place& p, cons
     y += y_token + head * y_head;
     y_head *= kGroups;
     for (int seg = seg0; seg < seg1; ++seg, head += kRows) {
-      Vec<T> na[kHeads], nb[kHeads];
-      if (seg + 1 < seg1) load(na, nb, token, seg + 1);
-      else if (next_token < a.tokens) load(na, nb, next_token, seg0);
+      copies_wait<kForwardStages - 2>();
+      Vec<T> xa[kHeads], xb[kHeads];
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i) {
+        xa[i].from_shared(ring + (stage * 2 * kHeads + 2 * i) * kVec);
+        xb[i].from_shared(ring + (stage * 2 * kHeads + 2 * i + 1) * kVec);
+      }
+      if (++stage == kForwardStages) stage = 0;
+      ask();                                                 // into the stage that the segment before this one was read from
 #pragma unroll
       for (int i = 0; i < kHeads; ++i, y += y_head) {
         if (seg * kRows + i * kGroups >= heads) break;       // (uniform in the warp: shuffles)
@@ -385,26 +429,28 @@ __device__ __forceinline__ void forward_kind(const Args& a, const Place& p, cons
           if (p.has_b) xb[i].store(y, p.b);
         }
       }
-#pragma unroll
-      for (int i = 0; i < kHeads; ++i) xa[i] = na[i], xb[i] = nb[i];
     }
   }
+  copies_wait<0>();
 }
 template <typename T, int kLanes, bool kHalf>
 __global__ void __launch_bounds__(kThreads, kForwardCtas) forward_kernel(const __grid_constant__ Args a) {
   ptx::grid_dependency_sync();
   const Place p = place_of<kLanes>(a, threadIdx.x & 31);
   const Share share = share_of(a);
+  __shared__ uint4 ring[kForwardStages * 2 * kForwardHeads<T> * (sizeof(T) / 2) * kThreads];
+  uint4* mine = ring + threadIdx.x;
   const int first_k = a.q_segments, first_v = first_k + a.kv_segments;
-  forward_kind<T, kLanes, kHalf, kQueries>(a, p, share, share.seg0, min(share.seg1, first_k));
-  forward_kind<T, kLanes, kHalf, kKeys>(a, p, share, max(share.seg0 - first_k, 0), min(share.seg1, first_v) - first_k);
-  forward_kind<T, kLanes, kHalf, kValues>(a, p, share, max(share.seg0 - first_v, 0), share.seg1 - first_v);
+  forward_kind<T, kLanes, kHalf, kQueries>(a, p, share, share.seg0, min(share.seg1, first_k), mine);
+  forward_kind<T, kLanes, kHalf, kKeys>(a, p, share, max(share.seg0 - first_k, 0), min(share.seg1, first_v) - first_k, mine);
+  forward_kind<T, kLanes, kHalf, kValues>(a, p, share, max(share.seg0 - first_v, 0), share.seg1 - first_v, mine);
 }
 
 // The same for the gradients; each lane sums the gains' gradients of its columns in registers over all tokens of its warp, then the
 // CTA's lanes of the same columns are added in order and leave as one row of partial sums.
 template <typename T, int kLanes, bool kHalf, int kKind>
-__device__ __forceinline__ void backward_kind(const Args& a, const Place& p, const Share& share, int seg0, int seg1, float (*sums)[kLanes * 16 + 4]) {
+__device__ __forceinline__ void backward_kind(const Args& a, const Place& p, const Share& share, int seg0, int seg1, uint4* ring,
+                                              float (*sums)[kLanes * 16 + 4]) {
   constexpr int kGroups = 32 / kLanes, kHeads = kBackwardHeads, kRows = kGroups * kHeads;
   const int lane = threadIdx.x & 31;
   Pairs acc_a, acc_b;
@@ -418,25 +464,38 @@ __device__ __forceinline__ void backward_kind(const Args& a, const Place& p, con
     const int64_t* gs = kKind == kQueries ? a.gq_strides : a.gk_strides;
     const int64_t* os = kKind == kQueries ? a.qo_strides : a.ko_strides;
     const int heads = kKind == kQueries ? a.heads : a.kv_heads;
-    const int64_t x_step = kGroups * xs[1], g_step = kGroups * gs[1], o_step = kGroups * os[1];
+    constexpr int kVec = sizeof(T) / 2 * kThreads, kStages = kBackwardStages<T>;
+    const int64_t o_step = kGroups * os[1];
     struct Heads {
       Vec<T> xa, xb, ga, gb;
     };
-    Heads now[kHeads];
-    auto load = [&](Heads (&v)[kHeads], int64_t token, int seg) {
-      const int head = seg * kRows + lane / kLanes;
-      const T* x = x_in + token * xs[0] + head * xs[1];
-      const T* g = g_in + token * gs[0] + head * gs[1];
+    int64_t ahead_token = share.token;
+    int ahead_seg = seg0, ahead = 0;
+    auto ask = [&]() {
+      if (ahead_token < a.tokens) {
+        const int head = ahead_seg * kRows + lane / kLanes;
+        const T* x = x_in + ahead_token * xs[0] + head * xs[1];
+        const T* g = g_in + ahead_token * gs[0] + head * gs[1];
+        uint4* to = ring + ahead * (4 * kHeads * kVec);
 #pragma unroll
-      for (int i = 0; i < kHeads; ++i, x += x_step, g += g_step) {
-        v[i].xa.zero(), v[i].xb.zero(), v[i].ga.zero(), v[i].gb.zero();
-        if (head + i * kGroups < heads) {
-          if (p.has_a) v[i].xa.load(x, p.a), v[i].ga.load(g, p.a);
-          if (p.has_b) v[i].xb.load(x, p.b), v[i].gb.load(g, p.b);
+        for (int i = 0; i < kHeads; ++i, x += kGroups * xs[1], g += kGroups * gs[1], to += 4 * kVec) {
+          const bool has_a = head + i * kGroups < heads && p.has_a, has_b = head + i * kGroups < heads && p.has_b;
+          copy_vec(to, has_a ? x + p.a : x_in, has_a);
+          copy_vec(to + kVec, has_b ? x + p.b : x_in, has_b);
+          copy_vec(to + 2 * kVec, has_a ? g + p.a : g_in, has_a);
+          copy_vec(to + 3 * kVec, has_b ? g + p.b : g_in, has_b);
+        }
+        if (++ahead_seg == seg1) {
+          ahead_seg = seg0;
+          ahead_token += share.step;
         }
       }
+      copies_commit();
+      if (++ahead == kStages) ahead = 0;
     };
-    load(now, share.token, seg0);
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) ask();
+    int stage = 0;
     const void* gain = kKind == kQueries ? a.q_gain : a.k_gain;
     const Pairs wa = load_weights<T>(a, gain, p.a, p.has_a), wb = load_weights<T>(a, gain, p.b, p.has_b);
     int64_t place = position_of(a, share.token);
@@ -448,9 +507,15 @@ __device__ __forceinline__ void backward_kind(const Args& a, const Place& p, con
       int head = seg0 * kRows + lane / kLanes;
       T* o = out + token * os[0] + head * os[1];
       for (int seg = seg0; seg < seg1; ++seg, head += kRows) {
-        Heads next[kHeads];
-        if (seg + 1 < seg1) load(next, token, seg + 1);
-        else if (next_token < a.tokens) load(next, next_token, seg0);
+        copies_wait<kStages - 2>();
+        Heads now[kHeads];
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+          const uint4* from = ring + (stage * kHeads + i) * 4 * kVec;
+          now[i].xa.from_shared(from), now[i].xb.from_shared(from + kVec), now[i].ga.from_shared(from + 2 * kVec), now[i].gb.from_shared(from + 3 * kVec);
+        }
+        if (++stage == kStages) stage = 0;
+        ask();
 #pragma unroll
         for (int i = 0; i < kHeads; ++i, o += o_step) {
           if (seg * kRows + i * kGroups >= heads) break;                  // (uniform in the warp: shuffles)
@@ -474,10 +539,9 @@ __device__ __forceinline__ void backward_kind(const Args& a, const Place& p, con
           if (p.has_a) now[i].ga.store(o, p.a);
           if (p.has_b) now[i].gb.store(o, p.b);
         }
-#pragma unroll
-        for (int i = 0; i < kHeads; ++i) now[i] = next[i];
       }
     }
+    copies_wait<0>();
   }
   if (!a.with_gains) return;
   __syncthreads();
@@ -499,10 +563,11 @@ template <typename T, int kLanes, bool kHalf>
 __global__ void __launch_bounds__(kThreads, kBackwardCtas) backward_kernel(const __grid_constant__ Args a) {
   ptx::grid_dependency_sync();
   __shared__ float sums[kWarps * (32 / kLanes)][kLanes * 16 + 4];
+  __shared__ uint4 ring[kBackwardStages<T> * 4 * kBackwardHeads * (sizeof(T) / 2) * kThreads];
   const Place p = place_of<kLanes>(a, threadIdx.x & 31);
   const Share share = share_of(a);
-  backward_kind<T, kLanes, kHalf, kQueries>(a, p, share, share.seg0, min(share.seg1, a.q_segments), sums);
-  backward_kind<T, kLanes, kHalf, kKeys>(a, p, share, max(share.seg0 - a.q_segments, 0), share.seg1 - a.q_segments, sums);
+  backward_kind<T, kLanes, kHalf, kQueries>(a, p, share, share.seg0, min(share.seg1, a.q_segments), ring + threadIdx.x, sums);
+  backward_kind<T, kLanes, kHalf, kKeys>(a, p, share, max(share.seg0 - a.q_segments, 0), share.seg1 - a.q_segments, ring + threadIdx.x, sums);
 }
 
 // The CTAs' rows of partial sums added up: 32 columns a CTA, 32 threads a column, then a tree over them.
@@ -582,7 +647,9 @@ Args base_args(const ixk_qk_desc* d) {
 
 int lanes_for(int head_size) { return head_size <= 64 ? 4 : head_size <= 128 ? 8 : 16; }
 
-// The segments of a token (of `rows` heads), and over how many warps they go: one, unless tokens are too few to fill the GPU.
+// The segments of a token (of `rows` heads), and over how many warps they go: one, unless tokens are too few to fill the GPU.  (More,
+// so that 3.46 turns of the warps become 6.92 in two parts, cost more than the idle half turn: 8192 x 32 heads of 256 forward and
+// backward 129 -> 136 us.)
 void split_heads(Args* a, int rows, bool with_v, int64_t warps) {
   a->q_segments = (a->heads + rows - 1) / rows;
   a->kv_segments = (a->kv_heads + rows - 1) / rows;
