@@ -71,7 +71,7 @@ struct ExtendArgs {
 // less than a second launch would cost) and writes its share of rows and pages: a row a thread.  Where the count is updated in
 // place, its CTAs are one cluster, and the update waits for all of them to have read it.
 __global__ void __launch_bounds__(kThreads) extend_kernel(const __grid_constant__ ExtendArgs a) {
-  extern __shared__ int smem[];
+  extern __shared__ __align__(16) int smem[];
   __shared__ long long scratch[32];
   __shared__ int taken_max[32];
   int* start = smem;                                    // [B + 1]
@@ -188,18 +188,36 @@ __device__ void keep_books(const KeepArgs& a, int* smem) {
   const int b0 = min(static_cast<int>(threadIdx.x) * per, B), b1 = min(b0 + per, B);
   const int count = min(max(*a.free_count, 0), a.pages);
   long long mine = 0, total;
-  if (a.path != nullptr) {             // how much of a request's path counts: a warp each, 32 entries at a time
-    const int lane = threadIdx.x & 31;
-    for (int b = threadIdx.x >> 5; b < B; b += threads >> 5) {
+  if (a.path != nullptr) {             // how much of a request's path counts: all entries of all requests, eight of a thread's at a time
+    for (int b = threadIdx.x; b < B; b += threads) {
       int L, n, kept;
       keep_range(a, b, &L, &n, &kept);
-      kept = min(kept, a.path_columns);
-      const int* path = a.path + b * a.path_stride;
-      for (int j = 0; j < kept; j += 32) {
-        const unsigned bad = __ballot_sync(0xffffffffu, j + lane < kept && !path_entry_ok(path, j + lane, n));
-        if (bad != 0) kept = j + __ffs(bad) - 1;
+      low[b] = min(kept, a.path_columns);
+      first[b] = n;
+    }
+    __syncthreads();
+    const int entries = B * a.path_columns;
+    for (int e0 = threadIdx.x; e0 < entries; e0 += 8 * threads) {
+      int now[8], before[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int e = e0 + i * threads;
+        now[i] = 0;
+        before[i] = -1;
+        if (e < entries) {
+          const int b = e / a.path_columns, j = e - b * a.path_columns;
+          const int* path = a.path + b * a.path_stride + j;
+          now[i] = path[0];
+          if (j > 0) before[i] = path[-1];
+        }
       }
-      if (lane == 0) low[b] = kept;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int e = e0 + i * threads;
+        if (e >= entries) break;
+        const int b = e / a.path_columns, j = e - b * a.path_columns;
+        if (now[i] >= first[b] || now[i] <= before[i]) atomicMin(&low[b], j);      // (the smallest, whoever comes first)
+      }
     }
     __syncthreads();
   }
@@ -238,12 +256,13 @@ constexpr int kMoveThreads = 256;
 constexpr int kMoveCtas = 6;           // on an SM
 constexpr int kBatch = 4;
 
-__device__ __forceinline__ int slot_of(const KeepArgs& a, const int* table, long long position) {
-  if (position >= static_cast<long long>(a.columns) * a.page_size) return -1;
-  const int place = static_cast<int>(static_cast<unsigned>(position) / static_cast<unsigned>(a.page_size));
-  const int p = table[place];
-  if (static_cast<unsigned>(p) >= static_cast<unsigned>(a.cache.pages)) return -1;
-  return p * a.page_size + static_cast<int>(position) - place * a.page_size;
+// A position's page and its place there; page -1: none.
+__device__ __forceinline__ int2 place_of(const KeepArgs& a, const int* table, long long position) {
+  if (position >= static_cast<long long>(a.columns) * a.page_size) return make_int2(-1, 0);
+  const int column = static_cast<int>(static_cast<unsigned>(position) / static_cast<unsigned>(a.page_size));
+  const int page = table[column];
+  if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.cache.pages)) return make_int2(-1, 0);
+  return make_int2(page, static_cast<int>(position) - column * a.page_size);
 }
 
 __device__ void keep_moves(const KeepArgs& a, int* smem, int block) {
@@ -255,16 +274,17 @@ __device__ void keep_moves(const KeepArgs& a, int* smem, int block) {
   if (kept <= 0) return;
   const int* path = a.path + b * a.path_stride;
   const int* table = a.page_table + b * a.table_stride;
-  int* source = smem;                  // [path_columns]; -1: nothing to move
-  int* target = smem + a.path_columns;
+  int4* moves = reinterpret_cast<int4*>(smem);       // [path_columns]: from (page, place) to (page, place); page -1: nothing moves
   if (threadIdx.x == 0) valid = kept;
   __syncthreads();
   for (int j = threadIdx.x; j < kept; j += blockDim.x) {
     if (!path_entry_ok(path, j, n)) atomicMin(&valid, j);
-    const int s = path[j] > j ? slot_of(a, table, static_cast<long long>(L) + path[j]) : -1;
-    const int t = s >= 0 ? slot_of(a, table, static_cast<long long>(L) + j) : -1;
-    source[j] = t >= 0 ? s : -1;
-    target[j] = t;
+    int2 from = make_int2(-1, 0), to = make_int2(-1, 0);
+    if (path[j] > j) {
+      from = place_of(a, table, static_cast<long long>(L) + path[j]);
+      to = place_of(a, table, static_cast<long long>(L) + j);
+    }
+    moves[j] = make_int4(to.x < 0 ? -1 : from.x, from.y, to.x, to.y);
   }
   __syncthreads();
   kept = valid;
@@ -279,31 +299,33 @@ __device__ void keep_moves(const KeepArgs& a, int* smem, int block) {
     const CacheArgs& c = a.cache;
     uint4* base = is_v ? c.v + layer * c.v_layer + head * c.v_head + in_head : c.k + layer * c.k_layer + head * c.k_head + in_head;
     const int64_t page_stride = is_v ? c.v_page : c.k_page, token_stride = is_v ? c.v_token : c.k_token;
-    auto at = [&](int slot) {
-      const unsigned p = static_cast<unsigned>(slot) / static_cast<unsigned>(a.page_size);
-      return base + p * page_stride + (slot - static_cast<int>(p) * a.page_size) * token_stride;
-    };
     for (int j0 = 0; j0 < kept; j0 += kBatch) {
       uint4 held[kBatch];
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i)
-        if (j0 + i < kept && source[j0 + i] >= 0) held[i] = *at(source[j0 + i]);
+      for (int i = 0; i < kBatch; ++i) {
+        if (j0 + i >= kept) break;
+        const int4 m = moves[j0 + i];
+        if (m.x >= 0) held[i] = base[m.x * page_stride + m.y * token_stride];
+      }
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i)
-        if (j0 + i < kept && source[j0 + i] >= 0) *at(target[j0 + i]) = held[i];
+      for (int i = 0; i < kBatch; ++i) {
+        if (j0 + i >= kept) break;
+        const int4 m = moves[j0 + i];
+        if (m.x >= 0) base[m.z * page_stride + m.w * token_stride] = held[i];
+      }
     }
   }
 }
 
 __global__ void __launch_bounds__(kThreads) keep_books_kernel(const __grid_constant__ KeepArgs a) {
-  extern __shared__ int smem[];
+  extern __shared__ __align__(16) int smem[];
   ptx::grid_dependency_sync();
   keep_books(a, smem);
 }
 // The moves, and with_books beside them, in CTA 0, the books.  (Where the new lengths go over the old ones, which the moves read,
 // the books wait for a launch of their own.)
 __global__ void __launch_bounds__(kMoveThreads, kMoveCtas) keep_moves_kernel(const __grid_constant__ KeepArgs a, int with_books) {
-  extern __shared__ int smem[];
+  extern __shared__ __align__(16) int smem[];
   ptx::grid_dependency_sync();
   if (with_books && blockIdx.x == 0) keep_books(a, smem);
   else keep_moves(a, smem, static_cast<int>(blockIdx.x) - with_books);
@@ -432,7 +454,7 @@ int ixk_paged_keep(const ixk_page_pool* pool, const int32_t* lengths, const int3
     // CTAs a request: as many as are on the GPU at one time, if there is work for them
     const int64_t resident = static_cast<int64_t>(info.sm_count) * paged::kMoveCtas;
     a.chunks = static_cast<int>(std::max<int64_t>(1, std::min((vecs + paged::kMoveThreads - 1) / paged::kMoveThreads, resident / a.requests)));
-    const size_t for_path = static_cast<size_t>(path_columns) * 8, for_books = (static_cast<size_t>(pool->requests) * 2 + 1) * 4;
+    const size_t for_path = static_cast<size_t>(path_columns) * 16, for_books = (static_cast<size_t>(pool->requests) * 2 + 1) * 4;
     const int with_books = lengths_out != lengths && pool->requests <= 1024 ? 1 : 0;
     if (int st = launch_overlapped(paged::keep_moves_kernel, dim3(static_cast<unsigned>(a.requests) * a.chunks + with_books), dim3(paged::kMoveThreads),
                                    with_books ? std::max(for_path, for_books) : for_path, s, a, with_books))
