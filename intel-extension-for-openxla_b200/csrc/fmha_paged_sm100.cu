@@ -655,13 +655,20 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             for (int i = 0; i < 64; ++i) r[i >> 5][i & 31] = __float_as_uint(__uint_as_float(r[i >> 5][i & 31]) * mult);
             mult = 1.0f;
           }
+          bool seen1 = true;        // some row of the warp sees keys of the second half
           if (masked) {
             const uint64_t bits = row_ok ? visible_keys(args, req, words, m0, m1, token, k0) : 0ull;
             const uint32_t lo = static_cast<uint32_t>(bits), hi = static_cast<uint32_t>(bits >> 32);
+            seen1 = __any_sync(0xffffffffu, hi != 0u);
+            if (!__all_sync(0xffffffffu, lo == 0xffffffffu)) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              if (!(lo >> i & 1u)) r[0][i] = 0xff800000u;
-              if (!(hi >> i & 1u)) r[1][i] = 0xff800000u;
+              for (int i = 0; i < 32; ++i)
+                if (!(lo >> i & 1u)) r[0][i] = 0xff800000u;
+            }
+            if (!__all_sync(0xffffffffu, hi == 0xffffffffu)) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!(hi >> i & 1u)) r[1][i] = 0xff800000u;
             }
           }
           float mx[8];
@@ -702,6 +709,12 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             uint32_t packed[16];
+            if (c == 1 && !seen1) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) packed[i] = 0u;
+              ptx::tmem_st_32x16(s_addr + c * 16, packed);
+              break;
+            }
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
               float x0, x1;
