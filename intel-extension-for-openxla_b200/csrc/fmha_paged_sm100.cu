@@ -29,6 +29,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "paged.h"
 #include "ptx.cuh"
@@ -83,7 +84,6 @@ struct Args {
   int rows_in;                // rows of q
   int columns, page_shift, pages;
   int cap;                    // keys that a table row can hold
-  int is_bf16;
   float scale_log2;
   int64_t table_stride, mask_stride;
   int mask_words;
@@ -199,8 +199,9 @@ struct Walk {
   }
 };
 
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, bool bf16) {
-  if (bf16) {
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (kBf16) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
@@ -213,8 +214,9 @@ __device__ __forceinline__ void store_sector(void* p, const uint32_t (&w)[8]) {
                "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
 }
-__device__ __forceinline__ float2 unpack2(uint32_t w, bool bf16) {
-  if (bf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+template <bool kBf16>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (kBf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
@@ -273,8 +275,9 @@ __device__ __forceinline__ uint64_t visible_keys(const Args& a, const Request& r
 }
 
 // 0 as long as all numbers were finite: each times 0, added up.
-__device__ __forceinline__ uint32_t finite_test(uint32_t acc, uint32_t w, bool bf16) {
-  if (bf16) {
+template <bool kBf16>
+__device__ __forceinline__ uint32_t finite_test(uint32_t acc, uint32_t w) {
+  if constexpr (kBf16) {
     const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w), __floats2bfloat162_rn(0.0f, 0.0f), *reinterpret_cast<const __nv_bfloat162*>(&acc));
     return *reinterpret_cast<const uint32_t*>(&r);
   }
@@ -295,10 +298,10 @@ __device__ __noinline__ void clear_odd_values(uint4* v, int pieces, int stride, 
 }
 // ... and the other end of it: a row that was written without them gets the odd values of the drafts [d0, d1) that it sees, out of
 // memory again.  `out`: the row itself, or `part`: its part in scratch.
+template <bool kBf16>
 __device__ __noinline__ void add_odd_values(const Args& a, int length, int b, int kv_head, int token, int q_row, int d0, int d1, uint16_t* out,
                                             float* part, int64_t part_pitch) {
   const int* words = a.mask != nullptr ? a.mask + q_row * a.mask_stride : nullptr;
-  const bool bf16 = a.is_bf16 != 0;
   for (int d = d0; d < d1; ++d) {
     if (words == nullptr ? d > token : (d >> 5) >= a.mask_words || !(static_cast<uint32_t>(words[d >> 5]) >> (d & 31) & 1u)) continue;
     const int k = length + d;
@@ -306,19 +309,18 @@ __device__ __noinline__ void add_odd_values(const Args& a, int length, int b, in
     if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.pages)) continue;
     const uint16_t* v = a.v + page * a.v_strides[0] + (k & ((1 << a.page_shift) - 1)) * a.v_strides[1] + kv_head * a.v_strides[2];
     for (int i = 0; i < a.head_size; ++i) {
-      const float x = bf16 ? __uint_as_float(static_cast<uint32_t>(v[i]) << 16) : __half2float(__ushort_as_half(v[i]));
+      const float x = unpack2<kBf16>(v[i]).x;
       if (fabsf(x) < INFINITY) continue;
       if (part != nullptr) {
         part[(i >> 2) * part_pitch + (i & 3)] += x;
       } else {
-        const float y = bf16 ? __uint_as_float(static_cast<uint32_t>(out[i]) << 16) : __half2float(__ushort_as_half(out[i]));
-        out[i] = static_cast<uint16_t>(pack2(y + x, 0.0f, bf16) & 0xffffu);
+        out[i] = static_cast<uint16_t>(pack2<kBf16>(unpack2<kBf16>(out[i]).x + x, 0.0f) & 0xffffu);
       }
     }
   }
 }
 
-template <int kHeadDim>
+template <int kHeadDim, bool kBf16>
 __global__ void __launch_bounds__(Cfg<kHeadDim>::kAllThreads, Cfg<kHeadDim>::kWorkers)
 fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                   const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ Args args) {
@@ -542,7 +544,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------------ products (all lanes; one elected per instruction)
-    const uint32_t fmt = args.is_bf16 ? 1u : 0u;
+    constexpr uint32_t fmt = kBf16 ? 1u : 0u;
     const uint32_t idesc_s = ptx::umma_idesc(fmt, fmt, 0, 0, kRows, kKeys);
     const uint32_t idesc_o = ptx::umma_idesc(fmt, fmt, 0, 1, kRows, kHeadDim);
     const uint64_t kmajor = ptx::umma_smem_desc(0, 16, 1024);
@@ -609,7 +611,6 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     }
   } else {
     // ------------------------------------------------------------------ softmax and results
-    const bool bf16 = args.is_bf16 != 0;
     const int row = warp * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(warp * 32) << 16;
     const uint32_t o_addr = tmem_base + lane_addr + C::kTmemO;
@@ -650,7 +651,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           ptx::tmem_ld_32x32(s_addr + 32, r[1]);
           ptx::tmem_ld_wait();
           float mult = args.scale_log2;
-          if (!(mult > 0.0f)) {       // (so that the maximum can be taken of r)
+          if (__builtin_expect(!(mult > 0.0f), 0)) {       // (so that the maximum can be taken of r)
 #pragma unroll
             for (int i = 0; i < 64; ++i) r[i >> 5][i & 31] = __float_as_uint(__uint_as_float(r[i >> 5][i & 31]) * mult);
             mult = 1.0f;
@@ -722,8 +723,8 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
               x0 = ptx::ex2_approx(x0);
               x1 = ptx::ex2_approx(x1);
               total2 = ptx::add2(total2, ptx::f32x2(x0, x1));
-              packed[i >> 1] = pack2(x0, x1, bf16);
-              const float2 rounded = unpack2(packed[i >> 1], bf16);
+              packed[i >> 1] = pack2<kBf16>(x0, x1);
+              const float2 rounded = unpack2<kBf16>(packed[i >> 1]);
               round2 = ptx::add2(round2, ptx::f32x2(rounded.x, rounded.y));
             }
             ptx::tmem_st_32x16(s_addr + c * 16, packed);
@@ -753,7 +754,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 #pragma unroll
             for (int c = 0; c < C::kChunks; ++c) {
               const uint4 w = v[c * kKeys * 8 + d0 * 8 + i];
-              test = finite_test(finite_test(finite_test(finite_test(test, w.x, bf16), w.y, bf16), w.z, bf16), w.w, bf16);
+              test = finite_test<kBf16>(finite_test<kBf16>(finite_test<kBf16>(finite_test<kBf16>(test, w.x), w.y), w.z), w.w);
             }
           }
           for (int i = row; i < stale; i += kSoftmaxThreads) {
@@ -761,7 +762,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             for (int c = 0; c < C::kChunks; ++c) v[c * kKeys * 8 + d1 * 8 + i] = make_uint4(0, 0, 0, 0);
           }
           if ((test & 0x7fff7fffu) != 0) {      // (this thread's own pieces)
-            for (int c = 0; c < C::kChunks; ++c) clear_odd_values(v + c * kKeys * 8 + d0 * 8, drafts, kSoftmaxThreads, row, bf16 ? 0x7f80u : 0x7c00u);
+            for (int c = 0; c < C::kChunks; ++c) clear_odd_values(v + c * kKeys * 8 + d0 * 8, drafts, kSoftmaxThreads, row, kBf16 ? 0x7f80u : 0x7c00u);
             odd_values[tiles % 3] = 1;
           }
           ptx::fence_proxy_async_smem();
@@ -803,7 +804,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           if (whole) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              o[i] = r_run == 0.0f ? 0u : pack2(__uint_as_float(o[2 * i]) * inv_l, __uint_as_float(o[2 * i + 1]) * inv_l, bf16);
+              o[i] = r_run == 0.0f ? 0u : pack2<kBf16>(__uint_as_float(o[2 * i]) * inv_l, __uint_as_float(o[2 * i + 1]) * inv_l);
             if (args.out_sectors) {
 #pragma unroll
               for (int e = 0; e < 4; ++e)
@@ -827,7 +828,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           else if (args.lse != nullptr)
             args.lse[static_cast<int64_t>(q_row) * args.heads + head] = l_run == 0.0f ? -INFINITY : (m_run + log2f(l_run)) * kLn2;
           if (odd)
-            add_odd_values(args, req.length, walk.b, walk.kv_head, token, q_row, max(first_unit * kKeys - req.length, 0),
+            add_odd_values<kBf16>(args, req.length, walk.b, walk.kv_head, token, q_row, max(first_unit * kKeys - req.length, 0),
                            min(walk.end * kKeys, keys_end) - req.length, out_row, whole ? nullptr : part_row, part_pitch);
         }
       }
@@ -854,13 +855,12 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 // two parts' numbers and values at a time are asked for together.
 constexpr int kJoinRows = 32;
 constexpr int kJoinParts = 2;
-template <int kHeadDim>
+template <int kHeadDim, bool kBf16>
 __global__ void __launch_bounds__(kHeadDim * 2) fmha_paged_join_kernel(const __grid_constant__ Args a) {
   ptx::grid_dependency_sync();
   const int4 tile = a.meta[blockIdx.x];        // first row, first head, rows, parts
   const int row = blockIdx.y * kJoinRows + (threadIdx.x & 31), column = (threadIdx.x >> 5) * 16;
   if (tile.w == 0 || row >= tile.z || column >= a.head_size) return;
-  const bool bf16 = a.is_bf16 != 0;
   const int64_t pitch = static_cast<int64_t>(a.part_rows) * 4;
   auto part_of = [&](int i) { return 2 * (static_cast<int64_t>(blockIdx.x) + i) + (i == 0 ? 1 : 0); };
   float top = -INFINITY, sum = 0.0f, rounded = 0.0f;
@@ -912,7 +912,7 @@ __global__ void __launch_bounds__(kHeadDim * 2) fmha_paged_join_kernel(const __g
   uint16_t* out = a.out + q_row * a.o_strides[0] + head * a.o_strides[1] + column;
   uint32_t w[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = rounded == 0.0f ? 0u : pack2(o[2 * e] * inv, o[2 * e + 1] * inv, bf16);
+  for (int e = 0; e < 8; ++e) w[e] = rounded == 0.0f ? 0u : pack2<kBf16>(o[2 * e] * inv, o[2 * e + 1] * inv);
   if (a.out_sectors) {
     store_sector(out, w);
   } else {
@@ -959,19 +959,19 @@ int check(const ixk_fmha_paged_desc* d, const ixk_paged_cache* c) {
   return IXK_OK;
 }
 
-template <int kHeadDim>
+template <int kHeadDim, bool kBf16>
 int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const Args& a, int device, int sm_count, cudaStream_t stream) {
   using C = Cfg<kHeadDim>;
   static std::atomic<uint64_t> allowed{0};      // devices on which the kernel may use its shared memory
   const uint64_t bit = 1ull << (device & 63);
   if ((allowed.load(std::memory_order_relaxed) & bit) == 0) {
-    IXK_CUDA_OK(cudaFuncSetAttribute(fmha_paged_kernel<kHeadDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
+    IXK_CUDA_OK(cudaFuncSetAttribute(fmha_paged_kernel<kHeadDim, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
   const int w = workers(kHeadDim, sm_count);
-  if (int st = launch_overlapped(fmha_paged_kernel<kHeadDim>, dim3(w), dim3(C::kAllThreads), C::kSmemBytes, stream, q, k, v, a)) return st;
+  if (int st = launch_overlapped(fmha_paged_kernel<kHeadDim, kBf16>, dim3(w), dim3(C::kAllThreads), C::kSmemBytes, stream, q, k, v, a)) return st;
   const unsigned blocks = static_cast<unsigned>((a.part_rows + kJoinRows - 1) / kJoinRows);
-  return launch_overlapped(fmha_paged_join_kernel<kHeadDim>, dim3(w, blocks), dim3(kHeadDim * 2), 0, stream, a);
+  return launch_overlapped(fmha_paged_join_kernel<kHeadDim, kBf16>, dim3(w, blocks), dim3(kHeadDim * 2), 0, stream, a);
 }
 
 }  // namespace
@@ -1029,7 +1029,6 @@ int ixk_fmha_paged_fwd(const ixk_fmha_paged_desc* d, const ixk_paged_cache* c, c
   a.page_shift = __builtin_ctz(static_cast<unsigned>(c->page_size));
   a.pages = c->pages;
   a.cap = d->columns * c->page_size;
-  a.is_bf16 = c->dtype == IXK_BF16;
   a.scale_log2 = d->head_scale * fmha_paged::kLog2e;
   a.table_stride = d->table_stride;
   a.mask_stride = d->mask_stride;
@@ -1048,7 +1047,7 @@ int ixk_fmha_paged_fwd(const ixk_fmha_paged_desc* d, const ixk_paged_cache* c, c
   a.part_stat = reinterpret_cast<float4*>(ws + scratch.stat);
   a.part_o = reinterpret_cast<float*>(ws + scratch.o);
 
-  const CUtensorMapDataType type = a.is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUtensorMapDataType type = c->dtype == IXK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   // (the stride of a dimension of one entry is never used: any that a map takes)
   auto bytes = [](int64_t stride, int64_t extent) { return static_cast<uint64_t>(extent > 1 ? stride * 2 : 512); };
   CUtensorMap mq, mk, mv;
@@ -1066,9 +1065,13 @@ int ixk_fmha_paged_fwd(const ixk_fmha_paged_desc* d, const ixk_paged_cache* c, c
   }
   auto s = static_cast<cudaStream_t>(cuda_stream);
   const int dim = fmha_paged::head_dim(c->head_size);
-  if (dim == 64) return fmha_paged::launch<64>(mq, mk, mv, a, info.device, info.sm_count, s);
-  if (dim == 128) return fmha_paged::launch<128>(mq, mk, mv, a, info.device, info.sm_count, s);
-  return fmha_paged::launch<256>(mq, mk, mv, a, info.device, info.sm_count, s);
+  auto with = [&](auto bf16) {
+    constexpr bool kBf16 = decltype(bf16)::value;
+    if (dim == 64) return fmha_paged::launch<64, kBf16>(mq, mk, mv, a, info.device, info.sm_count, s);
+    if (dim == 128) return fmha_paged::launch<128, kBf16>(mq, mk, mv, a, info.device, info.sm_count, s);
+    return fmha_paged::launch<256, kBf16>(mq, mk, mv, a, info.device, info.sm_count, s);
+  };
+  return c->dtype == IXK_BF16 ? with(std::true_type{}) : with(std::false_type{});
 }
 
 }  // extern "C"
