@@ -84,7 +84,8 @@ struct Args {
   int rows_in;                // rows of q
   int columns, page_shift, pages;
   int cap;                    // keys that a table row can hold
-  float scale_log2;
+  float scale_log2;           // > 0, so that the maximum can be taken of the raw products
+  int negate;                 // the scale is negative: S = -Q.K^T
   int64_t table_stride, mask_stride;
   int mask_words;
   const int *table, *lengths, *row_start, *granted, *mask;
@@ -113,6 +114,8 @@ __device__ __forceinline__ Request load_request(const Args& a, int b) {
   r.rows = start < 0 || start >= a.rows_in ? 0 : max(min(n, a.rows_in - start), 0);
   return r;
 }
+// (rarely called: kept out of the walks' code)
+__device__ __noinline__ Request far_request(const Args& a, int b) { return load_request(a, b); }
 // Keys and 64-key units of the block of tokens that starts at token t0.
 __device__ __forceinline__ int block_keys(const Args& a, const Request& r, int t0) {
   const int seen = a.mask != nullptr ? r.rows : min(r.rows, t0 + a.block_tokens);
@@ -143,7 +146,7 @@ struct Walk {
   __device__ __forceinline__ Request request(const Args& a, int i) const {
     const int k = i - table_base;
     if (k >= 0 && k < table_count) return Request{table[3 * k], table[3 * k + 1], table[3 * k + 2]};
-    return load_request(a, i);
+    return far_request(a, i);
   }
   // The tile at (b, kv_head, t0), whose first `from` costs lie before the run.
   __device__ __forceinline__ void enter(const Args& a, int from) {
@@ -545,7 +548,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------------ products (all lanes; one elected per instruction)
     constexpr uint32_t fmt = kBf16 ? 1u : 0u;
-    const uint32_t idesc_s = ptx::umma_idesc(fmt, fmt, 0, 0, kRows, kKeys);
+    const uint32_t idesc_s = ptx::umma_idesc(fmt, fmt, 0, 0, kRows, kKeys) | (args.negate ? 1u << 13 : 0u);      // (bit 13: A negated)
     const uint32_t idesc_o = ptx::umma_idesc(fmt, fmt, 0, 1, kRows, kHeadDim);
     const uint64_t kmajor = ptx::umma_smem_desc(0, 16, 1024);
     const uint64_t mnmajor = ptx::umma_smem_desc(0, C::kKvChunkBytes, 1024);
@@ -650,12 +653,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           ptx::tmem_ld_32x32(s_addr, r[0]);
           ptx::tmem_ld_32x32(s_addr + 32, r[1]);
           ptx::tmem_ld_wait();
-          float mult = args.scale_log2;
-          if (__builtin_expect(!(mult > 0.0f), 0)) {       // (so that the maximum can be taken of r)
-#pragma unroll
-            for (int i = 0; i < 64; ++i) r[i >> 5][i & 31] = __float_as_uint(__uint_as_float(r[i >> 5][i & 31]) * mult);
-            mult = 1.0f;
-          }
+          const float mult = args.scale_log2;
           bool seen1 = true;        // some row of the warp sees keys of the second half
           if (masked) {
             const uint64_t bits = row_ok ? visible_keys(args, req, words, m0, m1, token, k0) : 0ull;
@@ -749,7 +747,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           const int stale = (min(((keys_end - 1) >> args.page_shift << args.page_shift) + (1 << args.page_shift) - k0, kKeys) - d1) * 8;
           const int drafts = (d1 - d0) * 8;
           uint32_t test = 0;
-#pragma unroll 2
+#pragma unroll 1
           for (int i = row; i < drafts; i += kSoftmaxThreads) {
 #pragma unroll
             for (int c = 0; c < C::kChunks; ++c) {
@@ -757,6 +755,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
               test = finite_test<kBf16>(finite_test<kBf16>(finite_test<kBf16>(finite_test<kBf16>(test, w.x), w.y), w.z), w.w);
             }
           }
+#pragma unroll 1
           for (int i = row; i < stale; i += kSoftmaxThreads) {
 #pragma unroll
             for (int c = 0; c < C::kChunks; ++c) v[c * kKeys * 8 + d1 * 8 + i] = make_uint4(0, 0, 0, 0);
@@ -1029,7 +1028,9 @@ int ixk_fmha_paged_fwd(const ixk_fmha_paged_desc* d, const ixk_paged_cache* c, c
   a.page_shift = __builtin_ctz(static_cast<unsigned>(c->page_size));
   a.pages = c->pages;
   a.cap = d->columns * c->page_size;
-  a.scale_log2 = d->head_scale * fmha_paged::kLog2e;
+  a.negate = d->head_scale < 0.0f;
+  // (0: all weights alike; a tiny one, since masked scores are -inf)
+  a.scale_log2 = d->head_scale == 0.0f ? 1e-30f : std::fabs(d->head_scale) * fmha_paged::kLog2e;
   a.table_stride = d->table_stride;
   a.mask_stride = d->mask_stride;
   a.mask_words = d->mask_words;
