@@ -49,7 +49,7 @@ constexpr int kCopyVWarp = 6;
 constexpr int kSoftmaxThreads = 128;
 constexpr int kTable = 56;            // requests whose numbers a worker holds in shared memory
 constexpr int kTileCost = 3;          // what a tile costs beside its units (Q, masks, results)
-constexpr int kMinUnits = 2;          // shortest run: below that, joining parts costs more than it saves
+constexpr int kMinUnits = 2;          // shortest run: with one, the parts to join cost more than the second unit (5 rows, 705 keys: 11.9, 12.4 us)
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kRescaleThreshold = 8.0f;   // log2 units
@@ -97,7 +97,10 @@ struct Args {
   float* lse;
   int* status_word;
   int part_rows;              // rows of a part in scratch
-  int4* meta;                 // [workers] the tile that a worker began and did not finish: first row, first head, rows, parts
+  // Split tiles: first row, first head, rows, parts + (worker << 16).  By the worker that began it and did not finish it ([workers]; 0
+  // parts: none), or, where tiles are few, by tile ([requests][kv_heads][tile_blocks]; 0 parts: whole).
+  int4* meta;
+  int tile_blocks;            // 0: by worker
   float* part_o;              // [2 * workers][kHeadDim / 4][part_rows][4]: a warp's rows side by side
   float4* part_stat;          // [2 * workers][part_rows]: maximum (log2), sum, sum of rounded weights
 };
@@ -781,12 +784,16 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       const bool whole = first_unit == 0 && walk.end == walk.units;
       const int head = walk.kv_head * args.group + row_head;
       int64_t part = 2 * static_cast<int64_t>(blockIdx.x);
+      if (whole && args.tile_blocks != 0 && row == 0)
+        args.meta[(walk.b * args.kv_heads + walk.kv_head) * args.tile_blocks + walk.t0 / args.block_tokens] = make_int4(0, 0, 0, 0);
       if (!whole && first_unit == 0) {
         ++part;
         // (the workers behind this one have runs of `run`)
         const long long after = walk.units + kTileCost - walk.budget;
         begun = make_int4(req.row0 + walk.t0, walk.kv_head * args.group, min(args.block_tokens, req.rows - walk.t0) * args.group,
-                          static_cast<int>((after + run - 1) / run) + 1);
+                          static_cast<int>((after + run - 1) / run + 1) | static_cast<int>(blockIdx.x) << 16);
+        if (args.tile_blocks != 0 && row == 0)
+          args.meta[(walk.b * args.kv_heads + walk.kv_head) * args.tile_blocks + walk.t0 / args.block_tokens] = begun;
       }
       if (warp_ok) {
         const float inv_l = 1.0f / r_run;
@@ -835,7 +842,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       ptx::mbar_arrive(o_free);
       walk.next(args);
     }
-    if (threadIdx.x == 0) args.meta[blockIdx.x] = begun;
+    if (threadIdx.x == 0 && args.tile_blocks == 0) args.meta[blockIdx.x] = begun;
   }
 
   if (*abort_flag != 0) __nanosleep(2000000);
@@ -851,74 +858,121 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 //   o = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i
 // Worker w's own part is at 2 w + 1, those of the workers behind it at 2 (w + i).  A thread takes 16 columns of a row, a warp 32 rows
 // of these columns, as the parts lie in memory.  Bound by trips to memory: what it needs of the tile is one load, then
-// two parts' numbers and values at a time are asked for together.
+// two or four parts' numbers and values are asked for together.
 constexpr int kJoinRows = 32;
-constexpr int kJoinParts = 2;
+constexpr int kJoinWarps = 8;         // that share the parts, where there are many
+// A row's 16 columns, or what some of the parts add to them.
+struct Joined {
+  float top = -INFINITY, sum = 0.0f, rounded = 0.0f;
+  float o[16] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+};
+// Parts first, first + step, ... below `end`, kCount of them asked for together.
+template <int kHeadDim, int kCount>
+__device__ __forceinline__ void add_parts(const Args& a, int worker, int row, int column, int first, int step, int end, Joined* j) {
+  float4 stat[kCount], v[kCount][4];
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) {
+    stat[i] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[i][e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const int part = first + i * step;
+    if (part < end) {
+      const int64_t p = 2 * (static_cast<int64_t>(worker) + part) + (part == 0 ? 1 : 0);
+      stat[i] = a.part_stat[p * a.part_rows + row];
+      const float* src = a.part_o + (p * (kHeadDim / 4) * a.part_rows + row) * 4;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[i][e] = *reinterpret_cast<const float4*>(src + (column / 4 + e) * static_cast<int64_t>(a.part_rows) * 4);
+    }
+  }
+  float m = j->top;
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) m = fmaxf(m, stat[i].x);
+  const float use = m == -INFINITY ? 0.0f : m;
+  const float old = ptx::ex2_approx(j->top - use);       // (0 before the first part that saw anything)
+  j->top = m;
+  j->sum *= old;
+  j->rounded *= old;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) j->o[e] *= old;
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) {
+    const float weight = ptx::ex2_approx(stat[i].x - use);      // a part that saw nothing: 0, and nothing in it
+    j->sum = fmaf(weight, stat[i].y, j->sum);
+    j->rounded = fmaf(weight, stat[i].z, j->rounded);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      j->o[4 * e] = fmaf(weight, v[i][e].x, j->o[4 * e]);
+      j->o[4 * e + 1] = fmaf(weight, v[i][e].y, j->o[4 * e + 1]);
+      j->o[4 * e + 2] = fmaf(weight, v[i][e].z, j->o[4 * e + 2]);
+      j->o[4 * e + 3] = fmaf(weight, v[i][e].w, j->o[4 * e + 3]);
+    }
+  }
+}
 template <int kHeadDim, bool kBf16>
 __global__ void __launch_bounds__(kHeadDim * 2) fmha_paged_join_kernel(const __grid_constant__ Args a) {
   ptx::grid_dependency_sync();
-  const int4 tile = a.meta[blockIdx.x];        // first row, first head, rows, parts
+  const int4 tile = a.meta[blockIdx.x];
+  const int parts = tile.w & 0xffff;
   const int row = blockIdx.y * kJoinRows + (threadIdx.x & 31), column = (threadIdx.x >> 5) * 16;
-  if (tile.w == 0 || row >= tile.z || column >= a.head_size) return;
-  const int64_t pitch = static_cast<int64_t>(a.part_rows) * 4;
-  auto part_of = [&](int i) { return 2 * (static_cast<int64_t>(blockIdx.x) + i) + (i == 0 ? 1 : 0); };
-  float top = -INFINITY, sum = 0.0f, rounded = 0.0f;
-  float o[16];
-#pragma unroll
-  for (int e = 0; e < 16; ++e) o[e] = 0.0f;
-  for (int i0 = 0; i0 < tile.w; i0 += kJoinParts) {
-    float4 stat[kJoinParts], v[kJoinParts][4];
-#pragma unroll
-    for (int i = 0; i < kJoinParts; ++i) {
-      stat[i] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[i][e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (i0 + i < tile.w) {
-        const int64_t p = part_of(i0 + i);
-        stat[i] = a.part_stat[p * a.part_rows + row];
-        const float* src = a.part_o + (p * (kHeadDim / 4) * a.part_rows + row) * 4;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[i][e] = *reinterpret_cast<const float4*>(src + (column / 4 + e) * pitch);
-      }
-    }
-    float m = top;
-#pragma unroll
-    for (int i = 0; i < kJoinParts; ++i) m = fmaxf(m, stat[i].x);
-    const float use = m == -INFINITY ? 0.0f : m;
-    const float old = ptx::ex2_approx(top - use);       // (0 before the first part that saw anything)
-    top = m;
-    sum *= old;
-    rounded *= old;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) o[e] *= old;
-#pragma unroll
-    for (int i = 0; i < kJoinParts; ++i) {
-      const float weight = ptx::ex2_approx(stat[i].x - use);      // a part that saw nothing: 0, and nothing in it
-      sum = fmaf(weight, stat[i].y, sum);
-      rounded = fmaf(weight, stat[i].z, rounded);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        o[4 * e] = fmaf(weight, v[i][e].x, o[4 * e]);
-        o[4 * e + 1] = fmaf(weight, v[i][e].y, o[4 * e + 1]);
-        o[4 * e + 2] = fmaf(weight, v[i][e].z, o[4 * e + 2]);
-        o[4 * e + 3] = fmaf(weight, v[i][e].w, o[4 * e + 3]);
-      }
-    }
-  }
+  if (parts == 0 || row >= tile.z || column >= a.head_size) return;
+  Joined j;
+  for (int i0 = 0; i0 < parts; i0 += 2) add_parts<kHeadDim, 2>(a, blockIdx.x, row, column, i0, 1, parts, &j);
   const int token = row / a.group;
   const int64_t q_row = tile.x + token, head = tile.y + row - token * a.group;
-  const float inv = 1.0f / rounded;
+  const float inv = 1.0f / j.rounded;
   uint16_t* out = a.out + q_row * a.o_strides[0] + head * a.o_strides[1] + column;
   uint32_t w[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = rounded == 0.0f ? 0u : pack2<kBf16>(o[2 * e] * inv, o[2 * e + 1] * inv);
+  for (int e = 0; e < 8; ++e) w[e] = j.rounded == 0.0f ? 0u : pack2<kBf16>(j.o[2 * e] * inv, j.o[2 * e + 1] * inv);
   if (a.out_sectors) {
     store_sector(out, w);
   } else {
     reinterpret_cast<uint4*>(out)[0] = make_uint4(w[0], w[1], w[2], w[3]);
     if (column + 8 < a.head_size) reinterpret_cast<uint4*>(out)[1] = make_uint4(w[4], w[5], w[6], w[7]);
   }
-  if (column == 0 && a.lse != nullptr) a.lse[q_row * a.heads + head] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+  if (column == 0 && a.lse != nullptr) a.lse[q_row * a.heads + head] = j.sum == 0.0f ? -INFINITY : (j.top + log2f(j.sum)) * kLn2;
+}
+// The same for few tiles of many parts: a CTA takes 16 columns of 32 rows of one, its warps share the parts.
+template <int kHeadDim, bool kBf16>
+__global__ void __launch_bounds__(kJoinWarps * 32) fmha_paged_join_many_kernel(const __grid_constant__ Args a) {
+  ptx::grid_dependency_sync();
+  __shared__ float of_warp[kJoinWarps][19][33];
+  const int4 tile = a.meta[blockIdx.x];
+  const int parts = tile.w & 0xffff;
+  const int row0 = blockIdx.y * kJoinRows, column = blockIdx.z * 16, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // (a tile that this call does not have: what stands in its place is an earlier call's)
+  const Request req = load_request(a, blockIdx.x / (a.kv_heads * a.tile_blocks));
+  if (static_cast<int>(blockIdx.x) % a.tile_blocks * a.block_tokens >= req.rows || parts == 0 || row0 >= tile.z || column >= a.head_size) return;
+  Joined j;
+  if (row0 + lane < tile.z)
+    for (int i0 = warp; i0 < parts; i0 += 4 * kJoinWarps) add_parts<kHeadDim, 4>(a, tile.w >> 16, row0 + lane, column, i0, kJoinWarps, parts, &j);
+  of_warp[warp][0][lane] = j.top;
+  of_warp[warp][1][lane] = j.sum;
+  of_warp[warp][2][lane] = j.rounded;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) of_warp[warp][3 + e][lane] = j.o[e];
+  __syncthreads();
+  // two columns of a row a thread
+  const int row = threadIdx.x >> 3, pair = (threadIdx.x & 7) * 2;
+  if (row0 + row >= tile.z || column + pair >= a.head_size) return;
+  float top = -INFINITY, sum = 0.0f, rounded = 0.0f, x = 0.0f, y = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, of_warp[w][0][row]);
+  const float use = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) {
+    const float weight = ptx::ex2_approx(of_warp[w][0][row] - use);
+    sum = fmaf(weight, of_warp[w][1][row], sum);
+    rounded = fmaf(weight, of_warp[w][2][row], rounded);
+    x = fmaf(weight, of_warp[w][3 + pair][row], x);
+    y = fmaf(weight, of_warp[w][4 + pair][row], y);
+  }
+  const int token = (row0 + row) / a.group;
+  const int64_t q_row = tile.x + token, head = tile.y + row0 + row - token * a.group;
+  const float inv = 1.0f / rounded;
+  *reinterpret_cast<uint32_t*>(a.out + q_row * a.o_strides[0] + head * a.o_strides[1] + column + pair) =
+      rounded == 0.0f ? 0u : pack2<kBf16>(x * inv, y * inv);
+  if (column + pair == 0 && a.lse != nullptr) a.lse[q_row * a.heads + head] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
 int head_dim(int head_size) { return head_size <= 64 ? 64 : head_size <= 128 ? 128 : 256; }
@@ -952,7 +1006,7 @@ int check(const ixk_fmha_paged_desc* d, const ixk_paged_cache* c) {
   if (d->heads / c->heads > kRows) return fail(IXK_UNIMPLEMENTED, "fmha_paged: more than 128 query heads to a key head");
   if (c->page_size < 8 || c->page_size > 256 || (c->page_size & (c->page_size - 1)) != 0)
     return fail(IXK_UNIMPLEMENTED, "fmha_paged: page_size must be 8, 16, 32, 64, 128 or 256");
-  if (!std::isfinite(d->head_scale)) return fail(IXK_INVALID_ARGUMENT, "fmha_paged: head_scale is not finite");
+  if (!std::isfinite(d->head_scale * kLog2e)) return fail(IXK_INVALID_ARGUMENT, "fmha_paged: head_scale is not finite");
   if (d->rows > 0x7fffffff - 256 || static_cast<int64_t>(d->columns) * c->page_size > 0x7fffffff - 256)
     return fail(IXK_UNIMPLEMENTED, "fmha_paged: 2^31 rows, or keys of a request, or more");
   return IXK_OK;
@@ -970,6 +1024,9 @@ int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, con
   const int w = workers(kHeadDim, sm_count);
   if (int st = launch_overlapped(fmha_paged_kernel<kHeadDim, kBf16>, dim3(w), dim3(C::kAllThreads), C::kSmemBytes, stream, q, k, v, a)) return st;
   const unsigned blocks = static_cast<unsigned>((a.part_rows + kJoinRows - 1) / kJoinRows);
+  if (a.tile_blocks != 0)
+    return launch_overlapped(fmha_paged_join_many_kernel<kHeadDim, kBf16>, dim3(static_cast<unsigned>(a.requests) * a.kv_heads * a.tile_blocks, blocks, kHeadDim / 16),
+                             dim3(kJoinWarps * 32), 0, stream, a);
   return launch_overlapped(fmha_paged_join_kernel<kHeadDim, kBf16>, dim3(w, blocks), dim3(kHeadDim * 2), 0, stream, a);
 }
 
@@ -1043,6 +1100,10 @@ int ixk_fmha_paged_fwd(const ixk_fmha_paged_desc* d, const ixk_paged_cache* c, c
   a.lse = lse;
   a.status_word = info.status_word;
   a.part_rows = scratch.part_rows;
+  // Tiles of two parts and more (if they are of about one length): several warps share the parts of one in the join (one request, us:
+  // 8000 keys 27.4 -> 13.8, 60000 keys 49 -> 33; 4 trees of 16 over 4000 keys 21 -> 17.8).
+  const int64_t blocks = (d->rows + a.block_tokens - 1) / a.block_tokens, tiles = static_cast<int64_t>(d->requests) * c->heads * blocks;
+  a.tile_blocks = tiles * 2 <= fmha_paged::workers(fmha_paged::head_dim(c->head_size), info.sm_count) ? static_cast<int>(blocks) : 0;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   a.meta = reinterpret_cast<int4*>(ws + scratch.meta);
   a.part_stat = reinterpret_cast<float4*>(ws + scratch.stat);
