@@ -101,6 +101,7 @@ struct Args {
   // parts: none), or, where tiles are few, by tile ([requests][kv_heads][tile_blocks]; 0 parts: whole).
   int4* meta;
   int tile_blocks;            // 0: by worker
+  int workers;
   float* part_o;              // [2 * workers][kHeadDim / 4][part_rows][4]: a warp's rows side by side
   float4* part_stat;          // [2 * workers][part_rows]: maximum (log2), sum, sum of rounded weights
 };
@@ -937,15 +938,17 @@ template <int kHeadDim, bool kBf16>
 __global__ void __launch_bounds__(kJoinWarps * 32) fmha_paged_join_many_kernel(const __grid_constant__ Args a) {
   ptx::grid_dependency_sync();
   __shared__ float of_warp[kJoinWarps][19][33];
-  const int4 tile = a.meta[blockIdx.x];
-  const int parts = tile.w & 0xffff;
+  const int named = a.meta[blockIdx.x].w, parts = named & 0xffff, worker = named >> 16;
   const int row0 = blockIdx.y * kJoinRows, column = blockIdx.z * 16, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // (a tile that this call does not have: what stands in its place is an earlier call's)
-  const Request req = load_request(a, blockIdx.x / (a.kv_heads * a.tile_blocks));
-  if (static_cast<int>(blockIdx.x) % a.tile_blocks * a.block_tokens >= req.rows || parts == 0 || row0 >= tile.z || column >= a.head_size) return;
+  // The tile's numbers are made again: in the place of one that this call does not have stands an earlier call's.
+  const int head_tile = static_cast<int>(blockIdx.x) / a.tile_blocks, t0 = (static_cast<int>(blockIdx.x) - head_tile * a.tile_blocks) * a.block_tokens;
+  const int b = head_tile / a.kv_heads, head0 = (head_tile - b * a.kv_heads) * a.group;
+  const Request req = load_request(a, b);
+  const int rows = min(a.block_tokens, req.rows - t0) * a.group;
+  if (rows <= row0 || parts == 0 || worker < 0 || worker + parts > a.workers || column >= a.head_size) return;
   Joined j;
-  if (row0 + lane < tile.z)
-    for (int i0 = warp; i0 < parts; i0 += 4 * kJoinWarps) add_parts<kHeadDim, 4>(a, tile.w >> 16, row0 + lane, column, i0, kJoinWarps, parts, &j);
+  if (row0 + lane < rows)
+    for (int i0 = warp; i0 < parts; i0 += 4 * kJoinWarps) add_parts<kHeadDim, 4>(a, worker, row0 + lane, column, i0, kJoinWarps, parts, &j);
   of_warp[warp][0][lane] = j.top;
   of_warp[warp][1][lane] = j.sum;
   of_warp[warp][2][lane] = j.rounded;
@@ -954,7 +957,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fmha_paged_join_many_kernel(c
   __syncthreads();
   // two columns of a row a thread
   const int row = threadIdx.x >> 3, pair = (threadIdx.x & 7) * 2;
-  if (row0 + row >= tile.z || column + pair >= a.head_size) return;
+  if (row0 + row >= rows || column + pair >= a.head_size) return;
   float top = -INFINITY, sum = 0.0f, rounded = 0.0f, x = 0.0f, y = 0.0f;
 #pragma unroll
   for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, of_warp[w][0][row]);
@@ -968,7 +971,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fmha_paged_join_many_kernel(c
     y = fmaf(weight, of_warp[w][4 + pair][row], y);
   }
   const int token = (row0 + row) / a.group;
-  const int64_t q_row = tile.x + token, head = tile.y + row0 + row - token * a.group;
+  const int64_t q_row = req.row0 + t0 + token, head = head0 + row0 + row - token * a.group;
   const float inv = 1.0f / rounded;
   *reinterpret_cast<uint32_t*>(a.out + q_row * a.o_strides[0] + head * a.o_strides[1] + column + pair) =
       rounded == 0.0f ? 0u : pack2<kBf16>(x * inv, y * inv);
@@ -1100,10 +1103,11 @@ int ixk_fmha_paged_fwd(const ixk_fmha_paged_desc* d, const ixk_paged_cache* c, c
   a.lse = lse;
   a.status_word = info.status_word;
   a.part_rows = scratch.part_rows;
+  a.workers = fmha_paged::workers(fmha_paged::head_dim(c->head_size), info.sm_count);
   // Tiles of two parts and more (if they are of about one length): several warps share the parts of one in the join (one request, us:
   // 8000 keys 27.4 -> 13.8, 60000 keys 49 -> 33; 4 trees of 16 over 4000 keys 21 -> 17.8).
   const int64_t blocks = (d->rows + a.block_tokens - 1) / a.block_tokens, tiles = static_cast<int64_t>(d->requests) * c->heads * blocks;
-  a.tile_blocks = tiles * 2 <= fmha_paged::workers(fmha_paged::head_dim(c->head_size), info.sm_count) ? static_cast<int>(blocks) : 0;
+  a.tile_blocks = tiles * 2 <= a.workers ? static_cast<int>(blocks) : 0;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   a.meta = reinterpret_cast<int4*>(ws + scratch.meta);
   a.part_stat = reinterpret_cast<float4*>(ws + scratch.stat);
