@@ -185,8 +185,8 @@ def apply_rotary_half_(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, ro
     half = rotary_dim // 2
     x1, x2 = x[..., :half].float(), x[..., half:rotary_dim].float()
     c, s = cos[:, None, :], sin[:, None, :]
-    x[..., :half] = (x1 * c - x2 * s).to(x.dtype)
-    x[..., half:rotary_dim] = (x2 * c + x1 * s).to(x.dtype)
+    # (both before either is stored: of fp32 heads x1 and x2 are the heads themselves)
+    x[..., :half], x[..., half:rotary_dim] = (x1 * c - x2 * s).to(x.dtype), (x2 * c + x1 * s).to(x.dtype)
     return x
 
 
