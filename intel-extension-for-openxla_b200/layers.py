@@ -20,6 +20,8 @@ from typing import Optional
 import torch
 import torch.distributed as dist
 
+from . import PagedRows
+
 
 # ----------------------------------------------------------------------------- kernel calls
 
@@ -83,6 +85,22 @@ class KernelOps:
     def norm_backward(self, grad, x, mean, rstd, kind, gain, gain_offset, with_shift):
         return self.pkg.row_norm_backward(grad, x, mean, rstd, kind=self._kind(kind), gain=gain, gain_offset=gain_offset,
                                           with_shift=with_shift)
+
+    def paged_extend(self, page_table, lengths, new_tokens, free_pages, free_count, rows, page_size):
+        return self.pkg.paged_extend(page_table, lengths, new_tokens, free_pages, free_count, rows=rows, page_size=page_size)
+
+    def paged_keep_(self, page_table, lengths, granted, kept, free_pages, free_count, free_count_out, page_size, path, k_pages, v_pages):
+        self.pkg.paged_keep(page_table, lengths, granted, kept, free_pages, free_count, page_size=page_size, path=path,
+                            k_pages=None if path is None else k_pages, v_pages=None if path is None else v_pages,
+                            lengths_out=lengths, free_count_out=free_count_out)
+
+    def qk_norm_rotary_into_pages_(self, q, k, v, q_gain, k_gain, eps, cos, sin, positions, slots, k_pages, v_pages):
+        self.pkg.qk_norm_rotary_forward(q, k, q_gain=q_gain, k_gain=k_gain, gain_offset=1.0, eps=eps, cos=cos, sin=sin, positions=positions,
+                                        v=v, slots=slots, k_pages=k_pages, v_pages=v_pages, q_out=q)
+
+    def paged_attention_(self, q, k_pages, v_pages, page_table, lengths, row_start, granted, out, *, scale, mask=None, workspace=None):
+        self.pkg.fmha_paged_forward(q, k_pages, v_pages, page_table, lengths, row_start, granted, scale=scale, mask=mask, out=out,
+                                    workspace=workspace)
 
     def _kind(self, kind):
         return self.pkg.NORM_LAYER if kind == "layer" else self.pkg.NORM_RMS
@@ -335,9 +353,7 @@ def gemma_decode_step(x: torch.Tensor, w: GemmaLayerWeights, k_cache: torch.Tens
     rotary embedding on half-split pairs over the whole head, GeGLU with the tanh GELU."""
     B, _, hidden = x.shape
     hl, hd = w.heads_local, w.head_dim
-    norm = _glue(ops, "rms_norm", rms_norm)
-    add = _glue(ops, "residual_add", _residual_add_torch)
-    h = norm(x, gain=w.norm_attn).view(B, hidden)
+    h = _glue(ops, "rms_norm", rms_norm)(x, gain=w.norm_attn).view(B, hidden)
     qkv = ops.gemm(h, w.wqkv).view(B, 1, 3, hl, hd)
     cos, sin = rope if rope is not None else rotary_tables(torch.tensor([position], device=x.device), hd)
     _glue(ops, "rotary_qk_", _rotary_qk_torch_)(qkv, cos, sin, hd, half_split=True)
@@ -347,27 +363,35 @@ def gemma_decode_step(x: torch.Tensor, w: GemmaLayerWeights, k_cache: torch.Tens
     ctx = torch.empty(B, 1, hl, hd, dtype=x.dtype, device=x.device)
     ops.attention(q, k_cache[:, :T].permute(0, 2, 1, 3), v_cache[:, :T].permute(0, 2, 1, 3),
                   ctx.permute(0, 2, 1, 3), scale=1.0 / math.sqrt(hd), causal=False, workspace=workspace)
+    return _gemma_block_end(x, ctx.view(B, hl * hd), w, ops, group, reduce, comm)
+
+
+def _gemma_block_end(x, ctx, w: GemmaLayerWeights, ops, group=None, reduce=None, comm=None) -> torch.Tensor:
+    """What follows the attention in the Gemma block: x [..., hidden], ctx [tokens, heads_local * head_dim]."""
+    rows, hidden = ctx.shape[0], x.shape[-1]
+    norm = _glue(ops, "rms_norm", rms_norm)
+    add = _glue(ops, "residual_add", _residual_add_torch)
     # Nobody to exchange the partial sums with: the projections add the residual themselves, two launches less.
     joined = getattr(ops, "gemm_residual", None) if comm is None and reduce is None and not _distributed(group) else None
     reduce = reduce or all_reduce_sum
     if joined is not None:
-        x1 = joined(ctx.view(B, hl * hd), w.wo, x.view(B, hidden)).view(x.shape)
+        x1 = joined(ctx, w.wo, x.view(rows, hidden)).view(x.shape)
     elif comm is not None:
-        nbytes = (B * hidden * x.element_size() + 255) // 256 * 256
-        part = ops.gemm(ctx.view(B, hl * hd), w.wo, out=comm.view(0, (B, hidden), x.dtype))
+        nbytes = (rows * hidden * x.element_size() + 255) // 256 * 256
+        part = ops.gemm(ctx, w.wo, out=comm.view(0, (rows, hidden), x.dtype))
         x1 = comm.all_reduce_residual(part, x)
     else:
-        x1 = add(x, reduce(ops.gemm(ctx.view(B, hl * hd), w.wo), group))
-    h2 = norm(x1, gain=w.norm_mlp).view(B, hidden)
+        x1 = add(x, reduce(ops.gemm(ctx, w.wo), group))
+    h2 = norm(x1, gain=w.norm_mlp).view(rows, hidden)
     fused = getattr(ops, "gemm_geglu", None)
     act = fused(h2, w.wgateup) if fused is not None else None     # one GEMM for gate and up, GeGLU in its second pass
     if act is None:
         act = ops.gemm(h2, w.wgate, epilogue="GELU") * ops.gemm(h2, w.wup)
     if comm is not None:
-        part = ops.gemm(act, w.wdown, out=comm.view(nbytes, (B, hidden), x.dtype))
+        part = ops.gemm(act, w.wdown, out=comm.view(nbytes, (rows, hidden), x.dtype))
         return comm.all_reduce_residual(part, x1)
     if joined is not None:
-        return joined(act, w.wdown, x1.view(B, hidden)).view(x.shape)
+        return joined(act, w.wdown, x1.view(rows, hidden)).view(x.shape)
     return add(x1, reduce(ops.gemm(act, w.wdown), group))
 
 
@@ -376,6 +400,178 @@ def gemma_decode_bytes(B, T, hidden=3072, heads=16, head_dim=256, ffn=24576, ele
     attn = 2.0 * B * heads * T * head_dim * elem + 2.0 * B * heads * head_dim * elem
     weights = (hidden * 3 * heads * head_dim + heads * head_dim * hidden + 2 * hidden * ffn + ffn * hidden) * elem
     return attn + weights
+
+
+# ----------------------------------------------------------------------------- decoding over a paged cache
+
+@dataclass
+class GroupedLayerWeights(GemmaLayerWeights):
+    """The Gemma block with grouped key/value heads and an RMSNorm of every query's and key's head before the rotation.  wqkv
+    [hidden, (heads + 2 kv_heads) * head_dim], the blocks q | k | v with heads inside each; norm_q / norm_k [head_dim], applied
+    as (1 + w) (None = unit gain)."""
+    kv_heads_local: int = 1
+    norm_q: Optional[torch.Tensor] = None
+    norm_k: Optional[torch.Tensor] = None
+
+    @staticmethod
+    def shard(full: dict, num_heads: int, num_kv_heads: int, head_dim: int, rank: int, world: int):
+        hidden = full["wqkv"].shape[0]
+        heads = full["wqkv"].view(hidden, num_heads + 2 * num_kv_heads, head_dim)
+        (q0, q1), (k0, k1) = shard_range(num_heads, rank, world), shard_range(num_kv_heads, rank, world)
+        n, m = num_heads, num_heads + num_kv_heads
+        return GroupedLayerWeights(
+            wqkv=torch.cat((heads[:, q0:q1], heads[:, n + k0:n + k1], heads[:, m + k0:m + k1]), 1).reshape(hidden, -1).contiguous(),
+            wo=shard_rows(full["wo"], rank, world),
+            wgateup=torch.cat((shard_columns(full["wgate"], rank, world), shard_columns(full["wup"], rank, world)), dim=1),
+            wdown=shard_rows(full["wdown"], rank, world),
+            heads_local=q1 - q0, head_dim=head_dim, kv_heads_local=k1 - k0,
+            norm_attn=full.get("norm_attn"), norm_mlp=full.get("norm_mlp"), norm_q=full.get("norm_q"), norm_k=full.get("norm_k"))
+
+
+@dataclass
+class PagedCache:
+    """The keys and values of a batch of requests in pages of a common pool, all layers' with one page number: k_pages / v_pages
+    [layers, pages, page_size, kv_heads, head_dim]; page_table [requests, columns], lengths [requests], free_pages [pages] and
+    free_count [1] int32.  The tensors stay where they are from step to step, so that steps can be captured."""
+    k_pages: torch.Tensor
+    v_pages: torch.Tensor
+    page_table: torch.Tensor
+    lengths: torch.Tensor
+    free_pages: torch.Tensor
+    free_count: torch.Tensor
+
+    @staticmethod
+    def empty(layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, requests: int, most_tokens: int, *,
+              dtype=torch.bfloat16, device=None):
+        """All pages free; a request has room for `most_tokens`."""
+        ints = dict(dtype=torch.int32, device=device)
+        shape = (layers, pages, page_size, kv_heads, head_dim)
+        return PagedCache(torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device),
+                          torch.full((requests, -(-most_tokens // page_size)), -1, **ints), torch.zeros(requests, **ints),
+                          torch.arange(pages - 1, -1, -1, **ints), torch.full((1,), pages, **ints))
+
+    @property
+    def page_size(self) -> int:
+        return self.k_pages.shape[2]
+
+
+def _paged_extend_torch(page_table, lengths, new_tokens, free_pages, free_count, rows, page_size):
+    columns, left, start, granted = page_table.shape[1], int(free_count), [0], []
+    maps = torch.full((3, rows), -1, dtype=torch.int32, device=lengths.device)
+    free, wanted, end = left, 0, 0
+    for b, (n, length) in enumerate(zip(new_tokens.tolist(), lengths.tolist())):
+        n = max(n, 0)
+        end += n
+        fits = 0 <= length and length + n <= columns * page_size and end <= rows
+        c0, c1 = -(-length // page_size), -(-(length + n) // page_size)
+        need = c1 - c0 if fits else 0
+        wanted += need
+        if fits and (need == 0 or wanted <= free):
+            left -= need
+            page_table[b, c0:c1] = free_pages[left:left + need].flip(0)
+            place = torch.arange(length, length + n, device=lengths.device)
+            row = slice(start[-1], end)
+            maps[0, row], maps[1, row] = b, place.int()
+            maps[2, row] = page_table[b, place // page_size] * page_size + (place % page_size).int()
+            granted.append(n)
+        else:
+            granted.append(0)
+        start.append(min(end, rows))
+    ints = dict(dtype=torch.int32, device=lengths.device)
+    return PagedRows(torch.tensor(start, **ints), torch.tensor(granted, **ints), *maps.unbind(), torch.tensor([left], **ints))
+
+
+def _paged_keep_torch_(page_table, lengths, granted, kept, free_pages, free_count, free_count_out, page_size, path, k_pages, v_pages):
+    left = int(free_count)
+    for b, (length, n, k) in enumerate(zip(lengths.tolist(), granted.tolist(), kept.tolist())):
+        good = min(k, n)
+        if path is not None and good > 0:
+            drafts, last = [], -1
+            for draft in path[b, :good].tolist():
+                if not last < draft < n:
+                    break
+                drafts.append(draft)
+                last = draft
+            good = len(drafts)
+            source = length + torch.tensor(drafts, dtype=torch.long, device=lengths.device)
+            target = length + torch.arange(good, device=lengths.device)
+            for pages in (k_pages, v_pages):
+                moved = pages[:, page_table[b, source // page_size].long(), source % page_size]
+                pages[:, page_table[b, target // page_size].long(), target % page_size] = moved
+        after = 0 if k < 0 else length + good
+        back = page_table[b, -(-after // page_size):-(-(length + n) // page_size)]
+        free_pages[left:left + back.numel()] = back
+        left += back.numel()
+        lengths[b] = after
+    free_count_out.fill_(left)
+
+
+def _qk_norm_rotary_into_pages_torch_(q, k, v, q_gain, k_gain, eps, cos, sin, positions, slots, k_pages, v_pages):
+    page_size = k_pages.shape[1]
+    t = torch.nonzero((positions >= 0) & (positions < cos.shape[0]))[:, 0]
+    c, s = cos[positions[t].long()], sin[positions[t].long()]
+    turned = [apply_rotary_half_(rms_norm(x[t].float(), eps, gain), c, s, 2 * cos.shape[1]).to(x.dtype) for x, gain in ((q, q_gain), (k, k_gain))]
+    q[t] = turned[0]
+    here = (slots[t] >= 0) & (slots[t] < k_pages.shape[0] * page_size)
+    place = slots[t][here].long()
+    k_pages[place // page_size, place % page_size] = turned[1][here]
+    v_pages[place // page_size, place % page_size] = v[t][here]
+
+
+def _paged_attention_torch_(q, k_pages, v_pages, page_table, lengths, row_start, granted, out, *, scale, mask=None, workspace=None):
+    page_size, kv_heads = k_pages.shape[1:3]
+    group = q.shape[1] // kv_heads
+    for b, (length, r0, n) in enumerate(zip(lengths.tolist(), row_start.tolist(), granted.tolist())):
+        place = torch.arange(length + n, device=q.device)
+        at = page_table[b, place // page_size].long(), place % page_size
+        keys, values = (pages[at].float().repeat_interleave(group, 1) for pages in (k_pages, v_pages))
+        i = torch.arange(n, device=q.device)
+        new = i[None, :] <= i[:, None] if mask is None else ((mask[r0:r0 + n, i // 32] >> (i % 32).int()) & 1).bool()
+        seen = torch.cat((torch.ones(n, length, dtype=torch.bool, device=q.device), new), 1)
+        z = torch.where(seen, torch.einsum("ihd,jhd->hij", q[r0:r0 + n].float(), keys) * scale, -math.inf)
+        p = torch.exp(z - z.amax(-1, keepdim=True).clamp(min=-1e30)) if place.numel() else z
+        p = p / p.sum(-1, keepdim=True).clamp(min=1e-30)
+        out[r0:r0 + n] = torch.einsum("hij,jhd->ihd", p, values).to(out.dtype)
+
+
+def grouped_layer_step(x: torch.Tensor, w: GroupedLayerWeights, cache: PagedCache, layer: int, step: PagedRows, ctx: torch.Tensor, ops, *,
+                       rope, positions=None, mask=None, eps: float = 1e-6, group=None, workspace=None, reduce=None, comm=None) -> torch.Tensor:
+    """One layer of a step: x [rows, hidden].  Norms, rotation and the way into the pages are one pass over QKV, in which the
+    queries stay in their place; ctx [rows, heads_local, head_dim] is the attention's result."""
+    rows, hl, kl, hd = x.shape[0], w.heads_local, w.kv_heads_local, w.head_dim
+    h = _glue(ops, "rms_norm", rms_norm)(x, gain=w.norm_attn)
+    qkv = ops.gemm(h, w.wqkv).view(rows, hl + 2 * kl, hd)
+    q, k, v = qkv.split((hl, kl, kl), 1)
+    k_pages, v_pages = cache.k_pages[layer], cache.v_pages[layer]
+    _glue(ops, "qk_norm_rotary_into_pages_", _qk_norm_rotary_into_pages_torch_)(
+        q, k, v, w.norm_q, w.norm_k, eps, *rope, step.position if positions is None else positions, step.slot, k_pages, v_pages)
+    _glue(ops, "paged_attention_", _paged_attention_torch_)(q, k_pages, v_pages, cache.page_table, cache.lengths, step.row_start, step.granted, ctx,
+                                                            scale=1.0 / math.sqrt(hd), mask=mask, workspace=workspace)
+    return _gemma_block_end(x, ctx.view(rows, hl * hd), w, ops, group, reduce, comm)
+
+
+def paged_step(x: torch.Tensor, weights, cache: PagedCache, new_tokens: torch.Tensor, ops, *, rope, positions=None, mask=None, **more):
+    """A step of all requests over a paged cache, prompts, single tokens and drafted chains and trees together: x [rows, hidden]
+    holds the requests' new tokens one request after another, new_tokens [requests] of each (int32, on the GPU; rows behind
+    the last are of nobody).  Without `mask` a new token sees the new ones before it; a tree's mask [rows, words] has the bits of
+    the ones that it sees, itself among them, and `positions` [rows] its tokens' places in the text (a tree's slots follow one
+    another, its places its depths).  `rope`: (cos, sin) tables [places, rotary_dim / 2].  Returns (x after all layers, PagedRows);
+    commit what stays with paged_accept_ before the next step.  The host waits for nothing, and the step can be captured."""
+    step = _glue(ops, "paged_extend", _paged_extend_torch)(cache.page_table, cache.lengths, new_tokens, cache.free_pages, cache.free_count,
+                                                           x.shape[0], cache.page_size)
+    # (zeros once a step: the rows of nobody, which the attention leaves alone, stay numbers in all layers)
+    ctx = torch.zeros(x.shape[0], weights[0].heads_local, weights[0].head_dim, dtype=x.dtype, device=x.device)
+    for layer, w in enumerate(weights):
+        x = grouped_layer_step(x, w, cache, layer, step, ctx, ops, rope=rope, positions=positions, mask=mask, **more)
+    return x, step
+
+
+def paged_accept_(cache: PagedCache, step: PagedRows, kept: torch.Tensor, ops, *, path=None) -> None:
+    """kept[b] of request b's new tokens stay (int32; negative: the request is over), the ones that path[b, :kept[b]] lists in
+    ascending order or, without a path, the first; the other pages are free again.  All of the cache's books are brought up
+    to date in place."""
+    _glue(ops, "paged_keep_", _paged_keep_torch_)(cache.page_table, cache.lengths, step.granted, kept, cache.free_pages, step.free_count,
+                                                  cache.free_count, cache.page_size, path, cache.k_pages, cache.v_pages)
 
 
 # ----------------------------------------------------------------------------- the end of a training step
