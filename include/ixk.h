@@ -387,8 +387,8 @@ typedef struct ixk_page_pool {
  * needs pages when, together with all that fit before it, more are needed than there are, is not
  * served: granted[b] = 0, no page is taken, its rows' maps are -1.  Otherwise granted[b] =
  * new_tokens[b], and row r = row_start[b] + j has request[r] = b, position[r] = lengths[b] + j and slot[r].  Rows
- * behind the last request are -1 as well.  *free_count_out = pages left (may be free_count itself; no
- * other output may be one of the inputs).  lengths is left as it is until ixk_paged_keep. */
+ * behind the last request are -1 as well.  *free_count_out = pages left (may be free_count itself;
+ * otherwise no output may share memory with an input or another output).  lengths is left as it is until ixk_paged_keep. */
 int ixk_paged_extend(const ixk_page_pool* pool, const int32_t* lengths, const int32_t* new_tokens,
                      int32_t* page_table, const int32_t* free_pages, const int32_t* free_count,
                      int32_t* free_count_out, int32_t* granted, int32_t* row_start, int64_t rows,
@@ -410,7 +410,8 @@ typedef struct ixk_paged_cache {
  * granted[b], ends the path.  path NULL: the first kept[b] stay where they are.  Then lengths_out[b] = lengths[b]
  * + kept, and the pages above go back to the end of free_pages in the order of the requests.  kept[b] < 0
  * ends the request: lengths_out[b] = 0 and all of its pages go back.  lengths_out may be lengths,
- * free_count_out free_count.  The table itself is not written.  cache, k, v: NULL with path NULL.
+ * free_count_out free_count; nothing else that is written may share memory with anything.  The table
+ * itself is not written.  cache, k, v: NULL with path NULL.
  * path_columns at most 1024; K and V 16-byte aligned. */
 int ixk_paged_keep(const ixk_page_pool* pool, const int32_t* lengths, const int32_t* granted,
                    const int32_t* kept, const int32_t* path, int64_t path_columns, int64_t path_stride,
@@ -471,7 +472,7 @@ size_t ixk_qk_norm_rotary_bwd_workspace_bytes(const ixk_qk_desc* desc);
  * table row are not read.  Scores, statistics and sums are fp32; p is rounded to dtype (to nearest) as an operand
  * of the second product, and out is divided by the sum of the rounded p (lse: of the fp32 ones).  Results depend on
  * the lengths and sizes alone, not on timing.
- * page_size in {8, 16, 32, 64, 128, 256}; head_size a multiple of 8 up to 256; q, out, K and V 16-byte aligned
+ * out may be q, with its strides.  page_size in {8, 16, 32, 64, 128, 256}; head_size a multiple of 8 up to 256; q, out, K and V 16-byte aligned
  * with strides that are multiples of 8 elements; workspace: ixk_fmha_paged_fwd_workspace_bytes(desc, cache)
  * bytes, 16-byte aligned. */
 typedef struct ixk_fmha_paged_desc {

@@ -804,6 +804,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 #pragma unroll 1
         for (int c0 = 0; c0 < kHeadDim; c0 += 64) {
           uint32_t o[64];
+          __syncwarp();
           ptx::tmem_ld_32x32(o_addr + c0, *reinterpret_cast<uint32_t(*)[32]>(o));
           ptx::tmem_ld_32x32(o_addr + c0 + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
           ptx::tmem_ld_wait();
@@ -1068,6 +1069,9 @@ int ixk_fmha_paged_fwd(const ixk_fmha_paged_desc* d, const ixk_paged_cache* c, c
     if (extent > 1 && (d->q_strides[i] < c->head_size || d->o_strides[i] < c->head_size))
       return fail(IXK_INVALID_ARGUMENT, "fmha_paged: rows of q or out overlap");
   }
+  if (out == q && out != nullptr && ((d->rows > 1 && d->q_strides[0] != d->o_strides[0]) || (d->heads > 1 && d->q_strides[1] != d->o_strides[1])))
+    return fail(IXK_INVALID_ARGUMENT, "fmha_paged: out is in q's place, with other strides");
+  if (out != nullptr && (out == k_pages || out == v_pages)) return fail(IXK_INVALID_ARGUMENT, "fmha_paged: out is in the cache");
   DeviceInfo info;
   if (int st = get_device_info(&info)) return st;
   if (d->requests == 0 || d->rows == 0) return IXK_OK;

@@ -1,12 +1,33 @@
 // Checks and addresses shared by the calls on a paged key/value cache.
 #pragma once
 
+#include <initializer_list>
+
 #include "host_common.h"
 
 namespace ixk {
 namespace paged {
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// A call's int32 arrays: what it writes may share memory with nothing else of it, but an array that it updates in place (`with`).
+struct Ints {
+  const int32_t* p;
+  int64_t count;
+  bool written;
+  const int32_t* with;
+};
+inline bool ints_overlap(std::initializer_list<Ints> all) {
+  for (const Ints* a = all.begin(); a != all.end(); ++a) {
+    if (!a->written || a->p == nullptr || a->count <= 0) continue;
+    for (const Ints* b = all.begin(); b != all.end(); ++b) {
+      if (b == a || b->p == nullptr || b->count <= 0 || (a->with == b->p && a->p == b->p)) continue;
+      if (a->p < b->p + b->count && b->p < a->p + a->count) return true;
+    }
+  }
+  return false;
+}
+inline int64_t rows_extent(int64_t rows, int64_t stride, int64_t columns) { return rows < 1 ? 0 : (rows - 1) * stride + columns; }
 
 // What the kernels need of a cache to find a token's row: strides in 16-byte vectors.
 struct CacheArgs {

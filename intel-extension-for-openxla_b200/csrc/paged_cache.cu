@@ -363,11 +363,12 @@ int ixk_paged_extend(const ixk_page_pool* pool, const int32_t* lengths, const in
       (pool->requests > 0 && (lengths == nullptr || new_tokens == nullptr || page_table == nullptr || granted == nullptr)) ||
       (rows > 0 && (request == nullptr || position == nullptr || slot == nullptr)))
     return fail(IXK_INVALID_ARGUMENT, "paged_extend: null argument");
-  const void* inputs[] = {lengths, new_tokens, free_pages, free_count, page_table};
-  for (const void* out : {static_cast<void*>(granted), static_cast<void*>(row_start), static_cast<void*>(request),
-                          static_cast<void*>(position), static_cast<void*>(slot)})
-    for (const void* in : inputs)
-      if (out != nullptr && out == in) return fail(IXK_INVALID_ARGUMENT, "paged_extend: an output is one of the inputs");
+  const int64_t requests = pool->requests;
+  if (paged::ints_overlap({{lengths, requests, false, nullptr}, {new_tokens, requests, false, nullptr}, {free_pages, pool->pages, false, nullptr},
+                           {free_count, 1, false, nullptr}, {page_table, paged::rows_extent(requests, pool->table_stride, pool->columns), true, nullptr},
+                           {free_count_out, 1, true, free_count}, {granted, requests, true, nullptr}, {row_start, requests + 1, true, nullptr},
+                           {request, rows, true, nullptr}, {position, rows, true, nullptr}, {slot, rows, true, nullptr}}))
+    return fail(IXK_INVALID_ARGUMENT, "paged_extend: an output shares memory with an input or another output");
   DeviceInfo info;
   if (int st = get_device_info(&info)) return st;
   const bool in_place = free_count_out == free_count;
@@ -421,9 +422,14 @@ int ixk_paged_keep(const ixk_page_pool* pool, const int32_t* lengths, const int3
     if (int st = paged::check_cache(cache, k, v, "paged_keep")) return st;
     if (cache->page_size != pool->page_size || cache->pages != pool->pages)
       return fail(IXK_INVALID_ARGUMENT, "paged_keep: pool and cache differ in pages or page_size");
+    if (k == v) return fail(IXK_INVALID_ARGUMENT, "paged_keep: k and v are the same memory");
   }
-  if (lengths_out != nullptr && (lengths_out == granted || lengths_out == kept || lengths_out == path || lengths_out == page_table))
-    return fail(IXK_INVALID_ARGUMENT, "paged_keep: lengths_out may be lengths, but no other input");
+  const int64_t requests = pool->requests;
+  if (paged::ints_overlap({{lengths, requests, false, nullptr}, {granted, requests, false, nullptr}, {kept, requests, false, nullptr},
+                           {path, paged::rows_extent(path == nullptr ? 0 : requests, path_stride, path_columns), false, nullptr},
+                           {page_table, paged::rows_extent(requests, pool->table_stride, pool->columns), false, nullptr}, {free_pages, pool->pages, true, nullptr},
+                           {free_count, 1, false, nullptr}, {free_count_out, 1, true, free_count}, {lengths_out, requests, true, lengths}}))
+    return fail(IXK_INVALID_ARGUMENT, "paged_keep: what it writes shares memory with something else (lengths_out may be lengths, free_count_out free_count)");
   DeviceInfo info;
   if (int st = get_device_info(&info)) return st;
   paged::KeepArgs a{};

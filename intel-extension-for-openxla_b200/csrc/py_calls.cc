@@ -668,10 +668,14 @@ at::Tensor piece(const at::Tensor& whole, int64_t at, int64_t n) {
 }
 // _require_here: given tensors are on the current device.
 bool here(std::initializer_list<const at::Tensor*> tensors) {
-  const auto device = c10::cuda::current_device();
-  for (const at::Tensor* t : tensors)
-    if (t != nullptr && t->device().index() != device) return false;
-  return true;
+  const at::Tensor* one = nullptr;
+  for (const at::Tensor* t : tensors) {
+    if (t == nullptr) continue;
+    if (one == nullptr && t->device().index() != c10::cuda::current_device()) return false;
+    if (one != nullptr && t->device() != one->device()) return false;
+    one = t;
+  }
+  return true;      // (also where none is on a GPU: asking for the current device would be an error of its own)
 }
 // _int32
 bool ints(const at::Tensor* t, int64_t n) {
@@ -721,7 +725,7 @@ IXK_PY_FUNCTION(py_paged_extend, 9)
   int64_t rows, page_size;
   void* stream;
   ixk_page_pool d;
-  if (!integer(a[5], &rows) || !integer(a[6], &page_size) || rows < 0 || !stream_arg(a[8], &stream) ||
+  if (table == nullptr || !integer(a[5], &rows) || !integer(a[6], &page_size) || rows < 0 || !stream_arg(a[8], &stream) ||
       !page_pool(table, lengths, pages, count, page_size, &d) || !ints(fresh, d.requests) || !here({table, lengths, fresh, pages, count}))
     Py_RETURN_NONE;
   const int64_t shapes[6] = {d.requests + 1, d.requests, rows, rows, rows, 1};
@@ -760,7 +764,7 @@ IXK_PY_FUNCTION(py_paged_keep, 13)
   void* stream;
   ixk_page_pool d;
   ixk_paged_cache c;
-  if (!integer(a[6], &page_size) || !optional(a[7], &path) || !optional(a[8], &k) || !optional(a[9], &v) || !optional(a[10], &lengths_out) ||
+  if (table == nullptr || !integer(a[6], &page_size) || !optional(a[7], &path) || !optional(a[8], &k) || !optional(a[9], &v) || !optional(a[10], &lengths_out) ||
       !optional(a[11], &count_out) || !stream_arg(a[12], &stream) || !page_pool(table, lengths, pages, count, page_size, &d) ||
       !ints(granted, d.requests) || !ints(kept, d.requests) ||
       !here({table, lengths, granted, kept, pages, count, path, k, v, lengths_out, count_out}))
@@ -831,7 +835,7 @@ IXK_PY_FUNCTION(py_qk_forward, 17)
   void* stream;
   ixk_qk_desc d;
   ixk_paged_cache c;
-  if (!optional(a[2], &qg) || !optional(a[3], &kg) || !number(a[4], &offset) || !number(a[5], &eps) || !optional(a[8], &pos) ||
+  if (q == nullptr || !optional(a[2], &qg) || !optional(a[3], &kg) || !number(a[4], &offset) || !number(a[5], &eps) || !optional(a[8], &pos) ||
       !PyBool_Check(a[9]) || !optional(a[10], &v) || !optional(a[11], &slots) || !optional(a[12], &kp) || !optional(a[13], &vp) ||
       !optional(a[14], &qo) || !optional(a[15], &ko) || !stream_arg(a[16], &stream) ||
       !qk_desc(q, k, qg, kg, offset, eps, cos, sin, pos, a[9] == Py_True, &d) || !here({q, k, qg, kg, cos, sin, pos, v, slots, kp, vp, qo, ko}))
@@ -866,7 +870,7 @@ IXK_PY_FUNCTION(py_qk_backward, 16)
   double offset, eps;
   void* stream;
   ixk_qk_desc d;
-  if (!optional(a[4], &qg) || !optional(a[5], &kg) || !number(a[6], &offset) || !number(a[7], &eps) || !optional(a[10], &pos) ||
+  if (q == nullptr || !optional(a[4], &qg) || !optional(a[5], &kg) || !number(a[6], &offset) || !number(a[7], &eps) || !optional(a[10], &pos) ||
       !PyBool_Check(a[11]) || !optional(a[12], &dq) || !optional(a[13], &dk) || !optional(a[14], &ws) || !stream_arg(a[15], &stream) ||
       !qk_desc(q, k, qg, kg, offset, eps, cos, sin, pos, a[11] == Py_True, &d) || !heads_view(gq, q->sizes(), q->scalar_type(), d.gq_strides) ||
       !heads_view(gk, k->sizes(), q->scalar_type(), d.gk_strides) || !here({gq, gk, q, k, qg, kg, cos, sin, pos, dq, dk, ws}))

@@ -619,6 +619,18 @@ int check_strides(const int64_t (&s)[2], int64_t tokens, int64_t heads, int size
   return IXK_OK;
 }
 
+// A result in the place of its input lies as that does; anything else that is read or written, it is not.
+int check_in_place(const void* out, const int64_t (&os)[2], const void* in, const int64_t (&is)[2], int64_t tokens, int64_t heads, const char* who,
+                   const char* name) {
+  if (out != in || out == nullptr || ((tokens <= 1 || os[0] == is[0]) && (heads <= 1 || os[1] == is[1]))) return IXK_OK;
+  return fail(IXK_INVALID_ARGUMENT, std::string(who) + ": " + name + " is in the place of its input, with other strides");
+}
+int check_apart(const void* out, std::initializer_list<const void*> others, const char* who, const char* name) {
+  for (const void* p : others)
+    if (p != nullptr && p == out) return fail(IXK_INVALID_ARGUMENT, std::string(who) + ": " + name + " is in the place of another tensor");
+  return IXK_OK;
+}
+
 Args base_args(const ixk_qk_desc* d) {
   Args a{};
   a.heads = d->heads;
@@ -705,6 +717,7 @@ int ixk_qk_norm_rotary_fwd(const ixk_qk_desc* d, const void* q, const void* k, c
     if (int st = paged::check_cache(cache, k_pages, v_pages, who)) return st;
     if (cache->dtype != d->dtype || cache->heads != d->kv_heads || cache->head_size != d->head_size)
       return fail(IXK_INVALID_ARGUMENT, "qk_norm_rotary: the cache's type, heads or head_size are not those of k and v");
+    if (k_pages == v_pages) return fail(IXK_INVALID_ARGUMENT, "qk_norm_rotary: k and v of the cache are the same memory");
   }
   if (d->tokens > 0 && (q == nullptr || k == nullptr || cos_table == nullptr || sin_table == nullptr || q_out == nullptr ||
                         (paged ? v == nullptr || slots == nullptr : k_out == nullptr)))
@@ -716,6 +729,12 @@ int ixk_qk_norm_rotary_fwd(const ixk_qk_desc* d, const void* q, const void* k, c
     if (int st = qk::check_strides(d->v_strides, d->tokens, d->kv_heads, d->head_size, false, who, "v")) return st;
   } else if (int st = qk::check_strides(d->k_out_strides, d->tokens, d->kv_heads, d->head_size, true, who, "k_out")) {
     return st;
+  }
+  if (d->tokens > 0) {
+    if (int st = qk::check_in_place(q_out, d->q_out_strides, q, d->q_strides, d->tokens, d->heads, who, "q_out")) return st;
+    if (int st = qk::check_in_place(k_out, d->k_out_strides, k, d->k_strides, d->tokens, d->kv_heads, who, "k_out")) return st;
+    if (int st = qk::check_apart(q_out, {k, v, k_out, k_pages, v_pages, cos_table, sin_table, positions, q_gain, k_gain}, who, "q_out")) return st;
+    if (int st = qk::check_apart(k_out, {q, cos_table, sin_table, positions, q_gain, k_gain}, who, "k_out")) return st;
   }
   for (const void* p : {q, k, v, q_gain, k_gain, static_cast<const void*>(cos_table), static_cast<const void*>(sin_table),
                         static_cast<const void*>(q_out), static_cast<const void*>(k_out)})
@@ -760,6 +779,14 @@ int ixk_qk_norm_rotary_bwd(const ixk_qk_desc* d, const void* grad_q, const void*
   if (int st = qk::check_strides(d->gk_strides, d->tokens, d->kv_heads, d->head_size, false, who, "grad_k")) return st;
   if (int st = qk::check_strides(d->q_out_strides, d->tokens, d->heads, d->head_size, true, who, "dq")) return st;
   if (int st = qk::check_strides(d->k_out_strides, d->tokens, d->kv_heads, d->head_size, true, who, "dk")) return st;
+  if (d->tokens > 0) {
+    if (int st = qk::check_in_place(dq, d->q_out_strides, q, d->q_strides, d->tokens, d->heads, who, "dq")) return st;
+    if (int st = qk::check_in_place(dq, d->q_out_strides, grad_q, d->gq_strides, d->tokens, d->heads, who, "dq")) return st;
+    if (int st = qk::check_in_place(dk, d->k_out_strides, k, d->k_strides, d->tokens, d->kv_heads, who, "dk")) return st;
+    if (int st = qk::check_in_place(dk, d->k_out_strides, grad_k, d->gk_strides, d->tokens, d->kv_heads, who, "dk")) return st;
+    if (int st = qk::check_apart(dq, {k, grad_k, dk, cos_table, sin_table, positions, q_gain, k_gain, workspace}, who, "dq")) return st;
+    if (int st = qk::check_apart(dk, {q, grad_q, cos_table, sin_table, positions, q_gain, k_gain, workspace}, who, "dk")) return st;
+  }
   for (const void* p : {grad_q, grad_k, q, k, q_gain, k_gain, static_cast<const void*>(cos_table), static_cast<const void*>(sin_table),
                         static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(workspace)})
     if (!aligned16(p)) return fail(IXK_INVALID_ARGUMENT, "qk_norm_rotary backward: pointers must be 16-byte aligned");

@@ -349,3 +349,22 @@ def test_native_and_python_calls_agree(pkg, cuda, monkeypatch):
     monkeypatch.setattr(pkg, "_NATIVE", None)
     out, lse = call(pkg, s)
     assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+@pytest.mark.parametrize("size,lengths", [(128, [300, 20000, 7] + [40] * 50), (256, [9000] + [200, 3] * 40), (64, [30000, 30000] + [5] * 60), (128, [8000])])
+def test_one_long_request_among_short_ones(pkg, cuda, size, lengths):
+    """Tiles in parts of many workers beside tiles that one worker does whole."""
+    s = make(cuda, lengths, [3] * len(lengths), 8, 2, size, 16, torch.bfloat16, seed=4)
+    check(s, *call(pkg, s))
+
+
+@pytest.mark.parametrize("lengths", [[70, 2000, 9, 0], [40] * 90])
+def test_the_result_in_the_place_of_q(pkg, cuda, lengths):
+    s = make(cuda, lengths, [5] * len(lengths), 12, 4, 128, 16, torch.bfloat16, seed=2)
+    out, lse = call(pkg, s)
+    q = s["q"].clone()
+    again, lse2 = call(pkg, dict(s, q=q), out=q)
+    assert again is q and torch.equal(q, out) and torch.equal(lse, lse2)
+    with pytest.raises(pkg.IxkError):
+        wide = torch.zeros(q.shape[0], 24, 128, dtype=q.dtype, device=cuda)
+        call(pkg, dict(s, q=wide[:, :12]), out=wide[:, ::2])

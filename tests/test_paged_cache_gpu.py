@@ -179,7 +179,7 @@ def test_numbers_outside_their_ranges(pkg, cuda):
     table.copy_(ints(cuda, [[0, 1, -4, 2 ** 30, 5], [2 ** 31 - 1] * 5, [3, 4, 5, 6, 7], [-1] * 5]))
     extra = torch.full((pages + 8,), 55, dtype=torch.int32, device=cuda)
     free = extra[4:4 + pages].copy_(torch.arange(pages, device=cuda) * 3 - 9)
-    pool = torch.full((pages + 2, page, 2, 16), 1.0, dtype=torch.bfloat16, device=cuda)
+    pools = torch.full((2, pages + 2, page, 2, 16), 1.0, dtype=torch.bfloat16, device=cuda)
     for lengths, new, count, kept, path in (
             ([-1, 2 ** 31 - 1, 30, 3], [5, 5, 2 ** 31 - 1, -3], 2 ** 31 - 1, [3, 2 ** 31 - 1, 2, -1], [[0, 1, 2]] * 4),
             ([20, 17, 40, 0], [2, 9, 1, 40], -7, [2, 9, 1, 40], [[1, 3, 2 ** 31 - 1], [0, 8, 9], [-1, 0, 1], [5, 6, 39]])):
@@ -188,10 +188,10 @@ def test_numbers_outside_their_ranges(pkg, cuda):
         assert (r.slot < pages * page).all()
         granted = r.granted if count < 0 else ints(cuda, [2 ** 31 - 1, 5, -4, 9])
         after, left = pkg.paged_keep(table, ints(cuda, lengths), granted, ints(cuda, kept), free, ints(cuda, [count]), page_size=page,
-                                     path=ints(cuda, path), k_pages=pool[1:-1], v_pages=pool[1:-1])
+                                     path=ints(cuda, path), k_pages=pools[0, 1:-1], v_pages=pools[1, 1:-1])
         assert 0 <= left.item() <= pages and after.min() >= 0
     assert (whole[0] == 77).all() and (whole[5] == 77).all() and (whole[:, :2] == 77).all() and (whole[:, 7:] == 77).all()
-    assert (extra[:4] == 55).all() and (extra[4 + pages:] == 55).all() and (pool == 1.0).all()
+    assert (extra[:4] == 55).all() and (extra[4 + pages:] == 55).all() and (pools == 1.0).all()
 
 
 def test_refusals(pkg, cuda):
@@ -235,6 +235,7 @@ def test_refusals(pkg, cuda):
     refused(un, keep, path=path, k_pages=pool[..., :60], v_pages=pool[..., :60])
     refused(un, keep, path=torch.zeros(2, 2000, dtype=torch.int32, device=cuda), k_pages=pool, v_pages=pool)
     refused(bad, keep, lengths_out=new)
+    refused(bad, keep, path=path, k_pages=pool, v_pages=pool)           # the same memory twice: moved twice
     assert pkg.launch_count() == n0
 
 
@@ -246,13 +247,13 @@ def test_replayed_on_another_stream_and_without_native_calls(pkg, cuda, monkeypa
 
     a, table, lengths, free, count = state()
     new, kept, path = ints(cuda, [3, 4, 5, 1, 0, 9]), ints(cuda, [2, 4, 1, 0, 0, 3]), ints(cuda, [[0, 2, 8, 9]] * 6)
-    pool = torch.randn(200, 4, 1, 8, device=cuda).half()
+    pool, values = torch.randn(2, 200, 4, 1, 8, device=cuda).half()
     step_count = torch.zeros_like(count)
     out = pkg.PagedRows(*(torch.zeros(n, dtype=torch.int32, device=cuda) for n in (7, 6, 25, 25, 25)), step_count)
 
     def step(stream=None):
         r = pkg.paged_extend(table, lengths, new, free, count, rows=25, page_size=4, out=out, stream=stream)
-        pkg.paged_keep(table, lengths, r.granted, kept, free, r.free_count, page_size=4, path=path, k_pages=pool, v_pages=pool, lengths_out=lengths,
+        pkg.paged_keep(table, lengths, r.granted, kept, free, r.free_count, page_size=4, path=path, k_pages=pool, v_pages=values, lengths_out=lengths,
                        free_count_out=count, stream=stream)
 
     step()
