@@ -53,7 +53,8 @@ struct Args {
   paged::CacheArgs cache;
   const int* slots;                     // nullptr: k to ko
   int q_segments, kv_segments, segments;     // stretches of a token's heads: queries, then keys, then values
-  int parts;                            // warps that share a token's segments
+  int turns, parts;                     // tokens of every warp; warps that share the segments of a token of the last turn
+  int64_t rest;                         // tokens of the last turn
   float* partial;                       // backward: [CTA][2][256]
   int with_gains;
 };
@@ -232,6 +233,18 @@ __device__ __forceinline__ Pairs load_weights(const Args& a, const void* gain, i
   return w;
 }
 
+template <typename T>
+__device__ __forceinline__ float weight_of(const Args& a, const void* gain, int column) {
+  if (gain == nullptr || column >= a.head_chunks * 8) return 1.0f;
+  return a.gain_offset + (a.param_fp32 ? static_cast<const float*>(gain)[column] : static_cast<float>(static_cast<const T*>(gain)[column]));
+}
+__device__ __forceinline__ Pairs eight(const float* at) {
+  const float4 x = reinterpret_cast<const float4*>(at)[0], y = reinterpret_cast<const float4*>(at)[1];
+  Pairs r;
+  r.v[0] = ptx::f32x2(x.x, x.y), r.v[1] = ptx::f32x2(x.z, x.w), r.v[2] = ptx::f32x2(y.x, y.y), r.v[3] = ptx::f32x2(y.z, y.w);
+  return r;
+}
+
 // A lane's place in its head: its two chunks (behind the head's last: none), and whether they turn.
 struct Place {
   int a, b;          // first elements
@@ -306,6 +319,36 @@ __device__ __forceinline__ Turn turn_of(const Angles& g) {
   }
   return t;
 }
+// The turn backwards, without weights: half-split, of both chunks by the same angles.
+template <bool kHalf>
+struct BackTurn;
+template <>
+struct BackTurn<true> {
+  Pairs c, s;
+  __device__ __forceinline__ explicit BackTurn(const Angles& g) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      c.v[i] = ptx::f32x2(g.c[2 * i], g.c[2 * i + 1]);
+      s.v[i] = ptx::f32x2(g.s[2 * i], g.s[2 * i + 1]);
+    }
+  }
+  __device__ __forceinline__ void operator()(const Pairs& xa, const Pairs& xb, Pairs* ya, Pairs* yb) const {
+    Pairs across = mul(xa, s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) across.v[i] ^= 0x8000000080000000ull;
+    *ya = fma(xa, c, mul(xb, s));
+    *yb = fma(xb, c, across);
+  }
+};
+template <>
+struct BackTurn<false> {
+  Turn t;
+  __device__ __forceinline__ explicit BackTurn(const Angles& g) : t(turn_of<false, true>(g)) {}
+  __device__ __forceinline__ void operator()(const Pairs& xa, const Pairs& xb, Pairs* ya, Pairs* yb) const {
+    *ya = fma(xa, t.ca, mul(swapped(xa), t.sa));
+    *yb = fma(xb, t.cb, mul(swapped(xb), t.sb));
+  }
+};
 template <bool kHalf>
 __device__ __forceinline__ void turn(const Turn& t, const Pairs& xa, const Pairs& xb, Pairs* ya, Pairs* yb) {
   *ya = fma(xa, t.ca, mul(kHalf ? xb : swapped(xa), t.sa));
@@ -319,39 +362,44 @@ __device__ __forceinline__ float head_sum(float v) {
   return v;
 }
 
-// A warp's tokens, and which of their segments it takes.
+// A warp's tokens: first, first + step ... in `turns` turns, then, in a last one, segments [seg0, seg1) of the token `last`.
 struct Share {
-  int64_t token, step;
-  int seg0, seg1;
+  int64_t first, step, last;
+  int turns, seg0, seg1;
+  __device__ __forceinline__ int64_t token(int turn) const { return turn < turns ? first + turn * step : last; }
 };
 __device__ __forceinline__ Share share_of(const Args& a) {
   const unsigned warp = blockIdx.x * kWarps + (threadIdx.x >> 5), parts = a.parts;      // (a token's warps are neighbours)
-  const int part = static_cast<int>(warp % parts);
+  const unsigned mine = warp / parts;
+  const int part = static_cast<int>(warp - mine * parts);
   Share s;
-  s.step = gridDim.x * kWarps / parts;
-  s.token = warp < s.step * parts ? warp / parts : a.tokens;
+  s.first = warp;
+  s.step = gridDim.x * kWarps;
+  s.turns = a.turns;
+  s.last = a.turns * s.step + mine;
   s.seg0 = part * a.segments / a.parts;
-  s.seg1 = (part + 1) * a.segments / a.parts;
+  s.seg1 = mine < a.rest ? (part + 1) * a.segments / a.parts : 0;
   return s;
 }
 
-// All tokens' heads of one kind: a warp walks over its tokens and their segments [seg0, seg1) of this kind, the next segments' heads
-// (the next token's, behind the last) on their way to shared memory meanwhile.
+// All tokens' heads of one kind: a warp walks over its tokens and their segments of this kind (in the last turn [seg0, seg1)), the
+// next segments' heads (the next token's, behind the last) on their way to shared memory meanwhile.
 enum : int { kQueries = 0, kKeys = 1, kValues = 2 };
 template <typename T, int kLanes, bool kHalf, int kKind>
 __device__ __forceinline__ void forward_kind(const Args& a, const Place& p, const Share& share, int seg0, int seg1, uint4* ring) {
-  if (seg0 >= seg1 || share.token >= a.tokens) return;
+  const int turns = share.turns + (seg0 < seg1 ? 1 : 0);
+  if (turns == 0) return;
   constexpr int kGroups = 32 / kLanes, kHeads = kForwardHeads<T>, kRows = kGroups * kHeads;
   const int lane = threadIdx.x & 31;
   const T* in = static_cast<const T*>(kKind == kQueries ? a.q : kKind == kKeys ? a.k : a.v);
   const int64_t* strides = kKind == kQueries ? a.q_strides : kKind == kKeys ? a.k_strides : a.v_strides;
-  const int heads = kKind == kQueries ? a.heads : a.kv_heads;
+  const int heads = kKind == kQueries ? a.heads : a.kv_heads, segments = kKind == kQueries ? a.q_segments : a.kv_segments;
   constexpr int kVec = sizeof(T) / 2 * kThreads;        // places of eight elements
   // the segment that is asked for next, and its stage
-  int64_t ahead_token = share.token;
-  int ahead_seg = seg0, ahead = 0;
+  int64_t ahead_token = share.token(0);
+  int ahead_turn = 0, ahead_seg = share.turns > 0 ? 0 : seg0, ahead = 0;
   auto ask = [&]() {
-    if (ahead_token < a.tokens) {
+    if (ahead_turn < turns) {
       const int head = ahead_seg * kRows + lane / kLanes;
       const T* x = in + ahead_token * strides[0] + head * strides[1];
       uint4* to = ring + ahead * (2 * kHeads * kVec);
@@ -361,9 +409,10 @@ __device__ __forceinline__ void forward_kind(const Args& a, const Place& p, cons
         copy_vec(to + (2 * i) * kVec, there && p.has_a ? x + p.a : in, there && p.has_a);
         copy_vec(to + (2 * i + 1) * kVec, there && p.has_b ? x + p.b : in, there && p.has_b);
       }
-      if (++ahead_seg == seg1) {
-        ahead_seg = seg0;
-        ahead_token += share.step;
+      if (++ahead_seg == (ahead_turn < share.turns ? segments : seg1)) {
+        ++ahead_turn;
+        ahead_seg = ahead_turn < share.turns ? 0 : seg0;
+        ahead_token = share.token(ahead_turn);
       }
     }
     copies_commit();
@@ -372,9 +421,11 @@ __device__ __forceinline__ void forward_kind(const Args& a, const Place& p, cons
 #pragma unroll
   for (int i = 0; i < kForwardStages - 1; ++i) ask();
   int stage = 0;
-  int64_t place = position_of(a, share.token);
-  for (int64_t token = share.token; token < a.tokens; token += share.step) {
-    const int64_t next_token = token + share.step;
+  int64_t place = position_of(a, share.token(0));
+  for (int i_turn = 0; i_turn < turns; ++i_turn) {
+    const int64_t token = share.token(i_turn);
+    int seg = i_turn < share.turns ? 0 : seg0;
+    const int seg_end = i_turn < share.turns ? segments : seg1;
     const bool valid = place >= 0 && place < a.places;
     const int slot = kKind != kQueries && a.slots != nullptr ? a.slots[token] : 0;
     Turn t;
@@ -387,7 +438,7 @@ __device__ __forceinline__ void forward_kind(const Args& a, const Place& p, cons
       t.sa = mul(t.sa, kHalf ? wb : swapped(wa));
       t.sb = mul(t.sb, kHalf ? wa : swapped(wb));
     }
-    if (next_token < a.tokens) place = position_of(a, next_token);
+    if (i_turn + 1 < turns) place = position_of(a, share.token(i_turn + 1));
     T* y = static_cast<T*>(kKind == kQueries ? a.qo : a.ko);
     int64_t y_head = kKind == kQueries ? a.qo_strides[1] : a.ko_strides[1], y_token = token * (kKind == kQueries ? a.qo_strides[0] : a.ko_strides[0]);
     bool written = valid;
@@ -400,10 +451,10 @@ __device__ __forceinline__ void forward_kind(const Args& a, const Place& p, cons
       y_head = (kKind == kKeys ? c.k_head : c.v_head) * 8;
       y_token = (kKind == kKeys ? page * c.k_page + in_page * c.k_token : page * c.v_page + in_page * c.v_token) * 8;
     }
-    int head = seg0 * kRows + lane / kLanes;
+    int head = seg * kRows + lane / kLanes;
     y += y_token + head * y_head;
     y_head *= kGroups;
-    for (int seg = seg0; seg < seg1; ++seg, head += kRows) {
+    for (; seg < seg_end; ++seg, head += kRows) {
       copies_wait<kForwardStages - 2>();
       Vec<T> xa[kHeads], xb[kHeads];
 #pragma unroll
@@ -443,36 +494,37 @@ __global__ void __launch_bounds__(kThreads, kForwardCtas) forward_kernel(const _
   const int first_k = a.q_segments, first_v = first_k + a.kv_segments;
   forward_kind<T, kLanes, kHalf, kQueries>(a, p, share, share.seg0, min(share.seg1, first_k), mine);
   forward_kind<T, kLanes, kHalf, kKeys>(a, p, share, max(share.seg0 - first_k, 0), min(share.seg1, first_v) - first_k, mine);
-  forward_kind<T, kLanes, kHalf, kValues>(a, p, share, max(share.seg0 - first_v, 0), share.seg1 - first_v, mine);
+  if (a.slots != nullptr) forward_kind<T, kLanes, kHalf, kValues>(a, p, share, max(share.seg0 - first_v, 0), share.seg1 - first_v, mine);
 }
 
 // The same for the gradients; each lane sums the gains' gradients of its columns in registers over all tokens of its warp, then the
-// CTA's lanes of the same columns are added in order and leave as one row of partial sums.
+// lanes of the same columns are added, the CTA's warps in order, and leave as one row of partial sums.  The weights stay in shared
+// memory, 16 registers a lane less: what 128 could not hold went to memory in the inner loop, 137 -> 128 us forward and backward.
 template <typename T, int kLanes, bool kHalf, int kKind>
-__device__ __forceinline__ void backward_kind(const Args& a, const Place& p, const Share& share, int seg0, int seg1, uint4* ring,
-                                              float (*sums)[kLanes * 16 + 4]) {
+__device__ __forceinline__ void backward_kind(const Args& a, const Place& p, const Share& share, int seg0, int seg1, uint4* ring, const float* weights, float* row) {
   constexpr int kGroups = 32 / kLanes, kHeads = kBackwardHeads, kRows = kGroups * kHeads;
   const int lane = threadIdx.x & 31;
   Pairs acc_a, acc_b;
 #pragma unroll
   for (int i = 0; i < 4; ++i) acc_a.v[i] = acc_b.v[i] = 0;
-  if (seg0 < seg1 && share.token < a.tokens) {
+  const int turns = share.turns + (seg0 < seg1 ? 1 : 0);
+  if (turns > 0) {
     const T* x_in = static_cast<const T*>(kKind == kQueries ? a.q : a.k);
     const T* g_in = static_cast<const T*>(kKind == kQueries ? a.gq : a.gk);
     T* out = static_cast<T*>(kKind == kQueries ? a.qo : a.ko);
     const int64_t* xs = kKind == kQueries ? a.q_strides : a.k_strides;
     const int64_t* gs = kKind == kQueries ? a.gq_strides : a.gk_strides;
     const int64_t* os = kKind == kQueries ? a.qo_strides : a.ko_strides;
-    const int heads = kKind == kQueries ? a.heads : a.kv_heads;
+    const int heads = kKind == kQueries ? a.heads : a.kv_heads, segments = kKind == kQueries ? a.q_segments : a.kv_segments;
     constexpr int kVec = sizeof(T) / 2 * kThreads, kStages = kBackwardStages<T>;
     const int64_t o_step = kGroups * os[1];
     struct Heads {
       Vec<T> xa, xb, ga, gb;
     };
-    int64_t ahead_token = share.token;
-    int ahead_seg = seg0, ahead = 0;
+    int64_t ahead_token = share.token(0);
+    int ahead_turn = 0, ahead_seg = share.turns > 0 ? 0 : seg0, ahead = 0;
     auto ask = [&]() {
-      if (ahead_token < a.tokens) {
+      if (ahead_turn < turns) {
         const int head = ahead_seg * kRows + lane / kLanes;
         const T* x = x_in + ahead_token * xs[0] + head * xs[1];
         const T* g = g_in + ahead_token * gs[0] + head * gs[1];
@@ -485,9 +537,10 @@ __device__ __forceinline__ void backward_kind(const Args& a, const Place& p, con
           copy_vec(to + 2 * kVec, has_a ? g + p.a : g_in, has_a);
           copy_vec(to + 3 * kVec, has_b ? g + p.b : g_in, has_b);
         }
-        if (++ahead_seg == seg1) {
-          ahead_seg = seg0;
-          ahead_token += share.step;
+        if (++ahead_seg == (ahead_turn < share.turns ? segments : seg1)) {
+          ++ahead_turn;
+          ahead_seg = ahead_turn < share.turns ? 0 : seg0;
+          ahead_token = share.token(ahead_turn);
         }
       }
       copies_commit();
@@ -496,17 +549,17 @@ __device__ __forceinline__ void backward_kind(const Args& a, const Place& p, con
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) ask();
     int stage = 0;
-    const void* gain = kKind == kQueries ? a.q_gain : a.k_gain;
-    const Pairs wa = load_weights<T>(a, gain, p.a, p.has_a), wb = load_weights<T>(a, gain, p.b, p.has_b);
-    int64_t place = position_of(a, share.token);
-    for (int64_t token = share.token; token < a.tokens; token += share.step) {
-      const int64_t next_token = token + share.step;
+    int64_t place = position_of(a, share.token(0));
+    for (int i_turn = 0; i_turn < turns; ++i_turn) {
+      const int64_t token = share.token(i_turn);
+      int seg = i_turn < share.turns ? 0 : seg0;
+      const int seg_end = i_turn < share.turns ? segments : seg1;
       const bool valid = place >= 0 && place < a.places;
-      const Turn t = turn_of<kHalf, true>(load_angles<kHalf>(a, p, valid ? place : 0));
-      if (next_token < a.tokens) place = position_of(a, next_token);
-      int head = seg0 * kRows + lane / kLanes;
+      const BackTurn<kHalf> turn_back(load_angles<kHalf>(a, p, valid ? place : 0));
+      if (i_turn + 1 < turns) place = position_of(a, share.token(i_turn + 1));
+      int head = seg * kRows + lane / kLanes;
       T* o = out + token * os[0] + head * os[1];
-      for (int seg = seg0; seg < seg1; ++seg, head += kRows) {
+      for (; seg < seg_end; ++seg, head += kRows) {
         copies_wait<kStages - 2>();
         Heads now[kHeads];
 #pragma unroll
@@ -521,8 +574,8 @@ __device__ __forceinline__ void backward_kind(const Args& a, const Place& p, con
           if (seg * kRows + i * kGroups >= heads) break;                  // (uniform in the warp: shuffles)
           const Pairs fa = now[i].xa.get(), fb = now[i].xb.get();
           Pairs ha, hb;
-          turn<kHalf>(t, now[i].ga.get(), now[i].gb.get(), &ha, &hb);
-          const Pairs ua = mul(ha, wa), ub = mul(hb, wb);
+          turn_back(now[i].ga.get(), now[i].gb.get(), &ha, &hb);
+          const Pairs ua = mul(ha, eight(weights + p.a)), ub = mul(hb, eight(weights + p.b));
           const float square = head_sum<kLanes>(dot(fa, fa) + dot(fb, fb)), along = head_sum<kLanes>(dot(ua, fa) + dot(ub, fb));
           const float r = rsqrtf(square * a.inv_size + a.eps);
           if (head + i * kGroups >= heads) continue;
@@ -544,30 +597,44 @@ __device__ __forceinline__ void backward_kind(const Args& a, const Place& p, con
     copies_wait<0>();
   }
   if (!a.with_gains) return;
-  __syncthreads();
-  float* row = sums[(threadIdx.x >> 5) * kGroups + lane / kLanes];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if (p.has_a) ptx::f32x2_split(acc_a.v[i], row[p.a + 2 * i], row[p.a + 2 * i + 1]);
-    if (p.has_b) ptx::f32x2_split(acc_b.v[i], row[p.b + 2 * i], row[p.b + 2 * i + 1]);
-  }
-  __syncthreads();
-  for (int column = threadIdx.x; column < a.head_chunks * 8; column += kThreads) {
-    float v = 0.0f;
-#pragma unroll 4
-    for (int i = 0; i < kWarps * kGroups; ++i) v += sums[i][column];
-    a.partial[(static_cast<int64_t>(blockIdx.x) * 2 + kKind) * 256 + column] = v;
+    float x[4];
+    ptx::f32x2_split(acc_a.v[i], x[0], x[1]);
+    ptx::f32x2_split(acc_b.v[i], x[2], x[3]);
+#pragma unroll
+    for (int o = kLanes; o < 32; o *= 2) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] += __shfl_xor_sync(0xffffffffu, x[e], o);
+    }
+    if (lane < kLanes && p.has_a) *reinterpret_cast<float2*>(row + p.a + 2 * i) = make_float2(x[0], x[1]);
+    if (lane < kLanes && p.has_b) *reinterpret_cast<float2*>(row + p.b + 2 * i) = make_float2(x[2], x[3]);
   }
 }
 template <typename T, int kLanes, bool kHalf>
 __global__ void __launch_bounds__(kThreads, kBackwardCtas) backward_kernel(const __grid_constant__ Args a) {
   ptx::grid_dependency_sync();
-  __shared__ float sums[kWarps * (32 / kLanes)][kLanes * 16 + 4];
+  __shared__ __align__(16) float sums[2][kWarps][kLanes * 16];
   __shared__ uint4 ring[kBackwardStages<T> * 4 * kBackwardHeads * (sizeof(T) / 2) * kThreads];
+  __shared__ __align__(16) float weights[2][kLanes * 16];       // gain_offset + gain, of queries and of keys
+  for (int i = threadIdx.x; i < 2 * kLanes * 16; i += kThreads) {
+    const int kind = i / (kLanes * 16), column = i - kind * (kLanes * 16);
+    weights[kind][column] = weight_of<T>(a, kind ? a.k_gain : a.q_gain, column);
+  }
+  __syncthreads();
   const Place p = place_of<kLanes>(a, threadIdx.x & 31);
   const Share share = share_of(a);
-  backward_kind<T, kLanes, kHalf, kQueries>(a, p, share, share.seg0, min(share.seg1, a.q_segments), ring + threadIdx.x, sums);
-  backward_kind<T, kLanes, kHalf, kKeys>(a, p, share, max(share.seg0 - a.q_segments, 0), share.seg1 - a.q_segments, ring + threadIdx.x, sums);
+  backward_kind<T, kLanes, kHalf, kQueries>(a, p, share, share.seg0, min(share.seg1, a.q_segments), ring + threadIdx.x, weights[0], sums[0][threadIdx.x >> 5]);
+  backward_kind<T, kLanes, kHalf, kKeys>(a, p, share, max(share.seg0 - a.q_segments, 0), share.seg1 - a.q_segments, ring + threadIdx.x, weights[1], sums[1][threadIdx.x >> 5]);
+  if (!a.with_gains) return;
+  __syncthreads();           // (the only one: a CTA's warps may have unlike numbers of queries and of keys)
+  for (int i = threadIdx.x; i < 2 * a.head_chunks * 8; i += kThreads) {
+    const int kind = i >= a.head_chunks * 8, column = i - kind * a.head_chunks * 8;
+    float v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) v += sums[kind][w][column];
+    a.partial[(static_cast<int64_t>(blockIdx.x) * 2 + kind) * 256 + column] = v;
+  }
 }
 
 // The CTAs' rows of partial sums added up: 32 columns a CTA, 32 threads a column, then a tree over them.
@@ -579,8 +646,17 @@ __global__ void __launch_bounds__(1024) gains_kernel(const float* partial, int r
   const int blocks = (size + 31) / 32;
   const int which = blockIdx.x / blocks, column = (blockIdx.x - which * blocks) * 32 + lane;
   float v = 0.0f;
-  if (column < size)
-    for (int r = warp; r < rows; r += 32) v += partial[(static_cast<int64_t>(r) * 2 + which) * 256 + column];
+  constexpr int kAtOnce = 10;          // loads in flight (592 rows: two turns)
+  for (int r0 = warp; r0 < rows; r0 += 32 * kAtOnce) {
+    float x[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int r = r0 + 32 * i;
+      x[i] = column < size && r < rows ? partial[(static_cast<int64_t>(r) * 2 + which) * 256 + column] : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) v += x[i];
+  }
   part[lane][warp] = v;
   __syncthreads();
   v = part[warp][lane];
@@ -659,16 +735,20 @@ Args base_args(const ixk_qk_desc* d) {
 
 int lanes_for(int head_size) { return head_size <= 64 ? 4 : head_size <= 128 ? 8 : 16; }
 
-// The segments of a token (of `rows` heads), and over how many warps they go: one, unless tokens are too few to fill the GPU.  (More,
-// so that 3.46 turns of the warps become 6.92 in two parts, cost more than the idle half turn: 8192 x 32 heads of 256 forward and
-// backward 129 -> 136 us.)
-void split_heads(Args* a, int rows, bool with_v, int64_t warps) {
+// The segments of a token (of `rows` heads), and how tokens go over as many warps as are on the GPU at one time: whole turns of a
+// token a warp, then a last one in which several warps share a token if there are enough (8192 tokens of 16 + 16 heads of 256, 3.46
+// turns: forward 51.4 -> 48.4 us; all tokens in two parts, 6.92 turns, were slower than 4 whole ones).  Equal runs of segments
+// instead, whatever their kind, leave warps with nothing but keys, of which a token has few: 68 -> 96 us for 16384 tokens of 32 + 8 heads.
+int64_t split(Args* a, int rows, bool with_v, int64_t most) {
   a->q_segments = (a->heads + rows - 1) / rows;
   a->kv_segments = (a->kv_heads + rows - 1) / rows;
   a->segments = a->q_segments + a->kv_segments * (with_v ? 2 : 1);
-  a->parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(a->segments, warps / std::max<int64_t>(a->tokens, 1))));
+  const int64_t warps = most * kWarps;
+  a->turns = static_cast<int>(a->tokens / warps);
+  a->rest = a->tokens - a->turns * warps;
+  a->parts = a->rest == 0 ? 1 : static_cast<int>(std::min<int64_t>(a->segments, warps / a->rest));
+  return a->turns > 0 ? most : std::max<int64_t>(1, (a->tokens * a->parts + kWarps - 1) / kWarps);
 }
-int64_t ctas_for(const Args& a, int64_t most) { return std::max<int64_t>(1, std::min((a.tokens * a.parts + kWarps - 1) / kWarps, most)); }
 int forward_heads(int dtype) { return dtype == IXK_F32 ? kForwardHeads<float> : kForwardHeads<__half>; }
 
 template <template <typename, int> class Launcher, typename... More>
@@ -683,14 +763,14 @@ int dispatch(int dtype, int lanes, const More&... more) {
 }
 template <typename T, int kLanes>
 struct Forward {
-  static int run(const Args& a, unsigned grid, cudaStream_t s) { 
+  static int run(const Args& a, unsigned grid, cudaStream_t s) {
     return a.interleaved ? launch_overlapped(forward_kernel<T, kLanes, false>, dim3(grid), dim3(kThreads), 0, s, a)
                          : launch_overlapped(forward_kernel<T, kLanes, true>, dim3(grid), dim3(kThreads), 0, s, a);
   }
 };
 template <typename T, int kLanes>
 struct Backward {
-  static int run(const Args& a, unsigned grid, cudaStream_t s) { 
+  static int run(const Args& a, unsigned grid, cudaStream_t s) {
     return a.interleaved ? launch_overlapped(backward_kernel<T, kLanes, false>, dim3(grid), dim3(kThreads), 0, s, a)
                          : launch_overlapped(backward_kernel<T, kLanes, true>, dim3(grid), dim3(kThreads), 0, s, a);
   }
@@ -750,17 +830,14 @@ int ixk_qk_norm_rotary_fwd(const ixk_qk_desc* d, const void* q, const void* k, c
     a.cache = paged::cache_args(cache, k_pages, v_pages);
     a.slots = slots;
   }
-  const int64_t most = static_cast<int64_t>(info.sm_count) * qk::kForwardCtas;
-  qk::split_heads(&a, 32 / lanes * qk::forward_heads(d->dtype), paged, most * qk::kWarps);
-  const int64_t grid = qk::ctas_for(a, most);
+  const int64_t grid = qk::split(&a, 32 / lanes * qk::forward_heads(d->dtype), paged, static_cast<int64_t>(info.sm_count) * qk::kForwardCtas);
   return qk::dispatch<qk::Forward>(d->dtype, lanes, a, static_cast<unsigned>(grid), static_cast<cudaStream_t>(cuda_stream));
 }
 
 size_t ixk_qk_norm_rotary_bwd_workspace_bytes(const ixk_qk_desc* d) {
   if (qk::check(d, "qk_norm_rotary") != IXK_OK) return 0;
   qk::Args a = qk::base_args(d);
-  qk::split_heads(&a, 32 / qk::lanes_for(d->head_size) * qk::kBackwardHeads, false, qk::kMaxBwdCtas * qk::kWarps);
-  return static_cast<size_t>(qk::ctas_for(a, qk::kMaxBwdCtas)) * 2 * 256 * sizeof(float);
+  return static_cast<size_t>(qk::split(&a, 32 / qk::lanes_for(d->head_size) * qk::kBackwardHeads, false, qk::kMaxBwdCtas)) * 2 * 256 * sizeof(float);
 }
 
 int ixk_qk_norm_rotary_bwd(const ixk_qk_desc* d, const void* grad_q, const void* grad_k, const void* q, const void* k, const void* q_gain,
@@ -802,8 +879,7 @@ int ixk_qk_norm_rotary_bwd(const ixk_qk_desc* d, const void* grad_q, const void*
   a.partial = static_cast<float*>(workspace);
   a.with_gains = gains;
   const int lanes = qk::lanes_for(d->head_size);
-  qk::split_heads(&a, 32 / lanes * qk::kBackwardHeads, false, qk::kMaxBwdCtas * qk::kWarps);
-  const int ctas = static_cast<int>(qk::ctas_for(a, qk::kMaxBwdCtas));
+  const int ctas = static_cast<int>(qk::split(&a, 32 / lanes * qk::kBackwardHeads, false, qk::kMaxBwdCtas));
   auto s = static_cast<cudaStream_t>(cuda_stream);
   if (int st = qk::dispatch<qk::Backward>(d->dtype, lanes, a, static_cast<unsigned>(ctas), s)) return st;
   if (!gains) return IXK_OK;
