@@ -272,3 +272,35 @@ def test_replayed_on_another_stream_and_without_native_calls(pkg, cuda, monkeypa
         _, granted, _ = a.extend(new.tolist(), 25)
         a.keep(granted, kept.tolist(), path.tolist())
     assert lengths.tolist() == a.lengths and count.item() == len(a.free) and free[:len(a.free)].tolist() == a.free
+
+
+def test_paths_that_name_an_entry_twice_or_go_back(pkg, cuda):
+    """Such a path ends before the entry; what it kept so far moves."""
+    table, lengths, free, count = ints(cuda, [[0, 1], [2, 3], [4, 5]]), ints(cuda, [3, 0, 2]), ints(cuda, [-1] * 6), ints(cuda, [0])
+    granted, kept, path = ints(cuda, [5, 5, 5]), ints(cuda, [4, 4, 4]), ints(cuda, [[1, 1, 2, 3], [0, 3, 2, 4], [2, 3, 5, 4]])
+    k, v = torch.randn(2, 2, 6, 4, 1, 8, device=cuda).half()
+    flat = [t.clone().view(2, 24, 8) for t in (k, v)]
+    for t, before in zip(flat, [t.clone() for t in flat]):
+        for to, source in ((3, 4), (9, 11), (18, 20), (19, 21)):
+            t[:, to] = before[:, source]
+    after, left = pkg.paged_keep(table, lengths, granted, kept, free, count, page_size=4, path=path, k_pages=k, v_pages=v)
+    assert after.tolist() == [4, 2, 4] and torch.equal(k.view(2, 24, 8), flat[0]) and torch.equal(v.view(2, 24, 8), flat[1])
+    assert left.item() == 3 and free.tolist() == [1, 3, 5, -1, -1, -1]
+
+
+def test_a_cache_of_more_than_2_to_the_31_elements(pkg, cuda):
+    """Norm and rotation into its last page, and a move there."""
+    pages, page = 2 ** 31 // (16 * 8 * 64) + 40, 16
+    k = torch.empty(pages, page, 8, 64, dtype=torch.bfloat16, device=cuda)
+    v = torch.empty_like(k)
+    q, kk, vv = (torch.randn(3, n, 64, device=cuda).bfloat16() for n in (8, 8, 8))
+    cos, sin = torch.ones(20, 8, device=cuda), torch.zeros(20, 8, device=cuda)
+    last = pages - 1
+    slots = ints(cuda, [last * page + i for i in (9, 11, 14)])
+    pkg.qk_norm_rotary_forward(q, kk, cos=cos, sin=sin, positions=ints(cuda, [9, 11, 14]), v=vv, slots=slots, k_pages=k, v_pages=v)
+    _, dense = pkg.qk_norm_rotary_forward(q, kk, cos=cos, sin=sin, positions=ints(cuda, [9, 11, 14]))
+    assert torch.equal(k[last, [9, 11, 14]], dense) and torch.equal(v[last, [9, 11, 14]], vv)
+    after, left = pkg.paged_keep(ints(cuda, [[last]]), ints(cuda, [9]), ints(cuda, [7]), ints(cuda, [3]), torch.zeros(pages, dtype=torch.int32, device=cuda),
+                                 ints(cuda, [0]), page_size=page, path=ints(cuda, [[0, 2, 5]]), k_pages=k, v_pages=v)
+    assert after.item() == 12 and left.item() == 0
+    assert torch.equal(k[last, 9:12], dense) and torch.equal(v[last, 9:12], vv)

@@ -263,3 +263,51 @@ def test_captured_steps(pkg, cuda):
             assert torch.equal(getattr(eager.cache, name), getattr(captured.cache, name))
         eager.read(x, step.row_start.tolist(), step.granted.tolist(), kept, path)
         assert eager.cache.lengths.tolist() == [len(t) for t in eager.text]
+
+
+@pytest.mark.gpu
+def test_two_servers_at_once(pkg, cuda):
+    """Two batches on two streams, their steps on the GPU at one time: the bits of each alone."""
+    layers = importlib.import_module(pkg.__name__ + ".layers")
+    ops = layers.KernelOps(pkg)
+    ws = [layers.GroupedLayerWeights.shard({k: v.to(cuda) for k, v in w.items()}, HEADS, KV, HD, 0, 1) for w in weights(torch.bfloat16)]
+
+    def steps(seed):
+        server = Server(layers, torch.bfloat16, cuda, seed=seed, pages=90)
+        work = []
+        for _ in range(6):
+            x, new, positions, mask, lines = server.draw(203, 40)
+            kept, path = server.choose(lines, new)
+            start = [sum(new[:b]) for b in range(len(new))]
+            work.append((x.to(cuda), server.ints(new), server.ints(positions), mask.to(cuda), server.ints(kept), path.to(cuda)))
+            server.read(x, start, new, kept, path)
+        return server, work
+
+    def go(server, work):
+        results = []
+        for x, new, positions, mask, kept, path in work:
+            y, step = layers.paged_step(x, ws, server.cache, new, ops, rope=server.rope, positions=positions, mask=mask)
+            layers.paged_accept_(server.cache, step, kept, ops, path=path)
+            results += [y, step.slot, server.cache.lengths.clone()]
+        return results
+
+    alone = [go(*steps(seed)) for seed in (1, 2)]
+    both = [steps(seed) for seed in (1, 2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        results = []
+        for server, _ in both:
+            server.cache.lengths.zero_()
+            server.cache.free_count.fill_(90)
+            server.cache.free_pages.copy_(torch.arange(89, -1, -1))
+            server.cache.page_table.fill_(-1)
+        torch.cuda.synchronize()
+        for s, (server, work) in zip(streams, both):
+            with torch.cuda.stream(s):
+                torch.cuda._sleep(6000000)           # (both streams' work is there before either begins)
+                results.append(go(server, work))
+        torch.cuda.synchronize()
+        for one, other in zip(alone, results):
+            for a, b in zip(one, other):
+                assert torch.equal(a, b)
