@@ -797,7 +797,9 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           args.meta[(walk.b * args.kv_heads + walk.kv_head) * args.tile_blocks + walk.t0 / args.block_tokens] = begun;
       }
       if (warp_ok) {
-        const float inv_l = 1.0f / r_run;
+        // (nothing seen: its products are sums of 0 times numbers)
+        const float inv_l = r_run == 0.0f ? 0.0f : __fdividef(1.0f, r_run);
+        const uint64_t inv2 = ptx::f32x2(inv_l, inv_l);
         uint16_t* out_row = args.out + q_row * args.o_strides[0] + head * args.o_strides[1];
         float* part_row = args.part_o + (part * (kHeadDim / 4) * args.part_rows + row) * 4;
         const int64_t part_pitch = static_cast<int64_t>(args.part_rows) * 4;
@@ -811,8 +813,11 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           if (!row_ok) continue;
           if (whole) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              o[i] = r_run == 0.0f ? 0u : pack2<kBf16>(__uint_as_float(o[2 * i]) * inv_l, __uint_as_float(o[2 * i + 1]) * inv_l);
+            for (int i = 0; i < 32; ++i) {
+              float x, y;
+              ptx::f32x2_split(ptx::mul2(ptx::f32x2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), inv2), x, y);
+              o[i] = pack2<kBf16>(x, y);
+            }
             if (args.out_sectors) {
 #pragma unroll
               for (int e = 0; e < 4; ++e)
