@@ -1104,7 +1104,7 @@ def paged_extend(page_table: torch.Tensor, lengths: torch.Tensor, new_tokens: to
     if _NATIVE is not None:
         r = _NATIVE.paged_extend(page_table, lengths, new_tokens, free_pages, free_count, rows, page_size, out, stream)
         if r is not None:
-            return PagedRows(*_native_result(r))
+            return tuple.__new__(PagedRows, _native_result(r))      # (PagedRows(*...), without the way through its arguments)
     _require_here(page_table, lengths, new_tokens, free_pages, free_count, *(out or ()))
     d = _page_pool(page_table, lengths, free_pages, free_count, page_size)
     _int32("new_tokens", new_tokens, d.requests)

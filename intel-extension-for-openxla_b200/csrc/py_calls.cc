@@ -8,9 +8,11 @@
 // answers with None and leaves to the twin, which also words the errors.  Nothing is kept from one call to the next.
 #include <Python.h>
 
+#include <ATen/EmptyTensor.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/DispatchKeySet.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -659,6 +661,11 @@ IXK_PY_END
 
 // ------------------------------------------------------------------------------------------------ a paged cache
 
+// A new dense tensor on the current device (on which `here` has found the operands), from the same pool as any other's, without the way
+// through the dispatcher, which costs half as much as the launch.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type) {
+  return at::Tensor(at::detail::empty_generic(sizes, c10::cuda::CUDACachingAllocator::get(), c10::DispatchKeySet(c10::DispatchKey::CUDA), type, std::nullopt));
+}
 // A vector of `n` elements from element `at` of a tensor's memory on.
 at::Tensor piece(const at::Tensor& whole, int64_t at, int64_t n) {
   at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
@@ -721,12 +728,12 @@ bool paged_cache(const at::Tensor* k, const at::Tensor* v, bool layers, ixk_page
 
 // page_table, lengths, new_tokens, free_pages, free_count, rows, page_size, out, stream
 IXK_PY_FUNCTION(py_paged_extend, 9)
-  const at::Tensor *table = tensor(a[0]), *lengths = tensor(a[1]), *fresh = tensor(a[2]), *pages = tensor(a[3]), *count = tensor(a[4]);
+  const at::Tensor *table = tensor(a[0]), *lengths = tensor(a[1]), *added = tensor(a[2]), *pages = tensor(a[3]), *count = tensor(a[4]);
   int64_t rows, page_size;
   void* stream;
   ixk_page_pool d;
   if (table == nullptr || !integer(a[5], &rows) || !integer(a[6], &page_size) || rows < 0 || !stream_arg(a[8], &stream) ||
-      !page_pool(table, lengths, pages, count, page_size, &d) || !ints(fresh, d.requests) || !here({table, lengths, fresh, pages, count}))
+      !page_pool(table, lengths, pages, count, page_size, &d) || !ints(added, d.requests) || !here({table, lengths, added, pages, count}))
     Py_RETURN_NONE;
   const int64_t shapes[6] = {d.requests + 1, d.requests, rows, rows, rows, 1};
   at::Tensor made[6], whole;
@@ -737,7 +744,7 @@ IXK_PY_FUNCTION(py_paged_extend, 9)
     // six small results in one piece of memory, each from a 256-byte boundary on: six allocations would cost more than the kernel
     int64_t at[7] = {0};
     for (int i = 0; i < 6; ++i) at[i + 1] = at[i] + (shapes[i] + 63) / 64 * 64;
-    whole = like(*lengths, {at[6]}, at::kInt);
+    whole = fresh({at[6]}, at::kInt);
     for (int i = 0; i < 6; ++i) {
       made[i] = piece(whole, at[i], shapes[i]);
       o[i] = &made[i];
@@ -750,7 +757,7 @@ IXK_PY_FUNCTION(py_paged_extend, 9)
       if (!ints(o[i], shapes[i]) || !here({o[i]})) Py_RETURN_NONE;
     }
   }
-  int32_t *pt = ip(table), *pl = ip(lengths), *pn = ip(fresh), *pp = ip(pages), *pc = ip(count), *r[6];
+  int32_t *pt = ip(table), *pl = ip(lengths), *pn = ip(added), *pp = ip(pages), *pc = ip(count), *r[6];
   for (int i = 0; i < 6; ++i) r[i] = ip(o[i]);
   const int st = unlocked([&] { return g_extend(&d, pl, pn, pt, pp, pc, r[5], r[1], r[0], rows, r[2], r[3], r[4], stream); });
   return results(st, {{given[0], &made[0]}, {given[1], &made[1]}, {given[2], &made[2]}, {given[3], &made[3]}, {given[4], &made[4]}, {given[5], &made[5]}});
@@ -772,13 +779,17 @@ IXK_PY_FUNCTION(py_paged_keep, 13)
   if (path != nullptr ? !int_rows(path) || path->size(0) != d.requests || !paged_cache(k, v, true, &c) : k != nullptr || v != nullptr) Py_RETURN_NONE;
   if ((lengths_out == nullptr || count_out == nullptr) && a[12] != Py_None) Py_RETURN_NONE;
   at::Tensor made_lengths, made_count;
-  if (lengths_out == nullptr) {
-    made_lengths = like(*lengths, {d.requests}, at::kInt);
-    lengths_out = &made_lengths;
-  }
-  if (count_out == nullptr) {
-    made_count = like(*lengths, {1}, at::kInt);
-    count_out = &made_count;
+  if (lengths_out == nullptr || count_out == nullptr) {      // in one piece of memory, as extend's
+    const int64_t own = lengths_out == nullptr ? (d.requests + 63) / 64 * 64 : 0;
+    const at::Tensor whole = fresh({own + (count_out == nullptr ? 1 : 0)}, at::kInt);
+    if (lengths_out == nullptr) {
+      made_lengths = piece(whole, 0, d.requests);
+      lengths_out = &made_lengths;
+    }
+    if (count_out == nullptr) {
+      made_count = piece(whole, own, 1);
+      count_out = &made_count;
+    }
   }
   if (!ints(lengths_out, d.requests) || !ints(count_out, 1)) Py_RETURN_NONE;
   int32_t *pt = ip(table), *pl = ip(lengths), *pg = ip(granted), *pk = ip(kept), *pp = ip(pages), *pc = ip(count), *ppath = ip(path),
@@ -846,11 +857,11 @@ IXK_PY_FUNCTION(py_qk_forward, 17)
   if (a[16] != Py_None && (qo == nullptr || (!paged && ko == nullptr))) Py_RETURN_NONE;
   at::Tensor made_q, made_k;
   if (qo == nullptr) {
-    made_q = like(*q, q->sizes(), q->scalar_type());
+    made_q = fresh(q->sizes(), q->scalar_type());
     qo = &made_q;
   }
   if (!paged && ko == nullptr) {
-    made_k = like(*k, k->sizes(), k->scalar_type());
+    made_k = fresh(k->sizes(), k->scalar_type());
     ko = &made_k;
   }
   if (!heads_view(qo, q->sizes(), q->scalar_type(), d.q_out_strides) || (ko != nullptr && !heads_view(ko, k->sizes(), q->scalar_type(), d.k_out_strides)))
@@ -879,22 +890,22 @@ IXK_PY_FUNCTION(py_qk_backward, 16)
   if (a[15] != Py_None && (dq == nullptr || dk == nullptr || gains)) Py_RETURN_NONE;
   at::Tensor made_q, made_k, dqg, dkg, scratch;
   if (dq == nullptr) {
-    made_q = like(*q, q->sizes(), q->scalar_type());
+    made_q = fresh(q->sizes(), q->scalar_type());
     dq = &made_q;
   }
   if (dk == nullptr) {
-    made_k = like(*k, k->sizes(), k->scalar_type());
+    made_k = fresh(k->sizes(), k->scalar_type());
     dk = &made_k;
   }
   if (!heads_view(dq, q->sizes(), q->scalar_type(), d.q_out_strides) || !heads_view(dk, k->sizes(), q->scalar_type(), d.k_out_strides)) Py_RETURN_NONE;
   if (gains) {      // (both in one piece of memory, 16-byte boundaries for heads of any size)
     const int64_t n = (q->size(2) + 7) / 8 * 8;
-    const at::Tensor both = like(*q, {2 * n}, (qg != nullptr ? qg : kg)->scalar_type());
+    const at::Tensor both = fresh({2 * n}, (qg != nullptr ? qg : kg)->scalar_type());
     if (qg != nullptr) dqg = piece(both, 0, q->size(2));
     if (kg != nullptr) dkg = piece(both, n, q->size(2));
   }
   if (gains && ws == nullptr) {
-    scratch = like(*q, {static_cast<int64_t>(g_qk_bwd_bytes(&d))}, at::kByte);
+    scratch = fresh({static_cast<int64_t>(g_qk_bwd_bytes(&d))}, at::kByte);
     ws = &scratch;
   }
   void *pgq = ptr(gq), *pgk = ptr(gk), *pq = ptr(q), *pk = ptr(k), *pqg = ptr(qg), *pkg = ptr(kg), *ppos = ptr(pos), *pdq = ptr(dq), *pdk = ptr(dk),
@@ -926,7 +937,7 @@ IXK_PY_FUNCTION(py_fmha_paged, 14)
   if (a[13] != Py_None && (out == nullptr || (want_lse && lse == nullptr) || ws == nullptr)) Py_RETURN_NONE;
   at::Tensor made, made_lse, scratch;
   if (out == nullptr) {
-    made = like(*q, q->sizes(), q->scalar_type());
+    made = fresh(q->sizes(), q->scalar_type());
     out = &made;
   }
   d.rows = q->size(0);
@@ -941,12 +952,12 @@ IXK_PY_FUNCTION(py_fmha_paged, 14)
   }
   if (!heads_view(q, q->sizes(), q->scalar_type(), d.q_strides) || !heads_view(out, q->sizes(), q->scalar_type(), d.o_strides)) Py_RETURN_NONE;
   if (lse == nullptr && want_lse) {
-    made_lse = like(*q, {d.rows, q->size(1)}, at::kFloat);
+    made_lse = fresh({d.rows, q->size(1)}, at::kFloat);
     lse = &made_lse;
   }
   if (lse != nullptr && (lse->scalar_type() != at::kFloat || lse->sizes() != q->sizes().slice(0, 2) || !lse->is_contiguous())) Py_RETURN_NONE;
   if (ws == nullptr) {
-    scratch = like(*q, {static_cast<int64_t>(g_paged_fwd_bytes(&d, &c))}, at::kByte);
+    scratch = fresh({static_cast<int64_t>(g_paged_fwd_bytes(&d, &c))}, at::kByte);
     ws = &scratch;
   }
   void *pq = ptr(q), *pk = ptr(k), *pv = ptr(v), *po = ptr(out), *pw = ptr(ws);
