@@ -327,7 +327,9 @@ __device__ __noinline__ void add_odd_values(const Args& a, int length, int b, in
   }
 }
 
-template <int kHeadDim, bool kBf16>
+// kLse: the sum of the unrounded weights is wanted as well.  (Without it an instruction of eight in the inner loop is gone: 512 requests of 10 to
+// 300 keys 54.7 -> 50.9 us.)
+template <int kHeadDim, bool kBf16, bool kLse>
 __global__ void __launch_bounds__(Cfg<kHeadDim>::kAllThreads, Cfg<kHeadDim>::kWorkers)
 fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                   const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ Args args) {
@@ -727,7 +729,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
               ptx::f32x2_split(ptx::fma2(ptx::f32x2(__uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1])), mult2, minus2), x0, x1);
               x0 = ptx::ex2_approx(x0);
               x1 = ptx::ex2_approx(x1);
-              total2 = ptx::add2(total2, ptx::f32x2(x0, x1));
+              if constexpr (kLse) total2 = ptx::add2(total2, ptx::f32x2(x0, x1));
               packed[i >> 1] = pack2<kBf16>(x0, x1);
               const float2 rounded = unpack2<kBf16>(packed[i >> 1]);
               round2 = ptx::add2(round2, ptx::f32x2(rounded.x, rounded.y));
@@ -735,8 +737,10 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             ptx::tmem_st_32x16(s_addr + c * 16, packed);
           }
           float t0, t1;
-          ptx::f32x2_split(total2, t0, t1);
-          l_run = l_run * alpha + (t0 + t1);
+          if constexpr (kLse) {
+            ptx::f32x2_split(total2, t0, t1);
+            l_run = l_run * alpha + (t0 + t1);
+          }
           ptx::f32x2_split(round2, t0, t1);
           r_run = r_run * alpha + (t0 + t1);
           ptx::tmem_st_wait();
@@ -841,7 +845,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         }
         if (row_ok) {
           if (!whole) args.part_stat[part * args.part_rows + row] = make_float4(m_run, l_run, r_run, 0.0f);
-          else if (args.lse != nullptr)
+          else if (kLse)
             args.lse[static_cast<int64_t>(q_row) * args.heads + head] = l_run == 0.0f ? -INFINITY : (m_run + log2f(l_run)) * kLn2;
           if (odd)
             add_odd_values<kBf16>(args, req.length, walk.b, walk.kv_head, token, q_row, max(first_unit * kKeys - req.length, 0),
@@ -1024,17 +1028,17 @@ int check(const ixk_fmha_paged_desc* d, const ixk_paged_cache* c) {
   return IXK_OK;
 }
 
-template <int kHeadDim, bool kBf16>
+template <int kHeadDim, bool kBf16, bool kLse>
 int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const Args& a, int device, int sm_count, cudaStream_t stream) {
   using C = Cfg<kHeadDim>;
   static std::atomic<uint64_t> allowed{0};      // devices on which the kernel may use its shared memory
   const uint64_t bit = 1ull << (device & 63);
   if ((allowed.load(std::memory_order_relaxed) & bit) == 0) {
-    IXK_CUDA_OK(cudaFuncSetAttribute(fmha_paged_kernel<kHeadDim, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
+    IXK_CUDA_OK(cudaFuncSetAttribute(fmha_paged_kernel<kHeadDim, kBf16, kLse>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
   const int w = workers(kHeadDim, sm_count);
-  if (int st = launch_overlapped(fmha_paged_kernel<kHeadDim, kBf16>, dim3(w), dim3(C::kAllThreads), C::kSmemBytes, stream, q, k, v, a)) return st;
+  if (int st = launch_overlapped(fmha_paged_kernel<kHeadDim, kBf16, kLse>, dim3(w), dim3(C::kAllThreads), C::kSmemBytes, stream, q, k, v, a)) return st;
   const unsigned blocks = static_cast<unsigned>((a.part_rows + kJoinRows - 1) / kJoinRows);
   if (a.tile_blocks != 0)
     return launch_overlapped(fmha_paged_join_many_kernel<kHeadDim, kBf16>, dim3(static_cast<unsigned>(a.requests) * a.kv_heads * a.tile_blocks, blocks, kHeadDim / 16),
@@ -1143,13 +1147,16 @@ int ixk_fmha_paged_fwd(const ixk_fmha_paged_desc* d, const ixk_paged_cache* c, c
   }
   auto s = static_cast<cudaStream_t>(cuda_stream);
   const int dim = fmha_paged::head_dim(c->head_size);
-  auto with = [&](auto bf16) {
-    constexpr bool kBf16 = decltype(bf16)::value;
-    if (dim == 64) return fmha_paged::launch<64, kBf16>(mq, mk, mv, a, info.device, info.sm_count, s);
-    if (dim == 128) return fmha_paged::launch<128, kBf16>(mq, mk, mv, a, info.device, info.sm_count, s);
-    return fmha_paged::launch<256, kBf16>(mq, mk, mv, a, info.device, info.sm_count, s);
+  auto with = [&](auto bf16, auto with_lse) {
+    constexpr bool kBf16 = decltype(bf16)::value, kLse = decltype(with_lse)::value;
+    if (dim == 64) return fmha_paged::launch<64, kBf16, kLse>(mq, mk, mv, a, info.device, info.sm_count, s);
+    if (dim == 128) return fmha_paged::launch<128, kBf16, kLse>(mq, mk, mv, a, info.device, info.sm_count, s);
+    return fmha_paged::launch<256, kBf16, kLse>(mq, mk, mv, a, info.device, info.sm_count, s);
   };
-  return c->dtype == IXK_BF16 ? with(std::true_type{}) : with(std::false_type{});
+  const std::true_type yes;
+  const std::false_type no;
+  if (lse != nullptr) return c->dtype == IXK_BF16 ? with(yes, yes) : with(no, yes);
+  return c->dtype == IXK_BF16 ? with(yes, no) : with(no, no);
 }
 
 }  // extern "C"
