@@ -474,6 +474,12 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   walk.table_count = min(kTable, args.requests - walk.table_base);
   walk.begin(args, count > 0 ? *start_request : 0, count > 0 ? *start_offset : 0, count);
 
+  auto load_q = [&](const Walk& at) {
+    ptx::mbar_expect_tx(q_full, static_cast<uint32_t>(C::kChunks * args.group * args.block_tokens * 128));
+#pragma unroll
+    for (int c = 0; c < C::kChunks; ++c)
+      ptx::tma_load_3d(q_smem + c * C::kQChunkBytes, &tmap_q, q_full, c * kChunkElems, at.kv_head * args.group, at.req.row0 + at.t0);
+  };
   if (warp == kCopyWarp || (C::kTwoCopyWarps && warp == kCopyVWarp)) {
     // ------------------------------------------------------------------ copies: a page's 64 columns at a time
     const int box_keys = min(kKeys, 1 << args.page_shift);
@@ -510,22 +516,17 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
                          at.kv_head, (at.unit * kKeys) & ((1 << args.page_shift) - 1), page, at.req.rows > args.block_tokens ? again : once);
     };
     Walk k_walk = walk, v_walk = walk;
-    uint32_t tiles = 0, k_units = 0, v_units = 0;
+    uint32_t tiles = 1, k_units = 0, v_units = 0;       // (the first tile's Q: by the warp of the products)
     int next_pages = 0, pages0 = 0, pages1 = 0;
     auto load_k = [&]() {
-      if (k_walk.starts()) {       // a new tile: Q, once the products of the one before have read theirs
+      load_unit(k_walk, k_units < 2 ? k_units : 2 * k_units - 1, next_pages, &tmap_k);
+      // a new tile: Q, once the products of the one before have read theirs (behind its first keys, which then are on their way already)
+      if (alive && k_units > 0 && k_walk.starts()) {
         if (!wait(q_empty, (tiles & 1u) ^ 1u, kSiteLoadQ)) return;
         ++tiles;
-        if (lane == 0) {
-          ptx::mbar_expect_tx(q_full, static_cast<uint32_t>(C::kChunks * args.group * args.block_tokens * 128));
-#pragma unroll
-          for (int c = 0; c < C::kChunks; ++c)
-            ptx::tma_load_3d(q_smem + c * C::kQChunkBytes, &tmap_q, q_full, c * kChunkElems, k_walk.kv_head * args.group,
-                             k_walk.req.row0 + k_walk.t0);
-        }
+        if (lane == 0) load_q(k_walk);
         __syncwarp();
       }
-      load_unit(k_walk, k_units < 2 ? k_units : 2 * k_units - 1, next_pages, &tmap_k);
       // (in one warp V follows K by two units at most)
       if (k_units == v_units) pages0 = next_pages;
       else pages1 = next_pages;
@@ -556,6 +557,9 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------------ products (all lanes; one elected per instruction)
+    // The first tile's Q, while the copy warp looks up pages.
+    if (lane == 0 && !walk.done()) load_q(walk);
+    __syncwarp();
     constexpr uint32_t fmt = kBf16 ? 1u : 0u;
     const uint32_t idesc_s = ptx::umma_idesc(fmt, fmt, 0, 0, kRows, kKeys) | (args.negate ? 1u << 13 : 0u);      // (bit 13: A negated)
     const uint32_t idesc_o = ptx::umma_idesc(fmt, fmt, 0, 1, kRows, kHeadDim);
