@@ -292,8 +292,9 @@ __device__ __forceinline__ uint32_t finite_test(uint32_t acc, uint32_t w) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 // The rare case, kept out of the way: a stretch of V in shared memory with its NaN and infinities made zeros.
-__device__ __noinline__ void clear_odd_values(uint4* v, int pieces, int stride, int first, uint32_t expo) {
-  for (int i = first; i < pieces; i += stride) {
+__device__ __noinline__ void clear_odd_values(uint4* v, int begin, int pieces, int stride, int first, int pitch, uint32_t expo) {
+  for (int n = first; n < pieces; n += stride) {
+    const int i = ((begin + n) >> 6) * pitch + ((begin + n) & 63);
     const uint4 w = v[i];
     uint32_t words[4] = {w.x, w.y, w.z, w.w};
     for (int e = 0; e < 4; ++e) {
@@ -329,7 +330,10 @@ __device__ __noinline__ void add_odd_values(const Args& a, int length, int b, in
 
 // kLse: the sum of the unrounded weights is wanted as well.  (Without it an instruction of eight in the inner loop is gone: 512 requests of 10 to
 // 300 keys 54.7 -> 50.9 us.)
-template <int kHeadDim, bool kBf16, bool kLse>
+// kGroups: small pages.  A copy brings 8 keys, all 64-column chunks of them, and a slot is [8-key group][chunk][8 keys]; otherwise a copy
+// brings a page's (at most 64) keys of one chunk, and a slot is [chunk][keys].  Copies are what a unit waits for where there are more
+// than 8 of K or of V: 48 requests of 300 to 12000 keys in pages of 8 at head size 128 70 -> 57 us, at 256 88 -> 75.
+template <int kHeadDim, bool kBf16, bool kLse, bool kGroups>
 __global__ void __launch_bounds__(Cfg<kHeadDim>::kAllThreads, Cfg<kHeadDim>::kWorkers)
 fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                   const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ Args args) {
@@ -482,9 +486,10 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   };
   if (warp == kCopyWarp || (C::kTwoCopyWarps && warp == kCopyVWarp)) {
     // ------------------------------------------------------------------ copies: a page's 64 columns at a time
-    const int box_keys = min(kKeys, 1 << args.page_shift);
+    const int box_keys = kGroups ? 8 : min(kKeys, 1 << args.page_shift);
     const int pieces = kKeys / box_keys;
-    const int piece = lane / C::kChunks, chunk = lane - piece * C::kChunks;
+    const int piece = kGroups ? lane : lane / C::kChunks, chunk = kGroups ? 0 : lane - piece * C::kChunks;
+    const int to = piece * box_keys * 128 * (kGroups ? C::kChunks : 1) + chunk * C::kKvChunkBytes;
     // Keys and values that one tile reads leave L2 first: books, page table, Q and the parts in scratch stay (64 trees of 16 over 1024 to
     // 4096 keys 62.9 -> 57.3 us, 24 ragged ones at head size 256 73 -> 69.3).
     const uint64_t once = ptx::l2_evict_first(), again = ptx::l2_evict_normal();
@@ -511,9 +516,11 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       if (!wait(kv_empty(slot), ((load / kSlots) & 1u) ^ 1u, kSiteLoadKV)) return;
       if (lane == 0) ptx::mbar_expect_tx(kv_full(slot), C::kSlotBytes);
       __syncwarp();
-      if (piece < pieces)
-        ptx::tma_load_4d(kv_smem + slot * C::kSlotBytes + chunk * C::kKvChunkBytes + piece * box_keys * 128, map, kv_full(slot), chunk * kChunkElems,
-                         at.kv_head, (at.unit * kKeys) & ((1 << args.page_shift) - 1), page, at.req.rows > args.block_tokens ? again : once);
+      if (piece < pieces) {
+        const int in_page = (at.unit * kKeys + (kGroups ? piece * box_keys : 0)) & ((1 << args.page_shift) - 1);
+        ptx::tma_load_4d(kv_smem + slot * C::kSlotBytes + to, map, kv_full(slot), chunk * kChunkElems, kGroups ? in_page : at.kv_head,
+                         kGroups ? at.kv_head * C::kChunks : in_page, page, at.req.rows > args.block_tokens ? again : once);
+      }
     };
     Walk k_walk = walk, v_walk = walk;
     uint32_t tiles = 1, k_units = 0, v_units = 0;       // (the first tile's Q: by the warp of the products)
@@ -563,8 +570,11 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     constexpr uint32_t fmt = kBf16 ? 1u : 0u;
     const uint32_t idesc_s = ptx::umma_idesc(fmt, fmt, 0, 0, kRows, kKeys) | (args.negate ? 1u << 13 : 0u);      // (bit 13: A negated)
     const uint32_t idesc_o = ptx::umma_idesc(fmt, fmt, 0, 1, kRows, kHeadDim);
-    const uint64_t kmajor = ptx::umma_smem_desc(0, 16, 1024);
-    const uint64_t mnmajor = ptx::umma_smem_desc(0, C::kKvChunkBytes, 1024);
+    const uint32_t kv_chunk = kGroups ? 1024u : C::kKvChunkBytes, kv_group = kGroups ? C::kChunks * 1024u : 1024u;
+    const uint64_t qmajor = ptx::umma_smem_desc(0, 16, 1024);
+    const uint64_t kmajor = ptx::umma_smem_desc(0, 16, kv_group);
+    const uint64_t mnmajor = ptx::umma_smem_desc(0, kv_chunk, kv_group);
+    const uint32_t q_lo = static_cast<uint32_t>(qmajor), q_hi = static_cast<uint32_t>(qmajor >> 32);
     const uint32_t k_lo = static_cast<uint32_t>(kmajor), k_hi = static_cast<uint32_t>(kmajor >> 32);
     const uint32_t v_lo = static_cast<uint32_t>(mnmajor), v_hi = static_cast<uint32_t>(mnmajor >> 32);
     bool alive = true;
@@ -590,10 +600,10 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       if (!wait(kv_full(slot), slot_parity, kSiteMmaKV)) return;
       ptx::tc_fence_after_sync();
       const uint32_t d = tmem_base + (s_units & 1u) * kKeys;
-      const uint32_t qa = k_lo + (q_smem >> 4), kb = k_lo + ((kv_smem + slot * C::kSlotBytes) >> 4);
+      const uint32_t qa = q_lo + (q_smem >> 4), kb = k_lo + ((kv_smem + slot * C::kSlotBytes) >> 4);
 #pragma unroll
       for (int ks = 0; ks < kHeadDim / 16; ++ks)
-        mma_ss(d, qa + (((ks >> 2) * C::kQChunkBytes + (ks & 3) * 32) >> 4), k_hi, kb + (((ks >> 2) * C::kKvChunkBytes + (ks & 3) * 32) >> 4), k_hi,
+        mma_ss(d, qa + (((ks >> 2) * C::kQChunkBytes + (ks & 3) * 32) >> 4), q_hi, kb + (((ks >> 2) * kv_chunk + (ks & 3) * 32) >> 4), k_hi,
                idesc_s, ks != 0 ? 1u : 0u);
       ptx::umma_commit_elect(s_full(s_units & 1u));
       ptx::umma_commit_elect(kv_empty(slot));
@@ -618,7 +628,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       const uint32_t vb = v_lo + ((kv_smem + slot * C::kSlotBytes) >> 4);
 #pragma unroll
       for (int ks = 0; ks < kKeys / 16; ++ks)
-        mma_ts(d, a + ks * 8, vb + ((ks * 2048) >> 4), v_hi, idesc_o, (!o_walk.starts() || ks != 0) ? 1u : 0u);
+        mma_ts(d, a + ks * 8, vb + ((ks * 2 * kv_group) >> 4), v_hi, idesc_o, (!o_walk.starts() || ks != 0) ? 1u : 0u);
       ptx::umma_commit_elect(pv_done(o_units & 1u));
       ptx::umma_commit_elect(kv_empty(slot));
       advance();
@@ -761,22 +771,24 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           // (whole pages behind the last key were never copied: zeros already)
           const int stale = (min(((keys_end - 1) >> args.page_shift << args.page_shift) + (1 << args.page_shift) - k0, kKeys) - d1) * 8;
           const int drafts = (d1 - d0) * 8;
+          const int pitch = kGroups ? C::kChunks * 64 : 64, chunk = kGroups ? 64 : kKeys * 8;
+          auto piece = [&](int c, int i) -> uint4& { return kGroups ? v[c * chunk + (i >> 6) * pitch + (i & 63)] : v[c * chunk + i]; };
           uint32_t test = 0;
 #pragma unroll 1
           for (int i = row; i < drafts; i += kSoftmaxThreads) {
 #pragma unroll
             for (int c = 0; c < C::kChunks; ++c) {
-              const uint4 w = v[c * kKeys * 8 + d0 * 8 + i];
+              const uint4 w = piece(c, d0 * 8 + i);
               test = finite_test<kBf16>(finite_test<kBf16>(finite_test<kBf16>(finite_test<kBf16>(test, w.x), w.y), w.z), w.w);
             }
           }
 #pragma unroll 1
           for (int i = row; i < stale; i += kSoftmaxThreads) {
 #pragma unroll
-            for (int c = 0; c < C::kChunks; ++c) v[c * kKeys * 8 + d1 * 8 + i] = make_uint4(0, 0, 0, 0);
+            for (int c = 0; c < C::kChunks; ++c) piece(c, d1 * 8 + i) = make_uint4(0, 0, 0, 0);
           }
           if ((test & 0x7fff7fffu) != 0) {      // (this thread's own pieces)
-            for (int c = 0; c < C::kChunks; ++c) clear_odd_values(v + c * kKeys * 8 + d0 * 8, drafts, kSoftmaxThreads, row, kBf16 ? 0x7f80u : 0x7c00u);
+            for (int c = 0; c < C::kChunks; ++c) clear_odd_values(v + c * chunk, d0 * 8, drafts, kSoftmaxThreads, row, pitch, kBf16 ? 0x7f80u : 0x7c00u);
             odd_values[tiles % 3] = 1;
           }
           ptx::fence_proxy_async_smem();
@@ -1032,17 +1044,17 @@ int check(const ixk_fmha_paged_desc* d, const ixk_paged_cache* c) {
   return IXK_OK;
 }
 
-template <int kHeadDim, bool kBf16, bool kLse>
+template <int kHeadDim, bool kBf16, bool kLse, bool kGroups>
 int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const Args& a, int device, int sm_count, cudaStream_t stream) {
   using C = Cfg<kHeadDim>;
   static std::atomic<uint64_t> allowed{0};      // devices on which the kernel may use its shared memory
   const uint64_t bit = 1ull << (device & 63);
   if ((allowed.load(std::memory_order_relaxed) & bit) == 0) {
-    IXK_CUDA_OK(cudaFuncSetAttribute(fmha_paged_kernel<kHeadDim, kBf16, kLse>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
+    IXK_CUDA_OK(cudaFuncSetAttribute(fmha_paged_kernel<kHeadDim, kBf16, kLse, kGroups>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
   const int w = workers(kHeadDim, sm_count);
-  if (int st = launch_overlapped(fmha_paged_kernel<kHeadDim, kBf16, kLse>, dim3(w), dim3(C::kAllThreads), C::kSmemBytes, stream, q, k, v, a)) return st;
+  if (int st = launch_overlapped(fmha_paged_kernel<kHeadDim, kBf16, kLse, kGroups>, dim3(w), dim3(C::kAllThreads), C::kSmemBytes, stream, q, k, v, a)) return st;
   const unsigned blocks = static_cast<unsigned>((a.part_rows + kJoinRows - 1) / kJoinRows);
   if (a.tile_blocks != 0)
     return launch_overlapped(fmha_paged_join_many_kernel<kHeadDim, kBf16>, dim3(static_cast<unsigned>(a.requests) * a.kv_heads * a.tile_blocks, blocks, kHeadDim / 16),
@@ -1108,6 +1120,9 @@ int ixk_fmha_paged_fwd(const ixk_fmha_paged_desc* d, const ixk_paged_cache* c, c
   a.page_shift = __builtin_ctz(static_cast<unsigned>(c->page_size));
   a.pages = c->pages;
   a.cap = d->columns * c->page_size;
+  const uint32_t chunks = static_cast<uint32_t>(c->head_size / fmha_paged::kChunkElems);
+  const bool by_groups = c->head_size == fmha_paged::head_dim(c->head_size) && c->page_size < fmha_paged::kKeys && fmha_paged::kKeys / c->page_size * chunks > 8 &&
+                (c->heads == 1 || (c->k_strides[3] == c->head_size && c->v_strides[3] == c->head_size));
   a.negate = d->head_scale < 0.0f;
   // (0: all weights alike; a tiny one, since masked scores are -inf)
   a.scale_log2 = d->head_scale == 0.0f ? 1e-30f : std::fabs(d->head_scale) * fmha_paged::kLog2e;
@@ -1143,19 +1158,28 @@ int ixk_fmha_paged_fwd(const ixk_fmha_paged_desc* d, const ixk_paged_cache* c, c
   if (int st = encode_tmap(&mq, q, sq)) return st;
   for (int i = 0; i < 2; ++i) {
     const int64_t* s = i == 0 ? c->k_strides : c->v_strides;
+    const uint32_t keys = static_cast<uint32_t>(std::min(c->page_size, fmha_paged::kKeys));
     TmapSpec sk{type, 4,
                 {static_cast<uint64_t>(c->head_size), static_cast<uint64_t>(c->heads), static_cast<uint64_t>(c->page_size), static_cast<uint64_t>(c->pages)},
                 {bytes(s[3], c->heads), bytes(s[2], c->page_size), bytes(s[1], c->pages)},
-                {fmha_paged::kChunkElems, 1, static_cast<uint32_t>(std::min(c->page_size, fmha_paged::kKeys)), 1}, true};
+                {fmha_paged::kChunkElems, 1, keys, 1}, true};
+    if (by_groups)       // all chunks of all heads of a token behind one another
+      sk = TmapSpec{type, 4,
+                    {fmha_paged::kChunkElems, static_cast<uint64_t>(c->page_size), static_cast<uint64_t>(c->heads) * chunks, static_cast<uint64_t>(c->pages)},
+                    {bytes(s[2], c->page_size), fmha_paged::kChunkElems * 2, bytes(s[1], c->pages)},
+                    {fmha_paged::kChunkElems, 8, chunks, 1}, true};
     if (int st = encode_tmap(i == 0 ? &mk : &mv, i == 0 ? k_pages : v_pages, sk)) return st;
   }
   auto s = static_cast<cudaStream_t>(cuda_stream);
   const int dim = fmha_paged::head_dim(c->head_size);
   auto with = [&](auto bf16, auto with_lse) {
     constexpr bool kBf16 = decltype(bf16)::value, kLse = decltype(with_lse)::value;
-    if (dim == 64) return fmha_paged::launch<64, kBf16, kLse>(mq, mk, mv, a, info.device, info.sm_count, s);
-    if (dim == 128) return fmha_paged::launch<128, kBf16, kLse>(mq, mk, mv, a, info.device, info.sm_count, s);
-    return fmha_paged::launch<256, kBf16, kLse>(mq, mk, mv, a, info.device, info.sm_count, s);
+    if (dim == 64) return fmha_paged::launch<64, kBf16, kLse, false>(mq, mk, mv, a, info.device, info.sm_count, s);
+    if (dim == 128)
+      return by_groups ? fmha_paged::launch<128, kBf16, kLse, true>(mq, mk, mv, a, info.device, info.sm_count, s)
+                       : fmha_paged::launch<128, kBf16, kLse, false>(mq, mk, mv, a, info.device, info.sm_count, s);
+    return by_groups ? fmha_paged::launch<256, kBf16, kLse, true>(mq, mk, mv, a, info.device, info.sm_count, s)
+                     : fmha_paged::launch<256, kBf16, kLse, false>(mq, mk, mv, a, info.device, info.sm_count, s);
   };
   const std::true_type yes;
   const std::false_type no;

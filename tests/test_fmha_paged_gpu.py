@@ -368,3 +368,36 @@ def test_the_result_in_the_place_of_q(pkg, cuda, lengths):
     with pytest.raises(pkg.IxkError):
         wide = torch.zeros(q.shape[0], 24, 128, dtype=q.dtype, device=cuda)
         call(pkg, dict(s, q=wide[:, :12]), out=wide[:, ::2])
+
+
+@pytest.mark.parametrize("layout", ["tokens", "heads"])
+@pytest.mark.parametrize("size,page", [(128, 8), (256, 8), (256, 16), (256, 32), (192, 8)])
+def test_small_pages(pkg, cuda, size, page, layout):
+    """Copies of 8 keys over all of a head's columns, or (heads that do not follow one another) of a page's keys of 64 columns; ends of
+    requests at every place of a group of 8."""
+    lengths = [0, 3, 61, 64, 100, 127, 700] + list(range(40, 56))
+    s = make(cuda, lengths, [1 + i % 9 for i in range(len(lengths))], 6, 2, size, page, torch.float16, seed=3, layout=layout)
+    s["mask"] = random_mask(s, 1)
+    check(s, *call(pkg, s))
+
+
+@pytest.mark.parametrize("size,page", [(128, 8), (256, 8), (256, 16)])
+@pytest.mark.parametrize("L", [0, 5, 61, 203])
+def test_values_that_are_no_numbers_in_small_pages(pkg, cuda, size, page, L):
+    """Drafts whose values are no numbers reach the rows that see them, and only those."""
+    s = make(cuda, [L, 30], [13, 2], 4, 2, size, page, torch.bfloat16, seed=6)
+    s["mask"] = random_mask(s, 1)
+    bad = (2, 7, 8, 12)
+    for d in bad:
+        p = L + d
+        s["v"][s["table"][0, p // page].long(), p % page, :, d * 3] = float("inf") if d % 2 else float("nan")
+    out, _ = call(pkg, s)
+    clean = dict(s, v=torch.where(s["v"].isfinite(), s["v"], torch.zeros_like(s["v"])))
+    want, _ = call(pkg, clean)
+    for j in range(13):
+        for d in bad:
+            sees = bool(s["mask"][j, 0] >> d & 1)
+            assert bool(out[j, :, d * 3].isfinite().all()) != sees, (j, d)
+    odd = torch.zeros_like(out, dtype=torch.bool)
+    odd[:13, :, [d * 3 for d in bad]] = True
+    assert torch.equal(out[~odd], want[~odd])
