@@ -293,3 +293,37 @@ def test_refusals(pkg, cuda):
         pkg.qk_norm_rotary_backward(s["grad_q"], s["grad_k"], s["q"], s["k"], workspace=torch.empty(16, dtype=torch.uint8, device=cuda), **base)
     assert e.value.status == pkg.IXK_WORKSPACE_TOO_SMALL
     assert pkg.launch_count() == n0
+
+
+MORE = [(40, 3, 2, H, dtype, F32, rotary, half, torch.int32, 0.5)
+        for dtype in (HF, F32) for H, rotary, half in ((64, 24, False), (64, 40, False), (80, 72, False), (128, 56, False), (128, 72, False), (136, 136, False),
+                                                       (160, 80, True), (200, 16, True), (256, 136, False), (256, 240, True), (16, 8, False), (24, 16, True))]
+# just below and above whole turns of a token a warp (148 multiprocessors x 4 blocks x 4 warps), and last turns that several warps share
+MORE += [(T, 2, 1, 64, BF, BF, 64, True, torch.int64, 0.0) for T in (1183, 1184, 1185, 2367, 2368, 2369, 2400, 4736, 4737, 7200)]
+MORE += [(T, 9, 5, 128, HF, HF, 128, False, None, 0.0) for T in (2, 300, 2369, 2960, 5000)]
+
+
+@pytest.mark.parametrize("case", MORE, ids=[f"T{c[0]}N{c[1]}K{c[2]}H{c[3]}{str(c[4])[6:]}r{c[6]}{'h' if c[7] else 'i'}" for c in MORE])
+def test_parts_of_heads_and_turns(pkg, cuda, case):
+    test_forward_and_backward(pkg, cuda, case)
+
+
+@pytest.mark.parametrize("half", [True, False])
+def test_fp32_between_sectors(pkg, cuda, half):
+    """Tensors that begin in the middle of a 32-byte sector: the same bits."""
+    s = inputs(cuda, 70, 3, 1, 96, F32, F32, 96, seed=8)
+    common = dict(q_gain=s["q_gain"], k_gain=s["k_gain"], cos=s["cos"], sin=s["sin"], positions=s["positions"], half_split=half)
+    off = lambda t: torch.full((t.numel() + 8,), 7.0, device=cuda)[4:-4].view(t.shape)  # noqa: E731
+    moved = {n: off(s[n]).copy_(s[n]) for n in ("q", "k", "grad_q", "grad_k")}
+    assert moved["q"].data_ptr() % 32 == 16
+    want = pkg.qk_norm_rotary_forward(s["q"], s["k"], **common)
+    out = [off(t) for t in want]
+    pkg.qk_norm_rotary_forward(moved["q"], moved["k"], q_out=out[0], k_out=out[1], **common)
+    grads = pkg.qk_norm_rotary_backward(s["grad_q"], s["grad_k"], s["q"], s["k"], **common)
+    d = [off(t) for t in grads[:2]]
+    again = pkg.qk_norm_rotary_backward(moved["grad_q"], moved["grad_k"], moved["q"], moved["k"], dq=d[0], dk=d[1], **common)
+    for a, b in zip((*want, *grads), (*out, *again)):
+        assert torch.equal(a, b)
+    for t in out + d:
+        whole = torch.as_strided(t, (t.numel() + 8,), (1,), t.storage_offset() - 4)
+        assert (whole[:4] == 7.0).all() and (whole[-4:] == 7.0).all()
