@@ -13,9 +13,11 @@
 //
 // Bound by HBM: 64 keys of K and V take H * 256 bytes, 1340 cycles of an SM's share of the bandwidth at H = 128, the two products
 // 640 (the tile is padded to 128 rows), the softmax about 1000 and beside those of the other worker.
-// The running maximum is raised when it has moved by more than 2^8, so O is seldom rescaled.  P is rounded to nearest, and the
-// row is divided by the sum of the rounded values, so that a row with one large weight loses nothing; the log-sum-exp is
-// taken of the sum of the fp32 ones.
+// Weights are taken of a reference point near the running maximum, which is raised when that has moved by more than 2^8 (fp16: 2^4), so O
+// is seldom rescaled.  P is rounded to nearest, and the row is divided by the sum of the rounded values, so that a row with one
+// large weight loses nothing; the log-sum-exp is taken of the sum of the fp32 ones.  fp16 has few exponents: there the reference
+// point lies 2^11 below the maximum, so that the largest weights are 2^11 to 2^15 and those down to 2^-25 of them normal numbers
+// (with 1 to 2^8, thousands of keys at 2^-25 of the largest added up to nothing); smaller ones are off by 2^-36 of it at most.
 //
 // A tile whose units all lie in one run is written out; otherwise its parts go to scratch in fp32, and the second kernel joins
 // them.  A worker has at most two: the end of a tile that an earlier worker began, and the beginning of one that goes on.
@@ -52,7 +54,11 @@ constexpr int kTileCost = 3;          // what a tile costs beside its units (Q, 
 constexpr int kMinUnits = 2;          // shortest run: with one, the parts to join cost more than the second unit (5 rows, 705 keys: 11.9, 12.4 us)
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kRescaleThreshold = 8.0f;   // log2 units
+// Where the reference point of a row's weights lies below its maximum when it is set, and how far the maximum may then rise (log2 units).
+template <bool kBf16>
+constexpr float kBelowMaximum = kBf16 ? 0.0f : 11.0f;
+template <bool kBf16>
+constexpr float kRise = kBf16 ? 8.0f : 4.0f;
 
 enum : int { kSiteLoadQ = 801, kSiteLoadKV = 802, kSiteMmaQ = 803, kSiteMmaKV = 804, kSiteMmaP = 805, kSiteMmaO = 806, kSiteSoftmaxS = 807,
              kSiteSoftmaxO = 808, kSiteSoftmaxV = 809, kSiteAlign = 810 };
@@ -103,7 +109,7 @@ struct Args {
   int tile_blocks;            // 0: by worker
   int workers;
   float* part_o;              // [2 * workers][kHeadDim / 4][part_rows][4]: a warp's rows side by side
-  float4* part_stat;          // [2 * workers][part_rows]: maximum (log2), sum, sum of rounded weights
+  float4* part_stat;          // [2 * workers][part_rows]: reference point (log2), sum, sum of rounded weights
 };
 
 // A request's numbers, cut to what its buffers hold.
@@ -659,7 +665,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         m0 = words[0];
         if (args.mask_words > 1) m1 = words[1];
       }
-      float m_run = -INFINITY, l_run = 0.0f, r_run = 0.0f;     // maximum, sum, sum of the rounded weights
+      float m_run = -INFINITY, l_run = 0.0f, r_run = 0.0f;     // reference point, sum, sum of the rounded weights
       bool more = true;
       for (; more; ++g) {
         const int buf = g & 1u;
@@ -704,9 +710,10 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           }
           const float top = fmaxf(fmaxf(ptx::max3(mx[0], mx[1], mx[2]), mx[3]), fmaxf(ptx::max3(mx[4], mx[5], mx[6]), mx[7])) * mult;
           float alpha = 1.0f;
-          if (row_ok && top - m_run > kRescaleThreshold) {     // also where the row has seen nothing so far
-            alpha = ptx::ex2_approx(m_run - top);
-            m_run = top;
+          if (row_ok && top - m_run > kBelowMaximum<kBf16> + kRise<kBf16>) {     // also where the row has seen nothing so far
+            const float to = top - kBelowMaximum<kBf16>;
+            alpha = ptx::ex2_approx(m_run - to);
+            m_run = to;
           }
           if (walk.unit != first_unit && __any_sync(0xffffffffu, alpha != 1.0f)) {
             // (S of this unit was issued behind P.V of the unit before the last: only the last one's may still run)
@@ -884,7 +891,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   }
 }
 
-// Joins the parts of the tiles that several workers did.  With the parts' maxima m_i and sums l_i, M = max m_i:
+// Joins the parts of the tiles that several workers did.  With the parts' reference points m_i and sums l_i, M = max m_i:
 //   o = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i
 // Worker w's own part is at 2 w + 1, those of the workers behind it at 2 (w + i).  A thread takes 16 columns of a row, a warp 32 rows
 // of these columns, as the parts lie in memory.  Bound by trips to memory: what it needs of the tile is one load, then
