@@ -705,10 +705,11 @@ int ixk_all_reduce_slice(int dtype, size_t count, int rank, int world, size_t* b
 int ixk_device_status(int* status_word);
 /* Exercises that mechanism on purpose: launches one small CTA whose first warp waits, with a
  * budget of `limit_cycles` (at most 1e8, i.e. well under 0.1 s), for a barrier phase that nothing
- * completes, and whose second warp depends on the first.  The kernel returns by itself; afterwards
+ * completes, whose second warp depends on the first, and whose third waits with all lanes together.
+ * The kernel returns by itself; afterwards
  * ixk_device_status reports IXK_DEVICE_TIMEOUT with site code 901 and clears the word, and the
  * device is as usable as before.  cycles_out_device (device memory, may be NULL) receives the
- * cycles the CTA spent.  No counterpart in the reference, whose kernels have no device-side waits. */
+ * cycles the CTA spent, or -1 if lanes that wait together were given unlike answers.  No counterpart in the reference, whose kernels have no device-side waits. */
 int ixk_selftest_bounded_wait(long long limit_cycles, long long* cycles_out_device, void* cuda_stream);
 /* With IXK_NVTX=1 in the environment every entry point that launches work is wrapped in an NVTX
  * range of its own name (for timelines of the calling program); off by default. */

@@ -649,6 +649,11 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     const int row_token = row / args.group, row_head = row - row_token * args.group;
     uint32_t g = 0, tiles = 0;
     bool alive = true;
+    // (A warp's lanes go on together or give up together: what follows has them all, in votes and in accesses to tensor memory.)
+    auto wait = [&](uint32_t bar, uint32_t parity, int site) {
+      alive = ptx::mbar_wait_warp(bar, parity, ctl, site);
+      return alive;
+    };
     int4 begun = make_int4(0, 0, 0, 0);       // the tile that this worker leaves to others: none so far
     while (alive && !walk.done()) {
       const Request req = walk.req;
@@ -672,10 +677,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         const int k0 = walk.unit * kKeys;
         const bool masked = k0 + kKeys > req.length;
         const uint32_t s_addr = tmem_base + lane_addr + buf * kKeys;
-        if (!ptx::mbar_wait(s_full(buf), (g >> 1) & 1u, ctl, kSiteSoftmaxS)) {
-          alive = false;
-          break;
-        }
+        if (!wait(s_full(buf), (g >> 1) & 1u, kSiteSoftmaxS)) break;
         ptx::tc_fence_after_sync();
         if (warp_ok) {
           uint32_t r[2][32];
@@ -715,12 +717,10 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             alpha = ptx::ex2_approx(m_run - to);
             m_run = to;
           }
+          __syncwarp();          // (what follows accesses tensor memory with all lanes)
           if (walk.unit != first_unit && __any_sync(0xffffffffu, alpha != 1.0f)) {
             // (S of this unit was issued behind P.V of the unit before the last: only the last one's may still run)
-            if (!ptx::mbar_wait(pv_done((g - 1) & 1u), ((g - 1) >> 1) & 1u, ctl, kSiteSoftmaxO)) {
-              alive = false;
-              break;
-            }
+            if (!wait(pv_done((g - 1) & 1u), ((g - 1) >> 1) & 1u, kSiteSoftmaxO)) break;
             ptx::tc_fence_after_sync();
 #pragma unroll 1
             for (int c = 0; c < kHeadDim / 32; ++c) {
@@ -769,10 +769,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         if (masked) {
           // V behind the last key, and values of drafts that are no numbers
           const uint32_t load = walk.last() ? 2 * g + 1 : 2 * g + 2;
-          if (!ptx::mbar_wait(kv_full(load % kSlots), (load / kSlots) & 1u, ctl, kSiteSoftmaxV)) {
-            alive = false;
-            break;
-          }
+          if (!wait(kv_full(load % kSlots), (load / kSlots) & 1u, kSiteSoftmaxV)) break;
           uint4* v = reinterpret_cast<uint4*>(smem + C::kQBytes + (load % kSlots) * C::kSlotBytes);     // (16-byte pieces: a key is 8 in a chunk)
           const int d0 = max(req.length - k0, 0), d1 = min(keys_end - k0, kKeys);
           // (whole pages behind the last key were never copied: zeros already)
@@ -808,7 +805,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         if (more) walk.next(args);
       }
       if (!alive) break;
-      if (!ptx::mbar_wait(pv_done((g - 1) & 1u), ((g - 1) >> 1) & 1u, ctl, kSiteSoftmaxO)) break;
+      if (!wait(pv_done((g - 1) & 1u), ((g - 1) >> 1) & 1u, kSiteSoftmaxO)) break;
       ptx::tc_fence_after_sync();
       const bool odd = odd_values[tiles % 3] != 0;
       ++tiles;

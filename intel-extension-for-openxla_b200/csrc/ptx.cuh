@@ -120,6 +120,29 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const A
   return mbar_wait_limit(bar, parity, ctl, code, kWaitCycleLimit);
 }
 
+// The same by all lanes of a warp, which go on together or give up together: what follows a wait of single lanes (votes, accesses to
+// tensor memory) would find some of them gone.
+__device__ __forceinline__ bool mbar_wait_warp_limit(uint32_t bar, uint32_t parity, const AbortCtl& ctl, int code, long long limit) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const long long t0 = clock64();
+  uint32_t spins = 0;
+  while (true) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if ((++spins & 0x3ffu) == 0) {
+      bool give_up = *ctl.cta_abort != 0;
+      if (clock64() - t0 > limit) {
+        *ctl.cta_abort = 1;
+        atomicCAS(ctl.status_word, 0, code);
+        give_up = true;
+      }
+      if (__any_sync(0xffffffffu, give_up)) return false;
+    }
+  }
+}
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, const AbortCtl& ctl, int code) {
+  return mbar_wait_warp_limit(bar, parity, ctl, code, kWaitCycleLimit);
+}
+
 // Register re-partitioning between warpgroups (all four warps of a warpgroup execute it).
 template <int kRegs>
 __device__ __forceinline__ void setmaxnreg_inc() {
