@@ -22,9 +22,10 @@
 // A tile whose units all lie in one run is written out; otherwise its parts go to scratch in fp32, and the second kernel joins
 // them.  A worker has at most two: the end of a tile that an earlier worker began, and the beginning of one that goes on.
 //
-// Units that reach behind a request's committed tokens see masks, bit by bit, and the stale rest of its last page.  There the
-// softmax warps go through V in shared memory first: rows behind the end become zeros, and of drafts every NaN and infinity, since
-// 0 * NaN would reach rows that do not see the draft; rows that do see it get them back at the end (`odd_values`).
+// Units that reach behind the keys that all rows of a tile see (a request's committed tokens, and without a mask the new ones in front
+// of the tile's) see masks, bit by bit, and the stale rest of its last page.  There the softmax warps go through V in shared
+// memory first: rows behind the end become zeros, and of drafts every NaN and infinity, since 0 * NaN would reach rows that do not
+// see the draft; rows that do see it get them back at the end (`odd_values`).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -264,7 +265,7 @@ __device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_
 }
 
 // Which of keys [k0, k0 + 64) a row sees, as bits: committed ones, and drafts by its mask or, without one, up to itself.  Of a unit
-// with keys behind the committed ones (length - k0 < 64).  `words`: the row's mask, its first two words in m0 and m1.
+// with keys behind those that all rows see (so length - k0 < 64).  `words`: the row's mask, its first two words in m0 and m1.
 __device__ __forceinline__ uint64_t visible_keys(const Args& a, const Request& r, const int* words, uint32_t m0, uint32_t m1, int token, int k0) {
   auto below = [](int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1ull; };
   const int committed = r.length - k0, end = min(r.rows, a.cap - r.length) + committed;
@@ -310,25 +311,59 @@ __device__ __noinline__ void clear_odd_values(uint4* v, int begin, int pieces, i
     v[i] = make_uint4(words[0], words[1], words[2], words[3]);
   }
 }
-// ... and the other end of it: a row that was written without them gets the odd values of the drafts [d0, d1) that it sees, out of
-// memory again.  `out`: the row itself, or `part`: its part in scratch.
+// ... and the other end of it: rows that were written without them get the odd values of the drafts [d0, d1) that they see, out of memory
+// again.  `out`: a row itself, or `part`: its part in scratch.  All lanes of a warp call it; `row_ok`: those that have a row.  A
+// lane looks for odd values in one of 32 drafts; then the rows add up those that they see, 8 columns at a time, and change these once.
 template <bool kBf16>
-__device__ __noinline__ void add_odd_values(const Args& a, int length, int b, int kv_head, int token, int q_row, int d0, int d1, uint16_t* out,
+__device__ __noinline__ void add_odd_values(const Args& a, int length, int b, int kv_head, bool row_ok, int token, int q_row, int d0, int d1, uint16_t* out,
                                             float* part, int64_t part_pitch) {
-  const int* words = a.mask != nullptr ? a.mask + q_row * a.mask_stride : nullptr;
-  for (int d = d0; d < d1; ++d) {
-    if (words == nullptr ? d > token : (d >> 5) >= a.mask_words || !(static_cast<uint32_t>(words[d >> 5]) >> (d & 31) & 1u)) continue;
-    const int k = length + d;
-    const int page = a.table[b * a.table_stride + (k >> a.page_shift)];
-    if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.pages)) continue;
-    const uint16_t* v = a.v + page * a.v_strides[0] + (k & ((1 << a.page_shift) - 1)) * a.v_strides[1] + kv_head * a.v_strides[2];
-    for (int i = 0; i < a.head_size; ++i) {
-      const float x = unpack2<kBf16>(v[i]).x;
-      if (fabsf(x) < INFINITY) continue;
-      if (part != nullptr) {
-        part[(i >> 2) * part_pitch + (i & 3)] += x;
-      } else {
-        out[i] = static_cast<uint16_t>(pack2<kBf16>(unpack2<kBf16>(out[i]).x + x, 0.0f) & 0xffffu);
+  constexpr uint32_t kExponent = kBf16 ? 0x7f80u : 0x7c00u;
+  const int lane = threadIdx.x & 31, pieces = a.head_size / 8;
+  for (; d0 < d1; d0 += 32) {
+    const uint4* mine = nullptr;
+    uint32_t test = 0;
+    if (d0 + lane < d1) {
+      const int k = length + d0 + lane, page = a.table[b * a.table_stride + (k >> a.page_shift)];
+      if (static_cast<unsigned>(page) < static_cast<unsigned>(a.pages)) {
+        mine = reinterpret_cast<const uint4*>(a.v + page * a.v_strides[0] + (k & ((1 << a.page_shift) - 1)) * a.v_strides[1] + kv_head * a.v_strides[2]);
+#pragma unroll 8
+        for (int i = 0; i < pieces; ++i) {
+          const uint4 w = mine[i];
+          test = finite_test<kBf16>(finite_test<kBf16>(finite_test<kBf16>(finite_test<kBf16>(test, w.x), w.y), w.z), w.w);
+        }
+      }
+    }
+    const uint32_t found = __ballot_sync(0xffffffffu, (test & 0x7fff7fffu) != 0);
+    if (found == 0) continue;
+    uint32_t sees = 0;         // of the 32 drafts, by this lane's row
+    if (row_ok && a.mask == nullptr) {
+      const int n = token + 1 - d0;
+      sees = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+    } else if (row_ok) {
+      const int* words = a.mask + q_row * a.mask_stride;
+      const int w = d0 >> 5;
+      sees = __funnelshift_r(w < a.mask_words ? words[w] : 0, w + 1 < a.mask_words ? words[w + 1] : 0, d0 & 31);
+    }
+    for (int c = 0; c < pieces; ++c) {
+      float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+      for (uint32_t left = found; left != 0; left &= left - 1) {
+        const int i = __ffs(left) - 1;
+        const uint4* v = reinterpret_cast<const uint4*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), i));
+        if (!(sees >> i & 1u)) continue;
+        const uint4 w = v[c];
+        const uint32_t held[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t bits = held[e >> 1] >> 16 * (e & 1) & 0xffffu;
+          if ((bits & kExponent) == kExponent) sum[e] += unpack2<kBf16>(bits).x;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (sum[e] == 0.0f) continue;
+        const int i = c * 8 + e;
+        if (part != nullptr) part[(i >> 2) * part_pitch + (i & 3)] += sum[e];
+        else out[i] = static_cast<uint16_t>(pack2<kBf16>(unpack2<kBf16>(out[i]).x + sum[e], 0.0f) & 0xffffu);
       }
     }
   }
@@ -663,6 +698,8 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       const int q_row = req.row0 + token;
       const int keys_end = req.length + min(req.rows, args.cap - req.length);
       const int first_unit = walk.unit;
+      // the keys in front of this one are seen by all rows of the tile
+      const int common = req.length + (args.mask != nullptr ? 0 : min(walk.t0, args.cap - req.length));
       // the row's mask, asked for long before it is needed
       const int* words = args.mask != nullptr ? args.mask + q_row * args.mask_stride : nullptr;
       uint32_t m0 = 0, m1 = 0;
@@ -675,7 +712,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       for (; more; ++g) {
         const int buf = g & 1u;
         const int k0 = walk.unit * kKeys;
-        const bool masked = k0 + kKeys > req.length;
+        const bool masked = k0 + kKeys > common;
         const uint32_t s_addr = tmem_base + lane_addr + buf * kKeys;
         if (!wait(s_full(buf), (g >> 1) & 1u, kSiteSoftmaxS)) break;
         ptx::tc_fence_after_sync();
@@ -771,7 +808,7 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           const uint32_t load = walk.last() ? 2 * g + 1 : 2 * g + 2;
           if (!wait(kv_full(load % kSlots), (load / kSlots) & 1u, kSiteSoftmaxV)) break;
           uint4* v = reinterpret_cast<uint4*>(smem + C::kQBytes + (load % kSlots) * C::kSlotBytes);     // (16-byte pieces: a key is 8 in a chunk)
-          const int d0 = max(req.length - k0, 0), d1 = min(keys_end - k0, kKeys);
+          const int d0 = max(common - k0, 0), d1 = min(keys_end - k0, kKeys);
           // (whole pages behind the last key were never copied: zeros already)
           const int stale = (min(((keys_end - 1) >> args.page_shift << args.page_shift) + (1 << args.page_shift) - k0, kKeys) - d1) * 8;
           const int drafts = (d1 - d0) * 8;
@@ -867,9 +904,11 @@ fmha_paged_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           if (!whole) args.part_stat[part * args.part_rows + row] = make_float4(m_run, l_run, r_run, 0.0f);
           else if (kLse)
             args.lse[static_cast<int64_t>(q_row) * args.heads + head] = l_run == 0.0f ? -INFINITY : (m_run + log2f(l_run)) * kLn2;
-          if (odd)
-            add_odd_values<kBf16>(args, req.length, walk.b, walk.kv_head, token, q_row, max(first_unit * kKeys - req.length, 0),
-                           min(walk.end * kKeys, keys_end) - req.length, out_row, whole ? nullptr : part_row, part_pitch);
+        }
+        if (odd) {
+          __syncwarp();
+          add_odd_values<kBf16>(args, req.length, walk.b, walk.kv_head, row_ok, token, q_row, max(first_unit * kKeys, common) - req.length,
+                                min(walk.end * kKeys, keys_end) - req.length, out_row, whole ? nullptr : part_row, part_pitch);
         }
       }
       ptx::tc_fence_before_sync();
