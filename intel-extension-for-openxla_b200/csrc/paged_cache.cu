@@ -124,24 +124,26 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(const __grid_constant_
   __syncthreads();
   taken = __reduce_max_sync(0xffffffffu, static_cast<int>(threadIdx.x & 31) < (threads >> 5) ? taken_max[threadIdx.x & 31] : 0);
 
-  const int stride = static_cast<int>(gridDim.x) * threads;
-  const int me = static_cast<int>(blockIdx.x) * threads + static_cast<int>(threadIdx.x);
-  for (int b = me; b <= B; b += stride) {
+  // (Without a sign: rows and pages may be 2^31 less a little, and a thread's last index lies a stride behind them.)
+  const unsigned stride = gridDim.x * threads, me = blockIdx.x * threads + threadIdx.x;
+  for (int b = static_cast<int>(me); b <= B; b += static_cast<int>(stride)) {
     a.row_start[b] = start[b];
     if (b < B) a.granted[b] = fits[b] ? max(a.new_tokens[b], 0) : 0;
   }
-  for (int i = me; i < taken; i += stride) {
+  for (unsigned at = me; at < static_cast<unsigned>(taken); at += stride) {
+    const int i = static_cast<int>(at);
     const int b = owner(first, B, i);
     a.page_table[b * a.table_stride + pages_for(a.lengths[b], a.page_size) + i - first[b]] = a.free_pages[available - 1 - i];
   }
-  for (int r = me; r < a.rows; r += stride) {
+  for (unsigned at = me; at < static_cast<unsigned>(a.rows); at += stride) {
+    const int r = static_cast<int>(at);
     int request = -1, position = -1, slot = -1;
     if (r < total_rows) {
       const int b = owner(start, B, r);
       if (fits[b]) {
         const int L = a.lengths[b], have = pages_for(L, a.page_size);
         request = b;
-        position = L + r - start[b];
+        position = L + (r - start[b]);
         const int place = static_cast<int>(static_cast<unsigned>(position) / static_cast<unsigned>(a.page_size));
         const int p = place < have ? a.page_table[b * a.table_stride + place] : a.free_pages[available - 1 - (first[b] + place - have)];
         if (static_cast<unsigned>(p) < static_cast<unsigned>(a.pages)) slot = p * a.page_size + position - place * a.page_size;
@@ -242,8 +244,8 @@ __device__ void keep_books(const KeepArgs& a, int* smem) {
   const int back = static_cast<int>(min(total, static_cast<long long>(a.pages - count)));
   if (threadIdx.x == 0) first[B] = static_cast<int>(min(total, 0x7fffffffLL));
   __syncthreads();
-  for (int i = threadIdx.x; i < back; i += threads) {
-    const int b = owner(first, B, i);
+  for (unsigned at = threadIdx.x; at < static_cast<unsigned>(back); at += threads) {      // (as in extend_kernel)
+    const int i = static_cast<int>(at), b = owner(first, B, i);
     a.free_pages[count + i] = a.page_table[b * a.table_stride + low[b] + i - first[b]];
   }
   if (threadIdx.x == 0) *a.free_count_out = count + back;
