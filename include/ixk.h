@@ -472,7 +472,7 @@ size_t ixk_qk_norm_rotary_bwd_workspace_bytes(const ixk_qk_desc* desc);
  * table row are not read.  Scores, statistics and sums are fp32; p is rounded to dtype (to nearest) as an operand
  * of the second product, and out is divided by the sum of the rounded p (lse: of the fp32 ones); in F16 weights below
  * 2^-25 of a row's largest are off by up to 2^-36 of that.  Results depend on the lengths and sizes alone, not on timing.
- * out may be q, with its strides.  page_size in {8, 16, 32, 64, 128, 256}; head_size a multiple of 8 up to 256; q, out, K and V 16-byte aligned
+ * out may be q, with its strides.  Rows, requests and keys of a request are a little below 2^31 at most.  page_size in {8, 16, 32, 64, 128, 256}; head_size a multiple of 8 up to 256; q, out, K and V 16-byte aligned
  * with strides that are multiples of 8 elements; workspace: ixk_fmha_paged_fwd_workspace_bytes(desc, cache)
  * bytes, 16-byte aligned. */
 typedef struct ixk_fmha_paged_desc {

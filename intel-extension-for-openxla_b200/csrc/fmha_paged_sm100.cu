@@ -1082,8 +1082,9 @@ int check(const ixk_fmha_paged_desc* d, const ixk_paged_cache* c) {
   if (c->page_size < 8 || c->page_size > 256 || (c->page_size & (c->page_size - 1)) != 0)
     return fail(IXK_UNIMPLEMENTED, "fmha_paged: page_size must be 8, 16, 32, 64, 128 or 256");
   if (!std::isfinite(d->head_scale * kLog2e)) return fail(IXK_INVALID_ARGUMENT, "fmha_paged: head_scale is not finite");
-  if (d->rows > 0x7fffffff - 256 || static_cast<int64_t>(d->columns) * c->page_size > 0x7fffffff - 256)
-    return fail(IXK_UNIMPLEMENTED, "fmha_paged: 2^31 rows, or keys of a request, or more");
+  // (the kernel's counts run past these by a CTA's threads)
+  if (d->rows > 0x7fffffff - 256 || d->requests > 0x7fffffff - 65536 || static_cast<int64_t>(d->columns) * c->page_size > 0x7fffffff - 256)
+    return fail(IXK_UNIMPLEMENTED, "fmha_paged: 2^31 rows, requests, or keys of a request, or more");
   return IXK_OK;
 }
 
