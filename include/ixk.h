@@ -411,7 +411,7 @@ typedef struct ixk_paged_cache {
  * + kept, and the pages above go back to the end of free_pages in the order of the requests.  kept[b] < 0
  * ends the request: lengths_out[b] = 0 and all of its pages go back.  lengths_out may be lengths,
  * free_count_out free_count; nothing else that is written may share memory with anything.  The table
- * itself is not written.  cache, k, v: NULL with path NULL.
+ * itself is not written.  cache, k, v: NULL with path NULL; k and v share memory with nothing else.
  * path_columns at most 1024; K and V 16-byte aligned. */
 int ixk_paged_keep(const ixk_page_pool* pool, const int32_t* lengths, const int32_t* granted,
                    const int32_t* kept, const int32_t* path, int64_t path_columns, int64_t path_stride,
@@ -427,7 +427,8 @@ int ixk_paged_keep(const ixk_page_pool* pool, const int32_t* lengths, const int3
  * strides (they may be slices of one projection).  positions NULL: token t sits at t % places.  A token
  * whose position is outside [0, places) is left out: nothing of it is written, its gradient is 0, and
  * it takes no part in the gains' gradients.  Keys go to k_out, or, with `cache`, to their slots, and
- * values with them; a slot outside the cache is not written.  y may be x.
+ * values with them; a slot outside the cache is not written.  y may be x, in the same strides; nothing
+ * else that is written may share memory with another operand or with itself (slices of one buffer do not).
  * dtype in {BF16, F16, F32} (with a cache its type); gains NULL (1) or [head_size] of dtype or F32.
  * head_size a multiple of 8 up to 256, rotary_dim a multiple of 16 (interleaved: 8); strides multiples of 8
  * elements, pointers 16-byte aligned (positions and slots: as their elements are). */
@@ -451,7 +452,7 @@ int ixk_qk_norm_rotary_fwd(const ixk_qk_desc* desc, const void* q, const void* k
 /* dq, dk from the gradients of the rotated heads and the forward's inputs; dq_gain, dk_gain (NULL: not
  * wanted) [head_size] of param_dtype, the sums over tokens and heads in fp32 and in a fixed order: with
  * either, workspace holds ixk_qk_norm_rotary_bwd_workspace_bytes(desc) bytes, 16-byte aligned.  dq may
- * be q or grad_q, dk likewise. */
+ * be q or grad_q, dk likewise, dq_gain q_gain, dk_gain k_gain; else as in the forward pass. */
 int ixk_qk_norm_rotary_bwd(const ixk_qk_desc* desc, const void* grad_q, const void* grad_k,
                            const void* q, const void* k, const void* q_gain, const void* k_gain,
                            const float* cos_table, const float* sin_table, const void* positions,
@@ -472,7 +473,7 @@ size_t ixk_qk_norm_rotary_bwd_workspace_bytes(const ixk_qk_desc* desc);
  * table row are not read.  Scores, statistics and sums are fp32; p is rounded to dtype (to nearest) as an operand
  * of the second product, and out is divided by the sum of the rounded p (lse: of the fp32 ones); in F16 weights below
  * 2^-25 of a row's largest are off by up to 2^-36 of that.  Results depend on the lengths and sizes alone, not on timing.
- * out may be q, with its strides.  Rows, requests and keys of a request are a little below 2^31 at most.  page_size in {8, 16, 32, 64, 128, 256}; head_size a multiple of 8 up to 256; q, out, K and V 16-byte aligned
+ * out may be q, with its strides; out, lse and the workspace share memory with nothing else.  Rows, requests and keys of a request are a little below 2^31 at most.  page_size in {8, 16, 32, 64, 128, 256}; head_size a multiple of 8 up to 256; q, out, K and V 16-byte aligned
  * with strides that are multiples of 8 elements; workspace: ixk_fmha_paged_fwd_workspace_bytes(desc, cache)
  * bytes, 16-byte aligned. */
 typedef struct ixk_fmha_paged_desc {

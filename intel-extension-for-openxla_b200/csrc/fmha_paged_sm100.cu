@@ -1141,9 +1141,17 @@ int ixk_fmha_paged_fwd(const ixk_fmha_paged_desc* d, const ixk_paged_cache* c, c
     if (extent > 1 && (d->q_strides[i] < c->head_size || d->o_strides[i] < c->head_size))
       return fail(IXK_INVALID_ARGUMENT, "fmha_paged: rows of q or out overlap");
   }
-  if (out == q && out != nullptr && ((d->rows > 1 && d->q_strides[0] != d->o_strides[0]) || (d->heads > 1 && d->q_strides[1] != d->o_strides[1])))
-    return fail(IXK_INVALID_ARGUMENT, "fmha_paged: out is in q's place, with other strides");
-  if (out != nullptr && (out == k_pages || out == v_pages)) return fail(IXK_INVALID_ARGUMENT, "fmha_paged: out is in the cache");
+  if (d->requests > 0 && d->rows > 0) {
+    const int64_t rows = d->rows, requests = d->requests;
+    const paged::Operand mq(q, c->head_size * 2, {rows, d->heads}, d->q_strides, 2), mo(out, c->head_size * 2, {rows, d->heads}, d->o_strides, 2),
+        kp = paged::key_pages(c, k_pages), vp = paged::value_pages(c, v_pages), table(page_table, paged::rows_extent(requests, d->table_stride, d->columns) * 4),
+        books[3] = {{lengths, requests * 4}, {row_start, (requests + 1) * 4}, {granted, requests * 4}},
+        bits(mask, paged::rows_extent(rows, d->mask_stride, d->mask_words) * 4), ml(lse, rows * d->heads * 4),
+        scratch(workspace, static_cast<int64_t>(std::min(workspace_bytes, fmha_paged::scratch_of(d, c, 148).total)));
+    if (const char* name = paged::shared_memory({{"out", &mo, &mq, nullptr}, {"lse", &ml, nullptr, nullptr}, {"the workspace", &scratch, nullptr, nullptr}},
+                                                {&mq, &kp, &vp, &table, &books[0], &books[1], &books[2], &bits}))
+      return fail(IXK_INVALID_ARGUMENT, std::string("fmha_paged: ") + name + " shares memory with another operand or with itself");
+  }
   DeviceInfo info;
   if (int st = get_device_info(&info)) return st;
   if (d->requests == 0 || d->rows == 0) return IXK_OK;

@@ -424,7 +424,14 @@ int ixk_paged_keep(const ixk_page_pool* pool, const int32_t* lengths, const int3
     if (int st = paged::check_cache(cache, k, v, "paged_keep")) return st;
     if (cache->page_size != pool->page_size || cache->pages != pool->pages)
       return fail(IXK_INVALID_ARGUMENT, "paged_keep: pool and cache differ in pages or page_size");
-    if (k == v) return fail(IXK_INVALID_ARGUMENT, "paged_keep: k and v are the same memory");
+    const paged::Operand kp = paged::key_pages(cache, k), vp = paged::value_pages(cache, v);
+    const int64_t requests = pool->requests, table = paged::rows_extent(requests, pool->table_stride, pool->columns) * 4,
+                  paths = paged::rows_extent(requests, path_stride, path_columns) * 4;
+    const paged::Operand books[] = {{lengths, requests * 4}, {granted, requests * 4}, {kept, requests * 4}, {path, paths}, {page_table, table},
+                                    {free_pages, pool->pages * static_cast<int64_t>(4)}, {free_count, 4}, {free_count_out, 4}, {lengths_out, requests * 4}};
+    if (const char* name = paged::shared_memory({{"k", &kp, nullptr, nullptr}, {"v", &vp, nullptr, nullptr}},
+                                                {&books[0], &books[1], &books[2], &books[3], &books[4], &books[5], &books[6], &books[7], &books[8]}))
+      return fail(IXK_INVALID_ARGUMENT, std::string("paged_keep: ") + name + " of the cache shares memory with another operand or with itself");
   }
   const int64_t requests = pool->requests;
   if (paged::ints_overlap({{lengths, requests, false, nullptr}, {granted, requests, false, nullptr}, {kept, requests, false, nullptr},

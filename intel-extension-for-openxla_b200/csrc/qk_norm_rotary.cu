@@ -700,7 +700,7 @@ int check(const ixk_qk_desc* d, const char* who) {
   if (d->heads > 65536 || d->kv_heads > 65536 || d->tokens > 0x7fffffff) return fail(IXK_UNIMPLEMENTED, at + ": too many heads or tokens");
   return IXK_OK;
 }
-// Strides of a tensor: multiples of eight elements; of one that is written, rows must not overlap.
+// Strides of a tensor: multiples of eight elements; of one that is written, rows must not overlap (what else must not: shared_memory).
 int check_strides(const int64_t (&s)[2], int64_t tokens, int64_t heads, int size, bool written, const char* who, const char* name) {
   const std::string at = std::string(who) + ": " + name;
   if (s[0] % 8 != 0 || s[1] % 8 != 0) return fail(IXK_INVALID_ARGUMENT, at + ": strides must be multiples of 8 elements");
@@ -709,16 +709,19 @@ int check_strides(const int64_t (&s)[2], int64_t tokens, int64_t heads, int size
   return IXK_OK;
 }
 
-// A result in the place of its input lies as that does; anything else that is read or written, it is not.
-int check_in_place(const void* out, const int64_t (&os)[2], const void* in, const int64_t (&is)[2], int64_t tokens, int64_t heads, const char* who,
-                   const char* name) {
-  if (out != in || out == nullptr || ((tokens <= 1 || os[0] == is[0]) && (heads <= 1 || os[1] == is[1]))) return IXK_OK;
-  return fail(IXK_INVALID_ARGUMENT, std::string(who) + ": " + name + " is in the place of its input, with other strides");
+// The memory of a call's tensors.
+int element(const ixk_qk_desc* d) { return d->dtype == IXK_F32 ? 4 : 2; }
+paged::Operand heads_of(const ixk_qk_desc* d, const void* p, const int64_t (&s)[2], int64_t heads) {
+  return paged::Operand(p, d->head_size * element(d), {d->tokens, heads}, s, element(d));
 }
-int check_apart(const void* out, std::initializer_list<const void*> others, const char* who, const char* name) {
-  for (const void* p : others)
-    if (p != nullptr && p == out) return fail(IXK_INVALID_ARGUMENT, std::string(who) + ": " + name + " is in the place of another tensor");
-  return IXK_OK;
+paged::Operand gain_of(const ixk_qk_desc* d, const void* p) { return paged::Operand(p, d->head_size * (d->param_dtype == IXK_F32 ? 4 : 2)); }
+paged::Operand table_of(const ixk_qk_desc* d, const float* p) {
+  const int64_t row = d->rotary_dim * 2;
+  return paged::Operand(p, row, {d->places}, &row, 1);
+}
+paged::Operand positions_of(const ixk_qk_desc* d, const void* p) { return paged::Operand(p, d->tokens * d->position_bytes); }
+int shared(const char* name, const char* who) {
+  return name == nullptr ? IXK_OK : fail(IXK_INVALID_ARGUMENT, std::string(who) + ": " + name + " shares memory with another operand or with itself");
 }
 
 Args base_args(const ixk_qk_desc* d) {
@@ -811,7 +814,6 @@ int ixk_qk_norm_rotary_fwd(const ixk_qk_desc* d, const void* q, const void* k, c
     if (int st = paged::check_cache(cache, k_pages, v_pages, who)) return st;
     if (cache->dtype != d->dtype || cache->heads != d->kv_heads || cache->head_size != d->head_size)
       return fail(IXK_INVALID_ARGUMENT, "qk_norm_rotary: the cache's type, heads or head_size are not those of k and v");
-    if (k_pages == v_pages) return fail(IXK_INVALID_ARGUMENT, "qk_norm_rotary: k and v of the cache are the same memory");
   }
   if (d->tokens > 0 && (q == nullptr || k == nullptr || cos_table == nullptr || sin_table == nullptr || q_out == nullptr ||
                         (paged ? v == nullptr || slots == nullptr : k_out == nullptr)))
@@ -825,10 +827,23 @@ int ixk_qk_norm_rotary_fwd(const ixk_qk_desc* d, const void* q, const void* k, c
     return st;
   }
   if (d->tokens > 0) {
-    if (int st = qk::check_in_place(q_out, d->q_out_strides, q, d->q_strides, d->tokens, d->heads, who, "q_out")) return st;
-    if (int st = qk::check_in_place(k_out, d->k_out_strides, k, d->k_strides, d->tokens, d->kv_heads, who, "k_out")) return st;
-    if (int st = qk::check_apart(q_out, {k, v, k_out, k_pages, v_pages, cos_table, sin_table, positions, q_gain, k_gain}, who, "q_out")) return st;
-    if (int st = qk::check_apart(k_out, {q, cos_table, sin_table, positions, q_gain, k_gain}, who, "k_out")) return st;
+    const paged::Operand mq = qk::heads_of(d, q, d->q_strides, d->heads), mk = qk::heads_of(d, k, d->k_strides, d->kv_heads),
+                         mqo = qk::heads_of(d, q_out, d->q_out_strides, d->heads), gains[2] = {qk::gain_of(d, q_gain), qk::gain_of(d, k_gain)},
+                         tables[2] = {qk::table_of(d, cos_table), qk::table_of(d, sin_table)}, mp = qk::positions_of(d, positions);
+    if (paged) {
+      const paged::Operand mv = qk::heads_of(d, v, d->v_strides, d->kv_heads), ms(slots, d->tokens * 4), kp = paged::key_pages(cache, k_pages),
+                           vp = paged::value_pages(cache, v_pages);
+      if (int st = qk::shared(paged::shared_memory({{"q_out", &mqo, &mq, nullptr}, {"k_pages", &kp, nullptr, nullptr}, {"v_pages", &vp, nullptr, nullptr}},
+                                                   {&mq, &mk, &mv, &gains[0], &gains[1], &tables[0], &tables[1], &mp, &ms}),
+                              who))
+        return st;
+    } else {
+      const paged::Operand mko = qk::heads_of(d, k_out, d->k_out_strides, d->kv_heads);
+      if (int st = qk::shared(paged::shared_memory({{"q_out", &mqo, &mq, nullptr}, {"k_out", &mko, &mk, nullptr}},
+                                                   {&mq, &mk, &gains[0], &gains[1], &tables[0], &tables[1], &mp}),
+                              who))
+        return st;
+    }
   }
   for (const void* p : {q, k, v, q_gain, k_gain, static_cast<const void*>(cos_table), static_cast<const void*>(sin_table),
                         static_cast<const void*>(q_out), static_cast<const void*>(k_out)})
@@ -870,20 +885,26 @@ int ixk_qk_norm_rotary_bwd(const ixk_qk_desc* d, const void* grad_q, const void*
   if (int st = qk::check_strides(d->gk_strides, d->tokens, d->kv_heads, d->head_size, false, who, "grad_k")) return st;
   if (int st = qk::check_strides(d->q_out_strides, d->tokens, d->heads, d->head_size, true, who, "dq")) return st;
   if (int st = qk::check_strides(d->k_out_strides, d->tokens, d->kv_heads, d->head_size, true, who, "dk")) return st;
-  if (d->tokens > 0) {
-    if (int st = qk::check_in_place(dq, d->q_out_strides, q, d->q_strides, d->tokens, d->heads, who, "dq")) return st;
-    if (int st = qk::check_in_place(dq, d->q_out_strides, grad_q, d->gq_strides, d->tokens, d->heads, who, "dq")) return st;
-    if (int st = qk::check_in_place(dk, d->k_out_strides, k, d->k_strides, d->tokens, d->kv_heads, who, "dk")) return st;
-    if (int st = qk::check_in_place(dk, d->k_out_strides, grad_k, d->gk_strides, d->tokens, d->kv_heads, who, "dk")) return st;
-    if (int st = qk::check_apart(dq, {k, grad_k, dk, cos_table, sin_table, positions, q_gain, k_gain, workspace}, who, "dq")) return st;
-    if (int st = qk::check_apart(dk, {q, grad_q, cos_table, sin_table, positions, q_gain, k_gain, workspace}, who, "dk")) return st;
-  }
   for (const void* p : {grad_q, grad_k, q, k, q_gain, k_gain, static_cast<const void*>(cos_table), static_cast<const void*>(sin_table),
                         static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(workspace)})
     if (!aligned16(p)) return fail(IXK_INVALID_ARGUMENT, "qk_norm_rotary backward: pointers must be 16-byte aligned");
   const bool gains = dq_gain != nullptr || dk_gain != nullptr;
   if (gains && (workspace == nullptr || workspace_bytes < ixk_qk_norm_rotary_bwd_workspace_bytes(d)))
     return fail(IXK_WORKSPACE_TOO_SMALL, "qk_norm_rotary backward: workspace_bytes is below ixk_qk_norm_rotary_bwd_workspace_bytes");
+  {
+    const paged::Operand mq = qk::heads_of(d, q, d->q_strides, d->heads), mk = qk::heads_of(d, k, d->k_strides, d->kv_heads),
+                         mgq = qk::heads_of(d, grad_q, d->gq_strides, d->heads), mgk = qk::heads_of(d, grad_k, d->gk_strides, d->kv_heads),
+                         mdq = qk::heads_of(d, dq, d->q_out_strides, d->heads), mdk = qk::heads_of(d, dk, d->k_out_strides, d->kv_heads),
+                         in[2] = {qk::gain_of(d, q_gain), qk::gain_of(d, k_gain)}, out[2] = {qk::gain_of(d, dq_gain), qk::gain_of(d, dk_gain)},
+                         tables[2] = {qk::table_of(d, cos_table), qk::table_of(d, sin_table)}, mp = qk::positions_of(d, positions),
+                         scratch(gains ? workspace : nullptr, static_cast<int64_t>(ixk_qk_norm_rotary_bwd_workspace_bytes(d)));
+    // (a gain's gradient in the gain's place: written when the gain has been read)
+    if (int st = qk::shared(paged::shared_memory({{"dq", &mdq, &mq, &mgq}, {"dk", &mdk, &mk, &mgk}, {"dq_gain", &out[0], &in[0], nullptr},
+                                                  {"dk_gain", &out[1], &in[1], nullptr}, {"the workspace", &scratch, nullptr, nullptr}},
+                                                 {&mq, &mk, &mgq, &mgk, &in[0], &in[1], &tables[0], &tables[1], &mp}),
+                            who))
+      return st;
+  }
   DeviceInfo info;
   if (int st = get_device_info(&info)) return st;
   if (d->tokens == 0 && !gains) return IXK_OK;
