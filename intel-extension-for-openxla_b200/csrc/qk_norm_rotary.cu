@@ -258,12 +258,24 @@ __device__ __forceinline__ Pairs eight(const float* at) {
   return r;
 }
 
+// Chunks that do not turn have no other element's product, not even 0 times it, which is no number where the element is an infinity.
+// kWhole: heads that turn from end to end have no such chunks (these selects cost 8192 tokens of 16 + 4 heads of 128 17.7 -> 18.5 us).
+template <bool kWhole>
+__device__ __forceinline__ Pairs only(const Pairs& a, bool turns) {
+  if constexpr (kWhole) return a;
+  Pairs r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.v[i] = turns ? a.v[i] : 0ull;
+  return r;
+}
+
 // A lane's place in its head: its two chunks (behind the head's last: none).  The lanes' first chunks lie side by side, and the
 // second ones, so that a copy or store of the warp is of whole 32-byte sectors.  (Two neighbouring chunks a lane cost interleaved heads
 // twice the trips to L2: 8192 tokens of 16 + 4 heads of 128 forward 22.9 -> 16.4 us, backward 40.5 -> 28.9.)
 struct Place {
   int a, b;          // first elements
   bool has_a, has_b, turns;
+  bool turns_a, turns_b;         // the chunks' elements turn, into each other's or (interleaved) into their neighbours
 };
 template <int kLanes>
 __device__ __forceinline__ Place place_of(const Args& a, int lane) {
@@ -275,6 +287,8 @@ __device__ __forceinline__ Place place_of(const Args& a, int lane) {
   p.b = second * 8;
   p.has_a = first < a.head_chunks;
   p.has_b = second < a.head_chunks;
+  p.turns_a = a.interleaved ? first < a.rotary_chunks : p.turns;
+  p.turns_b = a.interleaved ? second < a.rotary_chunks : p.turns;
   return p;
 }
 
@@ -334,12 +348,13 @@ __device__ __forceinline__ Turn turn_of(const Angles& g) {
   return t;
 }
 // The turn backwards, without weights: half-split, of both chunks by the same angles.
-template <bool kHalf>
+template <bool kHalf, bool kWhole>
 struct BackTurn;
-template <>
-struct BackTurn<true> {
+template <bool kWhole>
+struct BackTurn<true, kWhole> {
   Pairs c, s;
-  __device__ __forceinline__ explicit BackTurn(const Angles& g) {
+  bool turns;
+  __device__ __forceinline__ BackTurn(const Angles& g, const Place& p) : turns(p.turns) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       c.v[i] = ptx::f32x2(g.c[2 * i], g.c[2 * i + 1]);
@@ -347,26 +362,27 @@ struct BackTurn<true> {
     }
   }
   __device__ __forceinline__ void operator()(const Pairs& xa, const Pairs& xb, Pairs* ya, Pairs* yb) const {
-    Pairs across = mul(xa, s);
+    Pairs across = mul(only<kWhole>(xa, turns), s);
 #pragma unroll
     for (int i = 0; i < 4; ++i) across.v[i] ^= 0x8000000080000000ull;
-    *ya = fma(xa, c, mul(xb, s));
+    *ya = fma(xa, c, mul(only<kWhole>(xb, turns), s));
     *yb = fma(xb, c, across);
   }
 };
-template <>
-struct BackTurn<false> {
+template <bool kWhole>
+struct BackTurn<false, kWhole> {
   Turn t;
-  __device__ __forceinline__ explicit BackTurn(const Angles& g) : t(turn_of<false, true>(g)) {}
+  bool turns_a, turns_b;
+  __device__ __forceinline__ BackTurn(const Angles& g, const Place& p) : t(turn_of<false, true>(g)), turns_a(p.turns_a), turns_b(p.turns_b) {}
   __device__ __forceinline__ void operator()(const Pairs& xa, const Pairs& xb, Pairs* ya, Pairs* yb) const {
-    *ya = fma(xa, t.ca, mul(swapped(xa), t.sa));
-    *yb = fma(xb, t.cb, mul(swapped(xb), t.sb));
+    *ya = fma(xa, t.ca, mul(only<kWhole>(swapped(xa), turns_a), t.sa));
+    *yb = fma(xb, t.cb, mul(only<kWhole>(swapped(xb), turns_b), t.sb));
   }
 };
-template <bool kHalf>
-__device__ __forceinline__ void turn(const Turn& t, const Pairs& xa, const Pairs& xb, Pairs* ya, Pairs* yb) {
-  *ya = fma(xa, t.ca, mul(kHalf ? xb : swapped(xa), t.sa));
-  *yb = fma(xb, t.cb, mul(kHalf ? xa : swapped(xb), t.sb));
+template <bool kHalf, bool kWhole>
+__device__ __forceinline__ void turn(const Turn& t, const Place& p, const Pairs& xa, const Pairs& xb, Pairs* ya, Pairs* yb) {
+  *ya = fma(xa, t.ca, mul(only<kWhole>(kHalf ? xb : swapped(xa), p.turns_a), t.sa));
+  *yb = fma(xb, t.cb, mul(only<kWhole>(kHalf ? xa : swapped(xb), p.turns_b), t.sb));
 }
 
 template <int kLanes>
@@ -399,7 +415,7 @@ __device__ __forceinline__ Share share_of(const Args& a) {
 // All tokens' heads of one kind: a warp walks over its tokens and their segments of this kind (in the last turn [seg0, seg1)), the
 // next segments' heads (the next token's, behind the last) on their way to shared memory meanwhile.
 enum : int { kQueries = 0, kKeys = 1, kValues = 2 };
-template <typename T, int kLanes, bool kHalf, int kKind>
+template <typename T, int kLanes, bool kHalf, bool kWhole, int kKind>
 __device__ __forceinline__ void forward_kind(const Args& a, const Place& p, const Share& share, int seg0, int seg1, uint4* ring) {
   const int turns = share.turns + (seg0 < seg1 ? 1 : 0);
   if (turns == 0) return;
@@ -449,8 +465,8 @@ __device__ __forceinline__ void forward_kind(const Args& a, const Place& p, cons
       const Pairs wa = load_weights<T>(a, gain, p.a, p.has_a), wb = load_weights<T>(a, gain, p.b, p.has_b);
       t.ca = mul(t.ca, wa);
       t.cb = mul(t.cb, wb);
-      t.sa = mul(t.sa, kHalf ? wb : swapped(wa));
-      t.sb = mul(t.sb, kHalf ? wa : swapped(wb));
+      t.sa = only<kWhole>(mul(t.sa, kHalf ? wb : swapped(wa)), p.turns_a);
+      t.sb = only<kWhole>(mul(t.sb, kHalf ? wa : swapped(wb)), p.turns_b);
     }
     if (i_turn + 1 < turns) place = position_of(a, share.token(i_turn + 1));
     T* y = static_cast<T*>(kKind == kQueries ? a.qo : a.ko);
@@ -485,7 +501,7 @@ __device__ __forceinline__ void forward_kind(const Args& a, const Place& p, cons
           const Pairs fa = xa[i].get(), fb = xb[i].get();
           const float r = rsqrtf(head_sum<kLanes>(dot(fa, fa) + dot(fb, fb)) * a.inv_size + a.eps);
           Pairs ya, yb;
-          turn<kHalf>(t, fa, fb, &ya, &yb);
+          turn<kHalf, kWhole>(t, p, fa, fb, &ya, &yb);
           xa[i].set(mul(ya, r));
           xb[i].set(mul(yb, r));
         }
@@ -498,7 +514,7 @@ __device__ __forceinline__ void forward_kind(const Args& a, const Place& p, cons
   }
   copies_wait<0>();
 }
-template <typename T, int kLanes, bool kHalf>
+template <typename T, int kLanes, bool kHalf, bool kWhole>
 __global__ void __launch_bounds__(kThreads, kForwardCtas) forward_kernel(const __grid_constant__ Args a) {
   ptx::grid_dependency_sync();
   const Place p = place_of<kLanes>(a, threadIdx.x & 31);
@@ -506,15 +522,15 @@ __global__ void __launch_bounds__(kThreads, kForwardCtas) forward_kernel(const _
   __shared__ uint4 ring[kForwardStages * 2 * kForwardHeads<T> * (sizeof(T) / 2) * kThreads];
   uint4* mine = ring + threadIdx.x;
   const int first_k = a.q_segments, first_v = first_k + a.kv_segments;
-  forward_kind<T, kLanes, kHalf, kQueries>(a, p, share, share.seg0, min(share.seg1, first_k), mine);
-  forward_kind<T, kLanes, kHalf, kKeys>(a, p, share, max(share.seg0 - first_k, 0), min(share.seg1, first_v) - first_k, mine);
-  if (a.slots != nullptr) forward_kind<T, kLanes, kHalf, kValues>(a, p, share, max(share.seg0 - first_v, 0), share.seg1 - first_v, mine);
+  forward_kind<T, kLanes, kHalf, kWhole, kQueries>(a, p, share, share.seg0, min(share.seg1, first_k), mine);
+  forward_kind<T, kLanes, kHalf, kWhole, kKeys>(a, p, share, max(share.seg0 - first_k, 0), min(share.seg1, first_v) - first_k, mine);
+  if (a.slots != nullptr) forward_kind<T, kLanes, kHalf, kWhole, kValues>(a, p, share, max(share.seg0 - first_v, 0), share.seg1 - first_v, mine);
 }
 
 // The same for the gradients; each lane sums the gains' gradients of its columns in registers over all tokens of its warp, then the
 // lanes of the same columns are added, the CTA's warps in order, and leave as one row of partial sums.  The weights stay in shared
 // memory, 16 registers a lane less: what 128 could not hold went to memory in the inner loop, 137 -> 128 us forward and backward.
-template <typename T, int kLanes, bool kHalf, int kKind>
+template <typename T, int kLanes, bool kHalf, bool kWhole, int kKind>
 __device__ __forceinline__ void backward_kind(const Args& a, const Place& p, const Share& share, int seg0, int seg1, uint4* ring, const float* weights, float* row) {
   constexpr int kGroups = 32 / kLanes, kHeads = kBackwardHeads, kRows = kGroups * kHeads;
   const int lane = threadIdx.x & 31;
@@ -569,7 +585,7 @@ __device__ __forceinline__ void backward_kind(const Args& a, const Place& p, con
       int seg = i_turn < share.turns ? 0 : seg0;
       const int seg_end = i_turn < share.turns ? segments : seg1;
       const bool valid = place >= 0 && place < a.places;
-      const BackTurn<kHalf> turn_back(load_angles<kHalf>(a, p, valid ? place : 0));
+      const BackTurn<kHalf, kWhole> turn_back(load_angles<kHalf>(a, p, valid ? place : 0), p);
       if (i_turn + 1 < turns) place = position_of(a, share.token(i_turn + 1));
       int head = seg * kRows + lane / kLanes;
       T* o = out + token * os[0] + head * os[1];
@@ -625,7 +641,7 @@ __device__ __forceinline__ void backward_kind(const Args& a, const Place& p, con
     if (lane < kLanes && p.has_b) *reinterpret_cast<float2*>(row + p.b + 2 * i) = make_float2(x[2], x[3]);
   }
 }
-template <typename T, int kLanes, bool kHalf>
+template <typename T, int kLanes, bool kHalf, bool kWhole>
 __global__ void __launch_bounds__(kThreads, kBackwardCtas) backward_kernel(const __grid_constant__ Args a) {
   ptx::grid_dependency_sync();
   __shared__ __align__(16) float sums[2][kWarps][kLanes * 16];
@@ -638,8 +654,8 @@ __global__ void __launch_bounds__(kThreads, kBackwardCtas) backward_kernel(const
   __syncthreads();
   const Place p = place_of<kLanes>(a, threadIdx.x & 31);
   const Share share = share_of(a);
-  backward_kind<T, kLanes, kHalf, kQueries>(a, p, share, share.seg0, min(share.seg1, a.q_segments), ring + threadIdx.x, weights[0], sums[0][threadIdx.x >> 5]);
-  backward_kind<T, kLanes, kHalf, kKeys>(a, p, share, max(share.seg0 - a.q_segments, 0), share.seg1 - a.q_segments, ring + threadIdx.x, weights[1], sums[1][threadIdx.x >> 5]);
+  backward_kind<T, kLanes, kHalf, kWhole, kQueries>(a, p, share, share.seg0, min(share.seg1, a.q_segments), ring + threadIdx.x, weights[0], sums[0][threadIdx.x >> 5]);
+  backward_kind<T, kLanes, kHalf, kWhole, kKeys>(a, p, share, max(share.seg0 - a.q_segments, 0), share.seg1 - a.q_segments, ring + threadIdx.x, weights[1], sums[1][threadIdx.x >> 5]);
   if (!a.with_gains) return;
   __syncthreads();           // (the only one: a CTA's warps may have unlike numbers of queries and of keys)
   for (int i = threadIdx.x; i < 2 * a.head_chunks * 8; i += kThreads) {
@@ -781,15 +797,19 @@ int dispatch(int dtype, int lanes, const More&... more) {
 template <typename T, int kLanes>
 struct Forward {
   static int run(const Args& a, unsigned grid, cudaStream_t s) {
-    return a.interleaved ? launch_overlapped(forward_kernel<T, kLanes, false>, dim3(grid), dim3(kThreads), 0, s, a)
-                         : launch_overlapped(forward_kernel<T, kLanes, true>, dim3(grid), dim3(kThreads), 0, s, a);
+    const bool whole = a.rotary_chunks == a.head_chunks;
+    const auto kernel = a.interleaved ? whole ? forward_kernel<T, kLanes, false, true> : forward_kernel<T, kLanes, false, false>
+                                      : whole ? forward_kernel<T, kLanes, true, true> : forward_kernel<T, kLanes, true, false>;
+    return launch_overlapped(kernel, dim3(grid), dim3(kThreads), 0, s, a);
   }
 };
 template <typename T, int kLanes>
 struct Backward {
   static int run(const Args& a, unsigned grid, cudaStream_t s) {
-    return a.interleaved ? launch_overlapped(backward_kernel<T, kLanes, false>, dim3(grid), dim3(kThreads), 0, s, a)
-                         : launch_overlapped(backward_kernel<T, kLanes, true>, dim3(grid), dim3(kThreads), 0, s, a);
+    const bool whole = a.rotary_chunks == a.head_chunks;
+    const auto kernel = a.interleaved ? whole ? backward_kernel<T, kLanes, false, true> : backward_kernel<T, kLanes, false, false>
+                                      : whole ? backward_kernel<T, kLanes, true, true> : backward_kernel<T, kLanes, true, false>;
+    return launch_overlapped(kernel, dim3(grid), dim3(kThreads), 0, s, a);
   }
 };
 
