@@ -9,13 +9,16 @@
 //
 //   warps 0-3   softmax: a thread owns a row (a lane of tensor memory); then the row's result
 //   warp 4      copies: Q, K_0, K_1, V_0, K_2, V_1 ... of the run through a ring of 64-key slots, page by page
-//   warp 5      tcgen05.mma: S_g = Q K_g^T two units ahead into one of two buffers, O += P_g V_g (P from tensor memory)
+//   warp 5      tcgen05.mma: S_g+1 = Q K_g+1^T into one of two buffers, then O += P_g V_g (P from tensor memory)
 //
 // Bound by HBM: 64 keys of K and V take H * 256 bytes, 1340 cycles of an SM's share of the bandwidth at H = 128, the two products
 // 640 (the tile is padded to 128 rows), the softmax about 1000 and beside those of the other worker.
 // Weights are taken of a reference point near the running maximum, which is raised when that has moved by more than 2^8 (fp16: 2^4), so O
 // is seldom rescaled.  P is rounded to nearest, and the row is divided by the sum of the rounded values, so that a row with one
-// large weight loses nothing; the log-sum-exp is taken of the sum of the fp32 ones.  fp16 has few exponents: there the reference
+// large weight loses nothing; the log-sum-exp is taken of the sum of the fp32 ones.  That rounding puts O 0.0021 to 0.0025 (bf16)
+// from 64 bits, where its own rounding alone is 0.0017 (fp16 2.7e-4, 2.1e-4).  P as two 16-bit parts is as good as fp32, but takes
+// half as many products again (64 trees of 16 55.4 -> 58.7 us, ragged ones at head size 256 69 -> 77, prompts 18 %), and a
+// lower part of 0 or below it makes of an infinite value no number.  fp16 has few exponents: there the reference
 // point lies 2^11 below the maximum, so that the largest weights are 2^11 to 2^15 and those down to 2^-25 of them normal numbers
 // (with 1 to 2^8, thousands of keys at 2^-25 of the largest added up to nothing); smaller ones are off by 2^-36 of it at most.
 //
@@ -72,8 +75,8 @@ struct Cfg {
   static constexpr int kQBytes = kChunks * kQChunkBytes;
   static constexpr int kSlotBytes = kChunks * kKvChunkBytes;
   static constexpr int kWorkers = kHeadDim <= 128 ? 2 : 1;        // on an SM
-  // A copy of a page's 64 columns costs its warp about 100 cycles: 32 a unit at head size 256 and 16-token pages, more than the
-  // 2700 that the unit's bytes take.
+  // A copy of a page's 64 columns costs its warp about 100 cycles: 32 a unit of K and as many of V in pages of 8 tokens and heads of less
+  // than 256 columns (or apart from one another, so that none holds more), more than the 2700 that the unit's bytes take.
   static constexpr bool kTwoCopyWarps = kHeadDim == 256;
   static constexpr int kAllThreads = kTwoCopyWarps ? kThreads + 32 : kThreads;
   static constexpr int kSlots = kHeadDim == 64 ? 8 : 5;
